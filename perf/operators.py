@@ -285,7 +285,7 @@ def _own_prompt(s):
     nh, nkv, hd = _sizes(s)
     q, keep = s["q"], s["keep"]
     if not keep:
-        keep["k"], keep["v"] = (torch.empty(s["k"].shape[0], nkv, PAGE, hd, dtype=q.dtype, device=q.device) for _ in range(2))
+        keep["k"], keep["v"] = (torch.zeros(s["k"].shape[0], nkv, PAGE, hd, dtype=q.dtype, device=q.device) for _ in range(2))
     out = torch.empty_like(q)
     kernels.kv4_attention_prefill(q, out, s["k"], s["v"], s["tables"], s["row_seq"], s["positions"], s["first_row"], s["start"], s["most"],
                                   nh, nkv, hd, PAGE, s["scale"], s["window"], s["reach"], keep["k"], keep["v"], s["status"])
