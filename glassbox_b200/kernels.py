@@ -171,6 +171,11 @@ _SIGNATURES = {
     "gb_ssd_chunk_rows": [],
     "gb_ssd_chunks_supported": [_I, _I],
     "gb_ssd_chunks": [_P, _LL, _P, _LL, _P, _P, _P, _P, _LL, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P],
+    "gb_kv4_write": [_P, _LL, _I, _P, _LL, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _LL, _I, _P, _P],
+    "gb_kv4_read": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _LL, _P, _P],
+    "gb_kv4_expand": [_P, _P, _P, _P, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _LL, _I, _P, _P],
+    "gb_kv4_attention_rows": [_P, _LL, _P, _LL, _I, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _LL, _F, _I, _I, _P, _P, _P],
+    "gb_token_logprobs": [_P, _I, _LL, _P, _P, _P, _P, _P, _I, _I, _I, _P],
     "gb_program_op_bytes": [],
     "gb_program_max_rows": [],
 }
@@ -2329,3 +2334,211 @@ def talk_combine(wide: torch.Tensor, talk: Optional[torch.Tensor], att: torch.Te
     assert talk is None or (talk.dtype == torch.float32 and talk.shape == (heads, heads) and talk.is_contiguous())
     _call("gb_talk_combine", _ptr(wide), _ptr(ml), _ptr(talk), _ptr(att), _dt(att), _ptr(positions), n, heads, kv_heads, vdim, value_heads,
           int(shares), 1.0 if unit_sink else 0.0, _stream())
+
+
+# ------------------------------------------------------------------------------------------------ a cache in 4 bits
+KV4_TILE = 16       # tokens of a tile of the layout: page sizes are multiples of it
+KV4_GROUP = 32      # neighbouring channels that share a scale
+
+
+def _require(condition, message: str) -> None:
+    if not condition:
+        raise KernelError(message)
+
+
+def _here(*tensors) -> None:
+    """The operands lie on the current device: the launch goes to its current stream."""
+    _cuda(*tensors)
+    device = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != device:
+            raise KernelError(f"kernel operands must lie on the current device cuda:{device}, not on {t.device}")
+
+
+def _ints(n: int, **named) -> None:
+    for name, t in named.items():
+        _require(t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] >= n and t.is_contiguous(),
+                 f"{name} must be a contiguous int32 vector of at least {n} numbers, not {t.dtype} {tuple(t.shape)}")
+
+
+def kv4_supported(hd: int, page_size: int) -> bool:
+    """Whether keys and values of this size can be held in 4 bits in pages of this many tokens."""
+    return hd % KV4_GROUP == 0 and 0 < hd <= 256 and page_size > 0 and page_size % KV4_TILE == 0
+
+
+def kv4_page_bytes(page_size: int, hd: int) -> int:
+    """Bytes of one head's page: half a byte a number and a two-byte scale for every 32 of them."""
+    return page_size * hd * 9 // 16
+
+
+def _kv4_pool(kcache: torch.Tensor, vcache: torch.Tensor, nkv: int, hd: int, page_size: int) -> None:
+    _require(kv4_supported(hd, page_size), f"a cache in 4 bits holds heads of a multiple of 32 channels up to 256 in pages of a multiple of 16 "
+                                           f"tokens, not heads of {hd} in pages of {page_size}")
+    size = kv4_page_bytes(page_size, hd)
+    for name, t in (("kcache", kcache), ("vcache", vcache)):
+        _require(t.dtype == torch.uint8 and t.dim() == 3 and t.shape[1] == nkv and t.shape[2] == size and t.is_contiguous(),
+                 f"{name} must be a contiguous uint8 tensor [pages, {nkv}, {size}], not {t.dtype} {tuple(t.shape)}")
+    _require(kcache.shape[0] == vcache.shape[0] > 0, "kcache and vcache must have the same number of pages, at least one")
+
+
+def kv4_write(qkv: torch.Tensor, q: torch.Tensor, cos_sin: Optional[torch.Tensor], positions: torch.Tensor, slots: torch.Tensor,
+              kcache: torch.Tensor, vcache: torch.Tensor, nh: int, nkv: int, hd: int, rot: int, page_size: int, write_kv: bool,
+              status: torch.Tensor) -> None:
+    """``rope_kv_write`` into a cache in 4 bits: the queries of each row rotated at its position into ``q`` [n, nh * hd] (which may be the
+    query columns of ``qkv``), its keys (rotated) and values rounded to 4 bits and stored at its slot; the key and value columns
+    of ``qkv`` [n, (nh + 2 nkv) * hd] stay as they are. kcache/vcache: uint8 [pages, nkv, kv4_page_bytes(page_size, hd)]; cos_sin: float32
+    [max_pos, rot/2, 2]. Rows of position < 0 are padding: nothing is read or written for them. Of the rows of one call no two may
+    share a slot.
+
+    How numbers are held: 32 neighbouring channels of a token and head share a scale, -m / 8 rounded to five significant bits with m the one
+    of the largest magnitude (the positive one of two); a number is the nearest of -8 .. 7 (ties to even) times the scale. bfloat16
+    holds every such product exactly. A group that holds a NaN or an infinity reads back as NaN, one whose numbers are
+    all below 2^-117 as zeros."""
+    n = qkv.shape[0]
+    _kv4_pool(kcache, vcache, nkv, hd, page_size)
+    _require(qkv.dim() == 2 and qkv.shape[1] == (nh + 2 * nkv) * hd and qkv.stride(1) == 1, f"qkv must hold rows of {(nh + 2 * nkv) * hd} numbers")
+    _require(q.shape == (n, nh * hd) and q.stride(1) == 1 and q.dtype == qkv.dtype, f"q must be {qkv.dtype} [{n}, {nh * hd}]")
+    _require(n <= 1 or min(qkv.stride(0) - qkv.shape[1], q.stride(0) - q.shape[1]) >= 0, "rows of qkv and of q must not overlap")
+    _ints(n, positions=positions)
+    if write_kv:
+        _ints(n, slots=slots)
+    rot = rot if cos_sin is not None else 0
+    _require(0 <= rot <= hd and rot % 2 == 0, f"rotary size {rot} must be even and at most the head size {hd}")
+    _require(rot == 0 or (cos_sin.dtype == torch.float32 and cos_sin.is_contiguous() and cos_sin.shape[1:] == (rot // 2, 2)),
+             f"cos_sin must be contiguous float32 [positions, {rot // 2}, 2]")
+    _here(qkv, q, cos_sin, positions, slots, kcache, vcache, status)
+    _call("gb_kv4_write", qkv.data_ptr(), qkv.stride(0), _dt(qkv), q.data_ptr(), q.stride(0), _ptr(cos_sin), positions.data_ptr(), slots.data_ptr(),
+          kcache.data_ptr(), vcache.data_ptr(), n, nh, nkv, hd, rot, cos_sin.shape[0] if rot else 0, page_size, kcache.shape[0],
+          1 if write_kv else 0, status.data_ptr(), _stream())
+
+
+def kv4_read(kcache: torch.Tensor, vcache: torch.Tensor, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor, page_size: int,
+             status: torch.Tensor) -> None:
+    """What a cache in 4 bits holds for the tokens at ``slots``: k and v [n, nkv, hd], bfloat16 or float32 (both exact). Rows of a negative
+    slot are left as they are."""
+    _require(k.dim() == 3 and k.shape == v.shape and k.dtype == v.dtype and k.is_contiguous() and v.is_contiguous(),
+             "k and v must be contiguous [rows, kv heads, head size] of one type")
+    n, nkv, hd = k.shape
+    _kv4_pool(kcache, vcache, nkv, hd, page_size)
+    _ints(n, slots=slots)
+    _here(kcache, vcache, slots, k, v, status)
+    _call("gb_kv4_read", kcache.data_ptr(), vcache.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), _dt(k), n, nkv, hd, page_size,
+          kcache.shape[0], status.data_ptr(), _stream())
+
+
+def _kv4_attention(q, out, kcache, vcache, block_tables, row_seq, positions, nh, nkv, hd, page_size, status) -> int:
+    n = q.shape[0]
+    _kv4_pool(kcache, vcache, nkv, hd, page_size)
+    _require(nh % nkv == 0, f"{nh} heads are not a multiple of {nkv} kv heads")
+    _require(q.shape == out.shape == (n, nh * hd) and q.dtype == out.dtype and q.stride(1) == 1 and out.stride(1) == 1,
+             f"q and out must be rows of {nh * hd} numbers of one type")
+    _require(n <= 1 or out.stride(0) >= nh * hd, "rows of out must not overlap")
+    _require(block_tables.dtype == torch.int32 and block_tables.dim() == 2 and block_tables.is_contiguous(), "block_tables must be contiguous int32 [requests, pages]")
+    _ints(n, row_seq=row_seq, positions=positions)
+    _dt(q)
+    _here(q, out, kcache, vcache, block_tables, row_seq, positions, status)
+    return n
+
+
+def kv4_decode_splits(n: int, nh: int, nkv: int, hd: int, max_context: int, dtype: torch.dtype = torch.bfloat16) -> int:
+    """How many shares the keys of a row are cut into: enough to fill the GPU, none much shorter than 128 keys. Depends on the batch shape
+    and the longest context alone, so a captured graph can fix it."""
+    return max(1, min(-(-max_context // 128), -(-148 * 4 // max(n * nh, 1))))
+
+
+def kv4_decode_parts(q: torch.Tensor, nh: int, nkv: int, hd: int, max_context: int) -> Optional[torch.Tensor]:
+    """The scratch that ``kv4_attention_decode`` needs for rows like ``q`` behind contexts up to ``max_context`` (None: it needs none).
+    Contents do not matter between calls; calls that may run at the same time need one each."""
+    splits = kv4_decode_splits(q.shape[0], nh, nkv, hd, max_context, q.dtype)
+    return torch.empty(q.shape[0] * nh * splits * (hd + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
+
+
+def kv4_attention_decode(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, block_tables: torch.Tensor,
+                         row_seq: torch.Tensor, positions: torch.Tensor, nh: int, nkv: int, hd: int, page_size: int, scale: float,
+                         window: Optional[int], max_context: int, parts: Optional[torch.Tensor], status: torch.Tensor) -> None:
+    """softmax(q k^T * scale) v over a cache in 4 bits (``kv4_write``), for rows that are few to a request: row r is a token of request
+    row_seq[r] at positions[r] and sees that request's keys up to its own position (the last ``window`` of them). q, out: bfloat16 or
+    float32 [n, nh * hd], rows may be strided; a row of position < 0 comes out as zeros. ``max_context``: no row has more keys in
+    sight than this matters for (it sizes the shares of a row's keys, longer rows are still right). ``parts``: ``kv4_decode_parts``."""
+    n = _kv4_attention(q, out, kcache, vcache, block_tables, row_seq, positions, nh, nkv, hd, page_size, status)
+    splits = kv4_decode_splits(n, nh, nkv, hd, max_context, q.dtype)
+    if splits > 1:
+        _require(parts is not None and parts.dtype == torch.float32 and parts.is_contiguous() and parts.numel() >= n * nh * splits * (hd + 2),
+                 f"{splits} shares need float32 scratch of {n * nh * splits * (hd + 2)} numbers")
+        _here(parts)
+    _call("gb_kv4_attention_rows", q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), _dt(q), kcache.data_ptr(), vcache.data_ptr(),
+          block_tables.data_ptr(), block_tables.shape[1], row_seq.data_ptr(), positions.data_ptr(), n, nh, nkv, hd, page_size, kcache.shape[0],
+          float(scale), int(window or 0), splits, _ptr(parts), status.data_ptr(), _stream())
+
+
+def kv4_expand(kcache: torch.Tensor, vcache: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor, block_tables: torch.Tensor,
+               seq_first_row: torch.Tensor, seq_start_pos: torch.Tensor, max_context: int, window: Optional[int], status: torch.Tensor) -> None:
+    """The pages that the rows of a step see, unpacked into pages of the same ids: kpages/vpages [pages, nkv, page_size, hd], bfloat16 or
+    float32. Request s brings rows seq_first_row[s] .. seq_first_row[s + 1] - 1 from position seq_start_pos[s] on (negative: a padding
+    request). NaNs of tokens that none of a request's rows sees become zeros."""
+    _require(kpages.dim() == 4 and kpages.shape == vpages.shape and kpages.dtype == vpages.dtype and kpages.is_contiguous() and vpages.is_contiguous(),
+             "kpages and vpages must be contiguous [pages, kv heads, page size, head size] of one type")
+    pages, nkv, page_size, hd = kpages.shape
+    _kv4_pool(kcache, vcache, nkv, hd, page_size)
+    _require(pages >= kcache.shape[0], f"{pages} pages to unpack into do not cover the pool's {kcache.shape[0]}")
+    _require(block_tables.dtype == torch.int32 and block_tables.dim() == 2 and block_tables.is_contiguous(), "block_tables must be contiguous int32 [requests, pages]")
+    S = block_tables.shape[0]
+    _ints(S + 1, seq_first_row=seq_first_row)
+    _ints(S, seq_start_pos=seq_start_pos)
+    _here(kcache, vcache, kpages, vpages, block_tables, seq_first_row, seq_start_pos, status)
+    _call("gb_kv4_expand", kcache.data_ptr(), vcache.data_ptr(), kpages.data_ptr(), vpages.data_ptr(), _dt(kpages), block_tables.data_ptr(),
+          block_tables.shape[1], seq_first_row.data_ptr(), seq_start_pos.data_ptr(), S, -(-int(max_context) // page_size), nkv, hd, page_size,
+          kcache.shape[0], int(window or 0), status.data_ptr(), _stream())
+
+
+def kv4_attention_prefill(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, block_tables: torch.Tensor,
+                          row_seq: torch.Tensor, positions: torch.Tensor, seq_first_row: torch.Tensor, seq_start_pos: torch.Tensor,
+                          max_rows_per_seq: int, nh: int, nkv: int, hd: int, page_size: int, scale: float, window: Optional[int],
+                          max_context: int, kpages: torch.Tensor, vpages: torch.Tensor, status: torch.Tensor) -> None:
+    """``kv4_attention_decode`` for portions of prompts, runs of consecutive rows of a request: the pages in sight are unpacked into
+    kpages/vpages (q's type, [pages, nkv, page_size, hd], numbers everywhere: zero them once) and read from there by the prompt kernel that
+    takes the shape. ``max_context`` bounds the tokens that a request holds after the step."""
+    n = _kv4_attention(q, out, kcache, vcache, block_tables, row_seq, positions, nh, nkv, hd, page_size, status)
+    _require(kpages.dtype == q.dtype and kpages.shape[1:] == (nkv, page_size, hd), f"kpages must be {q.dtype} [pages, {nkv}, {page_size}, {hd}]")
+    kv4_expand(kcache, vcache, kpages, vpages, block_tables, seq_first_row, seq_start_pos, max_context, window, status)
+    args = (q, out, kpages, vpages, block_tables, seq_first_row, seq_start_pos, max_rows_per_seq, nh, nkv, hd, page_size, scale, window, status)
+    aligned = q.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0 and q.stride(0) % 8 == 0 and out.stride(0) % 8 == 0
+    if attention_prefill_tc_supported(q, out, nh, nkv, hd, page_size):
+        attention_prefill_tc(*args)
+    elif aligned and attention_prefill_supported(q.dtype, nh, nkv, hd, page_size):
+        attention_prefill(*args)
+    elif attention_prefill_f32_supported(q, out, nh, nkv, hd):
+        attention_prefill_f32(*args)
+    elif aligned and q.is_contiguous() and out.is_contiguous() and sink_attention_tiles_supported(q.dtype, hd, hd):
+        sink_attention_tiles(q, out, kpages, vpages, block_tables, seq_first_row, seq_start_pos, max_rows_per_seq, r1=None, r2=None, sink=None,
+                             gate=None, heads=nh, kv_heads=nkv, dim=hd, vdim=hd, page_size=page_size, scale=scale, window=window, status=status)
+    else:
+        attention_rows(q, out, kpages, vpages, block_tables, row_seq, positions, nh, nkv, hd, page_size, scale, window, status)
+
+
+# ------------------------------------------------------------------------------------------------ scoring
+LOGPROBS_MAX_TOP = 32
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, logprob: torch.Tensor, entropy: Optional[torch.Tensor] = None,
+                   top_logprob: Optional[torch.Tensor] = None, top_ids: Optional[torch.Tensor] = None) -> None:
+    """logprob[r] = ln softmax(logits[r])[tokens[r]]; entropy[r] = the entropy of softmax(logits[r]), in nats; top_ids[r] the ids of the
+    most probable tokens in falling order (of equal ones the lower id first) and top_logprob[r] their log probabilities. logits
+    float32 or bfloat16 [rows, vocab], rows may be strided; tokens int32 [rows] (one outside the vocabulary: its log probability is NaN);
+    the results float32 and int32, top_* [rows, k] with k up to 32. A logit of minus infinity is a token of probability zero. A row
+    of nothing else, or with a NaN or plus infinity in it, has NaN for all but its ids."""
+    _require(logits.dim() == 2 and logits.stride(1) == 1, "logits must be [rows, vocab] with neighbouring numbers")
+    rows, vocab = logits.shape
+    _ints(rows, tokens=tokens)
+    for name, t in (("logprob", logprob), ("entropy", entropy)):
+        _require(t is None or (t.dtype == torch.float32 and t.shape == (rows,) and t.is_contiguous()), f"{name} must be contiguous float32 [{rows}]")
+    top = 0
+    if top_ids is not None:
+        top = top_ids.shape[1]
+        _require(top_ids.dtype == torch.int32 and top_ids.shape[0] == rows and top_ids.is_contiguous(), f"top_ids must be contiguous int32 [{rows}, k]")
+        _require(0 < top <= min(LOGPROBS_MAX_TOP, vocab), f"{top} alternatives: between 1 and {min(LOGPROBS_MAX_TOP, vocab)} can be asked for")
+    _require(top_logprob is None or (top_ids is not None and top_logprob.dtype == torch.float32 and top_logprob.shape == top_ids.shape
+                                     and top_logprob.is_contiguous()), "top_logprob must be contiguous float32 of top_ids' shape")
+    _here(logits, tokens, logprob, entropy, top_logprob, top_ids)
+    _call("gb_token_logprobs", logits.data_ptr(), _dt(logits), logits.stride(0), tokens.data_ptr(), logprob.data_ptr(), _ptr(entropy),
+          _ptr(top_logprob), _ptr(top_ids), top, rows, vocab, _stream())
