@@ -175,6 +175,7 @@ _SIGNATURES = {
     "gb_kv4_read": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _LL, _P, _P],
     "gb_kv4_expand": [_P, _P, _P, _P, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _LL, _I, _P, _P],
     "gb_kv4_attention_rows": [_P, _LL, _P, _LL, _I, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _LL, _F, _I, _I, _P, _P, _P],
+    "gb_kv4_attention_decode": [_P, _LL, _P, _LL, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _LL, _F, _I, _I, _I, _P, _P, _P],
     "gb_token_logprobs": [_P, _I, _LL, _P, _P, _P, _P, _P, _I, _I, _I, _P],
     "gb_program_op_bytes": [],
     "gb_program_max_rows": [],
@@ -2341,24 +2342,19 @@ KV4_TILE = 16       # tokens of a tile of the layout: page sizes are multiples o
 KV4_GROUP = 32      # neighbouring channels that share a scale
 
 
-def _require(condition, message: str) -> None:
-    if not condition:
-        raise KernelError(message)
-
-
 def _here(*tensors) -> None:
     """The operands lie on the current device: the launch goes to its current stream."""
-    _cuda(*tensors)
-    device = torch.cuda.current_device()
+    device = torch.cuda.current_device() if torch.cuda.is_available() else -2
     for t in tensors:
-        if t is not None and t.device.index != device:
+        if t is not None and t.get_device() != device:
+            if not t.is_cuda:
+                raise KernelError("kernel operands must be CUDA tensors; there is no CPU path")
             raise KernelError(f"kernel operands must lie on the current device cuda:{device}, not on {t.device}")
 
 
-def _ints(n: int, **named) -> None:
-    for name, t in named.items():
-        _require(t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] >= n and t.is_contiguous(),
-                 f"{name} must be a contiguous int32 vector of at least {n} numbers, not {t.dtype} {tuple(t.shape)}")
+def _vector(name: str, t: torch.Tensor, n: int) -> None:
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] < n or not t.is_contiguous():
+        raise KernelError(f"{name} must be a contiguous int32 vector of at least {n} numbers, not {t.dtype} {tuple(t.shape)}")
 
 
 def kv4_supported(hd: int, page_size: int) -> bool:
@@ -2372,13 +2368,15 @@ def kv4_page_bytes(page_size: int, hd: int) -> int:
 
 
 def _kv4_pool(kcache: torch.Tensor, vcache: torch.Tensor, nkv: int, hd: int, page_size: int) -> None:
-    _require(kv4_supported(hd, page_size), f"a cache in 4 bits holds heads of a multiple of 32 channels up to 256 in pages of a multiple of 16 "
-                                           f"tokens, not heads of {hd} in pages of {page_size}")
+    if not (kv4_supported(hd, page_size)):
+        raise KernelError(f"a cache in 4 bits holds heads of a multiple of 32 channels up to 256 in pages of a multiple of 16 "
+                          f"tokens, not heads of {hd} in pages of {page_size}")
     size = kv4_page_bytes(page_size, hd)
     for name, t in (("kcache", kcache), ("vcache", vcache)):
-        _require(t.dtype == torch.uint8 and t.dim() == 3 and t.shape[1] == nkv and t.shape[2] == size and t.is_contiguous(),
-                 f"{name} must be a contiguous uint8 tensor [pages, {nkv}, {size}], not {t.dtype} {tuple(t.shape)}")
-    _require(kcache.shape[0] == vcache.shape[0] > 0, "kcache and vcache must have the same number of pages, at least one")
+        if not (t.dtype == torch.uint8 and t.dim() == 3 and t.shape[1] == nkv and t.shape[2] == size and t.is_contiguous()):
+            raise KernelError(f"{name} must be a contiguous uint8 tensor [pages, {nkv}, {size}], not {t.dtype} {tuple(t.shape)}")
+    if not (kcache.shape[0] == vcache.shape[0] > 0):
+        raise KernelError("kcache and vcache must have the same number of pages, at least one")
 
 
 def kv4_write(qkv: torch.Tensor, q: torch.Tensor, cos_sin: Optional[torch.Tensor], positions: torch.Tensor, slots: torch.Tensor,
@@ -2396,16 +2394,20 @@ def kv4_write(qkv: torch.Tensor, q: torch.Tensor, cos_sin: Optional[torch.Tensor
     all below 2^-117 as zeros."""
     n = qkv.shape[0]
     _kv4_pool(kcache, vcache, nkv, hd, page_size)
-    _require(qkv.dim() == 2 and qkv.shape[1] == (nh + 2 * nkv) * hd and qkv.stride(1) == 1, f"qkv must hold rows of {(nh + 2 * nkv) * hd} numbers")
-    _require(q.shape == (n, nh * hd) and q.stride(1) == 1 and q.dtype == qkv.dtype, f"q must be {qkv.dtype} [{n}, {nh * hd}]")
-    _require(n <= 1 or min(qkv.stride(0) - qkv.shape[1], q.stride(0) - q.shape[1]) >= 0, "rows of qkv and of q must not overlap")
-    _ints(n, positions=positions)
+    if not (qkv.dim() == 2 and qkv.shape[1] == (nh + 2 * nkv) * hd and qkv.stride(1) == 1):
+        raise KernelError(f"qkv must hold rows of {(nh + 2 * nkv) * hd} numbers")
+    if not (q.shape == (n, nh * hd) and q.stride(1) == 1 and q.dtype == qkv.dtype):
+        raise KernelError(f"q must be {qkv.dtype} [{n}, {nh * hd}]")
+    if not (n <= 1 or min(qkv.stride(0) - qkv.shape[1], q.stride(0) - q.shape[1]) >= 0):
+        raise KernelError("rows of qkv and of q must not overlap")
+    _vector("positions", positions, n)
     if write_kv:
-        _ints(n, slots=slots)
+        _vector("slots", slots, n)
     rot = rot if cos_sin is not None else 0
-    _require(0 <= rot <= hd and rot % 2 == 0, f"rotary size {rot} must be even and at most the head size {hd}")
-    _require(rot == 0 or (cos_sin.dtype == torch.float32 and cos_sin.is_contiguous() and cos_sin.shape[1:] == (rot // 2, 2)),
-             f"cos_sin must be contiguous float32 [positions, {rot // 2}, 2]")
+    if not (0 <= rot <= hd and rot % 2 == 0):
+        raise KernelError(f"rotary size {rot} must be even and at most the head size {hd}")
+    if not (rot == 0 or (cos_sin.dtype == torch.float32 and cos_sin.is_contiguous() and cos_sin.shape[1:] == (rot // 2, 2))):
+        raise KernelError(f"cos_sin must be contiguous float32 [positions, {rot // 2}, 2]")
     _here(qkv, q, cos_sin, positions, slots, kcache, vcache, status)
     _call("gb_kv4_write", qkv.data_ptr(), qkv.stride(0), _dt(qkv), q.data_ptr(), q.stride(0), _ptr(cos_sin), positions.data_ptr(), slots.data_ptr(),
           kcache.data_ptr(), vcache.data_ptr(), n, nh, nkv, hd, rot, cos_sin.shape[0] if rot else 0, page_size, kcache.shape[0],
@@ -2416,11 +2418,11 @@ def kv4_read(kcache: torch.Tensor, vcache: torch.Tensor, slots: torch.Tensor, k:
              status: torch.Tensor) -> None:
     """What a cache in 4 bits holds for the tokens at ``slots``: k and v [n, nkv, hd], bfloat16 or float32 (both exact). Rows of a negative
     slot are left as they are."""
-    _require(k.dim() == 3 and k.shape == v.shape and k.dtype == v.dtype and k.is_contiguous() and v.is_contiguous(),
-             "k and v must be contiguous [rows, kv heads, head size] of one type")
+    if not (k.dim() == 3 and k.shape == v.shape and k.dtype == v.dtype and k.is_contiguous() and v.is_contiguous()):
+        raise KernelError("k and v must be contiguous [rows, kv heads, head size] of one type")
     n, nkv, hd = k.shape
     _kv4_pool(kcache, vcache, nkv, hd, page_size)
-    _ints(n, slots=slots)
+    _vector("slots", slots, n)
     _here(kcache, vcache, slots, k, v, status)
     _call("gb_kv4_read", kcache.data_ptr(), vcache.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), _dt(k), n, nkv, hd, page_size,
           kcache.shape[0], status.data_ptr(), _stream())
@@ -2429,28 +2431,46 @@ def kv4_read(kcache: torch.Tensor, vcache: torch.Tensor, slots: torch.Tensor, k:
 def _kv4_attention(q, out, kcache, vcache, block_tables, row_seq, positions, nh, nkv, hd, page_size, status) -> int:
     n = q.shape[0]
     _kv4_pool(kcache, vcache, nkv, hd, page_size)
-    _require(nh % nkv == 0, f"{nh} heads are not a multiple of {nkv} kv heads")
-    _require(q.shape == out.shape == (n, nh * hd) and q.dtype == out.dtype and q.stride(1) == 1 and out.stride(1) == 1,
-             f"q and out must be rows of {nh * hd} numbers of one type")
-    _require(n <= 1 or out.stride(0) >= nh * hd, "rows of out must not overlap")
-    _require(block_tables.dtype == torch.int32 and block_tables.dim() == 2 and block_tables.is_contiguous(), "block_tables must be contiguous int32 [requests, pages]")
-    _ints(n, row_seq=row_seq, positions=positions)
+    if not (nh % nkv == 0):
+        raise KernelError(f"{nh} heads are not a multiple of {nkv} kv heads")
+    if not (q.shape == out.shape == (n, nh * hd) and q.dtype == out.dtype and q.stride(1) == 1 and out.stride(1) == 1):
+        raise KernelError(f"q and out must be rows of {nh * hd} numbers of one type")
+    if not (n <= 1 or out.stride(0) >= nh * hd):
+        raise KernelError("rows of out must not overlap")
+    if not (block_tables.dtype == torch.int32 and block_tables.dim() == 2 and block_tables.is_contiguous()):
+        raise KernelError("block_tables must be contiguous int32 [requests, pages]")
+    _vector("row_seq", row_seq, n)
+    _vector("positions", positions, n)
     _dt(q)
     _here(q, out, kcache, vcache, block_tables, row_seq, positions, status)
     return n
 
 
-def kv4_decode_splits(n: int, nh: int, nkv: int, hd: int, max_context: int, dtype: torch.dtype = torch.bfloat16) -> int:
-    """How many shares the keys of a row are cut into: enough to fill the GPU, none much shorter than 128 keys. Depends on the batch shape
-    and the longest context alone, so a captured graph can fix it."""
-    return max(1, min(-(-max_context // 128), -(-148 * 4 // max(n * nh, 1))))
+KV4_MMA_HEADS = 8                          # query heads of a block of the tensor-core kernel
+KV4_MMA_SIZES = (32, 64, 96, 128, 256)      # head sizes it is built for
 
 
-def kv4_decode_parts(q: torch.Tensor, nh: int, nkv: int, hd: int, max_context: int) -> Optional[torch.Tensor]:
+def kv4_decode_plan(n: int, nh: int, nkv: int, hd: int, max_context: int, window: Optional[int] = None, dtype: torch.dtype = torch.bfloat16):
+    """(shares that the keys of a row are cut into, blocks of a cluster that adds them up). The tensor-core kernel runs one block a share, kv head
+    and eight query heads; enough of them to fill the GPU, none of much fewer than 128 keys. The kernel for other types and
+    head sizes runs one a share and query head, without clusters (0). Depends on the batch shape and the longest context alone, so a captured graph
+    can fix it."""
+    reach = min(max_context, window) + KV4_TILE if window else max_context
+    most = max(1, -(-reach // 128))
+    if dtype != torch.bfloat16 or hd not in KV4_MMA_SIZES:
+        return max(1, min(most, -(-148 * 4 // max(n * nh, 1)))), 0
+    blocks = max(n * nkv * -(-(nh // nkv) // KV4_MMA_HEADS), 1)
+    splits = max(1, min(most, -(-148 * 4 // blocks)))
+    cluster = 8 if splits >= 8 else 4 if splits >= 4 else 2 if splits >= 2 else 1
+    return splits // cluster * cluster, cluster
+
+
+def kv4_decode_parts(q: torch.Tensor, nh: int, nkv: int, hd: int, max_context: int, window: Optional[int] = None) -> Optional[torch.Tensor]:
     """The scratch that ``kv4_attention_decode`` needs for rows like ``q`` behind contexts up to ``max_context`` (None: it needs none).
     Contents do not matter between calls; calls that may run at the same time need one each."""
-    splits = kv4_decode_splits(q.shape[0], nh, nkv, hd, max_context, q.dtype)
-    return torch.empty(q.shape[0] * nh * splits * (hd + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
+    splits, cluster = kv4_decode_plan(q.shape[0], nh, nkv, hd, max_context, window, q.dtype)
+    shares = splits // max(cluster, 1)
+    return torch.empty(q.shape[0] * nh * shares * (hd + 2), dtype=torch.float32, device=q.device) if shares > 1 else None
 
 
 def kv4_attention_decode(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, block_tables: torch.Tensor,
@@ -2459,16 +2479,23 @@ def kv4_attention_decode(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tenso
     """softmax(q k^T * scale) v over a cache in 4 bits (``kv4_write``), for rows that are few to a request: row r is a token of request
     row_seq[r] at positions[r] and sees that request's keys up to its own position (the last ``window`` of them). q, out: bfloat16 or
     float32 [n, nh * hd], rows may be strided; a row of position < 0 comes out as zeros. ``max_context``: no row has more keys in
-    sight than this matters for (it sizes the shares of a row's keys, longer rows are still right). ``parts``: ``kv4_decode_parts``."""
+    sight than this matters for (it sizes the shares of a row's keys, longer rows are still right). ``parts``: ``kv4_decode_parts``
+    of the same sizes, or without its window."""
     n = _kv4_attention(q, out, kcache, vcache, block_tables, row_seq, positions, nh, nkv, hd, page_size, status)
-    splits = kv4_decode_splits(n, nh, nkv, hd, max_context, q.dtype)
-    if splits > 1:
-        _require(parts is not None and parts.dtype == torch.float32 and parts.is_contiguous() and parts.numel() >= n * nh * splits * (hd + 2),
-                 f"{splits} shares need float32 scratch of {n * nh * splits * (hd + 2)} numbers")
+    splits, cluster = kv4_decode_plan(n, nh, nkv, hd, max_context, window, q.dtype)
+    shares = splits // max(cluster, 1)
+    if shares > 1:
+        if parts is None or parts.dtype != torch.float32 or not parts.is_contiguous() or parts.numel() < n * nh * shares * (hd + 2):
+            raise KernelError(f"{shares} shares need contiguous float32 scratch of {n * nh * shares * (hd + 2)} numbers")
         _here(parts)
-    _call("gb_kv4_attention_rows", q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), _dt(q), kcache.data_ptr(), vcache.data_ptr(),
-          block_tables.data_ptr(), block_tables.shape[1], row_seq.data_ptr(), positions.data_ptr(), n, nh, nkv, hd, page_size, kcache.shape[0],
-          float(scale), int(window or 0), splits, _ptr(parts), status.data_ptr(), _stream())
+    if cluster:
+        _call("gb_kv4_attention_decode", q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), kcache.data_ptr(), vcache.data_ptr(),
+              block_tables.data_ptr(), block_tables.shape[1], row_seq.data_ptr(), positions.data_ptr(), n, nh, nkv, hd, page_size,
+              kcache.shape[0], float(scale), int(window or 0), splits, cluster, _ptr(parts), status.data_ptr(), _stream())
+    else:
+        _call("gb_kv4_attention_rows", q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), _dt(q), kcache.data_ptr(), vcache.data_ptr(),
+              block_tables.data_ptr(), block_tables.shape[1], row_seq.data_ptr(), positions.data_ptr(), n, nh, nkv, hd, page_size,
+              kcache.shape[0], float(scale), int(window or 0), splits, _ptr(parts), status.data_ptr(), _stream())
 
 
 def kv4_expand(kcache: torch.Tensor, vcache: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor, block_tables: torch.Tensor,
@@ -2476,15 +2503,17 @@ def kv4_expand(kcache: torch.Tensor, vcache: torch.Tensor, kpages: torch.Tensor,
     """The pages that the rows of a step see, unpacked into pages of the same ids: kpages/vpages [pages, nkv, page_size, hd], bfloat16 or
     float32. Request s brings rows seq_first_row[s] .. seq_first_row[s + 1] - 1 from position seq_start_pos[s] on (negative: a padding
     request). NaNs of tokens that none of a request's rows sees become zeros."""
-    _require(kpages.dim() == 4 and kpages.shape == vpages.shape and kpages.dtype == vpages.dtype and kpages.is_contiguous() and vpages.is_contiguous(),
-             "kpages and vpages must be contiguous [pages, kv heads, page size, head size] of one type")
+    if not (kpages.dim() == 4 and kpages.shape == vpages.shape and kpages.dtype == vpages.dtype and kpages.is_contiguous() and vpages.is_contiguous()):
+        raise KernelError("kpages and vpages must be contiguous [pages, kv heads, page size, head size] of one type")
     pages, nkv, page_size, hd = kpages.shape
     _kv4_pool(kcache, vcache, nkv, hd, page_size)
-    _require(pages >= kcache.shape[0], f"{pages} pages to unpack into do not cover the pool's {kcache.shape[0]}")
-    _require(block_tables.dtype == torch.int32 and block_tables.dim() == 2 and block_tables.is_contiguous(), "block_tables must be contiguous int32 [requests, pages]")
+    if not (pages >= kcache.shape[0]):
+        raise KernelError(f"{pages} pages to unpack into do not cover the pool's {kcache.shape[0]}")
+    if not (block_tables.dtype == torch.int32 and block_tables.dim() == 2 and block_tables.is_contiguous()):
+        raise KernelError("block_tables must be contiguous int32 [requests, pages]")
     S = block_tables.shape[0]
-    _ints(S + 1, seq_first_row=seq_first_row)
-    _ints(S, seq_start_pos=seq_start_pos)
+    _vector("seq_first_row", seq_first_row, S + 1)
+    _vector("seq_start_pos", seq_start_pos, S)
     _here(kcache, vcache, kpages, vpages, block_tables, seq_first_row, seq_start_pos, status)
     _call("gb_kv4_expand", kcache.data_ptr(), vcache.data_ptr(), kpages.data_ptr(), vpages.data_ptr(), _dt(kpages), block_tables.data_ptr(),
           block_tables.shape[1], seq_first_row.data_ptr(), seq_start_pos.data_ptr(), S, -(-int(max_context) // page_size), nkv, hd, page_size,
@@ -2499,7 +2528,8 @@ def kv4_attention_prefill(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tens
     kpages/vpages (q's type, [pages, nkv, page_size, hd], numbers everywhere: zero them once) and read from there by the prompt kernel that
     takes the shape. ``max_context`` bounds the tokens that a request holds after the step."""
     n = _kv4_attention(q, out, kcache, vcache, block_tables, row_seq, positions, nh, nkv, hd, page_size, status)
-    _require(kpages.dtype == q.dtype and kpages.shape[1:] == (nkv, page_size, hd), f"kpages must be {q.dtype} [pages, {nkv}, {page_size}, {hd}]")
+    if not (kpages.dtype == q.dtype and kpages.shape[1:] == (nkv, page_size, hd)):
+        raise KernelError(f"kpages must be {q.dtype} [pages, {nkv}, {page_size}, {hd}]")
     kv4_expand(kcache, vcache, kpages, vpages, block_tables, seq_first_row, seq_start_pos, max_context, window, status)
     args = (q, out, kpages, vpages, block_tables, seq_first_row, seq_start_pos, max_rows_per_seq, nh, nkv, hd, page_size, scale, window, status)
     aligned = q.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0 and q.stride(0) % 8 == 0 and out.stride(0) % 8 == 0
@@ -2527,18 +2557,22 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, logprob: torch.Te
     float32 or bfloat16 [rows, vocab], rows may be strided; tokens int32 [rows] (one outside the vocabulary: its log probability is NaN);
     the results float32 and int32, top_* [rows, k] with k up to 32. A logit of minus infinity is a token of probability zero. A row
     of nothing else, or with a NaN or plus infinity in it, has NaN for all but its ids."""
-    _require(logits.dim() == 2 and logits.stride(1) == 1, "logits must be [rows, vocab] with neighbouring numbers")
+    if not (logits.dim() == 2 and logits.stride(1) == 1):
+        raise KernelError("logits must be [rows, vocab] with neighbouring numbers")
     rows, vocab = logits.shape
-    _ints(rows, tokens=tokens)
+    _vector("tokens", tokens, rows)
     for name, t in (("logprob", logprob), ("entropy", entropy)):
-        _require(t is None or (t.dtype == torch.float32 and t.shape == (rows,) and t.is_contiguous()), f"{name} must be contiguous float32 [{rows}]")
+        if not (t is None or (t.dtype == torch.float32 and t.shape == (rows,) and t.is_contiguous())):
+            raise KernelError(f"{name} must be contiguous float32 [{rows}]")
     top = 0
     if top_ids is not None:
         top = top_ids.shape[1]
-        _require(top_ids.dtype == torch.int32 and top_ids.shape[0] == rows and top_ids.is_contiguous(), f"top_ids must be contiguous int32 [{rows}, k]")
-        _require(0 < top <= min(LOGPROBS_MAX_TOP, vocab), f"{top} alternatives: between 1 and {min(LOGPROBS_MAX_TOP, vocab)} can be asked for")
-    _require(top_logprob is None or (top_ids is not None and top_logprob.dtype == torch.float32 and top_logprob.shape == top_ids.shape
-                                     and top_logprob.is_contiguous()), "top_logprob must be contiguous float32 of top_ids' shape")
+        if not (top_ids.dtype == torch.int32 and top_ids.shape[0] == rows and top_ids.is_contiguous()):
+            raise KernelError(f"top_ids must be contiguous int32 [{rows}, k]")
+        if not (0 < top <= min(LOGPROBS_MAX_TOP, vocab)):
+            raise KernelError(f"{top} alternatives: between 1 and {min(LOGPROBS_MAX_TOP, vocab)} can be asked for")
+    if not (top_logprob is None or (top_ids is not None and top_logprob.dtype == torch.float32 and top_logprob.shape == top_ids.shape and top_logprob.is_contiguous())):
+        raise KernelError("top_logprob must be contiguous float32 of top_ids' shape")
     _here(logits, tokens, logprob, entropy, top_logprob, top_ids)
     _call("gb_token_logprobs", logits.data_ptr(), _dt(logits), logits.stride(0), tokens.data_ptr(), logprob.data_ptr(), _ptr(entropy),
           _ptr(top_logprob), _ptr(top_ids), top, rows, vocab, _stream())
