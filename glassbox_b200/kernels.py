@@ -8,6 +8,7 @@ no library stand-in: if the shared library cannot be built or loaded, the first 
 from __future__ import annotations
 
 import ctypes
+import functools
 import threading
 from typing import Optional
 
@@ -176,6 +177,8 @@ _SIGNATURES = {
     "gb_kv4_expand": [_P, _P, _P, _P, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _LL, _I, _P, _P],
     "gb_kv4_attention_rows": [_P, _LL, _P, _LL, _I, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _LL, _F, _I, _I, _P, _P, _P],
     "gb_kv4_attention_decode": [_P, _LL, _P, _LL, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _LL, _F, _I, _I, _I, _P, _P, _P],
+    "gb_kv4_attention_decode_supported": [_I],
+    "gb_kv4_attention_decode_blocks": [_I, _I, _I, _I, _LL],
     "gb_token_logprobs": [_P, _I, _LL, _P, _P, _P, _P, _P, _I, _I, _I, _P],
     "gb_program_op_bytes": [],
     "gb_program_max_rows": [],
@@ -2446,31 +2449,38 @@ def _kv4_attention(q, out, kcache, vcache, block_tables, row_seq, positions, nh,
     return n
 
 
-KV4_MMA_HEADS = 8                          # query heads of a block of the tensor-core kernel
-KV4_MMA_SIZES = (32, 64, 96, 128, 256)      # head sizes it is built for
+KV4_MMA_HEADS = 8       # query heads of a block of the tensor-core kernel
+KV4_EVEN_ROWS = 1024     # rows at most whose keys it shares evenly
 
 
+@functools.lru_cache(maxsize=4096)
 def kv4_decode_plan(n: int, nh: int, nkv: int, hd: int, max_context: int, window: Optional[int] = None, dtype: torch.dtype = torch.bfloat16):
-    """(shares that the keys of a row are cut into, blocks of a cluster that adds them up). The tensor-core kernel runs one block a share, kv head
-    and eight query heads; enough of them to fill the GPU, none of much fewer than 128 keys. The kernel for other types and
-    head sizes runs one a share and query head, without clusters (0). Depends on the batch shape and the longest context alone, so a captured graph
-    can fix it."""
-    reach = min(max_context, window) + KV4_TILE if window else max_context
-    most = max(1, -(-reach // 128))
-    if dtype != torch.bfloat16 or hd not in KV4_MMA_SIZES:
-        return max(1, min(most, -(-148 * 4 // max(n * nh, 1)))), 0
-    blocks = max(n * nkv * -(-(nh // nkv) // KV4_MMA_HEADS), 1)
-    splits = max(1, min(most, -(-148 * 4 // blocks)))
-    cluster = 8 if splits >= 8 else 4 if splits >= 4 else 2 if splits >= 2 else 1
-    return splits // cluster * cluster, cluster
+    """How the keys of n rows are shared among blocks, (kind, number), and the float32 numbers of scratch that this takes:
+
+    * "cluster": a cluster of that many blocks of the tensor-core kernel for every row, kv head and eight query heads,
+    * "even": that many blocks share all rows' keys evenly, whatever the rows' lengths,
+    * "rows": that many shares of the keys of every row and head (the kernel for other types and head sizes).
+
+    Depends on the batch shape and the longest context alone, so a captured graph can fix it."""
+    reach = max(1, min(max_context, window) if window else max_context)
+    if dtype != torch.bfloat16 or not lib().gb_kv4_attention_decode_supported(hd):
+        splits = max(1, min(-(-reach // 128), -(-148 * 4 // max(n * nh, 1))))
+        return "rows", splits, n * nh * splits * (hd + 2) if splits > 1 else 0
+    pairs = max(n * nkv * -(-(nh // nkv) // KV4_MMA_HEADS), 1)
+    cluster = 8
+    while cluster > 1 and (reach <= 64 * cluster or pairs * cluster > 148 * 4):
+        cluster //= 2
+    if n > KV4_EVEN_ROWS or (reach <= 512 * cluster and pairs * cluster <= 148 * 4):
+        return "cluster", cluster, 0
+    blocks = lib().gb_kv4_attention_decode_blocks(n, nh, nkv, hd, reach)
+    return ("even", blocks, 2 * blocks * KV4_MMA_HEADS * (hd + 2) + 4 * blocks) if blocks else ("cluster", cluster, 0)
 
 
 def kv4_decode_parts(q: torch.Tensor, nh: int, nkv: int, hd: int, max_context: int, window: Optional[int] = None) -> Optional[torch.Tensor]:
     """The scratch that ``kv4_attention_decode`` needs for rows like ``q`` behind contexts up to ``max_context`` (None: it needs none).
     Contents do not matter between calls; calls that may run at the same time need one each."""
-    splits, cluster = kv4_decode_plan(q.shape[0], nh, nkv, hd, max_context, window, q.dtype)
-    shares = splits // max(cluster, 1)
-    return torch.empty(q.shape[0] * nh * shares * (hd + 2), dtype=torch.float32, device=q.device) if shares > 1 else None
+    floats = kv4_decode_plan(q.shape[0], nh, nkv, hd, max_context, window, q.dtype)[2]
+    return torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
 
 
 def kv4_attention_decode(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, block_tables: torch.Tensor,
@@ -2480,22 +2490,22 @@ def kv4_attention_decode(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tenso
     row_seq[r] at positions[r] and sees that request's keys up to its own position (the last ``window`` of them). q, out: bfloat16 or
     float32 [n, nh * hd], rows may be strided; a row of position < 0 comes out as zeros. ``max_context``: no row has more keys in
     sight than this matters for (it sizes the shares of a row's keys, longer rows are still right). ``parts``: ``kv4_decode_parts``
-    of the same sizes, or without its window."""
+    of the same rows, heads and ``max_context`` (with the window or without)."""
     n = _kv4_attention(q, out, kcache, vcache, block_tables, row_seq, positions, nh, nkv, hd, page_size, status)
-    splits, cluster = kv4_decode_plan(n, nh, nkv, hd, max_context, window, q.dtype)
-    shares = splits // max(cluster, 1)
-    if shares > 1:
-        if parts is None or parts.dtype != torch.float32 or not parts.is_contiguous() or parts.numel() < n * nh * shares * (hd + 2):
-            raise KernelError(f"{shares} shares need contiguous float32 scratch of {n * nh * shares * (hd + 2)} numbers")
+    kind, number, floats = kv4_decode_plan(n, nh, nkv, hd, max_context, window, q.dtype)
+    if floats:
+        if parts is None or parts.dtype != torch.float32 or not parts.is_contiguous() or parts.numel() < floats:
+            raise KernelError(f"this batch needs contiguous float32 scratch of {floats} numbers (kv4_decode_parts)")
         _here(parts)
-    if cluster:
-        _call("gb_kv4_attention_decode", q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), kcache.data_ptr(), vcache.data_ptr(),
-              block_tables.data_ptr(), block_tables.shape[1], row_seq.data_ptr(), positions.data_ptr(), n, nh, nkv, hd, page_size,
-              kcache.shape[0], float(scale), int(window or 0), splits, cluster, _ptr(parts), status.data_ptr(), _stream())
-    else:
+    if kind == "rows":
         _call("gb_kv4_attention_rows", q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), _dt(q), kcache.data_ptr(), vcache.data_ptr(),
               block_tables.data_ptr(), block_tables.shape[1], row_seq.data_ptr(), positions.data_ptr(), n, nh, nkv, hd, page_size,
-              kcache.shape[0], float(scale), int(window or 0), splits, _ptr(parts), status.data_ptr(), _stream())
+              kcache.shape[0], float(scale), int(window or 0), number, _ptr(parts), status.data_ptr(), _stream())
+    else:
+        _call("gb_kv4_attention_decode", q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), kcache.data_ptr(), vcache.data_ptr(),
+              block_tables.data_ptr(), block_tables.shape[1], row_seq.data_ptr(), positions.data_ptr(), n, nh, nkv, hd, page_size,
+              kcache.shape[0], float(scale), int(window or 0), number if kind == "cluster" else 1, number if kind == "even" else 0, _ptr(parts),
+              status.data_ptr(), _stream())
 
 
 def kv4_expand(kcache: torch.Tensor, vcache: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor, block_tables: torch.Tensor,
