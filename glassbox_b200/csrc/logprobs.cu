@@ -1,13 +1,25 @@
 // Log probabilities of given tokens, with the entropy of each row's distribution and its most probable tokens.
 //
-// For a row x of logits: log p_i = x_i - m - ln Z with m the largest logit and Z = sum e^(x_i - m); entropy = ln Z - sum e^(x_i - m) (x_i - m) / Z.
-// Tokens of probability zero (a logit of minus infinity) add nothing. A row in which nothing has a probability (all minus infinity), or
-// that holds a NaN or plus infinity, has NaN for all of them. The most probable tokens come in falling order, of equal logits the lower id
-// first (0 and -0 are equal; a NaN comes last of all).
+// For a row x of logits and any reference r: with Z = sum e^(x_i - r) and H = sum e^(x_i - r) (x_i - r), log p_i = x_i - r - ln Z and the
+// entropy is ln Z - H / Z; when the reference rises by a, Z becomes Z e^-a and H becomes (H - a Z) e^-a. Tokens of probability zero (a logit of
+// minus infinity) add nothing. A row in which nothing has a probability (all minus infinity), or that holds a NaN or plus infinity, has NaN
+// for all of them. The most probable tokens come in falling order, of equal logits the lower id first (0 and -0 are equal; NaN comes last).
+//
+// What bounds it is reading the logits, once. A block takes a row (or, of few rows, a share of one: the blocks of a cluster add up) in
+// tiles of 4,096; the next tile's loads are under way while a tile is worked on. Every thread keeps a reference, Z and H of its own. The
+// most probable tokens are found in the same pass: k numbers at least as large as a threshold are known to exist once the threshold is the
+// smallest over the warps of each warp's ceil(k / warps)-th largest of its threads' maxima; only what reaches it is written down (some dozens a tile,
+// fewer and fewer as the threshold rises, which it does in tiles 0, 1, 3, 7 ...), and one warp picks the k largest of that. Behind the tile that set it a number
+// has to be larger, since equal ones of higher ids come too late. A row that leaves more than 2,048 candidates (one that only rises, or that holds thousands of
+// equal largest numbers) is searched k times instead.
 #include "common.cuh"
 
-constexpr int LP_THREADS = 512;
+#include <cooperative_groups.h>
+
+constexpr int LP_THREADS = 256, LP_WARPS = LP_THREADS / 32;
 constexpr int LP_MAX_TOP = 32;
+constexpr int LP_FLY = 4;               // 16-byte loads of a thread and tile
+constexpr int LP_KEEP = 2048;            // candidates
 
 // A logit as a whole number of the same order; ties between ids are broken by the low half of (order, ~id).
 __device__ __forceinline__ unsigned lp_order(float x) {
@@ -17,86 +29,338 @@ __device__ __forceinline__ unsigned lp_order(float x) {
     return b >> 31 ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ unsigned long long lp_key(float x, int id) { return (unsigned long long)lp_order(x) << 32 | (unsigned)~id; }
+__device__ __forceinline__ float lp_max_nan(float a, float b) {         // NaN where a is one
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float lp_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
-__device__ __forceinline__ float lp_block_sum(float v, float* s) {
-    v = gb_warp_sum(v);
+// The largest key of a warp's.
+__device__ __forceinline__ unsigned long long lp_warp_max(unsigned long long key) {
+    const unsigned high = __reduce_max_sync(0xffffffffu, (unsigned)(key >> 32));
+    const unsigned low = __reduce_max_sync(0xffffffffu, (unsigned)(key >> 32) == high ? (unsigned)key : 0u);
+    return (unsigned long long)high << 32 | low;
+}
+
+template <typename T> struct LpVec;        // 16 bytes of logits
+template <> struct LpVec<float> {
+    static constexpr int N = 4;
+    static __device__ __forceinline__ void unpack(const uint4& v, float (&x)[4]) {
+        x[0] = __uint_as_float(v.x); x[1] = __uint_as_float(v.y); x[2] = __uint_as_float(v.z); x[3] = __uint_as_float(v.w);
+    }
+    static __device__ __forceinline__ uint4 nothing() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
+};
+template <> struct LpVec<__nv_bfloat16> {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ void unpack(const uint4& v, float (&x)[8]) {
+        const unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = __uint_as_float(w[i] << 16);
+            x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+    static __device__ __forceinline__ uint4 nothing() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
+};
+
+struct LpArgs {
+    const void* logits;
+    long long stride;
+    const int* tokens;
+    float* logprob;
+    float* entropy;
+    float* top_logprob;
+    int* top_ids;
+    int top, vocab, shares;
+};
+
+struct LpShared {
+    float r[LP_WARPS], z[LP_WARPS], h[LP_WARPS];
+    float level[LP_WARPS];
+    float all[3];                              // of the block: reference, Z, H
+    int count, found;
+    unsigned long long best[LP_MAX_TOP];        // of the block, falling
+    unsigned long long keep[LP_KEEP];
+};
+
+// The running sums of a thread. r: the reference, minus infinity while all logits were.
+struct LpSums {
+    float r = -INFINITY, z = 0.f, h = 0.f;
+    __device__ __forceinline__ void rise(float to) {
+        if (to > r) {
+            const float d = r == -INFINITY ? 0.f : r - to, f = lp_exp2(d * 1.4426950408889634f);
+            h = f * fmaf(d, z, h);
+            z *= f;
+            r = to;
+        }
+    }
+    // (a token that is e^-150 times as likely as the likeliest adds nothing to a float32 sum of them)
+    __device__ __forceinline__ void add(float x, float from) {
+        const float d = lp_max_nan(x - from, -150.f), e = lp_exp2(d * 1.4426950408889634f);
+        z += e;
+        h = fmaf(e, d, h);
+    }
+    __device__ __forceinline__ void join(float ro, float zo, float ho) {
+        if (ro == -INFINITY) { z += zo; h += ho; return; }          // (nothing, or NaN)
+        rise(ro);
+        const float d = ro - r, f = lp_exp2(d * 1.4426950408889634f);
+        z = fmaf(zo, f, z);
+        h = fmaf(f, fmaf(d, zo, ho), h);
+    }
+};
+
+// How large a number has to be so that `top` are at least as large: the smallest over the warps of the ceil(top / warps)-th largest thread's maximum.
+__device__ __forceinline__ float lp_level(LpShared& s, float most, int top) {
+    const int lane = threadIdx.x & 31, nth = (top + LP_WARPS - 1) / LP_WARPS;      // 1 .. 4
+    unsigned left = lp_order(most);
+    if (left == 0u) left = lp_order(-INFINITY);
+    unsigned level = 0;
+    for (int i = 0; i < nth; ++i) {
+        level = __reduce_max_sync(0xffffffffu, left);
+        const unsigned who = __ballot_sync(0xffffffffu, left == level);
+        if (lane == __ffs(who) - 1) left = 0;
+    }
+    __syncthreads();                            // (the level before has been read)
+    if (lane == 0) s.level[threadIdx.x >> 5] = level >> 31 ? __uint_as_float(level & 0x7fffffffu) : __uint_as_float(~level);
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
-    __syncthreads();
-    float sum = 0.f;
-    for (int w = 0; w < LP_THREADS / 32; ++w) sum += s[w];
-    return sum;
+    float v = s.level[0];
+#pragma unroll
+    for (int w = 1; w < LP_WARPS; ++w) v = fminf(v, s.level[w]);
+    return v;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(const T* __restrict__ logits, long long stride, const int* __restrict__ tokens,
-                                                              float* __restrict__ logprob, float* __restrict__ entropy,
-                                                              float* __restrict__ top_logprob, int* __restrict__ top_ids, int top, int vocab) {
-    __shared__ float s[LP_THREADS / 32];
-    __shared__ unsigned long long sk[LP_THREADS / 32];
+__global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LpArgs a) {
+    using Vec = LpVec<T>;
+    constexpr int N = Vec::N, TILE = LP_THREADS * LP_FLY;         // (of 16-byte pieces)
+    __shared__ LpShared s;
+    namespace cg = cooperative_groups;
+    const int shares = a.shares, share = blockIdx.x % shares, row = blockIdx.x / shares, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     gb_pdl_launch_dependents();
     gb_pdl_wait();
-    const int row = blockIdx.x;
-    const T* x = logits + (size_t)row * stride;
-    float m = -INFINITY;
-    for (int i = threadIdx.x; i < vocab; i += LP_THREADS) m = fmaxf(m, gb_to_float(x[i]));
-    m = gb_warp_max(m);
-    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = m;
+    const T* x = (const T*)a.logits + (size_t)row * a.stride;
+    if (tid == 0) { s.count = 0; s.found = 0; }
     __syncthreads();
-    for (int w = 0; w < LP_THREADS / 32; ++w) m = fmaxf(m, s[w]);
-    float z = 0.f, h = 0.f;
-    for (int i = threadIdx.x; i < vocab; i += LP_THREADS) {
-        const float d = gb_to_float(x[i]) - m, e = expf(d);
-        z += e;
-        if (e > 0.f) h = fmaf(e, d, h);
-    }
-    z = lp_block_sum(z, s);
-    h = lp_block_sum(h, s);
-    const float norm = logf(z);
-    if (threadIdx.x == 0) {
-        const int token = tokens[row];
-        logprob[row] = token >= 0 && token < vocab ? gb_to_float(x[token]) - m - norm : __uint_as_float(0x7fc00000u);
-        if (entropy) entropy[row] = norm - h / z;
-    }
-    unsigned long long last = ~0ull;
-    for (int k = 0; k < top; ++k) {
-        unsigned long long best = 0;
-        for (int i = threadIdx.x; i < vocab; i += LP_THREADS) {
-            const unsigned long long key = lp_key(gb_to_float(x[i]), i);
-            if (key < last && key > best) best = key;
-        }
+
+    // The row's 16-byte pieces, in equal shares; what lies before the first of them goes to the first share, behind the last one to the last.
+    const int lead = min(a.vocab, (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T));
+    const int pieces = (a.vocab - lead) / N, begin = (int)((long long)pieces * share / shares), end = (int)((long long)pieces * (share + 1) / shares);
+    const uint4* body = reinterpret_cast<const uint4*>(x + lead);
+    const int lo = share == 0 ? 0 : lead + begin * N, hi = share == shares - 1 ? a.vocab : lead + end * N;      // ids of this block
+    LpSums sums;
+    float most = -INFINITY, level = -INFINITY;
+    auto keep = [&](float v, int id) {
+        const int at = atomicAdd(&s.count, 1);
+        if (at < LP_KEEP) s.keep[at] = lp_key(v, id);
+    };
+    uint4 raw[LP_FLY];
+    auto load = [&](int tile) {
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
-            if (other > best) best = other;
+        for (int u = 0; u < LP_FLY; ++u) {
+            const int i = begin + tile * TILE + u * LP_THREADS + tid;
+            raw[u] = i < end ? __ldcs(body + i) : Vec::nothing();
         }
-        __syncthreads();
-        if ((threadIdx.x & 31) == 0) sk[threadIdx.x >> 5] = best;
-        __syncthreads();
-        for (int w = 0; w < LP_THREADS / 32; ++w)
-            if (sk[w] > best) best = sk[w];
-        last = best;
-        if (threadIdx.x == 0) {
-            const int id = (int)~(unsigned)best;
-            top_ids[(size_t)row * top + k] = id;
-            if (top_logprob) top_logprob[(size_t)row * top + k] = gb_to_float(x[id]) - m - norm;
+    };
+    load(0);
+    // the ragged ends, up to N - 1 numbers each, one a thread
+    const int head = share == 0 ? lead : 0, tail = share == shares - 1 ? a.vocab - lead - pieces * N : 0;
+    float odd = -INFINITY;
+    int odd_id = -1;
+    if (tid < head + tail) {
+        odd_id = tid < head ? tid : lead + pieces * N + tid - head;
+        odd = gb_to_float(x[odd_id]);
+        sums.rise(odd);
+        sums.add(odd, sums.r == -INFINITY ? 0.f : sums.r);
+        if (tid < head) most = odd;             // (what has the highest ids says nothing about equal numbers before it)
+    }
+    const int tiles = max(1, (end - begin + TILE - 1) / TILE);
+    for (int tile = 0; tile < tiles; ++tile) {
+        float v[LP_FLY][N], up = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < LP_FLY; ++u) {
+            Vec::unpack(raw[u], v[u]);
+#pragma unroll
+            for (int e = 0; e < N; ++e) up = fmaxf(up, v[u][e]);
+        }
+        if (tile + 1 < tiles) load(tile + 1);
+        sums.rise(up);
+        const float from = sums.r == -INFINITY ? 0.f : sums.r;
+#pragma unroll
+        for (int u = 0; u < LP_FLY; ++u)
+#pragma unroll
+            for (int e = 0; e < N; ++e) sums.add(v[u][e], from);
+        if (a.top) {
+            most = fmaxf(most, up);
+            const bool fresh = (tile & (tile + 1)) == 0;
+            if (fresh) {
+                level = lp_level(s, most, a.top);
+                if (tile == 0 && odd_id >= 0 && odd >= level && odd > -INFINITY) keep(odd, odd_id);
+            }
+            if (fresh ? up >= level && up > -INFINITY : up > level) {
+#pragma unroll
+                for (int u = 0; u < LP_FLY; ++u)
+#pragma unroll
+                    for (int e = 0; e < N; ++e)
+                        if (fresh ? v[u][e] >= level && v[u][e] > -INFINITY : v[u][e] > level)
+                            keep(v[u][e], lead + (begin + tile * TILE + u * LP_THREADS + tid) * N + e);
+            }
         }
     }
+    // ---- the block's sums
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const float r = __shfl_xor_sync(0xffffffffu, sums.r, o), z = __shfl_xor_sync(0xffffffffu, sums.z, o), h = __shfl_xor_sync(0xffffffffu, sums.h, o);
+        sums.join(r, z, h);
+    }
+    if (lane == 0) { s.r[warp] = sums.r; s.z[warp] = sums.z; s.h[warp] = sums.h; }
+    __syncthreads();
+    const bool searched = a.top && s.count > LP_KEEP;
+    if (searched) {                             // k times through the block's share of the row
+        unsigned long long last = ~0ull;
+        for (int k = 0; k < a.top; ++k) {
+            unsigned long long best = 0;
+            for (int i = lo + tid; i < hi; i += LP_THREADS) {
+                const float v = gb_to_float(x[i]);
+                const unsigned long long key = lp_key(v, i);
+                if (v > -INFINITY && key < last && key > best) best = key;
+            }
+            best = lp_warp_max(best);
+            __syncthreads();
+            if (lane == 0) s.keep[warp] = best;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < LP_WARPS; ++w)
+                if (s.keep[w] > best) best = s.keep[w];
+            if (best == 0) break;
+            last = best;
+            if (tid == 0) { s.best[k] = best; s.found = k + 1; }
+        }
+        __syncthreads();
+    }
+    if (warp == 0) {
+        LpSums all;
+        if (lane < LP_WARPS) { all.r = s.r[lane]; all.z = s.z[lane]; all.h = s.h[lane]; }
+#pragma unroll
+        for (int o = LP_WARPS / 2; o > 0; o >>= 1) {
+            const float r = __shfl_xor_sync(0xffffffffu, all.r, o), z = __shfl_xor_sync(0xffffffffu, all.z, o), h = __shfl_xor_sync(0xffffffffu, all.h, o);
+            all.join(r, z, h);
+        }
+        if (lane == 0) { s.all[0] = all.r; s.all[1] = all.z; s.all[2] = all.h; }
+        if (a.top && !searched) {
+            const int count = s.count;
+            unsigned long long last = ~0ull;
+            for (int k = 0; k < a.top; ++k) {
+                unsigned long long best = 0;
+                for (int i = lane; i < count; i += 32) {
+                    const unsigned long long key = s.keep[i];
+                    if (key < last && key > best) best = key;
+                }
+                best = lp_warp_max(best);
+                if (best == 0) break;
+                last = best;
+                if (lane == 0) { s.best[k] = best; s.found = k + 1; }
+            }
+        }
+    }
+    // ---- the row's: the first block of a cluster takes what the others have
+    if (shares > 1) cg::this_cluster().sync();
+    if (share == 0 && warp == 0) {
+        __syncwarp();
+        LpSums all;
+        auto of = [&](int b) -> const LpShared* { return shares > 1 ? cg::this_cluster().map_shared_rank(&s, b) : &s; };
+        if (lane < shares) { const LpShared* o = of(lane); all.r = o->all[0]; all.z = o->all[1]; all.h = o->all[2]; }
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) {
+            const float r = __shfl_xor_sync(0xffffffffu, all.r, o), z = __shfl_xor_sync(0xffffffffu, all.z, o), h = __shfl_xor_sync(0xffffffffu, all.h, o);
+            all.join(r, z, h);
+        }
+        const float nan = __uint_as_float(0x7fc00000u);
+        const bool none = !(all.r > -INFINITY) || all.r == INFINITY;
+        const float r = __shfl_sync(0xffffffffu, none ? nan : all.r, 0), norm = __shfl_sync(0xffffffffu, logf(all.z), 0);
+        if (lane == 0) {
+            const int token = a.tokens[row];
+            a.logprob[row] = token >= 0 && token < a.vocab ? gb_to_float(x[token]) - r - norm : nan;
+            if (a.entropy) a.entropy[row] = none ? nan : norm - all.h / all.z;
+        }
+        if (a.top) {
+            int* ids = a.top_ids + (size_t)row * a.top;
+            float* lps = a.top_logprob ? a.top_logprob + (size_t)row * a.top : nullptr;
+            // lane b walks down block b's list
+            const LpShared* mine = of(lane < shares ? lane : 0);
+            const int has = lane < shares ? mine->found : 0;
+            int next = 0, k = 0;
+            unsigned long long key = has > 0 ? mine->best[0] : 0;
+            for (; k < a.top; ++k) {
+                const unsigned long long best = lp_warp_max(key);
+                if (best == 0) break;
+                if (key == best) key = ++next < has ? mine->best[next] : 0;
+                if (lane == 0) {
+                    const int id = (int)~(unsigned)best;
+                    ids[k] = id;
+                    if (lps) lps[k] = gb_to_float(x[id]) - r - norm;
+                }
+            }
+            // fewer tokens have a probability: the first ones that have none, then those that are NaN
+            for (int pass = 0; pass < 2 && k < a.top; ++pass)
+                for (int i0 = 0; i0 < a.vocab && k < a.top; i0 += 32) {
+                    const int i = i0 + lane;
+                    const float v = i < a.vocab ? gb_to_float(x[i]) : 0.f;
+                    unsigned hits = __ballot_sync(0xffffffffu, i < a.vocab && (pass == 0 ? v == -INFINITY : v != v));
+                    for (; hits && k < a.top; hits &= hits - 1, ++k)
+                        if (lane == 0) {
+                            const int id = i0 + __ffs(hits) - 1;
+                            ids[k] = id;
+                            if (lps) lps[k] = gb_to_float(x[id]) - r - norm;
+                        }
+                }
+        }
+    }
+    if (shares > 1) cg::this_cluster().sync();   // (its memory is read until here)
 }
 
+// top_ids [rows, top] (top 0: none), top_logprob and entropy may be missing. Rows `stride` numbers apart.
 GB_EXPORT int gb_token_logprobs(const void* logits, int dtype, long long stride, const int* tokens, float* logprob, float* entropy,
                                 float* top_logprob, int* top_ids, int top, int rows, int vocab, cudaStream_t stream) {
     GB_REQUIRE(rows >= 0 && vocab > 0 && (rows <= 1 || stride >= vocab), "gb_token_logprobs: bad sizes rows=%d vocab=%d", rows, vocab);
     GB_REQUIRE(top >= 0 && top <= LP_MAX_TOP && top <= vocab, "gb_token_logprobs: %d alternatives of %d tokens (at most %d)", top, vocab, LP_MAX_TOP);
     GB_REQUIRE(dtype == GB_F32 || dtype == GB_BF16, "gb_token_logprobs: unsupported dtype %d", dtype);
+    GB_REQUIRE(rows < (1 << 28), "gb_token_logprobs: %d rows are too many for one launch", rows);
     if (rows == 0) return 0;
     GB_REQUIRE(logits && tokens && logprob && (top == 0 || top_ids), "gb_token_logprobs: a tensor is missing");
-    const dim3 grid(rows), block(LP_THREADS);
-    if (dtype == GB_F32)
-        gb_launch(GB_PDL_ELEMENTWISE, logprobs_kernel<float>, grid, block, 0, stream, (const float*)logits, stride, tokens, logprob, entropy,
-                  top_logprob, top_ids, top, vocab);
-    else
-        gb_launch(GB_PDL_ELEMENTWISE, logprobs_kernel<__nv_bfloat16>, grid, block, 0, stream, (const __nv_bfloat16*)logits, stride, tokens, logprob,
-                  entropy, top_logprob, top_ids, top, vocab);
+    LpArgs a = {logits, stride, tokens, logprob, entropy, top_logprob, top_ids, top, vocab, 1};
+    const int size = dtype == GB_F32 ? 4 : 2;
+    // shares of at least 16 KB of a row while there is room for them
+    int shares = 8;
+    while (shares > 1 && ((long long)rows * shares > 2 * 148 || (long long)vocab * size < shares * 16384ll)) shares /= 2;
+    cudaLaunchConfig_t cfg = {};
+    a.shares = shares;
+    cfg.gridDim = dim3(shares * rows);
+    cfg.blockDim = dim3(LP_THREADS);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    int na = 0;
+    if (gb_pdl_enabled() & GB_PDL_ELEMENTWISE) {
+        attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[na].val.programmaticStreamSerializationAllowed = 1;
+        ++na;
+    }
+    if (shares > 1) {
+        attr[na].id = cudaLaunchAttributeClusterDimension;
+        attr[na].val.clusterDim.x = shares;
+        attr[na].val.clusterDim.y = attr[na].val.clusterDim.z = 1;
+        ++na;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = na;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, dtype == GB_F32 ? logprobs_kernel<float> : logprobs_kernel<__nv_bfloat16>, a);
+    if (e != cudaSuccess) {
+        gb_set_error("gb_token_logprobs: launch failed: %s", cudaGetErrorString(e));
+        return 2;
+    }
     return gb_check_launch("gb_token_logprobs");
 }
