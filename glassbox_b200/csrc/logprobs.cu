@@ -7,8 +7,8 @@
 //
 // What bounds it is reading the logits, once. A block takes a row (or, of few rows, a share of one: the blocks of a cluster add up) in
 // tiles of 4,096; the next tile's loads are under way while a tile is worked on. Every thread keeps a reference, Z and H of its own. The
-// most probable tokens are found in the same pass: k numbers at least as large as a threshold are known to exist once the threshold is the
-// smallest over the warps of each warp's ceil(k / warps)-th largest of its threads' maxima; only what reaches it is written down (some dozens a tile,
+// most probable tokens are found in the same pass: k numbers at least as large as a threshold are known to exist if it is the k-th
+// largest of the threads' maxima (four of each warp are looked at); only what reaches it is written down (some k numbers in the first tile,
 // fewer and fewer as the threshold rises, which it does in tiles 0, 1, 3, 7 ...), and one warp picks the k largest of that. Behind the tile that set it a number
 // has to be larger, since equal ones of higher ids come too late. A row that leaves more than 2,048 candidates (one that only rises, or that holds thousands of
 // equal largest numbers) is searched k times instead.
@@ -18,7 +18,7 @@
 
 constexpr int LP_THREADS = 256, LP_WARPS = LP_THREADS / 32;
 constexpr int LP_MAX_TOP = 32;
-constexpr int LP_FLY = 4;               // 16-byte loads of a thread and tile
+constexpr int LP_EACH = 16;             // numbers of a thread and tile
 constexpr int LP_KEEP = 2048;            // candidates
 
 // A logit as a whole number of the same order; ties between ids are broken by the low half of (order, ~id).
@@ -29,6 +29,9 @@ __device__ __forceinline__ unsigned lp_order(float x) {
     return b >> 31 ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ unsigned long long lp_key(float x, int id) { return (unsigned long long)lp_order(x) << 32 | (unsigned)~id; }
+__device__ __forceinline__ float lp_number(unsigned order) {            // the logit again (-0 as 0)
+    return order == 0u ? __uint_as_float(0x7fc00000u) : order >> 31 ? __uint_as_float(order & 0x7fffffffu) : __uint_as_float(~order);
+}
 __device__ __forceinline__ float lp_max_nan(float a, float b) {         // NaN where a is one
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -38,6 +41,12 @@ __device__ __forceinline__ float lp_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// The next smaller float32 of a number.
+__device__ __forceinline__ float lp_below(float x) {
+    const int b = __float_as_int(x);
+    return x == 0.f ? __uint_as_float(0x80000001u) : __int_as_float(b < 0 ? b + 1 : b - 1);
 }
 
 // The largest key of a warp's.
@@ -81,7 +90,8 @@ struct LpArgs {
 
 struct LpShared {
     float r[LP_WARPS], z[LP_WARPS], h[LP_WARPS];
-    float level[LP_WARPS];
+    unsigned maxima[LP_MAX_TOP];
+    float level;
     float all[3];                              // of the block: reference, Z, H
     int count, found;
     unsigned long long best[LP_MAX_TOP];        // of the block, falling
@@ -114,36 +124,45 @@ struct LpSums {
     }
 };
 
-// How large a number has to be so that `top` are at least as large: the smallest over the warps of the ceil(top / warps)-th largest thread's maximum.
+// How large a number has to be so that `top` are at least as large: the top-th largest of each warp's four largest threads' maxima.
 __device__ __forceinline__ float lp_level(LpShared& s, float most, int top) {
-    const int lane = threadIdx.x & 31, nth = (top + LP_WARPS - 1) / LP_WARPS;      // 1 .. 4
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     unsigned left = lp_order(most);
-    if (left == 0u) left = lp_order(-INFINITY);
-    unsigned level = 0;
-    for (int i = 0; i < nth; ++i) {
-        level = __reduce_max_sync(0xffffffffu, left);
+#pragma unroll
+    for (int i = 0; i < LP_MAX_TOP / LP_WARPS; ++i) {
+        const unsigned level = __reduce_max_sync(0xffffffffu, left);
         const unsigned who = __ballot_sync(0xffffffffu, left == level);
         if (lane == __ffs(who) - 1) left = 0;
+        if (lane == 0) s.maxima[warp * (LP_MAX_TOP / LP_WARPS) + i] = level;
     }
-    __syncthreads();                            // (the level before has been read)
-    if (lane == 0) s.level[threadIdx.x >> 5] = level >> 31 ? __uint_as_float(level & 0x7fffffffu) : __uint_as_float(~level);
     __syncthreads();
-    float v = s.level[0];
+    if (warp == 0) {
+        const unsigned mine = s.maxima[lane];
+        int before = 0;                         // how many come before this one in falling order
 #pragma unroll
-    for (int w = 1; w < LP_WARPS; ++w) v = fminf(v, s.level[w]);
-    return v;
+        for (int i = 0; i < LP_MAX_TOP; ++i) {
+            const unsigned other = __shfl_sync(0xffffffffu, mine, i);
+            before += other > mine || (other == mine && i < lane);
+        }
+        if (before == top - 1) s.level = lp_number(mine);
+    }
+    __syncthreads();
+    return s.level;
 }
 
 template <typename T>
 __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LpArgs a) {
     using Vec = LpVec<T>;
-    constexpr int N = Vec::N, TILE = LP_THREADS * LP_FLY;         // (of 16-byte pieces)
+    constexpr int N = Vec::N, LP_FLY = LP_EACH / N, TILE = LP_THREADS * LP_FLY;         // (of 16-byte pieces)
+    constexpr int AHEAD = 16 / sizeof(T) / 4;                                            // tiles that are under way beside the one worked on
     __shared__ LpShared s;
     namespace cg = cooperative_groups;
     const int shares = a.shares, share = blockIdx.x % shares, row = blockIdx.x / shares, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     gb_pdl_launch_dependents();
     gb_pdl_wait();
     const T* x = (const T*)a.logits + (size_t)row * a.stride;
+    const int token = tid == 0 && share == 0 ? a.tokens[row] : -1;
+    const float own = token >= 0 && token < a.vocab ? gb_to_float(x[token]) : 0.f;
     if (tid == 0) { s.count = 0; s.found = 0; }
     __syncthreads();
 
@@ -158,15 +177,16 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LpArgs a)
         const int at = atomicAdd(&s.count, 1);
         if (at < LP_KEEP) s.keep[at] = lp_key(v, id);
     };
-    uint4 raw[LP_FLY];
-    auto load = [&](int tile) {
+    uint4 raw[AHEAD][LP_FLY];
+    auto load = [&](int tile, uint4 (&to)[LP_FLY]) {
 #pragma unroll
         for (int u = 0; u < LP_FLY; ++u) {
             const int i = begin + tile * TILE + u * LP_THREADS + tid;
-            raw[u] = i < end ? __ldcs(body + i) : Vec::nothing();
+            to[u] = i < end ? __ldcs(body + i) : Vec::nothing();
         }
     };
-    load(0);
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) load(i, raw[i]);
     // the ragged ends, up to N - 1 numbers each, one a thread
     const int head = share == 0 ? lead : 0, tail = share == shares - 1 ? a.vocab - lead - pieces * N : 0;
     float odd = -INFINITY;
@@ -180,14 +200,20 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LpArgs a)
     }
     const int tiles = max(1, (end - begin + TILE - 1) / TILE);
     for (int tile = 0; tile < tiles; ++tile) {
-        float v[LP_FLY][N], up = -INFINITY;
+        float v[LP_FLY][N], ups[LP_FLY], up = -INFINITY;
 #pragma unroll
         for (int u = 0; u < LP_FLY; ++u) {
-            Vec::unpack(raw[u], v[u]);
+            Vec::unpack(raw[0][u], v[u]);
+            ups[u] = v[u][0];
 #pragma unroll
-            for (int e = 0; e < N; ++e) up = fmaxf(up, v[u][e]);
+            for (int e = 1; e < N; ++e) ups[u] = fmaxf(ups[u], v[u][e]);
+            up = fmaxf(up, ups[u]);
         }
-        if (tile + 1 < tiles) load(tile + 1);
+#pragma unroll
+        for (int i = 0; i + 1 < AHEAD; ++i)
+#pragma unroll
+            for (int u = 0; u < LP_FLY; ++u) raw[i][u] = raw[i + 1][u];
+        load(tile + AHEAD, raw[AHEAD - 1]);
         sums.rise(up);
         const float from = sums.r == -INFINITY ? 0.f : sums.r;
 #pragma unroll
@@ -201,13 +227,15 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LpArgs a)
                 level = lp_level(s, most, a.top);
                 if (tile == 0 && odd_id >= 0 && odd >= level && odd > -INFINITY) keep(odd, odd_id);
             }
-            if (fresh ? up >= level && up > -INFINITY : up > level) {
+            // (at the tile that set it a number at the threshold counts; minus infinity never does)
+            const float above = fresh && level > -INFINITY ? lp_below(level) : level;
+            if (up > above) {
 #pragma unroll
                 for (int u = 0; u < LP_FLY; ++u)
+                    if (ups[u] > above)
 #pragma unroll
-                    for (int e = 0; e < N; ++e)
-                        if (fresh ? v[u][e] >= level && v[u][e] > -INFINITY : v[u][e] > level)
-                            keep(v[u][e], lead + (begin + tile * TILE + u * LP_THREADS + tid) * N + e);
+                        for (int e = 0; e < N; ++e)
+                            if (v[u][e] > above) keep(v[u][e], lead + (begin + tile * TILE + u * LP_THREADS + tid) * N + e);
             }
         }
     }
@@ -253,10 +281,16 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LpArgs a)
         if (lane == 0) { s.all[0] = all.r; s.all[1] = all.z; s.all[2] = all.h; }
         if (a.top && !searched) {
             const int count = s.count;
-            unsigned long long last = ~0ull;
+            constexpr int HELD = 4;             // a lane's candidates that stay in registers: mostly all of them
+            unsigned long long held[HELD], last = ~0ull;
+#pragma unroll
+            for (int i = 0; i < HELD; ++i) held[i] = lane + 32 * i < count ? s.keep[lane + 32 * i] : 0;
             for (int k = 0; k < a.top; ++k) {
                 unsigned long long best = 0;
-                for (int i = lane; i < count; i += 32) {
+#pragma unroll
+                for (int i = 0; i < HELD; ++i)
+                    if (held[i] < last && held[i] > best) best = held[i];
+                for (int i = lane + 32 * HELD; i < count; i += 32) {
                     const unsigned long long key = s.keep[i];
                     if (key < last && key > best) best = key;
                 }
@@ -283,26 +317,26 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LpArgs a)
         const bool none = !(all.r > -INFINITY) || all.r == INFINITY;
         const float r = __shfl_sync(0xffffffffu, none ? nan : all.r, 0), norm = __shfl_sync(0xffffffffu, logf(all.z), 0);
         if (lane == 0) {
-            const int token = a.tokens[row];
-            a.logprob[row] = token >= 0 && token < a.vocab ? gb_to_float(x[token]) - r - norm : nan;
+            a.logprob[row] = token >= 0 && token < a.vocab ? own - r - norm : nan;
             if (a.entropy) a.entropy[row] = none ? nan : norm - all.h / all.z;
         }
         if (a.top) {
-            int* ids = a.top_ids + (size_t)row * a.top;
-            float* lps = a.top_logprob ? a.top_logprob + (size_t)row * a.top : nullptr;
-            // lane b walks down block b's list
-            const LpShared* mine = of(lane < shares ? lane : 0);
-            const int has = lane < shares ? mine->found : 0;
-            int next = 0, k = 0;
-            unsigned long long key = has > 0 ? mine->best[0] : 0;
-            for (; k < a.top; ++k) {
-                const unsigned long long best = lp_warp_max(key);
-                if (best == 0) break;
-                if (key == best) key = ++next < has ? mine->best[next] : 0;
-                if (lane == 0) {
-                    const int id = (int)~(unsigned)best;
-                    ids[k] = id;
-                    if (lps) lps[k] = gb_to_float(x[id]) - r - norm;
+            // lane b walks down block b's list; the k-th largest goes to lane k
+            unsigned long long out = 0;
+            int k = 0;
+            if (shares == 1) {
+                k = s.found;
+                if (lane < k) out = s.best[lane];
+            } else {
+                const LpShared* mine = of(lane < shares ? lane : 0);
+                const int has = lane < shares ? mine->found : 0;
+                int next = 0;
+                unsigned long long key = has > 0 ? mine->best[0] : 0;
+                for (; k < a.top; ++k) {
+                    const unsigned long long best = lp_warp_max(key);
+                    if (best == 0) break;
+                    if (lane == k) out = best;
+                    if (key == best) key = ++next < has ? mine->best[next] : 0;
                 }
             }
             // fewer tokens have a probability: the first ones that have none, then those that are NaN
@@ -312,12 +346,12 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LpArgs a)
                     const float v = i < a.vocab ? gb_to_float(x[i]) : 0.f;
                     unsigned hits = __ballot_sync(0xffffffffu, i < a.vocab && (pass == 0 ? v == -INFINITY : v != v));
                     for (; hits && k < a.top; hits &= hits - 1, ++k)
-                        if (lane == 0) {
-                            const int id = i0 + __ffs(hits) - 1;
-                            ids[k] = id;
-                            if (lps) lps[k] = gb_to_float(x[id]) - r - norm;
-                        }
+                        if (lane == k) out = lp_key(pass == 0 ? -INFINITY : nan, i0 + __ffs(hits) - 1);
                 }
+            if (lane < a.top) {
+                a.top_ids[(size_t)row * a.top + lane] = (int)~(unsigned)out;
+                if (a.top_logprob) a.top_logprob[(size_t)row * a.top + lane] = lp_number((unsigned)(out >> 32)) - r - norm;
+            }
         }
     }
     if (shares > 1) cg::this_cluster().sync();   // (its memory is read until here)
