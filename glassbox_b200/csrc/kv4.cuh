@@ -23,6 +23,13 @@ constexpr int KV4_MAX_HD = 256;
 
 __host__ __device__ __forceinline__ constexpr int kv4_tile_bytes(int hd) { return 9 * hd; }
 
+// Quotients by a divisor that a launch fixes: the high half of the product with 2^32 / d rounded up, exact while x d < 2^32.
+struct Kv4Div {
+    unsigned d, m;
+    __host__ Kv4Div(int divisor = 1) : d((unsigned)divisor), m(divisor > 1 ? (unsigned)(((1ull << 32) + divisor - 1) / divisor) : 0u) {}
+    __device__ __forceinline__ int of(int x) const { return d == 1u ? x : (int)__umulhi((unsigned)x, m); }
+};
+
 // The tile of token `off` of a page of kv head `head`, counted over the whole pool.
 __device__ __forceinline__ long long kv4_tile(long long page, int head, int off, int nkv, int page_size) {
     return (page * nkv + head) * (page_size / KV4_TILE) + off / KV4_TILE;
@@ -39,4 +46,5 @@ __device__ __forceinline__ float kv4_code(unsigned word, int j) { return (float)
 #define KV4_REQUIRE_SIZES(what)                                                                                                              \
     GB_REQUIRE(nkv > 0 && hd > 0 && hd % KV4_GROUP == 0 && hd <= KV4_MAX_HD, what ": head size %d must be a multiple of 32 up to 256", hd); \
     GB_REQUIRE(page_size > 0 && page_size % KV4_TILE == 0, what ": page size %d must be a multiple of 16", page_size);                       \
-    GB_REQUIRE(num_pages > 0 && num_pages * page_size < (1ll << 31), what ": the pool has %lld pages of %d tokens", (long long)num_pages, page_size);
+    GB_REQUIRE(num_pages > 0 && num_pages * page_size < (1ll << 31) && num_pages * page_size / KV4_TILE * nkv < (1ll << 31),               \
+               what ": a pool of %lld pages of %d tokens and %d heads is too large", (long long)num_pages, page_size, nkv);

@@ -5,16 +5,17 @@
 // All three only move memory. The sums that matter are bytes: a row of a wide layout (32/8 heads of 128, bfloat16) brings 12 KB in, 8 KB
 // of queries out and 1.1 KB of cache out.
 //
-// The rounding, for numbers y of a group (float32, after the rotation): one 32-bit key per number, its magnitude's bits with "not
-// negative" in the lowest, has the group's m as its maximum, infinities and NaN above every number; m's bits less 3 in the
-// exponent, rounded to four bits after the leading one, are |d|. The quotient y / d is the product with the reciprocal and one
-// correction by the remainder (exact in a fused multiply-add), so that a number half way between two codes is told as such: with bfloat16
-// values that is one in dozens, and ties go to the even code.
+// The rounding, for numbers y of a group: one whole-number key per number, its magnitude's bits with "not negative" in the lowest, has
+// the group's m as its maximum, infinities and NaN above every number; m's bits less 3 in the exponent, rounded to four bits after the leading
+// one, are |d|. A value's quotient y / d is the product with the reciprocal and one correction by the remainder (exact in a fused multiply-add),
+// so that a number half way between two codes is told as such: with bfloat16 values that is one in dozens, and ties go to the even
+// code. A rotated key is carried as two float32 (see kv4_turn2), so that its code and scale are those of the exact product of the
+// rotation; rounded to one float32 first, one number in some 10^6 gets the neighbouring code.
 #include "kv4.cuh"
 
 #include <type_traits>
 
-constexpr int KV4_THREADS = 256;
+constexpr int KV4_THREADS = 128;
 
 template <typename T, int N> struct Kv4Load;      // N neighbouring numbers as float32 (N * sizeof(T) bytes, aligned to 16 or to all of them)
 template <> struct Kv4Load<float, 8> {
@@ -105,18 +106,55 @@ __device__ __forceinline__ float kv4_make_scale(unsigned most) {
     return __uint_as_float(d | (most & 1u) << 31);                         // (m positive: d negative)
 }
 
-// Codes s + 8 of N numbers, N nibbles from the low end on.
+// A turned key as the sum of two float32, the first the nearest to the sum (what a float32 rounding would drop decides which code a number
+// next to a border between two gets, and which scale): products with their errors by fused multiply-add, the sum with its error as Knuth's
+// (The Art of Computer Programming 2, 4.2.2). x the channel's own number, o its partner's.
+__device__ __forceinline__ void kv4_turn2(float& x, float& lo, float o, float2 cs, bool second) {
+    o = second ? o : -o;
+    const float p = x * cs.x, q = o * cs.y, h = p + q, b = h - p;
+    const float l = ((p - (h - b)) + (q - b)) + (fmaf(x, cs.x, -p) + fmaf(o, cs.y, -q));
+    x = h + l;
+    lo = l - (x - h);
+}
+
+// The key whose maximum over a group names its m, of such numbers: the first part's magnitude, then how far the second goes beyond it, "not
+// negative" in the lowest bit.
+__device__ __forceinline__ unsigned long long kv4_most2(float hi, float lo) {
+    const unsigned b = __float_as_uint(hi);
+    const float beyond = (b >> 31 ? -lo : lo) + 0.f;                   // (no -0)
+    const unsigned l = __float_as_uint(beyond), order = l >> 31 ? ~l : l | 0x80000000u;
+    return (unsigned long long)(b & 0x7fffffffu) << 32 | (order & ~1u) | (b >> 31 ^ 1u);
+}
+
+// The scale from that key. Only where the first part lies half way between two scales does the second decide.
+__device__ __forceinline__ float kv4_make_scale2(unsigned long long most) {
+    const unsigned size = (unsigned)(most >> 32), order = (unsigned)most & ~1u;
+    if (size >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
+    if (size < 0x05000000u) return 0.f;
+    unsigned d = size - (3u << 23);
+    const unsigned even = (d >> 19) & 1u, up = order > 0x80000000u ? 1u : order < 0x80000000u ? 0u : even;
+    d = (d + 0x3ffffu + ((d & 0x7ffffu) == 0x40000u ? up : even)) & 0xfff80000u;
+    return __uint_as_float(d | (unsigned)(most & 1u) << 31);
+}
+
+// Codes s + 8 of N numbers hi + lo, N nibbles from the low end on. s is the whole number nearest to hi / d by the hardware's reciprocal (adding
+// 1.5 2^23 rounds to one); what it leaves, hi - s d (exact) and lo, is then compared with half a step.
 template <int N>
-__device__ __forceinline__ unsigned kv4_codes(const float (&y)[N], float d) {
+__device__ __forceinline__ unsigned kv4_codes(const float (&hi)[N], const float (&lo)[N], float d) {
     if (!(fabsf(d) > 0.f)) return 0x88888888u;                             // nothing, or NaN: s = 0
-    const float r = 1.0f / d;
+    constexpr float WHOLE = 12582912.f;
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+    const float half = 0.5f * fabsf(d), toward = d < 0.f ? -1.f : 1.f;
     unsigned w = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        float q = y[i] * r;
-        q = fmaf(fmaf(-q, d, y[i]), r, q);
-        const int s = __float2int_rn(fminf(fmaxf(q, -8.f), 7.f)) + 8;
-        w |= (unsigned)s << (4 * i);
+        const float t = fmaf(hi[i], r, WHOLE);
+        float s = t - WHOLE;
+        const float left = fmaf(-s, d, hi[i]);
+        const float over = (fabsf(left) - half) + (left < 0.f ? -lo[i] : lo[i]);
+        if (over > 0.f || (over == 0.f && (__float_as_uint(t) & 1u))) s += left < 0.f ? -toward : toward;
+        w |= (__float_as_uint(fminf(fmaxf(s, -8.f), 7.f) + (WHOLE + 8.f)) & 15u) << (4 * i);
     }
     return w;
 }
@@ -134,25 +172,24 @@ struct Kv4WriteArgs {
     const int* slots;
     unsigned char* kcache;
     unsigned char* vcache;
-    int n, nh, nkv, hd, rot, max_pos, page_size, write_kv;
+    int nh, nkv, hd, rot, max_pos, page_size, write_kv;
     long long num_slots;
     int* status;
-    int units, units_v, units_k, pairs;      // work items of a row: values, keys, then queries; items of a query head
+    int units_v, units_k, units_q;           // work items of a row: values, keys, queries
+    Kv4Div by_w, by_g, by_pairs;             // pairs of groups, groups, items of a query head
 };
 
-// Work items of a row, one a thread: values (four channels in each of two neighbouring groups: a word of codes), eight lanes to a
-// pair of groups; keys (eight channels of a group: a word), four lanes to a group; queries (eight pairs of channels, or eight channels
-// that do not turn). WIDE: everything starts on 16 bytes and rot / 2 is a multiple of 8.
+// One row a block (blockIdx.y: its items KV4_THREADS at a time). Work items, one a thread: values (four channels in each of two neighbouring
+// groups: a word of codes), eight lanes to a pair of groups; keys (eight channels of a group: a word), four lanes to a group; queries
+// (eight pairs of channels, or eight channels that do not turn). WIDE: everything starts on 16 bytes and rot / 2 is a multiple of 8.
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(KV4_THREADS) kv4_write_kernel(const Kv4WriteArgs a) {
     gb_pdl_launch_dependents();
     gb_pdl_wait();
-    const unsigned at = blockIdx.x * KV4_THREADS + threadIdx.x;
-    const int row = (int)(at / (unsigned)a.units), item = (int)(at % (unsigned)a.units);
-    if (row >= a.n) return;
+    const int row = blockIdx.x, item = blockIdx.y * KV4_THREADS + threadIdx.x;
     const int pos = a.positions[row];
     if (pos < 0) return;                     // a padding row: nothing to turn, nothing to store
-    const long long slot = a.write_kv ? a.slots[row] : 0;
+    const int slot = a.write_kv ? a.slots[row] : 0;
     const bool rotate = a.table != nullptr && pos < a.max_pos, store = a.write_kv && slot >= 0 && slot < a.num_slots;
     if (item == 0 && ((a.table != nullptr && !rotate) || (a.write_kv && !store)))
         atomicOr(a.status, (a.table != nullptr && !rotate ? GB_STATUS_BAD_POSITION : 0) | (a.write_kv && !store ? GB_STATUS_BAD_SLOT : 0));
@@ -162,11 +199,9 @@ __global__ void __launch_bounds__(KV4_THREADS) kv4_write_kernel(const Kv4WriteAr
 
     if (item < a.units_v + a.units_k) {
         if (!store) return;                  // (the same for all items of a row: no lane of a group is missing)
-        const int off = (int)(slot % a.page_size);
-        const long long page = slot / a.page_size;
-        const int r = off % KV4_TILE;
+        const int page = slot / a.page_size, off = slot - page * a.page_size, r = off % KV4_TILE;
         if (item < a.units_v) {
-            const int W = (G + 1) / 2, u = item & 7, w = (item >> 3) % W, h = (item >> 3) / W;
+            const int u = item & 7, h = a.by_w.of(item >> 3), w = (item >> 3) - h * (int)a.by_w.d;
             const bool two = 2 * w + 1 < G;
             const T* p = base + (size_t)(a.nh + a.nkv + h) * hd + 64 * w + 4 * u;
             float y0[4], y1[4] = {0.f, 0.f, 0.f, 0.f};
@@ -183,7 +218,8 @@ __global__ void __launch_bounds__(KV4_THREADS) kv4_write_kernel(const Kv4WriteAr
             unsigned char* tile = a.vcache + kv4_tile(page, h, off, a.nkv, a.page_size) * kv4_tile_bytes(hd);
             unsigned char* codes = tile + r * (hd / 2) + (u * G + 2 * w) * 2;
             unsigned short* scales = reinterpret_cast<unsigned short*>(tile + 8 * hd) + r * G + 2 * w;
-            const unsigned c0 = kv4_codes(y0, d0) & 0xffffu, c1 = kv4_codes(y1, d1) & 0xffffu;
+            const float none[4] = {0.f, 0.f, 0.f, 0.f};
+            const unsigned c0 = kv4_codes(y0, none, d0) & 0xffffu, c1 = kv4_codes(y1, none, d1) & 0xffffu;
             if (two && G % 2 == 0) {
                 *reinterpret_cast<unsigned*>(codes) = c0 | c1 << 16;
                 if (u == 0) *reinterpret_cast<unsigned*>(scales) = __float_as_uint(d0) >> 16 | (__float_as_uint(d1) & 0xffff0000u);
@@ -197,13 +233,15 @@ __global__ void __launch_bounds__(KV4_THREADS) kv4_write_kernel(const Kv4WriteAr
             }
             return;
         }
-        const int k = item - a.units_v, t = k & 3, g = (k >> 2) % G, h = (k >> 2) / G, c0 = KV4_GROUP * g + 8 * t;
+        const int k = item - a.units_v, t = k & 3, h = a.by_g.of(k >> 2), g = (k >> 2) - h * G, c0 = KV4_GROUP * g + 8 * t;
         const T* p = base + (size_t)(a.nh + h) * hd;
-        float y[8];
+        float y[8], lo[8];                   // the keys, turned: y + lo
         kv4_load<T, 8, WIDE>(p + c0, y);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) lo[j] = 0.f;
         if (rotate && c0 < a.rot) {
-            float o[8];
             if (WIDE) {
+                float o[8];
                 const bool second = c0 >= half;
                 const int i = second ? c0 - half : c0;
                 kv4_load<T, 8, WIDE>(p + (second ? i : i + half), o);
@@ -211,8 +249,8 @@ __global__ void __launch_bounds__(KV4_THREADS) kv4_write_kernel(const Kv4WriteAr
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const float4 f = cs[j];
-                    y[2 * j] = kv4_turn(y[2 * j], o[2 * j], make_float2(f.x, f.y), second);
-                    y[2 * j + 1] = kv4_turn(y[2 * j + 1], o[2 * j + 1], make_float2(f.z, f.w), second);
+                    kv4_turn2(y[2 * j], lo[2 * j], o[2 * j], make_float2(f.x, f.y), second);
+                    kv4_turn2(y[2 * j + 1], lo[2 * j + 1], o[2 * j + 1], make_float2(f.z, f.w), second);
                 }
             } else {
 #pragma unroll
@@ -220,25 +258,27 @@ __global__ void __launch_bounds__(KV4_THREADS) kv4_write_kernel(const Kv4WriteAr
                     const int c = c0 + j;
                     if (c >= a.rot) continue;
                     const bool second = c >= half;
-                    y[j] = kv4_turn(y[j], gb_to_float(p[second ? c - half : c + half]), turn[second ? c - half : c], second);
+                    kv4_turn2(y[j], lo[j], gb_to_float(p[second ? c - half : c + half]), turn[second ? c - half : c], second);
                 }
             }
         }
-        unsigned m = kv4_most(y);
+        unsigned long long m = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = max(m, kv4_most2(y[j], lo[j]));
         const unsigned mask = 0xfu << (lane & 28);
         m = max(m, __shfl_xor_sync(mask, m, 1));
         m = max(m, __shfl_xor_sync(mask, m, 2));
-        const float d = kv4_make_scale(m);
+        const float d = kv4_make_scale2(m);
         unsigned char* tile = a.kcache + kv4_tile(page, h, off, a.nkv, a.page_size) * kv4_tile_bytes(hd);
-        *reinterpret_cast<unsigned*>(tile + r * (hd / 2) + (t * G + g) * 4) = kv4_codes(y, d);
+        *reinterpret_cast<unsigned*>(tile + r * (hd / 2) + (t * G + g) * 4) = kv4_codes(y, lo, d);
         if (t == 0) reinterpret_cast<unsigned short*>(tile + 8 * hd)[r * G + g] = (unsigned short)(__float_as_uint(d) >> 16);
         return;
     }
 
     // queries
     const int k = item - a.units_v - a.units_k;
-    if (k >= a.nh * a.pairs) return;         // (items that fill a row up to a multiple of eight)
-    const int h = k / a.pairs, i = k % a.pairs;
+    if (k >= a.units_q) return;
+    const int h = a.by_pairs.of(k), i = k - h * (int)a.by_pairs.d;
     const T* p = base + (size_t)h * hd;
     T* to = (T*)a.q + (size_t)row * a.q_stride + (size_t)h * hd;
     if (WIDE) {
@@ -295,18 +335,21 @@ GB_EXPORT int gb_kv4_write(const void* qkv, long long qkv_stride, int dtype, voi
                       (q_stride * size) % 16 == 0;
     Kv4WriteArgs a = {};
     a.qkv = qkv; a.qkv_stride = qkv_stride; a.q = q; a.q_stride = q_stride; a.table = rot ? (const float2*)cos_sin : nullptr;
-    a.positions = positions; a.slots = slots; a.kcache = (unsigned char*)kcache; a.vcache = (unsigned char*)vcache; a.n = n; a.nh = nh;
+    a.positions = positions; a.slots = slots; a.kcache = (unsigned char*)kcache; a.vcache = (unsigned char*)vcache; a.nh = nh;
     a.nkv = nkv; a.hd = hd; a.rot = rot; a.max_pos = max_pos; a.page_size = page_size; a.write_kv = write_kv;
     a.num_slots = num_pages * page_size; a.status = status;
     a.units_v = write_kv ? nkv * ((G + 1) / 2) * 8 : 0;
     a.units_k = write_kv ? nkv * G * 4 : 0;
     // (channels that do not turn are copied only where the queries go somewhere else)
     const bool in_place = q == qkv && q_stride == qkv_stride;
-    a.pairs = wide ? rot / 16 + (in_place ? 0 : (hd - rot) / 8) : rot / 2 + (in_place ? 0 : hd - rot);
-    a.units = (a.units_v + a.units_k + nh * a.pairs + 7) / 8 * 8;
-    if (a.units == 0) return 0;
-    GB_REQUIRE((long long)n * a.units < (1ll << 31) - KV4_THREADS, "gb_kv4_write: %d rows are too many for one launch", n);
-    const dim3 grid(gb_ceil_div((long long)n * a.units, KV4_THREADS)), block(KV4_THREADS);
+    const int pairs = wide ? rot / 16 + (in_place ? 0 : (hd - rot) / 8) : rot / 2 + (in_place ? 0 : hd - rot);
+    a.units_q = nh * pairs;
+    a.by_w = Kv4Div((G + 1) / 2);
+    a.by_g = Kv4Div(G);
+    a.by_pairs = Kv4Div(pairs > 0 ? pairs : 1);
+    const int units = a.units_v + a.units_k + a.units_q;
+    if (units == 0) return 0;
+    const dim3 grid(n, gb_ceil_div(units, KV4_THREADS)), block(KV4_THREADS);
     if (dtype == GB_F32)
         gb_launch(GB_PDL_ELEMENTWISE, wide ? kv4_write_kernel<float, true> : kv4_write_kernel<float, false>, grid, block, 0, stream, a);
     else
@@ -314,53 +357,59 @@ GB_EXPORT int gb_kv4_write(const void* qkv, long long qkv_stride, int dtype, voi
     return gb_check_launch("gb_kv4_write");
 }
 
-// What eight channels of a key (group g, part t of four) or two times four channels of a value (part u of eight) stand for.
-__device__ __forceinline__ void kv4_key8(const unsigned char* tile, int hd, int r, int g, int t, float (&x)[8]) {
-    const unsigned w = *reinterpret_cast<const unsigned*>(tile + r * (hd / 2) + (t * (hd / KV4_GROUP) + g) * 4);
-    const float d = kv4_scale(tile, hd, r, g);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = kv4_code(w, j) * d;
-}
-__device__ __forceinline__ void kv4_value4(const unsigned char* tile, int hd, int r, int g, int u, float (&x)[4]) {
-    const unsigned w = *reinterpret_cast<const unsigned short*>(tile + r * (hd / 2) + (u * (hd / KV4_GROUP) + g) * 2);
-    const float d = kv4_scale(tile, hd, r, g);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = kv4_code(w, j) * d;
+// Eight neighbouring channels (part t of four of group g) of a key, or of a value: their codes as a word, the lowest channel's first.
+__device__ __forceinline__ unsigned kv4_word(const unsigned char* tile, int hd, int r, int g, int t, bool value) {
+    const int G = hd / KV4_GROUP;
+    const unsigned char* row = tile + r * (hd / 2);
+    if (!value) return *reinterpret_cast<const unsigned*>(row + (t * G + g) * 4);
+    return *reinterpret_cast<const unsigned short*>(row + (2 * t * G + g) * 2) | (unsigned)*reinterpret_cast<const unsigned short*>(row + ((2 * t + 1) * G + g) * 2) << 16;
 }
 
-// One thread: eight neighbouring channels of a key or of a value (two of its half words).
+// What such a word stands for, as eight bfloat16 (two a word): codes under 0x4300 are 128 + s + 8, and the product with the scale is exact.
+__device__ __forceinline__ void kv4_eight(unsigned w, unsigned short scale, uint32_t (&x)[4]) {
+    const unsigned d2 = scale | (unsigned)scale << 16, c2 = 0x43084308u;
+    uint32_t y[4];                           // channels i and i + 4
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const unsigned u = (w >> (4 * i) & 0x000f000fu) | 0x43004300u;
+        const __nv_bfloat162 v = __hmul2(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), *reinterpret_cast<const __nv_bfloat162*>(&c2)),
+                                         *reinterpret_cast<const __nv_bfloat162*>(&d2));
+        y[i] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+    x[0] = __byte_perm(y[0], y[1], 0x5410);
+    x[1] = __byte_perm(y[2], y[3], 0x5410);
+    x[2] = __byte_perm(y[0], y[1], 0x7632);
+    x[3] = __byte_perm(y[2], y[3], 0x7632);
+}
+__device__ __forceinline__ void kv4_put(__nv_bfloat16* p, const uint32_t (&x)[4]) { *reinterpret_cast<uint4*>(p) = make_uint4(x[0], x[1], x[2], x[3]); }
+__device__ __forceinline__ void kv4_put(float* p, const uint32_t (&x)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; i += 2)
+        *reinterpret_cast<uint4*>(p + 2 * i) = make_uint4(x[i] << 16, x[i] & 0xffff0000u, x[i + 1] << 16, x[i + 1] & 0xffff0000u);
+}
+
+// One row a block (blockIdx.y: its items KV4_THREADS at a time), eight neighbouring channels of a key or a value a thread.
 template <typename T>
 __global__ void __launch_bounds__(KV4_THREADS) kv4_read_kernel(const unsigned char* __restrict__ kcache, const unsigned char* __restrict__ vcache,
-                                                              const int* __restrict__ slots, T* __restrict__ k, T* __restrict__ v, int n, int nkv,
-                                                              int hd, int page_size, long long num_slots, int* __restrict__ status) {
+                                                              const int* __restrict__ slots, T* __restrict__ k, T* __restrict__ v, int nkv,
+                                                              int hd, int page_size, long long num_slots, Kv4Div by_g, int* __restrict__ status) {
     gb_pdl_launch_dependents();
     gb_pdl_wait();
-    const int per = nkv * (hd / 8);          // items of a row and tensor
-    const unsigned at = blockIdx.x * KV4_THREADS + threadIdx.x;
-    const int row = (int)(at / (unsigned)(2 * per));
-    int item = (int)(at % (unsigned)(2 * per));
-    if (row >= n) return;
-    const long long slot = slots[row];
-    if (slot < 0) return;
+    const int row = blockIdx.x, slot = slots[row], per = nkv * (hd / 8);
+    int item = blockIdx.y * KV4_THREADS + threadIdx.x;
+    if (slot < 0 || item >= 2 * per) return;
     if (slot >= num_slots) {
         if (item == 0) atomicOr(status, GB_STATUS_BAD_SLOT);
         return;
     }
     const bool value = item >= per;
     if (value) item -= per;
-    const int G = hd / KV4_GROUP, t = item & 3, g = (item >> 2) % G, h = (item >> 2) / G, off = (int)(slot % page_size), r = off % KV4_TILE;
-    const unsigned char* tile = (value ? vcache : kcache) + kv4_tile(slot / page_size, h, off, nkv, page_size) * kv4_tile_bytes(hd);
-    float x[8];
-    if (value) {
-        float lo[4], hi[4];
-        kv4_value4(tile, hd, r, g, 2 * t, lo);
-        kv4_value4(tile, hd, r, g, 2 * t + 1, hi);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) { x[j] = lo[j]; x[4 + j] = hi[j]; }
-    } else {
-        kv4_key8(tile, hd, r, g, t, x);
-    }
-    Kv4Load<T, 8>::store((value ? v : k) + ((size_t)row * nkv + h) * hd + KV4_GROUP * g + 8 * t, x);
+    const int G = hd / KV4_GROUP, t = item & 3, h = by_g.of(item >> 2), g = (item >> 2) - h * G;
+    const int page = slot / page_size, off = slot - page * page_size, r = off % KV4_TILE;
+    const unsigned char* tile = (value ? vcache : kcache) + kv4_tile(page, h, off, nkv, page_size) * kv4_tile_bytes(hd);
+    uint32_t x[4];
+    kv4_eight(kv4_word(tile, hd, r, g, t, value), reinterpret_cast<const unsigned short*>(tile + 8 * hd)[r * G + g], x);
+    kv4_put((value ? v : k) + ((size_t)row * nkv + h) * hd + KV4_GROUP * g + 8 * t, x);
 }
 
 GB_EXPORT int gb_kv4_read(const void* kcache, const void* vcache, const int* slots, void* k, void* v, int dtype, int n, int nkv, int hd,
@@ -369,64 +418,51 @@ GB_EXPORT int gb_kv4_read(const void* kcache, const void* vcache, const int* slo
     GB_REQUIRE(dtype == GB_F32 || dtype == GB_BF16, "gb_kv4_read: unsupported dtype %d", dtype);
     GB_REQUIRE(((uintptr_t)kcache | (uintptr_t)vcache | (uintptr_t)k | (uintptr_t)v) % 16 == 0, "gb_kv4_read: tensors must be 16-byte aligned");
     if (n <= 0) return 0;
-    const long long items = (long long)n * 2 * nkv * (hd / 8);
-    GB_REQUIRE(items < (1ll << 31) - KV4_THREADS, "gb_kv4_read: %d rows are too many for one launch", n);
-    const dim3 grid(gb_ceil_div(items, KV4_THREADS)), block(KV4_THREADS);
+    const dim3 grid(n, gb_ceil_div(2 * nkv * (hd / 8), KV4_THREADS)), block(KV4_THREADS);
     const unsigned char *kc = (const unsigned char*)kcache, *vc = (const unsigned char*)vcache;
+    const Kv4Div by_g(hd / KV4_GROUP);
     if (dtype == GB_F32)
-        gb_launch(GB_PDL_ELEMENTWISE, kv4_read_kernel<float>, grid, block, 0, stream, kc, vc, slots, (float*)k, (float*)v, n, nkv, hd, page_size,
-                  num_pages * page_size, status);
+        gb_launch(GB_PDL_ELEMENTWISE, kv4_read_kernel<float>, grid, block, 0, stream, kc, vc, slots, (float*)k, (float*)v, nkv, hd, page_size,
+                  num_pages * page_size, by_g, status);
     else
-        gb_launch(GB_PDL_ELEMENTWISE, kv4_read_kernel<__nv_bfloat16>, grid, block, 0, stream, kc, vc, slots, (__nv_bfloat16*)k, (__nv_bfloat16*)v, n,
-                  nkv, hd, page_size, num_pages * page_size, status);
+        gb_launch(GB_PDL_ELEMENTWISE, kv4_read_kernel<__nv_bfloat16>, grid, block, 0, stream, kc, vc, slots, (__nv_bfloat16*)k, (__nv_bfloat16*)v, nkv,
+                  hd, page_size, num_pages * page_size, by_g, status);
     return gb_check_launch("gb_kv4_read");
 }
 
-// Pages of 4 bits that the rows of a step see, as numbers into pages of the same ids: one block a page of a request, all heads.
+// Pages of 4 bits that the rows of a step see, as numbers into pages of the same ids: one block a page of a request and kv head.
 // Numbers of tokens outside the request's range (before its first row's window, behind its last row) that are NaN become zero: the
 // kernels that read the pages multiply what they mask by zero.
 template <typename T>
 __global__ void __launch_bounds__(KV4_THREADS) kv4_expand_kernel(const unsigned char* __restrict__ kcache, const unsigned char* __restrict__ vcache,
                                                                 T* __restrict__ k, T* __restrict__ v, const int* __restrict__ block_tables, int max_pages,
                                                                 const int* __restrict__ seq_first_row, const int* __restrict__ seq_start_pos, int nkv,
-                                                                int hd, int page_size, long long num_pages, int window, int* __restrict__ status) {
+                                                                int hd, int page_size, long long num_pages, int window, Kv4Div by_row,
+                                                                int* __restrict__ status) {
     gb_pdl_launch_dependents();
     gb_pdl_wait();
-    const int seq = blockIdx.y, start = seq_start_pos[seq], rows = seq_first_row[seq + 1] - seq_first_row[seq];
+    const int seq = blockIdx.z, start = seq_start_pos[seq], rows = seq_first_row[seq + 1] - seq_first_row[seq], h = blockIdx.y;
     if (start < 0 || rows <= 0) return;
     const long long end = (long long)start + rows, first = gb_first_key(start, window > 0 ? window : 0);
     const long long begin = (long long)blockIdx.x * page_size;
     if (begin >= end || begin + page_size <= first) return;
     const long long page = block_tables[(size_t)seq * max_pages + blockIdx.x];
     if (page < 0 || page >= num_pages) {
-        if (threadIdx.x == 0) atomicOr(status, GB_STATUS_BAD_SLOT);
+        if (threadIdx.x == 0 && h == 0) atomicOr(status, GB_STATUS_BAD_SLOT);
         return;
     }
-    const int G = hd / KV4_GROUP, per = page_size * G * 4;         // items of a head and tensor
-    for (int i = threadIdx.x; i < 2 * nkv * per; i += KV4_THREADS) {
-        const bool value = i >= nkv * per;
-        int item = value ? i - nkv * per : i;
-        const int t = item & 3;
-        item >>= 2;
-        const int g = item % G;
-        item /= G;
-        const int off = item % page_size, h = item / page_size, r = off % KV4_TILE;
-        const unsigned char* tile = (value ? vcache : kcache) + kv4_tile(page, h, off, nkv, page_size) * kv4_tile_bytes(hd);
-        float x[8];
-        if (value) {
-            float lo[4], hi[4];
-            kv4_value4(tile, hd, r, g, 2 * t, lo);
-            kv4_value4(tile, hd, r, g, 2 * t + 1, hi);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) { x[j] = lo[j]; x[4 + j] = hi[j]; }
-        } else {
-            kv4_key8(tile, hd, r, g, t, x);
-        }
-        if ((begin + off < first || begin + off >= end) && !(x[0] == x[0])) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = 0.f;
-        }
-        Kv4Load<T, 8>::store((value ? v : k) + (((size_t)page * nkv + h) * page_size + off) * hd + KV4_GROUP * g + 8 * t, x);
+    const int G = hd / KV4_GROUP, per_row = hd / 8;                 // items of a token
+    const long long head = page * nkv + h;
+    const bool inside = begin >= first && begin + page_size <= end;
+    for (int i = threadIdx.x; i < 2 * page_size * per_row; i += KV4_THREADS) {
+        const bool value = i >= page_size * per_row;
+        const int item = value ? i - page_size * per_row : i, off = by_row.of(item), c = item - off * per_row, t = c & 3, g = c >> 2, r = off % KV4_TILE;
+        const unsigned char* tile = (value ? vcache : kcache) + (head * (page_size / KV4_TILE) + off / KV4_TILE) * kv4_tile_bytes(hd);
+        unsigned short scale = reinterpret_cast<const unsigned short*>(tile + 8 * hd)[r * G + g];
+        if (!inside && (begin + off < first || begin + off >= end) && (scale & 0x7fffu) > 0x7f80u) scale = 0;
+        uint32_t x[4];
+        kv4_eight(kv4_word(tile, hd, r, g, t, value), scale, x);
+        kv4_put((value ? v : k) + (head * page_size + off) * hd + 8 * c, x);
     }
 }
 
@@ -436,16 +472,17 @@ GB_EXPORT int gb_kv4_expand(const void* kcache, const void* vcache, void* k, voi
     KV4_REQUIRE_SIZES("gb_kv4_expand")
     GB_REQUIRE(dtype == GB_F32 || dtype == GB_BF16, "gb_kv4_expand: unsupported dtype %d", dtype);
     GB_REQUIRE(((uintptr_t)kcache | (uintptr_t)vcache | (uintptr_t)k | (uintptr_t)v) % 16 == 0, "gb_kv4_expand: tensors must be 16-byte aligned");
-    GB_REQUIRE(num_seqs >= 0 && num_seqs <= 65535 && max_pages > 0, "gb_kv4_expand: bad batch shape");
+    GB_REQUIRE(num_seqs >= 0 && num_seqs <= 65535 && nkv <= 65535 && max_pages > 0, "gb_kv4_expand: bad batch shape");
     const int pages = reach_pages < max_pages ? reach_pages : max_pages;
     if (num_seqs == 0 || pages <= 0) return 0;
-    const dim3 grid(pages, num_seqs), block(KV4_THREADS);
+    const dim3 grid(pages, nkv, num_seqs), block(KV4_THREADS);
+    const Kv4Div by_row(hd / 8);
     const unsigned char *kc = (const unsigned char*)kcache, *vc = (const unsigned char*)vcache;
     if (dtype == GB_F32)
         gb_launch(GB_PDL_ELEMENTWISE, kv4_expand_kernel<float>, grid, block, 0, stream, kc, vc, (float*)k, (float*)v, block_tables, max_pages,
-                  seq_first_row, seq_start_pos, nkv, hd, page_size, num_pages, window, status);
+                  seq_first_row, seq_start_pos, nkv, hd, page_size, num_pages, window, by_row, status);
     else
         gb_launch(GB_PDL_ELEMENTWISE, kv4_expand_kernel<__nv_bfloat16>, grid, block, 0, stream, kc, vc, (__nv_bfloat16*)k, (__nv_bfloat16*)v,
-                  block_tables, max_pages, seq_first_row, seq_start_pos, nkv, hd, page_size, num_pages, window, status);
+                  block_tables, max_pages, seq_first_row, seq_start_pos, nkv, hd, page_size, num_pages, window, by_row, status);
     return gb_check_launch("gb_kv4_expand");
 }
