@@ -5,12 +5,11 @@
 // All three only move memory. The sums that matter are bytes: a row of a wide layout (32/8 heads of 128, bfloat16) brings 12 KB in, 8 KB
 // of queries out and 1.1 KB of cache out.
 //
-// The rounding, for numbers y of a group: one whole-number key per number, its magnitude's bits with "not negative" in the lowest, has
-// the group's m as its maximum, infinities and NaN above every number; m's bits less 3 in the exponent, rounded to four bits after the leading
-// one, are |d|. A value's quotient y / d is the product with the reciprocal and one correction by the remainder (exact in a fused multiply-add),
-// so that a number half way between two codes is told as such: with bfloat16 values that is one in dozens, and ties go to the even
-// code. A rotated key is carried as two float32 (see kv4_turn2), so that its code and scale are those of the exact product of the
-// rotation; rounded to one float32 first, one number in some 10^6 gets the neighbouring code.
+// The rounding: m's bits less 3 in the exponent, rounded to four bits after the leading one, are |d|. A quotient y / d is the product with the
+// reciprocal and one correction by the remainder (exact in a fused multiply-add), so that a number half way between two codes is told as such:
+// with bfloat16 values that is one in dozens, and ties go to the even code. A rotated key is a float32 product off by some 2^-23; where that
+// could change a code or the scale (one group in some 10^4) the group is held once more from two float32 a number, so that what
+// is stored is always what the exact rotation gives.
 #include "kv4.cuh"
 
 #include <type_traits>
@@ -84,26 +83,61 @@ __device__ __forceinline__ void kv4_store(T* p, const float (&f)[N]) {
     }
 }
 
-// The key whose maximum over a group names its m (see above), over N numbers of this thread.
+__device__ __forceinline__ float kv4_max_nan(float a, float b) {           // NaN where one of them is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float kv4_min_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// The largest and the smallest of N numbers of this thread.
 template <int N>
-__device__ __forceinline__ unsigned kv4_most(const float (&y)[N]) {
-    unsigned most = 0;
+__device__ __forceinline__ void kv4_ends(const float (&y)[N], float& high, float& low) {
+    high = low = y[0];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const unsigned b = __float_as_uint(y[i]);
-        most = max(most, (b << 1) | (b >> 31 ^ 1u));
+    for (int i = 1; i < N; ++i) {
+        high = kv4_max_nan(high, y[i]);
+        low = kv4_min_nan(low, y[i]);
     }
-    return most;
 }
 
-// The scale of a group from that key, as float32: zero, NaN, or a number of five significant bits.
-__device__ __forceinline__ float kv4_make_scale(unsigned most) {
-    const unsigned size = most >> 1;
-    if (size >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
-    if (size < 0x05000000u) return 0.f;                                    // 2^-117
-    unsigned d = size - (3u << 23);
-    d = (d + 0x3ffffu + ((d >> 19) & 1u)) & 0xfff80000u;                   // four bits after the leading one, ties to even
-    return __uint_as_float(d | (most & 1u) << 31);                         // (m positive: d negative)
+// Bits of a magnitude's scale: an eighth of it, four bits after the leading one, ties to even.
+__device__ __forceinline__ unsigned kv4_five(unsigned size) {
+    const unsigned d = size - (3u << 23);
+    return (d + 0x3ffffu + ((d >> 19) & 1u)) & 0xfff80000u;
+}
+
+// The scale of a group from its ends, as float32: zero, NaN, or a number of five significant bits.
+__device__ __forceinline__ float kv4_make_scale(float high, float low) {
+    const float m = high >= -low ? high : low, size = fabsf(m);
+    if (!(fmaxf(high, -low) <= FLT_MAX && high == high && low == low)) return __uint_as_float(0x7fc00000u);
+    if (size < 6.018531076210112e-36f) return 0.f;                         // 2^-117
+    return __uint_as_float(kv4_five(__float_as_uint(size)) | (m > 0.f ? 0x80000000u : 0u));
+}
+
+// Codes s + 8 of N numbers, N nibbles from the low end on: the quotient y / d (to within a rounding; exactly half way where it is), limited, plus
+// 1.5 2^23 + 8, which rounds it and leaves the code in the lowest bits; the words of bits are added up as digits of base 16 with what the
+// others of their bits come to taken off at the end. near: the farthest that a quotient lies from its code.
+template <int N>
+__device__ __forceinline__ unsigned kv4_codes(const float (&y)[N], float d, float& near) {
+    near = 0.f;
+    if (!(fabsf(d) > 0.f)) return 0x88888888u;                             // nothing, or NaN: s = 0
+    constexpr float WHOLE = 12582920.f;
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+    unsigned w = 0x100000000ull - 0x3f400000u;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        float q = y[i] * r;
+        q = fminf(fmaxf(fmaf(fmaf(-q, d, y[i]), r, q), -8.f), 7.f);
+        const float t = q + WHOLE;
+        near = fmaxf(near, fabsf(q - (t - WHOLE)));
+        w += __float_as_uint(t) << (4 * i);
+    }
+    return w;
 }
 
 // A turned key as the sum of two float32, the first the nearest to the sum (what a float32 rounding would drop decides which code a number
@@ -137,11 +171,11 @@ __device__ __forceinline__ float kv4_make_scale2(unsigned long long most) {
     return __uint_as_float(d | (unsigned)(most & 1u) << 31);
 }
 
-// Codes s + 8 of N numbers hi + lo, N nibbles from the low end on. s is the whole number nearest to hi / d by the hardware's reciprocal (adding
-// 1.5 2^23 rounds to one); what it leaves, hi - s d (exact) and lo, is then compared with half a step.
+// Codes of such numbers, hi + lo. s is the whole number nearest to hi / d by the hardware's reciprocal; what it leaves, hi - s d (exact) and
+// lo, is then compared with half a step.
 template <int N>
-__device__ __forceinline__ unsigned kv4_codes(const float (&hi)[N], const float (&lo)[N], float d) {
-    if (!(fabsf(d) > 0.f)) return 0x88888888u;                             // nothing, or NaN: s = 0
+__device__ __noinline__ unsigned kv4_codes2(const float (&hi)[N], const float (&lo)[N], float d) {
+    if (!(fabsf(d) > 0.f)) return 0x88888888u;
     constexpr float WHOLE = 12582912.f;
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
@@ -161,6 +195,25 @@ __device__ __forceinline__ unsigned kv4_codes(const float (&hi)[N], const float 
 
 // channel c of a head, turned: `x` the channel's own number, `o` its partner's, c and s of the pair's angle
 __device__ __forceinline__ float kv4_turn(float x, float o, float2 cs, bool second) { return second ? fmaf(x, cs.x, o * cs.y) : fmaf(x, cs.x, -o * cs.y); }
+
+// Scale and codes of this thread's eight channels of a key (from c0 on, those below rot turned), exactly; the four lanes of a group, `mask`, together.
+template <typename T>
+__device__ __noinline__ void kv4_key_again(const T* p, const float2* turn, int c0, int rot, int half, unsigned mask, float& d, unsigned& codes) {
+    float y[8], lo[8];
+    unsigned long long m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int c = c0 + j;
+        y[j] = gb_to_float(p[c]);
+        lo[j] = 0.f;
+        if (c < rot) kv4_turn2(y[j], lo[j], gb_to_float(p[c >= half ? c - half : c + half]), turn[c >= half ? c - half : c], c >= half);
+        m = max(m, kv4_most2(y[j], lo[j]));
+    }
+    m = max(m, __shfl_xor_sync(mask, m, 1));
+    m = max(m, __shfl_xor_sync(mask, m, 2));
+    d = kv4_make_scale2(m);
+    codes = kv4_codes2(y, lo, d);
+}
 
 struct Kv4WriteArgs {
     const void* qkv;
@@ -207,19 +260,29 @@ __global__ void __launch_bounds__(KV4_THREADS) kv4_write_kernel(const Kv4WriteAr
             float y0[4], y1[4] = {0.f, 0.f, 0.f, 0.f};
             kv4_load<T, 4, WIDE>(p, y0);
             if (two) kv4_load<T, 4, WIDE>(p + 32, y1);
-            unsigned m0 = kv4_most(y0), m1 = kv4_most(y1);
+            float high0, low0, high1, low1, near;
+            kv4_ends(y0, high0, low0);
+            kv4_ends(y1, high1, low1);
             const unsigned mask = 0xffu << (lane & 24);
 #pragma unroll
             for (int o = 1; o < 8; o <<= 1) {
-                m0 = max(m0, __shfl_xor_sync(mask, m0, o));
-                m1 = max(m1, __shfl_xor_sync(mask, m1, o));
+                high0 = kv4_max_nan(high0, __shfl_xor_sync(mask, high0, o));
+                low0 = kv4_min_nan(low0, __shfl_xor_sync(mask, low0, o));
+                high1 = kv4_max_nan(high1, __shfl_xor_sync(mask, high1, o));
+                low1 = kv4_min_nan(low1, __shfl_xor_sync(mask, low1, o));
             }
-            const float d0 = kv4_make_scale(m0), d1 = kv4_make_scale(m1);
+            const float d0 = kv4_make_scale(high0, low0), d1 = kv4_make_scale(high1, low1);
             unsigned char* tile = a.vcache + kv4_tile(page, h, off, a.nkv, a.page_size) * kv4_tile_bytes(hd);
             unsigned char* codes = tile + r * (hd / 2) + (u * G + 2 * w) * 2;
             unsigned short* scales = reinterpret_cast<unsigned short*>(tile + 8 * hd) + r * G + 2 * w;
+            unsigned c0 = kv4_codes(y0, d0, near);
             const float none[4] = {0.f, 0.f, 0.f, 0.f};
-            const unsigned c0 = kv4_codes(y0, none, d0) & 0xffffu, c1 = kv4_codes(y1, none, d1) & 0xffffu;
+            // (the quotient of a float32 may have been rounded to half way; that of a bfloat16 by five bits lies half way if it says so)
+            if (sizeof(T) == 4 && near == 0.5f) c0 = kv4_codes2(y0, none, d0);
+            unsigned c1 = kv4_codes(y1, d1, near);
+            if (sizeof(T) == 4 && near == 0.5f) c1 = kv4_codes2(y1, none, d1);
+            c0 &= 0xffffu;
+            c1 &= 0xffffu;
             if (two && G % 2 == 0) {
                 *reinterpret_cast<unsigned*>(codes) = c0 | c1 << 16;
                 if (u == 0) *reinterpret_cast<unsigned*>(scales) = __float_as_uint(d0) >> 16 | (__float_as_uint(d1) & 0xffff0000u);
@@ -235,11 +298,11 @@ __global__ void __launch_bounds__(KV4_THREADS) kv4_write_kernel(const Kv4WriteAr
         }
         const int k = item - a.units_v, t = k & 3, h = a.by_g.of(k >> 2), g = (k >> 2) - h * G, c0 = KV4_GROUP * g + 8 * t;
         const T* p = base + (size_t)(a.nh + h) * hd;
-        float y[8], lo[8];                   // the keys, turned: y + lo
+        const unsigned mask = 0xfu << (lane & 28);
+        const bool turns = rotate && c0 < a.rot;
+        float y[8], off_by = turns ? 1e-37f : 0.f;      // the keys, turned, and what a bound on their roundings goes by
         kv4_load<T, 8, WIDE>(p + c0, y);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) lo[j] = 0.f;
-        if (rotate && c0 < a.rot) {
+        if (turns) {
             if (WIDE) {
                 float o[8];
                 const bool second = c0 >= half;
@@ -249,8 +312,11 @@ __global__ void __launch_bounds__(KV4_THREADS) kv4_write_kernel(const Kv4WriteAr
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const float4 f = cs[j];
-                    kv4_turn2(y[2 * j], lo[2 * j], o[2 * j], make_float2(f.x, f.y), second);
-                    kv4_turn2(y[2 * j + 1], lo[2 * j + 1], o[2 * j + 1], make_float2(f.z, f.w), second);
+                    const float s0 = second ? f.y : -f.y, s1 = second ? f.w : -f.w;
+                    const float q0 = o[2 * j] * s0, q1 = o[2 * j + 1] * s1;
+                    off_by = fmaxf(off_by, fmaxf(fabsf(q0), fabsf(q1)));
+                    y[2 * j] = fmaf(y[2 * j], f.x, q0);
+                    y[2 * j + 1] = fmaf(y[2 * j + 1], f.z, q1);
                 }
             } else {
 #pragma unroll
@@ -258,19 +324,31 @@ __global__ void __launch_bounds__(KV4_THREADS) kv4_write_kernel(const Kv4WriteAr
                     const int c = c0 + j;
                     if (c >= a.rot) continue;
                     const bool second = c >= half;
-                    kv4_turn2(y[j], lo[j], gb_to_float(p[second ? c - half : c + half]), turn[second ? c - half : c], second);
+                    const float2 cs = turn[second ? c - half : c];
+                    const float q = gb_to_float(p[second ? c - half : c + half]) * (second ? cs.y : -cs.y);
+                    off_by = fmaxf(off_by, fabsf(q));
+                    y[j] = fmaf(y[j], cs.x, q);
                 }
             }
         }
-        unsigned long long m = 0;
+        float high, low, near;
+        kv4_ends(y, high, low);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) m = max(m, kv4_most2(y[j], lo[j]));
-        const unsigned mask = 0xfu << (lane & 28);
-        m = max(m, __shfl_xor_sync(mask, m, 1));
-        m = max(m, __shfl_xor_sync(mask, m, 2));
-        const float d = kv4_make_scale2(m);
+        for (int o = 1; o < 4; o <<= 1) {
+            high = kv4_max_nan(high, __shfl_xor_sync(mask, high, o));
+            low = kv4_min_nan(low, __shfl_xor_sync(mask, low, o));
+            off_by = fmaxf(off_by, __shfl_xor_sync(mask, off_by, o));
+        }
+        float d = kv4_make_scale(high, low);
+        unsigned codes = kv4_codes(y, d, near);
+        // Where what the roundings come to could change the sign or the size of the scale, or a code, the group is held once more, exactly.
+        const float size = fmaxf(high, -low), bound = 0x1p-22f * fmaxf(off_by, size);
+        const bool unsure = off_by > 0.f ? fabsf(high + low) <= 2.f * bound || kv4_five(__float_as_uint(size - bound)) != kv4_five(__float_as_uint(size + bound)) ||
+                                               (0.5f - near) * fabsf(d) <= 2.f * bound
+                                         : sizeof(T) == 4 && near == 0.5f;
+        if (__ballot_sync(mask, unsure)) kv4_key_again<T>(p, turn, c0, turns ? a.rot : 0, half, mask, d, codes);
         unsigned char* tile = a.kcache + kv4_tile(page, h, off, a.nkv, a.page_size) * kv4_tile_bytes(hd);
-        *reinterpret_cast<unsigned*>(tile + r * (hd / 2) + (t * G + g) * 4) = kv4_codes(y, lo, d);
+        *reinterpret_cast<unsigned*>(tile + r * (hd / 2) + (t * G + g) * 4) = codes;
         if (t == 0) reinterpret_cast<unsigned short*>(tile + 8 * hd)[r * G + g] = (unsigned short)(__float_as_uint(d) >> 16);
         return;
     }
@@ -303,9 +381,8 @@ __global__ void __launch_bounds__(KV4_THREADS) kv4_write_kernel(const Kv4WriteAr
             kv4_store<T, 8, WIDE>(to + 8 * i + half, z1);
         } else {
             const int c = a.rot + 8 * (i - half / 8);
-            float x[8];
-            kv4_load<T, 8, WIDE>(p + c, x);
-            kv4_store<T, 8, WIDE>(to + c, x);
+#pragma unroll
+            for (int j = 0; j < 8; j += 16 / sizeof(T)) *reinterpret_cast<uint4*>(to + c + j) = *reinterpret_cast<const uint4*>(p + c + j);
         }
     } else if (i < half) {                   // one pair, or one channel, a thread
         const float x0 = gb_to_float(p[i]), x1 = gb_to_float(p[i + half]);
