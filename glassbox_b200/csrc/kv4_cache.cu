@@ -240,75 +240,83 @@ __global__ void __launch_bounds__(KV4_THREADS) kv4_write_kernel(const Kv4WriteAr
     gb_pdl_launch_dependents();
     gb_pdl_wait();
     const int row = blockIdx.x, item = blockIdx.y * KV4_THREADS + threadIdx.x;
-    const int pos = a.positions[row];
-    if (pos < 0) return;                     // a padding row: nothing to turn, nothing to store
-    const int slot = a.write_kv ? a.slots[row] : 0;
-    const bool rotate = a.table != nullptr && pos < a.max_pos, store = a.write_kv && slot >= 0 && slot < a.num_slots;
-    if (item == 0 && ((a.table != nullptr && !rotate) || (a.write_kv && !store)))
-        atomicOr(a.status, (a.table != nullptr && !rotate ? GB_STATUS_BAD_POSITION : 0) | (a.write_kv && !store ? GB_STATUS_BAD_SLOT : 0));
+    if (item >= a.units_v + a.units_k + a.units_q) return;
+    // (asked for first and looked at behind the row's own loads, which do not depend on them)
+    const int pos = a.positions[row], slot = a.write_kv ? a.slots[row] : 0;
     const int hd = a.hd, G = hd / KV4_GROUP, half = a.rot / 2, lane = threadIdx.x & 31;
     const T* base = (const T*)a.qkv + (size_t)row * a.qkv_stride;
-    const float2* turn = rotate ? a.table + (size_t)pos * half : nullptr;
-
-    if (item < a.units_v + a.units_k) {
-        if (!store) return;                  // (the same for all items of a row: no lane of a group is missing)
-        const int page = slot / a.page_size, off = slot - page * a.page_size, r = off % KV4_TILE;
-        if (item < a.units_v) {
-            const int u = item & 7, h = a.by_w.of(item >> 3), w = (item >> 3) - h * (int)a.by_w.d;
-            const bool two = 2 * w + 1 < G;
-            const T* p = base + (size_t)(a.nh + a.nkv + h) * hd + 64 * w + 4 * u;
-            float y0[4], y1[4] = {0.f, 0.f, 0.f, 0.f};
-            kv4_load<T, 4, WIDE>(p, y0);
-            if (two) kv4_load<T, 4, WIDE>(p + 32, y1);
-            float high0, low0, high1, low1, near;
-            kv4_ends(y0, high0, low0);
-            kv4_ends(y1, high1, low1);
-            const unsigned mask = 0xffu << (lane & 24);
-#pragma unroll
-            for (int o = 1; o < 8; o <<= 1) {
-                high0 = kv4_max_nan(high0, __shfl_xor_sync(mask, high0, o));
-                low0 = kv4_min_nan(low0, __shfl_xor_sync(mask, low0, o));
-                high1 = kv4_max_nan(high1, __shfl_xor_sync(mask, high1, o));
-                low1 = kv4_min_nan(low1, __shfl_xor_sync(mask, low1, o));
-            }
-            const float d0 = kv4_make_scale(high0, low0), d1 = kv4_make_scale(high1, low1);
-            unsigned char* tile = a.vcache + kv4_tile(page, h, off, a.nkv, a.page_size) * kv4_tile_bytes(hd);
-            unsigned char* codes = tile + r * (hd / 2) + (u * G + 2 * w) * 2;
-            unsigned short* scales = reinterpret_cast<unsigned short*>(tile + 8 * hd) + r * G + 2 * w;
-            unsigned c0 = kv4_codes(y0, d0, near);
-            const float none[4] = {0.f, 0.f, 0.f, 0.f};
-            // (the quotient of a float32 may have been rounded to half way; that of a bfloat16 by five bits lies half way if it says so)
-            if (sizeof(T) == 4 && near == 0.5f) c0 = kv4_codes2(y0, none, d0);
-            unsigned c1 = kv4_codes(y1, d1, near);
-            if (sizeof(T) == 4 && near == 0.5f) c1 = kv4_codes2(y1, none, d1);
-            c0 &= 0xffffu;
-            c1 &= 0xffffu;
-            if (two && G % 2 == 0) {
-                *reinterpret_cast<unsigned*>(codes) = c0 | c1 << 16;
-                if (u == 0) *reinterpret_cast<unsigned*>(scales) = __float_as_uint(d0) >> 16 | (__float_as_uint(d1) & 0xffff0000u);
-            } else {
-                *reinterpret_cast<unsigned short*>(codes) = (unsigned short)c0;
-                if (u == 0) scales[0] = (unsigned short)(__float_as_uint(d0) >> 16);
-                if (two) {
-                    *reinterpret_cast<unsigned short*>(codes + 2) = (unsigned short)c1;
-                    if (u == 0) scales[1] = (unsigned short)(__float_as_uint(d1) >> 16);
-                }
-            }
-            return;
+    auto turns = [&]() { return a.table != nullptr && pos < a.max_pos; };
+    auto stores = [&]() { return slot >= 0 && slot < a.num_slots; };
+    auto report = [&]() {
+        if (item == 0 && pos >= 0) {
+            const int bad = (a.table != nullptr && !turns() ? GB_STATUS_BAD_POSITION : 0) | (a.write_kv && !stores() ? GB_STATUS_BAD_SLOT : 0);
+            if (bad) atomicOr(a.status, bad);
         }
+    };
+
+    if (item < a.units_v) {
+        const int u = item & 7, h = a.by_w.of(item >> 3), w = (item >> 3) - h * (int)a.by_w.d;
+        const bool two = 2 * w + 1 < G;
+        const T* p = base + (size_t)(a.nh + a.nkv + h) * hd + 64 * w + 4 * u;
+        float y0[4], y1[4] = {0.f, 0.f, 0.f, 0.f};
+        kv4_load<T, 4, WIDE>(p, y0);
+        if (two) kv4_load<T, 4, WIDE>(p + 32, y1);
+        report();
+        if (pos < 0 || !stores()) return;    // a padding row, or a bad slot (the same for all items of a row: no lane of a group is missing)
+        const int page = slot / a.page_size, off = slot - page * a.page_size, r = off % KV4_TILE;
+        float high0, low0, high1, low1, near;
+        kv4_ends(y0, high0, low0);
+        kv4_ends(y1, high1, low1);
+        const unsigned mask = 0xffu << (lane & 24);
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) {
+            high0 = kv4_max_nan(high0, __shfl_xor_sync(mask, high0, o));
+            low0 = kv4_min_nan(low0, __shfl_xor_sync(mask, low0, o));
+            high1 = kv4_max_nan(high1, __shfl_xor_sync(mask, high1, o));
+            low1 = kv4_min_nan(low1, __shfl_xor_sync(mask, low1, o));
+        }
+        const float d0 = kv4_make_scale(high0, low0), d1 = kv4_make_scale(high1, low1);
+        unsigned char* tile = a.vcache + kv4_tile(page, h, off, a.nkv, a.page_size) * kv4_tile_bytes(hd);
+        unsigned char* codes = tile + r * (hd / 2) + (u * G + 2 * w) * 2;
+        unsigned short* scales = reinterpret_cast<unsigned short*>(tile + 8 * hd) + r * G + 2 * w;
+        unsigned c0 = kv4_codes(y0, d0, near);
+        const float none[4] = {0.f, 0.f, 0.f, 0.f};
+        // (the quotient of a float32 may have been rounded to half way; that of a bfloat16 by five bits lies half way if it says so)
+        if (sizeof(T) == 4 && near == 0.5f) c0 = kv4_codes2(y0, none, d0);
+        unsigned c1 = kv4_codes(y1, d1, near);
+        if (sizeof(T) == 4 && near == 0.5f) c1 = kv4_codes2(y1, none, d1);
+        c0 &= 0xffffu;
+        c1 &= 0xffffu;
+        if (two && G % 2 == 0) {
+            *reinterpret_cast<unsigned*>(codes) = c0 | c1 << 16;
+            if (u == 0) *reinterpret_cast<unsigned*>(scales) = __float_as_uint(d0) >> 16 | (__float_as_uint(d1) & 0xffff0000u);
+        } else {
+            *reinterpret_cast<unsigned short*>(codes) = (unsigned short)c0;
+            if (u == 0) scales[0] = (unsigned short)(__float_as_uint(d0) >> 16);
+            if (two) {
+                *reinterpret_cast<unsigned short*>(codes + 2) = (unsigned short)c1;
+                if (u == 0) scales[1] = (unsigned short)(__float_as_uint(d1) >> 16);
+            }
+        }
+        return;
+    }
+    if (item < a.units_v + a.units_k) {
         const int k = item - a.units_v, t = k & 3, h = a.by_g.of(k >> 2), g = (k >> 2) - h * G, c0 = KV4_GROUP * g + 8 * t;
         const T* p = base + (size_t)(a.nh + h) * hd;
-        const unsigned mask = 0xfu << (lane & 28);
-        const bool turns = rotate && c0 < a.rot;
-        float y[8], off_by = turns ? 1e-37f : 0.f;      // the keys, turned, and what a bound on their roundings goes by
+        const bool second = c0 >= half;
+        const int first = second ? c0 - half : c0;      // (WIDE: of the pairs that these channels belong to)
+        float y[8], o[8];
         kv4_load<T, 8, WIDE>(p + c0, y);
-        if (turns) {
+        if (WIDE && a.table != nullptr && c0 < a.rot) kv4_load<T, 8, WIDE>(p + (second ? first : first + half), o);
+        if (pos < 0 || !stores()) return;
+        const int page = slot / a.page_size, off = slot - page * a.page_size, r = off % KV4_TILE;
+        const unsigned mask = 0xfu << (lane & 28);
+        const bool turn_them = turns() && c0 < a.rot;
+        const float2* turn = a.table + (size_t)pos * half;
+        float off_by = turn_them ? 1e-37f : 0.f;         // what a bound on the turned keys' roundings goes by
+        if (turn_them) {
             if (WIDE) {
-                float o[8];
-                const bool second = c0 >= half;
-                const int i = second ? c0 - half : c0;
-                kv4_load<T, 8, WIDE>(p + (second ? i : i + half), o);
-                const float4* cs = reinterpret_cast<const float4*>(turn + i);
+                const float4* cs = reinterpret_cast<const float4*>(turn + first);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const float4 f = cs[j];
@@ -323,9 +331,9 @@ __global__ void __launch_bounds__(KV4_THREADS) kv4_write_kernel(const Kv4WriteAr
                 for (int j = 0; j < 8; ++j) {
                     const int c = c0 + j;
                     if (c >= a.rot) continue;
-                    const bool second = c >= half;
-                    const float2 cs = turn[second ? c - half : c];
-                    const float q = gb_to_float(p[second ? c - half : c + half]) * (second ? cs.y : -cs.y);
+                    const bool late = c >= half;
+                    const float2 cs = turn[late ? c - half : c];
+                    const float q = gb_to_float(p[late ? c - half : c + half]) * (late ? cs.y : -cs.y);
                     off_by = fmaxf(off_by, fabsf(q));
                     y[j] = fmaf(y[j], cs.x, q);
                 }
@@ -334,10 +342,10 @@ __global__ void __launch_bounds__(KV4_THREADS) kv4_write_kernel(const Kv4WriteAr
         float high, low, near;
         kv4_ends(y, high, low);
 #pragma unroll
-        for (int o = 1; o < 4; o <<= 1) {
-            high = kv4_max_nan(high, __shfl_xor_sync(mask, high, o));
-            low = kv4_min_nan(low, __shfl_xor_sync(mask, low, o));
-            off_by = fmaxf(off_by, __shfl_xor_sync(mask, off_by, o));
+        for (int x = 1; x < 4; x <<= 1) {
+            high = kv4_max_nan(high, __shfl_xor_sync(mask, high, x));
+            low = kv4_min_nan(low, __shfl_xor_sync(mask, low, x));
+            off_by = fmaxf(off_by, __shfl_xor_sync(mask, off_by, x));
         }
         float d = kv4_make_scale(high, low);
         unsigned codes = kv4_codes(y, d, near);
@@ -346,7 +354,7 @@ __global__ void __launch_bounds__(KV4_THREADS) kv4_write_kernel(const Kv4WriteAr
         const bool unsure = off_by > 0.f ? fabsf(high + low) <= 2.f * bound || kv4_five(__float_as_uint(size - bound)) != kv4_five(__float_as_uint(size + bound)) ||
                                                (0.5f - near) * fabsf(d) <= 2.f * bound
                                          : sizeof(T) == 4 && near == 0.5f;
-        if (__ballot_sync(mask, unsure)) kv4_key_again<T>(p, turn, c0, turns ? a.rot : 0, half, mask, d, codes);
+        if (__ballot_sync(mask, unsure)) kv4_key_again<T>(p, turn, c0, turn_them ? a.rot : 0, half, mask, d, codes);
         unsigned char* tile = a.kcache + kv4_tile(page, h, off, a.nkv, a.page_size) * kv4_tile_bytes(hd);
         *reinterpret_cast<unsigned*>(tile + r * (hd / 2) + (t * G + g) * 4) = codes;
         if (t == 0) reinterpret_cast<unsigned short*>(tile + 8 * hd)[r * G + g] = (unsigned short)(__float_as_uint(d) >> 16);
@@ -354,41 +362,49 @@ __global__ void __launch_bounds__(KV4_THREADS) kv4_write_kernel(const Kv4WriteAr
     }
 
     // queries
-    const int k = item - a.units_v - a.units_k;
-    if (k >= a.units_q) return;
-    const int h = a.by_pairs.of(k), i = k - h * (int)a.by_pairs.d;
+    const int k = item - a.units_v - a.units_k, h = a.by_pairs.of(k), i = k - h * (int)a.by_pairs.d;
     const T* p = base + (size_t)h * hd;
     T* to = (T*)a.q + (size_t)row * a.q_stride + (size_t)h * hd;
     if (WIDE) {
         if (8 * i < half) {
-            float x0[8], x1[8], z0[8], z1[8];
+            float x0[8], x1[8];
             kv4_load<T, 8, WIDE>(p + 8 * i, x0);
             kv4_load<T, 8, WIDE>(p + 8 * i + half, x1);
+            report();
+            if (pos < 0) return;
+            if (turns()) {
+                const float4* cs = reinterpret_cast<const float4*>(a.table + (size_t)pos * half + 8 * i);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) { z0[j] = x0[j]; z1[j] = x1[j]; }
-            if (rotate) {
-                const float4* cs = reinterpret_cast<const float4*>(turn + 8 * i);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float4 f = cs[j];
-                    z0[2 * j] = kv4_turn(x0[2 * j], x1[2 * j], make_float2(f.x, f.y), false);
-                    z1[2 * j] = kv4_turn(x1[2 * j], x0[2 * j], make_float2(f.x, f.y), true);
-                    z0[2 * j + 1] = kv4_turn(x0[2 * j + 1], x1[2 * j + 1], make_float2(f.z, f.w), false);
-                    z1[2 * j + 1] = kv4_turn(x1[2 * j + 1], x0[2 * j + 1], make_float2(f.z, f.w), true);
+                for (int j = 0; j < 8; ++j) {
+                    const float4 f = cs[j / 2];
+                    const float2 c = j % 2 ? make_float2(f.z, f.w) : make_float2(f.x, f.y);
+                    const float z0 = kv4_turn(x0[j], x1[j], c, false), z1 = kv4_turn(x1[j], x0[j], c, true);
+                    x0[j] = z0;
+                    x1[j] = z1;
                 }
             }
-            kv4_store<T, 8, WIDE>(to + 8 * i, z0);
-            kv4_store<T, 8, WIDE>(to + 8 * i + half, z1);
+            kv4_store<T, 8, WIDE>(to + 8 * i, x0);
+            kv4_store<T, 8, WIDE>(to + 8 * i + half, x1);
         } else {
             const int c = a.rot + 8 * (i - half / 8);
+            uint4 raw[sizeof(T) / 2];
 #pragma unroll
-            for (int j = 0; j < 8; j += 16 / sizeof(T)) *reinterpret_cast<uint4*>(to + c + j) = *reinterpret_cast<const uint4*>(p + c + j);
+            for (int j = 0; j < (int)sizeof(T) / 2; ++j) raw[j] = reinterpret_cast<const uint4*>(p + c)[j];
+            report();
+            if (pos < 0) return;
+#pragma unroll
+            for (int j = 0; j < (int)sizeof(T) / 2; ++j) reinterpret_cast<uint4*>(to + c)[j] = raw[j];
         }
-    } else if (i < half) {                   // one pair, or one channel, a thread
+        return;
+    }
+    report();
+    if (pos < 0) return;
+    if (i < half) {                          // one pair, or one channel, a thread
         const float x0 = gb_to_float(p[i]), x1 = gb_to_float(p[i + half]);
-        const float2 cs = rotate ? turn[i] : make_float2(1.f, 0.f);
-        to[i] = gb_from_float<T>(rotate ? kv4_turn(x0, x1, cs, false) : x0);
-        to[i + half] = gb_from_float<T>(rotate ? kv4_turn(x1, x0, cs, true) : x1);
+        const bool turn = turns();
+        const float2 cs = turn ? a.table[(size_t)pos * half + i] : make_float2(1.f, 0.f);
+        to[i] = gb_from_float<T>(turn ? kv4_turn(x0, x1, cs, false) : x0);
+        to[i + half] = gb_from_float<T>(turn ? kv4_turn(x1, x0, cs, true) : x1);
     } else {
         const int c = a.rot + i - half;
         to[c] = p[c];
