@@ -1,0 +1,401 @@
+// Causal grouped-query flash attention for prompt portions at head size 128 on the 5th-generation tensor cores (sm_100a), over pages of
+// bfloat16. The scheme is attention_prefill_tc.cu's (head size 64), laid out for twice the channels:
+//
+// One block = 128 consecutive query rows of one request for one query head, over tiles of 128 keys.
+//   warp 0, 10  producers of keys (and the query tile, once) and of values: a page is two boxes of 64 channels, each issued by a lane of its own,
+//               into rings of three stages (two 128-byte-swizzled column blocks a tile, 32 KB).
+//   warp 1      issues S_j = Q K_j^T (M 128, N 128, K 128) into TMEM columns 128 g, g = j & 1, and O_g += P_j V_j (M 128, N 128, K 128).
+//   warps 2-9   softmax, two groups of four warps; group g takes the key tiles of parity g with an accumulator, running maximum and row sum of its
+//               own. A thread owns a row (a TMEM lane). P_j, rounded to bfloat16, goes back over the first half of S_j's own columns: two score
+//               buffers and two accumulators of 128 columns fill the 512 that there are, so there is no room for P beside them. The
+//               tensor core works in the order of issue, so S_{j+2} may be issued into the buffer right behind the product that reads P_j.
+// What bounds it: per tile the two products are 1,024 cycles of the tensor core, the 16,384 exponentials as many of the unit that forms
+// them; the two groups keep both busy in turn.
+// The mask is applied only in tiles that cross a boundary; key tiles that no row sees are skipped. Page 0 is read in the place of pages that
+// are missing, so that P = 0 meets finite numbers (the pages are zero-initialised).
+// Every wait is bounded: a wait that runs out sets GB_STATUS_WAIT_TIMEOUT and the block winds down (waits for its own copies, frees its TMEM,
+// returns). TMA loads use no multicast.
+// Measured (2,048 rows behind 2,048 tokens, 32/8 heads): mma.sync 750 us, this kernel 140.
+#include "tcgen05.cuh"
+
+constexpr int AL_HD = 128, AL_BM = 128, AL_BN = 128, AL_STAGES = 3, AL_WARPS = 11;
+constexpr int AL_BLOCK = 128 * 128;                     // bytes of 128 rows of 64 channels
+constexpr int AL_TILE = 2 * AL_BLOCK;
+constexpr int AL_K_OFF = AL_TILE, AL_V_OFF = AL_K_OFF + AL_STAGES * AL_TILE, AL_SH_OFF = AL_V_OFF + AL_STAGES * AL_TILE;
+constexpr int AL_SMEM = AL_SH_OFF + 2560;
+constexpr int AL_O_COL = 2 * AL_BN, AL_TMEM_COLS = 512;
+constexpr float AL_NEG_BIG = -1.0e30f;
+static_assert(AL_SMEM <= 227 * 1024 && AL_O_COL + 2 * AL_HD <= AL_TMEM_COLS, "the block does not fit");
+
+struct __align__(8) AlShared {
+    uint64_t q_full;
+    uint64_t k_full[AL_STAGES], k_empty[AL_STAGES];      // TMA -> MMA, MMA -> TMA
+    uint64_t v_full[AL_STAGES], v_empty[AL_STAGES];
+    uint64_t s_full[2];              // MMA -> softmax: S_j is complete in buffer j & 1
+    uint64_t p_ready[2];             // softmax -> MMA: P_j is in its place (and O is rescaled)
+    uint64_t pv_done[2];             // MMA -> softmax: O += P_j V_j is complete
+    uint64_t x_ready;                // softmax <-> softmax: both groups have posted their final maximum and sum
+    float row_stat[2][2][AL_BM];     // [group][maximum, sum][row]
+    uint32_t tmem_base;
+    int abort_flag;
+    int issued[2], consumed[2], q_issued;
+};
+static_assert(sizeof(AlShared) <= 2560, "shared memory layout");
+
+// MN-major B operand (rows are keys, a head's channels contiguous) in 128-byte-swizzled rows: groups of eight keys 1024 bytes apart, column blocks
+// of 64 channels lbo bytes apart.
+__device__ __forceinline__ uint64_t al_desc_mn(uint32_t smem_addr, uint32_t lbo_bytes) {
+    uint64_t d = 0;
+    d |= (uint64_t)((smem_addr & 0x3FFFF) >> 4);
+    d |= (uint64_t)((lbo_bytes >> 4) & 0x3FFF) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+// Two non-negative floats to a bfloat16 pair, rounding half up, on the integer pipe: the conversion shares its pipe with ex2.
+__device__ __forceinline__ uint32_t al_pack(float lo, float hi) { return __byte_perm(__float_as_uint(lo) + 0x8000u, __float_as_uint(hi) + 0x8000u, 0x7632); }
+__device__ __forceinline__ float al_max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float al_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__global__ void __launch_bounds__(AL_WARPS * 32) attention_prefill_128_kernel(
+    const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+    __nv_bfloat16* __restrict__ out, long long out_stride, const int* __restrict__ block_tables, int max_pages, const int* __restrict__ seq_first_row,
+    const int* __restrict__ seq_start_pos, int nh, int nkv, int page_size, int page_shift, long long num_pages, float scale, int window,
+    int* __restrict__ status) {
+    extern __shared__ __align__(1024) unsigned char al_smem[];
+    unsigned char* Qs = al_smem;
+    unsigned char* Ks = al_smem + AL_K_OFF;
+    unsigned char* Vs = al_smem + AL_V_OFF;
+    AlShared& sh = *reinterpret_cast<AlShared*>(al_smem + AL_SH_OFF);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    gb_pdl_wait();
+    gb_pdl_launch_dependents();
+    const int head = blockIdx.x, seq = blockIdx.y, qt = (int)gridDim.z - 1 - (int)blockIdx.z;      // (the longest blocks start first)
+    const int row0 = seq_first_row[seq], nrows = seq_first_row[seq + 1] - row0, q_lo = qt * AL_BM;
+    if (q_lo >= nrows) return;                    // uniform for the block, before anything is allocated
+    if (smem_u32(al_smem) & 1023u) {              // swizzled tiles want 1024-byte alignment: refuse rather than compute nonsense
+        if (tid == 0) atomicOr(status, GB_STATUS_WAIT_TIMEOUT);
+        return;
+    }
+    const int start_pos = seq_start_pos[seq];
+    if (start_pos < 0) {                          // a padding request: its rows read as zeros downstream
+        const int rows = min(AL_BM, nrows - q_lo);
+        for (int i = tid; i < rows * (AL_HD / 8); i += blockDim.x)
+            *reinterpret_cast<uint4*>(out + (size_t)(row0 + q_lo + i / (AL_HD / 8)) * out_stride + (size_t)head * AL_HD + i % (AL_HD / 8) * 8) = make_uint4(0, 0, 0, 0);
+        return;
+    }
+    const int kvh = head / (nh / nkv);
+    const int* table = block_tables + (size_t)seq * max_pages;
+    const int pos_lo = start_pos + q_lo, pos_hi = start_pos + min(nrows, q_lo + AL_BM) - 1;
+    const int key_lo = gb_first_key(pos_lo, window), kt_begin = key_lo / AL_BN, total = pos_hi / AL_BN - kt_begin + 1;
+
+    if (tid == 0) {
+        mbar_init(&sh.q_full, 1);
+        for (int b = 0; b < AL_STAGES; ++b) {
+            mbar_init(&sh.k_full[b], 1);
+            mbar_init(&sh.k_empty[b], 1);
+            mbar_init(&sh.v_full[b], 1);
+            mbar_init(&sh.v_empty[b], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&sh.s_full[b], 1);
+            mbar_init(&sh.p_ready[b], 4);
+            mbar_init(&sh.pv_done[b], 1);
+        }
+        mbar_init(&sh.x_ready, 8);
+        sh.abort_flag = 0;
+        sh.issued[0] = sh.issued[1] = sh.consumed[0] = sh.consumed[1] = sh.q_issued = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_base)), "r"(AL_TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem_base;
+    volatile int* abort_flag = &sh.abort_flag;
+
+    if (warp == 0 || warp == AL_WARPS - 1) {
+        // ------------------------------------------------------------------------- producers
+        const int what = warp == 0 ? 0 : 1;
+        const int ppt = AL_BN >> page_shift;      // pages per key tile (1 .. 16), two boxes each
+        uint64_t* full = what == 0 ? sh.k_full : sh.v_full;
+        uint64_t* empty = what == 0 ? sh.k_empty : sh.v_empty;
+        unsigned char* ring = what == 0 ? Ks : Vs;
+        const CUtensorMap* map = what == 0 ? &map_k : &map_v;
+        int bad = 0;
+        if (what == 0 && lane == 0) {
+            mbar_expect_tx(&sh.q_full, AL_TILE);
+            tma_load_2d(Qs, &map_q, &sh.q_full, head * AL_HD, row0 + q_lo);
+            tma_load_2d(Qs + AL_BLOCK, &map_q, &sh.q_full, head * AL_HD + 64, row0 + q_lo);
+            sh.q_issued = 1;
+        }
+        auto page_of = [&](int kt) -> long long {      // this lane's page of key tile kt: lanes 2 i and 2 i + 1 have page i
+            long long page = 0;
+            if (lane < 2 * ppt) {
+                const int pi = ((kt * AL_BN) >> page_shift) + (lane >> 1);
+                page = pi < max_pages ? table[pi] : -1;
+                if (page < 0 || page >= num_pages) {
+                    const int first = pi << page_shift, last = first + page_size - 1;      // only a page that holds a key some row can see is missed
+                    if (first <= pos_hi && last >= key_lo) bad = 1;
+                    page = 0;
+                }
+            }
+            return page;
+        };
+        long long page = page_of(kt_begin);
+        for (int j = 0; j < total; ++j) {
+            const int s = j % AL_STAGES;
+            const long long next_page = j + 1 < total ? page_of(kt_begin + j + 1) : 0;      // in flight during the wait
+            int ok = 1;
+            if (lane == 0 && j >= AL_STAGES) ok = mbar_wait(&empty[s], ((j / AL_STAGES) - 1) & 1, abort_flag, status) ? 1 : 0;
+            ok = __shfl_sync(0xffffffffu, ok, 0);
+            if (!ok) break;
+            if (lane == 0) mbar_expect_tx(&full[s], AL_TILE);
+            __syncwarp();
+            if (lane < 2 * ppt)
+                tma_load_2d(ring + s * AL_TILE + (lane & 1) * AL_BLOCK + (lane >> 1) * page_size * 128, map, &full[s], (lane & 1) * 64,
+                            (int)((page * nkv + kvh) * page_size));
+            __syncwarp();
+            if (lane == 0) sh.issued[what] = j + 1;
+            page = next_page;
+        }
+        if (bad && what == 0) atomicOr(status, GB_STATUS_BAD_SLOT);
+    } else if (warp == 1) {
+        // ------------------------------------------------------------------------- MMA issuer
+        if (elect_one()) {
+            const uint32_t idesc_qk = umma_idesc(AL_BM, AL_BN), idesc_pv = umma_idesc(AL_BM, AL_HD) | (1u << 16);   // (B of the second is MN-major)
+            const uint64_t q_desc = umma_desc(smem_u32(Qs)), k_desc = umma_desc(smem_u32(Ks)), v_desc = al_desc_mn(smem_u32(Vs), AL_BLOCK);
+            bool ok = mbar_wait(&sh.q_full, 0, abort_flag, status);
+            // Whatever is ready is issued. The loop polls without blocking; the limit counts from the first look that found nothing.
+            int next_qk = 0, next_pv = 0;
+            long long t_idle = 0;
+            while (ok && next_pv < total) {
+                bool progressed = false;
+                if (next_qk < total && next_qk < next_pv + 2) {      // (S_j takes the place of P_{j-2}, whose product has been issued)
+                    const int j = next_qk, st = j % AL_STAGES;
+                    if (mbar_test(&sh.k_full[st], (j / AL_STAGES) & 1)) {
+                        tc_fence_after();
+                        const uint64_t kd = k_desc + (uint64_t)((st * AL_TILE) >> 4);
+#pragma unroll
+                        for (int k = 0; k < AL_HD / 16; ++k) {
+                            const uint64_t at = (uint64_t)((k / 4) * (AL_BLOCK >> 4) + (k % 4) * 2);
+                            umma_bf16(tmem + (uint32_t)((j & 1) * AL_BN), q_desc + at, kd + at, idesc_qk, k ? 1u : 0u);
+                        }
+                        umma_commit(&sh.s_full[j & 1]);
+                        umma_commit(&sh.k_empty[st]);
+                        ++next_qk;
+                        progressed = true;
+                    }
+                }
+                if (next_pv < next_qk) {
+                    const int j = next_pv, st = j % AL_STAGES;
+                    if (mbar_test(&sh.p_ready[j & 1], (j >> 1) & 1) && mbar_test(&sh.v_full[st], (j / AL_STAGES) & 1)) {
+                        tc_fence_after();
+                        const uint64_t vd = v_desc + (uint64_t)((st * AL_TILE) >> 4);
+                        const uint32_t pt = tmem + (uint32_t)((j & 1) * AL_BN);
+#pragma unroll
+                        for (int kk = 0; kk < AL_BN / 16; ++kk)      // 16 keys per instruction: 8 columns of P
+                            umma_bf16_ts(tmem + (uint32_t)(AL_O_COL + (j & 1) * AL_HD), pt + (uint32_t)(kk * 8), vd + (uint64_t)(kk * 16 * 128 >> 4), idesc_pv,
+                                         (j >= 2 || kk) ? 1u : 0u);
+                        umma_commit(&sh.pv_done[j & 1]);
+                        umma_commit(&sh.v_empty[st]);
+                        ++next_pv;
+                        progressed = true;
+                    }
+                }
+                if (progressed) {
+                    t_idle = 0;
+                } else if (*abort_flag) {
+                    ok = false;
+                } else if (t_idle == 0) {
+                    t_idle = clock64();
+                } else if (clock64() - t_idle > TC_WAIT_CYCLES) {
+                    *abort_flag = 1;
+                    atomicOr(status, GB_STATUS_WAIT_TIMEOUT);
+                    ok = false;
+                }
+            }
+            sh.consumed[0] = next_qk;
+            sh.consumed[1] = next_pv;
+        }
+    } else {
+        // ------------------------------------------------------------------------- softmax
+        const int q = warp & 3;                        // the quarter of TMEM lanes this warp may read
+        const int g = (warp - 2) >> 2;                 // the group: parity of its key tiles
+        const int r = q * 32 + lane;                   // this thread's query row within the tile
+        const float sl2 = scale * 1.4426950408889634f;
+        const uint32_t lane_base = tmem + ((uint32_t)(q * 32) << 16), s_col = (uint32_t)(g * AL_BN), o_col = (uint32_t)(AL_O_COL + g * AL_HD);
+        const int pos = pos_lo + r, first = gb_first_key(pos, window), first_last = gb_first_key(pos_lo + AL_BM - 1, window);
+        float m_run = AL_NEG_BIG, l_run = 0.f;
+        bool ok = true;
+        for (int j = g; j < total; j += 2) {
+            const int i = j >> 1, key0 = (kt_begin + j) * AL_BN;
+            if (!mbar_wait_warp(&sh.s_full[g], i & 1, abort_flag, status)) { ok = false; break; }
+            tc_fence_after();
+            uint32_t sv[AL_BN];
+            tmem_load128(lane_base + s_col, sv);
+            if (key0 + AL_BN - 1 > pos_lo || key0 < first_last) {
+#pragma unroll
+                for (int k = 0; k < AL_BN; ++k)
+                    if (key0 + k > pos || key0 + k < first) sv[k] = __float_as_uint(AL_NEG_BIG);
+            }
+            float mx4[4] = {AL_NEG_BIG, AL_NEG_BIG, AL_NEG_BIG, AL_NEG_BIG};
+#pragma unroll
+            for (int k = 0; k < AL_BN; k += 8)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) mx4[u] = al_max3(mx4[u], __uint_as_float(sv[k + 2 * u]), __uint_as_float(sv[k + 2 * u + 1]));
+            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+            // O_g += P V of the group's previous tile is complete before O_g is rescaled (S_j was issued behind it)
+            if (i > 0 && !mbar_wait_warp(&sh.pv_done[g], (i - 1) & 1, abort_flag, status)) { ok = false; break; }
+            // the running maximum rises, and O_g is rescaled, only when it is exceeded by more than 2^8 in the exponent
+            const bool raise = (mx - m_run) * sl2 > 8.0f;
+            if (i == 0) {
+                if (raise) m_run = mx;
+            } else if (__any_sync(0xffffffffu, raise)) {
+                tc_fence_after();
+                const float corr = raise ? al_exp2((m_run - mx) * sl2) : 1.0f;
+                if (raise) m_run = mx;
+                l_run *= corr;
+#pragma unroll
+                for (int c = 0; c < AL_HD; c += 32) {
+                    uint32_t ov[32];
+                    tmem_load32(lane_base + o_col + (uint32_t)c, ov);
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) ov[k] = __float_as_uint(__uint_as_float(ov[k]) * corr);
+                    tmem_store32(lane_base + o_col + (uint32_t)c, ov);
+                }
+            }
+            // P = exp2(S sl2 - m sl2). A masked key holds -1e30 and comes out as exactly 0; a row that has seen no key yet (its maximum is still
+            // -1e30) must not cancel that, so its offset is 0.
+            const float msl = m_run <= AL_NEG_BIG ? 0.f : m_run * sl2;
+            const float2 scale2 = make_float2(sl2, sl2), off2 = make_float2(-msl, -msl);
+            float2 l2[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+            uint32_t pw[AL_BN / 2];
+#pragma unroll
+            for (int c = 0; c < AL_BN; c += 2) {
+                const float2 y = __ffma2_rn(make_float2(__uint_as_float(sv[c]), __uint_as_float(sv[c + 1])), scale2, off2);
+                const float2 p = make_float2(al_exp2(y.x), al_exp2(y.y));
+                l2[(c >> 1) & 3] = __fadd2_rn(l2[(c >> 1) & 3], p);
+                pw[c >> 1] = al_pack(p.x, p.y);
+            }
+            const float2 lsum = __fadd2_rn(__fadd2_rn(l2[0], l2[1]), __fadd2_rn(l2[2], l2[3]));
+            l_run += lsum.x + lsum.y;
+            tmem_store64(lane_base + s_col, pw);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.p_ready[g]);
+        }
+        // merge: the groups post their maximum and sum per row, then each writes half of the channels
+        if (ok) {
+            sh.row_stat[g][0][r] = m_run;
+            sh.row_stat[g][1][r] = l_run;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.x_ready);
+            ok = mbar_wait_warp(&sh.x_ready, 0, abort_flag, status);
+        }
+        for (int gg = 0; gg < 2 && ok; ++gg) {         // both accumulators must be final
+            const int last = total - 1 - ((total - 1 - gg) & 1);      // the group's last tile
+            if (last >= 0) ok = mbar_wait_warp(&sh.pv_done[gg], (last >> 1) & 1, abort_flag, status);
+        }
+        if (ok) {
+            tc_fence_after();
+            const float m0 = sh.row_stat[0][0][r], l0 = sh.row_stat[0][1][r], m1 = sh.row_stat[1][0][r], l1 = sh.row_stat[1][1][r];
+            const float m = fmaxf(m0, m1);
+            const bool two = total > 1;                // (a group without tiles has never written its accumulator: it is not read)
+            const float a0 = al_exp2((m0 - m) * sl2), a1 = two ? al_exp2((m1 - m) * sl2) : 0.f;
+            const float l = two ? l0 * a0 + l1 * a1 : l0 * a0, inv = l != 0.f ? 1.0f / l : 0.f;
+            __nv_bfloat16* dst = out + (size_t)(row0 + q_lo + r) * out_stride + (size_t)head * AL_HD + g * 64;
+#pragma unroll
+            for (int c = 0; c < 64; c += 32) {
+                float o[32];
+                uint32_t ov[32];
+                tmem_load32(lane_base + (uint32_t)(AL_O_COL + g * 64 + c), ov);
+#pragma unroll
+                for (int k = 0; k < 32; ++k) o[k] = __uint_as_float(ov[k]) * a0;
+                if (two) {
+                    tmem_load32(lane_base + (uint32_t)(AL_O_COL + AL_HD + g * 64 + c), ov);
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) o[k] = fmaf(__uint_as_float(ov[k]), a1, o[k]);
+                }
+                if (q_lo + r < nrows) {
+#pragma unroll
+                    for (int k = 0; k < 32; k += 8) {
+                        uint4 w;
+                        w.x = pack2(__float_as_uint(o[k] * inv), __float_as_uint(o[k + 1] * inv));
+                        w.y = pack2(__float_as_uint(o[k + 2] * inv), __float_as_uint(o[k + 3] * inv));
+                        w.z = pack2(__float_as_uint(o[k + 4] * inv), __float_as_uint(o[k + 5] * inv));
+                        w.w = pack2(__float_as_uint(o[k + 6] * inv), __float_as_uint(o[k + 7] * inv));
+                        *reinterpret_cast<uint4*>(dst + c + k) = w;
+                    }
+                }
+            }
+        }
+    }
+
+    // ------------------------------------------------------------------------------- wind down
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        if (lane == 0 && sh.abort_flag) {
+            // copies that were issued but never consumed may still be in flight: wait for them (bounded)
+            const long long t0 = clock64();
+            while (sh.q_issued && !mbar_try_wait(&sh.q_full, 0) && clock64() - t0 < TC_WAIT_CYCLES) {}
+            for (int what = 0; what < 2; ++what)
+                for (int it = sh.consumed[what]; it < sh.issued[what]; ++it) {
+                    uint64_t* bar = what == 0 ? &sh.k_full[it % AL_STAGES] : &sh.v_full[it % AL_STAGES];
+                    const long long t1 = clock64();
+                    while (!mbar_try_wait(bar, (it / AL_STAGES) & 1) && clock64() - t1 < TC_WAIT_CYCLES) {}
+                }
+        }
+        __syncwarp();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(AL_TMEM_COLS) : "memory");
+    }
+}
+
+GB_EXPORT int gb_attention_prefill_128_supported(int nh, int nkv, int hd, int page_size) {
+    return nkv > 0 && nh % nkv == 0 && hd == AL_HD && page_size >= 8 && page_size <= AL_BN && (page_size & (page_size - 1)) == 0;
+}
+
+// Rows of each request are consecutive: request s owns rows seq_first_row[s] .. seq_first_row[s+1]-1, at positions seq_start_pos[s] + local index.
+// q, out: bfloat16, rows aligned to 16 bytes; kcache, vcache: [num_pages, nkv, page_size, 128] contiguous.
+GB_EXPORT int gb_attention_prefill_128(const void* q, long long q_stride, int n_rows, void* out, long long out_stride, const void* kcache,
+                                       const void* vcache, const int* block_tables, int max_pages, const int* seq_first_row, const int* seq_start_pos,
+                                       int num_seqs, int max_rows_per_seq, int nh, int nkv, int hd, int page_size, long long num_pages, float scale,
+                                       int window, int* status, cudaStream_t stream) {
+    GB_REQUIRE(gb_attention_prefill_128_supported(nh, nkv, hd, page_size),
+               "gb_attention_prefill_128: %d/%d heads of %d in pages of %d (a power of two, 8..128) are not built", nh, nkv, hd, page_size);
+    GB_REQUIRE(q_stride % 8 == 0 && (uintptr_t)q % 16 == 0 && q_stride >= (long long)nh * hd && out_stride % 8 == 0 && (uintptr_t)out % 16 == 0,
+               "gb_attention_prefill_128: rows must be 16-byte aligned");
+    GB_REQUIRE((uintptr_t)kcache % 16 == 0 && (uintptr_t)vcache % 16 == 0, "gb_attention_prefill_128: the pages must be 16-byte aligned");
+    GB_REQUIRE(num_seqs >= 0 && num_seqs <= 65535 && max_pages > 0 && status != nullptr && n_rows >= 0 && window >= 0,
+               "gb_attention_prefill_128: bad batch shape");
+    GB_REQUIRE(num_pages > 0 && num_pages * nkv * page_size < (1ll << 31) && (long long)max_pages * page_size < (1ll << 31) - 256,
+               "gb_attention_prefill_128: the pages hold too many rows");
+    if (num_seqs == 0 || n_rows == 0 || max_rows_per_seq <= 0) return 0;
+    const int tiles = gb_ceil_div(max_rows_per_seq, AL_BM);
+    GB_REQUIRE(tiles <= 65535, "gb_attention_prefill_128: %d rows a request are too many for one launch", max_rows_per_seq);
+    CUtensorMap mq, mk, mv;
+    if (tc_make_map_2d(&mq, q, n_rows, (long long)nh * hd, q_stride, AL_BM, 64, "gb_attention_prefill_128")) return 1;
+    if (tc_make_map_2d(&mk, kcache, num_pages * nkv * page_size, hd, hd, page_size, 64, "gb_attention_prefill_128")) return 1;
+    if (tc_make_map_2d(&mv, vcache, num_pages * nkv * page_size, hd, hd, page_size, 64, "gb_attention_prefill_128")) return 1;
+    const cudaError_t e = cudaFuncSetAttribute(attention_prefill_128_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, AL_SMEM);
+    GB_REQUIRE(e == cudaSuccess, "gb_attention_prefill_128: %d bytes of shared memory refused: %s", AL_SMEM, cudaGetErrorString(e));
+    int page_shift = 0;
+    while ((1 << page_shift) < page_size) ++page_shift;
+    gb_launch(GB_PDL_ATTENTION, attention_prefill_128_kernel, dim3(nh, num_seqs, tiles), dim3(AL_WARPS * 32), AL_SMEM, stream, mq, mk, mv,
+              (__nv_bfloat16*)out, out_stride, block_tables, max_pages, seq_first_row, seq_start_pos, nh, nkv, page_size, page_shift, num_pages, scale,
+              window, status);
+    return gb_check_launch("gb_attention_prefill_128");
+}

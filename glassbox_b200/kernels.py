@@ -177,6 +177,8 @@ _SIGNATURES = {
     "gb_kv4_expand": [_P, _P, _P, _P, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _LL, _I, _P, _P],
     "gb_kv4_attention_rows": [_P, _LL, _P, _LL, _I, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _LL, _F, _I, _I, _P, _P, _P],
     "gb_kv4_attention_decode": [_P, _LL, _P, _LL, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _LL, _F, _I, _I, _I, _P, _P, _P],
+    "gb_attention_prefill_128_supported": [_I, _I, _I, _I],
+    "gb_attention_prefill_128": [_P, _LL, _I, _P, _LL, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _LL, _F, _I, _P, _P],
     "gb_kv4_attention_decode_supported": [_I],
     "gb_kv4_attention_decode_blocks": [_I, _I, _I, _I, _LL],
     "gb_token_logprobs": [_P, _I, _LL, _P, _P, _P, _P, _P, _I, _I, _I, _P],
@@ -2345,14 +2347,17 @@ KV4_TILE = 16       # tokens of a tile of the layout: page sizes are multiples o
 KV4_GROUP = 32      # neighbouring channels that share a scale
 
 
-def _here(*tensors) -> None:
-    """The operands lie on the current device: the launch goes to its current stream."""
-    device = torch.cuda.current_device() if torch.cuda.is_available() else -2
+def _here(*tensors) -> int:
+    """The stream to launch on: the current one of the current device, on which all operands must lie."""
+    if not tensors[0].is_cuda:
+        raise KernelError("kernel operands must be CUDA tensors; there is no CPU path")
+    device = torch.cuda.current_device()
     for t in tensors:
         if t is not None and t.get_device() != device:
             if not t.is_cuda:
                 raise KernelError("kernel operands must be CUDA tensors; there is no CPU path")
             raise KernelError(f"kernel operands must lie on the current device cuda:{device}, not on {t.device}")
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 def _vector(name: str, t: torch.Tensor, n: int) -> None:
@@ -2371,15 +2376,14 @@ def kv4_page_bytes(page_size: int, hd: int) -> int:
 
 
 def _kv4_pool(kcache: torch.Tensor, vcache: torch.Tensor, nkv: int, hd: int, page_size: int) -> None:
-    if not (kv4_supported(hd, page_size)):
+    if not kv4_supported(hd, page_size):
         raise KernelError(f"a cache in 4 bits holds heads of a multiple of 32 channels up to 256 in pages of a multiple of 16 "
                           f"tokens, not heads of {hd} in pages of {page_size}")
-    size = kv4_page_bytes(page_size, hd)
-    for name, t in (("kcache", kcache), ("vcache", vcache)):
-        if not (t.dtype == torch.uint8 and t.dim() == 3 and t.shape[1] == nkv and t.shape[2] == size and t.is_contiguous()):
-            raise KernelError(f"{name} must be a contiguous uint8 tensor [pages, {nkv}, {size}], not {t.dtype} {tuple(t.shape)}")
-    if not (kcache.shape[0] == vcache.shape[0] > 0):
-        raise KernelError("kcache and vcache must have the same number of pages, at least one")
+    shape = kcache.shape
+    if (kcache.dtype is not torch.uint8 or vcache.dtype is not torch.uint8 or vcache.shape != shape or len(shape) != 3 or shape[0] == 0
+            or shape[1] != nkv or shape[2] != kv4_page_bytes(page_size, hd) or not kcache.is_contiguous() or not vcache.is_contiguous()):
+        raise KernelError(f"kcache and vcache must be contiguous uint8 tensors [pages, {nkv}, {kv4_page_bytes(page_size, hd)}], not {kcache.dtype} "
+                          f"{tuple(shape)} and {vcache.dtype} {tuple(vcache.shape)}")
 
 
 def kv4_write(qkv: torch.Tensor, q: torch.Tensor, cos_sin: Optional[torch.Tensor], positions: torch.Tensor, slots: torch.Tensor,
@@ -2411,10 +2415,10 @@ def kv4_write(qkv: torch.Tensor, q: torch.Tensor, cos_sin: Optional[torch.Tensor
         raise KernelError(f"rotary size {rot} must be even and at most the head size {hd}")
     if not (rot == 0 or (cos_sin.dtype == torch.float32 and cos_sin.is_contiguous() and cos_sin.shape[1:] == (rot // 2, 2))):
         raise KernelError(f"cos_sin must be contiguous float32 [positions, {rot // 2}, 2]")
-    _here(qkv, q, cos_sin, positions, slots, kcache, vcache, status)
+    stream = _here(qkv, q, cos_sin, positions, slots, kcache, vcache, status)
     _call("gb_kv4_write", qkv.data_ptr(), qkv.stride(0), _dt(qkv), q.data_ptr(), q.stride(0), _ptr(cos_sin), positions.data_ptr(), slots.data_ptr(),
           kcache.data_ptr(), vcache.data_ptr(), n, nh, nkv, hd, rot, cos_sin.shape[0] if rot else 0, page_size, kcache.shape[0],
-          1 if write_kv else 0, status.data_ptr(), _stream())
+          1 if write_kv else 0, status.data_ptr(), stream)
 
 
 def kv4_read(kcache: torch.Tensor, vcache: torch.Tensor, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor, page_size: int,
@@ -2426,12 +2430,12 @@ def kv4_read(kcache: torch.Tensor, vcache: torch.Tensor, slots: torch.Tensor, k:
     n, nkv, hd = k.shape
     _kv4_pool(kcache, vcache, nkv, hd, page_size)
     _vector("slots", slots, n)
-    _here(kcache, vcache, slots, k, v, status)
+    stream = _here(kcache, vcache, slots, k, v, status)
     _call("gb_kv4_read", kcache.data_ptr(), vcache.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), _dt(k), n, nkv, hd, page_size,
-          kcache.shape[0], status.data_ptr(), _stream())
+          kcache.shape[0], status.data_ptr(), stream)
 
 
-def _kv4_attention(q, out, kcache, vcache, block_tables, row_seq, positions, nh, nkv, hd, page_size, status) -> int:
+def _kv4_attention(q, out, kcache, vcache, block_tables, row_seq, positions, nh, nkv, hd, page_size) -> int:
     n = q.shape[0]
     _kv4_pool(kcache, vcache, nkv, hd, page_size)
     if not (nh % nkv == 0):
@@ -2444,8 +2448,6 @@ def _kv4_attention(q, out, kcache, vcache, block_tables, row_seq, positions, nh,
         raise KernelError("block_tables must be contiguous int32 [requests, pages]")
     _vector("row_seq", row_seq, n)
     _vector("positions", positions, n)
-    _dt(q)
-    _here(q, out, kcache, vcache, block_tables, row_seq, positions, status)
     return n
 
 
@@ -2491,21 +2493,22 @@ def kv4_attention_decode(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tenso
     float32 [n, nh * hd], rows may be strided; a row of position < 0 comes out as zeros. ``max_context``: no row has more keys in
     sight than this matters for (it sizes the shares of a row's keys, longer rows are still right). ``parts``: ``kv4_decode_parts``
     of the same rows, heads and ``max_context`` (with the window or without)."""
-    n = _kv4_attention(q, out, kcache, vcache, block_tables, row_seq, positions, nh, nkv, hd, page_size, status)
+    n = _kv4_attention(q, out, kcache, vcache, block_tables, row_seq, positions, nh, nkv, hd, page_size)
+    dtype = _dt(q)
+    stream = _here(q, out, kcache, vcache, block_tables, row_seq, positions, status, parts)
     kind, number, floats = kv4_decode_plan(n, nh, nkv, hd, max_context, window, q.dtype)
     if floats:
         if parts is None or parts.dtype != torch.float32 or not parts.is_contiguous() or parts.numel() < floats:
             raise KernelError(f"this batch needs contiguous float32 scratch of {floats} numbers (kv4_decode_parts)")
-        _here(parts)
     if kind == "rows":
-        _call("gb_kv4_attention_rows", q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), _dt(q), kcache.data_ptr(), vcache.data_ptr(),
+        _call("gb_kv4_attention_rows", q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), dtype, kcache.data_ptr(), vcache.data_ptr(),
               block_tables.data_ptr(), block_tables.shape[1], row_seq.data_ptr(), positions.data_ptr(), n, nh, nkv, hd, page_size,
-              kcache.shape[0], float(scale), int(window or 0), number, _ptr(parts), status.data_ptr(), _stream())
+              kcache.shape[0], float(scale), int(window or 0), number, _ptr(parts), status.data_ptr(), stream)
     else:
         _call("gb_kv4_attention_decode", q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), kcache.data_ptr(), vcache.data_ptr(),
               block_tables.data_ptr(), block_tables.shape[1], row_seq.data_ptr(), positions.data_ptr(), n, nh, nkv, hd, page_size,
               kcache.shape[0], float(scale), int(window or 0), number if kind == "cluster" else 1, number if kind == "even" else 0, _ptr(parts),
-              status.data_ptr(), _stream())
+              status.data_ptr(), stream)
 
 
 def kv4_expand(kcache: torch.Tensor, vcache: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor, block_tables: torch.Tensor,
@@ -2524,10 +2527,10 @@ def kv4_expand(kcache: torch.Tensor, vcache: torch.Tensor, kpages: torch.Tensor,
     S = block_tables.shape[0]
     _vector("seq_first_row", seq_first_row, S + 1)
     _vector("seq_start_pos", seq_start_pos, S)
-    _here(kcache, vcache, kpages, vpages, block_tables, seq_first_row, seq_start_pos, status)
+    stream = _here(kcache, vcache, kpages, vpages, block_tables, seq_first_row, seq_start_pos, status)
     _call("gb_kv4_expand", kcache.data_ptr(), vcache.data_ptr(), kpages.data_ptr(), vpages.data_ptr(), _dt(kpages), block_tables.data_ptr(),
           block_tables.shape[1], seq_first_row.data_ptr(), seq_start_pos.data_ptr(), S, -(-int(max_context) // page_size), nkv, hd, page_size,
-          kcache.shape[0], int(window or 0), status.data_ptr(), _stream())
+          kcache.shape[0], int(window or 0), status.data_ptr(), stream)
 
 
 def kv4_attention_prefill(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, block_tables: torch.Tensor,
@@ -2537,14 +2540,20 @@ def kv4_attention_prefill(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tens
     """``kv4_attention_decode`` for portions of prompts, runs of consecutive rows of a request: the pages in sight are unpacked into
     kpages/vpages (q's type, [pages, nkv, page_size, hd], numbers everywhere: zero them once) and read from there by the prompt kernel that
     takes the shape. ``max_context`` bounds the tokens that a request holds after the step."""
-    n = _kv4_attention(q, out, kcache, vcache, block_tables, row_seq, positions, nh, nkv, hd, page_size, status)
+    n = _kv4_attention(q, out, kcache, vcache, block_tables, row_seq, positions, nh, nkv, hd, page_size)
     if not (kpages.dtype == q.dtype and kpages.shape[1:] == (nkv, page_size, hd)):
         raise KernelError(f"kpages must be {q.dtype} [pages, {nkv}, {page_size}, {hd}]")
+    _dt(q)
+    stream = _here(q, out, row_seq, positions, kpages)
     kv4_expand(kcache, vcache, kpages, vpages, block_tables, seq_first_row, seq_start_pos, max_context, window, status)
     args = (q, out, kpages, vpages, block_tables, seq_first_row, seq_start_pos, max_rows_per_seq, nh, nkv, hd, page_size, scale, window, status)
     aligned = q.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0 and q.stride(0) % 8 == 0 and out.stride(0) % 8 == 0
     if attention_prefill_tc_supported(q, out, nh, nkv, hd, page_size):
         attention_prefill_tc(*args)
+    elif aligned and q.dtype == torch.bfloat16 and lib().gb_attention_prefill_128_supported(nh, nkv, hd, page_size):
+        _call("gb_attention_prefill_128", q.data_ptr(), q.stride(0), n, out.data_ptr(), out.stride(0), kpages.data_ptr(), vpages.data_ptr(),
+              block_tables.data_ptr(), block_tables.shape[1], seq_first_row.data_ptr(), seq_start_pos.data_ptr(), block_tables.shape[0],
+              int(max_rows_per_seq), nh, nkv, hd, page_size, kpages.shape[0], float(scale), int(window or 0), status.data_ptr(), stream)
     elif aligned and attention_prefill_supported(q.dtype, nh, nkv, hd, page_size):
         attention_prefill(*args)
     elif attention_prefill_f32_supported(q, out, nh, nkv, hd):
@@ -2583,6 +2592,6 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, logprob: torch.Te
             raise KernelError(f"{top} alternatives: between 1 and {min(LOGPROBS_MAX_TOP, vocab)} can be asked for")
     if not (top_logprob is None or (top_ids is not None and top_logprob.dtype == torch.float32 and top_logprob.shape == top_ids.shape and top_logprob.is_contiguous())):
         raise KernelError("top_logprob must be contiguous float32 of top_ids' shape")
-    _here(logits, tokens, logprob, entropy, top_logprob, top_ids)
+    stream = _here(logits, tokens, logprob, entropy, top_logprob, top_ids)
     _call("gb_token_logprobs", logits.data_ptr(), _dt(logits), logits.stride(0), tokens.data_ptr(), logprob.data_ptr(), _ptr(entropy),
-          _ptr(top_logprob), _ptr(top_ids), top, rows, vocab, _stream())
+          _ptr(top_logprob), _ptr(top_ids), top, rows, vocab, stream)
