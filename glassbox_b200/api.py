@@ -6,13 +6,28 @@ token ids.
 """
 from __future__ import annotations
 
+from dataclasses import dataclass
 from typing import List, Optional, Sequence, Union
 
 import numpy as np
 
+from . import kernels
 from .engine.engine import Engine, StepEntry
 from .engine.scheduler import Request, Scheduler, SchedulerConfig
 from .sampling.sampler import SamplerConfig
+
+
+@dataclass
+class Score:
+    """What a model says of a text of n tokens: arrays with a row for each token but the first."""
+    logprobs: np.ndarray         # float32 [n - 1]: log probability of token i + 1 given tokens 0 .. i
+    entropies: np.ndarray        # float32 [n - 1]: entropy of the distribution that token i + 1 was drawn from, in nats
+    top_ids: np.ndarray          # int32 [n - 1, top]: its most probable tokens, in falling order
+    top_logprobs: np.ndarray     # float32 [n - 1, top]
+
+    @property
+    def perplexity(self) -> float:
+        return float(np.exp(-np.mean(self.logprobs, dtype=np.float64))) if len(self.logprobs) else float("nan")
 
 
 class LLM:
@@ -20,13 +35,15 @@ class LLM:
 
     Option names follow the reference's command line (crates/glassbox-server/src/main.rs:322-330):
     ``blocks`` pages of 16 tokens in the cache (2048), ``budget`` tokens per step (256),
-    ``max_seqs`` requests running at once (32), ``prefix_cache`` (on).
+    ``max_seqs`` requests running at once (32), ``prefix_cache`` (on). ``cache_bits`` 4 keeps keys and values in four
+    bits (``Engine``).
     """
 
     def __init__(self, model_dir: str, dtype: str = "bfloat16", *, blocks: int = 2048, budget: int = 256,
-                 max_seqs: int = 32, prefix_cache: bool = True, page_size: int = 16, device: str = "cuda:0"):
+                 max_seqs: int = 32, prefix_cache: bool = True, page_size: int = 16, device: str = "cuda:0",
+                 cache_bits: Optional[int] = None):
         self.engine = Engine(model_dir, dtype, num_pages=blocks, page_size=page_size, max_batch_tokens=budget,
-                             max_requests=max_seqs, share_prefixes=prefix_cache, device=device)
+                             max_requests=max_seqs, share_prefixes=prefix_cache, device=device, cache_bits=cache_bits)
         self.scheduler_config = SchedulerConfig(token_budget=budget, max_seqs=max_seqs)
         self.scheduler = Scheduler(self.engine, self.scheduler_config)
 
@@ -71,6 +88,38 @@ class LLM:
             return (outs[0], reasons[0]) if single else (outs, reasons)
         return outs[0] if single else outs
 
+    def score(self, prompts: Union[Sequence[int], Sequence[Sequence[int]]], *, top: int = 0):
+        """What the model says of given texts: a ``Score`` for each prompt (one, or a list in the order given), with the ``top``
+        most probable tokens at every place (up to 32). A prompt goes through the engine by itself, in portions of the step's token
+        budget; it needs a state slot and pages beside those of requests in flight, and gives them back."""
+        single = len(prompts) > 0 and not isinstance(prompts[0], (list, tuple, np.ndarray))
+        batch = [prompts] if single else list(prompts)
+        if not 0 <= top <= kernels.LOGPROBS_MAX_TOP:
+            raise ValueError(f"top {top} must be between 0 and {kernels.LOGPROBS_MAX_TOP}")
+        for i, p in enumerate(batch):
+            if not 0 < len(p) <= self.engine.max_position:
+                raise ValueError(f"prompt {i} has {len(p)} tokens; a prompt needs between 1 and max_position = {self.engine.max_position}")
+        scores = [self._score([int(t) for t in p], top) for p in batch]
+        return scores[0] if single else scores
+
+    def _score(self, tokens: List[int], top: int) -> Score:
+        engine, rows = self.engine, []
+        LLM._scored += 1
+        rid = ("score", LLM._scored)
+        engine.add_request(rid)
+        try:
+            for a in range(0, len(tokens) - 1, engine.max_batch_tokens):
+                part = tokens[a:min(a + engine.max_batch_tokens, len(tokens) - 1)]
+                logits = engine.step([StepEntry(rid, part, list(range(len(part))))])
+                rows.append(engine.logprobs(logits, tokens[a + 1:a + 1 + len(part)], top))
+            engine.check()
+        finally:
+            engine.free_request(rid)
+        if not rows:
+            rows = [(np.empty(0, np.float32), np.empty(0, np.float32), np.empty((0, top), np.int32), np.empty((0, top), np.float32))]
+        return Score(*(np.concatenate(column) for column in zip(*rows)))
+
+    _scored = 0
 
     def fork(self, request_id: int, **kwargs) -> int:
         """Fork a request that is in flight (see ``Scheduler.fork``); for callers that drive

@@ -3,7 +3,8 @@ fixed-size per-request state. This file allocates and hands out views; it decide
 
 Paged group storage: K and V each ``[cache layers of the group, pages, kv_heads, page_size,
 head_dim]`` in the activation dtype, so one (page, kv head) is a contiguous
-``page_size x head_dim`` tile, which is what the attention kernels stream.
+``page_size x head_dim`` tile, which is what the attention kernels stream. A group kept in 4 bits (``PagedKvSpec.bits``) holds
+bytes instead, ``[cache layers, pages, kv_heads, bytes of a head's page]``.
 State storage: one tensor ``[max_requests, *shape]`` per cache layer whose mixer asked for it.
 """
 from __future__ import annotations
@@ -13,13 +14,14 @@ from typing import Dict, List, Optional
 
 import torch
 
+from .. import kernels
 from ..parts.base import CombinedCacheSpec, PagedKvSpec, StateSpec
 
 
 @dataclass
 class PagedLayerView:
     """What a mixer sees of its cache layer during one step."""
-    k: torch.Tensor                 # [pages, kv_heads, page_size, head_dim]
+    k: torch.Tensor                 # [pages, kv_heads, page_size, head_dim]; in 4 bits: uint8 [pages, kv_heads, bytes of a page]
     v: torch.Tensor
     page_size: int
     group: int
@@ -97,6 +99,14 @@ class DeviceCache:
         for g, spec in enumerate(self.group_specs):
             shape = (len(members[g]), self.group_pages[g], spec.num_kv_heads, page_size, spec.head_dim)
             value_dim = spec.head_dim if spec.value_dim is None else spec.value_dim
+            if spec.bits is not None:
+                if spec.bits != 4 or value_dim != spec.head_dim or not kernels.kv4_supported(spec.head_dim, page_size):
+                    raise ValueError(f"a cache in {spec.bits} bits of heads of {spec.head_dim} / {value_dim} channels in pages of {page_size} tokens is "
+                                     f"not built (4 bits, a multiple of 32 channels up to 256, a multiple of 16 tokens)")
+                packed = shape[:3] + (kernels.kv4_page_bytes(page_size, spec.head_dim),)
+                self.k.append(torch.zeros(packed, dtype=torch.uint8, device=device))
+                self.v.append(torch.zeros(packed, dtype=torch.uint8, device=device))
+                continue
             self.k.append(torch.zeros(shape, dtype=dtype, device=device))
             self.v.append(torch.zeros(shape[:-1] + (value_dim,), dtype=dtype, device=device))
 
@@ -107,6 +117,9 @@ class DeviceCache:
     def bytes_per_token(self) -> int:
         total = 0
         for g, spec in enumerate(self.group_specs):
+            if spec.bits is not None:
+                total += (self.k[g][:, 0].numel() + self.v[g][:, 0].numel()) // self.page_size
+                continue
             value_dim = spec.head_dim if spec.value_dim is None else spec.value_dim
             total += self.k[g].shape[0] * spec.num_kv_heads * (spec.head_dim + value_dim) * self.k[g].element_size()
         return total

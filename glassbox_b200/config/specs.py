@@ -12,6 +12,7 @@ handed to the part that uses them, layer by layer.
 """
 from __future__ import annotations
 
+import dataclasses
 from dataclasses import dataclass, field
 from typing import Any, Optional, Tuple
 
@@ -96,7 +97,8 @@ class GqaAttentionSpec:
     """Causal grouped-query attention over a paged key/value cache.
 
     ``window`` None means every earlier key is visible; an integer w means a query at
-    position p sees keys p-w+1 .. p. ``scale`` multiplies the scores before softmax.
+    position p sees keys p-w+1 .. p. ``scale`` multiplies the scores before softmax. ``cache_bits`` None keeps keys and values
+    in the activation type; 4 keeps them as four-bit codes with a scale for every 32 channels.
     """
     num_heads: int
     num_kv_heads: int
@@ -104,6 +106,7 @@ class GqaAttentionSpec:
     scale: float
     position: Any
     window: Optional[int] = None
+    cache_bits: Optional[int] = None
     kind: str = "gqa_attention"
 
 
@@ -512,3 +515,16 @@ class ModelConfig:
         for c in range(self.num_cache_layers):
             if c not in writers:
                 raise ConfigError(f"cache layer {c} is never written")
+
+
+def with_cache_bits(config: "ModelConfig", bits: int) -> "ModelConfig":
+    """The same model with every attention layer's keys and values kept in ``bits`` bits (4)."""
+    if bits != 4:
+        raise ConfigError(f"a cache in {bits} bits is not built (4)")
+    layers = []
+    for i, layer in enumerate(config.layers):
+        if not hasattr(layer.mixer, "cache_bits"):
+            raise ConfigError(f"layer {i}: the cache of {getattr(layer.mixer, 'kind', layer.mixer)!r} cannot be kept in {bits} bits "
+                              f"(grouped-query attention's can)")
+        layers.append(dataclasses.replace(layer, mixer=dataclasses.replace(layer.mixer, cache_bits=bits)))
+    return dataclasses.replace(config, layers=type(config.layers)(layers))

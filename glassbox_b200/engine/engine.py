@@ -20,7 +20,7 @@ from .. import kernels
 from ..cache.device import DeviceCache
 from ..cache.manager import CacheManager, GroupSpec, OutOfPages
 from ..config.registry import get_architecture, load_config
-from ..config.specs import ModelConfig
+from ..config.specs import ModelConfig, with_cache_bits
 from ..weights.loader import load_parameters, open_model_weights
 from .context import Scratch, SeqInfo, StepContext, WeightOrder
 from .model import DecoderModel
@@ -54,10 +54,12 @@ class Engine:
                  num_pages: Optional[int] = None, page_size: int = 16, max_batch_tokens: int = 2048,
                  max_requests: int = 64, share_prefixes: bool = False, device: str = "cuda:0",
                  config: Optional[ModelConfig] = None, use_graphs: bool = True, use_programs: bool = False,
-                 group_pages=None):
+                 group_pages=None, cache_bits: Optional[int] = None):
         """``cache_tokens`` / ``num_pages`` size the page pool of every cache group alike; ``group_pages`` (a function
         from a group's ``PagedKvSpec`` to a number of pages) sizes each group on its own, for models whose groups need
-        different amounts: a group that keeps a window of keys needs far fewer pages than one that keeps them all."""
+        different amounts: a group that keeps a window of keys needs far fewer pages than one that keeps them all. ``cache_bits`` 4
+        keeps the keys and values of grouped-query attention in four bits (``kernels.kv4_write``): 0.5625 bytes a number; prompts then
+        need pages of the activation type for one layer beside them."""
         if not torch.cuda.is_available():
             raise RuntimeError("glassbox_b200 needs a CUDA device: every kernel is CUDA and there is no CPU path")
         self.device = torch.device(device)
@@ -65,6 +67,8 @@ class Engine:
         kernels.lib()  # build/load now, so a missing toolchain fails here and loudly
         self.dtype = parse_dtype(dtype)
         self.config = config if config is not None else load_config(model_dir)
+        if cache_bits is not None:
+            self.config = with_cache_bits(self.config, cache_bits)
         self.model = DecoderModel(self.config)
         arch = get_architecture(self.config.architecture)
         with open_model_weights(model_dir) as st:
@@ -575,6 +579,21 @@ class Engine:
             else:
                 result.append(int(picked[r]))
         return result
+
+    def logprobs(self, logits: torch.Tensor, tokens: Sequence[int], top: int = 0):
+        """Of each row of ``logits`` (as ``step`` returned them): the log probability of its token, the entropy of its distribution in
+        nats, and the ``top`` most probable tokens with their log probabilities. NumPy arrays (logprob, entropy, top_ids,
+        top_logprobs), the last two [rows, top] (``kernels.token_logprobs``)."""
+        n = logits.shape[0]
+        if len(tokens) != n:
+            raise ValueError(f"{len(tokens)} tokens for {n} rows of logits")
+        asked = torch.tensor([int(t) for t in tokens], dtype=torch.int32, device=self.device)
+        logprob, entropy = torch.empty(n, device=self.device), torch.empty(n, device=self.device)
+        best = torch.empty(n, top, device=self.device)
+        ids = torch.empty(n, top, dtype=torch.int32, device=self.device)
+        if n:
+            kernels.token_logprobs(logits, asked, logprob, entropy, best if top else None, ids if top else None)
+        return logprob.cpu().numpy(), entropy.cpu().numpy(), ids.cpu().numpy(), best.cpu().numpy()
 
     def check(self) -> None:
         """Synchronise and raise if any kernel since the last check skipped a bad index."""

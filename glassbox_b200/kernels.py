@@ -2533,36 +2533,54 @@ def kv4_expand(kcache: torch.Tensor, vcache: torch.Tensor, kpages: torch.Tensor,
           kcache.shape[0], int(window or 0), status.data_ptr(), stream)
 
 
+def kv4_prompt_kernel(q: torch.Tensor, out: torch.Tensor, nh: int, nkv: int, hd: int, page_size: int) -> Optional[str]:
+    """Which kernel over unpacked pages takes portions of prompts of this shape; None: there is none that works on tiles of rows."""
+    if attention_prefill_tc_supported(q, out, nh, nkv, hd, page_size):
+        return "tcgen05"
+    if attention_prefill_f32_supported(q, out, nh, nkv, hd):
+        return "float32"
+    if q.dtype != torch.bfloat16 or q.data_ptr() % 16 or out.data_ptr() % 16 or q.stride(0) % 8 or out.stride(0) % 8:
+        return None
+    if lib().gb_attention_prefill_128_supported(nh, nkv, hd, page_size):
+        return "tcgen05_128"
+    if attention_prefill_supported(q.dtype, nh, nkv, hd, page_size):
+        return "mma"
+    return "tiles" if q.is_contiguous() and out.is_contiguous() and sink_attention_tiles_supported(q.dtype, hd, hd) else None
+
+
 def kv4_attention_prefill(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, block_tables: torch.Tensor,
                           row_seq: torch.Tensor, positions: torch.Tensor, seq_first_row: torch.Tensor, seq_start_pos: torch.Tensor,
                           max_rows_per_seq: int, nh: int, nkv: int, hd: int, page_size: int, scale: float, window: Optional[int],
                           max_context: int, kpages: torch.Tensor, vpages: torch.Tensor, status: torch.Tensor) -> None:
     """``kv4_attention_decode`` for portions of prompts, runs of consecutive rows of a request: the pages in sight are unpacked into
     kpages/vpages (q's type, [pages, nkv, page_size, hd], numbers everywhere: zero them once) and read from there by the prompt kernel that
-    takes the shape. ``max_context`` bounds the tokens that a request holds after the step."""
+    takes the shape (``kv4_prompt_kernel``); where none does, row by row. ``max_context`` bounds the tokens that a request holds after the
+    step. Two calls that may run at the same time need pages of their own to unpack into."""
     n = _kv4_attention(q, out, kcache, vcache, block_tables, row_seq, positions, nh, nkv, hd, page_size)
     if not (kpages.dtype == q.dtype and kpages.shape[1:] == (nkv, page_size, hd)):
         raise KernelError(f"kpages must be {q.dtype} [pages, {nkv}, {page_size}, {hd}]")
     _dt(q)
     stream = _here(q, out, row_seq, positions, kpages)
+    kind = kv4_prompt_kernel(q, out, nh, nkv, hd, page_size)
+    if kind is None and q.dtype == torch.bfloat16 and lib().gb_kv4_attention_decode_supported(hd):
+        _here(kcache, vcache, block_tables, status)
+        _call("gb_kv4_attention_decode", q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), kcache.data_ptr(), vcache.data_ptr(),
+              block_tables.data_ptr(), block_tables.shape[1], row_seq.data_ptr(), positions.data_ptr(), n, nh, nkv, hd, page_size,
+              kcache.shape[0], float(scale), int(window or 0), 1, 0, 0, status.data_ptr(), stream)
+        return
     kv4_expand(kcache, vcache, kpages, vpages, block_tables, seq_first_row, seq_start_pos, max_context, window, status)
-    args = (q, out, kpages, vpages, block_tables, seq_first_row, seq_start_pos, max_rows_per_seq, nh, nkv, hd, page_size, scale, window, status)
-    aligned = q.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0 and q.stride(0) % 8 == 0 and out.stride(0) % 8 == 0
-    if attention_prefill_tc_supported(q, out, nh, nkv, hd, page_size):
-        attention_prefill_tc(*args)
-    elif aligned and q.dtype == torch.bfloat16 and lib().gb_attention_prefill_128_supported(nh, nkv, hd, page_size):
+    if kind is None:
+        attention_rows(q, out, kpages, vpages, block_tables, row_seq, positions, nh, nkv, hd, page_size, scale, window, status)
+    elif kind == "tcgen05_128":
         _call("gb_attention_prefill_128", q.data_ptr(), q.stride(0), n, out.data_ptr(), out.stride(0), kpages.data_ptr(), vpages.data_ptr(),
               block_tables.data_ptr(), block_tables.shape[1], seq_first_row.data_ptr(), seq_start_pos.data_ptr(), block_tables.shape[0],
               int(max_rows_per_seq), nh, nkv, hd, page_size, kpages.shape[0], float(scale), int(window or 0), status.data_ptr(), stream)
-    elif aligned and attention_prefill_supported(q.dtype, nh, nkv, hd, page_size):
-        attention_prefill(*args)
-    elif attention_prefill_f32_supported(q, out, nh, nkv, hd):
-        attention_prefill_f32(*args)
-    elif aligned and q.is_contiguous() and out.is_contiguous() and sink_attention_tiles_supported(q.dtype, hd, hd):
+    elif kind == "tiles":
         sink_attention_tiles(q, out, kpages, vpages, block_tables, seq_first_row, seq_start_pos, max_rows_per_seq, r1=None, r2=None, sink=None,
                              gate=None, heads=nh, kv_heads=nkv, dim=hd, vdim=hd, page_size=page_size, scale=scale, window=window, status=status)
     else:
-        attention_rows(q, out, kpages, vpages, block_tables, row_seq, positions, nh, nkv, hd, page_size, scale, window, status)
+        attend = {"tcgen05": attention_prefill_tc, "mma": attention_prefill, "float32": attention_prefill_f32}[kind]
+        attend(q, out, kpages, vpages, block_tables, seq_first_row, seq_start_pos, max_rows_per_seq, nh, nkv, hd, page_size, scale, window, status)
 
 
 # ------------------------------------------------------------------------------------------------ scoring

@@ -6,6 +6,10 @@ position, k and v stored at the row's cache slot (all rows of the step before an
 -> per (row, head) softmax(q k^T * scale) v over the row's visible keys of its own request
 -> residual += att Wo^T. No bias anywhere. With ``writes_cache`` False the keys and values of
 this run are not stored and attention reads what the named cache layer already holds.
+
+``cache_bits`` 4: keys and values are rounded to four bits on their way into the pages, one kernel rotates and stores; decoded
+tokens read the pages as they are, portions of prompts from pages of the activation type that they are unpacked into, one
+layer's worth that all layers share.
 """
 from __future__ import annotations
 
@@ -30,6 +34,8 @@ class GqaAttention(Mixer):
             raise ValueError(f"head_dim {s.head_dim} must be even and at most 256")
         if s.window is not None and s.window <= 0:
             raise ValueError(f"window {s.window} must be positive")
+        if s.cache_bits is not None and (s.cache_bits != 4 or s.head_dim % kernels.KV4_GROUP):
+            raise ValueError(f"a cache in {s.cache_bits} bits for heads of {s.head_dim} is not built (4 bits, a multiple of {kernels.KV4_GROUP} channels)")
         self.hidden_size = hidden_size
         self.nh, self.nkv, self.hd = s.num_heads, s.num_kv_heads, s.head_dim
         self.qd, self.kvd = self.nh * self.hd, self.nkv * self.hd
@@ -46,12 +52,23 @@ class GqaAttention(Mixer):
                 "wo": ParamSpec((d, self.qd))}
 
     def cache_spec(self):
-        return PagedKvSpec(self.nkv, self.hd, self.spec.window)
+        return PagedKvSpec(self.nkv, self.hd, self.spec.window, bits=self.spec.cache_bits)
 
     def forward(self, ctx, h, residual, cache, writes_cache: bool) -> None:
         n = h.shape[0]
         qkv = ctx.scratch("qkv", (n, self.qd + 2 * self.kvd))
         table = self.position.fused_table(qkv.device)
+        if self.spec.cache_bits is not None:
+            linear(ctx, h, self.params["wqkv"], qkv)
+            if table is None:
+                self.position.apply_qk(ctx, qkv, self.nh, self.nkv, self.hd)
+            q = qkv[:, :self.qd]
+            kernels.kv4_write(qkv, q, table, ctx.positions, cache.slots, cache.k, cache.v, self.nh, self.nkv, self.hd, self.position.rotary_dim,
+                              cache.page_size, writes_cache, ctx.status)
+            att = ctx.scratch("att", (n, self.qd))
+            self._attend_4(ctx, q, att, cache)
+            linear(ctx, att, self.params["wo"], residual, accumulate=True)
+            return
         plain_rotary = (table is not None and self.position.rotary_dim == self.hd) or \
             (table is None and type(self.position).apply_qk is Position.apply_qk)
         few = _few_rows(h, self.params["wqkv"], qkv) if plain_rotary and qkv.dtype == torch.bfloat16 and self.hd in (64, 128) else None
@@ -104,6 +121,27 @@ class GqaAttention(Mixer):
                 return
         kernels.attention_rows(q, att, cache.k, cache.v, cache.block_tables, ctx.row_seq, ctx.positions, self.nh,
                                self.nkv, self.hd, cache.page_size, self.spec.scale, self.spec.window, ctx.status)
+
+    def _attend_4(self, ctx, q, att, cache) -> None:
+        """``attend`` over pages of 4 bits: the single tokens that lead a step take the decode kernel, the requests behind them the
+        prompt kernels, for which the pages in sight are unpacked first (where no such kernel takes the shape, all rows the
+        decode kernel)."""
+        n, s = q.shape[0], self.spec
+        alone = ctx.decode_only or kernels.kv4_prompt_kernel(q, att, self.nh, self.nkv, self.hd, cache.page_size) is None
+        single = n if alone else ctx.leading_single
+        if single:
+            floats = kernels.kv4_decode_plan(single, self.nh, self.nkv, self.hd, ctx.max_context, s.window, q.dtype)[2]
+            parts = ctx.scratch("kv4_parts", (1, floats), torch.float32, grow=True).view(-1) if floats else None
+            kernels.kv4_attention_decode(q[:single], att[:single], cache.k, cache.v, cache.block_tables, ctx.row_seq[:single], ctx.positions[:single],
+                                         self.nh, self.nkv, self.hd, cache.page_size, s.scale, s.window, ctx.max_context, parts, ctx.status)
+        if alone or cache.block_tables.shape[0] == single:
+            return
+        shape = (cache.k.shape[0], self.nkv, cache.page_size, self.hd)
+        count = shape[0] * shape[1] * shape[2] * shape[3]
+        kpages, vpages = (ctx.zeros_once(f"kv4_{name}{cache.group}", count, q.dtype)[:count].view(shape) for name in ("keys", "values"))
+        kernels.kv4_attention_prefill(q, att, cache.k, cache.v, cache.block_tables[single:], ctx.row_seq, ctx.positions, ctx.seq_first_row[single:],
+                                      ctx.seq_start_pos[single:], ctx.max_rows_per_seq, self.nh, self.nkv, self.hd, cache.page_size, s.scale,
+                                      s.window, ctx.max_context, kpages, vpages, ctx.status)
 
     def _attend_decode(self, ctx, q, att, cache, n: int) -> bool:
         """Rows 0 .. n-1, one per request (request i is row i); False if no decode kernel takes the shape."""

@@ -42,12 +42,14 @@ class PagedKvSpec:
     keeps only the last ``window`` tokens, and pages behind the window are given back; ``chunk`` keeps only the tokens of the
     run of ``chunk`` positions (counted from position 0) that the next token belongs to. ``value_dim`` is the size of the
     second tensor per token and head (None: ``head_dim``; 0: the mixer keeps one tensor per token, the second pool is
-    empty)."""
+    empty). ``bits`` None: numbers of the activation type; 4: bytes in the layout of ``kernels.kv4_write`` (heads of a multiple of 32
+    channels in pages of a multiple of 16 tokens)."""
     num_kv_heads: int
     head_dim: int
     window: Optional[int] = None
     value_dim: Optional[int] = None
     chunk: Optional[int] = None
+    bits: Optional[int] = None
 
 
 @dataclass(frozen=True)

@@ -370,7 +370,10 @@ def test_prompts(dtype, nh, nkv, hd, page_size, window):
     # (float32 prompts form products of exact three-term splits: a few more roundings than a fused sum, all within hd + 16)
     off = (out[:n].cpu().to(F64) - want).abs() - allowed(dtype, want, size, 2 * most, hd, 140)
     assert (off <= 0).all(), float(off.max())
-    # the pages in sight hold exactly what the codes stand for
+    # unpacked, the pages in sight hold exactly what the codes stand for
+    dev = [t.to(DEV) for t in (*pools, tables, ints[2], ints[3])]
+    kernels.kv4_expand(dev[0], dev[1], kp.zero_(), vp.zero_(), *dev[2:], max(total), window, st)
+    assert int(st) == 0
     for d, p in zip(dense, (kp, vp)):
         for i, x in enumerate(total):
             lo = max(0, past[i] + 1 - window) if window else 0
