@@ -2,15 +2,16 @@
 // bfloat16. The scheme is attention_prefill_tc.cu's (head size 64), laid out for twice the channels:
 //
 // One block = 128 consecutive query rows of one request for one query head, over tiles of 128 keys.
-//   warp 0, 10  producers of keys (and the query tile, once) and of values: a page is two boxes of 64 channels, each issued by a lane of its own,
-//               into rings of three stages (two 128-byte-swizzled column blocks a tile, 32 KB).
+//   warp 0, 18  producers of keys (and the query tile, once) and of values: a page is two boxes of 64 channels, each issued by a lane of its own,
+//               into rings of two stages (two 128-byte-swizzled column blocks a tile, 32 KB).
 //   warp 1      issues S_j = Q K_j^T (M 128, N 128, K 128) into TMEM columns 128 g, g = j & 1, and O_g += P_j V_j (M 128, N 128, K 128).
-//   warps 2-9   softmax, two groups of four warps; group g takes the key tiles of parity g with an accumulator, running maximum and row sum of its
-//               own. A thread owns a row (a TMEM lane). P_j, rounded to bfloat16, goes back over the first half of S_j's own columns: two score
-//               buffers and two accumulators of 128 columns fill the 512 that there are, so there is no room for P beside them. The
-//               tensor core works in the order of issue, so S_{j+2} may be issued into the buffer right behind the product that reads P_j.
-// What bounds it: per tile the two products are 1,024 cycles of the tensor core, the 16,384 exponentials as many of the unit that forms
-// them; the two groups keep both busy in turn.
+//   warps 2-17  softmax, two groups of eight warps; group g takes the key tiles of parity g with an accumulator, running maximum and row sum of its
+//               own. Two threads share a row (a TMEM lane), 64 keys each; they hand each other their maxima through shared memory. P_j, rounded
+//               to bfloat16, goes back over the first half of S_j's own columns: two score buffers and two accumulators of 128 columns fill
+//               the 512 that there are, so there is no room for P beside them. The tensor core works in the order of issue, so S_{j+2} is
+//               issued into the buffer right behind the product that reads P_j.
+// What bounds it: a group's chain of scores, softmax and weighted sum, each of which waits for the one before. Per tile the two products are 1,024
+// cycles of the tensor core and the 16,384 exponentials as many of the unit that forms them; the two groups keep both busy in turn.
 // The mask is applied only in tiles that cross a boundary; key tiles that no row sees are skipped. Page 0 is read in the place of pages that
 // are missing, so that P = 0 meets finite numbers (the pages are zero-initialised).
 // Every wait is bounded: a wait that runs out sets GB_STATUS_WAIT_TIMEOUT and the block winds down (waits for its own copies, frees its TMEM,
@@ -18,29 +19,29 @@
 // Measured (2,048 rows behind 2,048 tokens, 32/8 heads): mma.sync 750 us, this kernel 140.
 #include "tcgen05.cuh"
 
-constexpr int AL_HD = 128, AL_BM = 128, AL_BN = 128, AL_STAGES = 3, AL_WARPS = 11;
+constexpr int AL_HD = 128, AL_BM = 128, AL_BN = 128, AL_STAGES = 2, AL_WARPS = 19;
 constexpr int AL_BLOCK = 128 * 128;                     // bytes of 128 rows of 64 channels
 constexpr int AL_TILE = 2 * AL_BLOCK;
 constexpr int AL_K_OFF = AL_TILE, AL_V_OFF = AL_K_OFF + AL_STAGES * AL_TILE, AL_SH_OFF = AL_V_OFF + AL_STAGES * AL_TILE;
-constexpr int AL_SMEM = AL_SH_OFF + 2560;
+constexpr int AL_SMEM = AL_SH_OFF + 6144;
 constexpr int AL_O_COL = 2 * AL_BN, AL_TMEM_COLS = 512;
 constexpr float AL_NEG_BIG = -1.0e30f;
 static_assert(AL_SMEM <= 227 * 1024 && AL_O_COL + 2 * AL_HD <= AL_TMEM_COLS, "the block does not fit");
 
 struct __align__(8) AlShared {
     uint64_t q_full;
-    uint64_t k_full[AL_STAGES], k_empty[AL_STAGES];      // TMA -> MMA, MMA -> TMA
-    uint64_t v_full[AL_STAGES], v_empty[AL_STAGES];
-    uint64_t s_full[2];              // MMA -> softmax: S_j is complete in buffer j & 1
+    uint64_t k_full[AL_STAGES], v_full[AL_STAGES];       // TMA -> MMA
+    uint64_t s_full[2];              // MMA -> softmax and the keys' producer: S_j is complete in buffer j & 1
     uint64_t p_ready[2];             // softmax -> MMA: P_j is in its place (and O is rescaled)
-    uint64_t pv_done[2];             // MMA -> softmax: O += P_j V_j is complete
-    uint64_t x_ready;                // softmax <-> softmax: both groups have posted their final maximum and sum
-    float row_stat[2][2][AL_BM];     // [group][maximum, sum][row]
+    uint64_t pv_done[2];             // MMA -> softmax and the values' producer: O += P_j V_j is complete
+    uint64_t x_ready;                // softmax <-> softmax: all warps have posted their final maximum and sum
+    float pair_max[2][2][AL_BM];     // [group][half][row]: the halves' maxima of one tile
+    float row_max[2][AL_BM], row_sum[2][2][AL_BM];       // [group]([half])[row]
     uint32_t tmem_base;
     int abort_flag;
     int issued[2], consumed[2], q_issued;
 };
-static_assert(sizeof(AlShared) <= 2560, "shared memory layout");
+static_assert(sizeof(AlShared) <= 6144, "shared memory layout");
 
 // MN-major B operand (rows are keys, a head's channels contiguous) in 128-byte-swizzled rows: groups of eight keys 1024 bytes apart, column blocks
 // of 64 channels lbo bytes apart.
@@ -53,8 +54,6 @@ __device__ __forceinline__ uint64_t al_desc_mn(uint32_t smem_addr, uint32_t lbo_
     d |= (uint64_t)2 << 61;
     return d;
 }
-// Two non-negative floats to a bfloat16 pair, rounding half up, on the integer pipe: the conversion shares its pipe with ex2.
-__device__ __forceinline__ uint32_t al_pack(float lo, float hi) { return __byte_perm(__float_as_uint(lo) + 0x8000u, __float_as_uint(hi) + 0x8000u, 0x7632); }
 __device__ __forceinline__ float al_max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -64,6 +63,21 @@ __device__ __forceinline__ float al_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// Sixteen columns of this thread's TMEM lane; the caller waits for the stores.
+__device__ __forceinline__ void al_store16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+                 "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
+// The two warps of a pair meet; true in both if ok was true in all their threads.
+__device__ __forceinline__ bool al_pair_sync(int id, bool ok) {
+    uint32_t all;
+    asm volatile("{\n\t.reg .pred p, r;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.and.pred r, %2, 64, p;\n\tselp.u32 %0, 1, 0, r;\n\t}"
+                 : "=r"(all) : "r"((uint32_t)ok), "r"(id) : "memory");
+    return all != 0;
 }
 
 __global__ void __launch_bounds__(AL_WARPS * 32) attention_prefill_128_kernel(
@@ -102,16 +116,12 @@ __global__ void __launch_bounds__(AL_WARPS * 32) attention_prefill_128_kernel(
         mbar_init(&sh.q_full, 1);
         for (int b = 0; b < AL_STAGES; ++b) {
             mbar_init(&sh.k_full[b], 1);
-            mbar_init(&sh.k_empty[b], 1);
             mbar_init(&sh.v_full[b], 1);
-            mbar_init(&sh.v_empty[b], 1);
-        }
-        for (int b = 0; b < 2; ++b) {
             mbar_init(&sh.s_full[b], 1);
-            mbar_init(&sh.p_ready[b], 4);
+            mbar_init(&sh.p_ready[b], 8);
             mbar_init(&sh.pv_done[b], 1);
         }
-        mbar_init(&sh.x_ready, 8);
+        mbar_init(&sh.x_ready, 16);
         sh.abort_flag = 0;
         sh.issued[0] = sh.issued[1] = sh.consumed[0] = sh.consumed[1] = sh.q_issued = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -131,7 +141,7 @@ __global__ void __launch_bounds__(AL_WARPS * 32) attention_prefill_128_kernel(
         const int what = warp == 0 ? 0 : 1;
         const int ppt = AL_BN >> page_shift;      // pages per key tile (1 .. 16), two boxes each
         uint64_t* full = what == 0 ? sh.k_full : sh.v_full;
-        uint64_t* empty = what == 0 ? sh.k_empty : sh.v_empty;
+        uint64_t* empty = what == 0 ? sh.s_full : sh.pv_done;      // (two stages and two buffers: a stage is free when its tile's product is done)
         unsigned char* ring = what == 0 ? Ks : Vs;
         const CUtensorMap* map = what == 0 ? &map_k : &map_v;
         int bad = 0;
@@ -177,104 +187,105 @@ __global__ void __launch_bounds__(AL_WARPS * 32) attention_prefill_128_kernel(
         if (elect_one()) {
             const uint32_t idesc_qk = umma_idesc(AL_BM, AL_BN), idesc_pv = umma_idesc(AL_BM, AL_HD) | (1u << 16);   // (B of the second is MN-major)
             const uint64_t q_desc = umma_desc(smem_u32(Qs)), k_desc = umma_desc(smem_u32(Ks)), v_desc = al_desc_mn(smem_u32(Vs), AL_BLOCK);
+            // All that a step needs is waited for first; then its products are issued back to back. (A test of a barrier behind a commit
+            // does not return before the commit's products are done: 145 us with one between the two.)
             bool ok = mbar_wait(&sh.q_full, 0, abort_flag, status);
-            // Whatever is ready is issued. The loop polls without blocking; the limit counts from the first look that found nothing.
-            int next_qk = 0, next_pv = 0;
-            long long t_idle = 0;
-            while (ok && next_pv < total) {
-                bool progressed = false;
-                if (next_qk < total && next_qk < next_pv + 2) {      // (S_j takes the place of P_{j-2}, whose product has been issued)
-                    const int j = next_qk, st = j % AL_STAGES;
-                    if (mbar_test(&sh.k_full[st], (j / AL_STAGES) & 1)) {
-                        tc_fence_after();
-                        const uint64_t kd = k_desc + (uint64_t)((st * AL_TILE) >> 4);
+            int seen_k = 0, seen_v = 0;
+            auto scores = [&](int j) {
+                const uint64_t kd = k_desc + (uint64_t)(((j & 1) * AL_TILE) >> 4);
 #pragma unroll
-                        for (int k = 0; k < AL_HD / 16; ++k) {
-                            const uint64_t at = (uint64_t)((k / 4) * (AL_BLOCK >> 4) + (k % 4) * 2);
-                            umma_bf16(tmem + (uint32_t)((j & 1) * AL_BN), q_desc + at, kd + at, idesc_qk, k ? 1u : 0u);
-                        }
-                        umma_commit(&sh.s_full[j & 1]);
-                        umma_commit(&sh.k_empty[st]);
-                        ++next_qk;
-                        progressed = true;
-                    }
+                for (int k = 0; k < AL_HD / 16; ++k) {
+                    const uint64_t at = (uint64_t)((k / 4) * (AL_BLOCK >> 4) + (k % 4) * 2);
+                    umma_bf16(tmem + (uint32_t)((j & 1) * AL_BN), q_desc + at, kd + at, idesc_qk, k ? 1u : 0u);
                 }
-                if (next_pv < next_qk) {
-                    const int j = next_pv, st = j % AL_STAGES;
-                    if (mbar_test(&sh.p_ready[j & 1], (j >> 1) & 1) && mbar_test(&sh.v_full[st], (j / AL_STAGES) & 1)) {
-                        tc_fence_after();
-                        const uint64_t vd = v_desc + (uint64_t)((st * AL_TILE) >> 4);
-                        const uint32_t pt = tmem + (uint32_t)((j & 1) * AL_BN);
-#pragma unroll
-                        for (int kk = 0; kk < AL_BN / 16; ++kk)      // 16 keys per instruction: 8 columns of P
-                            umma_bf16_ts(tmem + (uint32_t)(AL_O_COL + (j & 1) * AL_HD), pt + (uint32_t)(kk * 8), vd + (uint64_t)(kk * 16 * 128 >> 4), idesc_pv,
-                                         (j >= 2 || kk) ? 1u : 0u);
-                        umma_commit(&sh.pv_done[j & 1]);
-                        umma_commit(&sh.v_empty[st]);
-                        ++next_pv;
-                        progressed = true;
-                    }
-                }
-                if (progressed) {
-                    t_idle = 0;
-                } else if (*abort_flag) {
-                    ok = false;
-                } else if (t_idle == 0) {
-                    t_idle = clock64();
-                } else if (clock64() - t_idle > TC_WAIT_CYCLES) {
-                    *abort_flag = 1;
-                    atomicOr(status, GB_STATUS_WAIT_TIMEOUT);
-                    ok = false;
-                }
+                umma_commit(&sh.s_full[j & 1]);
+            };
+            for (int j = 0; ok && j < min(total, 2); ++j) {
+                ok = mbar_wait(&sh.k_full[j], 0, abort_flag, status);
+                if (!ok) break;
+                seen_k = j + 1;
+                tc_fence_after();
+                scores(j);
             }
-            sh.consumed[0] = next_qk;
-            sh.consumed[1] = next_pv;
+            for (int j = 0; ok && j < total; ++j) {
+                if (j + 2 < total) {
+                    ok = mbar_wait(&sh.k_full[j & 1], ((j >> 1) + 1) & 1, abort_flag, status);
+                    if (!ok) break;
+                    seen_k = j + 3;
+                }
+                ok = mbar_wait(&sh.v_full[j & 1], (j >> 1) & 1, abort_flag, status);
+                if (!ok) break;
+                seen_v = j + 1;
+                ok = mbar_wait(&sh.p_ready[j & 1], (j >> 1) & 1, abort_flag, status);
+                if (!ok) break;
+                tc_fence_after();
+                const uint64_t vd = v_desc + (uint64_t)(((j & 1) * AL_TILE) >> 4);
+                const uint32_t pt = tmem + (uint32_t)((j & 1) * AL_BN);
+#pragma unroll
+                for (int kk = 0; kk < AL_BN / 16; ++kk)      // 16 keys per instruction: 8 columns of P
+                    umma_bf16_ts(tmem + (uint32_t)(AL_O_COL + (j & 1) * AL_HD), pt + (uint32_t)(kk * 8), vd + (uint64_t)(kk * 16 * 128 >> 4), idesc_pv,
+                                 (j >= 2 || kk) ? 1u : 0u);
+                umma_commit(&sh.pv_done[j & 1]);
+                if (j + 2 < total) scores(j + 2);      // (S_{j+2} takes the place of P_j)
+            }
+            sh.consumed[0] = seen_k;
+            sh.consumed[1] = seen_v;
         }
     } else {
         // ------------------------------------------------------------------------- softmax
         const int q = warp & 3;                        // the quarter of TMEM lanes this warp may read
-        const int g = (warp - 2) >> 2;                 // the group: parity of its key tiles
+        const int g = (warp - 2) >> 3;                 // the group: parity of its key tiles
+        const int half = ((warp - 2) >> 2) & 1;        // the half of a tile's keys, and of the accumulator's channels
         const int r = q * 32 + lane;                   // this thread's query row within the tile
         const float sl2 = scale * 1.4426950408889634f;
-        const uint32_t lane_base = tmem + ((uint32_t)(q * 32) << 16), s_col = (uint32_t)(g * AL_BN), o_col = (uint32_t)(AL_O_COL + g * AL_HD);
+        const uint32_t lane_base = tmem + ((uint32_t)(q * 32) << 16), s_col = (uint32_t)(g * AL_BN), o_col = (uint32_t)(AL_O_COL + g * AL_HD + half * 64);
         const int pos = pos_lo + r, first = gb_first_key(pos, window), first_last = gb_first_key(pos_lo + AL_BM - 1, window);
         float m_run = AL_NEG_BIG, l_run = 0.f;
         bool ok = true;
         for (int j = g; j < total; j += 2) {
-            const int i = j >> 1, key0 = (kt_begin + j) * AL_BN;
-            if (!mbar_wait_warp(&sh.s_full[g], i & 1, abort_flag, status)) { ok = false; break; }
-            tc_fence_after();
-            uint32_t sv[AL_BN];
-            tmem_load128(lane_base + s_col, sv);
-            if (key0 + AL_BN - 1 > pos_lo || key0 < first_last) {
+            const int i = j >> 1, key0 = (kt_begin + j) * AL_BN + half * 64;
+            ok = ok && mbar_wait_warp(&sh.s_full[g], i & 1, abort_flag, status);
+            uint32_t sv[64];
+            float mx = AL_NEG_BIG;
+            if (ok) {
+                tc_fence_after();
+                tmem_load64(lane_base + s_col + (uint32_t)(half * 64), sv);
+                if (key0 + 63 > pos_lo || key0 < first_last) {
 #pragma unroll
-                for (int k = 0; k < AL_BN; ++k)
-                    if (key0 + k > pos || key0 + k < first) sv[k] = __float_as_uint(AL_NEG_BIG);
+                    for (int k = 0; k < 64; ++k)
+                        if (key0 + k > pos || key0 + k < first) sv[k] = __float_as_uint(AL_NEG_BIG);
+                }
+                float mx4[4] = {AL_NEG_BIG, AL_NEG_BIG, AL_NEG_BIG, AL_NEG_BIG};
+#pragma unroll
+                for (int k = 0; k < 64; k += 8)
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) mx4[u] = al_max3(mx4[u], __uint_as_float(sv[k + 2 * u]), __uint_as_float(sv[k + 2 * u + 1]));
+                mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+                sh.pair_max[g][half][r] = mx;
             }
-            float mx4[4] = {AL_NEG_BIG, AL_NEG_BIG, AL_NEG_BIG, AL_NEG_BIG};
-#pragma unroll
-            for (int k = 0; k < AL_BN; k += 8)
-#pragma unroll
-                for (int u = 0; u < 4; ++u) mx4[u] = al_max3(mx4[u], __uint_as_float(sv[k + 2 * u]), __uint_as_float(sv[k + 2 * u + 1]));
-            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-            // O_g += P V of the group's previous tile is complete before O_g is rescaled (S_j was issued behind it)
-            if (i > 0 && !mbar_wait_warp(&sh.pv_done[g], (i - 1) & 1, abort_flag, status)) { ok = false; break; }
+            // Both halves of the scores have been read behind this (P is stored over them), and both maxima are there. A wait that ran out
+            // ends the pair together.
+            ok = al_pair_sync(1 + g * 4 + q, ok);
+            if (!ok) break;
+            mx = fmaxf(mx, sh.pair_max[g][half ^ 1][r]);
             // the running maximum rises, and O_g is rescaled, only when it is exceeded by more than 2^8 in the exponent
             const bool raise = (mx - m_run) * sl2 > 8.0f;
             if (i == 0) {
                 if (raise) m_run = mx;
-            } else if (__any_sync(0xffffffffu, raise)) {
+            } else if (__any_sync(0xffffffffu, raise)) {      // (the same rows and maxima in both warps)
+                // O_g += P V of the group's previous tile is complete (S_j was issued behind it)
+                ok = mbar_wait_warp(&sh.pv_done[g], (i - 1) & 1, abort_flag, status);
                 tc_fence_after();
                 const float corr = raise ? al_exp2((m_run - mx) * sl2) : 1.0f;
                 if (raise) m_run = mx;
                 l_run *= corr;
 #pragma unroll
-                for (int c = 0; c < AL_HD; c += 32) {
-                    uint32_t ov[32];
-                    tmem_load32(lane_base + o_col + (uint32_t)c, ov);
+                for (int c = 0; c < 64; c += 16) {
+                    uint32_t ov[16];
+                    tmem_load16(lane_base + o_col + (uint32_t)c, ov);
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) ov[k] = __float_as_uint(__uint_as_float(ov[k]) * corr);
-                    tmem_store32(lane_base + o_col + (uint32_t)c, ov);
+                    for (int k = 0; k < 16; ++k) ov[k] = __float_as_uint(__uint_as_float(ov[k]) * corr);
+                    al_store16(lane_base + o_col + (uint32_t)c, ov);
                 }
             }
             // P = exp2(S sl2 - m sl2). A masked key holds -1e30 and comes out as exactly 0; a row that has seen no key yet (its maximum is still
@@ -282,25 +293,29 @@ __global__ void __launch_bounds__(AL_WARPS * 32) attention_prefill_128_kernel(
             const float msl = m_run <= AL_NEG_BIG ? 0.f : m_run * sl2;
             const float2 scale2 = make_float2(sl2, sl2), off2 = make_float2(-msl, -msl);
             float2 l2[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-            uint32_t pw[AL_BN / 2];
 #pragma unroll
-            for (int c = 0; c < AL_BN; c += 2) {
-                const float2 y = __ffma2_rn(make_float2(__uint_as_float(sv[c]), __uint_as_float(sv[c + 1])), scale2, off2);
-                const float2 p = make_float2(al_exp2(y.x), al_exp2(y.y));
-                l2[(c >> 1) & 3] = __fadd2_rn(l2[(c >> 1) & 3], p);
-                pw[c >> 1] = al_pack(p.x, p.y);
+            for (int part = 0; part < 64; part += 32) {
+                uint32_t pw[16];
+#pragma unroll
+                for (int c = 0; c < 32; c += 2) {
+                    const float2 y = __ffma2_rn(make_float2(__uint_as_float(sv[part + c]), __uint_as_float(sv[part + c + 1])), scale2, off2);
+                    const float2 p = make_float2(al_exp2(y.x), al_exp2(y.y));
+                    l2[(c >> 1) & 3] = __fadd2_rn(l2[(c >> 1) & 3], p);
+                    pw[c >> 1] = pack2(__float_as_uint(p.x), __float_as_uint(p.y));
+                }
+                al_store16(lane_base + s_col + (uint32_t)(half * 32 + part / 2), pw);
             }
             const float2 lsum = __fadd2_rn(__fadd2_rn(l2[0], l2[1]), __fadd2_rn(l2[2], l2[3]));
             l_run += lsum.x + lsum.y;
-            tmem_store64(lane_base + s_col, pw);
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.p_ready[g]);
         }
-        // merge: the groups post their maximum and sum per row, then each writes half of the channels
+        // merge: the warps post their maximum and sum per row, then each writes a quarter of the channels
         if (ok) {
-            sh.row_stat[g][0][r] = m_run;
-            sh.row_stat[g][1][r] = l_run;
+            sh.row_max[g][r] = m_run;                  // (the same in both halves)
+            sh.row_sum[g][half][r] = l_run;
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.x_ready);
             ok = mbar_wait_warp(&sh.x_ready, 0, abort_flag, status);
@@ -311,34 +326,32 @@ __global__ void __launch_bounds__(AL_WARPS * 32) attention_prefill_128_kernel(
         }
         if (ok) {
             tc_fence_after();
-            const float m0 = sh.row_stat[0][0][r], l0 = sh.row_stat[0][1][r], m1 = sh.row_stat[1][0][r], l1 = sh.row_stat[1][1][r];
-            const float m = fmaxf(m0, m1);
+            const float m0 = sh.row_max[0][r], m1 = sh.row_max[1][r], m = fmaxf(m0, m1);
+            const float l0 = sh.row_sum[0][0][r] + sh.row_sum[0][1][r], l1 = sh.row_sum[1][0][r] + sh.row_sum[1][1][r];
             const bool two = total > 1;                // (a group without tiles has never written its accumulator: it is not read)
             const float a0 = al_exp2((m0 - m) * sl2), a1 = two ? al_exp2((m1 - m) * sl2) : 0.f;
             const float l = two ? l0 * a0 + l1 * a1 : l0 * a0, inv = l != 0.f ? 1.0f / l : 0.f;
-            __nv_bfloat16* dst = out + (size_t)(row0 + q_lo + r) * out_stride + (size_t)head * AL_HD + g * 64;
+            const int c = g * 64 + half * 32;
+            float o[32];
+            uint32_t ov[32];
+            tmem_load32(lane_base + (uint32_t)(AL_O_COL + c), ov);
 #pragma unroll
-            for (int c = 0; c < 64; c += 32) {
-                float o[32];
-                uint32_t ov[32];
-                tmem_load32(lane_base + (uint32_t)(AL_O_COL + g * 64 + c), ov);
+            for (int k = 0; k < 32; ++k) o[k] = __uint_as_float(ov[k]) * a0;
+            if (two) {
+                tmem_load32(lane_base + (uint32_t)(AL_O_COL + AL_HD + c), ov);
 #pragma unroll
-                for (int k = 0; k < 32; ++k) o[k] = __uint_as_float(ov[k]) * a0;
-                if (two) {
-                    tmem_load32(lane_base + (uint32_t)(AL_O_COL + AL_HD + g * 64 + c), ov);
+                for (int k = 0; k < 32; ++k) o[k] = fmaf(__uint_as_float(ov[k]), a1, o[k]);
+            }
+            if (q_lo + r < nrows) {
+                __nv_bfloat16* dst = out + (size_t)(row0 + q_lo + r) * out_stride + (size_t)head * AL_HD + c;
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) o[k] = fmaf(__uint_as_float(ov[k]), a1, o[k]);
-                }
-                if (q_lo + r < nrows) {
-#pragma unroll
-                    for (int k = 0; k < 32; k += 8) {
-                        uint4 w;
-                        w.x = pack2(__float_as_uint(o[k] * inv), __float_as_uint(o[k + 1] * inv));
-                        w.y = pack2(__float_as_uint(o[k + 2] * inv), __float_as_uint(o[k + 3] * inv));
-                        w.z = pack2(__float_as_uint(o[k + 4] * inv), __float_as_uint(o[k + 5] * inv));
-                        w.w = pack2(__float_as_uint(o[k + 6] * inv), __float_as_uint(o[k + 7] * inv));
-                        *reinterpret_cast<uint4*>(dst + c + k) = w;
-                    }
+                for (int k = 0; k < 32; k += 8) {
+                    uint4 w;
+                    w.x = pack2(__float_as_uint(o[k] * inv), __float_as_uint(o[k + 1] * inv));
+                    w.y = pack2(__float_as_uint(o[k + 2] * inv), __float_as_uint(o[k + 3] * inv));
+                    w.z = pack2(__float_as_uint(o[k + 4] * inv), __float_as_uint(o[k + 5] * inv));
+                    w.w = pack2(__float_as_uint(o[k + 6] * inv), __float_as_uint(o[k + 7] * inv));
+                    *reinterpret_cast<uint4*>(dst + k) = w;
                 }
             }
         }
