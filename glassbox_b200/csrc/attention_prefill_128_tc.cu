@@ -1,17 +1,20 @@
 // Causal grouped-query flash attention for prompt portions at head size 128 on the 5th-generation tensor cores (sm_100a), over pages of
 // bfloat16. The scheme is attention_prefill_tc.cu's (head size 64), laid out for twice the channels:
 //
-// One block = 128 consecutive query rows of one request for one query head, over tiles of 128 keys.
-//   warp 0, 18  producers of keys (and the query tile, once) and of values: a page is two boxes of 64 channels, each issued by a lane of its own,
-//               into rings of two stages (two 128-byte-swizzled column blocks a tile, 32 KB).
-//   warp 1      issues S_j = Q K_j^T (M 128, N 128, K 128) into TMEM columns 128 g, g = j & 1, and O_g += P_j V_j (M 128, N 128, K 128).
-//   warps 2-17  softmax, two groups of eight warps; group g takes the key tiles of parity g with an accumulator, running maximum and row sum of its
-//               own. Two threads share a row (a TMEM lane), 64 keys each; they hand each other their maxima through shared memory. P_j, rounded
-//               to bfloat16, goes back over the first half of S_j's own columns: two score buffers and two accumulators of 128 columns fill
-//               the 512 that there are, so there is no room for P beside them. The tensor core works in the order of issue, so S_{j+2} is
-//               issued into the buffer right behind the product that reads P_j.
-// What bounds it: a group's chain of scores, softmax and weighted sum, each of which waits for the one before. Per tile the two products are 1,024
-// cycles of the tensor core and the 16,384 exponentials as many of the unit that forms them; the two groups keep both busy in turn.
+// One block = two units that share a head of keys and values, over tiles of 128 keys; a unit is 128 consecutive query rows of one request for one
+// query head. (Units of a key/value head are counted over its query heads first, then over the rows, so that a pair covers nearly the same keys: at an
+// odd number of query heads a key/value head some pairs straddle two row tiles, and run over the union of what the two need.)
+//   warp 0, 10  producers of keys (and the query tiles, once) and of values: a page is two boxes of 64 channels, each issued by a lane of its own,
+//               into rings of three and two stages (two 128-byte-swizzled column blocks a tile, 32 KB).
+//   warp 1      issues S_gj = Q_g K_j^T (M 128, N 128, K 128) into TMEM columns 128 g and O_g += P_gj V_j (M 128, N 128, K 128), unit g = 0, 1.
+//   warps 2-9   softmax, four warps a unit. A thread owns a row (a TMEM lane). P, rounded to bfloat16, goes back over the first half of S's own
+//               columns: two score buffers and two accumulators of 128 columns fill the 512 that there are, so there is no room for P beside
+//               them. The tensor core works in the order of issue, so the unit's next scores are issued right behind the product that reads P;
+//               that product starts on the first 96 keys' weights while the last 32 are formed.
+// What bounds it: a unit's chain of scores, softmax and weighted sum, each of which waits for the one before. Per unit and tile the two products are
+// 1,024 cycles of the tensor core and the 16,384 exponentials as many of the unit that forms them; the two units keep both busy in turn. One
+// unit a block (its key tiles in two interleaved chains) took 128 us of the case below where this takes 105: a tile of keys and values is 64 KB,
+// and 148 blocks at one in 1,024 cycles each want more than the L2 cache hands out.
 // The mask is applied only in tiles that cross a boundary; key tiles that no row sees are skipped. Page 0 is read in the place of pages that
 // are missing, so that P = 0 meets finite numbers (the pages are zero-initialised).
 // Every wait is bounded: a wait that runs out sets GB_STATUS_WAIT_TIMEOUT and the block winds down (waits for its own copies, frees its TMEM,
@@ -19,29 +22,26 @@
 // Measured (2,048 rows behind 2,048 tokens, 32/8 heads): mma.sync 750 us, this kernel 140.
 #include "tcgen05.cuh"
 
-constexpr int AL_HD = 128, AL_BM = 128, AL_BN = 128, AL_STAGES = 2, AL_WARPS = 19;
+constexpr int AL_HD = 128, AL_BM = 128, AL_BN = 128, AL_KSTAGES = 3, AL_VSTAGES = 2, AL_WARPS = 11;
 constexpr int AL_BLOCK = 128 * 128;                     // bytes of 128 rows of 64 channels
 constexpr int AL_TILE = 2 * AL_BLOCK;
-constexpr int AL_K_OFF = AL_TILE, AL_V_OFF = AL_K_OFF + AL_STAGES * AL_TILE, AL_SH_OFF = AL_V_OFF + AL_STAGES * AL_TILE;
-constexpr int AL_SMEM = AL_SH_OFF + 6144;
+constexpr int AL_K_OFF = 2 * AL_TILE, AL_V_OFF = AL_K_OFF + AL_KSTAGES * AL_TILE, AL_SH_OFF = AL_V_OFF + AL_VSTAGES * AL_TILE;
+constexpr int AL_SMEM = AL_SH_OFF + 512;
 constexpr int AL_O_COL = 2 * AL_BN, AL_TMEM_COLS = 512;
 constexpr float AL_NEG_BIG = -1.0e30f;
 static_assert(AL_SMEM <= 227 * 1024 && AL_O_COL + 2 * AL_HD <= AL_TMEM_COLS, "the block does not fit");
 
 struct __align__(8) AlShared {
     uint64_t q_full;
-    uint64_t k_full[AL_STAGES], v_full[AL_STAGES];       // TMA -> MMA
-    uint64_t s_full[2];              // MMA -> softmax and the keys' producer: S_j is complete in buffer j & 1
-    uint64_t p_ready[2];             // softmax -> MMA: P_j is in its place (and O is rescaled)
-    uint64_t pv_done[2];             // MMA -> softmax and the values' producer: O += P_j V_j is complete
-    uint64_t x_ready;                // softmax <-> softmax: all warps have posted their final maximum and sum
-    float pair_max[2][2][AL_BM];     // [group][half][row]: the halves' maxima of one tile
-    float row_max[2][AL_BM], row_sum[2][2][AL_BM];       // [group]([half])[row]
+    uint64_t k_full[AL_KSTAGES], v_full[AL_VSTAGES];     // TMA -> MMA
+    uint64_t s_full[2][AL_KSTAGES];  // MMA -> softmax and the keys' producer: the unit's scores of a tile are complete (by the keys' stage)
+    uint64_t p_most[2], p_ready[2];  // softmax -> MMA: three quarters of the unit's P are in their place (and O is rescaled), all of it
+    uint64_t pv_done[2][AL_VSTAGES]; // MMA -> softmax and the values' producer: O += P V is complete (by the values' stage)
     uint32_t tmem_base;
     int abort_flag;
     int issued[2], consumed[2], q_issued;
 };
-static_assert(sizeof(AlShared) <= 6144, "shared memory layout");
+static_assert(sizeof(AlShared) <= 512, "shared memory layout");
 
 // MN-major B operand (rows are keys, a head's channels contiguous) in 128-byte-swizzled rows: groups of eight keys 1024 bytes apart, column blocks
 // of 64 channels lbo bytes apart.
@@ -65,19 +65,12 @@ __device__ __forceinline__ float al_exp2(float x) {
     return y;
 }
 
-// Sixteen columns of this thread's TMEM lane; the caller waits for the stores.
+// 16 of a thread's weights, rounded to bfloat16, to eight columns of its TMEM lane; the caller waits for the stores.
 __device__ __forceinline__ void al_store16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
                  "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
                  "r"(r[14]), "r"(r[15])
                  : "memory");
-}
-// The two warps of a pair meet; true in both if ok was true in all their threads.
-__device__ __forceinline__ bool al_pair_sync(int id, bool ok) {
-    uint32_t all;
-    asm volatile("{\n\t.reg .pred p, r;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.and.pred r, %2, 64, p;\n\tselp.u32 %0, 1, 0, r;\n\t}"
-                 : "=r"(all) : "r"((uint32_t)ok), "r"(id) : "memory");
-    return all != 0;
 }
 
 __global__ void __launch_bounds__(AL_WARPS * 32) attention_prefill_128_kernel(
@@ -93,35 +86,38 @@ __global__ void __launch_bounds__(AL_WARPS * 32) attention_prefill_128_kernel(
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     gb_pdl_wait();
     gb_pdl_launch_dependents();
-    const int head = blockIdx.x, seq = blockIdx.y, qt = (int)gridDim.z - 1 - (int)blockIdx.z;      // (the longest blocks start first)
-    const int row0 = seq_first_row[seq], nrows = seq_first_row[seq + 1] - row0, q_lo = qt * AL_BM;
-    if (q_lo >= nrows) return;                    // uniform for the block, before anything is allocated
+    const int kvh = blockIdx.x, seq = blockIdx.y, group = nh / nkv, u0 = 2 * ((int)gridDim.z - 1 - (int)blockIdx.z);      // (the longest blocks start first)
+    const int row0 = seq_first_row[seq], nrows = seq_first_row[seq + 1] - row0;
+    const int q_lo0 = u0 / group * AL_BM, q_lo1 = (u0 + 1) / group * AL_BM;
+    if (q_lo0 >= nrows) return;                   // uniform for the block, before anything is allocated
+    const int units = q_lo1 < nrows ? 2 : 1;
     if (smem_u32(al_smem) & 1023u) {              // swizzled tiles want 1024-byte alignment: refuse rather than compute nonsense
         if (tid == 0) atomicOr(status, GB_STATUS_WAIT_TIMEOUT);
         return;
     }
     const int start_pos = seq_start_pos[seq];
     if (start_pos < 0) {                          // a padding request: its rows read as zeros downstream
-        const int rows = min(AL_BM, nrows - q_lo);
-        for (int i = tid; i < rows * (AL_HD / 8); i += blockDim.x)
-            *reinterpret_cast<uint4*>(out + (size_t)(row0 + q_lo + i / (AL_HD / 8)) * out_stride + (size_t)head * AL_HD + i % (AL_HD / 8) * 8) = make_uint4(0, 0, 0, 0);
+        for (int g = 0; g < units; ++g) {
+            const int lo = g ? q_lo1 : q_lo0, rows = min(AL_BM, nrows - lo), head = kvh * group + (u0 + g) % group;
+            for (int i = tid; i < rows * (AL_HD / 8); i += blockDim.x)
+                *reinterpret_cast<uint4*>(out + (size_t)(row0 + lo + i / (AL_HD / 8)) * out_stride + (size_t)head * AL_HD + i % (AL_HD / 8) * 8) = make_uint4(0, 0, 0, 0);
+        }
         return;
     }
-    const int kvh = head / (nh / nkv);
     const int* table = block_tables + (size_t)seq * max_pages;
-    const int pos_lo = start_pos + q_lo, pos_hi = start_pos + min(nrows, q_lo + AL_BM) - 1;
-    const int key_lo = gb_first_key(pos_lo, window), kt_begin = key_lo / AL_BN, total = pos_hi / AL_BN - kt_begin + 1;
+    const int pos_hi = start_pos + min(nrows, (units == 2 ? q_lo1 : q_lo0) + AL_BM) - 1;
+    const int key_lo = gb_first_key(start_pos + q_lo0, window), kt_begin = key_lo / AL_BN, total = pos_hi / AL_BN - kt_begin + 1;
 
     if (tid == 0) {
         mbar_init(&sh.q_full, 1);
-        for (int b = 0; b < AL_STAGES; ++b) {
-            mbar_init(&sh.k_full[b], 1);
-            mbar_init(&sh.v_full[b], 1);
-            mbar_init(&sh.s_full[b], 1);
-            mbar_init(&sh.p_ready[b], 8);
-            mbar_init(&sh.pv_done[b], 1);
+        for (int b = 0; b < AL_KSTAGES; ++b) mbar_init(&sh.k_full[b], 1);
+        for (int b = 0; b < AL_VSTAGES; ++b) mbar_init(&sh.v_full[b], 1);
+        for (int g = 0; g < 2; ++g) {
+            for (int b = 0; b < AL_KSTAGES; ++b) mbar_init(&sh.s_full[g][b], 1);
+            for (int b = 0; b < AL_VSTAGES; ++b) mbar_init(&sh.pv_done[g][b], 1);
+            mbar_init(&sh.p_most[g], 4);
+            mbar_init(&sh.p_ready[g], 4);
         }
-        mbar_init(&sh.x_ready, 16);
         sh.abort_flag = 0;
         sh.issued[0] = sh.issued[1] = sh.consumed[0] = sh.consumed[1] = sh.q_issued = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -141,14 +137,16 @@ __global__ void __launch_bounds__(AL_WARPS * 32) attention_prefill_128_kernel(
         const int what = warp == 0 ? 0 : 1;
         const int ppt = AL_BN >> page_shift;      // pages per key tile (1 .. 16), two boxes each
         uint64_t* full = what == 0 ? sh.k_full : sh.v_full;
-        uint64_t* empty = what == 0 ? sh.s_full : sh.pv_done;      // (two stages and two buffers: a stage is free when its tile's product is done)
         unsigned char* ring = what == 0 ? Ks : Vs;
         const CUtensorMap* map = what == 0 ? &map_k : &map_v;
         int bad = 0;
         if (what == 0 && lane == 0) {
-            mbar_expect_tx(&sh.q_full, AL_TILE);
-            tma_load_2d(Qs, &map_q, &sh.q_full, head * AL_HD, row0 + q_lo);
-            tma_load_2d(Qs + AL_BLOCK, &map_q, &sh.q_full, head * AL_HD + 64, row0 + q_lo);
+            mbar_expect_tx(&sh.q_full, units * AL_TILE);
+            for (int g = 0; g < units; ++g) {
+                const int head = kvh * group + (u0 + g) % group, row = row0 + (g ? q_lo1 : q_lo0);
+                tma_load_2d(Qs + g * AL_TILE, &map_q, &sh.q_full, head * AL_HD, row);
+                tma_load_2d(Qs + g * AL_TILE + AL_BLOCK, &map_q, &sh.q_full, head * AL_HD + 64, row);
+            }
             sh.q_issued = 1;
         }
         auto page_of = [&](int kt) -> long long {      // this lane's page of key tile kt: lanes 2 i and 2 i + 1 have page i
@@ -166,10 +164,13 @@ __global__ void __launch_bounds__(AL_WARPS * 32) attention_prefill_128_kernel(
         };
         long long page = page_of(kt_begin);
         for (int j = 0; j < total; ++j) {
-            const int s = j % AL_STAGES;
+            const int s = what == 0 ? j % AL_KSTAGES : j % AL_VSTAGES;
             const long long next_page = j + 1 < total ? page_of(kt_begin + j + 1) : 0;      // in flight during the wait
             int ok = 1;
-            if (lane == 0 && j >= AL_STAGES) ok = mbar_wait(&empty[s], ((j / AL_STAGES) - 1) & 1, abort_flag, status) ? 1 : 0;
+            if (lane == 0) {      // a stage is free when the last product of the tile that was in it is done
+                if (what == 0 && j >= AL_KSTAGES) ok = mbar_wait(&sh.s_full[units - 1][s], (j / AL_KSTAGES - 1) & 1, abort_flag, status) ? 1 : 0;
+                if (what == 1 && j >= AL_VSTAGES) ok = mbar_wait(&sh.pv_done[units - 1][s], (j / AL_VSTAGES - 1) & 1, abort_flag, status) ? 1 : 0;
+            }
             ok = __shfl_sync(0xffffffffu, ok, 0);
             if (!ok) break;
             if (lane == 0) mbar_expect_tx(&full[s], AL_TILE);
@@ -187,100 +188,97 @@ __global__ void __launch_bounds__(AL_WARPS * 32) attention_prefill_128_kernel(
         if (elect_one()) {
             const uint32_t idesc_qk = umma_idesc(AL_BM, AL_BN), idesc_pv = umma_idesc(AL_BM, AL_HD) | (1u << 16);   // (B of the second is MN-major)
             const uint64_t q_desc = umma_desc(smem_u32(Qs)), k_desc = umma_desc(smem_u32(Ks)), v_desc = al_desc_mn(smem_u32(Vs), AL_BLOCK);
-            // All that a step needs is waited for first; then its products are issued back to back. (A test of a barrier behind a commit
-            // does not return before the commit's products are done: 145 us with one between the two.)
+            // What a step needs is waited for first; then the last of its weighted sum and the next scores are issued back to back.
             bool ok = mbar_wait(&sh.q_full, 0, abort_flag, status);
             int seen_k = 0, seen_v = 0;
-            auto scores = [&](int j) {
-                const uint64_t kd = k_desc + (uint64_t)(((j & 1) * AL_TILE) >> 4);
+            auto scores = [&](int g, int j) {
+                const uint64_t qd = q_desc + (uint64_t)((g * AL_TILE) >> 4), kd = k_desc + (uint64_t)(((j % AL_KSTAGES) * AL_TILE) >> 4);
 #pragma unroll
                 for (int k = 0; k < AL_HD / 16; ++k) {
                     const uint64_t at = (uint64_t)((k / 4) * (AL_BLOCK >> 4) + (k % 4) * 2);
-                    umma_bf16(tmem + (uint32_t)((j & 1) * AL_BN), q_desc + at, kd + at, idesc_qk, k ? 1u : 0u);
+                    umma_bf16(tmem + (uint32_t)(g * AL_BN), qd + at, kd + at, idesc_qk, k ? 1u : 0u);
                 }
-                umma_commit(&sh.s_full[j & 1]);
+                umma_commit(&sh.s_full[g][j % AL_KSTAGES]);
             };
-            for (int j = 0; ok && j < min(total, 2); ++j) {
-                ok = mbar_wait(&sh.k_full[j], 0, abort_flag, status);
-                if (!ok) break;
+            auto keys = [&](int j) {
+                if (!mbar_wait(&sh.k_full[j % AL_KSTAGES], (j / AL_KSTAGES) & 1, abort_flag, status)) return false;
                 seen_k = j + 1;
+                return true;
+            };
+            if (ok) ok = keys(0);
+            if (ok) {
                 tc_fence_after();
-                scores(j);
+                for (int g = 0; g < units; ++g) scores(g, 0);
             }
             for (int j = 0; ok && j < total; ++j) {
-                if (j + 2 < total) {
-                    ok = mbar_wait(&sh.k_full[j & 1], ((j >> 1) + 1) & 1, abort_flag, status);
-                    if (!ok) break;
-                    seen_k = j + 3;
-                }
-                ok = mbar_wait(&sh.v_full[j & 1], (j >> 1) & 1, abort_flag, status);
+                if (j + 1 < total) ok = keys(j + 1);
+                if (ok) ok = mbar_wait(&sh.v_full[j % AL_VSTAGES], (j / AL_VSTAGES) & 1, abort_flag, status);
                 if (!ok) break;
                 seen_v = j + 1;
-                ok = mbar_wait(&sh.p_ready[j & 1], (j >> 1) & 1, abort_flag, status);
-                if (!ok) break;
-                tc_fence_after();
-                const uint64_t vd = v_desc + (uint64_t)(((j & 1) * AL_TILE) >> 4);
-                const uint32_t pt = tmem + (uint32_t)((j & 1) * AL_BN);
+                const uint64_t vd = v_desc + (uint64_t)(((j % AL_VSTAGES) * AL_TILE) >> 4);
+                for (int g = 0; g < units; ++g) {
+                    const uint32_t pt = tmem + (uint32_t)(g * AL_BN), ot = tmem + (uint32_t)(AL_O_COL + g * AL_HD);
+                    ok = mbar_wait(&sh.p_most[g], j & 1, abort_flag, status);
+                    if (!ok) break;
+                    tc_fence_after();
 #pragma unroll
-                for (int kk = 0; kk < AL_BN / 16; ++kk)      // 16 keys per instruction: 8 columns of P
-                    umma_bf16_ts(tmem + (uint32_t)(AL_O_COL + (j & 1) * AL_HD), pt + (uint32_t)(kk * 8), vd + (uint64_t)(kk * 16 * 128 >> 4), idesc_pv,
-                                 (j >= 2 || kk) ? 1u : 0u);
-                umma_commit(&sh.pv_done[j & 1]);
-                if (j + 2 < total) scores(j + 2);      // (S_{j+2} takes the place of P_j)
+                    for (int kk = 0; kk < 6; ++kk)      // 16 keys per instruction: 8 columns of P
+                        umma_bf16_ts(ot, pt + (uint32_t)(kk * 8), vd + (uint64_t)(kk * 16 * 128 >> 4), idesc_pv, (j || kk) ? 1u : 0u);
+                    ok = mbar_wait(&sh.p_ready[g], j & 1, abort_flag, status);
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int kk = 6; kk < 8; ++kk) umma_bf16_ts(ot, pt + (uint32_t)(kk * 8), vd + (uint64_t)(kk * 16 * 128 >> 4), idesc_pv, 1u);
+                    umma_commit(&sh.pv_done[g][j % AL_VSTAGES]);
+                    if (j + 1 < total) scores(g, j + 1);      // (over the unit's P, which the product just issued reads before)
+                }
             }
             sh.consumed[0] = seen_k;
             sh.consumed[1] = seen_v;
         }
-    } else {
+    } else if ((warp - 2) >> 2 < units) {
         // ------------------------------------------------------------------------- softmax
         const int q = warp & 3;                        // the quarter of TMEM lanes this warp may read
-        const int g = (warp - 2) >> 3;                 // the group: parity of its key tiles
-        const int half = ((warp - 2) >> 2) & 1;        // the half of a tile's keys, and of the accumulator's channels
+        const int g = (warp - 2) >> 2;                 // the unit
         const int r = q * 32 + lane;                   // this thread's query row within the tile
         const float sl2 = scale * 1.4426950408889634f;
-        const uint32_t lane_base = tmem + ((uint32_t)(q * 32) << 16), s_col = (uint32_t)(g * AL_BN), o_col = (uint32_t)(AL_O_COL + g * AL_HD + half * 64);
+        const uint32_t lane_base = tmem + ((uint32_t)(q * 32) << 16), s_col = (uint32_t)(g * AL_BN), o_col = (uint32_t)(AL_O_COL + g * AL_HD);
+        const int q_lo = g ? q_lo1 : q_lo0, pos_lo = start_pos + q_lo;
         const int pos = pos_lo + r, first = gb_first_key(pos, window), first_last = gb_first_key(pos_lo + AL_BM - 1, window);
         float m_run = AL_NEG_BIG, l_run = 0.f;
         bool ok = true;
-        for (int j = g; j < total; j += 2) {
-            const int i = j >> 1, key0 = (kt_begin + j) * AL_BN + half * 64;
-            ok = ok && mbar_wait_warp(&sh.s_full[g], i & 1, abort_flag, status);
-            uint32_t sv[64];
-            float mx = AL_NEG_BIG;
-            if (ok) {
-                tc_fence_after();
-                tmem_load64(lane_base + s_col + (uint32_t)(half * 64), sv);
-                if (key0 + 63 > pos_lo || key0 < first_last) {
+        int stage = 0, phase = 0;                      // of the keys
+        for (int j = 0; j < total; ++j) {
+            const int key0 = (kt_begin + j) * AL_BN;
+            if (!mbar_wait_warp(&sh.s_full[g][stage], phase, abort_flag, status)) { ok = false; break; }
+            if (++stage == AL_KSTAGES) { stage = 0; phase ^= 1; }
+            tc_fence_after();
+            uint32_t sv[AL_BN];
+            tmem_load128(lane_base + s_col, sv);
+            if (key0 + AL_BN - 1 > pos_lo || key0 < first_last) {
 #pragma unroll
-                    for (int k = 0; k < 64; ++k)
-                        if (key0 + k > pos || key0 + k < first) sv[k] = __float_as_uint(AL_NEG_BIG);
-                }
-                float mx4[4] = {AL_NEG_BIG, AL_NEG_BIG, AL_NEG_BIG, AL_NEG_BIG};
-#pragma unroll
-                for (int k = 0; k < 64; k += 8)
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) mx4[u] = al_max3(mx4[u], __uint_as_float(sv[k + 2 * u]), __uint_as_float(sv[k + 2 * u + 1]));
-                mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-                sh.pair_max[g][half][r] = mx;
+                for (int k = 0; k < AL_BN; ++k)
+                    if (key0 + k > pos || key0 + k < first) sv[k] = __float_as_uint(AL_NEG_BIG);
             }
-            // Both halves of the scores have been read behind this (P is stored over them), and both maxima are there. A wait that ran out
-            // ends the pair together.
-            ok = al_pair_sync(1 + g * 4 + q, ok);
-            if (!ok) break;
-            mx = fmaxf(mx, sh.pair_max[g][half ^ 1][r]);
+            float mx4[4] = {AL_NEG_BIG, AL_NEG_BIG, AL_NEG_BIG, AL_NEG_BIG};
+#pragma unroll
+            for (int k = 0; k < AL_BN; k += 8)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) mx4[u] = al_max3(mx4[u], __uint_as_float(sv[k + 2 * u]), __uint_as_float(sv[k + 2 * u + 1]));
+            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
             // the running maximum rises, and O_g is rescaled, only when it is exceeded by more than 2^8 in the exponent
             const bool raise = (mx - m_run) * sl2 > 8.0f;
-            if (i == 0) {
+            if (j == 0) {
                 if (raise) m_run = mx;
-            } else if (__any_sync(0xffffffffu, raise)) {      // (the same rows and maxima in both warps)
-                // O_g += P V of the group's previous tile is complete (S_j was issued behind it)
-                ok = mbar_wait_warp(&sh.pv_done[g], (i - 1) & 1, abort_flag, status);
+            } else if (__any_sync(0xffffffffu, raise)) {
+                // O += P V of the previous tile is complete (these scores were issued behind it)
+                if (!mbar_wait_warp(&sh.pv_done[g][(j - 1) % AL_VSTAGES], ((j - 1) / AL_VSTAGES) & 1, abort_flag, status)) { ok = false; break; }
                 tc_fence_after();
                 const float corr = raise ? al_exp2((m_run - mx) * sl2) : 1.0f;
                 if (raise) m_run = mx;
                 l_run *= corr;
 #pragma unroll
-                for (int c = 0; c < 64; c += 16) {
+                for (int c = 0; c < AL_HD; c += 16) {
                     uint32_t ov[16];
                     tmem_load16(lane_base + o_col + (uint32_t)c, ov);
 #pragma unroll
@@ -294,7 +292,7 @@ __global__ void __launch_bounds__(AL_WARPS * 32) attention_prefill_128_kernel(
             const float2 scale2 = make_float2(sl2, sl2), off2 = make_float2(-msl, -msl);
             float2 l2[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-            for (int part = 0; part < 64; part += 32) {
+            for (int part = 0; part < AL_BN; part += 32) {
                 uint32_t pw[16];
 #pragma unroll
                 for (int c = 0; c < 32; c += 2) {
@@ -303,55 +301,37 @@ __global__ void __launch_bounds__(AL_WARPS * 32) attention_prefill_128_kernel(
                     l2[(c >> 1) & 3] = __fadd2_rn(l2[(c >> 1) & 3], p);
                     pw[c >> 1] = pack2(__float_as_uint(p.x), __float_as_uint(p.y));
                 }
-                al_store16(lane_base + s_col + (uint32_t)(half * 32 + part / 2), pw);
+                al_store16(lane_base + s_col + (uint32_t)(part / 2), pw);
+                if (part >= 64) {      // three quarters, and the rest
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(part == 64 ? &sh.p_most[g] : &sh.p_ready[g]);
+                }
             }
             const float2 lsum = __fadd2_rn(__fadd2_rn(l2[0], l2[1]), __fadd2_rn(l2[2], l2[3]));
             l_run += lsum.x + lsum.y;
-            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.p_ready[g]);
         }
-        // merge: the warps post their maximum and sum per row, then each writes a quarter of the channels
-        if (ok) {
-            sh.row_max[g][r] = m_run;                  // (the same in both halves)
-            sh.row_sum[g][half][r] = l_run;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.x_ready);
-            ok = mbar_wait_warp(&sh.x_ready, 0, abort_flag, status);
-        }
-        for (int gg = 0; gg < 2 && ok; ++gg) {         // both accumulators must be final
-            const int last = total - 1 - ((total - 1 - gg) & 1);      // the group's last tile
-            if (last >= 0) ok = mbar_wait_warp(&sh.pv_done[gg], (last >> 1) & 1, abort_flag, status);
-        }
+        // O / l, 32 channels at a time, to global memory
+        if (ok) ok = mbar_wait_warp(&sh.pv_done[g][(total - 1) % AL_VSTAGES], ((total - 1) / AL_VSTAGES) & 1, abort_flag, status);
         if (ok) {
             tc_fence_after();
-            const float m0 = sh.row_max[0][r], m1 = sh.row_max[1][r], m = fmaxf(m0, m1);
-            const float l0 = sh.row_sum[0][0][r] + sh.row_sum[0][1][r], l1 = sh.row_sum[1][0][r] + sh.row_sum[1][1][r];
-            const bool two = total > 1;                // (a group without tiles has never written its accumulator: it is not read)
-            const float a0 = al_exp2((m0 - m) * sl2), a1 = two ? al_exp2((m1 - m) * sl2) : 0.f;
-            const float l = two ? l0 * a0 + l1 * a1 : l0 * a0, inv = l != 0.f ? 1.0f / l : 0.f;
-            const int c = g * 64 + half * 32;
-            float o[32];
-            uint32_t ov[32];
-            tmem_load32(lane_base + (uint32_t)(AL_O_COL + c), ov);
+            const float inv = l_run != 0.f ? 1.0f / l_run : 0.f;
+            __nv_bfloat16* dst = out + (size_t)(row0 + q_lo + r) * out_stride + (size_t)(kvh * group + (u0 + g) % group) * AL_HD;
 #pragma unroll
-            for (int k = 0; k < 32; ++k) o[k] = __uint_as_float(ov[k]) * a0;
-            if (two) {
-                tmem_load32(lane_base + (uint32_t)(AL_O_COL + AL_HD + c), ov);
+            for (int c = 0; c < AL_HD; c += 32) {
+                uint32_t ov[32];
+                tmem_load32(lane_base + o_col + (uint32_t)c, ov);
+                if (q_lo + r < nrows) {
 #pragma unroll
-                for (int k = 0; k < 32; ++k) o[k] = fmaf(__uint_as_float(ov[k]), a1, o[k]);
-            }
-            if (q_lo + r < nrows) {
-                __nv_bfloat16* dst = out + (size_t)(row0 + q_lo + r) * out_stride + (size_t)head * AL_HD + c;
-#pragma unroll
-                for (int k = 0; k < 32; k += 8) {
-                    uint4 w;
-                    w.x = pack2(__float_as_uint(o[k] * inv), __float_as_uint(o[k + 1] * inv));
-                    w.y = pack2(__float_as_uint(o[k + 2] * inv), __float_as_uint(o[k + 3] * inv));
-                    w.z = pack2(__float_as_uint(o[k + 4] * inv), __float_as_uint(o[k + 5] * inv));
-                    w.w = pack2(__float_as_uint(o[k + 6] * inv), __float_as_uint(o[k + 7] * inv));
-                    *reinterpret_cast<uint4*>(dst + k) = w;
+                    for (int k = 0; k < 32; k += 8) {
+                        uint4 w;
+                        w.x = pack2(__float_as_uint(__uint_as_float(ov[k]) * inv), __float_as_uint(__uint_as_float(ov[k + 1]) * inv));
+                        w.y = pack2(__float_as_uint(__uint_as_float(ov[k + 2]) * inv), __float_as_uint(__uint_as_float(ov[k + 3]) * inv));
+                        w.z = pack2(__float_as_uint(__uint_as_float(ov[k + 4]) * inv), __float_as_uint(__uint_as_float(ov[k + 5]) * inv));
+                        w.w = pack2(__float_as_uint(__uint_as_float(ov[k + 6]) * inv), __float_as_uint(__uint_as_float(ov[k + 7]) * inv));
+                        *reinterpret_cast<uint4*>(dst + c + k) = w;
+                    }
                 }
             }
         }
@@ -367,9 +347,10 @@ __global__ void __launch_bounds__(AL_WARPS * 32) attention_prefill_128_kernel(
             while (sh.q_issued && !mbar_try_wait(&sh.q_full, 0) && clock64() - t0 < TC_WAIT_CYCLES) {}
             for (int what = 0; what < 2; ++what)
                 for (int it = sh.consumed[what]; it < sh.issued[what]; ++it) {
-                    uint64_t* bar = what == 0 ? &sh.k_full[it % AL_STAGES] : &sh.v_full[it % AL_STAGES];
+                    uint64_t* bar = what == 0 ? &sh.k_full[it % AL_KSTAGES] : &sh.v_full[it % AL_VSTAGES];
+                    const int phase = (what == 0 ? it / AL_KSTAGES : it / AL_VSTAGES) & 1;
                     const long long t1 = clock64();
-                    while (!mbar_try_wait(bar, (it / AL_STAGES) & 1) && clock64() - t1 < TC_WAIT_CYCLES) {}
+                    while (!mbar_try_wait(bar, phase) && clock64() - t1 < TC_WAIT_CYCLES) {}
                 }
         }
         __syncwarp();
@@ -397,8 +378,8 @@ GB_EXPORT int gb_attention_prefill_128(const void* q, long long q_stride, int n_
     GB_REQUIRE(num_pages > 0 && num_pages * nkv * page_size < (1ll << 31) && (long long)max_pages * page_size < (1ll << 31) - 256,
                "gb_attention_prefill_128: the pages hold too many rows");
     if (num_seqs == 0 || n_rows == 0 || max_rows_per_seq <= 0) return 0;
-    const int tiles = gb_ceil_div(max_rows_per_seq, AL_BM);
-    GB_REQUIRE(tiles <= 65535, "gb_attention_prefill_128: %d rows a request are too many for one launch", max_rows_per_seq);
+    const long long pairs = ((long long)gb_ceil_div(max_rows_per_seq, AL_BM) * (nh / nkv) + 1) / 2;
+    GB_REQUIRE(pairs <= 65535, "gb_attention_prefill_128: %d rows a request are too many for one launch", max_rows_per_seq);
     CUtensorMap mq, mk, mv;
     if (tc_make_map_2d(&mq, q, n_rows, (long long)nh * hd, q_stride, AL_BM, 64, "gb_attention_prefill_128")) return 1;
     if (tc_make_map_2d(&mk, kcache, num_pages * nkv * page_size, hd, hd, page_size, 64, "gb_attention_prefill_128")) return 1;
@@ -407,7 +388,7 @@ GB_EXPORT int gb_attention_prefill_128(const void* q, long long q_stride, int n_
     GB_REQUIRE(e == cudaSuccess, "gb_attention_prefill_128: %d bytes of shared memory refused: %s", AL_SMEM, cudaGetErrorString(e));
     int page_shift = 0;
     while ((1 << page_shift) < page_size) ++page_shift;
-    gb_launch(GB_PDL_ATTENTION, attention_prefill_128_kernel, dim3(nh, num_seqs, tiles), dim3(AL_WARPS * 32), AL_SMEM, stream, mq, mk, mv,
+    gb_launch(GB_PDL_ATTENTION, attention_prefill_128_kernel, dim3(nkv, num_seqs, (unsigned)pairs), dim3(AL_WARPS * 32), AL_SMEM, stream, mq, mk, mv,
               (__nv_bfloat16*)out, out_stride, block_tables, max_pages, seq_first_row, seq_start_pos, nh, nkv, page_size, page_shift, num_pages, scale,
               window, status);
     return gb_check_launch("gb_attention_prefill_128");
