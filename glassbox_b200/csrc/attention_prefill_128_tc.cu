@@ -13,13 +13,13 @@
 //               that product starts on the first 96 keys' weights while the last 32 are formed.
 // What bounds it: a unit's chain of scores, softmax and weighted sum, each of which waits for the one before. Per unit and tile the two products are
 // 1,024 cycles of the tensor core and the 16,384 exponentials as many of the unit that forms them; the two units keep both busy in turn. One
-// unit a block (its key tiles in two interleaved chains) took 128 us of the case below where this takes 105: a tile of keys and values is 64 KB,
+// unit a block (its key tiles in two interleaved chains) took 137 us with the unpacking below where this took 113: a tile of keys and values is 64 KB,
 // and 148 blocks at one in 1,024 cycles each want more than the L2 cache hands out.
 // The mask is applied only in tiles that cross a boundary; key tiles that no row sees are skipped. Page 0 is read in the place of pages that
 // are missing, so that P = 0 meets finite numbers (the pages are zero-initialised).
 // Every wait is bounded: a wait that runs out sets GB_STATUS_WAIT_TIMEOUT and the block winds down (waits for its own copies, frees its TMEM,
 // returns). TMA loads use no multicast.
-// Measured (2,048 rows behind 2,048 tokens, 32/8 heads): mma.sync 750 us, this kernel 140.
+// Measured (2,048 rows behind 2,048 tokens, 32/8 heads, with the unpacking of 9 us): mma.sync 751 us, this kernel 109.
 #include "tcgen05.cuh"
 
 constexpr int AL_HD = 128, AL_BM = 128, AL_BN = 128, AL_KSTAGES = 3, AL_VSTAGES = 2, AL_WARPS = 11;
@@ -248,6 +248,13 @@ __global__ void __launch_bounds__(AL_WARPS * 32) attention_prefill_128_kernel(
         float m_run = AL_NEG_BIG, l_run = 0.f;
         bool ok = true;
         int stage = 0, phase = 0;                      // of the keys
+        // A branch around the arrival for the first three quarters of P: across it the compiler forms no weights of the last quarter, which it
+        // would do first otherwise (113 us of 109).
+        auto gave_up = [&]() {
+            if (!__any_sync(0xffffffffu, *abort_flag)) return false;
+            ok = false;
+            return true;
+        };
         for (int j = 0; j < total; ++j) {
             const int key0 = (kt_begin + j) * AL_BN;
             if (!mbar_wait_warp(&sh.s_full[g][stage], phase, abort_flag, status)) { ok = false; break; }
@@ -302,11 +309,13 @@ __global__ void __launch_bounds__(AL_WARPS * 32) attention_prefill_128_kernel(
                     pw[c >> 1] = pack2(__float_as_uint(p.x), __float_as_uint(p.y));
                 }
                 al_store16(lane_base + s_col + (uint32_t)(part / 2), pw);
+                if (part == 64 && gave_up()) break;
                 if (part >= 64) {      // three quarters, and the rest
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(part == 64 ? &sh.p_most[g] : &sh.p_ready[g]);
+                    if (part == 64 && gave_up()) break;
                 }
             }
             const float2 lsum = __fadd2_rn(__fadd2_rn(l2[0], l2[1]), __fadd2_rn(l2[2], l2[3]));
