@@ -2435,8 +2435,10 @@ def kv4_read(kcache: torch.Tensor, vcache: torch.Tensor, slots: torch.Tensor, k:
           kcache.shape[0], status.data_ptr(), stream)
 
 
-def _kv4_attention(q, out, kcache, vcache, block_tables, row_seq, positions, nh, nkv, hd, page_size) -> int:
+def _kv4_attention(q, out, kcache, vcache, block_tables, row_seq, positions, nh, nkv, hd, page_size, scale) -> int:
     n = q.shape[0]
+    if not 0.0 < scale < float("inf"):      # (maxima are taken before the scores are scaled)
+        raise KernelError(f"scores must be scaled by a positive number, not by {scale}")
     _kv4_pool(kcache, vcache, nkv, hd, page_size)
     if not (nh % nkv == 0):
         raise KernelError(f"{nh} heads are not a multiple of {nkv} kv heads")
@@ -2452,7 +2454,6 @@ def _kv4_attention(q, out, kcache, vcache, block_tables, row_seq, positions, nh,
 
 
 KV4_MMA_HEADS = 8       # query heads of a block of the tensor-core kernel
-KV4_EVEN_ROWS = 1024     # rows at most whose keys it shares evenly
 
 
 @functools.lru_cache(maxsize=4096)
@@ -2463,19 +2464,28 @@ def kv4_decode_plan(n: int, nh: int, nkv: int, hd: int, max_context: int, window
     * "even": that many blocks share all rows' keys evenly, whatever the rows' lengths,
     * "rows": that many shares of the keys of every row and head (the kernel for other types and head sizes).
 
-    Depends on the batch shape and the longest context alone, so a captured graph can fix it."""
+    Depends on the batch shape and the longest context alone, so a captured graph can fix it. Measured, in us:
+
+    * blocks of a cluster 1 / 2 / 4 / 8. A share wants 128 keys: one row of 9/3 heads of 64 at 256 keys 4.8 / 5.1 / 4.9 / 5.0, at 1,024
+      8.9 / 7.2 / 5.8 / 5.3. The more blocks there are anyway, the more keys a further one has to bring: 64 such rows at 1,024 keys 10.6 / 12.3 /
+      13.4 / 18.8, at 4,096 31 / 32 / 25 / 29; 300 at 2,048 46 / 48 / 61 / 90, at 4,096 84 / 80 / 91 / 119; 64 of 32/32 heads at 4,096 157 / 164 / 191 / 253.
+    * "even" against the best cluster costs its second launch and pays where eight blocks a row are too few: 2 rows of 32/8 heads of 128 up to 4,096
+      keys 16.5 to 10.6, up to 16,384 21.3 to 24.8; 24 of them at 8,192 75 to 71, one of them at 16,384 and the rest at 2,048 36 to 45.
+    * "rows": 16 rows of 8/2 float32 heads of 160 at 2,048 keys in 4 / 8 / 16 / 32 shares 96 / 66 / 52 / 76, one row of 9/3 heads of 64 at 512
+      keys in 2 / 4 / 8 / 16 23 / 14 / 14 / 15."""
     reach = max(1, min(max_context, window) if window else max_context)
     if dtype != torch.bfloat16 or not lib().gb_kv4_attention_decode_supported(hd):
-        splits = max(1, min(-(-reach // 128), -(-148 * 4 // max(n * nh, 1))))
+        splits = max(1, min(-(-reach // 128), -(-148 * 16 // max(n * nh, 1))))
         return "rows", splits, n * nh * splits * (hd + 2) if splits > 1 else 0
-    pairs = max(n * nkv * -(-(nh // nkv) // KV4_MMA_HEADS), 1)
+    if reach > 8192:
+        blocks = lib().gb_kv4_attention_decode_blocks(n, nh, nkv, hd, reach)
+        if blocks:
+            return "even", blocks, 2 * blocks * KV4_MMA_HEADS * (hd + 2) + 4 * blocks
+    pairs = n * nkv * -(-(nh // nkv) // KV4_MMA_HEADS)
     cluster = 8
-    while cluster > 1 and (reach <= 64 * cluster or pairs * cluster > 148 * 4):
+    while cluster > 1 and reach < cluster * max(128, pairs * cluster):
         cluster //= 2
-    if n > KV4_EVEN_ROWS or (reach <= 512 * cluster and pairs * cluster <= 148 * 4):
-        return "cluster", cluster, 0
-    blocks = lib().gb_kv4_attention_decode_blocks(n, nh, nkv, hd, reach)
-    return ("even", blocks, 2 * blocks * KV4_MMA_HEADS * (hd + 2) + 4 * blocks) if blocks else ("cluster", cluster, 0)
+    return "cluster", cluster, 0
 
 
 def kv4_decode_parts(q: torch.Tensor, nh: int, nkv: int, hd: int, max_context: int, window: Optional[int] = None) -> Optional[torch.Tensor]:
@@ -2493,7 +2503,7 @@ def kv4_attention_decode(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tenso
     float32 [n, nh * hd], rows may be strided; a row of position < 0 comes out as zeros. ``max_context``: no row has more keys in
     sight than this matters for (it sizes the shares of a row's keys, longer rows are still right). ``parts``: ``kv4_decode_parts``
     of the same rows, heads and ``max_context`` (with the window or without)."""
-    n = _kv4_attention(q, out, kcache, vcache, block_tables, row_seq, positions, nh, nkv, hd, page_size)
+    n = _kv4_attention(q, out, kcache, vcache, block_tables, row_seq, positions, nh, nkv, hd, page_size, scale)
     dtype = _dt(q)
     stream = _here(q, out, kcache, vcache, block_tables, row_seq, positions, status, parts)
     kind, number, floats = kv4_decode_plan(n, nh, nkv, hd, max_context, window, q.dtype)
@@ -2555,8 +2565,9 @@ def kv4_attention_prefill(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tens
     """``kv4_attention_decode`` for portions of prompts, runs of consecutive rows of a request: the pages in sight are unpacked into
     kpages/vpages (q's type, [pages, nkv, page_size, hd], numbers everywhere: zero them once) and read from there by the prompt kernel that
     takes the shape (``kv4_prompt_kernel``); where none does, row by row. ``max_context`` bounds the tokens that a request holds after the
-    step. Two calls that may run at the same time need pages of their own to unpack into."""
-    n = _kv4_attention(q, out, kcache, vcache, block_tables, row_seq, positions, nh, nkv, hd, page_size)
+    step. A value that is not a number and that a later row of the portion sees may reach the earlier ones (weight 0 times NaN), as in every prompt
+    kernel here. Two calls that may run at the same time need pages of their own to unpack into."""
+    n = _kv4_attention(q, out, kcache, vcache, block_tables, row_seq, positions, nh, nkv, hd, page_size, scale)
     if not (kpages.dtype == q.dtype and kpages.shape[1:] == (nkv, page_size, hd)):
         raise KernelError(f"kpages must be {q.dtype} [pages, {nkv}, {page_size}, {hd}]")
     _dt(q)

@@ -105,3 +105,9 @@ def test_refused_scores():
                  (x[:, :3], t, lp, None, None, i), (x, t, lp, None, None, i[:, :0])):
         with pytest.raises(kernels.KernelError):
             kernels.token_logprobs(*args)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1, float("nan"), float("inf")])
+def test_refused_scales(scale):
+    with pytest.raises(kernels.KernelError, match="positive"):
+        kernels.kv4_attention_decode(**{**_attention(), "scale": scale})
