@@ -14,12 +14,17 @@
 //     the tensor cores) and turned over in registers, codes less 136 are whole numbers that bfloat16 holds. (Values cannot keep their 128 + 8: the
 //     sum over thousands of keys would be 136 sum p against results near zero.)
 // (With the queries as the 16 rows of A, eight of them zero, the scores lie as the second product wants them, but take twice the products, twice
-// the scales and a move for each operand register: 64 rows of 32/32 heads of 64, 4,096 keys 182 to 200 us.)
+// the scales and a move for each operand register: 64 rows of 32/32 heads of 64, 4,096 keys in even shares 182 to 200 us.)
 // The reference that is subtracted from scores rises only when one exceeds it by 2^8 (weights up to 256 cost the float32 sums nothing), so that
 // the sums of O are hardly ever rescaled.
-// The warps of a block add up in shared memory. How the keys are shared among blocks: few rows of short contexts, where latency is all, get
-// a cluster of up to eight blocks a row and chunk of heads, which add up from each other's shared memory; otherwise all rows' steps are cut evenly
-// among the blocks that run at once (kv4_decode_even_kernel). Nothing is left behind for the next call.
+// The warps of a block add up in shared memory. How the keys are shared among blocks: a cluster of up to eight blocks a row and chunk of heads, which
+// add up from each other's shared memory, or, behind the longest contexts, all rows' steps cut evenly among the blocks that run at once
+// (kv4_decode_even_kernel). Nothing is left behind for the next call.
+//
+// What bounds it: issuing instructions, some 450 for 32 keys of a head of 64 and their values (2.4 of 4 a cycle and multiprocessor), not the
+// memory. 64 rows of 32/32 heads of 64 behind 4,096 keys, 605 MB, take 157 us (3.8 TB/s); 2 rows of 32/8 heads of 128 behind 131,072, 302 MB, 87 us.
+// The second without taking codes apart 72, without the second product 63, without copies 80; one multiprocessor's blocks 3 / 4 / 5 of them 90 / 87 /
+// 115, of heads of 64 (the first, in even shares) 4 / 5 / 6 183 / 180 / 189, with one tile a step instead of two 203.
 #include <atomic>
 
 #include "kv4_attention.cuh"
@@ -188,14 +193,13 @@ __device__ __forceinline__ float* kv4_segment(const Kv4AttnArgs& a, unsigned cha
     }
 
     // Q^T as the B operand: column g is head head0 + g; the two k16 steps of a group take channels 8 t + {0, 4, 1, 5} and {2, 6, 3, 7} of it
-    // at this thread's places, as a word of eight codes yields them. (A negative factor of the scores turns the queries' signs.)
+    // at this thread's places, as a word of eight codes yields them.
     uint32_t qf[G][4];
     float from[G][4];                        // -136 times a group's sum of q, heads 2 t and 2 t + 1: where the sums of its products start
-    const float scale = fmaxf(fabsf(a.scale), 1e-30f);
+    const float scale = a.scale;
     {
         const __nv_bfloat16* q = (const __nv_bfloat16*)a.q + (size_t)row * a.q_stride + (size_t)(head0 + g) * HD + 8 * t;
         const bool wide = (((uintptr_t)a.q | (uintptr_t)(a.q_stride * 2)) & 15) == 0;
-        const uint32_t turn = a.scale < 0.f ? 0x80008000u : 0u;
 #pragma unroll
         for (int i = 0; i < G; ++i) {
             uint32_t w[4] = {0, 0, 0, 0};
@@ -209,8 +213,6 @@ __device__ __forceinline__ float* kv4_segment(const Kv4AttnArgs& a, unsigned cha
                     for (int j = 0; j < 4; ++j) w[j] = p[2 * j] | (uint32_t)p[2 * j + 1] << 16;
                 }
             }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] ^= turn;
             qf[i][0] = __byte_perm(w[0], w[2], 0x5410);
             qf[i][1] = __byte_perm(w[0], w[2], 0x7632);
             qf[i][2] = __byte_perm(w[1], w[3], 0x5410);
@@ -713,6 +715,7 @@ GB_EXPORT int gb_kv4_attention_decode(const void* q, long long q_stride, void* o
                                       int* status, cudaStream_t stream) {
     KV4_REQUIRE_SIZES("gb_kv4_attention_decode")
     GB_REQUIRE(n >= 0 && nh > 0 && nh % nkv == 0 && max_pages > 0, "gb_kv4_attention_decode: bad sizes (rows %d, heads %d of %d, tables of %d pages)", n, nh, nkv, max_pages);
+    GB_REQUIRE(scale > 0.f && scale < INFINITY, "gb_kv4_attention_decode: scores must be scaled by a positive number");
     GB_REQUIRE(cluster == 1 || cluster == 2 || cluster == 4 || cluster == 8, "gb_kv4_attention_decode: clusters of %d are not built", cluster);
     GB_REQUIRE(blocks == 0 || (blocks > 0 && n <= KV4E_ROWS && parts != nullptr && (uintptr_t)parts % 16 == 0),
                "gb_kv4_attention_decode: even shares among %d blocks take up to %d rows and aligned scratch", blocks, KV4E_ROWS);
