@@ -528,7 +528,8 @@ GB_EXPORT int gb_kv4_read(const void* kcache, const void* vcache, const int* slo
 
 // Pages of 4 bits that the rows of a step see, as numbers into pages of the same ids: one block a page of a request and kv head.
 // Numbers of tokens outside the request's range (before its first row's window, behind its last row) that are NaN become zero: the
-// kernels that read the pages multiply what they mask by zero.
+// kernels that read the pages multiply what they mask by zero. (Of two requests that share a page, a NaN in which lies before the window of one and
+// in sight of the other, either may have its way.) Bound by the latency of a page's few loads: 9 us for 4,096 tokens of 8 heads of 128, 21 MB, 17 of them written.
 template <typename T>
 __global__ void __launch_bounds__(KV4_THREADS) kv4_expand_kernel(const unsigned char* __restrict__ kcache, const unsigned char* __restrict__ vcache,
                                                                 T* __restrict__ k, T* __restrict__ v, const int* __restrict__ block_tables, int max_pages,
@@ -541,6 +542,7 @@ __global__ void __launch_bounds__(KV4_THREADS) kv4_expand_kernel(const unsigned 
     if (start < 0 || rows <= 0) return;
     const long long end = (long long)start + rows, first = gb_first_key(start, window > 0 ? window : 0);
     const long long begin = (long long)blockIdx.x * page_size;
+    if (end > (long long)gridDim.x * page_size && threadIdx.x == 0 && h == 0 && blockIdx.x == 0) atomicOr(status, GB_STATUS_BAD_POSITION);      // tokens that no block unpacks
     if (begin >= end || begin + page_size <= first) return;
     const long long page = block_tables[(size_t)seq * max_pages + blockIdx.x];
     if (page < 0 || page >= num_pages) {

@@ -2525,7 +2525,8 @@ def kv4_expand(kcache: torch.Tensor, vcache: torch.Tensor, kpages: torch.Tensor,
                seq_first_row: torch.Tensor, seq_start_pos: torch.Tensor, max_context: int, window: Optional[int], status: torch.Tensor) -> None:
     """The pages that the rows of a step see, unpacked into pages of the same ids: kpages/vpages [pages, nkv, page_size, hd], bfloat16 or
     float32. Request s brings rows seq_first_row[s] .. seq_first_row[s + 1] - 1 from position seq_start_pos[s] on (negative: a padding
-    request). NaNs of tokens that none of a request's rows sees become zeros."""
+    request). NaNs of tokens that none of a request's rows sees become zeros. A request that holds more than ``max_context`` tokens is reported
+    (a bad position)."""
     if not (kpages.dim() == 4 and kpages.shape == vpages.shape and kpages.dtype == vpages.dtype and kpages.is_contiguous() and vpages.is_contiguous()):
         raise KernelError("kpages and vpages must be contiguous [pages, kv heads, page size, head size] of one type")
     pages, nkv, page_size, hd = kpages.shape

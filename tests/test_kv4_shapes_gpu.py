@@ -166,6 +166,17 @@ def test_two_steps_at_once():
         assert torch.equal(a[1], b[1]) and int(a[4]) == int(b[4]) == 0
 
 
+def test_a_context_longer_than_said_is_reported():
+    from glassbox_b200 import kernels
+    pools, _ = pool_of(8, 1, 16, 64, 5)
+    ints = [torch.tensor(v, dtype=torch.int32, device=DEV) for v in ([[0, 1, 2, 3]], [0] * 6, list(range(40, 46)), [0, 6], [40])]
+    q = torch.randn(6, 64, device=DEV).to(BF16)
+    for most, said in ((46, 0), (48, 0), (32, 4)):
+        pages, st = [torch.zeros(8, 1, 16, 64, dtype=BF16, device=DEV) for _ in range(2)], status()
+        kernels.kv4_attention_prefill(q, torch.empty_like(q), *pools, *ints, 6, 1, 1, 64, 16, 0.1, None, most, *pages, st)
+        assert int(st) == said
+
+
 @pytest.mark.parametrize("hd", [64, 128])
 def test_recorded_prompts(hd):
     from glassbox_b200 import kernels
