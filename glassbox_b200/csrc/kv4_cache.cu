@@ -237,7 +237,7 @@ struct Kv4WriteArgs {
 
 // One row a block (blockIdx.y: its items KV4_THREADS at a time). Work items, one a thread: values (four channels in each of two neighbouring
 // groups: a word of codes), eight lanes to a pair of groups; keys (eight channels of a group: a word), four lanes to a group; queries
-// (eight pairs of channels, or eight channels that do not turn). WIDE: everything starts on 16 bytes and rot / 2 is a multiple of 8.
+// (eight pairs of channels, or twice eight channels that do not turn). WIDE: everything starts on 16 bytes and rot / 2 is a multiple of 8.
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(KV4_THREADS) kv4_write_kernel(const Kv4WriteArgs a) {
     gb_pdl_launch_dependents();
@@ -389,14 +389,15 @@ __global__ void __launch_bounds__(KV4_THREADS) kv4_write_kernel(const Kv4WriteAr
             kv4_store<T, 8, WIDE>(to + 8 * i, x0);
             kv4_store<T, 8, WIDE>(to + 8 * i + half, x1);
         } else {
-            const int c = a.rot + 8 * (i - half / 8);
-            uint4 raw[sizeof(T) / 2];
+            const int c = a.rot + 8 * (i - half / 8), second = (hd - a.rot) / 2;
+            constexpr int EACH = (int)sizeof(T) / 2;
+            uint4 raw[2 * EACH];
 #pragma unroll
-            for (int j = 0; j < (int)sizeof(T) / 2; ++j) raw[j] = reinterpret_cast<const uint4*>(p + c)[j];
+            for (int j = 0; j < 2 * EACH; ++j) raw[j] = reinterpret_cast<const uint4*>(p + c + (j < EACH ? 0 : second))[j % EACH];
             report();
             if (pos < 0) return;
 #pragma unroll
-            for (int j = 0; j < (int)sizeof(T) / 2; ++j) reinterpret_cast<uint4*>(to + c)[j] = raw[j];
+            for (int j = 0; j < 2 * EACH; ++j) reinterpret_cast<uint4*>(to + c + (j < EACH ? 0 : second))[j % EACH] = raw[j];
         }
         return;
     }
@@ -438,7 +439,7 @@ GB_EXPORT int gb_kv4_write(const void* qkv, long long qkv_stride, int dtype, voi
     a.units_k = write_kv ? nkv * G * 4 : 0;
     // (channels that do not turn are copied only where the queries go somewhere else)
     const bool in_place = q == qkv && q_stride == qkv_stride;
-    const int pairs = wide ? rot / 16 + (in_place ? 0 : (hd - rot) / 8) : rot / 2 + (in_place ? 0 : hd - rot);
+    const int pairs = wide ? rot / 16 + (in_place ? 0 : (hd - rot) / 16) : rot / 2 + (in_place ? 0 : hd - rot);
     a.units_q = nh * pairs;
     a.by_w = Kv4Div((G + 1) / 2);
     a.by_g = Kv4Div(G);
@@ -484,28 +485,31 @@ __device__ __forceinline__ void kv4_put(float* p, const uint32_t (&x)[4]) {
         *reinterpret_cast<uint4*>(p + 2 * i) = make_uint4(x[i] << 16, x[i] & 0xffff0000u, x[i + 1] << 16, x[i + 1] & 0xffff0000u);
 }
 
-// One row a block (blockIdx.y: its items KV4_THREADS at a time), eight neighbouring channels of a key or a value a thread.
+// One row a block (blockIdx.y: its items KV4_THREADS at a time), eight neighbouring channels of a key and of its value a thread.
 template <typename T>
 __global__ void __launch_bounds__(KV4_THREADS) kv4_read_kernel(const unsigned char* __restrict__ kcache, const unsigned char* __restrict__ vcache,
                                                               const int* __restrict__ slots, T* __restrict__ k, T* __restrict__ v, int nkv,
                                                               int hd, int page_size, long long num_slots, Kv4Div by_g, int* __restrict__ status) {
     gb_pdl_launch_dependents();
     gb_pdl_wait();
-    const int row = blockIdx.x, slot = slots[row], per = nkv * (hd / 8);
-    int item = blockIdx.y * KV4_THREADS + threadIdx.x;
-    if (slot < 0 || item >= 2 * per) return;
+    const int row = blockIdx.x, slot = slots[row], item = blockIdx.y * KV4_THREADS + threadIdx.x;
+    if (slot < 0 || item >= nkv * (hd / 8)) return;
     if (slot >= num_slots) {
         if (item == 0) atomicOr(status, GB_STATUS_BAD_SLOT);
         return;
     }
-    const bool value = item >= per;
-    if (value) item -= per;
     const int G = hd / KV4_GROUP, t = item & 3, h = by_g.of(item >> 2), g = (item >> 2) - h * G;
     const int page = slot / page_size, off = slot - page * page_size, r = off % KV4_TILE;
-    const unsigned char* tile = (value ? vcache : kcache) + kv4_tile(page, h, off, nkv, page_size) * kv4_tile_bytes(hd);
+    const long long at = kv4_tile(page, h, off, nkv, page_size) * kv4_tile_bytes(hd);
+    const unsigned key = kv4_word(kcache + at, hd, r, g, t, false), value = kv4_word(vcache + at, hd, r, g, t, true);
+    const int scale = 8 * hd + (r * G + g) * 2;
+    const unsigned short dk = *reinterpret_cast<const unsigned short*>(kcache + at + scale), dv = *reinterpret_cast<const unsigned short*>(vcache + at + scale);
+    const size_t to = ((size_t)row * nkv + h) * hd + KV4_GROUP * g + 8 * t;
     uint32_t x[4];
-    kv4_eight(kv4_word(tile, hd, r, g, t, value), reinterpret_cast<const unsigned short*>(tile + 8 * hd)[r * G + g], x);
-    kv4_put((value ? v : k) + ((size_t)row * nkv + h) * hd + KV4_GROUP * g + 8 * t, x);
+    kv4_eight(key, dk, x);
+    kv4_put(k + to, x);
+    kv4_eight(value, dv, x);
+    kv4_put(v + to, x);
 }
 
 GB_EXPORT int gb_kv4_read(const void* kcache, const void* vcache, const int* slots, void* k, void* v, int dtype, int n, int nkv, int hd,
@@ -514,7 +518,7 @@ GB_EXPORT int gb_kv4_read(const void* kcache, const void* vcache, const int* slo
     GB_REQUIRE(dtype == GB_F32 || dtype == GB_BF16, "gb_kv4_read: unsupported dtype %d", dtype);
     GB_REQUIRE(((uintptr_t)kcache | (uintptr_t)vcache | (uintptr_t)k | (uintptr_t)v) % 16 == 0, "gb_kv4_read: tensors must be 16-byte aligned");
     if (n <= 0) return 0;
-    const dim3 grid(n, gb_ceil_div(2 * nkv * (hd / 8), KV4_THREADS)), block(KV4_THREADS);
+    const dim3 grid(n, gb_ceil_div(nkv * (hd / 8), KV4_THREADS)), block(KV4_THREADS);
     const unsigned char *kc = (const unsigned char*)kcache, *vc = (const unsigned char*)vcache;
     const Kv4Div by_g(hd / KV4_GROUP);
     if (dtype == GB_F32)
