@@ -86,6 +86,24 @@ __device__ __forceinline__ void kv4_store(T* p, const float (&f)[N]) {
     }
 }
 
+// N numbers in 16-byte pieces, asked for and looked at later.
+template <typename T, int N> struct Kv4Asked {
+    static constexpr int WORDS = N * (int)sizeof(T) / 4;
+    uint32_t w[WORDS];
+    __device__ __forceinline__ void ask(const T* p) {
+#pragma unroll
+        for (int i = 0; i < WORDS; i += 4) {
+            const uint4 v = *reinterpret_cast<const uint4*>(p + i * 4 / (int)sizeof(T));
+            w[i] = v.x; w[i + 1] = v.y; w[i + 2] = v.z; w[i + 3] = v.w;
+        }
+    }
+    __device__ __forceinline__ void get(float (&f)[N]) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            f[i] = sizeof(T) == 4 ? __uint_as_float(w[i % WORDS]) : __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    }
+};
+
 __device__ __forceinline__ float kv4_max_nan(float a, float b) {           // NaN where one of them is
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -364,40 +382,61 @@ __global__ void __launch_bounds__(KV4_THREADS) kv4_write_kernel(const Kv4WriteAr
         return;
     }
 
-    // queries
+    // queries: of a head, or (WIDE, an even number of them) of two heads nh / 2 apart, which turn by the same angles
     const int k = item - a.units_v - a.units_k, h = a.by_pairs.of(k), i = k - h * (int)a.by_pairs.d;
     const T* p = base + (size_t)h * hd;
     T* to = (T*)a.q + (size_t)row * a.q_stride + (size_t)h * hd;
     if (WIDE) {
+        const bool twins = a.nh % 2 == 0;
+        const size_t twin = (size_t)(a.nh / 2) * hd;
         if (8 * i < half) {
-            float x0[8], x1[8];
-            kv4_load<T, 8, WIDE>(p + 8 * i, x0);
-            kv4_load<T, 8, WIDE>(p + 8 * i + half, x1);
+            Kv4Asked<T, 8> x[4];
+            x[0].ask(p + 8 * i);
+            x[1].ask(p + 8 * i + half);
+            if (twins) {
+                x[2].ask(p + twin + 8 * i);
+                x[3].ask(p + twin + 8 * i + half);
+            }
             report();
             if (pos < 0) return;
-            if (turns()) {
-                const float4* cs = reinterpret_cast<const float4*>(a.table + (size_t)pos * half + 8 * i);
+            const float4* cs = reinterpret_cast<const float4*>(a.table + (size_t)pos * half + 8 * i);
+            float4 angle[4];
+            const bool turn = turns();
+            if (turn) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float4 f = cs[j / 2];
-                    const float2 c = j % 2 ? make_float2(f.z, f.w) : make_float2(f.x, f.y);
-                    const float z0 = kv4_turn(x0[j], x1[j], c, false), z1 = kv4_turn(x1[j], x0[j], c, true);
-                    x0[j] = z0;
-                    x1[j] = z1;
-                }
+                for (int j = 0; j < 4; ++j) angle[j] = cs[j];
             }
-            kv4_store<T, 8, WIDE>(to + 8 * i, x0);
-            kv4_store<T, 8, WIDE>(to + 8 * i + half, x1);
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                if (y == 1 && !twins) break;
+                float x0[8], x1[8];
+                x[2 * y].get(x0);
+                x[2 * y + 1].get(x1);
+                if (turn) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float2 c = j % 2 ? make_float2(angle[j / 2].z, angle[j / 2].w) : make_float2(angle[j / 2].x, angle[j / 2].y);
+                        const float z0 = kv4_turn(x0[j], x1[j], c, false), z1 = kv4_turn(x1[j], x0[j], c, true);
+                        x0[j] = z0;
+                        x1[j] = z1;
+                    }
+                }
+                kv4_store<T, 8, WIDE>(to + y * twin + 8 * i, x0);
+                kv4_store<T, 8, WIDE>(to + y * twin + 8 * i + half, x1);
+            }
         } else {
             const int c = a.rot + 8 * (i - half / 8), second = (hd - a.rot) / 2;
             constexpr int EACH = (int)sizeof(T) / 2;
-            uint4 raw[2 * EACH];
+            uint4 raw[4 * EACH];
+            auto at = [&](int j) { return c + (size_t)(j / EACH % 2) * second + (size_t)(j / EACH / 2) * twin; };
 #pragma unroll
-            for (int j = 0; j < 2 * EACH; ++j) raw[j] = reinterpret_cast<const uint4*>(p + c + (j < EACH ? 0 : second))[j % EACH];
+            for (int j = 0; j < 4 * EACH; ++j)
+                if (j < 2 * EACH || twins) raw[j] = reinterpret_cast<const uint4*>(p + at(j))[j % EACH];
             report();
             if (pos < 0) return;
 #pragma unroll
-            for (int j = 0; j < 2 * EACH; ++j) reinterpret_cast<uint4*>(to + c + (j < EACH ? 0 : second))[j % EACH] = raw[j];
+            for (int j = 0; j < 4 * EACH; ++j)
+                if (j < 2 * EACH || twins) reinterpret_cast<uint4*>(to + at(j))[j % EACH] = raw[j];
         }
         return;
     }
@@ -440,7 +479,7 @@ GB_EXPORT int gb_kv4_write(const void* qkv, long long qkv_stride, int dtype, voi
     // (channels that do not turn are copied only where the queries go somewhere else)
     const bool in_place = q == qkv && q_stride == qkv_stride;
     const int pairs = wide ? rot / 16 + (in_place ? 0 : (hd - rot) / 16) : rot / 2 + (in_place ? 0 : hd - rot);
-    a.units_q = nh * pairs;
+    a.units_q = (wide && nh % 2 == 0 ? nh / 2 : nh) * pairs;
     a.by_w = Kv4Div((G + 1) / 2);
     a.by_g = Kv4Div(G);
     a.by_pairs = Kv4Div(pairs > 0 ? pairs : 1);
