@@ -114,14 +114,25 @@ __device__ __forceinline__ float kv4_min_nan(float a, float b) {
     asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
+__device__ __forceinline__ float kv4_max_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float kv4_min_nan(float a, float b, float c) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 // The largest and the smallest of N numbers of this thread.
 template <int N>
 __device__ __forceinline__ void kv4_ends(const float (&y)[N], float& high, float& low) {
-    high = low = y[0];
+    high = kv4_max_nan(y[0], y[1]);
+    low = kv4_min_nan(y[0], y[1]);
 #pragma unroll
-    for (int i = 1; i < N; ++i) {
-        high = kv4_max_nan(high, y[i]);
-        low = kv4_min_nan(low, y[i]);
+    for (int i = 2; i < N; i += 2) {
+        high = kv4_max_nan(high, y[i], y[i + 1]);
+        low = kv4_min_nan(low, y[i], y[i + 1]);
     }
 }
 
@@ -158,6 +169,21 @@ __device__ __forceinline__ unsigned kv4_codes(const float (&y)[N], float d, floa
         near = fmaxf(near, fabsf(q - (t - WHOLE)));
         w += __float_as_uint(t) << (4 * i);
     }
+    return w;
+}
+
+// The same for numbers that are bfloat16. 2 y / d has a denominator of at most 31 (d's five bits) behind the digits of y's eight, so a quotient that
+// is not half way between two codes is 2^-9 off at least, and one rounded to 2^-13 by a first sum (the product with the reciprocal is off by less than
+// 2^-19) is half way where y / d is. The largest magnitude has the sign of -8, so that only 7 limits; its 8.26 at most rounds to 8.
+template <int N>
+__device__ __forceinline__ unsigned kv4_codes_bf16(const float (&y)[N], float d) {
+    if (!(fabsf(d) > 0.f)) return 0x88888888u;
+    constexpr float WHOLE = 12582920.f, FINE = 1536.f;
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+    unsigned w = 0x100000000ull - 0x3f400000u;
+#pragma unroll
+    for (int i = 0; i < N; ++i) w += __float_as_uint(fminf(fmaf(y[i], r, FINE) + (WHOLE - FINE), WHOLE + 7.f)) << (4 * i);
     return w;
 }
 
@@ -236,6 +262,14 @@ __device__ __noinline__ void kv4_key_again(const T* p, const float2* turn, int c
     codes = kv4_codes2(y, lo, d);
 }
 
+// The page of a slot; shift: of a page size that is a power of two, else -1.
+__device__ __forceinline__ int kv4_page(int slot, int page_size, int shift) { return shift >= 0 ? slot >> shift : slot / page_size; }
+static int kv4_page_shift(int page_size) {
+    int shift = 0;
+    while (shift < 30 && (1 << shift) < page_size) ++shift;
+    return (1 << shift) == page_size ? shift : -1;
+}
+
 struct Kv4WriteArgs {
     const void* qkv;
     long long qkv_stride;
@@ -246,7 +280,7 @@ struct Kv4WriteArgs {
     const int* slots;
     unsigned char* kcache;
     unsigned char* vcache;
-    int nh, nkv, hd, rot, max_pos, page_size, write_kv;
+    int nh, nkv, hd, rot, max_pos, page_size, page_shift, write_kv;
     long long num_slots;
     int* status;
     int units_v, units_k, units_q;           // work items of a row: values, keys, queries
@@ -284,8 +318,8 @@ __global__ void __launch_bounds__(KV4_THREADS) kv4_write_kernel(const Kv4WriteAr
         if (two) kv4_load<T, 4, WIDE>(p + 32, y1);
         report();
         if (pos < 0 || !stores()) return;    // a padding row, or a bad slot (the same for all items of a row: no lane of a group is missing)
-        const int page = slot / a.page_size, off = slot - page * a.page_size, r = off % KV4_TILE;
-        float high0, low0, high1, low1, near;
+        const int page = kv4_page(slot, a.page_size, a.page_shift), off = slot - page * a.page_size, r = off % KV4_TILE;
+        float high0, low0, high1, low1;
         kv4_ends(y0, high0, low0);
         kv4_ends(y1, high1, low1);
         const unsigned mask = 0xffu << (lane & 24);
@@ -300,12 +334,18 @@ __global__ void __launch_bounds__(KV4_THREADS) kv4_write_kernel(const Kv4WriteAr
         unsigned char* tile = a.vcache + kv4_tile(page, h, off, a.nkv, a.page_size) * kv4_tile_bytes(hd);
         unsigned char* codes = tile + r * (hd / 2) + (u * G + 2 * w) * 2;
         unsigned short* scales = reinterpret_cast<unsigned short*>(tile + 8 * hd) + r * G + 2 * w;
-        unsigned c0 = kv4_codes(y0, d0, near);
-        const float none[4] = {0.f, 0.f, 0.f, 0.f};
-        // (the quotient of a float32 may have been rounded to half way; that of a bfloat16 by five bits lies half way if it says so)
-        if (sizeof(T) == 4 && near == 0.5f) c0 = kv4_codes2(y0, none, d0);
-        unsigned c1 = kv4_codes(y1, d1, near);
-        if (sizeof(T) == 4 && near == 0.5f) c1 = kv4_codes2(y1, none, d1);
+        unsigned c0, c1;
+        if (sizeof(T) == 2) {
+            c0 = kv4_codes_bf16(y0, d0);
+            c1 = kv4_codes_bf16(y1, d1);
+        } else {                             // (the quotient of a float32 may have been rounded to half way)
+            const float none[4] = {0.f, 0.f, 0.f, 0.f};
+            float near;
+            c0 = kv4_codes(y0, d0, near);
+            if (near == 0.5f) c0 = kv4_codes2(y0, none, d0);
+            c1 = kv4_codes(y1, d1, near);
+            if (near == 0.5f) c1 = kv4_codes2(y1, none, d1);
+        }
         c0 &= 0xffffu;
         c1 &= 0xffffu;
         if (two && G % 2 == 0) {
@@ -330,7 +370,7 @@ __global__ void __launch_bounds__(KV4_THREADS) kv4_write_kernel(const Kv4WriteAr
         kv4_load<T, 8, WIDE>(p + c0, y);
         if (WIDE && a.table != nullptr && c0 < a.rot) kv4_load<T, 8, WIDE>(p + (second ? first : first + half), o);
         if (pos < 0 || !stores()) return;
-        const int page = slot / a.page_size, off = slot - page * a.page_size, r = off % KV4_TILE;
+        const int page = kv4_page(slot, a.page_size, a.page_shift), off = slot - page * a.page_size, r = off % KV4_TILE;
         const unsigned mask = 0xfu << (lane & 28);
         const bool turn_them = turns() && c0 < a.rot;
         const float2* turn = a.table + (size_t)pos * half;
@@ -472,7 +512,7 @@ GB_EXPORT int gb_kv4_write(const void* qkv, long long qkv_stride, int dtype, voi
     Kv4WriteArgs a = {};
     a.qkv = qkv; a.qkv_stride = qkv_stride; a.q = q; a.q_stride = q_stride; a.table = rot ? (const float2*)cos_sin : nullptr;
     a.positions = positions; a.slots = slots; a.kcache = (unsigned char*)kcache; a.vcache = (unsigned char*)vcache; a.nh = nh;
-    a.nkv = nkv; a.hd = hd; a.rot = rot; a.max_pos = max_pos; a.page_size = page_size; a.write_kv = write_kv;
+    a.nkv = nkv; a.hd = hd; a.rot = rot; a.max_pos = max_pos; a.page_size = page_size; a.page_shift = kv4_page_shift(page_size); a.write_kv = write_kv;
     a.num_slots = num_pages * page_size; a.status = status;
     a.units_v = write_kv ? nkv * ((G + 1) / 2) * 8 : 0;
     a.units_k = write_kv ? nkv * G * 4 : 0;
@@ -528,7 +568,7 @@ __device__ __forceinline__ void kv4_put(float* p, const uint32_t (&x)[4]) {
 template <typename T>
 __global__ void __launch_bounds__(KV4_THREADS) kv4_read_kernel(const unsigned char* __restrict__ kcache, const unsigned char* __restrict__ vcache,
                                                               const int* __restrict__ slots, T* __restrict__ k, T* __restrict__ v, int nkv,
-                                                              int hd, int page_size, long long num_slots, Kv4Div by_g, int* __restrict__ status) {
+                                                              int hd, int page_size, int page_shift, long long num_slots, Kv4Div by_g, int* __restrict__ status) {
     gb_pdl_launch_dependents();
     gb_pdl_wait();
     const int row = blockIdx.x, slot = slots[row], item = blockIdx.y * KV4_THREADS + threadIdx.x;
@@ -538,7 +578,7 @@ __global__ void __launch_bounds__(KV4_THREADS) kv4_read_kernel(const unsigned ch
         return;
     }
     const int G = hd / KV4_GROUP, t = item & 3, h = by_g.of(item >> 2), g = (item >> 2) - h * G;
-    const int page = slot / page_size, off = slot - page * page_size, r = off % KV4_TILE;
+    const int page = kv4_page(slot, page_size, page_shift), off = slot - page * page_size, r = off % KV4_TILE;
     const long long at = kv4_tile(page, h, off, nkv, page_size) * kv4_tile_bytes(hd);
     const unsigned key = kv4_word(kcache + at, hd, r, g, t, false), value = kv4_word(vcache + at, hd, r, g, t, true);
     const int scale = 8 * hd + (r * G + g) * 2;
@@ -562,10 +602,10 @@ GB_EXPORT int gb_kv4_read(const void* kcache, const void* vcache, const int* slo
     const Kv4Div by_g(hd / KV4_GROUP);
     if (dtype == GB_F32)
         gb_launch(GB_PDL_ELEMENTWISE, kv4_read_kernel<float>, grid, block, 0, stream, kc, vc, slots, (float*)k, (float*)v, nkv, hd, page_size,
-                  num_pages * page_size, by_g, status);
+                  kv4_page_shift(page_size), num_pages * page_size, by_g, status);
     else
         gb_launch(GB_PDL_ELEMENTWISE, kv4_read_kernel<__nv_bfloat16>, grid, block, 0, stream, kc, vc, slots, (__nv_bfloat16*)k, (__nv_bfloat16*)v, nkv,
-                  hd, page_size, num_pages * page_size, by_g, status);
+                  hd, page_size, kv4_page_shift(page_size), num_pages * page_size, by_g, status);
     return gb_check_launch("gb_kv4_read");
 }
 
