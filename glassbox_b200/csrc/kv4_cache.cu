@@ -635,15 +635,24 @@ __global__ void __launch_bounds__(KV4_THREADS) kv4_expand_kernel(const unsigned 
     const int G = hd / KV4_GROUP, per_row = hd / 8;                 // items of a token
     const long long head = page * nkv + h;
     const bool inside = begin >= first && begin + page_size <= end;
-    for (int i = threadIdx.x; i < 2 * page_size * per_row; i += KV4_THREADS) {
-        const bool value = i >= page_size * per_row;
-        const int item = value ? i - page_size * per_row : i, off = by_row.of(item), c = item - off * per_row, t = c & 3, g = c >> 2, r = off % KV4_TILE;
-        const unsigned char* tile = (value ? vcache : kcache) + (head * (page_size / KV4_TILE) + off / KV4_TILE) * kv4_tile_bytes(hd);
-        unsigned short scale = reinterpret_cast<const unsigned short*>(tile + 8 * hd)[r * G + g];
-        if (!inside && (begin + off < first || begin + off >= end) && (scale & 0x7fffu) > 0x7f80u) scale = 0;
+    const unsigned char* const keys = kcache + head * (page_size / KV4_TILE) * kv4_tile_bytes(hd);
+    const unsigned char* const values = vcache + head * (page_size / KV4_TILE) * kv4_tile_bytes(hd);
+#pragma unroll 2
+    for (int i = threadIdx.x; i < page_size * per_row; i += KV4_THREADS) {      // eight channels of a key and of its value
+        const int off = by_row.of(i), c = i - off * per_row, t = c & 3, g = c >> 2, r = off % KV4_TILE;
+        const int tile = off / KV4_TILE * kv4_tile_bytes(hd), scale = tile + 8 * hd + (r * G + g) * 2;
+        const unsigned key = kv4_word(keys + tile, hd, r, g, t, false), value = kv4_word(values + tile, hd, r, g, t, true);
+        unsigned short dk = *reinterpret_cast<const unsigned short*>(keys + scale), dv = *reinterpret_cast<const unsigned short*>(values + scale);
+        if (!inside && (begin + off < first || begin + off >= end)) {
+            if ((dk & 0x7fffu) > 0x7f80u) dk = 0;
+            if ((dv & 0x7fffu) > 0x7f80u) dv = 0;
+        }
+        const size_t to = (size_t)(head * page_size + off) * hd + 8 * c;
         uint32_t x[4];
-        kv4_eight(kv4_word(tile, hd, r, g, t, value), scale, x);
-        kv4_put((value ? v : k) + (head * page_size + off) * hd + 8 * c, x);
+        kv4_eight(key, dk, x);
+        kv4_put(k + to, x);
+        kv4_eight(value, dv, x);
+        kv4_put(v + to, x);
     }
 }
 
