@@ -14,9 +14,10 @@
 
 #include <type_traits>
 
-// Measured (bfloat16, 32/8 heads of 128 of which 64 channels turn, 8,000 rows written and read back, 217 MB): 84 us, of which 65 write; bound by the
-// latency of loads (a third of the stalls) and 58 % of the issue slots. With 64 / 256 threads a block 117 / 87; squeezed into 32 registers, 14 blocks a
-// multiprocessor, 76, but 8 rows 4.8 to 4.2; several rows a block, the next one's numbers asked for ahead (80 registers), 85.
+// Measured (bfloat16, 32/8 heads of 128 of which 64 channels turn, 8,000 rows written and read back, 217 MB): 62 us; without the queries 40, without
+// keys 46, without values 53. Bound by instructions (58 % of the issue slots) and the loads' latency. A thread has two loads or more under way: with one
+// piece of a query a thread and keys and values read back apart it took 84, with two pieces of one head 67. 64 / 256 threads a block took 117 / 87
+// where 128 took 84; 40 registers (12 blocks a multiprocessor) take 72 where 56 take 62.
 constexpr int KV4_THREADS = 128;
 
 template <typename T, int N> struct Kv4Load;      // N neighbouring numbers as float32 (N * sizeof(T) bytes, aligned to 16 or to all of them)
@@ -612,7 +613,7 @@ GB_EXPORT int gb_kv4_read(const void* kcache, const void* vcache, const int* slo
 // Pages of 4 bits that the rows of a step see, as numbers into pages of the same ids: one block a page of a request and kv head.
 // Numbers of tokens outside the request's range (before its first row's window, behind its last row) that are NaN become zero: the
 // kernels that read the pages multiply what they mask by zero. (Of two requests that share a page, a NaN in which lies before the window of one and
-// in sight of the other, either may have its way.) Bound by the latency of a page's few loads: 9 us for 4,096 tokens of 8 heads of 128, 21 MB, 17 of them written.
+// in sight of the other, either may have its way.) Bound by the latency of a page's few loads: 7 us for 4,096 tokens of 8 heads of 128, 21 MB, 17 of them written.
 template <typename T>
 __global__ void __launch_bounds__(KV4_THREADS) kv4_expand_kernel(const unsigned char* __restrict__ kcache, const unsigned char* __restrict__ vcache,
                                                                 T* __restrict__ k, T* __restrict__ v, const int* __restrict__ block_tables, int max_pages,

@@ -12,14 +12,14 @@
 // fewer and fewer as the threshold rises, which it does in tiles 0, 3, 15 ...), and one warp picks the k largest of that. Behind the tile that set it a number
 // has to be larger, since equal ones of higher ids come too late. A row that leaves more than 2,048 candidates (one that only rises, or that holds thousands of
 // equal largest numbers) is searched k times instead.
-// Measured: 2,048 rows of 49,152 float32 (403 MB) with 20 alternatives 90 us, 4.5 TB/s; 1,000 rows of 100,003 bfloat16 that start at odd places, with 5, 66 us.
+// Measured: 2,048 rows of 49,152 float32 (403 MB) with 20 alternatives 89 us, 4.5 TB/s; 1,000 rows of 100,003 bfloat16 that start at odd places, with 5, 62 us.
 // Between loads it is bound by the instructions for sums and exponentials, two exponentials' worth a number.
 #include "common.cuh"
 
 #include <cooperative_groups.h>
 
-// (2,048 rows of 49,152 float32 with 20 alternatives, threads a block and blocks a multiprocessor: 256 and 3 / 4 / 5 107 / 90 / 93 us, 512 and 2
-// 112; without alternatives 67)
+// (2,048 rows of 49,152 float32 with 20 alternatives, threads a block and blocks a multiprocessor: 256 and 3 / 4 / 5 105 / 89 / 92 us, 512 and 2
+// 112; thresholds in tiles 0, 1, 3, 7 ... 90, in the first alone 108; without alternatives 67)
 constexpr int LP_THREADS = 256, LP_WARPS = LP_THREADS / 32;
 constexpr int LP_MAX_TOP = 32;
 constexpr int LP_EACH = 16;             // numbers of a thread and tile
