@@ -2565,7 +2565,8 @@ def kv4_attention_prefill(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tens
                           max_context: int, kpages: torch.Tensor, vpages: torch.Tensor, status: torch.Tensor) -> None:
     """``kv4_attention_decode`` for portions of prompts, runs of consecutive rows of a request: the pages in sight are unpacked into
     kpages/vpages (q's type, [pages, nkv, page_size, hd], numbers everywhere: zero them once) and read from there by the prompt kernel that
-    takes the shape (``kv4_prompt_kernel``); where none does, row by row. ``max_context`` bounds the tokens that a request holds after the
+    takes the shape (``kv4_prompt_kernel``); where none does, row by row. Rows of a padding request come out as zeros or stay as they are, as
+    that kernel has it. ``max_context`` bounds the tokens that a request holds after the
     step. A value that is not a number and that a later row of the portion sees may reach the earlier ones (weight 0 times NaN), as in every prompt
     kernel here. Two calls that may run at the same time need pages of their own to unpack into."""
     n = _kv4_attention(q, out, kcache, vcache, block_tables, row_seq, positions, nh, nkv, hd, page_size, scale)
