@@ -23,8 +23,8 @@
 //
 // What bounds it: issuing instructions, some 450 for 32 keys of a head of 64 and their values (2.4 of 4 a cycle and multiprocessor), not the
 // memory. 64 rows of 32/32 heads of 64 behind 4,096 keys, 605 MB, take 157 us (3.8 TB/s); 2 rows of 32/8 heads of 128 behind 131,072, 302 MB, 87 us.
-// The second without taking codes apart 72, without the second product 63, without copies 80; one multiprocessor's blocks 3 / 4 / 5 of them 90 / 87 /
-// 115, of heads of 64 (the first, in even shares) 4 / 5 / 6 183 / 180 / 189, with one tile a step instead of two 203.
+// The second without taking codes apart 72, without the second product 63, without copies 80; one multiprocessor's blocks 3 / 4 / 5 of them 91 / 87 /
+// 115, of heads of 64 (the first) 4 / 5 / 6 159 / 157 / 165; a ring of five steps 163; in even shares with one tile a step instead of two 180 to 203.
 #include <atomic>
 
 #include "kv4_attention.cuh"
