@@ -21,8 +21,9 @@
 // add up from each other's shared memory, or, behind the longest contexts, all rows' steps cut evenly among the blocks that run at once
 // (kv4_decode_even_kernel). Nothing is left behind for the next call.
 //
-// What bounds it: issuing instructions, some 450 for 32 keys of a head of 64 and their values (2.4 of 4 a cycle and multiprocessor), not the
-// memory. 64 rows of 32/32 heads of 64 behind 4,096 keys, 605 MB, take 157 us (3.8 TB/s); 2 rows of 32/8 heads of 128 behind 131,072, 302 MB, 87 us.
+// What bounds it: issuing instructions, some 430 for 32 keys of a head of 64 and their values (2.4 of 4 a cycle and multiprocessor), not the
+// memory. 64 rows of 32/32 heads of 64 behind 4,096 keys, 605 MB, take 154 us (3.9 TB/s); 2 rows of 32/8 heads of 128 behind 131,072, 302 MB, 86 us
+// (157 and 87 with one float32 where two go into an instruction, which is the form that the next figures are from).
 // The second without taking codes apart 72, without the second product 63, without copies 80; one multiprocessor's blocks 3 / 4 / 5 of them 91 / 87 /
 // 115, of heads of 64 (the first) 4 / 5 / 6 159 / 157 / 165; a ring of five steps 163; in even shares with one tile a step instead of two 180 to 203.
 #include <atomic>
@@ -271,7 +272,7 @@ __device__ __forceinline__ float* kv4_segment(const Kv4AttnArgs& a, unsigned cha
             __syncwarp();
         }
         // ---- scores of keys g and g + 8 of tile x, heads 2 t and 2 t + 1
-        float sc[TILES][2][2];
+        float2 sc[TILES][2];
 #pragma unroll
         for (int x = 0; x < TILES; ++x) {
             uint32_t w[2][G];
@@ -287,9 +288,10 @@ __device__ __forceinline__ float* kv4_segment(const Kv4AttnArgs& a, unsigned cha
                 kv4_mma_from(c, from[k], kv4_up(w[0][k], 0), kv4_up(w[1][k], 0), kv4_up(w[0][k], 1), kv4_up(w[1][k], 1), qf[k][0], qf[k][1]);
                 kv4_mma(c, kv4_up(w[0][k], 2), kv4_up(w[1][k], 2), kv4_up(w[0][k], 3), kv4_up(w[1][k], 3), qf[k][2], qf[k][3]);
 #pragma unroll
-                for (int y = 0; y < 2; ++y)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) sc[x][y][e] = k == 0 ? d[y][k] * c[2 * y + e] : fmaf(d[y][k], c[2 * y + e], sc[x][y][e]);
+                for (int y = 0; y < 2; ++y) {
+                    const float2 both = make_float2(d[y][k], d[y][k]), of = make_float2(c[2 * y], c[2 * y + 1]);
+                    sc[x][y] = k == 0 ? __fmul2_rn(both, of) : __ffma2_rn(both, of, sc[x][y]);
+                }
             }
         }
         if (edge) {
@@ -299,15 +301,16 @@ __device__ __forceinline__ float* kv4_segment(const Kv4AttnArgs& a, unsigned cha
 #pragma unroll
                 for (int y = 0; y < 2; ++y) {
                     const int key = key0 + KV4_TILE * x + 8 * y + g;
-                    if (key < first || key > pos || !(have >> x & 1u)) sc[x][y][0] = sc[x][y][1] = -INFINITY;
+                    if (key < first || key > pos || !(have >> x & 1u)) sc[x][y] = make_float2(-INFINITY, -INFINITY);
                 }
         }
         // ---- weights
-        float most[2] = {fmaxf(sc[0][0][0], sc[0][1][0]), fmaxf(sc[0][0][1], sc[0][1][1])};
+        float most[2] = {fmaxf(sc[0][0].x, sc[0][1].x), fmaxf(sc[0][0].y, sc[0][1].y)};
 #pragma unroll
-        for (int x = 1; x < TILES; ++x)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) most[e] = fmaxf(most[e], fmaxf(sc[x][0][e], sc[x][1][e]));
+        for (int x = 1; x < TILES; ++x) {
+            most[0] = fmaxf(most[0], fmaxf(sc[x][0].x, sc[x][1].x));
+            most[1] = fmaxf(most[1], fmaxf(sc[x][0].y, sc[x][1].y));
+        }
         if (__any_sync(0xffffffffu, fmaf(most[0], scale, -m[0]) > 8.f || fmaf(most[1], scale, -m[1]) > 8.f)) {
             float corr[2];
 #pragma unroll
@@ -333,15 +336,17 @@ __device__ __forceinline__ float* kv4_segment(const Kv4AttnArgs& a, unsigned cha
             uint32_t b[2][G];
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
-                float p[2], d[G];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    p[e] = kv4_exp2(fmaf(sc[x][y][e], scale, -m[e]));
-                    l[e] += p[e];
-                }
+                float d[G];
+                const float2 over = __ffma2_rn(sc[x][y], make_float2(scale, scale), make_float2(-m[0], -m[1]));
+                const float2 p = make_float2(kv4_exp2(over.x), kv4_exp2(over.y)), sum = __fadd2_rn(make_float2(l[0], l[1]), p);
+                l[0] = sum.x;
+                l[1] = sum.y;
                 kv4_scales<G>(dbase + offset + TILE + x * 2 * TILE + y * 8 * G * 2, d);
 #pragma unroll
-                for (int k = 0; k < G; ++k) b[y][k] = kv4_turned(kv4_pack(p[0] * d[k], p[1] * d[k]));
+                for (int k = 0; k < G; ++k) {
+                    const float2 w = __fmul2_rn(p, make_float2(d[k], d[k]));
+                    b[y][k] = kv4_turned(kv4_pack(w.x, w.y));
+                }
             }
             const unsigned char* vr = vbase + offset + x * 2 * TILE;
             uint32_t w[4][(G + 1) / 2];      // half words of the four keys, two groups a word
