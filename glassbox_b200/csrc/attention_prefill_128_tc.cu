@@ -17,6 +17,8 @@
 // and 148 blocks at one in 1,024 cycles each want more than the L2 cache hands out.
 // The mask is applied only in tiles that cross a boundary; key tiles that no row sees are skipped. Page 0 is read in the place of pages that
 // are missing, so that P = 0 meets finite numbers (the pages are zero-initialised).
+// Where blocks are few, a cluster of two or four shares a pair's key tiles; each block leaves O, maxima and sums in its shared memory, over what it has
+// read, and adds up and writes its part of the channels from all of theirs.
 // Every wait is bounded: a wait that runs out sets GB_STATUS_WAIT_TIMEOUT and the block winds down (waits for its own copies, frees its TMEM,
 // returns). TMA loads use no multicast.
 // Measured (2,048 rows behind 2,048 tokens, 32/8 heads, with the unpacking of 7 us): mma.sync 751 us, this kernel 107.
@@ -29,6 +31,9 @@ constexpr int AL_K_OFF = 2 * AL_TILE, AL_V_OFF = AL_K_OFF + AL_KSTAGES * AL_TILE
 constexpr int AL_SMEM = AL_SH_OFF + 512;
 constexpr int AL_O_COL = 2 * AL_BN, AL_TMEM_COLS = 512;
 constexpr float AL_NEG_BIG = -1.0e30f;
+constexpr int AL_MAX_CLUSTER = 4;
+constexpr int AL_STAT_OFF = 2 * AL_BM * AL_HD * 4;      // behind the two units' O as float32
+static_assert(AL_STAT_OFF + 2 * 2 * AL_BM * 4 <= AL_SH_OFF, "a block's results lie over its queries and keys");
 static_assert(AL_SMEM <= 227 * 1024 && AL_O_COL + 2 * AL_HD <= AL_TMEM_COLS, "the block does not fit");
 
 struct __align__(8) AlShared {
@@ -73,6 +78,27 @@ __device__ __forceinline__ void al_store16(uint32_t taddr, const uint32_t (&r)[1
                  : "memory");
 }
 
+// Four channels of a unit's row of O, in an order that keeps the rows of a warp in different banks.
+__device__ __forceinline__ int al_piece(int g, int row, int four) { return ((g * AL_BM + row) * (AL_HD / 4) + (four ^ (row & 31))) * 16; }
+__device__ __forceinline__ void al_cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t al_peer_address(const void* own, int block) {      // where a block of the cluster has what lies here at `own`
+    uint32_t p;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(p) : "r"(smem_u32(own)), "r"(block));
+    return p;
+}
+__device__ __forceinline__ float al_peer(const void* own, int block) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(al_peer_address(own, block)) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 al_peer4(const void* own, int block) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(al_peer_address(own, block)) : "memory");
+    return v;
+}
+
+// CLUSTERS: the blocks of a cluster share a pair's keys. (One form for both costs the other registers: 108.5 us of 107.)
+template <bool CLUSTERS>
 __global__ void __launch_bounds__(AL_WARPS * 32) attention_prefill_128_kernel(
     const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
     __nv_bfloat16* __restrict__ out, long long out_stride, const int* __restrict__ block_tables, int max_pages, const int* __restrict__ seq_first_row,
@@ -86,7 +112,8 @@ __global__ void __launch_bounds__(AL_WARPS * 32) attention_prefill_128_kernel(
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     gb_pdl_wait();
     gb_pdl_launch_dependents();
-    const int kvh = blockIdx.x, seq = blockIdx.y, group = nh / nkv, u0 = 2 * ((int)gridDim.z - 1 - (int)blockIdx.z);      // (the longest blocks start first)
+    const int cluster = CLUSTERS ? gridDim.x / nkv : 1, kvh = blockIdx.x / cluster, rank = blockIdx.x % cluster;      // (all that returns early does so for a whole cluster)
+    const int seq = blockIdx.y, group = nh / nkv, u0 = 2 * ((int)gridDim.z - 1 - (int)blockIdx.z);      // (the longest blocks start first)
     const int row0 = seq_first_row[seq], nrows = seq_first_row[seq + 1] - row0;
     const int q_lo0 = u0 / group * AL_BM, q_lo1 = (u0 + 1) / group * AL_BM;
     if (q_lo0 >= nrows) return;                   // uniform for the block, before anything is allocated
@@ -97,7 +124,7 @@ __global__ void __launch_bounds__(AL_WARPS * 32) attention_prefill_128_kernel(
     }
     const int start_pos = seq_start_pos[seq];
     if (start_pos < 0) {                          // a padding request: its rows read as zeros downstream
-        for (int g = 0; g < units; ++g) {
+        for (int g = 0; g < units && rank == 0; ++g) {
             const int lo = g ? q_lo1 : q_lo0, rows = min(AL_BM, nrows - lo), head = kvh * group + (u0 + g) % group;
             for (int i = tid; i < rows * (AL_HD / 8); i += blockDim.x)
                 *reinterpret_cast<uint4*>(out + (size_t)(row0 + lo + i / (AL_HD / 8)) * out_stride + (size_t)head * AL_HD + i % (AL_HD / 8) * 8) = make_uint4(0, 0, 0, 0);
@@ -106,7 +133,9 @@ __global__ void __launch_bounds__(AL_WARPS * 32) attention_prefill_128_kernel(
     }
     const int* table = block_tables + (size_t)seq * max_pages;
     const int pos_hi = start_pos + min(nrows, (units == 2 ? q_lo1 : q_lo0) + AL_BM) - 1;
-    const int key_lo = gb_first_key(start_pos + q_lo0, window), kt_begin = key_lo / AL_BN, total = pos_hi / AL_BN - kt_begin + 1;
+    const int key_lo = gb_first_key(start_pos + q_lo0, window), all_tiles = pos_hi / AL_BN - key_lo / AL_BN + 1;
+    auto share = [&](int of) { return (int)((long long)all_tiles * of / cluster); };      // where the tiles of the cluster's block `of` begin
+    const int kt_begin = key_lo / AL_BN + share(rank), total = share(rank + 1) - share(rank);
 
     if (tid == 0) {
         mbar_init(&sh.q_full, 1);
@@ -140,7 +169,7 @@ __global__ void __launch_bounds__(AL_WARPS * 32) attention_prefill_128_kernel(
         unsigned char* ring = what == 0 ? Ks : Vs;
         const CUtensorMap* map = what == 0 ? &map_k : &map_v;
         int bad = 0;
-        if (what == 0 && lane == 0) {
+        if (what == 0 && lane == 0 && total > 0) {
             mbar_expect_tx(&sh.q_full, units * AL_TILE);
             for (int g = 0; g < units; ++g) {
                 const int head = kvh * group + (u0 + g) % group, row = row0 + (g ? q_lo1 : q_lo0);
@@ -162,7 +191,7 @@ __global__ void __launch_bounds__(AL_WARPS * 32) attention_prefill_128_kernel(
             }
             return page;
         };
-        long long page = page_of(kt_begin);
+        long long page = total > 0 ? page_of(kt_begin) : 0;
         for (int j = 0; j < total; ++j) {
             const int s = what == 0 ? j % AL_KSTAGES : j % AL_VSTAGES;
             const long long next_page = j + 1 < total ? page_of(kt_begin + j + 1) : 0;      // in flight during the wait
@@ -185,7 +214,7 @@ __global__ void __launch_bounds__(AL_WARPS * 32) attention_prefill_128_kernel(
         if (bad && what == 0) atomicOr(status, GB_STATUS_BAD_SLOT);
     } else if (warp == 1) {
         // ------------------------------------------------------------------------- MMA issuer
-        if (elect_one()) {
+        if (total > 0 && elect_one()) {
             const uint32_t idesc_qk = umma_idesc(AL_BM, AL_BN), idesc_pv = umma_idesc(AL_BM, AL_HD) | (1u << 16);   // (B of the second is MN-major)
             const uint64_t q_desc = umma_desc(smem_u32(Qs)), k_desc = umma_desc(smem_u32(Ks)), v_desc = al_desc_mn(smem_u32(Vs), AL_BLOCK);
             // What a step needs is waited for first; then the last of its weighted sum and the next scores are issued back to back.
@@ -321,9 +350,26 @@ __global__ void __launch_bounds__(AL_WARPS * 32) attention_prefill_128_kernel(
             const float2 lsum = __fadd2_rn(__fadd2_rn(l2[0], l2[1]), __fadd2_rn(l2[2], l2[3]));
             l_run += lsum.x + lsum.y;
         }
-        // O / l, 32 channels at a time, to global memory
-        if (ok) ok = mbar_wait_warp(&sh.pv_done[g][(total - 1) % AL_VSTAGES], ((total - 1) / AL_VSTAGES) & 1, abort_flag, status);
-        if (ok) {
+        if (ok && total > 0) ok = mbar_wait_warp(&sh.pv_done[g][(total - 1) % AL_VSTAGES], ((total - 1) / AL_VSTAGES) & 1, abort_flag, status);
+        if constexpr (CLUSTERS) {
+            // O, maxima and sums to shared memory, where the cluster finds them: over the queries and keys, which both units have to be done with
+            asm volatile("barrier.cta.sync 1, %0;" ::"r"(units * 128) : "memory");
+            if (ok && total > 0) {
+                tc_fence_after();
+#pragma unroll
+                for (int c = 0; c < AL_HD; c += 32) {
+                    uint32_t ov[32];
+                    tmem_load32(lane_base + o_col + (uint32_t)c, ov);
+#pragma unroll
+                    for (int k = 0; k < 32; k += 4)
+                        *reinterpret_cast<uint4*>(al_smem + al_piece(g, r, (c + k) / 4)) = make_uint4(ov[k], ov[k + 1], ov[k + 2], ov[k + 3]);
+                }
+                float* stat = reinterpret_cast<float*>(al_smem + AL_STAT_OFF) + g * 2 * AL_BM;
+                stat[r] = m_run;
+                stat[AL_BM + r] = l_run;
+            }
+        } else if (ok) {
+            // O / l, 32 channels at a time, to global memory
             tc_fence_after();
             const float inv = l_run != 0.f ? 1.0f / l_run : 0.f;
             __nv_bfloat16* dst = out + (size_t)(row0 + q_lo + r) * out_stride + (size_t)(kvh * group + (u0 + g) % group) * AL_HD;
@@ -344,6 +390,54 @@ __global__ void __launch_bounds__(AL_WARPS * 32) attention_prefill_128_kernel(
                 }
             }
         }
+    }
+
+    // ------------------------------------------------------------------------------- the cluster's shares of the keys
+    if constexpr (CLUSTERS) {
+        tc_fence_before();
+        al_cluster_sync();                       // (every block comes here: all waits before are bounded)
+        const int g = (warp - 2) >> 2, r = (warp & 3) * 32 + lane, q_lo = g == 1 ? q_lo1 : q_lo0;
+        if (warp >= 2 && warp < AL_WARPS - 1 && g < units && q_lo + r < nrows) {
+            // each block adds up and writes its part of a row's channels
+            const float sl2 = scale * 1.4426950408889634f;
+            float most = AL_NEG_BIG, sum = 0.f, f[AL_MAX_CLUSTER];
+            bool whole = true;
+#pragma unroll
+            for (int b = 0; b < AL_MAX_CLUSTER; ++b)
+                if (b < cluster) {
+                    whole = whole && __float_as_uint(al_peer(&sh.abort_flag, b)) == 0;
+                    f[b] = share(b + 1) > share(b) ? al_peer(reinterpret_cast<float*>(al_smem + AL_STAT_OFF) + g * 2 * AL_BM + r, b) : AL_NEG_BIG;
+                    most = fmaxf(most, f[b]);
+                }
+#pragma unroll
+            for (int b = 0; b < AL_MAX_CLUSTER; ++b)
+                if (b < cluster) {
+                    f[b] = al_exp2((f[b] - most) * sl2);
+                    if (share(b + 1) > share(b)) sum = fmaf(al_peer(reinterpret_cast<float*>(al_smem + AL_STAT_OFF) + g * 2 * AL_BM + AL_BM + r, b), f[b], sum);
+                }
+            const float inv = sum != 0.f ? 1.0f / sum : 0.f;
+            const int width = AL_HD / cluster, c0 = rank * width;
+            __nv_bfloat16* dst = out + (size_t)(row0 + q_lo + r) * out_stride + (size_t)(kvh * group + (u0 + g) % group) * AL_HD;
+            for (int c = c0; c < c0 + width && whole; c += 8) {
+                float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int b = 0; b < AL_MAX_CLUSTER; ++b)
+                    if (b < cluster && share(b + 1) > share(b))
+#pragma unroll
+                        for (int k = 0; k < 8; k += 4) {
+                            const float4 v = al_peer4(al_smem + al_piece(g, r, (c + k) / 4), b);
+                            o[k] = fmaf(v.x, f[b], o[k]); o[k + 1] = fmaf(v.y, f[b], o[k + 1]);
+                            o[k + 2] = fmaf(v.z, f[b], o[k + 2]); o[k + 3] = fmaf(v.w, f[b], o[k + 3]);
+                        }
+                uint4 w;
+                w.x = pack2(__float_as_uint(o[0] * inv), __float_as_uint(o[1] * inv));
+                w.y = pack2(__float_as_uint(o[2] * inv), __float_as_uint(o[3] * inv));
+                w.z = pack2(__float_as_uint(o[4] * inv), __float_as_uint(o[5] * inv));
+                w.w = pack2(__float_as_uint(o[6] * inv), __float_as_uint(o[7] * inv));
+                *reinterpret_cast<uint4*>(dst + c) = w;
+            }
+        }
+        al_cluster_sync();                       // (shared memory is read until here)
     }
 
     // ------------------------------------------------------------------------------- wind down
@@ -375,7 +469,7 @@ GB_EXPORT int gb_attention_prefill_128_supported(int nh, int nkv, int hd, int pa
 // q, out: bfloat16, rows aligned to 16 bytes; kcache, vcache: [num_pages, nkv, page_size, 128] contiguous.
 GB_EXPORT int gb_attention_prefill_128(const void* q, long long q_stride, int n_rows, void* out, long long out_stride, const void* kcache,
                                        const void* vcache, const int* block_tables, int max_pages, const int* seq_first_row, const int* seq_start_pos,
-                                       int num_seqs, int max_rows_per_seq, int nh, int nkv, int hd, int page_size, long long num_pages, float scale,
+                                       int num_seqs, int max_rows_per_seq, int max_context, int nh, int nkv, int hd, int page_size, long long num_pages, float scale,
                                        int window, int* status, cudaStream_t stream) {
     GB_REQUIRE(gb_attention_prefill_128_supported(nh, nkv, hd, page_size),
                "gb_attention_prefill_128: %d/%d heads of %d in pages of %d (a power of two, 8..128) are not built", nh, nkv, hd, page_size);
@@ -393,12 +487,42 @@ GB_EXPORT int gb_attention_prefill_128(const void* q, long long q_stride, int n_
     if (tc_make_map_2d(&mq, q, n_rows, (long long)nh * hd, q_stride, AL_BM, 64, "gb_attention_prefill_128")) return 1;
     if (tc_make_map_2d(&mk, kcache, num_pages * nkv * page_size, hd, hd, page_size, 64, "gb_attention_prefill_128")) return 1;
     if (tc_make_map_2d(&mv, vcache, num_pages * nkv * page_size, hd, hd, page_size, 64, "gb_attention_prefill_128")) return 1;
-    const cudaError_t e = cudaFuncSetAttribute(attention_prefill_128_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, AL_SMEM);
+    // Few blocks behind many keys leave multiprocessors idle: clusters of two or four blocks then share a pair's keys, three tiles each at least. With
+    // the unpacking, 32/8 heads, in clusters of 1 / 2 / 4: 256 rows behind 16,000 tokens 244 / 145 / 96 us, behind 4,000 73 / 53 / 46, 64 behind 2,000
+    // 41 / 34 / 32, 16 behind 900 23 / 22 / 22; 4/2 heads, 512 behind 4,000 73 / 51 / 41. (Handing over and adding up costs some 8.)
+    const long long blocks = pairs * nkv * num_seqs, reach = window > 0 && window + 2 * AL_BM < max_context ? window + 2 * AL_BM : max_context;
+    int cluster = 1;
+    while (cluster < AL_MAX_CLUSTER && blocks * cluster * 2 <= 148 && reach >= 3 * AL_BN * cluster * 2) cluster *= 2;
+    const auto kernel = cluster > 1 ? attention_prefill_128_kernel<true> : attention_prefill_128_kernel<false>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, AL_SMEM);
     GB_REQUIRE(e == cudaSuccess, "gb_attention_prefill_128: %d bytes of shared memory refused: %s", AL_SMEM, cudaGetErrorString(e));
     int page_shift = 0;
     while ((1 << page_shift) < page_size) ++page_shift;
-    gb_launch(GB_PDL_ATTENTION, attention_prefill_128_kernel, dim3(nkv, num_seqs, (unsigned)pairs), dim3(AL_WARPS * 32), AL_SMEM, stream, mq, mk, mv,
-              (__nv_bfloat16*)out, out_stride, block_tables, max_pages, seq_first_row, seq_start_pos, nh, nkv, page_size, page_shift, num_pages, scale,
-              window, status);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(nkv * cluster, num_seqs, (unsigned)pairs);
+    cfg.blockDim = dim3(AL_WARPS * 32);
+    cfg.dynamicSmemBytes = AL_SMEM;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    int na = 0;
+    if (gb_pdl_enabled() & GB_PDL_ATTENTION) {
+        attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[na].val.programmaticStreamSerializationAllowed = 1;
+        ++na;
+    }
+    if (cluster > 1) {
+        attr[na].id = cudaLaunchAttributeClusterDimension;
+        attr[na].val.clusterDim.x = cluster;
+        attr[na].val.clusterDim.y = attr[na].val.clusterDim.z = 1;
+        ++na;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = na;
+    const cudaError_t launched = cudaLaunchKernelEx(&cfg, kernel, mq, mk, mv, (__nv_bfloat16*)out, out_stride, block_tables, max_pages,
+                                                    seq_first_row, seq_start_pos, nh, nkv, page_size, page_shift, num_pages, scale, window, status);
+    if (launched != cudaSuccess) {
+        gb_set_error("gb_attention_prefill_128: launch failed: %s", cudaGetErrorString(launched));
+        return 2;
+    }
     return gb_check_launch("gb_attention_prefill_128");
 }

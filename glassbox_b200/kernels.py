@@ -178,7 +178,7 @@ _SIGNATURES = {
     "gb_kv4_attention_rows": [_P, _LL, _P, _LL, _I, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _LL, _F, _I, _I, _P, _P, _P],
     "gb_kv4_attention_decode": [_P, _LL, _P, _LL, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _LL, _F, _I, _I, _I, _P, _P, _P],
     "gb_attention_prefill_128_supported": [_I, _I, _I, _I],
-    "gb_attention_prefill_128": [_P, _LL, _I, _P, _LL, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _LL, _F, _I, _P, _P],
+    "gb_attention_prefill_128": [_P, _LL, _I, _P, _LL, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _LL, _F, _I, _P, _P],
     "gb_kv4_attention_decode_supported": [_I],
     "gb_kv4_attention_decode_blocks": [_I, _I, _I, _I, _LL],
     "gb_token_logprobs": [_P, _I, _LL, _P, _P, _P, _P, _P, _I, _I, _I, _P],
@@ -2545,7 +2545,9 @@ def kv4_expand(kcache: torch.Tensor, vcache: torch.Tensor, kpages: torch.Tensor,
 
 
 def kv4_prompt_kernel(q: torch.Tensor, out: torch.Tensor, nh: int, nkv: int, hd: int, page_size: int) -> Optional[str]:
-    """Which kernel over unpacked pages takes portions of prompts of this shape; None: there is none that works on tiles of rows."""
+    """Which kernel over unpacked pages takes portions of prompts of this shape; None: there is none that works on tiles of rows. Where two do,
+    "tcgen05" and "tcgen05_128" come before "mma": at head size 128, 32/8 heads, with the unpacking, 300 rows of four requests behind 100 tokens 31 to
+    73 us, 256 rows behind 4,000 46 to 142, 16 behind 500 18 to 24; 5 rows alone 9.9 to 8.5, the one size where it loses."""
     if attention_prefill_tc_supported(q, out, nh, nkv, hd, page_size):
         return "tcgen05"
     if attention_prefill_f32_supported(q, out, nh, nkv, hd):
@@ -2587,7 +2589,8 @@ def kv4_attention_prefill(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tens
     elif kind == "tcgen05_128":
         _call("gb_attention_prefill_128", q.data_ptr(), q.stride(0), n, out.data_ptr(), out.stride(0), kpages.data_ptr(), vpages.data_ptr(),
               block_tables.data_ptr(), block_tables.shape[1], seq_first_row.data_ptr(), seq_start_pos.data_ptr(), block_tables.shape[0],
-              int(max_rows_per_seq), nh, nkv, hd, page_size, kpages.shape[0], float(scale), int(window or 0), status.data_ptr(), stream)
+              int(max_rows_per_seq), min(int(max_context), 1 << 30), nh, nkv, hd, page_size, kpages.shape[0], float(scale), int(window or 0),
+              status.data_ptr(), stream)
     elif kind == "tiles":
         sink_attention_tiles(q, out, kpages, vpages, block_tables, seq_first_row, seq_start_pos, max_rows_per_seq, r1=None, r2=None, sink=None,
                              gate=None, heads=nh, kv_heads=nkv, dim=hd, vdim=hd, page_size=page_size, scale=scale, window=window, status=status)

@@ -56,7 +56,10 @@ PROMPTS = [  # nh, nkv, hd, page size, window, (rows, tokens before) of the requ
     (4, 4, 128, 16, None, [(300, 0), (129, 200), None, (1, 511)]), (6, 2, 128, 32, 150, [(257, 70), (128, 1), (130, 300)]),
     (5, 1, 128, 128, None, [(140, 33), (260, 0)]), (3, 3, 128, 16, 1, [(200, 5), (3, 0)]), (8, 1, 128, 8 * 16, 129, [(127, 129), (385, 0)]),
     (7, 1, 64, 16, None, [(300, 0), None, (129, 200)]), (2, 1, 256, 16, 100, [(140, 33)]), (3, 1, 160, 48, None, [(40, 100), (1, 0)]),
-    (2, 2, 128, 48, None, [(150, 20)]), (2, 2, 128, 256, 40, [(150, 20)])]
+    (2, 2, 128, 48, None, [(150, 20)]), (2, 2, 128, 256, 40, [(150, 20)]),
+    # few blocks behind many keys, which clusters share: all of four, one tile of a request that is short, a window, a row behind its last tile
+    (8, 2, 128, 16, None, [(200, 3000)]), (4, 2, 128, 32, None, [(5, 0), None, (130, 2500), (1, 1700)]), (6, 2, 128, 16, 900, [(256, 4000), (128, 0)]),
+    (3, 1, 128, 64, None, [(257, 1664), (1, 1535)]), (1, 1, 128, 16, None, [(129, 800)])]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
