@@ -15,8 +15,8 @@
 // 1,024 cycles of the tensor core and the 16,384 exponentials as many of the unit that forms them; the two units keep both busy in turn. One
 // unit a block (its key tiles in two interleaved chains) took 137 us with the unpacking below where this took 113: a tile of keys and values is 64 KB,
 // and 148 blocks at one in 1,024 cycles each want more than the L2 cache hands out.
-// The mask is applied only in tiles that cross a boundary; key tiles that no row sees are skipped. Page 0 is read in the place of pages that
-// are missing, so that P = 0 meets finite numbers (the pages are zero-initialised).
+// The mask is applied only in tiles that cross a boundary; key tiles that no row sees are skipped. Zeros stand in the place of pages that no row of the
+// block sees (behind its last row, before its window) or that are missing, so that P = 0 meets numbers whatever lies in other pages.
 // Where blocks are few, a cluster of two or four shares a pair's key tiles; each block leaves O, maxima and sums in its shared memory, over what it has
 // read, and adds up and writes its part of the channels from all of theirs.
 // Every wait is bounded: a wait that runs out sets GB_STATUS_WAIT_TIMEOUT and the block winds down (waits for its own copies, frees its TMEM,
@@ -168,6 +168,7 @@ __global__ void __launch_bounds__(AL_WARPS * 32) attention_prefill_128_kernel(
         uint64_t* full = what == 0 ? sh.k_full : sh.v_full;
         unsigned char* ring = what == 0 ? Ks : Vs;
         const CUtensorMap* map = what == 0 ? &map_k : &map_v;
+        const int nowhere = (int)(num_pages * nkv * page_size);
         int bad = 0;
         if (what == 0 && lane == 0 && total > 0) {
             mbar_expect_tx(&sh.q_full, units * AL_TILE);
@@ -178,23 +179,20 @@ __global__ void __launch_bounds__(AL_WARPS * 32) attention_prefill_128_kernel(
             }
             sh.q_issued = 1;
         }
-        auto page_of = [&](int kt) -> long long {      // this lane's page of key tile kt: lanes 2 i and 2 i + 1 have page i
-            long long page = 0;
-            if (lane < 2 * ppt) {
-                const int pi = ((kt * AL_BN) >> page_shift) + (lane >> 1);
-                page = pi < max_pages ? table[pi] : -1;
-                if (page < 0 || page >= num_pages) {
-                    const int first = pi << page_shift, last = first + page_size - 1;      // only a page that holds a key some row can see is missed
-                    if (first <= pos_hi && last >= key_lo) bad = 1;
-                    page = 0;
-                }
-            }
-            return page;
+        // The first row of this lane's page of key tile kt (lanes 2 i and 2 i + 1 have page i). A page that no row of the block sees, or that is missing,
+        // lies behind all pages, where a copy reads zeros: what other requests, or earlier steps, left in a page must not meet a weight of zero.
+        auto row_of = [&](int kt) -> int {
+            const int pi = ((kt * AL_BN) >> page_shift) + (lane >> 1), first = pi << page_shift;
+            if (lane >= 2 * ppt || first > pos_hi || first + page_size <= key_lo) return nowhere;
+            const long long page = pi < max_pages ? table[pi] : -1;
+            if (page >= 0 && page < num_pages) return (int)((page * nkv + kvh) * page_size);
+            bad = 1;
+            return nowhere;
         };
-        long long page = total > 0 ? page_of(kt_begin) : 0;
+        int row = total > 0 ? row_of(kt_begin) : nowhere;
         for (int j = 0; j < total; ++j) {
             const int s = what == 0 ? j % AL_KSTAGES : j % AL_VSTAGES;
-            const long long next_page = j + 1 < total ? page_of(kt_begin + j + 1) : 0;      // in flight during the wait
+            const int next_row = j + 1 < total ? row_of(kt_begin + j + 1) : nowhere;      // in flight during the wait
             int ok = 1;
             if (lane == 0) {      // a stage is free when the last product of the tile that was in it is done
                 if (what == 0 && j >= AL_KSTAGES) ok = mbar_wait(&sh.s_full[units - 1][s], (j / AL_KSTAGES - 1) & 1, abort_flag, status) ? 1 : 0;
@@ -205,11 +203,10 @@ __global__ void __launch_bounds__(AL_WARPS * 32) attention_prefill_128_kernel(
             if (lane == 0) mbar_expect_tx(&full[s], AL_TILE);
             __syncwarp();
             if (lane < 2 * ppt)
-                tma_load_2d(ring + s * AL_TILE + (lane & 1) * AL_BLOCK + (lane >> 1) * page_size * 128, map, &full[s], (lane & 1) * 64,
-                            (int)((page * nkv + kvh) * page_size));
+                tma_load_2d(ring + s * AL_TILE + (lane & 1) * AL_BLOCK + (lane >> 1) * page_size * 128, map, &full[s], (lane & 1) * 64, row);
             __syncwarp();
             if (lane == 0) sh.issued[what] = j + 1;
-            page = next_page;
+            row = next_row;
         }
         if (bad && what == 0) atomicOr(status, GB_STATUS_BAD_SLOT);
     } else if (warp == 1) {

@@ -31,9 +31,8 @@
 // A query at position p sees keys max(0, p-window+1) .. p (crates/glassbox-core/src/model.rs:278-317), or, window < 0, the
 // keys of its own chunk of -window positions up to p;
 // the mask is applied only in tiles that cross a boundary, and key tiles no row can see are skipped.
-// Pages that are missing (beyond what is reserved, or given back behind a window) can only hold
-// masked keys; page 0 is read in their place, so that P = 0 never meets anything but finite numbers
-// (the cache is zero-initialised and only ever holds finite values).
+// Pages that are missing (beyond what is reserved, or given back behind a window) can only hold masked keys; zeros stand in the
+// place of these and of pages that no row of the block sees, so that P = 0 meets numbers whatever lies in other pages.
 //
 // Every wait is bounded: a wait that exceeds its limit sets GB_STATUS_WAIT_TIMEOUT in the status
 // word and the block winds down (waits, again bounded, for its own TMA copies, frees its TMEM,
@@ -277,6 +276,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32) attention_prefill_tc_kernel(
         // stages free again) earlier than values, so the two rings run at their own pace
         const int what = warp == 0 ? 0 : 1;
         const int ppt = AT_BN >> page_shift;   // pages per key tile (1 .. 16)
+        const int nowhere = (int)(num_pages * nkv * page_size);
         int bad = 0;
         uint64_t* full = what == 0 ? sh.k_full : sh.v_full;
         uint64_t* empty = what == 0 ? sh.k_empty : sh.v_empty;
@@ -293,24 +293,20 @@ __global__ void __launch_bounds__(AT_WARPS * 32) attention_prefill_tc_kernel(
                 tma_load_2d(Qs + item * G::Q_BYTES, &map_q, &sh.q_full[item], head * HD, row0 + it.q_lo);
                 sh.q_issued = item + 1;
             }
-            auto page_of = [&](int kt) -> long long {   // this lane's page of key tile kt
-                long long page = 0;
-                if (lane < ppt) {
-                    const int pi = ((kt * AT_BN) >> page_shift) + lane;
-                    page = pi < max_pages ? table[pi] : -1;
-                    if (page < 0 || page >= num_pages) {
-                        // only a page that holds a key some row can see is missed
-                        const int first = pi << page_shift, last = first + page_size - 1;
-                        if (first <= it.pos_hi && last >= it.key_lo) bad = 1;
-                        page = 0;
-                    }
-                }
-                return page;
+            // The first row of this lane's page of key tile kt. A page that no row of the block sees, or that is missing, lies behind all
+            // pages, where a copy reads zeros: what other requests, or earlier steps, left in a page must not meet a weight of zero.
+            auto row_of = [&](int kt) -> int {
+                const int pi = ((kt * AT_BN) >> page_shift) + lane, first = pi << page_shift;
+                if (lane >= ppt || first > it.pos_hi || first + page_size <= it.key_lo) return nowhere;
+                const long long page = pi < max_pages ? table[pi] : -1;
+                if (page >= 0 && page < num_pages) return (int)((page * nkv + kvh) * page_size);
+                bad = 1;
+                return nowhere;
             };
-            long long page = page_of(it.kt_begin);
+            int row = row_of(it.kt_begin);
             for (int t = 0; t < it.ntiles; ++t, ++j) {
                 const int s = j % AT_STAGES;
-                const long long next_page = t + 1 < it.ntiles ? page_of(it.kt_begin + t + 1) : 0;   // in flight during the wait
+                const int next_row = t + 1 < it.ntiles ? row_of(it.kt_begin + t + 1) : nowhere;   // in flight during the wait
                 int ok = 1;
                 if (lane == 0 && j >= AT_STAGES)
                     ok = mbar_wait(&empty[s], ((j / AT_STAGES) - 1) & 1, abort_flag, status) ? 1 : 0;
@@ -318,13 +314,10 @@ __global__ void __launch_bounds__(AT_WARPS * 32) attention_prefill_tc_kernel(
                 if (!ok) { go = false; break; }
                 if (lane == 0) mbar_expect_tx(&full[s], G::KV_BYTES);
                 __syncwarp();
-                if (lane < ppt) {
-                    const int row = (int)((page * nkv + kvh) * page_size);
-                    tma_load_2d(ring + s * G::KV_BYTES + lane * page_size * HD * 2, map, &full[s], 0, row);
-                }
+                if (lane < ppt) tma_load_2d(ring + s * G::KV_BYTES + lane * page_size * HD * 2, map, &full[s], 0, row);
                 __syncwarp();
                 if (lane == 0) sh.issued[what] = j + 1;
-                page = next_page;
+                row = next_row;
             }
         }
         if (bad && what == 0) atomicOr(status, GB_STATUS_BAD_SLOT);

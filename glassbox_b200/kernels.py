@@ -2566,11 +2566,11 @@ def kv4_attention_prefill(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tens
                           max_rows_per_seq: int, nh: int, nkv: int, hd: int, page_size: int, scale: float, window: Optional[int],
                           max_context: int, kpages: torch.Tensor, vpages: torch.Tensor, status: torch.Tensor) -> None:
     """``kv4_attention_decode`` for portions of prompts, runs of consecutive rows of a request: the pages in sight are unpacked into
-    kpages/vpages (q's type, [pages, nkv, page_size, hd], numbers everywhere: zero them once) and read from there by the prompt kernel that
+    kpages/vpages (q's type, [pages, nkv, page_size, hd], whatever they hold) and read from there by the prompt kernel that
     takes the shape (``kv4_prompt_kernel``); where none does, row by row. Rows of a padding request come out as zeros or stay as they are, as
     that kernel has it. ``max_context`` bounds the tokens that a request holds after the
-    step. A value that is not a number and that a later row of the portion sees may reach the earlier ones (weight 0 times NaN), as in every prompt
-    kernel here. Two calls that may run at the same time need pages of their own to unpack into."""
+    step. A value that is not a number and that one row of a portion sees may reach other rows of the portion (weight 0 times NaN), as in every prompt
+    kernel here, and no other request's. Two calls that may run at the same time need pages of their own to unpack into."""
     n = _kv4_attention(q, out, kcache, vcache, block_tables, row_seq, positions, nh, nkv, hd, page_size, scale)
     if not (kpages.dtype == q.dtype and kpages.shape[1:] == (nkv, page_size, hd)):
         raise KernelError(f"kpages must be {q.dtype} [pages, {nkv}, {page_size}, {hd}]")
