@@ -9,7 +9,7 @@
 // reciprocal and one correction by the remainder (exact in a fused multiply-add), so that a number half way between two codes is told as such:
 // with bfloat16 values that is one in dozens, and ties go to the even code. A rotated key is a float32 product off by some 2^-23; where that
 // could change a code or the scale (one group in some 10^4) the group is held once more from two float32 a number, so that what
-// is stored is always what the exact rotation gives.
+// is stored is what the exact rotation gives wherever that is not nearer than some 2^-46 of a pair's size to a border.
 #include "kv4.cuh"
 
 #include <type_traits>
@@ -190,13 +190,15 @@ __device__ __forceinline__ unsigned kv4_codes_bf16(const float (&y)[N], float d)
 
 // A turned key as the sum of two float32, the first the nearest to the sum (what a float32 rounding would drop decides which code a number
 // next to a border between two gets, and which scale): products with their errors by fused multiply-add, the sum with its error as Knuth's
-// (The Art of Computer Programming 2, 4.2.2). x the channel's own number, o its partner's.
+// (The Art of Computer Programming 2, 4.2.2). Each operation is named, so that the compiler cannot fuse a product into the sum whose error is
+// taken behind it. What is left out is the roundings of the errors' sum, some 2^-46 of the pair's size. x the channel's own number, o its partner's.
 __device__ __forceinline__ void kv4_turn2(float& x, float& lo, float o, float2 cs, bool second) {
     o = second ? o : -o;
-    const float p = x * cs.x, q = o * cs.y, h = p + q, b = h - p;
-    const float l = ((p - (h - b)) + (q - b)) + (fmaf(x, cs.x, -p) + fmaf(o, cs.y, -q));
-    x = h + l;
-    lo = l - (x - h);
+    const float p = __fmul_rn(x, cs.x), q = __fmul_rn(o, cs.y), h = __fadd_rn(p, q), b = __fsub_rn(h, p);
+    const float rest = __fadd_rn(__fsub_rn(p, __fsub_rn(h, b)), __fsub_rn(q, b));
+    const float l = __fadd_rn(rest, __fadd_rn(__fmaf_rn(x, cs.x, -p), __fmaf_rn(o, cs.y, -q)));
+    x = __fadd_rn(h, l);
+    lo = __fsub_rn(l, __fsub_rn(x, h));
 }
 
 // The key whose maximum over a group names its m, of such numbers: the first part's magnitude, then how far the second goes beyond it, "not
