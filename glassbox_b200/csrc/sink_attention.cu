@@ -341,8 +341,8 @@ constexpr float SK_LOG2E = 1.4426950408889634f;
 // (three blocks on a multiprocessor where their shared memory allows it: the registers must then fit as well)
 template <int D, int V, bool CAP>
 __global__ void __launch_bounds__(128, D + V <= 192 ? 3 : 2) sink_attention_tiles_kernel(
-    const __nv_bfloat16* __restrict__ q, __nv_bfloat16* __restrict__ out, const __nv_bfloat16* __restrict__ kcache,
-    const __nv_bfloat16* __restrict__ vcache, const int* __restrict__ block_tables, int max_pages, const int* __restrict__ seq_first_row,
+    const __nv_bfloat16* __restrict__ q, long long q_stride, __nv_bfloat16* __restrict__ out, long long out_stride,
+    const __nv_bfloat16* __restrict__ kcache, const __nv_bfloat16* __restrict__ vcache, const int* __restrict__ block_tables, int max_pages, const int* __restrict__ seq_first_row,
     const int* __restrict__ seq_start_pos, const float* __restrict__ r1, const float* __restrict__ r2, const float* __restrict__ sink,
     const float* __restrict__ gate, long long ld_gate, int num_seqs, int tiles_per_seq, int H, int G, int page_size, long long num_pages,
     float scale, float cap, int mask, int gate_channels, int* __restrict__ status) {
@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(128, D + V <= 192 ? 3 : 2) sink_attention_tile
     // Q tile
     for (int chunk = tid; chunk < SKT_BM * (D / 8); chunk += 128) {
         const int r = chunk / (D / 8), c = (chunk % (D / 8)) * 8;
-        sat_cp16(sq + r * LDK + c, q + ((size_t)(row0 + (r < rows ? r : 0)) * H + head) * D + c, r < rows);
+        sat_cp16(sq + r * LDK + c, q + (size_t)(row0 + (r < rows ? r : 0)) * q_stride + (size_t)head * D + c, r < rows);
     }
     // Where the keys of a tile lie is looked up a tile ahead of its loads, one key per thread, and kept in shared memory; the
     // loads then go piece by piece along the rows (the key row, then the value row), so that neighbouring lanes fetch
@@ -552,7 +552,7 @@ __global__ void __launch_bounds__(128, D + V <= 192 ? 3 : 2) sink_attention_tile
         if (r >= rows) continue;
         float f = den > 0.f ? 1.0f / den : 0.f;
         if (gate && !gate_channels) f *= sk_sigmoid(gate[(size_t)(row0 + r) * ld_gate + head]);
-        __nv_bfloat16* dst = out + ((size_t)(row0 + r) * H + head) * V;
+        __nv_bfloat16* dst = out + (size_t)(row0 + r) * out_stride + (size_t)head * V;
 #pragma unroll
         for (int j = 0; j < V / 8; ++j) {
             float a = o[j][half * 2] * f, b = o[j][half * 2 + 1] * f;
@@ -571,22 +571,23 @@ GB_EXPORT int gb_sink_attention_tiles_supported(int D, int V) {
 }
 
 template <int D, int V>
-static int skt_launch(const void* q, void* out, const void* kcache, const void* vcache, const int* block_tables, int max_pages,
-                      const int* seq_first_row, const int* seq_start_pos, const float* r1, const float* r2, const float* sink,
+static int skt_launch(const void* q, long long q_stride, void* out, long long out_stride, const void* kcache, const void* vcache,
+                      const int* block_tables, int max_pages, const int* seq_first_row, const int* seq_start_pos, const float* r1, const float* r2, const float* sink,
                       const float* gate, long long ld_gate, int num_seqs, int tiles_per_seq, int H, int G, int page_size,
                       long long num_pages, float scale, float cap, int mask, int gate_channels, int* status, cudaStream_t stream) {
     const size_t smem = ((size_t)3 * SKT_BM * (D + 8) + (size_t)2 * SKT_BN * (V + 8)) * 2;
     auto kernel = cap > 0.f ? sink_attention_tiles_kernel<D, V, true> : sink_attention_tiles_kernel<D, V, false>;
     cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     gb_launch(GB_PDL_ATTENTION, kernel, dim3(num_seqs * tiles_per_seq, H), dim3(128), smem, stream,
-              (const __nv_bfloat16*)q, (__nv_bfloat16*)out, (const __nv_bfloat16*)kcache, (const __nv_bfloat16*)vcache, block_tables,
-              max_pages, seq_first_row, seq_start_pos, r1, r2, sink, gate, ld_gate, num_seqs, tiles_per_seq, H, G, page_size, num_pages,
+              (const __nv_bfloat16*)q, q_stride, (__nv_bfloat16*)out, out_stride, (const __nv_bfloat16*)kcache,
+              (const __nv_bfloat16*)vcache, block_tables, max_pages, seq_first_row, seq_start_pos, r1, r2, sink, gate, ld_gate, num_seqs, tiles_per_seq, H, G, page_size, num_pages,
               scale, cap, mask, gate_channels, status);
     return gb_check_launch("gb_sink_attention_tiles");
 }
 
-GB_EXPORT int gb_sink_attention_tiles(const void* q, void* out, const void* kcache, const void* vcache, const int* block_tables,
-                                      int max_pages, const int* seq_first_row, const int* seq_start_pos, const float* r1, const float* r2,
+// Rows of q and out q_stride and out_stride numbers apart.
+GB_EXPORT int gb_sink_attention_tiles(const void* q, long long q_stride, void* out, long long out_stride, const void* kcache,
+                                      const void* vcache, const int* block_tables, int max_pages, const int* seq_first_row, const int* seq_start_pos, const float* r1, const float* r2,
                                       const float* sink, const float* gate, long long ld_gate, int num_seqs, int max_rows_per_seq, int H,
                                       int G, int D, int V, int page_size, long long num_pages, float scale, float cap, int mask, int gate_channels,
                                       int* status, cudaStream_t stream) {
@@ -594,12 +595,14 @@ GB_EXPORT int gb_sink_attention_tiles(const void* q, void* out, const void* kcac
     SK_COMMON_CHECKS("gb_sink_attention_tiles")
     GB_REQUIRE(gb_sink_attention_tiles_supported(D, V), "gb_sink_attention_tiles: head sizes %d / %d are not built", D, V);
     GB_REQUIRE(max_rows_per_seq > 0, "gb_sink_attention_tiles: bad sizes");
+    GB_REQUIRE(q_stride % 8 == 0 && (uintptr_t)q % 16 == 0 && out_stride % 2 == 0 && (uintptr_t)out % 4 == 0,
+               "gb_sink_attention_tiles: rows of q must be 16-byte aligned, rows of out 4-byte aligned");
     if (num_seqs == 0) return 0;
     const int tiles = gb_ceil_div(max_rows_per_seq, SKT_BM);
 #define SKT_CASE(DD, VV)                                                                                                              \
     if (D == DD && V == VV)                                                                                                           \
-        return skt_launch<DD, VV>(q, out, kcache, vcache, block_tables, max_pages, seq_first_row, seq_start_pos, r1, r2, sink, gate,   \
-                                  ld_gate, num_seqs, tiles, H, G, page_size, num_pages, scale, cap, mask, gate_channels, status, stream);
+        return skt_launch<DD, VV>(q, q_stride, out, out_stride, kcache, vcache, block_tables, max_pages, seq_first_row, seq_start_pos,  \
+                                  r1, r2, sink, gate, ld_gate, num_seqs, tiles, H, G, page_size, num_pages, scale, cap, mask, gate_channels, status, stream);
     SKT_CASE(32, 32) SKT_CASE(32, 64) SKT_CASE(32, 128) SKT_CASE(64, 32) SKT_CASE(64, 64) SKT_CASE(64, 128) SKT_CASE(128, 32)
     SKT_CASE(128, 64) SKT_CASE(128, 128) SKT_CASE(48, 48) SKT_CASE(80, 80) SKT_CASE(96, 96)
 #undef SKT_CASE

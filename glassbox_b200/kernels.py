@@ -149,7 +149,7 @@ _SIGNATURES = {
     "gb_sink_attention_decode": [_P, _P, _I, _P, _P, _P, _I, _P, _P, _P, _P, _P, _P, _LL, _I, _I, _I, _I, _I, _I, _LL, _F, _F, _I, _I, _P, _P],
     "gb_sink_attention_decode_supported": [_I],
     "gb_sink_attention_tiles_supported": [_I, _I],
-    "gb_sink_attention_tiles": [_P, _P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _P, _LL, _I, _I, _I, _I, _I, _I, _I, _LL, _F, _F, _I, _I, _P, _P],
+    "gb_sink_attention_tiles": [_P, _LL, _P, _LL, _P, _P, _P, _I, _P, _P, _P, _P, _P, _P, _LL, _I, _I, _I, _I, _I, _I, _I, _LL, _F, _F, _I, _I, _P, _P],
     "gb_sigmoid_attention_rows": [_P, _P, _I, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _LL, _F, _I, _P, _P],
     "gb_sigmoid_attention_decode": [_P, _P, _I, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _LL, _F, _I, _P, _P],
     "gb_sigmoid_attention_decode_supported": [_I],
@@ -2043,15 +2043,16 @@ def sink_attention_tiles(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tenso
                          window: Optional[int], status: torch.Tensor, softcap: Optional[float] = None,
                          chunk: Optional[int] = None) -> None:
     """``sink_attention_rows`` for runs of consecutive rows (prompt portions) in bfloat16 on the tensor cores: a block
-    takes 64 rows of one request and one head; ``max_rows_per_seq`` bounds the rows a request brings (it sizes the grid)."""
+    takes 64 rows of one request and one head; ``max_rows_per_seq`` bounds the rows a request brings (it sizes the grid). Rows of q
+    and out may be strided (q in eights of numbers)."""
     _cuda(q, out, kcache, vcache, block_tables, seq_first_row, seq_start_pos, r1, r2, sink, gate, status)
     n = q.shape[0]
     assert q.dtype == out.dtype == kcache.dtype == vcache.dtype == torch.bfloat16
-    assert q.shape == (n, heads * dim) and out.shape == (n, heads * vdim) and q.is_contiguous() and out.is_contiguous()
+    assert q.shape == (n, heads * dim) and out.shape == (n, heads * vdim) and q.stride(1) == 1 and out.stride(1) == 1
     assert block_tables.is_contiguous() and seq_first_row.shape[0] == seq_start_pos.shape[0] + 1
     terms, by_channel = _sink_args(r1, r2, sink, gate, heads, vdim)
-    _call("gb_sink_attention_tiles", _ptr(q), _ptr(out), _ptr(kcache), _ptr(vcache), _ptr(block_tables), block_tables.shape[1],
-          _ptr(seq_first_row), _ptr(seq_start_pos), *terms, seq_start_pos.shape[0],
+    _call("gb_sink_attention_tiles", _ptr(q), q.stride(0) if n > 1 else q.shape[1], _ptr(out), out.stride(0) if n > 1 else out.shape[1], _ptr(kcache),
+          _ptr(vcache), _ptr(block_tables), block_tables.shape[1], _ptr(seq_first_row), _ptr(seq_start_pos), *terms, seq_start_pos.shape[0],
           max(int(max_rows_per_seq), 1), heads, kv_heads, dim, vdim, page_size, kcache.shape[0], float(scale),
           float(softcap or 0.0), _mask(window, chunk), by_channel, _ptr(status), _stream())
 
@@ -2544,10 +2545,18 @@ def kv4_expand(kcache: torch.Tensor, vcache: torch.Tensor, kpages: torch.Tensor,
           kcache.shape[0], int(window or 0), status.data_ptr(), stream)
 
 
+#: from so many blocks of the decode kernel on (20 a multiprocessor) prompts of the head sizes that only ``sink_attention_tiles`` takes go through it
+KV4_TILES_FROM = 20 * 148
+
+
 def kv4_prompt_kernel(q: torch.Tensor, out: torch.Tensor, nh: int, nkv: int, hd: int, page_size: int) -> Optional[str]:
-    """Which kernel over unpacked pages takes portions of prompts of this shape; None: there is none that works on tiles of rows. Where two do,
-    "tcgen05" and "tcgen05_128" come before "mma": at head size 128, 32/8 heads, with the unpacking, 300 rows of four requests behind 100 tokens 31 to
-    73 us, 256 rows behind 4,000 46 to 142, 16 behind 500 18 to 24; 5 rows alone 9.9 to 8.5, the one size where it loses."""
+    """Which kernel over unpacked pages takes portions of prompts of this shape; None: none that works on tiles of rows, or none that would
+    be faster than the decode kernel row by row. Where two do, "tcgen05" and "tcgen05_128" come before "mma": at head size 128, 32/8 heads, with the
+    unpacking, 300 rows of four requests behind 100 tokens 31 to 73 us, 256 rows behind 4,000 46 to 142, 16 behind 500 18 to 24; 5 rows alone 9.9
+    to 8.5, the one size where it loses. "tiles" (bfloat16 heads of 32 and 96, and of 64 and 128 in pages of other sizes) walks through all keys in each of
+    few blocks; the decode kernel reads them for every row and eight heads, in many. Tiles / row by row, us, with the unpacking: heads of 96, 8/2 of them, 64 rows
+    behind 2,000 tokens 131 / 17, 1,024 181 / 150, 2,048 238 / 343; 32/8, 512 rows 158 / 259; 12/12, 512 rows 156 / 380; heads of 32, 9/3, 1,024 106 / 99, 2,048
+    138 / 226; 32/8, 512 rows 92 / 117; heads of 128 in pages of 48, 32/8, 512 rows 130 / 304, 256 (row by row by the rule) 112 / 149."""
     if attention_prefill_tc_supported(q, out, nh, nkv, hd, page_size):
         return "tcgen05"
     if attention_prefill_f32_supported(q, out, nh, nkv, hd):
@@ -2558,7 +2567,8 @@ def kv4_prompt_kernel(q: torch.Tensor, out: torch.Tensor, nh: int, nkv: int, hd:
         return "tcgen05_128"
     if attention_prefill_supported(q.dtype, nh, nkv, hd, page_size):
         return "mma"
-    return "tiles" if q.is_contiguous() and out.is_contiguous() and sink_attention_tiles_supported(q.dtype, hd, hd) else None
+    few = q.shape[0] * nkv * -(-(nh // nkv) // KV4_MMA_HEADS) < KV4_TILES_FROM and lib().gb_kv4_attention_decode_supported(hd)
+    return "tiles" if not few and sink_attention_tiles_supported(q.dtype, hd, hd) else None
 
 
 def kv4_attention_prefill(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, block_tables: torch.Tensor,
