@@ -110,7 +110,9 @@ class LLM:
         try:
             for a in range(0, len(tokens) - 1, engine.max_batch_tokens):
                 part = tokens[a:min(a + engine.max_batch_tokens, len(tokens) - 1)]
-                logits = engine.step([StepEntry(rid, part, list(range(len(part))))])
+                # (texts come in every length: portions of 64 rows, 128 and so on, so that few shapes are recorded)
+                room = min(engine.max_batch_tokens, max(64, 1 << (len(part) - 1).bit_length()))
+                logits = engine.step([StepEntry(rid, part, list(range(len(part))))], room=room)
                 rows.append(engine.logprobs(logits, tokens[a + 1:a + 1 + len(part)], top))
             engine.check()
         finally:

@@ -274,7 +274,7 @@ class Engine:
         return n
 
     def step(self, entries: Sequence[StepEntry], reserve: bool = True, commit: bool = True,
-             sampling=None) -> torch.Tensor:
+             sampling=None, room: int = 0) -> torch.Tensor:
         """Run one batch. Returns float32 logits ``[total wanted, vocab]`` on the device, in the
         order of the entries and of each entry's ``want``; the tensor is scratch that the next
         step overwrites. With ``reserve`` True room is reserved for every entry first, all or nothing:
@@ -287,7 +287,9 @@ class Engine:
 
         A step made only of single decoded tokens runs as a CUDA graph of fixed shape (batch and
         table sizes rounded up to powers of two, padding rows skipped by every kernel); any other
-        step launches its kernels one by one. Both run the same kernels on the same data."""
+        step launches its kernels one by one. Both run the same kernels on the same data. Recorded steps are kept for good, each with
+        a logits buffer of its own: a caller whose steps come in every size names a ``room``, and steps that are not made of single
+        tokens are recorded for at least that many rows and wanted rows."""
         n = self._validate(entries)
         self.sampled = None
         if reserve:
@@ -314,11 +316,12 @@ class Engine:
             logits = self._step_graph(entries, S, max_pages, sampling)
         else:
             logits = None
+            room = min(room, self.max_batch_tokens)
             max_rows = max(len(e.tokens) for e in entries)
             lead = 0                      # single-token requests at the head of the batch (the scheduler's order)
             while lead < S and len(entries[lead].tokens) == 1:
                 lead += 1
-            small_logits = (n_want + 8) * self.config.vocab_size * 4 <= (64 << 20)   # each graph owns its logits buffer
+            small_logits = (max(n_want, room) + 8) * self.config.vocab_size * 4 <= (64 << 20)   # each graph owns its logits buffer
             if self.use_graphs and small_logits and self.model.recordable(n == S):
                 # A step is replayed as a CUDA graph of a rounded shape, so that batches which differ a little share
                 # one: the single-token requests at its head counted in eights (padding sequences behind them), the
@@ -330,8 +333,8 @@ class Engine:
                 rest = S - lead
                 rest_b = 1 << max(rest - 1, 0).bit_length() if rest else 0
                 S_b = lead_b + rest_b
-                n_b = lead_b + -(-(n - lead + rest_b - rest) // 64) * 64
-                want_b = -(-n_want // 8) * 8
+                n_b = lead_b + -(-max(n - lead + rest_b - rest, room) // 64) * 64
+                want_b = -(-max(n_want, room) // 8) * 8
                 tiles = -(-(n_b - lead_b) // 128)      # the most row tiles a request of this shape can have
                 key = ("step", n_b, lead_b, rest_b, want_b, Pb)
                 g = self._graphs.get(key)

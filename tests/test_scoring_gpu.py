@@ -1,0 +1,35 @@
+"""Scoring texts beside serving: what it refuses, and what it leaves behind in the engine."""
+import random
+
+import numpy as np
+import pytest
+import torch
+
+import glassbox_b200
+
+pytestmark = pytest.mark.gpu
+
+
+def load(model_dirs, **kw):
+    return glassbox_b200.load(model_dirs("D", "bfloat16"), "bfloat16", **{"blocks": 64, "budget": 64, **kw})
+
+
+@pytest.mark.parametrize("cache_bits", [None, 4])
+def test_scoring_leaves_room_for_serving(model_dirs, cache_bits):
+    """Texts of every length, each twice: recorded steps are kept for good, a bounded number of them and of bytes."""
+    llm = load(model_dirs, cache_bits=cache_bits)
+    rng = random.Random(1)
+    texts = [[rng.randrange(300) for _ in range(n)] for n in range(2, 300, 7)]
+    first = llm.score(texts)
+    torch.cuda.synchronize()
+    held, graphs = torch.cuda.memory_allocated(), len(llm.engine._graphs)
+    again = llm.score(texts + texts)
+    torch.cuda.synchronize()
+    # (portions are recorded at one size, 64 rows, for each width of the block tables, 8, 16 and 32 pages here, and single tokens likewise)
+    assert graphs <= len(llm.engine._graphs) <= 2 * 3
+    assert torch.cuda.memory_allocated() - held <= 3 * 64 * 300 * 4 + (1 << 20)
+    replays = llm.engine.graph_replays
+    llm.score(texts[:4])
+    assert llm.engine.graph_replays == replays + 4               # (and short texts do replay them)
+    for a, b in zip(first + first, again):
+        assert np.abs(a.logprobs - b.logprobs).max() < 1e-3 and a.top_ids.shape == b.top_ids.shape
