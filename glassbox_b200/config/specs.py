@@ -523,8 +523,9 @@ def with_cache_bits(config: "ModelConfig", bits: int) -> "ModelConfig":
         raise ConfigError(f"a cache in {bits} bits is not built (4)")
     layers = []
     for i, layer in enumerate(config.layers):
-        if not hasattr(layer.mixer, "cache_bits"):
-            raise ConfigError(f"layer {i}: the cache of {getattr(layer.mixer, 'kind', layer.mixer)!r} cannot be kept in {bits} bits "
+        mixer = getattr(layer, "mixer", None)
+        if not hasattr(mixer, "cache_bits"):
+            raise ConfigError(f"layer {i}: the cache of {getattr(mixer, 'kind', layer)!r} cannot be kept in {bits} bits "
                               f"(grouped-query attention's can)")
-        layers.append(dataclasses.replace(layer, mixer=dataclasses.replace(layer.mixer, cache_bits=bits)))
+        layers.append(dataclasses.replace(layer, mixer=dataclasses.replace(mixer, cache_bits=bits)))
     return dataclasses.replace(config, layers=type(config.layers)(layers))
