@@ -94,11 +94,15 @@ class LLM:
         budget; it needs a state slot and pages beside those of requests in flight, and gives them back."""
         single = len(prompts) > 0 and not isinstance(prompts[0], (list, tuple, np.ndarray))
         batch = [prompts] if single else list(prompts)
-        if not 0 <= top <= kernels.LOGPROBS_MAX_TOP:
-            raise ValueError(f"top {top} must be between 0 and {kernels.LOGPROBS_MAX_TOP}")
+        vocab = self.config.vocab_size
+        if not 0 <= top <= min(kernels.LOGPROBS_MAX_TOP, vocab):
+            raise ValueError(f"top {top} must be between 0 and {min(kernels.LOGPROBS_MAX_TOP, vocab)}")
         for i, p in enumerate(batch):
             if not 0 < len(p) <= self.engine.max_position:
                 raise ValueError(f"prompt {i} has {len(p)} tokens; a prompt needs between 1 and max_position = {self.engine.max_position}")
+            for t in p:
+                if not 0 <= int(t) < vocab:
+                    raise ValueError(f"prompt {i}: token {int(t)} is outside the vocabulary of {vocab}")
         scores = [self._score([int(t) for t in p], top) for p in batch]
         return scores[0] if single else scores
 

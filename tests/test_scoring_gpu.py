@@ -33,3 +33,13 @@ def test_scoring_leaves_room_for_serving(model_dirs, cache_bits):
     assert llm.engine.graph_replays == replays + 4               # (and short texts do replay them)
     for a, b in zip(first + first, again):
         assert np.abs(a.logprobs - b.logprobs).max() < 1e-3 and a.top_ids.shape == b.top_ids.shape
+
+
+def test_tokens_outside_the_vocabulary_are_refused(model_dirs):
+    llm = load(model_dirs)
+    free = llm.engine.cache.free_pages(0)
+    for text in ([1, 2, 300], [1, -1, 2], [300], [1, 2, 1 << 40]):
+        with pytest.raises(ValueError, match="prompt 1.*vocabulary"):
+            llm.score([[5, 6, 7], text])
+    assert llm.engine.cache.free_pages(0) == free
+    assert np.isfinite(llm.score([1, 2, 299]).logprobs).all()
