@@ -59,7 +59,8 @@ class Engine:
         from a group's ``PagedKvSpec`` to a number of pages) sizes each group on its own, for models whose groups need
         different amounts: a group that keeps a window of keys needs far fewer pages than one that keeps them all. ``cache_bits`` 4
         keeps the keys and values of grouped-query attention in four bits (``kernels.kv4_write``): 0.5625 bytes a number; prompts then
-        need pages of the activation type for one layer beside them."""
+        need pages of the activation type for one layer of each group beside them, which are allocated here, too (as much as 3.6 layers in
+        4 bits in bfloat16, 7.1 in float32; ``cache_bytes_per_token`` counts what a token keeps, without them)."""
         if not torch.cuda.is_available():
             raise RuntimeError("glassbox_b200 needs a CUDA device: every kernel is CUDA and there is no CPU path")
         self.device = torch.device(device)
@@ -97,6 +98,8 @@ class Engine:
         self.ctx.weight_order = self.weight_order
         self.side_stream = torch.cuda.Stream(device=self.device)
         self.ctx.side_stream = self.side_stream
+        for part in self.model.parts():
+            part.reserve(self.ctx)
         self.use_programs = bool(use_programs) and self.dtype == torch.bfloat16 and self.model.program_safe
         if self.use_programs:
             self.ctx.program = kernels.Program()

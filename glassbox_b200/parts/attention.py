@@ -122,6 +122,24 @@ class GqaAttention(Mixer):
         kernels.attention_rows(q, att, cache.k, cache.v, cache.block_tables, ctx.row_seq, ctx.positions, self.nh,
                                self.nkv, self.hd, cache.page_size, self.spec.scale, self.spec.window, ctx.status)
 
+    def reserve(self, ctx) -> None:
+        """The pages that prompts over a cache in 4 bits are unpacked into, where any number of rows takes a kernel that reads them."""
+        if self.spec.cache_bits is None:
+            return
+        cache, spec = ctx.cache, self.cache_spec()
+        if spec not in cache.group_specs:
+            return
+        q = ctx.scratch("qkv", (ctx.max_rows, self.qd + 2 * self.kvd))[:, :self.qd]
+        if kernels.kv4_prompt_kernel(q, ctx.scratch("att", (ctx.max_rows, self.qd)), self.nh, self.nkv, self.hd, cache.page_size) is not None:
+            group = cache.group_specs.index(spec)
+            self._unpacked(ctx, group, cache.group_pages[group], cache.page_size, q.dtype)
+
+    def _unpacked(self, ctx, group: int, pages: int, page_size: int, dtype):
+        """Pages of numbers with the ids of a group's, for keys and for values: one layer's worth, which all layers of the group share."""
+        shape = (pages, self.nkv, page_size, self.hd)
+        count = shape[0] * shape[1] * shape[2] * shape[3]
+        return tuple(ctx.zeros_once(f"kv4_{name}{group}", count, dtype)[:count].view(shape) for name in ("keys", "values"))
+
     def _attend_4(self, ctx, q, att, cache) -> None:
         """``attend`` over pages of 4 bits: the single tokens that lead a step take the decode kernel, the requests behind them the
         prompt kernels, for which the pages in sight are unpacked first (where no such kernel takes the shape, all rows the
@@ -137,9 +155,7 @@ class GqaAttention(Mixer):
                                          self.nh, self.nkv, self.hd, cache.page_size, s.scale, s.window, ctx.max_context, parts, ctx.status)
         if alone or cache.block_tables.shape[0] == single:
             return
-        shape = (cache.k.shape[0], self.nkv, cache.page_size, self.hd)
-        count = shape[0] * shape[1] * shape[2] * shape[3]
-        kpages, vpages = (ctx.zeros_once(f"kv4_{name}{cache.group}", count, q.dtype)[:count].view(shape) for name in ("keys", "values"))
+        kpages, vpages = self._unpacked(ctx, cache.group, cache.k.shape[0], cache.page_size, q.dtype)
         kernels.kv4_attention_prefill(q, att, cache.k, cache.v, cache.block_tables[single:], ctx.row_seq, ctx.positions, ctx.seq_first_row[single:],
                                       ctx.seq_start_pos[single:], ctx.max_rows_per_seq, self.nh, self.nkv, self.hd, cache.page_size, s.scale,
                                       s.window, ctx.max_context, kpages, vpages, ctx.status)

@@ -133,6 +133,10 @@ class Part:
         """Parts this part owns (their parameters are loaded under ``<name>.``)."""
         return {}
 
+    def reserve(self, ctx) -> None:
+        """Called once the cache is there and before the first step: a part whose buffers grow with the cache asks for them here, so that an
+        engine that does not fit its device says so when it is made (``ctx``: without rows yet)."""
+
 
 class Norm(Part):
     def forward(self, ctx, x, out, rows=None) -> None:
