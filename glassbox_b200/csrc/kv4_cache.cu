@@ -2,8 +2,8 @@
 //   kv4_write   rotates the queries and keys of a step's rows, rounds keys and values to 4 bits and stores them in their pages;
 //   kv4_read    what the cache holds for given slots, as numbers;
 //   kv4_expand  the pages that a step's requests see, as pages of bfloat16 or float32 that the prompt kernels read.
-// All three only move memory. The sums that matter are bytes: a row of a wide layout (32/8 heads of 128, bfloat16) brings 12 KB in, 8 KB
-// of queries out and 1.1 KB of cache out.
+// What they cannot do without is bytes: a row of a wide layout (32/8 heads of 128, bfloat16) brings 12 KB in, 8 KB of queries out and 1.1 KB of
+// cache out.
 //
 // The rounding: m's bits less 3 in the exponent, rounded to four bits after the leading one, are |d|. A quotient y / d is the product with the
 // reciprocal and one correction by the remainder (exact in a fused multiply-add), so that a number half way between two codes is told as such:
@@ -15,7 +15,8 @@
 #include <type_traits>
 
 // Measured (bfloat16, 32/8 heads of 128 of which 64 channels turn, 8,000 rows written and read back, 217 MB): 62 us; without the queries 40, without
-// keys 46, without values 53. Bound by instructions (58 % of the issue slots) and the loads' latency. A thread has two loads or more under way: with one
+// keys 46, without values 53. Neither instructions (58 % of the issue slots) nor memory (32 % of its rate) fill it: what bounds it is a block's one
+// round of loads and the chain of maxima and codes behind them. A thread has two loads or more under way: with one
 // piece of a query a thread and keys and values read back apart it took 84, with two pieces of one head 67. 64 / 256 threads a block took 117 / 87
 // where 128 took 84; 40 registers (12 blocks a multiprocessor) take 72 where 56 take 62.
 constexpr int KV4_THREADS = 128;

@@ -21,8 +21,8 @@
 // add up from each other's shared memory, or, behind the longest contexts, all rows' steps cut evenly among the blocks that run at once
 // (kv4_decode_even_kernel). Nothing is left behind for the next call.
 //
-// What bounds it: issuing instructions, some 430 for 32 keys of a head of 64 and their values (2.4 of 4 a cycle and multiprocessor), not the
-// memory. 64 rows of 32/32 heads of 64 behind 4,096 keys, 605 MB, take 154 us (3.9 TB/s); 2 rows of 32/8 heads of 128 behind 131,072, 302 MB, 86 us
+// What bounds it: instructions, some 430 for 32 keys of a head of 64 and their values, and how they wait for one another: 2.4 of 4 are issued a cycle
+// and multiprocessor (all 4 would be 97 of the 154 us below, the memory's share is 92). 64 rows of 32/32 heads of 64 behind 4,096 keys, 605 MB, take 154 us (3.9 TB/s); 2 rows of 32/8 heads of 128 behind 131,072, 302 MB, 86 us
 // (157 and 87 with one float32 where two go into an instruction, which is the form that the next figures are from).
 // The second without taking codes apart 72, without the second product 63, without copies 80; one multiprocessor's blocks 3 / 4 / 5 of them 91 / 87 /
 // 115, of heads of 64 (the first) 4 / 5 / 6 159 / 157 / 165; a ring of five steps 163; in even shares with one tile a step instead of two 180 to 203.

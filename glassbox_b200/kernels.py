@@ -2469,7 +2469,7 @@ def kv4_decode_plan(n: int, nh: int, nkv: int, hd: int, max_context: int, window
 
     * blocks of a cluster 1 / 2 / 4 / 8. A share wants 128 keys: one row of 9/3 heads of 64 at 256 keys 4.8 / 5.1 / 4.9 / 5.0, at 1,024
       8.9 / 7.2 / 5.8 / 5.3. The more blocks there are anyway, the more keys a further one has to bring: 64 such rows at 1,024 keys 10.6 / 12.3 /
-      13.4 / 18.8, at 4,096 31 / 32 / 25 / 29; 300 at 2,048 46 / 48 / 61 / 90, at 4,096 84 / 80 / 91 / 119; 64 of 32/32 heads at 4,096 157 / 164 / 191 / 253.
+      13.4 / 18.8 (the rule takes two here, not the best), at 4,096 31 / 32 / 25 / 29; 300 at 2,048 46 / 48 / 61 / 90, at 4,096 84 / 80 / 91 / 119; 64 of 32/32 heads at 4,096 157 / 164 / 191 / 253.
     * "even" against the best cluster costs its second launch and pays where eight blocks a row are too few: 2 rows of 32/8 heads of 128 up to 4,096
       keys 16.5 to 10.6, up to 16,384 21.3 to 24.8; 24 of them at 8,192 75 to 71, one of them at 16,384 and the rest at 2,048 36 to 45.
     * "rows": 16 rows of 8/2 float32 heads of 160 at 2,048 keys in 4 / 8 / 16 / 32 shares 96 / 66 / 52 / 76, one row of 9/3 heads of 64 at 512

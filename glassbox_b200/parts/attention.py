@@ -143,8 +143,9 @@ class GqaAttention(Mixer):
     def _attend_4(self, ctx, q, att, cache) -> None:
         """``attend`` over pages of 4 bits: the single tokens that lead a step take the decode kernel, the requests behind them the
         prompt kernels, for which the pages in sight are unpacked first (where no such kernel takes the shape, all rows the
-        decode kernel). Beside a prompt of 256 rows, 9/3 heads of 64, all through the prompt kernel or so divided: 32 single tokens behind 2,000
-        60 or 19 us, 1 behind 2,000 22 or 15, 8 behind 200 10 or 14, 1 behind 200 9 or 13; 32/8 heads of 128 207 or 41, 39 or 22, 24 or 21, 14 or 20."""
+        decode kernel). Always so: where single tokens are behind long contexts that is several times faster, behind short ones it costs a launch. Beside a
+        prompt of 256 rows, 9/3 heads of 64, all through the prompt kernel or so divided: 32 single tokens behind 2,000 60 or 19 us, 1 behind 2,000 22
+        or 15, 8 behind 200 10 or 14, 1 behind 200 9 or 13; 32/8 heads of 128 207 or 41, 39 or 22, 24 or 21, 14 or 20."""
         n, s = q.shape[0], self.spec
         alone = ctx.decode_only or kernels.kv4_prompt_kernel(q, att, self.nh, self.nkv, self.hd, cache.page_size) is None
         single = n if alone else ctx.leading_single
