@@ -2589,9 +2589,10 @@ def kv4_attention_prefill(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tens
     kind = kv4_prompt_kernel(q, out, nh, nkv, hd, page_size)
     if kind is None and q.dtype == torch.bfloat16 and lib().gb_kv4_attention_decode_supported(hd):
         _here(kcache, vcache, block_tables, status)
+        cluster = kv4_decode_plan(n, nh, nkv, hd, min(int(max_context), 8192), window)[1]       # (no even shares, which need scratch)
         _call("gb_kv4_attention_decode", q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), kcache.data_ptr(), vcache.data_ptr(),
               block_tables.data_ptr(), block_tables.shape[1], row_seq.data_ptr(), positions.data_ptr(), n, nh, nkv, hd, page_size,
-              kcache.shape[0], float(scale), int(window or 0), 1, 0, 0, status.data_ptr(), stream)
+              kcache.shape[0], float(scale), int(window or 0), cluster, 0, 0, status.data_ptr(), stream)
         return
     kv4_expand(kcache, vcache, kpages, vpages, block_tables, seq_first_row, seq_start_pos, max_context, window, status)
     if kind is None:
