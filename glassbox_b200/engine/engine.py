@@ -319,8 +319,8 @@ class Engine:
             logits = self._step_graph(entries, S, max_pages, sampling)
         else:
             logits = None
-            room = min(room, self.max_batch_tokens)
             max_rows = max(len(e.tokens) for e in entries)
+            room = min(room, self.max_batch_tokens) if max_rows > 1 else 0
             lead = 0                      # single-token requests at the head of the batch (the scheduler's order)
             while lead < S and len(entries[lead].tokens) == 1:
                 lead += 1

@@ -43,3 +43,19 @@ def test_tokens_outside_the_vocabulary_are_refused(model_dirs):
             llm.score([[5, 6, 7], text])
     assert llm.engine.cache.free_pages(0) == free
     assert np.isfinite(llm.score([1, 2, 299]).logprobs).all()
+
+
+def test_room_is_for_steps_with_portions_of_prompts(model_dirs):
+    """Single tokens, one of which wants no logits, are recorded at their own size whatever room is asked for, and come out the same."""
+    from glassbox_b200.engine.engine import StepEntry
+    got = []
+    for room in (0, 64):
+        eng = load(model_dirs).engine
+        for r in "ab":
+            eng.add_request(r)
+            eng.step([StepEntry(r, list(range(1, 30)), [])])
+        for t in range(4):
+            got.append(eng.step([StepEntry("a", [t], []), StepEntry("b", [t + 7], [0])], room=room).clone())
+        eng.check()
+        assert all(key[1] == 8 for key in eng._graphs if key[0] == "step" and key[3] == 0) and eng.graph_replays > 0
+    assert all(torch.equal(x, y) for x, y in zip(got[:4], got[4:]))
