@@ -48,6 +48,10 @@ _SIGNATURES = {
     "gb_gemm_f32_tc_supported": [_P, _P, _I, _I, _LL, _LL],
     "gb_gemm_f32_tc": [_P, _P, _I, _P, _I, _I, _I, _I, _LL, _LL, _LL, _P, _P],
     "gb_gemm_simt": [_P, _I, _P, _I, _P, _I, _I, _I, _I, _I, _LL, _LL, _LL, _P],
+    "gb_tree_attention": [_I, _P, _LL, _P, _LL, _I, _P, _P, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _LL, _F, _I, _I, _P, _P, _P],
+    "gb_tree_attention_splits": [_I, _I, _I, _I, _I, _I, _I, _I],
+    "gb_verify_tree": [_P, _I, _LL, _P, _LL, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P],
+    "gb_keep_rows": [_P, _P, _I, _I, _I, _LL, _I, _I, _P, _I, _P, _P, _P, _P, _I, _I, _P, _P],
     "gb_attention_rows": [_P, _LL, _P, _LL, _I, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _LL, _F, _I, _P, _P],
     "gb_sample": [_P, _LL, _P, _P, _P, _P, _I, _P, _P, _I, _I, _P],
     "gb_resolve_tokens": [_P, _P, _P, _I, _I, _P],
@@ -2640,3 +2644,141 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, logprob: torch.Te
     stream = _here(logits, tokens, logprob, entropy, top_logprob, top_ids)
     _call("gb_token_logprobs", logits.data_ptr(), _dt(logits), logits.stride(0), tokens.data_ptr(), logprob.data_ptr(), _ptr(entropy),
           _ptr(top_logprob), _ptr(top_ids), top, rows, vocab, stream)
+
+
+# ------------------------------------------------------------------------------------------------ drafted tokens
+TREE_WORD = 32                 # rows of a tree that a word of ``visible`` names
+TREE_MAX_ROWS = 1024           # rows of a request's tree
+VERIFY_MAX_VOCAB = 4096 * 512
+
+
+def tree_attention_kind(q: torch.Tensor, out: torch.Tensor, hd: int, page_size: int) -> int:
+    """Which kernel ``tree_attention`` runs: 1 the tensor cores' (bfloat16, head sizes 32, 64, 96 and 128, rows that start at 4 bytes, pages of a
+    power of two), 0 the one for everything else."""
+    return int(q.dtype == torch.bfloat16 and hd in (32, 64, 96, 128) and page_size & (page_size - 1) == 0
+               and q.stride(0) % 2 == 0 and q.data_ptr() % 4 == 0 and out.stride(0) % 2 == 0 and out.data_ptr() % 4 == 0)
+
+
+@functools.lru_cache(maxsize=1024)
+def _tree_splits(kind: int, num_seqs: int, most: int, nh: int, nkv: int, hd: int, max_context: int, window: int) -> int:
+    return lib().gb_tree_attention_splits(kind, num_seqs, most, nh, nkv, hd, max_context, window)
+
+
+def tree_attention_parts(q: torch.Tensor, nh: int, nkv: int, hd: int, num_seqs: int, max_rows_per_seq: int, max_context: int,
+                         window: Optional[int] = None) -> Optional[torch.Tensor]:
+    """Scratch for ``tree_attention`` of these sizes (None: it needs none). Calls that follow one another on a stream may share it."""
+    # (the kernel is chosen by the tensors' alignment, too: as much as the one that needs more)
+    splits = max(_tree_splits(kind, num_seqs, max_rows_per_seq, nh, nkv, hd, max_context, int(window or 0)) for kind in (0, 1))
+    return torch.empty(splits * q.shape[0] * nh * (hd + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
+
+
+def _tree_batch(block_tables, seq_first_row, seq_start_pos) -> int:
+    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.shape[1] < 1 or not block_tables.is_contiguous():
+        raise KernelError("block_tables must be contiguous int32 [requests, pages]")
+    num_seqs = block_tables.shape[0]
+    _vector("seq_first_row", seq_first_row, num_seqs + 1)
+    _vector("seq_start_pos", seq_start_pos, num_seqs)
+    return num_seqs
+
+
+def tree_attention(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, block_tables: torch.Tensor,
+                   seq_first_row: torch.Tensor, seq_start_pos: torch.Tensor, positions: torch.Tensor, visible: torch.Tensor, max_rows_per_seq: int,
+                   nh: int, nkv: int, hd: int, page_size: int, scale: float, window: Optional[int], max_context: int, parts: Optional[torch.Tensor],
+                   status: torch.Tensor) -> None:
+    """softmax(q k^T * scale) v for rows that are trees of drafted tokens. Request s brings rows seq_first_row[s] .. seq_first_row[s + 1] - 1; row i of
+    it has its key and value in the cache at place seq_start_pos[s] + i, and is at positions[row] of the text (not before seq_start_pos[s]). It sees all
+    places before seq_start_pos[s] and of its own request's rows those that ``visible`` (int32 [n, words]: bit i % 32 of word i // 32 is row i) names; with
+    a ``window``, of these the ones that are fewer than that many positions back. A row that sees nothing comes out as zeros, so do the rows of a request
+    with a negative start; rows that belong to no request stay as they are. q, out: bfloat16 or float32 [n, nh * hd], rows may be strided; kcache, vcache
+    [pages, nkv, page_size, hd] of the same type. No request has more than ``max_rows_per_seq`` rows; ``max_context`` sizes the shares of the keys
+    (longer contexts are still right), ``parts`` comes from ``tree_attention_parts`` of the same sizes."""
+    if not (q.dim() == 2 and q.shape[1] == nh * hd and q.stride(1) == 1 and out.shape == q.shape and out.stride(1) == 1):
+        raise KernelError(f"q and out must be [n, {nh * hd}] with neighbouring numbers")
+    n = q.shape[0]
+    if nkv < 1 or nh < 1 or nh % nkv or not 0 < hd <= 256:
+        raise KernelError(f"{nh}/{nkv} heads of {hd} channels are not built")
+    if not (q.dtype == out.dtype == kcache.dtype == vcache.dtype):
+        raise KernelError("q, out and the cache must be of one type")
+    for name, t in (("kcache", kcache), ("vcache", vcache)):
+        if t.dim() != 4 or t.shape[1:] != (nkv, page_size, hd) or t.shape[0] < 1 or t.shape != kcache.shape or not t.is_contiguous():
+            raise KernelError(f"{name} must be contiguous [pages, {nkv}, {page_size}, {hd}]")
+    num_seqs = _tree_batch(block_tables, seq_first_row, seq_start_pos)
+    _vector("positions", positions, n)
+    if visible.dtype != torch.int32 or visible.dim() != 2 or visible.shape[0] < n or visible.shape[1] < 1 or not visible.is_contiguous():
+        raise KernelError(f"visible must be contiguous int32 [{n}, words]")
+    if not 0 <= max_rows_per_seq <= TREE_MAX_ROWS:
+        raise KernelError(f"a tree of {max_rows_per_seq} rows is not built (up to {TREE_MAX_ROWS})")
+    if window is not None and window < 1:
+        raise KernelError(f"a window of {window}")
+    dtype = _dt(q)
+    stream = _here(q, out, kcache, vcache, block_tables, seq_first_row, seq_start_pos, positions, visible, parts, status)
+    if not n or not num_seqs or not max_rows_per_seq:
+        return
+    kind = tree_attention_kind(q, out, hd, page_size)
+    splits = _tree_splits(kind, num_seqs, max_rows_per_seq, nh, nkv, hd, int(max_context), int(window or 0))
+    if splits > 1 and (parts is None or parts.dtype != torch.float32 or not parts.is_contiguous() or parts.numel() < splits * n * nh * (hd + 2)):
+        raise KernelError(f"this batch needs contiguous float32 scratch of {splits * n * nh * (hd + 2)} numbers (tree_attention_parts)")
+    _call("gb_tree_attention", kind, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), dtype, kcache.data_ptr(), vcache.data_ptr(),
+          block_tables.data_ptr(), block_tables.shape[1], seq_first_row.data_ptr(), seq_start_pos.data_ptr(), positions.data_ptr(), visible.data_ptr(),
+          visible.shape[1], n, num_seqs, int(max_rows_per_seq), nh, nkv, hd, page_size, kcache.shape[0], float(scale), int(window or 0), splits, _ptr(parts),
+          status.data_ptr(), stream)
+
+
+def verify_tree(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, seq_first_row: torch.Tensor, uniform: torch.Tensor,
+                temperature: torch.Tensor, path: torch.Tensor, accepted: torch.Tensor, next_token: torch.Tensor,
+                draft_logits: Optional[torch.Tensor] = None) -> None:
+    """Which rows of each request's tree of drafted tokens are kept, and the token that follows them, from given random numbers.
+
+    Request s brings rows seq_first_row[s] .. seq_first_row[s + 1] - 1 of logits (float32 or bfloat16 [n, vocab], rows may be strided): row 0 of its tree is
+    the token it was given last, row i holds tokens[i] and follows row parents[i] < i of the same tree. The walk begins at row 0. Without
+    ``draft_logits`` a token is drawn at the row it has reached: the first one, in the order of the ids, at which the sum of softmax(logits / temperature[s])
+    exceeds uniform[row, 1] (at a temperature that is not above 0: the largest logit, of equal ones the lowest id); the walk goes on at the first child that
+    holds that token, and ends where none does. With ``draft_logits`` (like logits: what the children of each row were drawn from, independently and at the
+    same temperature, as q) a child of token x is taken where uniform[child, 0] * q(x) * sum(r) < r(x), r being p = softmax(logits / temperature) at first and
+    max(r - sum(r) q, 0) behind a child that was not taken; behind the last child the token that follows is drawn from r by uniform[row, 1] (from p where
+    nothing is left). So what comes out is distributed as what the model writes by itself. At temperature 0 drafted distributions play no part.
+
+    Results, int32: accepted[s] rows are kept (row 0 always is; 0 for a request without rows), path[seq_first_row[s] + j] is the j-th of them (-1 behind the
+    last), next_token[s] the token that follows (-1: the logits that the walk reached hold a NaN or plus infinity, or nothing but minus infinity; a greedy walk
+    passes over NaN). A child whose token is outside the vocabulary is never taken."""
+    if not (logits.dim() == 2 and logits.stride(1) == 1):
+        raise KernelError("logits must be [rows, vocab] with neighbouring numbers")
+    n, vocab = logits.shape
+    num_seqs = temperature.shape[0]
+    if not 0 < vocab <= VERIFY_MAX_VOCAB:
+        raise KernelError(f"a vocabulary of {vocab} is not built (up to {VERIFY_MAX_VOCAB})")
+    if draft_logits is not None and not (draft_logits.shape == logits.shape and draft_logits.dtype == logits.dtype and draft_logits.stride(1) == 1):
+        raise KernelError(f"draft_logits must be {logits.dtype} [{n}, {vocab}] with neighbouring numbers, as logits are")
+    for name, t, size in (("tokens", tokens, n), ("parents", parents, n), ("seq_first_row", seq_first_row, num_seqs + 1), ("path", path, n),
+                          ("accepted", accepted, num_seqs), ("next_token", next_token, num_seqs)):
+        _vector(name, t, size)
+    if temperature.dtype != torch.float32 or temperature.dim() != 1 or not temperature.is_contiguous():
+        raise KernelError("temperature must be contiguous float32 [requests]")
+    if uniform.dtype != torch.float32 or uniform.shape != (n, 2) or not uniform.is_contiguous():
+        raise KernelError(f"uniform must be contiguous float32 [{n}, 2]")
+    dtype = _dt(logits)
+    stream = _here(logits, tokens, parents, seq_first_row, uniform, temperature, path, accepted, next_token, draft_logits)
+    _call("gb_verify_tree", logits.data_ptr(), dtype, logits.stride(0), _ptr(draft_logits), 0 if draft_logits is None else draft_logits.stride(0),
+          tokens.data_ptr(), parents.data_ptr(), seq_first_row.data_ptr(), uniform.data_ptr(), temperature.data_ptr(), path.data_ptr(), accepted.data_ptr(),
+          next_token.data_ptr(), n, num_seqs, vocab, stream)
+
+
+def keep_rows(kpool: torch.Tensor, vpool: torch.Tensor, block_tables: torch.Tensor, seq_first_row: torch.Tensor, seq_start_pos: torch.Tensor,
+              path: torch.Tensor, accepted: torch.Tensor, page_size: int, max_rows_per_seq: int, status: torch.Tensor) -> None:
+    """The keys and values of the rows that ``verify_tree`` kept move, in every layer, to the places directly behind what the cache held before the step: place
+    seq_start_pos[s] + path[seq_first_row[s] + j] goes to seq_start_pos[s] + j for j < accepted[s], path ascending. kpool, vpool: contiguous [layers, pages,
+    heads, page_size, channels] of any type of 2 bytes or more, values may have other channels than keys. Requests with a negative start are passed over; where a
+    path leaves its tree or a page is missing nothing of the request moves, and ``status`` says so."""
+    for name, t in (("kpool", kpool), ("vpool", vpool)):
+        if t.dim() != 5 or t.shape[:4] != kpool.shape[:4] or t.shape[3] != page_size or not t.is_contiguous() or t.element_size() < 2 or not t.numel():
+            raise KernelError(f"{name} must be contiguous [layers, pages, heads, {page_size}, channels] of numbers of 2 bytes or more")
+    num_seqs = _tree_batch(block_tables, seq_first_row, seq_start_pos)
+    n = path.shape[0]
+    _vector("path", path, n)
+    _vector("accepted", accepted, num_seqs)
+    if not 0 <= max_rows_per_seq <= TREE_MAX_ROWS:
+        raise KernelError(f"a tree of {max_rows_per_seq} rows is not built (up to {TREE_MAX_ROWS})")
+    stream = _here(kpool, vpool, block_tables, seq_first_row, seq_start_pos, path, accepted, status)
+    _call("gb_keep_rows", kpool.data_ptr(), vpool.data_ptr(), kpool.shape[4] * kpool.element_size(), vpool.shape[4] * vpool.element_size(), kpool.shape[0],
+          kpool.shape[1], kpool.shape[2], page_size, block_tables.data_ptr(), block_tables.shape[1], seq_first_row.data_ptr(), seq_start_pos.data_ptr(),
+          path.data_ptr(), accepted.data_ptr(), n, num_seqs, status.data_ptr(), stream)
