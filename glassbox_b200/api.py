@@ -12,6 +12,7 @@ from typing import List, Optional, Sequence, Union
 import numpy as np
 
 from . import kernels
+from .engine import drafts as drafted
 from .engine.engine import Engine, StepEntry
 from .engine.scheduler import Request, Scheduler, SchedulerConfig
 from .sampling.sampler import SamplerConfig
@@ -63,16 +64,24 @@ class LLM:
     def generate(self, prompts: Union[Sequence[int], Sequence[Sequence[int]]], max_tokens: int = 128, *,
                  temperature: float = 0.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0,
                  repetition_penalty: float = 1.0, seed: int = 0, stop: Sequence[int] = (),
-                 return_reasons: bool = False):
+                 return_reasons: bool = False, drafts=None):
         """Generate up to ``max_tokens`` tokens after each prompt. ``prompts`` is one list of token
         ids or a list of such lists; request i samples with seed ``seed + i``. Returns the new
-        tokens (one list, or a list of lists in the order given)."""
+        tokens (one list, or a list of lists in the order given). With ``drafts`` (``PromptLookup``, ``DraftModel``) several tokens a step are
+        guessed and verified (``engine.drafts``; greedy or with a temperature alone): the model's own text, in fewer steps where the guesses
+        are good; ``self.draft_counts`` says how they fared. Such requests go by themselves, not through the scheduler's queue."""
         single = len(prompts) > 0 and not isinstance(prompts[0], (list, tuple, np.ndarray))
         batch = [prompts] if single else list(prompts)
         limit = self.engine.max_position
         for i, p in enumerate(batch):
             if not 0 < len(p) <= limit:
                 raise ValueError(f"prompt {i} has {len(p)} tokens; a prompt needs between 1 and max_position = {limit}")
+        if drafts is not None:
+            cfg = SamplerConfig(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p, repetition_penalty=repetition_penalty, seed=seed)
+            outs, reasons, self.draft_counts = drafted.generate(self.engine, batch, max_tokens, drafts, cfg, tuple(stop), self.scheduler_config.max_seqs)
+            if return_reasons:
+                return (outs[0], reasons[0]) if single else (outs, reasons)
+            return outs[0] if single else outs
         ids = []
         for i, p in enumerate(batch):
             cfg = SamplerConfig(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p,

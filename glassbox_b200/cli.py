@@ -4,6 +4,7 @@
     python -m glassbox_b200 generate --model DIR --prompt "5 17 3" [-n 128] [--dtype bf16|f32]
         [--temp T] [--top-p P] [--top-k K] [--min-p P] [--repeat-penalty R] [--seed N]
         [--blocks 2048] [--budget 256] [--max-seqs 32] [--no-prefix-cache] [--cache-bits 4]
+        [--draft-lookup K | --draft-model DIR [--draft-tokens K]]
     python -m glassbox_b200 score --model DIR --prompt "5 17 3 ..." [--top K] [--dtype bf16|f32]
         [--blocks 2048] [--budget 256] [--cache-bits 4]
     python -m glassbox_b200 random-model --config FILE --seed N --out DIR [--store bf16|f32]
@@ -12,9 +13,10 @@ Text and tokenizers are outside this engine, so ``--prompt`` takes token ids (se
 or commas; ``;`` separates several prompts, which are then batched) and the reply is printed as
 token ids. ``score`` prints, for each token but the first, its id, its log probability given those before it, the entropy of the
 distribution it came from and, with ``--top K``, the K most probable tokens as id:log probability; the perplexity of each prompt
-goes to the error stream. ``--raw`` is accepted and changes nothing: there is no chat template to skip. The
+goes to the error stream. ``--draft-lookup`` guesses up to K tokens a step from the text itself, ``--draft-model`` lets a smaller model write K (4) ahead; what
+comes out is the model's own text either way. ``--raw`` is accepted and changes nothing: there is no chat template to skip. The
 chat, serve, anatomy, trace and spec-trace subcommands of the reference belong to its server,
-visualizer and speculative decoder and are not part of this engine.
+visualizer and are not part of this engine; what its speculative decoder does is ``generate`` with drafts.
 """
 from __future__ import annotations
 
@@ -75,6 +77,8 @@ def main(argv=None) -> int:
         if not prompts:
             return _die("--prompt holds no token ids")
         from .api import LLM
+        from .engine.drafts import DraftModel, PromptLookup
+        from .engine.engine import Engine
         dtype = {"f32": "float32", "fp32": "float32", "float32": "float32"}.get(args.get("--dtype", "bf16"), "bfloat16")
         t0 = time.time()
         llm = LLM(model, dtype, blocks=args.num("--blocks", 2048, int), budget=args.num("--budget", 256, int),
@@ -90,16 +94,26 @@ def main(argv=None) -> int:
                 print(f"perplexity {score.perplexity:.4f} over {len(score.logprobs)} tokens", file=sys.stderr)
             return 0
         n = args.num("-n", 128, int)
+        drafts = None
+        if args.has("--draft-lookup"):
+            drafts = PromptLookup(tokens=args.num("--draft-lookup", 8, int))
+        elif args.get("--draft-model"):
+            small = Engine(args.get("--draft-model"), dtype, num_pages=args.num("--blocks", 2048, int), max_batch_tokens=args.num("--budget", 256, int),
+                           max_requests=args.num("--max-seqs", 32, int))
+            drafts = DraftModel(small, tokens=args.num("--draft-tokens", 4, int), seed=args.num("--seed", 0, int))
         t1 = time.time()
         outs = llm.generate(prompts, n, temperature=args.num("--temp", 0.0), top_p=args.num("--top-p", 1.0),
                             top_k=args.num("--top-k", 0, int), min_p=args.num("--min-p", 0.0),
-                            repetition_penalty=args.num("--repeat-penalty", 1.0), seed=args.num("--seed", 0, int))
+                            repetition_penalty=args.num("--repeat-penalty", 1.0), seed=args.num("--seed", 0, int), drafts=drafts)
         secs = time.time() - t1
         for out in outs:
             print(" ".join(str(t) for t in out))
         total = sum(len(o) for o in outs)
         print(f"prompt {sum(len(p) for p in prompts)} tokens, generated {total} tokens: {total / secs:.1f} tok/s",
               file=sys.stderr)
+        if drafts is not None:
+            c = llm.draft_counts
+            print(f"{c.accepted} of {c.drafted} drafted tokens accepted in {c.steps} steps", file=sys.stderr)
         return 0
     if cmd == "random-model":
         cfg, out = args.get("--config"), args.get("--out")

@@ -76,6 +76,13 @@ class Scratch:
         return buf
 
 
+@dataclass
+class TreeRows:
+    """The rows of a step whose requests bring trees of drafted tokens."""
+    visible: torch.Tensor    # int32 [n, words]: of each row the rows of its request that it sees (``kernels.tree_attention``)
+    max_rows: int            # no request brings more
+
+
 class WeightOrder:
     """Learns the order in which weight matrices are used in a step (it is the same in every step of
     one model) from the calls themselves, so that a product can ask the memory system for the weights
@@ -126,6 +133,7 @@ class StepContext:
         self.num_seqs = 0
         self.decode_only = False          # every sequence of the step brings exactly one row
         self.leading_single = 0           # the first this many sequences bring one row each (rows 0 .. this - 1)
+        self.tree: Optional[TreeRows] = None   # requests bring trees of drafted tokens, at positions that count their depths
         self.token_slots = None           # int32 [rows]: state slot of the rows whose token the device supplies itself, else -1
         self.want_slots = None            # int32 [wanted rows]: state slot of the rows that are sampled from their own state, else -1
         self.weight_order: Optional[WeightOrder] = None

@@ -1,0 +1,258 @@
+"""Generation with drafted tokens (crates/glassbox-core/src/spec.rs:79-240): a cheap guess at a request's next tokens, one step of the model over all of
+them, and what the model would have written itself is kept (``Engine.verify_step``). The text that comes out is the model's: greedy requests get
+the tokens that they would get one by one, requests with a temperature tokens of the same distribution.
+
+Two sources of drafts, as there: ``PromptLookup`` takes what followed earlier where the text's last tokens occurred before (of several such places a
+tree), ``DraftModel`` lets a smaller model of the same vocabulary write ahead (a chain, with the distributions it was drawn from).
+"""
+from __future__ import annotations
+
+from collections import deque
+from dataclasses import dataclass, field
+from typing import Deque, Dict, List, Optional, Sequence, Tuple
+
+import numpy as np
+import torch
+
+from .. import kernels
+from ..cache.manager import OutOfPages
+from ..sampling.sampler import Rng, Sampler, SamplerConfig
+from .engine import Engine, StepEntry
+from .scheduler import LENGTH, STOP
+
+
+class PromptLookup:
+    """Drafts from the text itself: where its last ``match`` tokens (or fewer, down to one) occurred before, what followed there, up to ``tokens`` of
+    them, for up to ``branches`` such places, the latest first. Places that go on alike share the tokens that are alike."""
+
+    def __init__(self, tokens: int = 8, match: int = 3, branches: int = 3):
+        if tokens < 1 or match < 1 or branches < 1:
+            raise ValueError("a lookup needs at least one token, one token to match and one branch")
+        self.tokens, self.match, self.branches = int(tokens), int(match), int(branches)
+
+    def propose(self, text: Sequence[int], room: int) -> Tuple[List[int], List[int]]:
+        """(tokens, parents) of a tree whose first token is the text's last one, with at most ``room`` drafts."""
+        x = np.asarray(text, dtype=np.int64)
+        tokens, parents, children = [int(x[-1])], [-1], {}
+        places: List[int] = []
+        for m in range(min(self.match, len(x) - 1), 0, -1):
+            windows = np.lib.stride_tricks.sliding_window_view(x[:-1], m)
+            ends = np.nonzero((windows == x[-m:]).all(axis=1))[0] + m          # what followed begins here
+            places += [int(e) for e in ends[::-1] if int(e) not in places]
+            if len(places) >= self.branches:
+                break
+        for place in places[:self.branches]:
+            at = 0
+            for t in x[place:place + self.tokens].tolist():
+                if (at, t) not in children:
+                    if len(tokens) > room:
+                        break
+                    children[(at, t)] = len(tokens)
+                    tokens.append(t)
+                    parents.append(at)
+                at = children[(at, t)]
+        return tokens, parents
+
+    def drop(self, rid) -> None:
+        pass
+
+
+class DraftModel:
+    """Drafts from a smaller model: ``tokens`` of them, written one after another by ``engine`` (an ``Engine`` of a model with the same vocabulary, used for
+    nothing else meanwhile), greedily for greedy requests, else drawn at the request's temperature by random numbers of its own (``seed``)."""
+
+    def __init__(self, engine: Engine, tokens: int = 4, seed: int = 0):
+        if tokens < 1:
+            raise ValueError("a drafting model needs to write at least one token")
+        self.engine, self.tokens, self.rng = engine, int(tokens), Rng(seed)
+
+    def propose_all(self, rids: Sequence[object], texts: Sequence[Sequence[int]], rooms: Sequence[int], temperatures: Sequence[float]):
+        """For each request ``(tokens, parents)`` as ``PromptLookup.propose``, and of all rows the logits that their children were drawn from."""
+        engine = self.engine
+        for rid, text in zip(rids, texts):
+            if not engine.cache.has(rid):
+                engine.add_request(rid, list(text))
+            held = engine.cache.tokens(rid)[:engine.length(rid)]
+            same = 0
+            limit = min(len(held), len(text) - 1)
+            if limit:
+                differ = np.nonzero(np.asarray(held[:limit]) != np.asarray(text[:limit]))[0]
+                same = int(differ[0]) if len(differ) else limit
+            if same < len(held):
+                engine.cache.truncate(rid, same)         # (what was drafted and not kept)
+            for a in range(same, len(text) - 1, engine.max_batch_tokens):
+                engine.step([StepEntry(rid, list(text[a:min(a + engine.max_batch_tokens, len(text) - 1)]))])
+        counts = [max(0, min(self.tokens, room, engine.max_position - len(text))) for room, text in zip(rooms, texts)]
+        firsts = np.concatenate([[0], np.cumsum([c + 1 for c in counts])])
+        logits = torch.zeros(int(firsts[-1]), engine.config.vocab_size, device=engine.device)
+        drafts = [[int(text[-1])] for text in texts]
+        heat = torch.tensor(temperatures, dtype=torch.float32)
+        for i in range(max(counts, default=0)):
+            live = [j for j, c in enumerate(counts) if c > i]
+            rows = engine.step([StepEntry(rids[j], [drafts[j][-1]], [0]) for j in live])
+            logits.index_copy_(0, torch.tensor([int(firsts[j]) + i for j in live], device=engine.device), rows)
+            picked = torch.empty(len(live), dtype=torch.int32, device=engine.device)
+            draws = torch.tensor([self.rng.next_f32() for _ in live], dtype=torch.float32).to(engine.device)
+            kernels.sample(rows, picked, heat[live].to(engine.device), draws)
+            for j, t in zip(live, picked.tolist()):
+                drafts[j].append(t)
+        return [(d, list(range(-1, len(d) - 1))) for d in drafts], logits
+
+    def drop(self, rid) -> None:
+        if self.engine.cache.has(rid):
+            self.engine.free_request(rid)
+
+
+@dataclass
+class _Text:
+    rid: object
+    index: int
+    tokens: List[int]
+    prompt: int
+    sampler: Sampler
+    order: int = 0
+    reason: Optional[str] = None
+    draws: List[float] = field(default_factory=list)     # random numbers ahead of the generator: one for each token that is next to be drawn
+
+
+@dataclass
+class DraftCounts:
+    """How drafts fared in a run of ``generate``."""
+    steps: int = 0           # steps of the model, of one request each
+    drafted: int = 0
+    accepted: int = 0
+
+
+def generate(engine: Engine, prompts: Sequence[Sequence[int]], max_tokens: int, drafts, config: SamplerConfig, stop: Sequence[int] = (),
+             max_seqs: Optional[int] = None) -> Tuple[List[List[int]], List[str], DraftCounts]:
+    """Generate after each prompt with ``drafts`` (a ``PromptLookup`` or ``DraftModel``); request i samples with seed ``config.seed + i``. Returns the new tokens and
+    why each request ended, in the order given, and how the drafts fared. Prompts are read one by one, all running requests go through the model in one
+    step. When pages run out drafts go first, then the request that was admitted last waits and is read again."""
+    if config.needs_host:
+        raise ValueError("drafted generation is greedy or at a temperature: top_k, top_p, min_p and repetition_penalty are not built for it")
+    if not engine.model.takes_trees:
+        raise ValueError(f"{engine.config.architecture} takes no drafted trees with this cache (a part carries something from row to row, or the cache holds 4 bits)")
+    if isinstance(drafts, DraftModel):
+        if drafts.engine is engine:
+            raise ValueError("a model cannot draft for itself")
+        if drafts.engine.config.vocab_size != engine.config.vocab_size:
+            raise ValueError(f"the drafting model knows {drafts.engine.config.vocab_size} tokens, the model {engine.config.vocab_size}")
+        if drafts.engine.max_requests < min(len(prompts), max_seqs or engine.max_requests):
+            raise ValueError(f"the drafting model's engine holds {drafts.engine.max_requests} requests, fewer than run at once")
+    limit = engine.max_position
+    generate.runs += 1
+    texts = [_Text(("drafted", generate.runs, i), i, [int(t) for t in p], len(p), Sampler(SamplerConfig(temperature=config.temperature, seed=config.seed + i)))
+             for i, p in enumerate(prompts)]
+    counts = DraftCounts()
+    waiting: Deque[_Text] = deque(texts)
+    running: List[_Text] = []
+    most = min(max_seqs or engine.max_requests, engine.max_requests, engine.max_batch_tokens)
+
+    def leave(t: _Text, reason: Optional[str]) -> None:
+        t.reason = reason
+        if engine.cache.has(t.rid):
+            engine.free_request(t.rid)
+        drafts.drop(t.rid)
+
+    def read(t: _Text) -> None:
+        """All of a text but its last token into the cache."""
+        engine.add_request(t.rid, t.tokens)
+        for a in range(engine.length(t.rid), len(t.tokens) - 1, engine.max_batch_tokens):
+            engine.step([StepEntry(t.rid, t.tokens[a:min(a + engine.max_batch_tokens, len(t.tokens) - 1)])])
+
+    def propose(room: int):
+        rooms = [max(0, min(room, max_tokens - (len(t.tokens) - t.prompt) - 1, limit - len(t.tokens))) for t in running]
+        if isinstance(drafts, DraftModel) and max(rooms) > 0:
+            try:
+                trees, logits = drafts.propose_all([t.rid for t in running], [t.tokens for t in running], rooms, [config.temperature] * len(running))
+                return trees, None if config.greedy else logits
+            except OutOfPages:                           # (of the drafting model: it begins anew with the next step)
+                for t in running:
+                    drafts.drop(t.rid)
+        return [drafts.propose(t.tokens, r) if r and isinstance(drafts, PromptLookup) else ([t.tokens[-1]], [-1]) for t, r in zip(running, rooms)], None
+
+    def numbers(trees) -> Optional[np.ndarray]:
+        """The requests' random numbers: a row's second one is that of the token behind it, counted from the text's end, so that what is drawn
+        does not depend on what was drafted; the first ones, of drafts with a distribution, come behind those."""
+        if config.greedy:
+            return None
+        parts = []
+        for t, (_, parents) in zip(running, trees):
+            depth = []
+            for p in parents:
+                depth.append(depth[p] + 1 if depth else 0)
+            while len(t.draws) <= max(depth):
+                t.draws.append(t.sampler.rng.next_f32())
+            coins = [coin.next_f32() for _ in parents]
+            parts.append(np.stack([np.array(coins, np.float32), np.array([t.draws[d] for d in depth], np.float32)], axis=1))
+        return np.concatenate(parts)
+
+    coin = Rng(config.seed ^ 0x5DEECE66D)
+    try:
+        while waiting or running:
+            while waiting and len(running) < most:
+                t = waiting[0]
+                if max_tokens <= len(t.tokens) - t.prompt or len(t.tokens) >= limit:
+                    waiting.popleft()
+                    leave(t, LENGTH)
+                    continue
+                try:
+                    read(t)
+                except OutOfPages:
+                    leave(t, LENGTH if not running else None)      # alone it is too long for the cache
+                    if running:
+                        break
+                    waiting.popleft()
+                    continue
+                waiting.popleft()
+                running.append(t)
+            if not running:
+                continue
+            room = engine.max_batch_tokens // len(running) - 1
+            trees, logits = propose(min(room, kernels.TREE_MAX_ROWS - 1))
+            kept = None
+            while kept is None:
+                entries = [StepEntry(t.rid, tokens, parents=parents) for t, (tokens, parents) in zip(running, trees)]
+                try:
+                    kept = engine.verify_step(entries, [config.temperature] * len(running), numbers(trees), logits)
+                except OutOfPages:
+                    if any(len(tokens) > 1 for tokens, _ in trees):
+                        trees, logits = [([t.tokens[-1]], [-1]) for t in running], None
+                        continue
+                    t = running.pop()
+                    if not running:
+                        leave(t, LENGTH)
+                        break
+                    leave(t, None)
+                    waiting.appendleft(t)
+                    trees = trees[:-1]
+            if kept is None:
+                continue
+            done = []
+            for t, k, (tokens, _) in zip(running, kept, trees):
+                if k.next_token < 0:
+                    raise ValueError(f"prompt {t.index}: the model's logits are no distribution")
+                counts.steps += 1
+                counts.drafted += len(tokens) - 1
+                counts.accepted += len(k.tokens)
+                for token in k.tokens + [k.next_token]:
+                    if t.draws:
+                        t.draws.pop(0)
+                    if token in stop:
+                        done.append((t, STOP))
+                        break
+                    t.tokens.append(token)
+                    if len(t.tokens) - t.prompt >= max_tokens or len(t.tokens) >= limit:
+                        done.append((t, LENGTH))
+                        break
+            for t, reason in done:
+                running.remove(t)
+                leave(t, reason)
+        engine.check()
+    finally:
+        for t in running + list(waiting):
+            leave(t, t.reason)
+    return [t.tokens[t.prompt:] for t in texts], [t.reason for t in texts], counts
+
+
+generate.runs = 0

@@ -9,6 +9,7 @@ Trace replay, the scheduler and the generator all drive this same function.
 """
 from __future__ import annotations
 
+import functools
 import gc
 from dataclasses import dataclass, field
 from typing import Dict, List, Optional, Sequence
@@ -22,7 +23,7 @@ from ..cache.manager import CacheManager, GroupSpec, OutOfPages
 from ..config.registry import get_architecture, load_config
 from ..config.specs import ModelConfig, with_cache_bits
 from ..weights.loader import load_parameters, open_model_weights
-from .context import Scratch, SeqInfo, StepContext, WeightOrder
+from .context import Scratch, SeqInfo, StepContext, TreeRows, WeightOrder
 from .model import DecoderModel
 
 _DTYPES = {"bfloat16": torch.bfloat16, "bf16": torch.bfloat16, "float32": torch.float32, "fp32": torch.float32,
@@ -43,10 +44,34 @@ def parse_dtype(name) -> torch.dtype:
 @dataclass
 class StepEntry:
     """One request's share of a step: its next tokens, and the indices among them whose logits
-    are wanted (possibly none)."""
+    are wanted (possibly none). With ``parents`` the tokens are a tree: the first one follows what the cache holds (its parent is
+    -1), token i follows token parents[i] < i, and several may follow the same one (drafts, see ``Engine.verify_step``)."""
     request: object
     tokens: Sequence[int]
     want: Sequence[int] = field(default_factory=list)
+    parents: Optional[Sequence[int]] = None
+
+
+@dataclass
+class Kept:
+    """What became of a request's tree of drafted tokens (``Engine.verify_step``)."""
+    rows: List[int]          # the tree's rows that the cache keeps: the first one, then the drafted tokens that were accepted
+    tokens: List[int]        # the accepted tokens (rows[1:])
+    next_token: int          # the token that follows them, not in the cache yet
+
+
+@functools.lru_cache(maxsize=4096)
+def tree_layout(parents: tuple):
+    """(depths int32 [rows], bits uint32 [rows, words] of the rows that each sees, whether the tree is a chain) of a tree."""
+    if not parents or parents[0] != -1 or any(not 0 <= p < i for i, p in enumerate(parents) if i):
+        raise ValueError("a tree's parents are -1 for its first token and earlier tokens of the tree for all others")
+    depths, see = [], []
+    for i, p in enumerate(parents):
+        depths.append(depths[p] + 1 if i else 0)
+        see.append((see[p] if i else 0) | 1 << i)
+    words = -(-len(parents) // kernels.TREE_WORD)
+    bits = np.array([[s >> kernels.TREE_WORD * w & 0xFFFFFFFF for w in range(words)] for s in see], dtype=np.uint32)
+    return np.array(depths, dtype=np.int32), bits, all(p == i - 1 for i, p in enumerate(parents))
 
 
 class Engine:
@@ -117,7 +142,9 @@ class Engine:
         self.max_graphs = 128
         self.graph_replays = 0
         self.sampled: Optional[torch.Tensor] = None
+        self._draws = self._trees = None
         self._sampled_host: Optional[torch.Tensor] = None
+        self._kept_host: Optional[torch.Tensor] = None
         self._ones = np.ones(self.max_graph_batch, dtype=np.int32)
         self._zeros = np.zeros(self.max_graph_batch, dtype=np.int32)
         self._ones_u8 = np.ones(self.max_graph_batch, dtype=np.uint8)
@@ -184,8 +211,9 @@ class Engine:
         self._stage_events[i].record()
         self.h2d_bytes_last = n * 4
 
-    def _layout(self, n: int, S: int, n_want: int, max_pages: int):
-        key = (n, S, n_want, max_pages)
+    def _layout(self, n: int, S: int, n_want: int, max_pages: int, words: int = 0):
+        """Where the step's metadata lie in their block. ``words``: the step's rows are trees, whose rows see others by bits, so many words each."""
+        key = (n, S, n_want, max_pages, words)
         off = self._layouts.get(key)
         if off is not None:
             return off
@@ -202,6 +230,10 @@ class Engine:
             cur += n
             off[f"tables{g}"] = cur
             cur += S * max_pages
+        if words:
+            for name, size in (("visible", n * words), ("parents", n), ("uniform", 2 * n), ("temperature", S)):
+                off[name] = cur
+                cur += size
         off["_size"] = cur
         names = ["tokens", "positions", "row_seq", "want", "seq_first_row", "seq_start_pos", "seq_slots", "want_slots",
                  "token_slots"] + \
@@ -235,9 +267,10 @@ class Engine:
                               first_row=int(info[i, 2])) for i, e in enumerate(entries)]
         return host
 
-    def _bind(self, ctx: StepContext, dev: torch.Tensor, off, n, S, n_want, max_pages) -> None:
+    def _bind(self, ctx: StepContext, dev: torch.Tensor, off, n, S, n_want, max_pages, words: int = 0, most: int = 0) -> None:
         n_groups = len(self.cache.groups)
         ctx.n, ctx.num_wanted = n, n_want
+        ctx.tree = TreeRows(dev[off["visible"]:off["visible"] + n * words].view(n, words), most) if words else None
         ctx.tokens = dev[off["tokens"]:off["tokens"] + n]
         ctx.positions = dev[off["positions"]:off["positions"] + n]
         ctx.row_seq = dev[off["row_seq"]:off["row_seq"] + n]
@@ -274,6 +307,8 @@ class Engine:
             for w in e.want:
                 if not 0 <= w < k:
                     raise ValueError(f"request {e.request!r}: wanted index {w} outside its {k} tokens")
+            if e.parents is not None and len(e.parents) != k:
+                raise ValueError(f"request {e.request!r}: {len(e.parents)} parents for its {k} tokens")
         return n
 
     def step(self, entries: Sequence[StepEntry], reserve: bool = True, commit: bool = True,
@@ -292,8 +327,16 @@ class Engine:
         table sizes rounded up to powers of two, padding rows skipped by every kernel); any other
         step launches its kernels one by one. Both run the same kernels on the same data. Recorded steps are kept for good, each with
         a logits buffer of its own: a caller whose steps come in every size names a ``room``, and steps that are not made of single
-        tokens are recorded for at least that many rows and wanted rows."""
+        tokens are recorded for at least that many rows and wanted rows.
+
+        Where an entry names ``parents``, every request brings a tree (one without is a chain). Which of its rows stay is known only
+        afterwards: ``commit`` has to be False then, and ``verify_step`` does all of it."""
         n = self._validate(entries)
+        trees = any(e.parents is not None for e in entries)
+        if trees:
+            if commit or sampling is not None:
+                raise ValueError("a step of drafted trees commits and samples nothing by itself (verify_step)")
+            self._validate_trees(entries)
         self.sampled = None
         if reserve:
             done = []
@@ -313,6 +356,10 @@ class Engine:
         max_pages = max(max(self.cache.table_len(g, e.request) for e in entries) for g in range(n_groups)) \
             if n_groups else 1
         n_want = sum(len(e.want) for e in entries)
+        if trees:
+            logits = self._step_trees(entries, n, S, n_want, max_pages)
+            self.steps += 1
+            return logits
         decode_only = self.use_graphs and n == S and n_want == S and S <= self.max_graph_batch \
             and self.model.recordable(True)
         if decode_only:
@@ -382,6 +429,137 @@ class Engine:
             self.cache.commit_many([e.request for e in entries], self._tok_count, self._tokens)
         self.steps += 1
         return logits
+
+    def _validate_trees(self, entries) -> None:
+        if not self.model.takes_trees:
+            raise ValueError(f"{self.config.architecture} takes no drafted trees with this cache (a part carries something from row to row, "
+                             f"or the cache holds 4 bits)")
+        most = max(len(e.tokens) for e in entries)
+        if most > kernels.TREE_MAX_ROWS:
+            raise ValueError(f"a tree of {most} tokens is not built (up to {kernels.TREE_MAX_ROWS})")
+        for e in entries:
+            if e.parents is not None:
+                tree_layout(tuple(e.parents))
+
+    def _step_trees(self, entries, n: int, S: int, n_want: int, max_pages: int) -> torch.Tensor:
+        """The rows of trees of drafted tokens through the model; nothing is committed. Like other steps they are replayed as graphs of a rounded shape: rows
+        and wanted rows in eights (above 64 in 64s), requests, the longest tree and the table width in powers of two. What the step's trees look
+        like stays in ``self._trees`` for the verification."""
+        trees = [tree_layout(tuple(e.parents) if e.parents is not None else tuple(range(-1, len(e.tokens) - 1))) for e in entries]
+        most = max(8, 1 << (max(len(e.tokens) for e in entries) - 1).bit_length())
+        words = -(-most // kernels.TREE_WORD)
+        small_logits = (n_want + 64) * self.config.vocab_size * 4 <= (64 << 20)      # each graph owns its logits buffer
+        recorded = self.use_graphs and small_logits and self.model.recordable(False)
+        g, shape = None, (n, S, n_want, max_pages)
+        if recorded:
+            rounded = lambda rows: -(-rows // 8) * 8 if rows <= 64 else -(-rows // 64) * 64
+            S_b = 1 << (S - 1).bit_length()
+            shape = (rounded(n + S_b - S), S_b, rounded(n_want), max(8, 1 << max(max_pages - 1, 0).bit_length()))
+            key = ("trees",) + shape + (most,)
+            g = self._graphs.get(key)
+            if g is None:
+                if len(self._seen) > 4096:
+                    self._seen.clear()
+                self._seen[key] = self._seen.get(key, 0) + 1
+                if self._seen[key] < 2 or len(self._graphs) >= self.max_graphs:
+                    recorded, shape = False, (n, S, n_want, max_pages)
+        off = self._layout(*shape, words)
+        host = self._fill(entries, off, *shape)
+        row = 0
+        parents, positions = host[off["parents"]:off["parents"] + shape[0]], host[off["positions"]:off["positions"] + shape[0]]
+        visible = host[off["visible"]:off["visible"] + shape[0] * words].view(np.uint32).reshape(shape[0], words)
+        for e, seq, (depths, bits, _) in zip(entries, self._seqs, trees):
+            k = len(e.tokens)
+            parents[row:row + k] = e.parents if e.parents is not None else np.arange(-1, k - 1)
+            positions[row:row + k] = seq.start_pos + depths
+            visible[row:row + k, :bits.shape[1]] = bits
+            row += k
+        uniform, temperature = self._draws if self._draws is not None else (None, None)
+        if uniform is not None:
+            host[off["uniform"]:off["uniform"] + 2 * n] = uniform.reshape(-1).view(np.int32)
+        if temperature is not None:
+            host[off["temperature"]:off["temperature"] + S] = temperature.view(np.int32)
+        if recorded and g is None:
+            g = self._capture(key, off, host, *shape, most, decode_only=False, words=words)
+            logits, dev = g["logits"][:n_want], g["meta"]      # (the warm-up run of the capture computed this step)
+        elif g is not None:
+            self._stage_copy(host, g["meta"])
+            g["graph"].replay()
+            kernels.launch_count += g["nodes"]
+            self.graph_replays += 1
+            logits, dev = g["logits"][:n_want], g["meta"]
+        else:
+            if off["_size"] > self._meta_dev.numel():
+                self._meta_dev = torch.empty(1 << int(off["_size"] - 1).bit_length(), dtype=torch.int32, device=self.device)
+            self._stage_copy(host, self._meta_dev)
+            ctx, dev = self.ctx, self._meta_dev
+            self._bind(ctx, dev, off, *shape, words, most)
+            ctx.seqs, ctx.max_context = self._seqs, self._max_ctx
+            ctx.max_rows_per_seq, ctx.decode_only, ctx.leading_single = most, False, 0
+            logits = self.model.forward(ctx)
+        self._trees = (dev, off, shape, most, all(chain for _, _, chain in trees))
+        return logits
+
+    def verify_step(self, entries: Sequence[StepEntry], temperatures: Optional[Sequence[float]] = None, uniform: Optional[np.ndarray] = None,
+                    draft_logits: Optional[torch.Tensor] = None, reserve: bool = True) -> List[Kept]:
+        """Run trees of drafted tokens and keep of each what the model would have written itself. An entry's first token is the one that its request was
+        given last, the others are drafts (``parents`` None: a chain of them; a single token: no drafts, one step of decoding). ``temperatures`` of the
+        requests (None: greedy). ``uniform`` float32 [all rows, 2], in the order of the entries and their tokens, are the random numbers that
+        requests with a temperature use up; ``draft_logits`` [all rows, vocab] (float32, on the device) the logits that each row's children
+        were drawn from, None for drafts that come from no distribution (``kernels.verify_tree``).
+
+        The cache then holds the kept rows of each request one behind the other, as if they had been decoded one by one, and knows their tokens."""
+        n = sum(len(e.tokens) for e in entries)
+        temperature = np.zeros(len(entries), dtype=np.float32) if temperatures is None else np.ascontiguousarray(temperatures, dtype=np.float32)
+        if temperature.shape != (len(entries),):
+            raise ValueError(f"{temperature.shape} temperatures for {len(entries)} requests")
+        if uniform is None:
+            if (temperature > 0).any():
+                raise ValueError("requests with a temperature need random numbers")
+        else:
+            uniform = np.ascontiguousarray(uniform, dtype=np.float32)
+            if uniform.shape != (n, 2):
+                raise ValueError(f"random numbers of shape {uniform.shape} for {n} rows, not {(n, 2)}")
+        vocab = self.config.vocab_size
+        if draft_logits is not None and (draft_logits.shape != (n, vocab) or draft_logits.dtype != torch.float32):
+            raise ValueError(f"draft_logits must be float32 [{n}, {vocab}]")
+        for e in entries:
+            for t in e.tokens:
+                if not 0 <= t < vocab:
+                    raise ValueError(f"request {e.request!r}: token {int(t)} is outside the vocabulary of {vocab}")
+        trees = [StepEntry(e.request, e.tokens, range(len(e.tokens)), e.parents if e.parents is not None else range(-1, len(e.tokens) - 1)) for e in entries]
+        self._draws = (uniform, temperature)
+        try:
+            logits = self.step(trees, reserve=reserve, commit=False)
+        finally:
+            self._draws = None
+        dev, off, shape, most, chains = self._trees
+        S = len(entries)
+        part = lambda name, count: dev[off[name]:off[name] + count]
+        out = self.scratch.flat("kept", self.max_batch_tokens + 2 * self.max_requests, torch.int32)[:n + 2 * S]
+        path, accepted, following = out[:n], out[n:n + S], out[n + S:]
+        first_row = part("seq_first_row", S + 1)
+        kernels.verify_tree(logits, part("tokens", n), part("parents", n), first_row, part("uniform", 2 * n).view(torch.float32).view(n, 2),
+                            part("temperature", S).view(torch.float32), path, accepted, following, draft_logits)
+        if not chains:                                   # (a chain's kept rows are where they belong)
+            for g in range(len(self.cache.groups)):
+                tables = part(f"tables{g}", S * shape[3]).view(S, shape[3])
+                kernels.keep_rows(self.device_cache.k[g], self.device_cache.v[g], tables, first_row, part("seq_start_pos", S), path, accepted, self.page_size, most,
+                                  self.status)
+        if self._kept_host is None or self._kept_host.numel() < out.numel():
+            self._kept_host = torch.empty(max(256, 1 << (out.numel() - 1).bit_length()), dtype=torch.int32).pin_memory()
+        self._kept_host[:out.numel()].copy_(out, non_blocking=True)
+        torch.cuda.current_stream().synchronize()
+        host = self._kept_host.numpy()[:out.numel()].tolist()
+        result, row = [], 0
+        for i, e in enumerate(entries):
+            rows = host[row:row + host[n + i]]
+            tokens = [int(e.tokens[r]) for r in rows]
+            result.append(Kept(rows, tokens[1:], host[n + S + i]))
+            self.cache.commit(e.request, tokens)
+            self.cache.truncate(e.request, self.cache.length(e.request))       # (pages for rows that were not kept)
+            row += len(e.tokens)
+        return result
 
     def _decode_graph(self, Sb: int, Pb: int):
         """The CUDA graph of a decode step of ``Sb`` rows with block tables ``Pb`` wide, recorded if new."""
@@ -492,7 +670,7 @@ class Engine:
         handle = self.decode_launch(requests, tokens, sample_mask)
         return None if handle is None else self.decode_wait(handle)
 
-    def _capture(self, key, off, host, n, S, n_want, Pb, max_rows, decode_only, lead=0):
+    def _capture(self, key, off, host, n, S, n_want, Pb, max_rows, decode_only, lead=0, words=0):
         """Record the kernels of one step shape into a CUDA graph with a metadata block, logits and
         scratch of its own. The kernels run once outside capture first, on the metadata given (for a
         decode shape an all-padding batch; otherwise the real step, which is thereby computed), so
@@ -500,7 +678,7 @@ class Engine:
         meta = torch.empty(off["_size"], dtype=torch.int32, device=self.device)
         ctx = StepContext(scratch=self.scratch, cache=self.device_cache, status=self.status, dtype=self.dtype,
                           grow_scratch=Scratch(self._scratch_rows, self.dtype, self.device))
-        self._bind(ctx, meta, off, n, S, n_want, Pb)
+        self._bind(ctx, meta, off, n, S, n_want, Pb, words, max_rows)
         ctx.weight_order = self.weight_order
         ctx.side_stream = self.side_stream
         if self.use_programs:
@@ -517,6 +695,8 @@ class Engine:
             if decode_only and S == n:      # rows whose token is what the step before sampled take it on the device
                 kernels.resolve_tokens(ctx.tokens, ctx.token_slots, self.device_cache.last_token)
             logits = self.model.forward(ctx)
+            if words:                       # (drafted trees are verified, not sampled)
+                return logits
             kernels.sample(logits, sampled[:n_want], want_slots=ctx.want_slots, state=self.device_cache.sampling,
                            last_token=self.device_cache.last_token)
             return logits

@@ -53,6 +53,9 @@ class DecoderModel:
         #: no part enqueues device work behind the kernel library's back
         self.program_safe = all(p.launches_through_kernels_only for p in self.parts())
 
+        #: whether requests may bring trees of drafted tokens: only when every part knows such rows
+        self.takes_trees = all(p.takes_trees for p in self.parts())
+
     def param_specs(self) -> Dict[str, ParamSpec]:
         return dict(self._specs)
 

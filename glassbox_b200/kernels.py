@@ -2667,9 +2667,15 @@ def _tree_splits(kind: int, num_seqs: int, most: int, nh: int, nkv: int, hd: int
 def tree_attention_parts(q: torch.Tensor, nh: int, nkv: int, hd: int, num_seqs: int, max_rows_per_seq: int, max_context: int,
                          window: Optional[int] = None) -> Optional[torch.Tensor]:
     """Scratch for ``tree_attention`` of these sizes (None: it needs none). Calls that follow one another on a stream may share it."""
+    floats = tree_attention_floats(q.shape[0], nh, nkv, hd, num_seqs, max_rows_per_seq, max_context, window)
+    return torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
+
+
+def tree_attention_floats(n: int, nh: int, nkv: int, hd: int, num_seqs: int, max_rows_per_seq: int, max_context: int, window: Optional[int] = None) -> int:
+    """Numbers of the scratch for ``tree_attention`` of ``n`` rows (0: it needs none)."""
     # (the kernel is chosen by the tensors' alignment, too: as much as the one that needs more)
-    splits = max(_tree_splits(kind, num_seqs, max_rows_per_seq, nh, nkv, hd, max_context, int(window or 0)) for kind in (0, 1))
-    return torch.empty(splits * q.shape[0] * nh * (hd + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
+    splits = max(_tree_splits(kind, num_seqs, max_rows_per_seq, nh, nkv, hd, int(max_context), int(window or 0)) for kind in (0, 1))
+    return splits * n * nh * (hd + 2) if splits > 1 else 0
 
 
 def _tree_batch(block_tables, seq_first_row, seq_start_pos) -> int:

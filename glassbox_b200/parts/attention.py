@@ -10,6 +10,9 @@ this run are not stored and attention reads what the named cache layer already h
 ``cache_bits`` 4: keys and values are rounded to four bits on their way into the pages, one kernel rotates and stores; decoded
 tokens read the pages as they are, portions of prompts from pages of the activation type that they are unpacked into, one
 layer's worth that all layers share.
+
+Rows that are a tree of drafted tokens (``ctx.tree``) see what the cache held before and of the tree their ancestors and themselves; a cache in 4 bits takes no
+trees.
 """
 from __future__ import annotations
 
@@ -42,6 +45,10 @@ class GqaAttention(Mixer):
         self.position = build_part("position", s.position)
         if getattr(self.position, "pairing", "half") != "half":
             raise ValueError("grouped-query attention rotates channel i with channel i + rotary_dim/2 only")
+
+    @property
+    def takes_trees(self) -> bool:
+        return self.spec.cache_bits is None
 
     def sub_parts(self):
         return {"position": self.position}
@@ -109,6 +116,13 @@ class GqaAttention(Mixer):
         decode kernel, the portions to the flash kernel, which would otherwise spend a 128-row tile per
         head on each of them."""
         n = q.shape[0]
+        if getattr(ctx, "tree", None) is not None:
+            s, most = self.spec, ctx.tree.max_rows
+            floats = kernels.tree_attention_floats(n, self.nh, self.nkv, self.hd, ctx.num_seqs, most, ctx.max_context, s.window)
+            parts = ctx.scratch("tree_parts", (1, floats), torch.float32, grow=True).view(-1) if floats else None
+            kernels.tree_attention(q, att, cache.k, cache.v, cache.block_tables, ctx.seq_first_row, ctx.seq_start_pos, ctx.positions, ctx.tree.visible, most,
+                                   self.nh, self.nkv, self.hd, cache.page_size, s.scale, s.window, ctx.max_context, parts, ctx.status)
+            return
         if ctx.decode_only:
             if self._attend_decode(ctx, q, att, cache, n):
                 return

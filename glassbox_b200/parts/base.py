@@ -110,6 +110,11 @@ class Part:
     #: kernel by kernel.
     launches_through_kernels_only = False
 
+    #: True when a request's rows of a step may be a tree of drafted tokens (``ctx.tree``) and not only neighbours in the text: the part
+    #: takes every row by itself, from its position, or looks at what the tree's rows see. Parts that carry something from
+    #: row to row keep the default, and their models take no drafted trees.
+    takes_trees = False
+
     def recordable(self, decode_only: bool) -> bool:
         """Whether a step through this part can be recorded once and replayed as a CUDA graph (``decode_only``: a step
         in which every request brings exactly one row). It can when the part reads everything that changes from step

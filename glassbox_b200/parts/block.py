@@ -21,6 +21,7 @@ from .norm import ResidualItself
 
 class PreNormBlock(Part):
     launches_through_kernels_only = True
+    takes_trees = True
 
     def __init__(self, spec, *, hidden_size: int):
         super().__init__(spec)

@@ -14,6 +14,7 @@ from .linear import linear
 
 class Embedding(TokenEmbedding):
     launches_through_kernels_only = True
+    takes_trees = True
 
     def __init__(self, spec=None, *, vocab_size: int, hidden_size: int):
         super().__init__(spec)
@@ -28,6 +29,7 @@ class Embedding(TokenEmbedding):
 
 class LmHead(OutputHead):
     launches_through_kernels_only = True
+    takes_trees = True
 
     def __init__(self, spec=None, *, vocab_size: int, hidden_size: int):
         super().__init__(spec)

@@ -14,6 +14,7 @@ from .linear import activated_linear, clamped_glu_linear, gated_linear, linear, 
 class SwiGlu(FeedForward):
     accepts_deferred_input = True
     launches_through_kernels_only = True
+    takes_trees = True
 
     def __init__(self, spec, *, hidden_size: int):
         super().__init__(spec)
@@ -40,6 +41,7 @@ class GeluGlu(FeedForward):
     product."""
     accepts_deferred_input = True
     launches_through_kernels_only = True
+    takes_trees = True
     can_overwrite_output = True
 
     def __init__(self, spec, *, hidden_size: int):
@@ -65,6 +67,7 @@ class SquaredRelu(FeedForward):
     """Dense feed-forward without a gate: residual += (relu(h Wup^T))^2 Wdown^T, no bias."""
     accepts_deferred_input = True
     launches_through_kernels_only = True
+    takes_trees = True
     can_overwrite_output = True
 
     def __init__(self, spec, *, hidden_size: int):
@@ -91,6 +94,7 @@ class GeluMlp(FeedForward):
     in float32 from the float32 sums of the first product."""
     accepts_deferred_input = True
     launches_through_kernels_only = True
+    takes_trees = True
     can_overwrite_output = True
 
     def __init__(self, spec, *, hidden_size: int):

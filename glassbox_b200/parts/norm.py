@@ -9,6 +9,7 @@ from .base import Norm, register_part
 
 class RmsNorm(Norm):
     launches_through_kernels_only = True
+    takes_trees = True
     renorms_parts = True
 
     def __init__(self, spec, *, hidden_size: int):
@@ -61,6 +62,7 @@ class LayerNorm(Norm):
     """out_j = (x_j - mean) / sqrt(var + eps) * w_j + b_j over a row, var the mean of the squared deviations; statistics
     and the result in float32, rounded once to the activation dtype. The bias is optional (``spec.bias``)."""
     launches_through_kernels_only = True
+    takes_trees = True
 
     def __init__(self, spec, *, hidden_size: int):
         super().__init__(spec)

@@ -67,6 +67,7 @@ class Rope(Position):
     ask for ``inv_freq`` and ``magnitude`` and form the angle float32(position) * inv_freq[i] and its sine and cosine, times
     the magnitude, on the device, so no largest position has to be known beforehand."""
     launches_through_kernels_only = True
+    takes_trees = True
 
     def __init__(self, spec, **_):
         super().__init__(spec)
@@ -98,6 +99,7 @@ class Rope(Position):
 
 class NoPosition(Position):
     launches_through_kernels_only = True
+    takes_trees = True
 
     def __init__(self, spec=None, **_):
         super().__init__(spec)
