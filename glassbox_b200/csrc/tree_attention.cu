@@ -207,31 +207,56 @@ static int ta_dispatch(const TreeArgs& a, int num_seqs, int max_rows, cudaStream
     return rc ? rc : gb_check_launch("gb_tree_attention");
 }
 
-int gb_tree_attention_mma(const TreeArgs& a, int num_seqs, int max_rows, cudaStream_t stream);      // tree_attention_mma.cu
+// tree_attention_mma.cu
+int gb_tree_attention_mma(const TreeArgs& a, const TreePlan& plan, int num_seqs, int max_rows, cudaStream_t stream);
+TreePlan tree_plan_mma(int num_seqs, int max_rows, int nh, int nkv, int hd, int max_context, int window);
 
-// kind 0: this file's kernel; 1: the tensor cores (bfloat16). q, out: [n, nh * hd], rows `stride` numbers apart; kcache, vcache: [num_pages, nkv, page_size, hd].
+// Shares of a request's keys in this file's kernel, so that blocks fill the GPU, of 128 keys at least.
+static int ta_splits(int num_seqs, int max_rows, int nh, int nkv, int max_context, int window) {
+    const long long blocks = (long long)num_seqs * nkv * gb_ceil_div((long long)max_rows * (nh / nkv), TA_ROWS);
+    const int reach = window > 0 && window + max_rows < max_context ? window + max_rows : max_context, most = reach <= 128 ? 1 : gb_ceil_div(reach, 128);
+    const long long splits = 148ll * 3 / blocks;
+    return splits > most ? most : splits < 1 ? 1 : (int)splits;
+}
+
+// Numbers (float32) of the scratch that a call needs; -1: more than there can be. kind as below.
+GB_EXPORT int gb_tree_attention_floats(int kind, int n, int num_seqs, int max_rows, int nh, int nkv, int hd, int max_context, int window) {
+    if (n <= 0 || num_seqs <= 0 || max_rows <= 0 || nkv <= 0 || nh % nkv) return 0;
+    long long floats;
+    if (kind == 1) {
+        floats = tree_plan_mma(num_seqs, max_rows, nh, nkv, hd, max_context, window).floats;
+    } else {
+        const int splits = ta_splits(num_seqs, max_rows, nh, nkv, max_context, window);
+        floats = splits > 1 ? (long long)splits * n * nh * (hd + 2) : 0;
+    }
+    return floats < (1ll << 31) ? (int)floats : -1;
+}
+
+// kind 0: this file's kernel; 1: the tensor cores (bfloat16). q, out: [n, nh * hd], rows `stride` numbers apart; kcache, vcache: [num_pages, nkv, page_size, hd];
+// parts: gb_tree_attention_floats of the same sizes.
 GB_EXPORT int gb_tree_attention(int kind, const void* q, long long q_stride, void* out, long long out_stride, int dtype, const void* kcache, const void* vcache,
                                 const int* block_tables, int max_pages, const int* first_row, const int* start_pos, const int* positions, const int* visible,
                                 int words, int n, int num_seqs, int max_rows, int nh, int nkv, int hd, int page_size, long long num_pages, float scale,
-                                int window, int splits, float* parts, int* status, cudaStream_t stream) {
+                                int window, int max_context, float* parts, int* status, cudaStream_t stream) {
     GB_REQUIRE(nkv > 0 && nh > 0 && nh % nkv == 0 && hd > 0 && hd <= TA_MAX_HD, "gb_tree_attention: %d/%d heads of %d are not built", nh, nkv, hd);
     GB_REQUIRE(n >= 0 && num_seqs >= 0 && num_seqs <= 65535 && max_rows >= 0 && max_pages > 0 && page_size > 0 && num_pages > 0 && words > 0 && window >= 0,
                "gb_tree_attention: bad batch shape");
-    GB_REQUIRE(splits >= 1 && splits <= 65535 && (splits == 1 || parts != nullptr), "gb_tree_attention: bad split count or scratch");
     GB_REQUIRE(dtype == GB_F32 || dtype == GB_BF16, "gb_tree_attention: unsupported dtype %d", dtype);
     GB_REQUIRE((long long)max_pages * page_size < (1ll << 31) - 4096, "gb_tree_attention: the block tables reach too far");
     if (n == 0 || num_seqs == 0 || max_rows == 0) return 0;
     GB_REQUIRE(q && out && kcache && vcache && block_tables && first_row && start_pos && positions && visible && status, "gb_tree_attention: a tensor is missing");
     TreeArgs a = {q, q_stride, out, out_stride, kcache, vcache, block_tables, max_pages, first_row, start_pos, positions, visible, words, n, nh, nkv, hd, page_size,
-                  num_pages, scale, window, splits, parts, status};
-    int rc;
+                  num_pages, scale, window, 1, parts, status};
     if (kind == 1) {
         GB_REQUIRE(dtype == GB_BF16, "gb_tree_attention: the tensor cores' kernel takes bfloat16");
-        rc = gb_tree_attention_mma(a, num_seqs, max_rows, stream);
-    } else {
-        rc = dtype == GB_F32 ? ta_dispatch<float>(a, num_seqs, max_rows, stream) : ta_dispatch<__nv_bfloat16>(a, num_seqs, max_rows, stream);
+        const TreePlan plan = tree_plan_mma(num_seqs, max_rows, nh, nkv, hd, max_context, window);
+        GB_REQUIRE(plan.floats == 0 || parts != nullptr, "gb_tree_attention: the scratch is missing");
+        return gb_tree_attention_mma(a, plan, num_seqs, max_rows, stream);
     }
-    if (rc || splits == 1) return rc;
+    a.splits = ta_splits(num_seqs, max_rows, nh, nkv, max_context, window);
+    GB_REQUIRE(a.splits == 1 || parts != nullptr, "gb_tree_attention: the scratch is missing");
+    const int rc = dtype == GB_F32 ? ta_dispatch<float>(a, num_seqs, max_rows, stream) : ta_dispatch<__nv_bfloat16>(a, num_seqs, max_rows, stream);
+    if (rc || a.splits == 1) return rc;
     const unsigned blocks = (unsigned)(((size_t)n * nh + 3) / 4);
     const cudaError_t e = dtype == GB_F32 ? gb_launch(GB_PDL_ATTENTION, tree_merge_kernel<float>, dim3(blocks), dim3(128), 0, stream, a, num_seqs)
                                           : gb_launch(GB_PDL_ATTENTION, tree_merge_kernel<__nv_bfloat16>, dim3(blocks), dim3(128), 0, stream, a, num_seqs);

@@ -25,9 +25,17 @@ struct TreeArgs {
     long long num_pages;
     float scale;
     int window;              // 0: none
-    int splits;
-    float* parts;            // splits > 1: [splits, n, nh, hd] unnormalised outputs, then [splits, n, nh, 2] maxima (of scores times scale, base 2) and sums
+    int splits;              // (tree_attention.cu)
+    float* parts;
     int* status;
+};
+
+// How a batch is laid out over the GPU.
+struct TreePlan {
+    int rows = 0;            // query rows of an item
+    int cluster = 0;         // blocks that share an item's keys, a cluster; 0: all items' keys are cut evenly among `blocks`
+    int blocks = 0;
+    long long floats = 0;    // of scratch
 };
 
 // A request of the step. rows 0: nothing to do.
@@ -46,6 +54,8 @@ struct TreeSeq {
         length = start + rows;
         key_lo = a.window > 0 ? max(0, start - a.window + 1) : 0;
     }
+    // Tiles of `keys` keys (a multiple of them behind place 0) that hold what any row sees.
+    __device__ __forceinline__ int tiles(int keys) const { return rows > 0 && start >= 0 ? (length + keys - 1) / keys - key_lo / keys : 0; }
     // The page of a place, -1 where there is none.
     __device__ __forceinline__ int page(const TreeArgs& a, int index) const {
         const int p = index < a.max_pages ? table[index] : -1;
@@ -58,5 +68,82 @@ struct TreeSeq {
         const int d = key - start;
         if ((d >> 5) >= a.words || !((unsigned)a.visible[(size_t)row * a.words + (d >> 5)] >> (d & 31) & 1u)) return false;
         return a.window <= 0 || pos - a.positions[row0 + d] < a.window;
+    }
+};
+
+constexpr int TREE_LEAST_SHARE = 4;      // tiles of keys of a block, where there are enough
+
+// All items' tiles of keys in one row, request by request, key/value head by head, `rows` query rows at a time, cut evenly among the blocks. Every warp works
+// it out for itself from the requests' lengths, which only the device knows.
+struct TreeCut {
+    const TreeArgs& a;
+    int num_seqs, rows, keys;
+    long long total, share;
+    int seq;                 // a request, the tiles and items before it
+    long long tile0, item0, tiles_here;
+    __device__ __forceinline__ void of(int s, long long& tiles, long long& items) const {
+        tiles = items = 0;
+        if (s >= num_seqs) return;
+        const int n = a.first_row[s + 1] - a.first_row[s], start = a.start_pos[s];
+        if (n <= 0 || start < 0 || a.first_row[s] < 0 || a.first_row[s] > a.n - n) return;
+        const int low = a.window > 0 ? max(0, start - a.window + 1) : 0;
+        items = (long long)a.nkv * ((n * (a.nh / a.nkv) + rows - 1) / rows);
+        tiles = items * ((start + n + keys - 1) / keys - low / keys);
+    }
+    __device__ __forceinline__ static long long scan(long long v) {
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long up = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += up;
+        }
+        return v;
+    }
+    __device__ __forceinline__ TreeCut(const TreeArgs& a, int num_seqs, int rows, int keys, int blocks, int least) : a(a), num_seqs(num_seqs), rows(rows), keys(keys) {
+        long long sum = 0;
+        for (int s0 = 0; s0 < num_seqs; s0 += 32) {
+            long long t, i;
+            of(s0 + (threadIdx.x & 31), t, i);
+            sum += t;
+        }
+        total = __shfl_sync(0xffffffffu, scan(sum), 31);
+        share = (total + blocks - 1) / blocks;
+        if (share < least) share = least;
+    }
+    // The request that holds tile `at`.
+    __device__ __forceinline__ void seek(long long at) { find(at, -1); }
+    __device__ __forceinline__ void seek_seq(int s) { find(-1, s); }
+    __device__ __forceinline__ void find(long long at, int want) {
+        const int lane = threadIdx.x & 31;
+        long long tiles_before = 0, items_before = 0;
+        for (int s0 = 0; s0 < num_seqs; s0 += 32) {
+            long long t, i;
+            of(s0 + lane, t, i);
+            const long long ts = scan(t), is = scan(i);
+            const unsigned hit = __ballot_sync(0xffffffffu, want >= 0 ? s0 + lane == want : t > 0 && tiles_before + ts > at);
+            if (hit) {
+                const int l = __ffs(hit) - 1;
+                seq = s0 + l;
+                tiles_here = __shfl_sync(0xffffffffu, t, l);
+                tile0 = tiles_before + __shfl_sync(0xffffffffu, ts, l) - tiles_here;
+                item0 = items_before + __shfl_sync(0xffffffffu, is - i, l);
+                return;
+            }
+            tiles_before += __shfl_sync(0xffffffffu, ts, 31);
+            items_before += __shfl_sync(0xffffffffu, is, 31);
+        }
+        seq = -1;
+        tile0 = item0 = tiles_here = 0;
+    }
+    // On to the request that holds tile `at`, which comes later.
+    __device__ __forceinline__ void reach(long long at) {
+        while (at >= tile0 + tiles_here) {
+            long long t, i;
+            of(seq, t, i);
+            tile0 += tiles_here;
+            item0 += i;
+            ++seq;
+            of(seq, tiles_here, i);
+        }
     }
 };

@@ -18,6 +18,8 @@ constexpr int VT_THREADS = 256, VT_WARPS = VT_THREADS / 32;
 constexpr int VT_SEG = 512, VT_EACH = VT_SEG / 32;      // tokens of a segment, and of a lane
 constexpr int VT_MAX_SEGS = 4097;
 constexpr int VT_MAX_CLUSTER = 8;
+constexpr int VT_TABLE = 256;                           // 2^(j / 256)
+constexpr int VT_ROWS = 512;                            // rows of a tree whose parents and tokens stay in shared memory
 
 struct VerifyArgs {
     const void* logits;
@@ -45,13 +47,12 @@ struct VtShare {
 
 struct VtShared {
     VtShare mine[2][2];                // [turn][p, q]
-    double left[2];                    // [turn] of the leftover
-    int token[2];                      // [turn] that the block found, -1: none
-    double warp_sum[VT_WARPS], warp_sum2[VT_WARPS];
-    float warp_most[VT_WARPS], warp_most2[VT_WARPS];
-    int warp_wrong[VT_WARPS];
+    double left;                       // of the leftover
+    int token[2];                      // [turn] that the block found
+    int warp_wrong[2][VT_WARPS];
     unsigned long long warp_best[VT_WARPS];
-    int child, seen;
+    double table[VT_TABLE];
+    int parents[VT_ROWS], tokens[VT_ROWS];
 };
 
 __device__ __forceinline__ unsigned long long vt_key(float x, int id) {      // NaN is below everything
@@ -64,16 +65,59 @@ __device__ __forceinline__ unsigned long long vt_warp_max(unsigned long long key
     const unsigned low = __reduce_max_sync(0xffffffffu, (unsigned)(key >> 32) == high ? (unsigned)key : 0u);
     return (unsigned long long)high << 32 | low;
 }
+__device__ __forceinline__ float vt_warp_max(float v) {                     // (not of NaN)
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
 __device__ __forceinline__ double vt_warp_sum(double v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
+__device__ __forceinline__ double vt_warp_scan(double v) {                  // sums up to and with a lane's
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const double up = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += up;
+    }
+    return v;
+}
 
-// A lane's tokens of a segment, 16 bytes at a time: piece u * 32 + lane of the segment's. Segments begin at multiples of 16 bytes: `lead` numbers before the
-// row's first one. Tokens outside the row have minus infinity.
+// A float32 as a double, by its bits (0 and subnormal ones come out as numbers below 2^-126, as good as 0 beside a logit; infinities as finite ones
+// beyond 2^127): the conversion proper goes through a unit that takes 16 a cycle.
+__device__ __forceinline__ double vt_double(float x) {
+    const unsigned b = __float_as_uint(x);
+    return __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + 0x38000000u)), (int)(b << 29));
+}
+
+// Weights exp((x - most) / T) of logits x <= most: 2^(k / 256) from a table, whole powers of two added to its exponent, and three terms of the exponential
+// series for the rest, at most 1/512 of an octave: a relative error below (ln 2 / 512)^4 / 24 = 2^-42.7. Below e^-700 a weight is nothing.
+struct VtWeight {
+    const double* table;
+    double heat, most;                 // 256 / (T ln 2)
+    float least;
+    __device__ __forceinline__ VtWeight(const double* table, double heat, float temp, float most)
+        : table(table), heat(heat), most(vt_double(most)), least(fmaf(-700.0f, temp, most)) {}
+    __device__ __forceinline__ double operator()(float x) const {
+        constexpr double MAGIC = 6755399441055744.0;                  // 1.5 2^52: the low word of a sum with it is the nearest whole number
+        constexpr double C1 = 0.0027076061740622863, C2 = 3.665565596910106e-06, C3 = 3.308302680541371e-09;      // (ln 2 / 256)^i / i!
+        const double d = vt_double(fmaxf(x, least)) - most;
+        const double s = fma(d, heat, MAGIC);
+        const int k = __double2loint(s);
+        const double r = fma(d, heat, MAGIC - s);
+        const double t = table[k & (VT_TABLE - 1)];
+        const double w = __hiloint2double(__double2hiint(t) + ((k >> 8) << 20), __double2loint(t));
+        const double v = fma(w * r, fma(fma(C3, r, C2), r, C1), w);
+        return x >= least && x > -INFINITY ? v : 0.0;
+    }
+};
+
+// A lane's tokens of a segment, 16 bytes at a time: piece u * 32 + lane of the segment's. Segments begin at multiples of 16 bytes of one tensor's rows, `lead`
+// numbers before the row's first; `aligned`: of this one's, too. Tokens outside the row have minus infinity.
 template <typename T>
-__device__ __forceinline__ void vt_load(const T* x, int lead, int vocab, int seg, float (&v)[VT_EACH]) {
+__device__ __forceinline__ void vt_load(const T* x, int lead, bool aligned, int vocab, int seg, float (&v)[VT_EACH]) {
     constexpr int N = 16 / sizeof(T);
     const int lane = threadIdx.x & 31;
     uint4 raw[VT_EACH / N];
@@ -81,7 +125,7 @@ __device__ __forceinline__ void vt_load(const T* x, int lead, int vocab, int seg
 #pragma unroll
     for (int u = 0; u < VT_EACH / N; ++u) {
         const int i = seg * VT_SEG + (u * 32 + lane) * N - lead;
-        whole[u] = i >= 0 && i + N <= vocab;
+        whole[u] = aligned && i >= 0 && i + N <= vocab;
         raw[u] = whole[u] ? *reinterpret_cast<const uint4*>(x + i) : make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
@@ -101,17 +145,21 @@ __device__ __forceinline__ void vt_load(const T* x, int lead, int vocab, int seg
 }
 
 template <typename T>
-__global__ void __launch_bounds__(VT_THREADS) verify_tree_kernel(const VerifyArgs a) {
+__global__ void __launch_bounds__(VT_THREADS, 2) verify_tree_kernel(const VerifyArgs a) {
     namespace cg = cooperative_groups;
     constexpr int N = 16 / sizeof(T);
     extern __shared__ __align__(16) double vt_mem[];
     __shared__ VtShared sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int C = a.blocks, rank = blockIdx.x % C, seq = blockIdx.x / C, vocab = a.vocab;
-    const int most_segs = (vocab + N + VT_SEG - 1) / VT_SEG, per = (most_segs + C - 1) / C;
-    double* p_sum = vt_mem;                            // of the block's segments: sums of exp((x - most) / T), then (drafted) the leftover's
-    double* r_sum = p_sum + per;
-    float* p_most = reinterpret_cast<float*>(r_sum + (a.draft ? per : 0));
+    const int per = ((vocab + N + VT_SEG - 1) / VT_SEG + C - 1) / C;
+    // of the block's segments: sums and largest logits of p, with drafted distributions of q, too, and the leftover's sums
+    double* p_sum = vt_mem;
+    double* q_sum = p_sum + per;
+    double* r_sum = a.draft ? q_sum + per : q_sum;
+    float* p_most = reinterpret_cast<float*>(a.draft ? r_sum + per : q_sum);
+    float* q_most = p_most + per;
+    for (int i = tid; i < VT_TABLE; i += VT_THREADS) sh.table[i] = exp2((double)i / VT_TABLE);
     gb_pdl_launch_dependents();
     gb_pdl_wait();
     const int row0 = a.first_row[seq], rows = a.first_row[seq + 1] - row0;
@@ -123,22 +171,22 @@ __global__ void __launch_bounds__(VT_THREADS) verify_tree_kernel(const VerifyArg
     }
     const float temp = a.temperature[seq];
     const bool draws = temp > 0.f, drafted = draws && a.draft != nullptr;
-    const double heat = draws ? 1.0 / (double)temp : 0.0;
+    const double heat = draws ? (double)VT_TABLE / ((double)temp * 0.6931471805599453) : 0.0;
+    for (int i = tid; i < rows && i < VT_ROWS; i += VT_THREADS) { sh.parents[i] = a.parents[row0 + i]; sh.tokens[i] = a.tokens[row0 + i]; }
     if (rank == 0)
         for (int i = tid; i < rows; i += VT_THREADS) a.path[row0 + i] = i == 0 ? 0 : -1;
     __syncthreads();
 
-    // The block's share of a row: its segments' sums (and largest logits, if `keep`), its own in `to`.
-    auto scan = [&](const T* x, bool keep, VtShare& to) {
-        const int lead = (int)((uintptr_t)x & 15) / (int)sizeof(T), segs = (lead + vocab + VT_SEG - 1) / VT_SEG;
-        const int lo = min(rank * per, segs), hi = min(lo + per, segs);
-        float w_most = -INFINITY;
-        double w_sum = 0.0;
+    // The block's share of a row: largest logits and sums of its segments, and its own in `to` (for whom the cluster's barrier is still to come).
+    auto scan = [&](const T* x, int lead, int lo, int hi, double* sums, float* mosts, int which, VtShare& to) {
+        const bool aligned = ((uintptr_t)(x - lead) & 15) == 0;
         bool wrong = false;
         unsigned long long best = 0;
+        float v[VT_EACH];
+        if (lo + warp < hi) vt_load(x, lead, aligned, vocab, lo + warp, v);
         for (int seg = lo + warp; seg < hi; seg += VT_WARPS) {
-            float v[VT_EACH];
-            vt_load(x, lead, vocab, seg, v);
+            float next[VT_EACH];
+            if (seg + VT_WARPS < hi) vt_load(x, lead, aligned, vocab, seg + VT_WARPS, next);
             float most = -INFINITY;
 #pragma unroll
             for (int i = 0; i < VT_EACH; ++i) {
@@ -150,58 +198,52 @@ __global__ void __launch_bounds__(VT_THREADS) verify_tree_kernel(const VerifyArg
                     best = key > best && v[i] == v[i] && (unsigned)id < (unsigned)vocab ? key : best;
                 }
             }
-            if (!draws) continue;
+            if (draws) {
+                most = vt_warp_max(most);
+                double sum = 0.0;
+                if (most > -INFINITY && most < INFINITY) {
+                    const VtWeight weight(sh.table, heat, temp, most);
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-            double sum = 0.0;
-            if (most > -INFINITY && most < INFINITY)
-#pragma unroll
-                for (int i = 0; i < VT_EACH; ++i) sum += exp(((double)v[i] - (double)most) * heat);
-            sum = vt_warp_sum(sum);
-            if (keep && lane == 0) { p_sum[seg - lo] = sum; p_most[seg - lo] = most; }
-            if (most > w_most) {
-                w_sum = w_sum * exp(((double)w_most - (double)most) * heat) + sum;
-                w_most = most;
-            } else if (most > -INFINITY) {
-                w_sum += sum * exp(((double)most - (double)w_most) * heat);
+                    for (int i = 0; i < VT_EACH; ++i) sum += weight(v[i]);
+                }
+                sum = vt_warp_sum(sum);
+                if (lane == 0) { sums[seg - lo] = sum; mosts[seg - lo] = most; }
             }
+#pragma unroll
+            for (int i = 0; i < VT_EACH; ++i) v[i] = next[i];
         }
-        best = vt_warp_max(best);
+        if (!draws) best = vt_warp_max(best);
         wrong = __any_sync(0xffffffffu, wrong);
-        if (lane == 0) { sh.warp_sum[warp] = w_sum; sh.warp_most[warp] = w_most; sh.warp_wrong[warp] = wrong; sh.warp_best[warp] = best; }
+        if (lane == 0) { sh.warp_wrong[which][warp] = wrong; sh.warp_best[warp] = best; }
         __syncthreads();
-        if (tid == 0) {
+        if (warp == which) {
+            wrong = __any_sync(0xffffffffu, lane < VT_WARPS && sh.warp_wrong[which][lane % VT_WARPS]);
+            best = draws ? 0 : vt_warp_max(sh.warp_best[lane % VT_WARPS]);
             float most = -INFINITY;
             double sum = 0.0;
-            int bad = 0;
-            unsigned long long top = 0;
-            for (int w = 0; w < VT_WARPS; ++w) {
-                most = fmaxf(most, sh.warp_most[w]);
-                bad |= sh.warp_wrong[w];
-                top = sh.warp_best[w] > top ? sh.warp_best[w] : top;
+            if (draws) {
+                for (int i = lane; i < hi - lo; i += 32) most = fmaxf(most, mosts[i]);
+                most = vt_warp_max(most);
+                if (most > -INFINITY && most < INFINITY) {
+                    const VtWeight weight(sh.table, heat, temp, most);
+                    for (int i = lane; i < hi - lo; i += 32) sum = fma(sums[i], weight(mosts[i]), sum);
+                }
+                sum = vt_warp_sum(sum);
             }
-            if (most > -INFINITY && most < INFINITY)
-                for (int w = 0; w < VT_WARPS; ++w)
-                    if (sh.warp_most[w] > -INFINITY) sum += sh.warp_sum[w] * exp(((double)sh.warp_most[w] - (double)most) * heat);
-            to.sum = sum; to.most = most; to.wrong = bad; to.best = top;
+            if (lane == 0) { to.sum = sum; to.most = most; to.wrong = wrong; to.best = best; }
         }
-        __syncthreads();
     };
-    // All blocks' shares, behind the cluster's barrier.
-    auto whole = [&](int turn, int which, float& most, double& sum) -> bool {
-        most = -INFINITY;
-        sum = 0.0;
-        bool wrong = false;
-        for (int b = 0; b < C; ++b) {
-            const VtShare* o = &of(b)->mine[turn][which];
-            most = fmaxf(most, o->most);
-            wrong = wrong || o->wrong;
-        }
-        if (wrong || !(most > -INFINITY)) return false;
-        for (int b = 0; b < C; ++b) {
-            const VtShare* o = &of(b)->mine[turn][which];
-            if (o->most > -INFINITY) sum += o->sum * exp(((double)o->most - (double)most) * heat);
-        }
+    // All blocks' shares, behind the cluster's barrier: lane b has block b's. False: no distribution.
+    auto whole = [&](int turn, int which, float& most, double& sum, double& mine) -> bool {
+        float m = -INFINITY;
+        double s = 0.0;
+        int bad = 0;
+        if (lane < C) { const VtShare* o = &of(lane)->mine[turn][which]; m = o->most; s = o->sum; bad = o->wrong; }
+        most = vt_warp_max(m);
+        mine = 0.0;
+        if (__any_sync(0xffffffffu, bad) || !(most > -INFINITY)) return false;
+        mine = s * VtWeight(sh.table, heat, temp, most)(m);
+        sum = vt_warp_sum(mine);
         return true;
     };
     // The token at which the sum of the weights exceeds `target`: seg_sum(i) is the sum of the block's segment i, weights(seg, w) are a lane's of one. Called by
@@ -210,13 +252,7 @@ __global__ void __launch_bounds__(VT_THREADS) verify_tree_kernel(const VerifyArg
     auto find = [&](int lo, int hi, int lead, double before, bool behind, double target, auto seg_sum, auto weights) -> int {
         int last = -1;                                 // the last segment that holds a weight
         for (int s0 = lo; s0 < hi; s0 += 32) {
-            const double mine = s0 + lane < hi ? seg_sum(s0 + lane - lo) : 0.0;
-            double upto = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const double up = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += up;
-            }
+            const double mine = s0 + lane < hi ? seg_sum(s0 + lane - lo) : 0.0, upto = vt_warp_scan(mine);
             const unsigned some = __ballot_sync(0xffffffffu, mine > 0.0), hit = __ballot_sync(0xffffffffu, mine > 0.0 && !behind && before + upto > target);
             if (hit) {
                 const int at = __ffs(hit) - 1;
@@ -236,12 +272,7 @@ __global__ void __launch_bounds__(VT_THREADS) verify_tree_kernel(const VerifyArg
             double mine = 0.0;
 #pragma unroll
             for (int e = 0; e < N; ++e) mine += w[u * N + e];
-            double upto = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const double up = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += up;
-            }
+            const double upto = vt_warp_scan(mine);
             double sum = before + upto - mine;
             int found = -1, held = -1;                 // where the sum passes the target, and the lane's last weight
 #pragma unroll
@@ -260,7 +291,22 @@ __global__ void __launch_bounds__(VT_THREADS) verify_tree_kernel(const VerifyArg
         }
         return token;
     };
+    // The first row behind `after` that is a child of `of_row` (and holds `like`, unless that is negative); every warp for itself.
+    auto next_child = [&](int of_row, int after, int like) -> int {
+        for (int c0 = max(of_row, after) + 1; c0 < rows; c0 += 32) {
+            const int c = c0 + lane;
+            bool is = false;
+            if (c < rows) {
+                const int p = c < VT_ROWS ? sh.parents[c] : a.parents[row0 + c];
+                is = p == of_row && (like < 0 || (c < VT_ROWS ? sh.tokens[c] : a.tokens[row0 + c]) == like);
+            }
+            const unsigned hit = __ballot_sync(0xffffffffu, is);
+            if (hit) return c0 + __ffs(hit) - 1;
+        }
+        return -1;
+    };
 
+    // Every warp of every block takes the same decisions from the same numbers.
     int cur = 0, kept = 1, token = -1;
     for (int step = 0;; ++step) {                      // (a child lies behind its parent: at most `rows` steps)
         const int turn = step & 1;
@@ -268,112 +314,86 @@ __global__ void __launch_bounds__(VT_THREADS) verify_tree_kernel(const VerifyArg
         const T* y = drafted ? (const T*)a.draft + (size_t)(row0 + cur) * a.draft_stride : nullptr;
         const int lead = (int)((uintptr_t)x & 15) / (int)sizeof(T), segs = (lead + vocab + VT_SEG - 1) / VT_SEG;
         const int lo = min(rank * per, segs), hi = min(lo + per, segs);
-        scan(x, true, sh.mine[turn][0]);
-        if (drafted) scan(y, false, sh.mine[turn][1]);
+        const bool y_aligned = drafted && ((uintptr_t)(y - lead) & 15) == 0;
+        const double u = draws ? (double)a.uniform[2 * (size_t)(row0 + cur) + 1] : 0.0;
+        scan(x, lead, lo, hi, p_sum, p_most, 0, sh.mine[turn][0]);
+        if (drafted) scan(y, lead, lo, hi, q_sum, q_most, 1, sh.mine[turn][1]);
         cluster_sync();
         int child = -1;                                // where the walk goes on
         token = -1;
-        // the first row behind `after` that is a child of this one (and holds `like`, if that is a token)
-        auto next_child = [&](int after, int like) -> int {
-            __syncthreads();
-            if (tid == 0) sh.child = rows;
-            __syncthreads();
-            for (int c = max(cur, after) + 1 + tid; c < rows; c += VT_THREADS)
-                if (a.parents[row0 + c] == cur && (like < 0 || a.tokens[row0 + c] == like)) { atomicMin(&sh.child, c); break; }
-            __syncthreads();
-            return sh.child < rows ? sh.child : -1;
-        };
         if (!draws) {
-            unsigned long long best = 0;
-            for (int b = 0; b < C; ++b) { const unsigned long long o = of(b)->mine[turn][0].best; best = o > best ? o : best; }
+            const unsigned long long best = vt_warp_max(lane < C ? of(lane)->mine[turn][0].best : 0ull);
             token = best ? (int)~(unsigned)best : -1;
-            if (token >= 0) child = next_child(cur, token);
+            if (token >= 0) child = next_child(cur, cur, token);
         } else {
-            float most, q_most = 0.f;
-            double sum, q_sum = 1.0;
-            const bool fine = whole(turn, 0, most, sum), q_fine = !drafted || whole(turn, 1, q_most, q_sum);
-            const double u = (double)a.uniform[2 * (size_t)(row0 + cur) + 1];
+            float most, q_most_all = 0.f;
+            double sum = 1.0, q_all = 1.0, mine, unused;
+            const bool fine = whole(turn, 0, most, sum, mine), q_fine = !drafted || whole(turn, 1, q_most_all, q_all, unused);
+            const VtWeight weight(sh.table, heat, temp, most), q_weight(sh.table, heat, temp, q_most_all);
+            const double p_one = 1.0 / sum, q_one = 1.0 / q_all;
             double away = 0.0, left = 1.0;             // s and sum(r)
-            bool drawn_from_left = false;
+            bool from_left = false;
+            auto leftover = [&](int seg, double (&w)[VT_EACH]) {
+                float v[VT_EACH], z[VT_EACH];
+                vt_load(x, lead, true, vocab, seg, v);
+                vt_load(y, lead, y_aligned, vocab, seg, z);
+#pragma unroll
+                for (int i = 0; i < VT_EACH; ++i) w[i] = fmax(weight(v[i]) * p_one - away * (q_weight(z[i]) * q_one), 0.0);
+            };
             if (fine && q_fine && drafted) {
-                for (int c = next_child(cur, -1); c >= 0; c = next_child(c, -1)) {
-                    const int t = a.tokens[row0 + c];
+                for (int c = next_child(cur, cur, -1); c >= 0; c = next_child(cur, c, -1)) {
+                    const int t = c < VT_ROWS ? sh.tokens[c] : a.tokens[row0 + c];
                     if (t < 0 || t >= vocab) continue;     // (nothing that q could have given)
-                    const double p = exp(((double)gb_to_float(x[t]) - (double)most) * heat) / sum, q = exp(((double)gb_to_float(y[t]) - (double)q_most) * heat) / q_sum;
-                    const double r = fmax(p - away * q, 0.0);
+                    const double p = weight(gb_to_float(x[t])) * p_one, q = q_weight(gb_to_float(y[t])) * q_one, r = fmax(p - away * q, 0.0);
                     if ((double)a.uniform[2 * (size_t)(row0 + c)] * q * left < r) { child = c; break; }
                     // not taken: what is left without it
                     away += left;
-                    drawn_from_left = true;
-                    double w_sum = 0.0;
                     for (int seg = lo + warp; seg < hi; seg += VT_WARPS) {
-                        float v[VT_EACH];
-                        vt_load(x, lead, vocab, seg, v);
-                        double s = 0.0;
+                        double w[VT_EACH], s = 0.0;
+                        leftover(seg, w);
 #pragma unroll
-                        for (int i = 0; i < VT_EACH; ++i) {
-                            const int id = seg * VT_SEG + (i / N * 32 + lane) * N + i % N - lead;
-                            if (v[i] > -INFINITY) s += fmax(exp(((double)v[i] - (double)most) * heat) / sum - away * (exp(((double)gb_to_float(y[id]) - (double)q_most) * heat) / q_sum), 0.0);
-                        }
+                        for (int i = 0; i < VT_EACH; ++i) s += w[i];
                         s = vt_warp_sum(s);
                         if (lane == 0) r_sum[seg - lo] = s;
-                        w_sum += s;
                     }
-                    if (lane == 0) sh.warp_sum2[warp] = w_sum;
                     cluster_sync();                    // (the leftover before has been read by all)
-                    if (tid == 0) {
+                    if (warp == 0) {
                         double s = 0.0;
-                        for (int w = 0; w < VT_WARPS; ++w) s += sh.warp_sum2[w];
-                        sh.left[0] = s;
+                        for (int i = lane; i < hi - lo; i += 32) s += r_sum[i];
+                        s = vt_warp_sum(s);
+                        if (lane == 0) sh.left = s;
                     }
                     cluster_sync();
-                    left = 0.0;
-                    for (int b = 0; b < C; ++b) left += of(b)->left[0];
-                    if (!(left > 0.0)) { drawn_from_left = false; break; }
+                    mine = lane < C ? of(lane)->left : 0.0;
+                    left = vt_warp_sum(mine);
+                    from_left = left > 0.0;
+                    if (!from_left) {                  // nothing is left of r: p itself
+                        whole(turn, 0, most, sum, mine);
+                        break;
+                    }
                 }
             }
             if (fine && q_fine && child < 0) {
-                // draw: the block whose share holds the target finds the token
-                const double target = u * (drawn_from_left ? left : sum);
-                double before = 0.0, mine = 0.0;
-                int owner = -1, filled = -1;           // (filled: the last block that holds a weight; rounding may leave the target behind it)
-                double owner_before = 0.0;
-                for (int b = 0; b < C; ++b) {
-                    const VtShared* o = of(b);
-                    mine = drawn_from_left ? o->left[0] : o->mine[turn][0].most > -INFINITY ? o->mine[turn][0].sum * exp(((double)o->mine[turn][0].most - (double)most) * heat) : 0.0;
-                    if (mine > 0.0) {
-                        filled = b;
-                        if (owner < 0 && before + mine > target) { owner = b; owner_before = before; }
-                    }
-                    before += mine;
-                }
-                const bool behind = owner < 0;
-                if (behind) owner = filled;
+                // draw: the block whose share holds the target finds the token (mine: lane b has block b's share)
+                const double target = u * (from_left ? left : sum), upto = vt_warp_scan(mine);
+                const unsigned hit = __ballot_sync(0xffffffffu, mine > 0.0 && upto > target), some = __ballot_sync(0xffffffffu, mine > 0.0);
+                const int owner = hit ? __ffs(hit) - 1 : 31 - __clz(some);
+                const double before = __shfl_sync(0xffffffffu, upto - mine, max(owner, 0));
                 if (owner == rank && warp == 0) {
-                    auto weight = [&](float v) { return v > -INFINITY ? exp(((double)v - (double)most) * heat) : 0.0; };
-                    auto p_seg = [&](int i) { return p_most[i] > -INFINITY ? p_sum[i] * exp(((double)p_most[i] - (double)most) * heat) : 0.0; };
+                    auto p_seg = [&](int i) { return p_sum[i] * weight(p_most[i]); };
                     auto r_seg = [&](int i) { return r_sum[i]; };
                     auto p_weights = [&](int seg, double (&w)[VT_EACH]) {
                         float v[VT_EACH];
-                        vt_load(x, lead, vocab, seg, v);
+                        vt_load(x, lead, true, vocab, seg, v);
 #pragma unroll
                         for (int i = 0; i < VT_EACH; ++i) w[i] = weight(v[i]);
                     };
-                    auto r_weights = [&](int seg, double (&w)[VT_EACH]) {
-                        float v[VT_EACH];
-                        vt_load(x, lead, vocab, seg, v);
-#pragma unroll
-                        for (int i = 0; i < VT_EACH; ++i) {
-                            const int id = seg * VT_SEG + (i / N * 32 + lane) * N + i % N - lead;
-                            w[i] = v[i] > -INFINITY ? fmax(weight(v[i]) / sum - away * (exp(((double)gb_to_float(y[id]) - (double)q_most) * heat) / q_sum), 0.0) : 0.0;
-                        }
-                    };
-                    const int found = drawn_from_left ? find(lo, hi, lead, owner_before, behind, target, r_seg, r_weights) : find(lo, hi, lead, owner_before, behind, target, p_seg, p_weights);
+                    const int found = from_left ? find(lo, hi, lead, before, !hit, target, r_seg, leftover) : find(lo, hi, lead, before, !hit, target, p_seg, p_weights);
                     if (lane == 0) sh.token[turn] = found;
                 }
                 cluster_sync();
                 token = owner >= 0 ? of(owner)->token[turn] : -1;
-                if (!drafted && token >= 0) child = next_child(cur, token);
+                if (!drafted && token >= 0) child = next_child(cur, cur, token);
             }
         }
         if (child < 0) break;
@@ -403,7 +423,7 @@ GB_EXPORT int gb_verify_tree(const void* logits, int dtype, long long stride, co
     while (blocks > 1 && ((long long)num_seqs * blocks > 2 * 148 || vocab < blocks * VT_SEG * VT_WARPS)) blocks /= 2;
     a.blocks = blocks;
     const int lanes = dtype == GB_F32 ? 4 : 8, per = gb_ceil_div(gb_ceil_div(vocab + lanes, VT_SEG), blocks);
-    const int smem = per * (draft ? 20 : 12);
+    const int smem = per * (draft ? 3 * 8 + 2 * 4 : 8 + 4);
     const auto kernel = dtype == GB_F32 ? verify_tree_kernel<float> : verify_tree_kernel<__nv_bfloat16>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     GB_REQUIRE(e == cudaSuccess, "gb_verify_tree: %d bytes of shared memory refused: %s", smem, cudaGetErrorString(e));

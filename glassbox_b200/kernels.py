@@ -49,7 +49,7 @@ _SIGNATURES = {
     "gb_gemm_f32_tc": [_P, _P, _I, _P, _I, _I, _I, _I, _LL, _LL, _LL, _P, _P],
     "gb_gemm_simt": [_P, _I, _P, _I, _P, _I, _I, _I, _I, _I, _LL, _LL, _LL, _P],
     "gb_tree_attention": [_I, _P, _LL, _P, _LL, _I, _P, _P, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _LL, _F, _I, _I, _P, _P, _P],
-    "gb_tree_attention_splits": [_I, _I, _I, _I, _I, _I, _I, _I],
+    "gb_tree_attention_floats": [_I, _I, _I, _I, _I, _I, _I, _I, _I],
     "gb_verify_tree": [_P, _I, _LL, _P, _LL, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P],
     "gb_keep_rows": [_P, _P, _I, _I, _I, _LL, _I, _I, _P, _I, _P, _P, _P, _P, _I, _I, _P, _P],
     "gb_attention_rows": [_P, _LL, _P, _LL, _I, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _LL, _F, _I, _P, _P],
@@ -2659,9 +2659,12 @@ def tree_attention_kind(q: torch.Tensor, out: torch.Tensor, hd: int, page_size: 
                and q.stride(0) % 2 == 0 and q.data_ptr() % 4 == 0 and out.stride(0) % 2 == 0 and out.data_ptr() % 4 == 0)
 
 
-@functools.lru_cache(maxsize=1024)
-def _tree_splits(kind: int, num_seqs: int, most: int, nh: int, nkv: int, hd: int, max_context: int, window: int) -> int:
-    return lib().gb_tree_attention_splits(kind, num_seqs, most, nh, nkv, hd, max_context, window)
+@functools.lru_cache(maxsize=4096)
+def _tree_floats(kind: int, n: int, num_seqs: int, most: int, nh: int, nkv: int, hd: int, max_context: int, window: int) -> int:
+    floats = lib().gb_tree_attention_floats(kind, n, num_seqs, most, nh, nkv, hd, max_context, window)
+    if floats < 0:
+        raise KernelError(f"{num_seqs} trees of up to {most} rows need more scratch than there can be")
+    return floats
 
 
 def tree_attention_parts(q: torch.Tensor, nh: int, nkv: int, hd: int, num_seqs: int, max_rows_per_seq: int, max_context: int,
@@ -2674,8 +2677,7 @@ def tree_attention_parts(q: torch.Tensor, nh: int, nkv: int, hd: int, num_seqs: 
 def tree_attention_floats(n: int, nh: int, nkv: int, hd: int, num_seqs: int, max_rows_per_seq: int, max_context: int, window: Optional[int] = None) -> int:
     """Numbers of the scratch for ``tree_attention`` of ``n`` rows (0: it needs none)."""
     # (the kernel is chosen by the tensors' alignment, too: as much as the one that needs more)
-    splits = max(_tree_splits(kind, num_seqs, max_rows_per_seq, nh, nkv, hd, int(max_context), int(window or 0)) for kind in (0, 1))
-    return splits * n * nh * (hd + 2) if splits > 1 else 0
+    return max(_tree_floats(kind, n, num_seqs, max_rows_per_seq, nh, nkv, hd, int(max_context), int(window or 0)) for kind in (0, 1))
 
 
 def _tree_batch(block_tables, seq_first_row, seq_start_pos) -> int:
@@ -2721,12 +2723,13 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vca
     if not n or not num_seqs or not max_rows_per_seq:
         return
     kind = tree_attention_kind(q, out, hd, page_size)
-    splits = _tree_splits(kind, num_seqs, max_rows_per_seq, nh, nkv, hd, int(max_context), int(window or 0))
-    if splits > 1 and (parts is None or parts.dtype != torch.float32 or not parts.is_contiguous() or parts.numel() < splits * n * nh * (hd + 2)):
-        raise KernelError(f"this batch needs contiguous float32 scratch of {splits * n * nh * (hd + 2)} numbers (tree_attention_parts)")
+    max_context, window = int(max_context), int(window or 0)
+    floats = _tree_floats(kind, n, num_seqs, max_rows_per_seq, nh, nkv, hd, max_context, window)
+    if floats and (parts is None or parts.dtype != torch.float32 or not parts.is_contiguous() or parts.numel() < floats):
+        raise KernelError(f"this batch needs contiguous float32 scratch of {floats} numbers (tree_attention_parts)")
     _call("gb_tree_attention", kind, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), dtype, kcache.data_ptr(), vcache.data_ptr(),
           block_tables.data_ptr(), block_tables.shape[1], seq_first_row.data_ptr(), seq_start_pos.data_ptr(), positions.data_ptr(), visible.data_ptr(),
-          visible.shape[1], n, num_seqs, int(max_rows_per_seq), nh, nkv, hd, page_size, kcache.shape[0], float(scale), int(window or 0), splits, _ptr(parts),
+          visible.shape[1], n, num_seqs, int(max_rows_per_seq), nh, nkv, hd, page_size, kcache.shape[0], float(scale), window, max_context, _ptr(parts),
           status.data_ptr(), stream)
 
 
