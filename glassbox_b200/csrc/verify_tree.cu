@@ -14,11 +14,13 @@
 
 #include <cooperative_groups.h>
 
-constexpr int VT_THREADS = 256, VT_WARPS = VT_THREADS / 32;
+constexpr int VT_MOST_WARPS = 8;
 constexpr int VT_SEG = 512, VT_EACH = VT_SEG / 32;      // tokens of a segment, and of a lane
 constexpr int VT_MAX_SEGS = 4097;
 constexpr int VT_MAX_CLUSTER = 8;
-constexpr int VT_TABLE = 256;                           // 2^(j / 256)
+constexpr int VT_TABLE = 64, VT_COPIES = 16;            // 2^(j / 64), for every lane of a half warp in banks of its own
+constexpr double VT_NOTHING = 1e-290;                     // sums of weights below it hold none
+constexpr int VT_MAX_ROWS = 8192;                        // rows of a batch whose outcomes fit shared memory
 constexpr int VT_ROWS = 512;                            // rows of a tree whose parents and tokens stay in shared memory
 
 struct VerifyArgs {
@@ -49,9 +51,9 @@ struct VtShared {
     VtShare mine[2][2];                // [turn][p, q]
     double left;                       // of the leftover
     int token[2];                      // [turn] that the block found
-    int warp_wrong[2][VT_WARPS];
-    unsigned long long warp_best[VT_WARPS];
-    double table[VT_TABLE];
+    int warp_wrong[2][VT_MOST_WARPS];
+    unsigned long long warp_best[VT_MOST_WARPS];
+    double table[VT_TABLE * VT_COPIES];
     int parents[VT_ROWS], tokens[VT_ROWS];
 };
 
@@ -65,9 +67,14 @@ __device__ __forceinline__ unsigned long long vt_warp_max(unsigned long long key
     const unsigned low = __reduce_max_sync(0xffffffffu, (unsigned)(key >> 32) == high ? (unsigned)key : 0u);
     return (unsigned long long)high << 32 | low;
 }
-__device__ __forceinline__ float vt_warp_max(float v) {                     // (not of NaN)
+__device__ __forceinline__ float vt_max(float a, float b) {                 // NaN where one is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float vt_warp_max(float v) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    for (int o = 16; o > 0; o >>= 1) v = vt_max(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
 __device__ __forceinline__ double vt_warp_sum(double v) {
@@ -85,32 +92,26 @@ __device__ __forceinline__ double vt_warp_scan(double v) {                  // s
     return v;
 }
 
-// A float32 as a double, by its bits (0 and subnormal ones come out as numbers below 2^-126, as good as 0 beside a logit; infinities as finite ones
-// beyond 2^127): the conversion proper goes through a unit that takes 16 a cycle.
-__device__ __forceinline__ double vt_double(float x) {
-    const unsigned b = __float_as_uint(x);
-    return __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + 0x38000000u)), (int)(b << 29));
-}
-
-// Weights exp((x - most) / T) of logits x <= most: 2^(k / 256) from a table, whole powers of two added to its exponent, and three terms of the exponential
-// series for the rest, at most 1/512 of an octave: a relative error below (ln 2 / 512)^4 / 24 = 2^-42.7. Below e^-700 a weight is nothing.
+// Weights exp((x - most) / T) of logits x <= most: 2^(k / 64) from a table, whole powers of two added to its exponent, and a polynomial for the rest, at most
+// h = ln 2 / 128 in the exponent: 1 + r + r^2 / 2 + r^3 / 6 + r^4 / 24 with h^2 r^2 in the place of r^4, a relative error of at most h^4 / 96 = 2^-36.7. Below
+// e^-700 all weights are that, nothing (VT_NOTHING). (One table of 256 for all lanes: 800 rows of 49,152 tokens 81 us, its banks' conflicts half of it.)
 struct VtWeight {
-    const double* table;
-    double heat, most;                 // 256 / (T ln 2)
+    unsigned table;                    // (its address in shared memory: where it lies has to be known to be read there without detours)
+    double heat, most;                 // 64 / (T ln 2)
     float least;
     __device__ __forceinline__ VtWeight(const double* table, double heat, float temp, float most)
-        : table(table), heat(heat), most(vt_double(most)), least(fmaf(-700.0f, temp, most)) {}
+        : table((unsigned)__cvta_generic_to_shared(table) + (threadIdx.x & (VT_COPIES - 1)) * 8), heat(heat), most((double)most), least(fmaxf(fmaf(-700.0f, temp, most), -FLT_MAX)) {}
     __device__ __forceinline__ double operator()(float x) const {
         constexpr double MAGIC = 6755399441055744.0;                  // 1.5 2^52: the low word of a sum with it is the nearest whole number
-        constexpr double C1 = 0.0027076061740622863, C2 = 3.665565596910106e-06, C3 = 3.308302680541371e-09;      // (ln 2 / 256)^i / i!
-        const double d = vt_double(fmaxf(x, least)) - most;
+        constexpr double C1 = 0.010830424696249145, C2 = 5.864919287185391e-05, C3 = 2.1173137155464774e-07;
+        const double d = (double)fmaxf(x, least) - most;
         const double s = fma(d, heat, MAGIC);
         const int k = __double2loint(s);
         const double r = fma(d, heat, MAGIC - s);
-        const double t = table[k & (VT_TABLE - 1)];
-        const double w = __hiloint2double(__double2hiint(t) + ((k >> 8) << 20), __double2loint(t));
-        const double v = fma(w * r, fma(fma(C3, r, C2), r, C1), w);
-        return x >= least && x > -INFINITY ? v : 0.0;
+        double t;
+        asm("ld.shared.f64 %0, [%1];" : "=d"(t) : "r"(table + (unsigned)(k & (VT_TABLE - 1)) * (VT_COPIES * 8)));
+        const double w = __hiloint2double(__double2hiint(t) + (k & ~(VT_TABLE - 1)) * (1 << 14), __double2loint(t));
+        return fma(w * r, fma(fma(C3, r, C2), r, C1), w);
     }
 };
 
@@ -119,110 +120,127 @@ struct VtWeight {
 template <typename T>
 __device__ __forceinline__ void vt_load(const T* x, int lead, bool aligned, int vocab, int seg, float (&v)[VT_EACH]) {
     constexpr int N = 16 / sizeof(T);
-    const int lane = threadIdx.x & 31;
-    uint4 raw[VT_EACH / N];
-    bool whole[VT_EACH / N];
+    const int lane = threadIdx.x & 31, first = seg * VT_SEG - lead;
+    if (aligned && first >= 0 && first + VT_SEG <= vocab) {
+        uint4 raw[VT_EACH / N];
 #pragma unroll
-    for (int u = 0; u < VT_EACH / N; ++u) {
-        const int i = seg * VT_SEG + (u * 32 + lane) * N - lead;
-        whole[u] = aligned && i >= 0 && i + N <= vocab;
-        raw[u] = whole[u] ? *reinterpret_cast<const uint4*>(x + i) : make_uint4(0, 0, 0, 0);
+        for (int u = 0; u < VT_EACH / N; ++u) raw[u] = *reinterpret_cast<const uint4*>(x + first + (u * 32 + lane) * N);
+#pragma unroll
+        for (int u = 0; u < VT_EACH / N; ++u) {
+            const unsigned w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                v[u * N + e] = N == 4 ? __uint_as_float(w[e % 4]) : __uint_as_float(e & 1 ? w[(e >> 1) % 4] & 0xffff0000u : w[(e >> 1) % 4] << 16);
+        }
+        return;
     }
 #pragma unroll
-    for (int u = 0; u < VT_EACH / N; ++u) {
-        const unsigned w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
-#pragma unroll
-        for (int e = 0; e < N; ++e)
-            v[u * N + e] = N == 4 ? __uint_as_float(w[e % 4]) : __uint_as_float(e & 1 ? w[(e >> 1) % 4] & 0xffff0000u : w[(e >> 1) % 4] << 16);
-        if (!whole[u]) {
-#pragma unroll
-            for (int e = 0; e < N; ++e) {
-                const int i = seg * VT_SEG + (u * 32 + lane) * N + e - lead;
-                v[u * N + e] = i >= 0 && i < vocab ? gb_to_float(x[i]) : -INFINITY;
-            }
-        }
+    for (int i = 0; i < VT_EACH; ++i) {
+        const int id = first + (i / N * 32 + lane) * N + i % N;
+        v[i] = id >= 0 && id < vocab ? gb_to_float(x[id]) : -INFINITY;
     }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(VT_THREADS, 2) verify_tree_kernel(const VerifyArgs a) {
-    namespace cg = cooperative_groups;
-    constexpr int N = 16 / sizeof(T);
-    extern __shared__ __align__(16) double vt_mem[];
-    __shared__ VtShared sh;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int C = a.blocks, rank = blockIdx.x % C, seq = blockIdx.x / C, vocab = a.vocab;
-    const int per = ((vocab + N + VT_SEG - 1) / VT_SEG + C - 1) / C;
+// What follows a row of a tree: the child that the walk goes on to, or (child -1) the token that follows it.
+struct VtOutcome {
+    int child, token;
+};
+
+// One row, by a cluster of C blocks (one: the block alone). Every warp of every block takes the same decisions from the same numbers.
+// NW warps a block: 8 with the next segment's loads under way where few blocks have the GPU to themselves, else 4, so that many rows are in flight.
+template <typename T, bool DRAFTED, int NW>
+struct VtRow {
+    static constexpr int VT_WARPS = NW, VT_THREADS = NW * 32;
+    static constexpr bool AHEAD = NW == VT_MOST_WARPS;
+    static constexpr int N = 16 / sizeof(T);
+    const VerifyArgs& a;
+    VtShared& sh;
+    int C, rank, per, lane, warp;
     // of the block's segments: sums and largest logits of p, with drafted distributions of q, too, and the leftover's sums
-    double* p_sum = vt_mem;
-    double* q_sum = p_sum + per;
-    double* r_sum = a.draft ? q_sum + per : q_sum;
-    float* p_most = reinterpret_cast<float*>(a.draft ? r_sum + per : q_sum);
-    float* q_most = p_most + per;
-    for (int i = tid; i < VT_TABLE; i += VT_THREADS) sh.table[i] = exp2((double)i / VT_TABLE);
-    gb_pdl_launch_dependents();
-    gb_pdl_wait();
-    const int row0 = a.first_row[seq], rows = a.first_row[seq + 1] - row0;
-    auto cluster_sync = [&]() { if (C > 1) cg::this_cluster().sync(); else __syncthreads(); };
-    auto of = [&](int b) -> const VtShared* { return C > 1 ? cg::this_cluster().map_shared_rank(&sh, b) : &sh; };
-    if (rows <= 0 || row0 < 0 || row0 > a.n - rows) {  // (the same in all blocks of a cluster)
-        if (rank == 0 && tid == 0) { a.accepted[seq] = 0; a.next[seq] = -1; }
-        return;
+    double *p_sum, *q_sum, *r_sum;
+    float *p_most, *q_most;
+    int row0, rows;                    // of the request
+    float temp;
+    bool draws;
+    double heat;
+
+    __device__ __forceinline__ VtRow(const VerifyArgs& a, VtShared& sh, double* mem, int rank) : a(a), sh(sh), C(a.blocks), rank(rank) {
+        lane = threadIdx.x & 31;
+        warp = threadIdx.x >> 5;
+        per = ((a.vocab + N + VT_SEG - 1) / VT_SEG + C - 1) / C;
+        p_sum = mem;
+        q_sum = p_sum + per;
+        r_sum = DRAFTED ? q_sum + per : q_sum;
+        p_most = reinterpret_cast<float*>(DRAFTED ? r_sum + per : q_sum);
+        q_most = p_most + per;
+        static_assert(VT_THREADS % VT_TABLE == 0, "a thread has copies of one entry");
+        const double entry = exp2((double)(threadIdx.x % VT_TABLE) / VT_TABLE);
+        for (int i = threadIdx.x / VT_TABLE; i < VT_COPIES; i += VT_THREADS / VT_TABLE) sh.table[threadIdx.x % VT_TABLE * VT_COPIES + i] = entry;
     }
-    const float temp = a.temperature[seq];
-    const bool draws = temp > 0.f, drafted = draws && a.draft != nullptr;
-    const double heat = draws ? (double)VT_TABLE / ((double)temp * 0.6931471805599453) : 0.0;
-    for (int i = tid; i < rows && i < VT_ROWS; i += VT_THREADS) { sh.parents[i] = a.parents[row0 + i]; sh.tokens[i] = a.tokens[row0 + i]; }
-    if (rank == 0)
-        for (int i = tid; i < rows; i += VT_THREADS) a.path[row0 + i] = i == 0 ? 0 : -1;
-    __syncthreads();
+    __device__ __forceinline__ void request(int first, int count, float t) {
+        row0 = first;
+        rows = count;
+        temp = t;
+        draws = temp > 0.f;
+        heat = draws ? (double)VT_TABLE / ((double)temp * 0.6931471805599453) : 0.0;
+        for (int i = threadIdx.x; i < rows && i < VT_ROWS; i += VT_THREADS) { sh.parents[i] = a.parents[row0 + i]; sh.tokens[i] = a.tokens[row0 + i]; }
+    }
+    __device__ __forceinline__ void cluster_sync() const {
+        namespace cg = cooperative_groups;
+        if (C > 1) cg::this_cluster().sync(); else __syncthreads();
+    }
+    __device__ __forceinline__ const VtShared* of(int b) const {
+        namespace cg = cooperative_groups;
+        return C > 1 ? cg::this_cluster().map_shared_rank(&sh, b) : &sh;
+    }
 
     // The block's share of a row: largest logits and sums of its segments, and its own in `to` (for whom the cluster's barrier is still to come).
-    auto scan = [&](const T* x, int lead, int lo, int hi, double* sums, float* mosts, int which, VtShare& to) {
+    __device__ __forceinline__ void scan(const T* x, int lead, int lo, int hi, double* sums, float* mosts, int which, VtShare& to) const {
         const bool aligned = ((uintptr_t)(x - lead) & 15) == 0;
         bool wrong = false;
-        unsigned long long best = 0;
+        float largest = -INFINITY;
+        int largest_id = -1;
         float v[VT_EACH];
-        if (lo + warp < hi) vt_load(x, lead, aligned, vocab, lo + warp, v);
+        if (AHEAD && lo + warp < hi) vt_load(x, lead, aligned, a.vocab, lo + warp, v);
         for (int seg = lo + warp; seg < hi; seg += VT_WARPS) {
-            float next[VT_EACH];
-            if (seg + VT_WARPS < hi) vt_load(x, lead, aligned, vocab, seg + VT_WARPS, next);
-            float most = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < VT_EACH; ++i) {
-                most = fmaxf(most, v[i]);
-                wrong = wrong || !(v[i] < INFINITY);
-                if (!draws) {
-                    const int id = seg * VT_SEG + (i / N * 32 + lane) * N + i % N - lead;
-                    const unsigned long long key = vt_key(v[i], id);
-                    best = key > best && v[i] == v[i] && (unsigned)id < (unsigned)vocab ? key : best;
-                }
-            }
+            float next[AHEAD ? VT_EACH : 1];
+            if constexpr (!AHEAD) vt_load(x, lead, aligned, a.vocab, seg, v);
+            else if (seg + VT_WARPS < hi) vt_load(x, lead, aligned, a.vocab, seg + VT_WARPS, next);
             if (draws) {
+                float most = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < VT_EACH; ++i) most = vt_max(most, v[i]);
                 most = vt_warp_max(most);
-                double sum = 0.0;
+                wrong = wrong || !(most < INFINITY);
+                double part[4] = {0.0, 0.0, 0.0, 0.0};
                 if (most > -INFINITY && most < INFINITY) {
                     const VtWeight weight(sh.table, heat, temp, most);
 #pragma unroll
-                    for (int i = 0; i < VT_EACH; ++i) sum += weight(v[i]);
+                    for (int i = 0; i < VT_EACH; ++i) part[i & 3] += weight(v[i]);
                 }
-                sum = vt_warp_sum(sum);
+                const double sum = vt_warp_sum((part[0] + part[1]) + (part[2] + part[3]));
                 if (lane == 0) { sums[seg - lo] = sum; mosts[seg - lo] = most; }
+            } else {
+#pragma unroll
+                for (int i = 0; i < VT_EACH; ++i) {      // (a lane's ids ascend: of equal logits the first stays; NaN is passed over)
+                    const int id = seg * VT_SEG + (i / N * 32 + lane) * N + i % N - lead;
+                    if (v[i] > largest || (largest_id < 0 && v[i] == v[i] && (unsigned)id < (unsigned)a.vocab)) { largest = v[i]; largest_id = id; }
+                }
             }
 #pragma unroll
-            for (int i = 0; i < VT_EACH; ++i) v[i] = next[i];
+            for (int i = 0; AHEAD && i < VT_EACH; ++i) v[i] = next[i];
         }
-        if (!draws) best = vt_warp_max(best);
         wrong = __any_sync(0xffffffffu, wrong);
+        const unsigned long long best = draws ? 0 : vt_warp_max(largest_id >= 0 ? vt_key(largest, largest_id) : 0ull);
         if (lane == 0) { sh.warp_wrong[which][warp] = wrong; sh.warp_best[warp] = best; }
         __syncthreads();
         if (warp == which) {
             wrong = __any_sync(0xffffffffu, lane < VT_WARPS && sh.warp_wrong[which][lane % VT_WARPS]);
-            best = draws ? 0 : vt_warp_max(sh.warp_best[lane % VT_WARPS]);
+            const unsigned long long top = draws ? 0 : vt_warp_max(sh.warp_best[lane % VT_WARPS]);
             float most = -INFINITY;
             double sum = 0.0;
             if (draws) {
-                for (int i = lane; i < hi - lo; i += 32) most = fmaxf(most, mosts[i]);
+                for (int i = lane; i < hi - lo; i += 32) most = vt_max(most, mosts[i]);
                 most = vt_warp_max(most);
                 if (most > -INFINITY && most < INFINITY) {
                     const VtWeight weight(sh.table, heat, temp, most);
@@ -230,11 +248,11 @@ __global__ void __launch_bounds__(VT_THREADS, 2) verify_tree_kernel(const Verify
                 }
                 sum = vt_warp_sum(sum);
             }
-            if (lane == 0) { to.sum = sum; to.most = most; to.wrong = wrong; to.best = best; }
+            if (lane == 0) { to.sum = sum; to.most = most; to.wrong = wrong; to.best = top; }
         }
-    };
+    }
     // All blocks' shares, behind the cluster's barrier: lane b has block b's. False: no distribution.
-    auto whole = [&](int turn, int which, float& most, double& sum, double& mine) -> bool {
+    __device__ __forceinline__ bool whole(int turn, int which, float& most, double& sum, double& mine) const {
         float m = -INFINITY;
         double s = 0.0;
         int bad = 0;
@@ -245,15 +263,16 @@ __global__ void __launch_bounds__(VT_THREADS, 2) verify_tree_kernel(const Verify
         mine = s * VtWeight(sh.table, heat, temp, most)(m);
         sum = vt_warp_sum(mine);
         return true;
-    };
+    }
     // The token at which the sum of the weights exceeds `target`: seg_sum(i) is the sum of the block's segment i, weights(seg, w) are a lane's of one. Called by
     // warp 0 of the block in whose share it lies; `before`: the sum of the shares before; `behind`: rounding has left the target behind every weight, the last
     // one is taken.
-    auto find = [&](int lo, int hi, int lead, double before, bool behind, double target, auto seg_sum, auto weights) -> int {
+    template <class Sum, class Weights>
+    __device__ __forceinline__ int find(int lo, int hi, int lead, double before, bool behind, double target, Sum seg_sum, Weights weights) const {
         int last = -1;                                 // the last segment that holds a weight
         for (int s0 = lo; s0 < hi; s0 += 32) {
             const double mine = s0 + lane < hi ? seg_sum(s0 + lane - lo) : 0.0, upto = vt_warp_scan(mine);
-            const unsigned some = __ballot_sync(0xffffffffu, mine > 0.0), hit = __ballot_sync(0xffffffffu, mine > 0.0 && !behind && before + upto > target);
+            const unsigned some = __ballot_sync(0xffffffffu, mine > VT_NOTHING), hit = __ballot_sync(0xffffffffu, mine > VT_NOTHING && !behind && before + upto > target);
             if (hit) {
                 const int at = __ffs(hit) - 1;
                 before = __shfl_sync(0xffffffffu, before + upto - mine, at);
@@ -264,22 +283,25 @@ __global__ void __launch_bounds__(VT_THREADS, 2) verify_tree_kernel(const Verify
             before += __shfl_sync(0xffffffffu, upto, 31);
         }
         if (last < 0) return -1;
-        double w[VT_EACH];
+        double w[VT_EACH], mine[VT_EACH / N], upto[VT_EACH / N];
         weights(last, w);
+#pragma unroll
+        for (int u = 0; u < VT_EACH / N; ++u) {
+            mine[u] = 0.0;
+#pragma unroll
+            for (int e = 0; e < N; ++e) mine[u] += w[u * N + e];
+            upto[u] = vt_warp_scan(mine[u]);
+        }
         int token = -1;
 #pragma unroll
         for (int u = 0; u < VT_EACH / N; ++u) {
-            double mine = 0.0;
-#pragma unroll
-            for (int e = 0; e < N; ++e) mine += w[u * N + e];
-            const double upto = vt_warp_scan(mine);
-            double sum = before + upto - mine;
+            double sum = before + upto[u] - mine[u];
             int found = -1, held = -1;                 // where the sum passes the target, and the lane's last weight
 #pragma unroll
             for (int e = 0; e < N; ++e) {
                 const int id = last * VT_SEG + (u * 32 + lane) * N + e - lead;
                 sum += w[u * N + e];
-                if (w[u * N + e] > 0.0) {
+                if (w[u * N + e] > VT_NOTHING) {
                     held = id;
                     if (found < 0 && sum > target && !behind) found = id;
                 }
@@ -287,12 +309,12 @@ __global__ void __launch_bounds__(VT_THREADS, 2) verify_tree_kernel(const Verify
             const unsigned hit = __ballot_sync(0xffffffffu, found >= 0), some = __ballot_sync(0xffffffffu, held >= 0);
             if (hit) return __shfl_sync(0xffffffffu, found, __ffs(hit) - 1);
             if (some) token = __shfl_sync(0xffffffffu, held, 31 - __clz(some));
-            before += __shfl_sync(0xffffffffu, upto, 31);
+            before += __shfl_sync(0xffffffffu, upto[u], 31);
         }
         return token;
-    };
+    }
     // The first row behind `after` that is a child of `of_row` (and holds `like`, unless that is negative); every warp for itself.
-    auto next_child = [&](int of_row, int after, int like) -> int {
+    __device__ __forceinline__ int next_child(int of_row, int after, int like) const {
         for (int c0 = max(of_row, after) + 1; c0 < rows; c0 += 32) {
             const int c = c0 + lane;
             bool is = false;
@@ -304,12 +326,12 @@ __global__ void __launch_bounds__(VT_THREADS, 2) verify_tree_kernel(const Verify
             if (hit) return c0 + __ffs(hit) - 1;
         }
         return -1;
-    };
+    }
 
-    // Every warp of every block takes the same decisions from the same numbers.
-    int cur = 0, kept = 1, token = -1;
-    for (int step = 0;; ++step) {                      // (a child lies behind its parent: at most `rows` steps)
-        const int turn = step & 1;
+    // turn: 0 and 1 from call to call, so that what blocks still read of one is not written by the next.
+    __device__ __forceinline__ VtOutcome outcome(int cur, int turn) const {
+        const int vocab = a.vocab;
+        const bool drafted = DRAFTED && draws;
         const T* x = (const T*)a.logits + (size_t)(row0 + cur) * a.stride;
         const T* y = drafted ? (const T*)a.draft + (size_t)(row0 + cur) * a.draft_stride : nullptr;
         const int lead = (int)((uintptr_t)x & 15) / (int)sizeof(T), segs = (lead + vocab + VT_SEG - 1) / VT_SEG;
@@ -319,117 +341,174 @@ __global__ void __launch_bounds__(VT_THREADS, 2) verify_tree_kernel(const Verify
         scan(x, lead, lo, hi, p_sum, p_most, 0, sh.mine[turn][0]);
         if (drafted) scan(y, lead, lo, hi, q_sum, q_most, 1, sh.mine[turn][1]);
         cluster_sync();
-        int child = -1;                                // where the walk goes on
-        token = -1;
         if (!draws) {
             const unsigned long long best = vt_warp_max(lane < C ? of(lane)->mine[turn][0].best : 0ull);
-            token = best ? (int)~(unsigned)best : -1;
-            if (token >= 0) child = next_child(cur, cur, token);
-        } else {
-            float most, q_most_all = 0.f;
-            double sum = 1.0, q_all = 1.0, mine, unused;
-            const bool fine = whole(turn, 0, most, sum, mine), q_fine = !drafted || whole(turn, 1, q_most_all, q_all, unused);
-            const VtWeight weight(sh.table, heat, temp, most), q_weight(sh.table, heat, temp, q_most_all);
-            const double p_one = 1.0 / sum, q_one = 1.0 / q_all;
-            double away = 0.0, left = 1.0;             // s and sum(r)
-            bool from_left = false;
-            auto leftover = [&](int seg, double (&w)[VT_EACH]) {
-                float v[VT_EACH], z[VT_EACH];
-                vt_load(x, lead, true, vocab, seg, v);
-                vt_load(y, lead, y_aligned, vocab, seg, z);
+            const int token = best ? (int)~(unsigned)best : -1;
+            return {token >= 0 ? next_child(cur, cur, token) : -1, token};
+        }
+        float most, q_most_all = 0.f;
+        double sum = 1.0, q_all = 1.0, mine, unused;
+        if (!whole(turn, 0, most, sum, mine)) return {-1, -1};
+        if (drafted && !whole(turn, 1, q_most_all, q_all, unused)) return {-1, -1};
+        const VtWeight weight(sh.table, heat, temp, most), q_weight(sh.table, heat, temp, q_most_all);
+        const double p_one = 1.0 / sum, q_one = 1.0 / q_all;
+        double away = 0.0, left = 1.0;                 // s and sum(r)
+        bool from_left = false;
+        auto leftover = [&](int seg, double (&w)[VT_EACH]) {
+            float v[VT_EACH], z[VT_EACH];
+            vt_load(x, lead, true, vocab, seg, v);
+            vt_load(y, lead, y_aligned, vocab, seg, z);
 #pragma unroll
-                for (int i = 0; i < VT_EACH; ++i) w[i] = fmax(weight(v[i]) * p_one - away * (q_weight(z[i]) * q_one), 0.0);
-            };
-            if (fine && q_fine && drafted) {
-                for (int c = next_child(cur, cur, -1); c >= 0; c = next_child(cur, c, -1)) {
-                    const int t = c < VT_ROWS ? sh.tokens[c] : a.tokens[row0 + c];
-                    if (t < 0 || t >= vocab) continue;     // (nothing that q could have given)
-                    const double p = weight(gb_to_float(x[t])) * p_one, q = q_weight(gb_to_float(y[t])) * q_one, r = fmax(p - away * q, 0.0);
-                    if ((double)a.uniform[2 * (size_t)(row0 + c)] * q * left < r) { child = c; break; }
-                    // not taken: what is left without it
-                    away += left;
-                    for (int seg = lo + warp; seg < hi; seg += VT_WARPS) {
-                        double w[VT_EACH], s = 0.0;
-                        leftover(seg, w);
+            for (int i = 0; i < VT_EACH; ++i) w[i] = fmax(weight(v[i]) * p_one - away * (q_weight(z[i]) * q_one), 0.0);
+        };
+        if (drafted) {
+            for (int c = next_child(cur, cur, -1); c >= 0; c = next_child(cur, c, -1)) {
+                const int t = c < VT_ROWS ? sh.tokens[c] : a.tokens[row0 + c];
+                if (t < 0 || t >= vocab) continue;     // (nothing that q could have given)
+                const double p = weight(gb_to_float(x[t])) * p_one, q = q_weight(gb_to_float(y[t])) * q_one, r = fmax(p - away * q, 0.0);
+                if (r > VT_NOTHING && (double)a.uniform[2 * (size_t)(row0 + c)] * q * left < r) return {c, t};
+                // not taken: what is left without it
+                away += left;
+                for (int seg = lo + warp; seg < hi; seg += VT_WARPS) {
+                    double w[VT_EACH], s = 0.0;
+                    leftover(seg, w);
 #pragma unroll
-                        for (int i = 0; i < VT_EACH; ++i) s += w[i];
-                        s = vt_warp_sum(s);
-                        if (lane == 0) r_sum[seg - lo] = s;
-                    }
-                    cluster_sync();                    // (the leftover before has been read by all)
-                    if (warp == 0) {
-                        double s = 0.0;
-                        for (int i = lane; i < hi - lo; i += 32) s += r_sum[i];
-                        s = vt_warp_sum(s);
-                        if (lane == 0) sh.left = s;
-                    }
-                    cluster_sync();
-                    mine = lane < C ? of(lane)->left : 0.0;
-                    left = vt_warp_sum(mine);
-                    from_left = left > 0.0;
-                    if (!from_left) {                  // nothing is left of r: p itself
-                        whole(turn, 0, most, sum, mine);
-                        break;
-                    }
+                    for (int i = 0; i < VT_EACH; ++i) s += w[i];
+                    s = vt_warp_sum(s);
+                    if (lane == 0) r_sum[seg - lo] = s;
                 }
-            }
-            if (fine && q_fine && child < 0) {
-                // draw: the block whose share holds the target finds the token (mine: lane b has block b's share)
-                const double target = u * (from_left ? left : sum), upto = vt_warp_scan(mine);
-                const unsigned hit = __ballot_sync(0xffffffffu, mine > 0.0 && upto > target), some = __ballot_sync(0xffffffffu, mine > 0.0);
-                const int owner = hit ? __ffs(hit) - 1 : 31 - __clz(some);
-                const double before = __shfl_sync(0xffffffffu, upto - mine, max(owner, 0));
-                if (owner == rank && warp == 0) {
-                    auto p_seg = [&](int i) { return p_sum[i] * weight(p_most[i]); };
-                    auto r_seg = [&](int i) { return r_sum[i]; };
-                    auto p_weights = [&](int seg, double (&w)[VT_EACH]) {
-                        float v[VT_EACH];
-                        vt_load(x, lead, true, vocab, seg, v);
-#pragma unroll
-                        for (int i = 0; i < VT_EACH; ++i) w[i] = weight(v[i]);
-                    };
-                    const int found = from_left ? find(lo, hi, lead, before, !hit, target, r_seg, leftover) : find(lo, hi, lead, before, !hit, target, p_seg, p_weights);
-                    if (lane == 0) sh.token[turn] = found;
+                cluster_sync();                        // (the leftover before has been read by all)
+                if (warp == 0) {
+                    double s = 0.0;
+                    for (int i = lane; i < hi - lo; i += 32) s += r_sum[i];
+                    s = vt_warp_sum(s);
+                    if (lane == 0) sh.left = s;
                 }
                 cluster_sync();
-                token = owner >= 0 ? of(owner)->token[turn] : -1;
-                if (!drafted && token >= 0) child = next_child(cur, cur, token);
+                mine = lane < C ? of(lane)->left : 0.0;
+                left = vt_warp_sum(mine);
+                from_left = left > VT_NOTHING;
+                if (!from_left) {                      // nothing is left of r: p itself
+                    whole(turn, 0, most, sum, mine);
+                    break;
+                }
             }
         }
-        if (child < 0) break;
-        cur = child;
-        if (rank == 0 && tid == 0) a.path[row0 + kept] = cur;
+        // draw: the block whose share holds the target finds the token (mine: lane b has block b's share)
+        const double target = u * (from_left ? left : sum), upto = vt_warp_scan(mine);
+        const unsigned hit = __ballot_sync(0xffffffffu, mine > VT_NOTHING && upto > target), some = __ballot_sync(0xffffffffu, mine > VT_NOTHING);
+        const int owner = hit ? __ffs(hit) - 1 : 31 - __clz(some);
+        const double before = __shfl_sync(0xffffffffu, upto - mine, max(owner, 0));
+        if (owner == rank && warp == 0) {
+            auto p_seg = [&](int i) { return p_sum[i] * weight(p_most[i]); };
+            auto r_seg = [&](int i) { return r_sum[i]; };
+            auto p_weights = [&](int seg, double (&w)[VT_EACH]) {
+                float v[VT_EACH];
+                vt_load(x, lead, true, vocab, seg, v);
+#pragma unroll
+                for (int i = 0; i < VT_EACH; ++i) w[i] = weight(v[i]);
+            };
+            int found;
+            if (DRAFTED && from_left) found = find(lo, hi, lead, before, !hit, target, r_seg, leftover);
+            else found = find(lo, hi, lead, before, !hit, target, p_seg, p_weights);
+            if (lane == 0) sh.token[turn] = found;
+        }
+        cluster_sync();
+        const int token = owner >= 0 ? of(owner)->token[turn] : -1;
+        return {!drafted && token >= 0 ? next_child(cur, cur, token) : -1, token};
+    }
+};
+
+// A cluster walks with a request: only the rows that it reaches are read.
+template <typename T, bool DRAFTED, int NW>
+__global__ void __launch_bounds__(NW * 32, 16 / NW) verify_walk_kernel(const VerifyArgs a) {
+    extern __shared__ __align__(16) double vt_mem[];
+    __shared__ VtShared sh;
+    const int rank = blockIdx.x % a.blocks, seq = blockIdx.x / a.blocks;
+    VtRow<T, DRAFTED, NW> row(a, sh, vt_mem, rank);
+    gb_pdl_launch_dependents();
+    gb_pdl_wait();
+    const int row0 = a.first_row[seq], rows = a.first_row[seq + 1] - row0;
+    if (rows <= 0 || row0 < 0 || row0 > a.n - rows) {  // (the same in all blocks of a cluster)
+        if (rank == 0 && threadIdx.x == 0) { a.accepted[seq] = 0; a.next[seq] = -1; }
+        return;
+    }
+    row.request(row0, rows, a.temperature[seq]);
+    if (rank == 0)
+        for (int i = threadIdx.x; i < rows; i += NW * 32) a.path[row0 + i] = i == 0 ? 0 : -1;
+    __syncthreads();
+    int cur = 0, kept = 1;
+    for (int step = 0;; ++step) {                      // (a child lies behind its parent: at most `rows` steps)
+        const VtOutcome o = row.outcome(cur, step & 1);
+        if (o.child < 0) {
+            if (rank == 0 && threadIdx.x == 0) { a.accepted[seq] = kept; a.next[seq] = o.token; }
+            break;
+        }
+        cur = o.child;
+        if (rank == 0 && threadIdx.x == 0) a.path[row0 + kept] = cur;
         ++kept;
     }
-    if (rank == 0 && tid == 0) {
-        a.accepted[seq] = kept;
-        a.next[seq] = token;
-    }
-    cluster_sync();                                    // (shared memory is read until here)
+    row.cluster_sync();                                // (shared memory is read until here)
 }
 
-// logits, draft: [n, vocab] of one type, rows `stride` numbers apart (draft: or none). Everything else as above; path [n], accepted and next [requests].
-GB_EXPORT int gb_verify_tree(const void* logits, int dtype, long long stride, const void* draft, long long draft_stride, const int* tokens, const int* parents,
-                             const int* first_row, const float* uniform, const float* temperature, int* path, int* accepted, int* next, int n, int num_seqs,
-                             int vocab, cudaStream_t stream) {
-    GB_REQUIRE(n >= 0 && num_seqs >= 0 && vocab > 0 && (n <= 1 || stride >= vocab) && (draft == nullptr || n <= 1 || draft_stride >= vocab), "gb_verify_tree: bad sizes n=%d vocab=%d", n, vocab);
-    GB_REQUIRE(vocab <= (VT_MAX_SEGS - 1) * VT_SEG, "gb_verify_tree: a vocabulary of %d is not built (%d)", vocab, (VT_MAX_SEGS - 1) * VT_SEG);
-    GB_REQUIRE(dtype == GB_F32 || dtype == GB_BF16, "gb_verify_tree: unsupported dtype %d", dtype);
-    GB_REQUIRE(num_seqs < (1 << 27), "gb_verify_tree: %d requests are too many for one launch", num_seqs);
-    if (num_seqs == 0) return 0;
-    GB_REQUIRE(first_row && temperature && accepted && next && (n == 0 || (logits && tokens && parents && uniform && path)), "gb_verify_tree: a tensor is missing");
-    VerifyArgs a = {logits, stride, draft, draft_stride, tokens, parents, first_row, uniform, temperature, path, accepted, next, n, vocab, 1};
-    int blocks = VT_MAX_CLUSTER;
-    while (blocks > 1 && ((long long)num_seqs * blocks > 2 * 148 || vocab < blocks * VT_SEG * VT_WARPS)) blocks /= 2;
+// Every row's outcome at once, a cluster a row: the child, or -2 - token, in the row's place of `path`, from which verify_path_kernel walks.
+template <typename T, bool DRAFTED, int NW>
+__global__ void __launch_bounds__(NW * 32, (DRAFTED ? 20 : NW == VT_MOST_WARPS ? 24 : 32) / NW) verify_rows_kernel(const VerifyArgs a, int num_seqs) {
+    extern __shared__ __align__(16) double vt_mem[];
+    __shared__ VtShared sh;
+    const int rank = blockIdx.x % a.blocks, r = blockIdx.x / a.blocks, lane = threadIdx.x & 31;
+    VtRow<T, DRAFTED, NW> row(a, sh, vt_mem, rank);
+    gb_pdl_launch_dependents();
+    gb_pdl_wait();
+    int seq = -1;                                      // the last request that begins at the row or before it and is not empty
+    for (int s0 = 0; s0 < num_seqs; s0 += 32) {
+        const int s = s0 + lane, first = s < num_seqs ? a.first_row[s] : 0, next = s < num_seqs ? a.first_row[s + 1] : 0;
+        const unsigned hit = __ballot_sync(0xffffffffu, s < num_seqs && first >= 0 && first <= r && r < next && next <= a.n);
+        if (hit) { seq = s0 + __ffs(hit) - 1; break; }
+    }
+    if (seq < 0) return;                               // (a row of no request)
+    const int row0 = a.first_row[seq];
+    row.request(row0, a.first_row[seq + 1] - row0, a.temperature[seq]);
+    __syncthreads();
+    const VtOutcome o = row.outcome(r - row0, 0);
+    if (rank == 0 && threadIdx.x == 0) a.path[r] = o.child >= 0 ? o.child : -2 - o.token;
+    row.cluster_sync();                                // (shared memory is read until here)
+}
+
+// The walk over the rows' outcomes: a warp a request.
+__global__ void __launch_bounds__(32) verify_path_kernel(const VerifyArgs a) {
+    extern __shared__ int vt_next[];
+    const int seq = blockIdx.x, lane = threadIdx.x;
+    gb_pdl_launch_dependents();
+    gb_pdl_wait();
+    const int row0 = a.first_row[seq], rows = a.first_row[seq + 1] - row0;
+    if (rows <= 0 || row0 < 0 || row0 > a.n - rows) {
+        if (lane == 0) { a.accepted[seq] = 0; a.next[seq] = -1; }
+        return;
+    }
+    for (int i = lane; i < rows; i += 32) vt_next[i] = a.path[row0 + i];
+    __syncwarp();
+    int kept = 0;
+    for (int cur = 0;;) {
+        if (lane == 0) a.path[row0 + kept] = cur;
+        ++kept;
+        const int o = vt_next[cur];
+        if (o <= cur || o >= rows) {                   // (a child lies behind its row)
+            if (lane == 0) { a.accepted[seq] = kept; a.next[seq] = o < 0 ? -2 - o : -1; }
+            break;
+        }
+        cur = o;
+    }
+    for (int i = kept + lane; i < rows; i += 32) a.path[row0 + i] = -1;
+}
+
+template <typename T, bool DRAFTED, int NW>
+static int vt_launch(VerifyArgs a, int num_seqs, bool walk, int groups, int blocks, cudaStream_t stream) {
     a.blocks = blocks;
-    const int lanes = dtype == GB_F32 ? 4 : 8, per = gb_ceil_div(gb_ceil_div(vocab + lanes, VT_SEG), blocks);
-    const int smem = per * (draft ? 3 * 8 + 2 * 4 : 8 + 4);
-    const auto kernel = dtype == GB_F32 ? verify_tree_kernel<float> : verify_tree_kernel<__nv_bfloat16>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    GB_REQUIRE(e == cudaSuccess, "gb_verify_tree: %d bytes of shared memory refused: %s", smem, cudaGetErrorString(e));
+    const int per = gb_ceil_div(gb_ceil_div(a.vocab + 16 / (int)sizeof(T), VT_SEG), blocks), smem = per * (DRAFTED ? 3 * 8 + 2 * 4 : 8 + 4);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(num_seqs * blocks);
-    cfg.blockDim = dim3(VT_THREADS);
+    cfg.gridDim = dim3((unsigned)(groups * blocks));
+    cfg.blockDim = dim3(NW * 32);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
@@ -447,7 +526,44 @@ GB_EXPORT int gb_verify_tree(const void* logits, int dtype, long long stride, co
     }
     cfg.attrs = attr;
     cfg.numAttrs = na;
-    e = cudaLaunchKernelEx(&cfg, kernel, a);
+    cudaError_t e = walk ? cudaFuncSetAttribute(verify_walk_kernel<T, DRAFTED, NW>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)
+                         : cudaFuncSetAttribute(verify_rows_kernel<T, DRAFTED, NW>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    GB_REQUIRE(e == cudaSuccess, "gb_verify_tree: %d bytes of shared memory refused: %s", smem, cudaGetErrorString(e));
+    e = walk ? cudaLaunchKernelEx(&cfg, verify_walk_kernel<T, DRAFTED, NW>, a) : cudaLaunchKernelEx(&cfg, verify_rows_kernel<T, DRAFTED, NW>, a, num_seqs);
     GB_REQUIRE(e == cudaSuccess, "gb_verify_tree: launch failed: %s", cudaGetErrorString(e));
+    return 0;
+}
+
+template <typename T, bool DRAFTED>
+static int vt_dispatch(const VerifyArgs& a, int num_seqs, bool walk, cudaStream_t stream) {
+    // Blocks that share a row while all find room at once, eight of four warps a multiprocessor, two segments a warp at least: 388 rows of 100,003 bfloat16 in
+    // clusters of 1 / 2 / 4 70 / 49 / 53 us, 768 of 49,152 float32 64 / 66 / 76. Up to two blocks a multiprocessor have eight warps.
+    const int groups = walk ? num_seqs : a.n;
+    int blocks = VT_MAX_CLUSTER;
+    while (blocks > 1 && ((long long)groups * blocks > 8 * 148 || a.vocab < blocks * VT_SEG * VT_MOST_WARPS)) blocks /= 2;
+    if ((long long)groups * blocks <= 2 * 148) return vt_launch<T, DRAFTED, VT_MOST_WARPS>(a, num_seqs, walk, groups, blocks, stream);
+    return vt_launch<T, DRAFTED, VT_MOST_WARPS / 2>(a, num_seqs, walk, groups, blocks, stream);
+}
+
+// logits, draft: [n, vocab] of one type, rows `stride` numbers apart (draft: or none). Everything else as above; path [n], accepted and next [requests]. walk: as
+// verify_walk_kernel, else all rows at once; no request has more than max_rows rows then.
+GB_EXPORT int gb_verify_tree(const void* logits, int dtype, long long stride, const void* draft, long long draft_stride, const int* tokens, const int* parents,
+                             const int* first_row, const float* uniform, const float* temperature, int* path, int* accepted, int* next, int n, int num_seqs,
+                             int vocab, int walk, cudaStream_t stream) {
+    GB_REQUIRE(n >= 0 && num_seqs >= 0 && vocab > 0 && (n <= 1 || stride >= vocab) && (draft == nullptr || n <= 1 || draft_stride >= vocab), "gb_verify_tree: bad sizes n=%d vocab=%d", n, vocab);
+    GB_REQUIRE(vocab <= (VT_MAX_SEGS - 1) * VT_SEG, "gb_verify_tree: a vocabulary of %d is not built (%d)", vocab, (VT_MAX_SEGS - 1) * VT_SEG);
+    GB_REQUIRE(dtype == GB_F32 || dtype == GB_BF16, "gb_verify_tree: unsupported dtype %d", dtype);
+    GB_REQUIRE(num_seqs < (1 << 27) && n < (1 << 27), "gb_verify_tree: %d requests, %d rows are too many for one launch", num_seqs, n);
+    if (num_seqs == 0) return 0;
+    GB_REQUIRE(first_row && temperature && accepted && next && (n == 0 || (logits && tokens && parents && uniform && path)), "gb_verify_tree: a tensor is missing");
+    const VerifyArgs a = {logits, stride, draft, draft_stride, tokens, parents, first_row, uniform, temperature, path, accepted, next, n, vocab, 1};
+    if (n > VT_MAX_ROWS || n == 0) walk = 1;           // (a request's outcomes fit shared memory)
+    const int rc = dtype == GB_F32 ? (draft ? vt_dispatch<float, true>(a, num_seqs, walk, stream) : vt_dispatch<float, false>(a, num_seqs, walk, stream))
+                                   : (draft ? vt_dispatch<__nv_bfloat16, true>(a, num_seqs, walk, stream) : vt_dispatch<__nv_bfloat16, false>(a, num_seqs, walk, stream));
+    if (rc) return rc;
+    if (!walk) {
+        const cudaError_t e = gb_launch(GB_PDL_ELEMENTWISE, verify_path_kernel, dim3(num_seqs), dim3(32), n * sizeof(int), stream, a);
+        GB_REQUIRE(e == cudaSuccess, "gb_verify_tree: launch failed: %s", cudaGetErrorString(e));
+    }
     return gb_check_launch("gb_verify_tree");
 }

@@ -50,7 +50,7 @@ _SIGNATURES = {
     "gb_gemm_simt": [_P, _I, _P, _I, _P, _I, _I, _I, _I, _I, _LL, _LL, _LL, _P],
     "gb_tree_attention": [_I, _P, _LL, _P, _LL, _I, _P, _P, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _LL, _F, _I, _I, _P, _P, _P],
     "gb_tree_attention_floats": [_I, _I, _I, _I, _I, _I, _I, _I, _I],
-    "gb_verify_tree": [_P, _I, _LL, _P, _LL, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P],
+    "gb_verify_tree": [_P, _I, _LL, _P, _LL, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P],
     "gb_keep_rows": [_P, _P, _I, _I, _I, _LL, _I, _I, _P, _I, _P, _P, _P, _P, _I, _I, _P, _P],
     "gb_attention_rows": [_P, _LL, _P, _LL, _I, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _LL, _F, _I, _P, _P],
     "gb_sample": [_P, _LL, _P, _P, _P, _P, _I, _P, _P, _I, _I, _P],
@@ -2733,6 +2733,14 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vca
           status.data_ptr(), stream)
 
 
+def verify_walks(n: int, num_seqs: int, vocab: int, size: int, drafted: bool) -> bool:
+    """Whether ``verify_tree`` reads only the rows that the walk reaches, one after the other, and not all rows at once."""
+    return n * vocab * size * (2 if drafted else 1) > VERIFY_ROWS_BYTES
+
+
+VERIFY_ROWS_BYTES = 400 << 20
+
+
 def verify_tree(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, seq_first_row: torch.Tensor, uniform: torch.Tensor,
                 temperature: torch.Tensor, path: torch.Tensor, accepted: torch.Tensor, next_token: torch.Tensor,
                 draft_logits: Optional[torch.Tensor] = None) -> None:
@@ -2769,7 +2777,7 @@ def verify_tree(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tenso
     stream = _here(logits, tokens, parents, seq_first_row, uniform, temperature, path, accepted, next_token, draft_logits)
     _call("gb_verify_tree", logits.data_ptr(), dtype, logits.stride(0), _ptr(draft_logits), 0 if draft_logits is None else draft_logits.stride(0),
           tokens.data_ptr(), parents.data_ptr(), seq_first_row.data_ptr(), uniform.data_ptr(), temperature.data_ptr(), path.data_ptr(), accepted.data_ptr(),
-          next_token.data_ptr(), n, num_seqs, vocab, stream)
+          next_token.data_ptr(), n, num_seqs, vocab, int(verify_walks(n, num_seqs, vocab, logits.element_size(), draft_logits is not None)), stream)
 
 
 def keep_rows(kpool: torch.Tensor, vpool: torch.Tensor, block_tables: torch.Tensor, seq_first_row: torch.Tensor, seq_start_pos: torch.Tensor,

@@ -12,6 +12,11 @@ pytestmark = pytest.mark.gpu
 DEV = "cuda"
 
 
+@pytest.fixture(autouse=True, params=[False, True], ids=["all rows", "the walk's rows"])
+def either_way(request, monkeypatch):
+    monkeypatch.setattr(kernels, "verify_walks", lambda *sizes: request.param)
+
+
 def make(shapes, vocab, dtype, seed, drafted, temps, agree=0.7, odd=0, masked=False):
     rng, g = random.Random(seed), torch.Generator().manual_seed(seed)
     firsts, parents = [0], []
