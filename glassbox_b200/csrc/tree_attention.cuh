@@ -35,6 +35,8 @@ struct TreePlan {
     int rows = 0;            // query rows of an item
     int cluster = 0;         // blocks that share an item's keys, a cluster; 0: all items' keys are cut evenly among `blocks`
     int blocks = 0;
+    bool tc = false;         // whole tiles before the trees by tree_attention_tc.cu, `blocks` of it; items of what is left have `rows` query rows
+    bool same = false;       // its items have at most 128 query rows
     long long floats = 0;    // of scratch
 };
 
@@ -71,6 +73,7 @@ struct TreeSeq {
     }
 };
 
+constexpr int TREE_TC_KEYS = 128, TREE_TC_ROWS = 128;      // keys of a tile and rows of a unit of tree_attention_tc.cu
 constexpr int TREE_LEAST_SHARE = 4;      // tiles of keys of a block, where there are enough
 
 // All items' tiles of keys in one row, request by request, key/value head by head, `rows` query rows at a time, cut evenly among the blocks. Every warp works
@@ -78,6 +81,7 @@ constexpr int TREE_LEAST_SHARE = 4;      // tiles of keys of a block, where ther
 struct TreeCut {
     const TreeArgs& a;
     int num_seqs, rows, keys;
+    bool before;             // only whole tiles before the trees
     long long total, share;
     int seq;                 // a request, the tiles and items before it
     long long tile0, item0, tiles_here;
@@ -88,7 +92,7 @@ struct TreeCut {
         if (n <= 0 || start < 0 || a.first_row[s] < 0 || a.first_row[s] > a.n - n) return;
         const int low = a.window > 0 ? max(0, start - a.window + 1) : 0;
         items = (long long)a.nkv * ((n * (a.nh / a.nkv) + rows - 1) / rows);
-        tiles = items * ((start + n + keys - 1) / keys - low / keys);
+        tiles = items * (before ? start / keys : (start + n + keys - 1) / keys - low / keys);
     }
     __device__ __forceinline__ static long long scan(long long v) {
         const int lane = threadIdx.x & 31;
@@ -99,7 +103,8 @@ struct TreeCut {
         }
         return v;
     }
-    __device__ __forceinline__ TreeCut(const TreeArgs& a, int num_seqs, int rows, int keys, int blocks, int least) : a(a), num_seqs(num_seqs), rows(rows), keys(keys) {
+    __device__ __forceinline__ TreeCut(const TreeArgs& a, int num_seqs, int rows, int keys, int blocks, int least, bool before = false)
+        : a(a), num_seqs(num_seqs), rows(rows), keys(keys), before(before) {
         long long sum = 0;
         for (int s0 = 0; s0 < num_seqs; s0 += 32) {
             long long t, i;

@@ -65,11 +65,15 @@ struct TmShape {
 
 // CLUSTER: the blocks of a cluster share one item's keys (blockIdx.x of gridDim.x of them; item: blockIdx.y, request: blockIdx.z) and add up through distributed
 // shared memory. Otherwise all items' tiles of keys are cut evenly among the blocks; what a block finds of an item that it shares with others goes to the
-// scratch, piece number (item + block), and tree_pieces_kernel adds up.
-template <int HD, int WM, int WK, bool CLUSTER>
-__global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const TreeArgs a, int num_seqs) {
+// scratch, piece number (item + block), and tree_pieces_kernel adds up. TAIL: a block an item, the keys behind the whole tiles that tree_attention_tc.cu takes in
+// `tc_blocks` blocks, whose pieces (in units of 128 rows, two a piece) are added to them.
+enum TmMode { TM_EVEN, TM_CLUSTER, TM_TAIL };
+
+template <int HD, int WM, int WK, TmMode MODE>
+__global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const TreeArgs a, int num_seqs, int tc_blocks, bool tc_same) {
     namespace cg = cooperative_groups;
     using Sh = TmShape<HD, WM, WK>;
+    constexpr bool CLUSTER = MODE == TM_CLUSTER;
     constexpr int CH = HD / 8, KS = HD / 16, NT = HD / 8, KW = Sh::KW, KT = KW / 8, P = Sh::P;
     extern __shared__ __align__(16) unsigned char tm_mem[];
     unsigned char* Ks = tm_mem;
@@ -79,7 +83,9 @@ __global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const T
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wm = warp % WM, wk = warp / WM, g = lane >> 2, t = lane & 3;
     const int G = a.nh / a.nkv;
     gb_pdl_launch_dependents();
-    gb_pdl_wait();
+    // (the kernel before a tail is tree_attention_tc.cu's, which lets this one start once it has waited for all before it: its pieces alone are waited for, where
+    // they are read)
+    if constexpr (MODE != TM_TAIL) gb_pdl_wait();
     __nv_bfloat16* out = (__nv_bfloat16*)a.out;
     const __nv_bfloat16* kc = (const __nv_bfloat16*)a.kcache;
     const __nv_bfloat16* vc = (const __nv_bfloat16*)a.vcache;
@@ -266,6 +272,22 @@ __global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const T
             for (int j = 0; j < NT; ++j) *reinterpret_cast<float2*>(to + 8 * j + 2 * t) = make_float2(acc[j][2 * h], acc[j][2 * h + 1]);
             if (t == 0) *reinterpret_cast<float2*>(to + HD) = make_float2(m_run[h], l_run[h]);
         }
+        long long b0 = 0, b1 = -1;                    // the blocks that have pieces of the item, and the first of them
+        const float* pieces = nullptr;
+        const int tc_rows = tc_same ? TREE_TC_ROWS : 2 * TREE_TC_ROWS;
+        if constexpr (MODE == TM_TAIL) {
+            gb_pdl_wait();
+            const int all = s.start / TREE_TC_KEYS;
+            if (all > 0) {
+                TreeCut cut(a, num_seqs, tc_rows, TREE_TC_KEYS, tc_blocks, TREE_LEAST_SHARE, true);
+                cut.seek_seq(blockIdx.z);
+                const int item = kvh * ((M + tc_rows - 1) / tc_rows) + m0 / tc_rows;
+                const long long t0 = cut.tile0 + (long long)item * all;
+                b0 = t0 / cut.share;
+                b1 = (t0 + all - 1) / cut.share;
+                pieces = a.parts + (size_t)(cut.item0 + item + b0) * (2 * TREE_TC_ROWS * P);
+            }
+        }
         const int parts = CLUSTER ? gridDim.x : 1, rank = CLUSTER ? blockIdx.x : 0;
         if (CLUSTER && parts > 1) cg::this_cluster().sync(); else __syncthreads();
         // a pair of channels of every parts-th row
@@ -278,7 +300,25 @@ __global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const T
 #pragma unroll
                 for (int w = 0; w < WK; ++w) top = fmaxf(top, from[((size_t)w * Sh::ROWS + r) * P + HD]);
             }
+            // (TAIL) the pieces' rows: both units where they have the same rows, else the one that has this row
+            const int unit = m % tc_rows / TREE_TC_ROWS, count = MODE == TM_TAIL ? (int)(b1 - b0 + 1) * (tc_same ? 2 : 1) : 0, step = (tc_same ? 1 : 2) * TREE_TC_ROWS * P;
+            const float* piece_row = MODE == TM_TAIL ? pieces + (size_t)(unit * TREE_TC_ROWS + m % TREE_TC_ROWS) * P : nullptr;
+            if constexpr (MODE == TM_TAIL) {
+#pragma unroll 8
+                for (int b = 0; b < count; ++b) top = fmaxf(top, piece_row[(size_t)b * step + HD]);
+            }
             const float o = top == -INFINITY ? 0.f : top;
+            if constexpr (MODE == TM_TAIL) {
+#pragma unroll 8
+                for (int b = 0; b < count; ++b) {
+                    const float* from = piece_row + (size_t)b * step;
+                    const float2 ml = *reinterpret_cast<const float2*>(from + HD), v = *reinterpret_cast<const float2*>(from + c);
+                    const float f = tm_exp2(ml.x - o);
+                    l = fmaf(ml.y, f, l);
+                    x = fmaf(v.x, f, x);
+                    y = fmaf(v.y, f, y);
+                }
+            }
             for (int b = 0; b < parts; ++b) {
                 const float* all = CLUSTER && parts > 1 ? cg::this_cluster().map_shared_rank(res, b) : res;
 #pragma unroll
@@ -291,7 +331,7 @@ __global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const T
                     y = fmaf(v.y, f, y);
                 }
             }
-            if (CLUSTER || tile1 - tile0 == tiles_all) {
+            if (MODE != TM_EVEN || tile1 - tile0 == tiles_all) {
                 const float inv = l != 0.f ? 1.0f / l : 0.f;
                 *reinterpret_cast<uint32_t*>(out + (size_t)(s.row0 + m / G) * a.out_stride + (kvh * G + m % G) * HD + c) = tm_pack(x * inv, y * inv);
             } else {
@@ -316,6 +356,15 @@ __global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const T
         }
         const int all = s.tiles(TM_KEYS), share = (all + gridDim.x - 1) / gridDim.x, tile0 = min(all, (int)blockIdx.x * share);
         work(s, blockIdx.y % a.nkv, m0, tile0, min(all, tile0 + share), all, 0);
+    } else if constexpr (MODE == TM_TAIL) {
+        const TreeSeq s(a, blockIdx.z);
+        const int m0 = blockIdx.y / a.nkv * Sh::ROWS;
+        if (s.start < 0 || m0 >= s.rows * G) {
+            gb_pdl_wait();
+            if (s.start < 0 && blockIdx.y == 0) zeros(s);
+            return;
+        }
+        work(s, blockIdx.y % a.nkv, m0, s.start / TREE_TC_KEYS * (TREE_TC_KEYS / TM_KEYS), s.tiles(TM_KEYS), s.tiles(TM_KEYS), 0);
     } else {
         TreeCut cut(a, num_seqs, Sh::ROWS, TM_KEYS, gridDim.x, TREE_LEAST_SHARE);
         long long at = min(cut.total, blockIdx.x * cut.share);
@@ -379,14 +428,27 @@ __global__ void __launch_bounds__(128) tree_pieces_kernel(const TreeArgs a, int 
     }
 }
 
+int gb_tree_attention_tc(const TreeArgs& a, const TreePlan& plan, int num_seqs, cudaStream_t stream);      // tree_attention_tc.cu
+
 template <int HD, int WM, int WK>
 static int tm_launch(const TreeArgs& a, const TreePlan& plan, int num_seqs, int max_rows, cudaStream_t stream) {
     using Sh = TmShape<HD, WM, WK>;
     const int m_tiles = gb_ceil_div((long long)max_rows * (a.nh / a.nkv), Sh::ROWS);
     GB_REQUIRE((long long)m_tiles * a.nkv * (Sh::ROWS / 8) <= 65535ll * 1024 && (long long)m_tiles * a.nkv <= 65535, "gb_tree_attention: %d rows a request are too many for one launch", max_rows);
     cudaError_t e;
+    if constexpr ((HD == 64 || HD == 128) && ((WM == 1 && WK == 4) || (WM == 4 && WK == 1)))
+        if (plan.tc) {
+            if (gb_tree_attention_tc(a, plan, num_seqs, stream)) return 1;
+            const auto kernel = tree_attention_mma_kernel<HD, WM, WK, TM_TAIL>;
+            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM);
+            GB_REQUIRE(e == cudaSuccess, "gb_tree_attention: %d bytes of shared memory refused: %s", Sh::SMEM, cudaGetErrorString(e));
+            e = gb_launch(GB_PDL_ATTENTION, kernel, dim3(1, m_tiles * a.nkv, num_seqs), dim3(Sh::THREADS), Sh::SMEM, stream, a, num_seqs, plan.blocks, plan.same);
+            GB_REQUIRE(e == cudaSuccess, "gb_tree_attention: launch failed: %s", cudaGetErrorString(e));
+            return gb_check_launch("gb_tree_attention");
+        }
+    GB_REQUIRE(!plan.tc, "gb_tree_attention: no such plan");
     if (plan.cluster) {
-        const auto kernel = tree_attention_mma_kernel<HD, WM, WK, true>;
+        const auto kernel = tree_attention_mma_kernel<HD, WM, WK, TM_CLUSTER>;
         e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM);
         GB_REQUIRE(e == cudaSuccess, "gb_tree_attention: %d bytes of shared memory refused: %s", Sh::SMEM, cudaGetErrorString(e));
         cudaLaunchConfig_t cfg = {};
@@ -407,14 +469,14 @@ static int tm_launch(const TreeArgs& a, const TreePlan& plan, int num_seqs, int 
         ++na;
         cfg.attrs = attr;
         cfg.numAttrs = na;
-        e = cudaLaunchKernelEx(&cfg, kernel, a, num_seqs);
+        e = cudaLaunchKernelEx(&cfg, kernel, a, num_seqs, 0, false);
         GB_REQUIRE(e == cudaSuccess, "gb_tree_attention: launch failed: %s", cudaGetErrorString(e));
         return gb_check_launch("gb_tree_attention");
     }
-    const auto kernel = tree_attention_mma_kernel<HD, WM, WK, false>;
+    const auto kernel = tree_attention_mma_kernel<HD, WM, WK, TM_EVEN>;
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM);
     GB_REQUIRE(e == cudaSuccess, "gb_tree_attention: %d bytes of shared memory refused: %s", Sh::SMEM, cudaGetErrorString(e));
-    e = gb_launch(GB_PDL_ATTENTION, kernel, dim3(plan.blocks), dim3(Sh::THREADS), Sh::SMEM, stream, a, num_seqs);
+    e = gb_launch(GB_PDL_ATTENTION, kernel, dim3(plan.blocks), dim3(Sh::THREADS), Sh::SMEM, stream, a, num_seqs, 0, false);
     GB_REQUIRE(e == cudaSuccess, "gb_tree_attention: launch failed: %s", cudaGetErrorString(e));
     e = gb_launch(GB_PDL_ATTENTION, tree_pieces_kernel<HD, Sh::ROWS>, dim3(m_tiles * a.nkv * (Sh::ROWS / 8), num_seqs), dim3(128), 0, stream, a, num_seqs, m_tiles, plan.blocks);
     GB_REQUIRE(e == cudaSuccess, "gb_tree_attention: launch failed: %s", cudaGetErrorString(e));
@@ -442,11 +504,21 @@ int gb_tree_attention_mma(const TreeArgs& a, const TreePlan& plan, int num_seqs,
     return tm_dispatch<128>(a, plan, num_seqs, max_rows, stream);
 }
 
+constexpr int TREE_TC_ABOVE = 64, TREE_TC_CONTEXT = 512;
+
 // Clusters while every item's blocks find room at once, or all tiles evenly among the blocks that do and a second launch that adds up: whichever this estimate
 // has end sooner.
-TreePlan tree_plan_mma(int num_seqs, int max_rows, int nh, int nkv, int hd, int max_context, int window) {
+TreePlan tree_plan_mma(int num_seqs, int max_rows, int nh, int nkv, int hd, int max_context, int window, bool tc) {
     TreePlan p;
     const long long M = (long long)max_rows * (nh / nkv);
+    if (tc && (hd == 64 || hd == 128) && window == 0 && M > TREE_TC_ABOVE && max_context >= TREE_TC_CONTEXT) {
+        p.tc = true;
+        p.same = M <= TREE_TC_ROWS;
+        p.blocks = 148;
+        p.rows = (long long)num_seqs * nkv * gb_ceil_div(M, 16) <= 4 * 148 ? 16 : 64;
+        p.floats = ((long long)num_seqs * nkv * gb_ceil_div(M, p.same ? TREE_TC_ROWS : 2 * TREE_TC_ROWS) + p.blocks) * 2 * TREE_TC_ROWS * (hd + 2);
+        return p;
+    }
     p.rows = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
     const int room = 148 * (hd > 64 ? (p.rows == 128 && hd == 128 ? 1 : 2) : hd == 64 ? 3 : 4);
     const long long items = (long long)num_seqs * nkv * gb_ceil_div(M, p.rows);

@@ -1,0 +1,412 @@
+// Attention of trees of drafted tokens over the paged cache on the 5th-generation tensor cores (sm_100a), bfloat16 at head sizes 64 and 128: the part of the
+// keys that every row of a request's tree sees, whole tiles of 128 before the tree. What is left of them, the tree itself, its masks and the sum of all parts
+// is tree_attention_mma.cu's.
+//
+// A block has two units of 128 query rows (rows of the tree x query heads that share a key/value head; TMEM lanes). Where a request has at most 128 of them
+// (SAME) both units have the same ones and take the tiles of keys in turn, else they are 256 rows that take every tile. Either way two chains of
+// scores -> softmax -> product keep tensor cores and exponentials busy in turn. Tiles of all items (request, key/value head, 256 rows) are cut evenly among one
+// block a multiprocessor; a block goes through its pieces of items without draining its pipelines.
+//   warp 0, 10  producers of keys and of values: a page is HD / 64 boxes of 64 channels, rings of stages in 128-byte-swizzled rows.
+//   warp 1      issues S_g = Q_g K^T (M 128, N 128, K HD) and O_g += P_g V (M 128, N HD, K 128); the next scores of a unit right behind the product that reads P,
+//               which lies over the first half of the scores' columns.
+//   warps 2-9   softmax, four a unit, a row a thread; they lay the unit's queries out in shared memory, and write O, maxima and sums to the scratch.
+// Without masks there is nothing to compare: a row's tile is 128 exponentials. The scale is above 0. What bounds it: memory where rows are few, else a unit's chain.
+// Every wait is bounded: a wait that runs out sets GB_STATUS_WAIT_TIMEOUT and the block winds down.
+#include "tcgen05.cuh"
+#include "tree_attention.cuh"
+
+constexpr int TC5_M = 128, TC5_KEYS = 128, TC5_WARPS = 11, TC5_SEGS = 64;
+constexpr int TC5_BLOCK = 128 * 128;      // bytes of 128 rows of 64 channels
+constexpr float TC5_NEG_BIG = -1.0e30f;
+
+template <int HD, bool SAME>
+struct Tc5Shape {
+    static constexpr int COLS = HD / 64, TILE = COLS * TC5_BLOCK;
+    static constexpr int STAGES_K = HD == 128 ? 3 : SAME ? 6 : 5, STAGES_V = HD == 128 ? (SAME ? 3 : 2) : SAME ? 6 : 5;
+    static constexpr int K_OFF = (SAME ? 1 : 2) * TILE, V_OFF = K_OFF + STAGES_K * TILE, SH_OFF = V_OFF + STAGES_V * TILE;
+    static constexpr int O_COL = 2 * TC5_KEYS;
+};
+
+struct __align__(16) Tc5Shared {
+    int4 seg[TC5_SEGS];                   // request, item of the request, first tile, tiles
+    int piece[TC5_SEGS];
+    uint64_t q_full;                      // softmax -> MMA: the queries of a piece lie in shared memory (and O of the one before has been read)
+    uint64_t k_full[6], v_full[6], k_free[6], v_free[6];
+    uint64_t s_full[2], p_most[2], p_ready[2], pv_done[2];
+    long long at, end;                    // tiles of all items: the block's next, and the end of its share
+    uint32_t tmem_base;
+    int abort_flag, segs;                 // (segs: negative where the share ends with them)
+    int issued[2], consumed[2];
+};
+static_assert(sizeof(Tc5Shared) <= 2048, "shared memory layout");
+
+__device__ __forceinline__ uint64_t tc5_desc_mn(uint32_t smem_addr) {      // MN-major B operand: column blocks of 64 channels TC5_BLOCK bytes apart
+    uint64_t d = 0;
+    d |= (uint64_t)((smem_addr & 0x3FFFF) >> 4);
+    d |= (uint64_t)((TC5_BLOCK >> 4) & 0x3FFF) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+__device__ __forceinline__ float tc5_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float tc5_max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ void tc5_store16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+                 "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
+
+template <int HD, bool SAME>
+__global__ void __launch_bounds__(TC5_WARPS * 32) tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                                                                           const TreeArgs a, int num_seqs, int page_shift) {
+    using Sh = Tc5Shape<HD, SAME>;
+    constexpr int SK = Sh::STAGES_K, SV = Sh::STAGES_V, COLS = Sh::COLS, ROWS = SAME ? TC5_M : 2 * TC5_M, P = HD + 2;
+    extern __shared__ __align__(1024) unsigned char tc5_mem[];
+    unsigned char* Qs = tc5_mem;
+    unsigned char* Ks = tc5_mem + Sh::K_OFF;
+    unsigned char* Vs = tc5_mem + Sh::V_OFF;
+    Tc5Shared& sh = *reinterpret_cast<Tc5Shared*>(tc5_mem + Sh::SH_OFF);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.nh / a.nkv;
+    gb_pdl_wait();
+    gb_pdl_launch_dependents();
+    if (smem_u32(tc5_mem) & 1023u) {              // swizzled tiles want 1024-byte alignment: refuse rather than compute nonsense
+        if (tid == 0) atomicOr(a.status, GB_STATUS_WAIT_TIMEOUT);
+        return;
+    }
+    {
+        const TreeCut cut(a, num_seqs, ROWS, TC5_KEYS, gridDim.x, TREE_LEAST_SHARE, true);
+        const long long at = min(cut.total, blockIdx.x * cut.share), end = min(cut.total, at + cut.share);
+        if (at >= end) return;                    // uniform for the block, before anything is allocated
+        if (tid == 0) { sh.at = at; sh.end = end; }
+    }
+    if (tid == 0) {
+        mbar_init(&sh.q_full, 8);
+        for (int b = 0; b < SK; ++b) { mbar_init(&sh.k_full[b], 1); mbar_init(&sh.k_free[b], 1); }
+        for (int b = 0; b < SV; ++b) { mbar_init(&sh.v_full[b], 1); mbar_init(&sh.v_free[b], 1); }
+        for (int g = 0; g < 2; ++g) {
+            mbar_init(&sh.s_full[g], 1);
+            mbar_init(&sh.pv_done[g], 1);
+            mbar_init(&sh.p_most[g], 4);
+            mbar_init(&sh.p_ready[g], 4);
+        }
+        sh.abort_flag = 0;
+        sh.issued[0] = sh.issued[1] = sh.consumed[0] = sh.consumed[1] = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem_base)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem_base;
+    volatile int* abort_flag = &sh.abort_flag;
+
+    // what each role counts over all pieces
+    int tiles_done = 0;                           // producers and the issuer: tiles of keys and values
+    int pieces_done = 0, steps = 0, steps1 = 0;   // the issuer and the softmax: pieces, and their unit's tiles (the issuer: unit 0's and unit 1's)
+    bool ok = true;
+    while (true) {
+        // ------------------------------------------------------------------------- the next pieces, up to TC5_SEGS
+        if (warp == 0) {
+            int count = 0;
+            long long at = sh.at;
+            const long long end = sh.end;
+            TreeCut cut(a, num_seqs, ROWS, TC5_KEYS, gridDim.x, TREE_LEAST_SHARE, true);
+            cut.seek(at);
+            for (; at < end && count < TC5_SEGS; ++count) {
+                const TreeSeq s(a, cut.seq);
+                const int all = s.start / TC5_KEYS;
+                const long long off = at - cut.tile0;
+                const int item = (int)(off / all), tile0 = (int)(off % all), tiles = (int)min((long long)all - tile0, end - at);
+                if (lane == 0) {
+                    sh.seg[count] = make_int4(cut.seq, item, tile0, tiles);
+                    sh.piece[count] = (int)(cut.item0 + item + blockIdx.x);
+                }
+                at += tiles;
+                if (at < end) cut.reach(at);
+            }
+            __syncwarp();
+            if (lane == 0) { sh.segs = at < end ? count : -count; sh.at = at; }
+        }
+        __syncthreads();
+        const bool more = sh.segs > 0;
+        const int segs = abs(sh.segs);
+
+        if (warp == 0 || warp == TC5_WARPS - 1) {
+            // --------------------------------------------------------------------- producers
+            const int what = warp == 0 ? 0 : 1, ppt = TC5_KEYS >> page_shift;      // pages per tile (1 .. 16), COLS boxes each
+            uint64_t* full = what == 0 ? sh.k_full : sh.v_full;
+            uint64_t* freed = what == 0 ? sh.k_free : sh.v_free;
+            unsigned char* ring = what == 0 ? Ks : Vs;
+            const CUtensorMap* map = what == 0 ? &map_k : &map_v;
+            const int stages = what == 0 ? SK : SV, nowhere = (int)(a.num_pages * a.nkv * a.page_size);
+            bool bad = false;
+            for (int i = 0; i < segs && ok; ++i) {
+                const int4 seg = sh.seg[i];
+                const TreeSeq s(a, seg.x);
+                const int kvh = seg.y / ((s.rows * G + ROWS - 1) / ROWS);
+                // the first row of this lane's page of a tile (lanes COLS i .. have page i); one that is missing lies behind all pages, where a copy reads zeros
+                auto row_of = [&](int tile) -> int {
+                    if (lane >= COLS * ppt) return nowhere;
+                    const long long page = s.page(a, ((tile * TC5_KEYS) >> page_shift) + lane / COLS);
+                    if (page >= 0) return (int)((page * a.nkv + kvh) * a.page_size);
+                    bad = true;
+                    return nowhere;
+                };
+                int row = row_of(seg.z);
+                for (int j = 0; j < seg.w; ++j, ++tiles_done) {
+                    const int st = tiles_done % stages, next_row = j + 1 < seg.w ? row_of(seg.z + j + 1) : nowhere;      // in flight during the wait
+                    if (lane == 0 && tiles_done >= stages) ok = mbar_wait(&freed[st], (tiles_done / stages - 1) & 1, abort_flag, a.status);
+                    ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+                    if (!ok) break;
+                    if (lane == 0) mbar_expect_tx(&full[st], Sh::TILE);
+                    __syncwarp();
+                    if (lane < COLS * ppt)
+                        tma_load_2d(ring + st * Sh::TILE + lane % COLS * TC5_BLOCK + lane / COLS * a.page_size * 128, map, &full[st], lane % COLS * 64, row);
+                    __syncwarp();
+                    if (lane == 0) sh.issued[what] = tiles_done + 1;
+                    row = next_row;
+                }
+            }
+            if (bad && what == 0) atomicOr(a.status, GB_STATUS_BAD_SLOT);
+        } else if (warp == 1) {
+            // --------------------------------------------------------------------- MMA issuer
+            const uint32_t idesc_qk = umma_idesc(TC5_M, TC5_KEYS), idesc_pv = umma_idesc(TC5_M, HD) | (1u << 16);   // (B of the second is MN-major)
+            const uint64_t q_desc = umma_desc(smem_u32(Qs)), k_desc = umma_desc(smem_u32(Ks)), v_desc = tc5_desc_mn(smem_u32(Vs));
+            for (int i = 0; i < segs && ok; ++i) {
+                const int4 seg = sh.seg[i];
+                int units = 2;
+                if constexpr (!SAME) {
+                    const TreeSeq s(a, seg.x);
+                    const int pairs = (s.rows * G + ROWS - 1) / ROWS;
+                    units = s.rows * G - seg.y % pairs * ROWS > TC5_M ? 2 : 1;
+                }
+                // steps: (tile, unit) in the order in which they are taken; in turn over the tiles, or both units of each
+                const int n = SAME ? seg.w : seg.w * units, ahead = SAME ? 2 : units;
+                if (elect_one()) {
+                    auto tile_of = [&](int x) { return tiles_done + (SAME ? x : x / units); };
+                    auto unit_of = [&](int x) { return SAME ? x & 1 : x % units; };
+                    auto last_of = [&](int x) { return SAME || unit_of(x) == units - 1; };      // the last step that reads its tile
+                    auto scores = [&](int x) {
+                        const int tile = tile_of(x), g = unit_of(x), st = tile % SK;
+                        if (SAME || unit_of(x) == 0) {
+                            if (!mbar_wait(&sh.k_full[st], (tile / SK) & 1, abort_flag, a.status)) return false;
+                            sh.consumed[0] = tile + 1;
+                            tc_fence_after();
+                        }
+                        const uint64_t qd = q_desc + (uint64_t)((SAME ? 0 : g * Sh::TILE) >> 4), kd = k_desc + (uint64_t)((st * Sh::TILE) >> 4);
+#pragma unroll
+                        for (int k = 0; k < HD / 16; ++k) {
+                            const uint64_t o = (uint64_t)((k / 4) * (TC5_BLOCK >> 4) + (k % 4) * 2);
+                            umma_bf16(tmem + (uint32_t)(g * TC5_KEYS), qd + o, kd + o, idesc_qk, k ? 1u : 0u);
+                        }
+                        umma_commit(&sh.s_full[g]);
+                        if (last_of(x)) umma_commit(&sh.k_free[st]);
+                        return true;
+                    };
+                    ok = mbar_wait(&sh.q_full, pieces_done & 1, abort_flag, a.status);
+                    if (ok) {
+                        tc_fence_after();
+                        for (int x = 0; x < ahead && x < n && ok; ++x) ok = scores(x);
+                    }
+                    for (int x = 0; x < n && ok; ++x) {
+                        const int tile = tile_of(x), g = unit_of(x), st = tile % SV;
+                        if (SAME || g == 0) {
+                            ok = mbar_wait(&sh.v_full[st], (tile / SV) & 1, abort_flag, a.status);
+                            if (!ok) break;
+                            sh.consumed[1] = tile + 1;
+                        }
+                        const uint64_t vd = v_desc + (uint64_t)((st * Sh::TILE) >> 4);
+                        const uint32_t pt = tmem + (uint32_t)(g * TC5_KEYS), ot = tmem + (uint32_t)(Sh::O_COL + g * HD);
+                        const bool first = SAME ? x < 2 : x < units;      // the unit's first of the piece: O begins anew
+                        const int step = g ? steps1 : steps;
+                        ok = mbar_wait(&sh.p_most[g], step & 1, abort_flag, a.status);
+                        if (!ok) break;
+                        tc_fence_after();
+#pragma unroll
+                        for (int kk = 0; kk < 6; ++kk)      // 16 keys per instruction: 8 columns of P
+                            umma_bf16_ts(ot, pt + (uint32_t)(kk * 8), vd + (uint64_t)(kk * 16 * 128 >> 4), idesc_pv, (first && kk == 0) ? 0u : 1u);
+                        ok = mbar_wait(&sh.p_ready[g], step & 1, abort_flag, a.status);
+                        if (!ok) break;
+                        tc_fence_after();
+#pragma unroll
+                        for (int kk = 6; kk < 8; ++kk) umma_bf16_ts(ot, pt + (uint32_t)(kk * 8), vd + (uint64_t)(kk * 16 * 128 >> 4), idesc_pv, 1u);
+                        umma_commit(&sh.pv_done[g]);
+                        if (last_of(x)) umma_commit(&sh.v_free[st]);
+                        if (g) ++steps1; else ++steps;
+                        if (x + ahead < n) ok = scores(x + ahead);      // (over the unit's P, which the product just issued reads before)
+                    }
+                }
+                ok = __all_sync(0xffffffffu, ok);
+                steps = __reduce_max_sync(0xffffffffu, steps);      // (one lane has counted them)
+                steps1 = __reduce_max_sync(0xffffffffu, steps1);
+                tiles_done += seg.w;
+                ++pieces_done;
+            }
+        } else {
+            // --------------------------------------------------------------------- softmax
+            const int q = warp & 3;                       // the quarter of TMEM lanes this warp may read
+            const int g = (warp - 2) >> 2;                // the unit
+            const int r = q * 32 + lane;                  // this thread's row of the unit
+            const float sl2 = a.scale * 1.4426950408889634f;
+            const uint32_t lane_base = tmem + ((uint32_t)(q * 32) << 16), s_col = (uint32_t)(g * TC5_KEYS), o_col = (uint32_t)(Sh::O_COL + g * HD);
+            auto gave_up = [&]() {
+                if (!__any_sync(0xffffffffu, *abort_flag)) return false;
+                ok = false;
+                return true;
+            };
+            for (int i = 0; i < segs; ++i) {
+                const int4 seg = sh.seg[i];
+                int mine, units = 2;                      // tiles of this unit
+                // both units are done with the piece before (every warp comes here for every piece, also one that has given up)
+                asm volatile("barrier.cta.sync 1, 256;" ::: "memory");
+                if (!ok) continue;
+                {
+                    const TreeSeq s(a, seg.x);
+                    const int M = s.rows * G, pairs = (M + ROWS - 1) / ROWS, m = seg.y % pairs * ROWS + (SAME ? 0 : g * TC5_M) + r;
+                    if constexpr (!SAME) units = M - seg.y % pairs * ROWS > TC5_M ? 2 : 1;
+                    mine = SAME ? (seg.w + 1 - g) / 2 : g < units ? seg.w : 0;
+                    // the unit's queries into swizzled rows (zeros behind the last)
+                    if (!SAME || g == 0) {
+                        const uint4* from = reinterpret_cast<const uint4*>((const __nv_bfloat16*)a.q + (size_t)(s.row0 + m / G) * a.q_stride + (size_t)(seg.y / pairs * G + m % G) * HD);
+                        unsigned char* to = Qs + (SAME ? 0 : g * Sh::TILE) + r * 128;
+#pragma unroll
+                        for (int c = 0; c < HD / 8; ++c)
+                            *reinterpret_cast<uint4*>(to + c / 8 * TC5_BLOCK + ((c % 8) ^ (r & 7)) * 16) = m < M ? from[c] : make_uint4(0, 0, 0, 0);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    tc_fence_before();                    // (O of the piece before has been read)
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.q_full);
+                }
+                float m_run = TC5_NEG_BIG, l_run = 0.f;
+                for (int j = 0; j < mine; ++j) {
+                    if (!mbar_wait_warp(&sh.s_full[g], steps & 1, abort_flag, a.status)) { ok = false; break; }
+                    tc_fence_after();
+                    uint32_t sv[TC5_KEYS];
+                    tmem_load128(lane_base + s_col, sv);
+                    float mx4[4] = {TC5_NEG_BIG, TC5_NEG_BIG, TC5_NEG_BIG, TC5_NEG_BIG};
+#pragma unroll
+                    for (int k = 0; k < TC5_KEYS; k += 8)
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) mx4[u] = tc5_max3(mx4[u], __uint_as_float(sv[k + 2 * u]), __uint_as_float(sv[k + 2 * u + 1]));
+                    const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sl2;
+                    // the running maximum (in the exponent, base 2) rises, and O is rescaled, only when it is exceeded by more than 8
+                    const bool raise = mx - m_run > 8.0f;
+                    if (j == 0) {
+                        if (raise) m_run = mx;
+                    } else if (__any_sync(0xffffffffu, raise)) {
+                        // the unit's product before is complete (these scores were issued behind it)
+                        if (!mbar_wait_warp(&sh.pv_done[g], (steps - 1) & 1, abort_flag, a.status)) { ok = false; break; }
+                        tc_fence_after();
+                        const float corr = raise ? tc5_exp2(m_run - mx) : 1.0f;
+                        if (raise) m_run = mx;
+                        l_run *= corr;
+#pragma unroll
+                        for (int c = 0; c < HD; c += 16) {
+                            uint32_t ov[16];
+                            tmem_load16(lane_base + o_col + (uint32_t)c, ov);
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) ov[k] = __float_as_uint(__uint_as_float(ov[k]) * corr);
+                            tc5_store16(lane_base + o_col + (uint32_t)c, ov);
+                        }
+                    }
+                    const float2 scale2 = make_float2(sl2, sl2), off2 = make_float2(-m_run, -m_run);
+                    float2 l2[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+                    for (int part = 0; part < TC5_KEYS; part += 32) {
+                        uint32_t pw[16];
+#pragma unroll
+                        for (int c = 0; c < 32; c += 2) {
+                            const float2 y = __ffma2_rn(make_float2(__uint_as_float(sv[part + c]), __uint_as_float(sv[part + c + 1])), scale2, off2);
+                            const float2 p = make_float2(tc5_exp2(y.x), tc5_exp2(y.y));
+                            l2[(c >> 1) & 3] = __fadd2_rn(l2[(c >> 1) & 3], p);
+                            pw[c >> 1] = pack2(__float_as_uint(p.x), __float_as_uint(p.y));
+                        }
+                        tc5_store16(lane_base + s_col + (uint32_t)(part / 2), pw);
+                        if (part == 64 && gave_up()) break;
+                        if (part >= 64) {      // three quarters, and the rest
+                            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(part == 64 ? &sh.p_most[g] : &sh.p_ready[g]);
+                            if (part == 64 && gave_up()) break;
+                        }
+                    }
+                    if (!ok) break;
+                    const float2 lsum = __fadd2_rn(__fadd2_rn(l2[0], l2[1]), __fadd2_rn(l2[2], l2[3]));
+                    l_run += lsum.x + lsum.y;
+                    ++steps;
+                }
+                if (ok && mine > 0) ok = mbar_wait_warp(&sh.pv_done[g], (steps - 1) & 1, abort_flag, a.status);
+                if (!ok) continue;
+                tc_fence_after();
+                // O, maximum (base 2) and sum to the scratch
+                float* to = a.parts + ((size_t)sh.piece[i] * 2 + g) * TC5_M * P + (size_t)r * P;
+#pragma unroll
+                for (int c = 0; c < HD; c += 32) {
+                    uint32_t ov[32];
+                    if (mine > 0) tmem_load32(lane_base + o_col + (uint32_t)c, ov);
+#pragma unroll
+                    for (int k = 0; k < 32; k += 2) *reinterpret_cast<float2*>(to + c + k) = mine > 0 ? make_float2(__uint_as_float(ov[k]), __uint_as_float(ov[k + 1])) : make_float2(0.f, 0.f);
+                }
+                *reinterpret_cast<float2*>(to + HD) = mine > 0 ? make_float2(m_run, l_run) : make_float2(-INFINITY, 0.f);
+            }
+        }
+        __syncthreads();                          // (the list has been read)
+        if (*abort_flag || !more) break;
+    }
+
+    // ------------------------------------------------------------------------------- wind down
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        if (lane == 0 && sh.abort_flag) {
+            // copies that were issued but never consumed may still be in flight: wait for them (bounded)
+            for (int what = 0; what < 2; ++what)
+                for (int it = sh.consumed[what]; it < sh.issued[what]; ++it) {
+                    const int stages = what == 0 ? SK : SV;
+                    uint64_t* bar = what == 0 ? &sh.k_full[it % stages] : &sh.v_full[it % stages];
+                    const long long t1 = clock64();
+                    while (!mbar_try_wait(bar, (it / stages) & 1) && clock64() - t1 < TC_WAIT_CYCLES) {}
+                }
+        }
+        __syncwarp();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+template <int HD, bool SAME>
+static int tc5_launch(const TreeArgs& a, int blocks, int num_seqs, cudaStream_t stream) {
+    using Sh = Tc5Shape<HD, SAME>;
+    constexpr int SMEM = Sh::SH_OFF + (int)sizeof(Tc5Shared);
+    static_assert(SMEM <= 227 * 1024, "the block does not fit");
+    CUtensorMap mk, mv;
+    if (tc_make_map_2d(&mk, a.kcache, a.num_pages * a.nkv * a.page_size, HD, HD, a.page_size, 64, "gb_tree_attention")) return 1;
+    if (tc_make_map_2d(&mv, a.vcache, a.num_pages * a.nkv * a.page_size, HD, HD, a.page_size, 64, "gb_tree_attention")) return 1;
+    cudaError_t e = cudaFuncSetAttribute(tree_attention_tc_kernel<HD, SAME>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+    GB_REQUIRE(e == cudaSuccess, "gb_tree_attention: %d bytes of shared memory refused: %s", SMEM, cudaGetErrorString(e));
+    int page_shift = 0;
+    while ((1 << page_shift) < a.page_size) ++page_shift;
+    e = gb_launch(GB_PDL_ATTENTION, tree_attention_tc_kernel<HD, SAME>, dim3(blocks), dim3(TC5_WARPS * 32), SMEM, stream, mk, mv, a, num_seqs, page_shift);
+    GB_REQUIRE(e == cudaSuccess, "gb_tree_attention: launch failed: %s", cudaGetErrorString(e));
+    return gb_check_launch("gb_tree_attention");
+}
+
+int gb_tree_attention_tc(const TreeArgs& a, const TreePlan& plan, int num_seqs, cudaStream_t stream) {
+    GB_REQUIRE(a.num_pages * a.nkv * a.page_size < (1ll << 31), "gb_tree_attention: the pages hold too many rows");
+    if (a.hd == 64) return plan.same ? tc5_launch<64, true>(a, plan.blocks, num_seqs, stream) : tc5_launch<64, false>(a, plan.blocks, num_seqs, stream);
+    return plan.same ? tc5_launch<128, true>(a, plan.blocks, num_seqs, stream) : tc5_launch<128, false>(a, plan.blocks, num_seqs, stream);
+}
