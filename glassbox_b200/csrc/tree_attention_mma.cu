@@ -288,6 +288,100 @@ __global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const T
                 pieces = a.parts + (size_t)(cut.item0 + item + b0) * (2 * TREE_TC_ROWS * P);
             }
         }
+        if constexpr (MODE == TM_TAIL) {
+            // The pieces' rows (both units where they have the same rows, else the one that has the row) and the warps' own: first every row's maximum and sum over
+            // all of them, then their channels in fours, several sources' loads under way at once.
+            const int each = tc_same ? 2 : 1, count = (int)(b1 - b0 + 1) * each, step = tc_same ? TREE_TC_ROWS * P : 2 * TREE_TC_ROWS * P;
+            float2* stats = reinterpret_cast<float2*>(pages);      // of a row: maximum, 1 / sum
+            // (rows behind the request's last are the last one once more, and not written; sources behind the last have no weight)
+            auto piece_row = [&](int r) -> const float* {
+                const int m = min(m0 + r, M - 1);
+                return pieces + (size_t)((tc_same ? 0 : m % tc_rows / TREE_TC_ROWS) * TREE_TC_ROWS + m % TREE_TC_ROWS) * P;
+            };
+            __syncthreads();
+            constexpr int LANES = Sh::THREADS / Sh::ROWS;      // threads of a row: 8 or 2
+            {
+                const int r = tid / LANES;
+                float top = -INFINITY, l = 0.f;
+                auto add = [&](float2 ml) {
+                    const float up = fmaxf(top, ml.x), o = up == -INFINITY ? 0.f : up;
+                    l = l * tm_exp2(top - o) + ml.y * tm_exp2(ml.x - o);
+                    top = up;
+                };
+                if (tid % LANES == 0)
+#pragma unroll
+                    for (int w = 0; w < WK; ++w) add(*reinterpret_cast<const float2*>(res + ((size_t)w * Sh::ROWS + r) * P + HD));
+                const float* from = piece_row(r) + HD;
+                for (int b = tid % LANES; b < count; b += 8 * LANES) {
+                    float2 ml[8];
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) ml[u] = *reinterpret_cast<const float2*>(from + (size_t)min(b + u * LANES, count - 1) * step);
+#pragma unroll
+                    for (int u = 0; u < 8; ++u)
+                        if (b + u * LANES < count) add(ml[u]);
+                }
+                float most = top;
+#pragma unroll
+                for (int o = 1; o < LANES; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                const float o = most == -INFINITY ? 0.f : most;
+                l *= tm_exp2(top - o);
+#pragma unroll
+                for (int k = 1; k < LANES; k <<= 1) l += __shfl_xor_sync(0xffffffffu, l, k);
+                if (tid % LANES == 0) stats[r] = make_float2(o, l != 0.f ? 1.0f / l : 0.f);
+            }
+            __syncthreads();
+            constexpr int QUADS = HD / 4, AT_ONCE = Sh::THREADS / QUADS, TURNS = 2, BATCH = 6;
+            for (int r0 = tid / QUADS; r0 < Sh::ROWS; r0 += AT_ONCE * TURNS) {
+                const int c = tid % QUADS * 4;
+                float4 sum[TURNS] = {};
+                float2 stat[TURNS];
+                const float* from[TURNS];
+                auto add = [&](int k, float2 lo, float2 hi, float m) {
+                    const float f = tm_exp2(m - stat[k].x) * stat[k].y;
+                    sum[k].x = fmaf(lo.x, f, sum[k].x);
+                    sum[k].y = fmaf(lo.y, f, sum[k].y);
+                    sum[k].z = fmaf(hi.x, f, sum[k].z);
+                    sum[k].w = fmaf(hi.y, f, sum[k].w);
+                };
+#pragma unroll
+                for (int k = 0; k < TURNS; ++k) {
+                    const int r = min(r0 + k * AT_ONCE, Sh::ROWS - 1);
+                    stat[k] = stats[r];
+                    from[k] = piece_row(r);
+#pragma unroll
+                    for (int w = 0; w < WK; ++w) {
+                        const float* own = res + ((size_t)w * Sh::ROWS + r) * P;
+                        add(k, *reinterpret_cast<const float2*>(own + c), *reinterpret_cast<const float2*>(own + c + 2), own[HD]);
+                    }
+                }
+                for (int b = 0; b < count; b += BATCH) {
+                    float2 lo[BATCH][TURNS], hi[BATCH][TURNS];
+                    float top[BATCH][TURNS];
+#pragma unroll
+                    for (int u = 0; u < BATCH; ++u)
+#pragma unroll
+                        for (int k = 0; k < TURNS; ++k) {
+                            const float* at = from[k] + (size_t)min(b + u, count - 1) * step;      // (rows of HD + 2 numbers: 8-byte aligned)
+                            lo[u][k] = *reinterpret_cast<const float2*>(at + c);
+                            hi[u][k] = *reinterpret_cast<const float2*>(at + c + 2);
+                            top[u][k] = b + u < count ? at[HD] : -INFINITY;
+                        }
+#pragma unroll
+                    for (int u = 0; u < BATCH; ++u)
+#pragma unroll
+                        for (int k = 0; k < TURNS; ++k) add(k, lo[u][k], hi[u][k], top[u][k]);
+                }
+#pragma unroll
+                for (int k = 0; k < TURNS; ++k) {
+                    const int r = r0 + k * AT_ONCE, m = m0 + r;
+                    if (r >= Sh::ROWS || m >= M) continue;
+                    uint32_t* to = reinterpret_cast<uint32_t*>(out + (size_t)(s.row0 + m / G) * a.out_stride + (kvh * G + m % G) * HD + c);
+                    to[0] = tm_pack(sum[k].x, sum[k].y);
+                    to[1] = tm_pack(sum[k].z, sum[k].w);
+                }
+            }
+            return;
+        }
         const int parts = CLUSTER ? gridDim.x : 1, rank = CLUSTER ? blockIdx.x : 0;
         if (CLUSTER && parts > 1) cg::this_cluster().sync(); else __syncthreads();
         // a pair of channels of every parts-th row
@@ -300,25 +394,7 @@ __global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const T
 #pragma unroll
                 for (int w = 0; w < WK; ++w) top = fmaxf(top, from[((size_t)w * Sh::ROWS + r) * P + HD]);
             }
-            // (TAIL) the pieces' rows: both units where they have the same rows, else the one that has this row
-            const int unit = m % tc_rows / TREE_TC_ROWS, count = MODE == TM_TAIL ? (int)(b1 - b0 + 1) * (tc_same ? 2 : 1) : 0, step = (tc_same ? 1 : 2) * TREE_TC_ROWS * P;
-            const float* piece_row = MODE == TM_TAIL ? pieces + (size_t)(unit * TREE_TC_ROWS + m % TREE_TC_ROWS) * P : nullptr;
-            if constexpr (MODE == TM_TAIL) {
-#pragma unroll 8
-                for (int b = 0; b < count; ++b) top = fmaxf(top, piece_row[(size_t)b * step + HD]);
-            }
             const float o = top == -INFINITY ? 0.f : top;
-            if constexpr (MODE == TM_TAIL) {
-#pragma unroll 8
-                for (int b = 0; b < count; ++b) {
-                    const float* from = piece_row + (size_t)b * step;
-                    const float2 ml = *reinterpret_cast<const float2*>(from + HD), v = *reinterpret_cast<const float2*>(from + c);
-                    const float f = tm_exp2(ml.x - o);
-                    l = fmaf(ml.y, f, l);
-                    x = fmaf(v.x, f, x);
-                    y = fmaf(v.y, f, y);
-                }
-            }
             for (int b = 0; b < parts; ++b) {
                 const float* all = CLUSTER && parts > 1 ? cg::this_cluster().map_shared_rank(res, b) : res;
 #pragma unroll
@@ -331,7 +407,7 @@ __global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const T
                     y = fmaf(v.y, f, y);
                 }
             }
-            if (MODE != TM_EVEN || tile1 - tile0 == tiles_all) {
+            if (CLUSTER || tile1 - tile0 == tiles_all) {
                 const float inv = l != 0.f ? 1.0f / l : 0.f;
                 *reinterpret_cast<uint32_t*>(out + (size_t)(s.row0 + m / G) * a.out_stride + (kvh * G + m % G) * HD + c) = tm_pack(x * inv, y * inv);
             } else {

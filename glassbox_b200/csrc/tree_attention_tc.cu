@@ -295,13 +295,17 @@ __global__ void __launch_bounds__(TC5_WARPS * 32) tree_attention_tc_kernel(const
                 for (int j = 0; j < mine; ++j) {
                     if (!mbar_wait_warp(&sh.s_full[g], steps & 1, abort_flag, a.status)) { ok = false; break; }
                     tc_fence_after();
-                    uint32_t sv[TC5_KEYS];
-                    tmem_load128(lane_base + s_col, sv);
+                    // The scores of the last 64 keys stay in registers; the first 64 are read once more (all 128 beside the rest spill)
                     float mx4[4] = {TC5_NEG_BIG, TC5_NEG_BIG, TC5_NEG_BIG, TC5_NEG_BIG};
+                    uint32_t sv[TC5_KEYS / 2];
 #pragma unroll
-                    for (int k = 0; k < TC5_KEYS; k += 8)
+                    for (int half = 0; half < TC5_KEYS; half += 64) {
+                        tmem_load64(lane_base + s_col + (uint32_t)half, sv);
 #pragma unroll
-                        for (int u = 0; u < 4; ++u) mx4[u] = tc5_max3(mx4[u], __uint_as_float(sv[k + 2 * u]), __uint_as_float(sv[k + 2 * u + 1]));
+                        for (int k = 0; k < 64; k += 8)
+#pragma unroll
+                            for (int u = 0; u < 4; ++u) mx4[u] = tc5_max3(mx4[u], __uint_as_float(sv[k + 2 * u]), __uint_as_float(sv[k + 2 * u + 1]));
+                    }
                     const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sl2;
                     // the running maximum (in the exponent, base 2) rises, and O is rescaled, only when it is exceeded by more than 8
                     const bool raise = mx - m_run > 8.0f;
@@ -327,10 +331,12 @@ __global__ void __launch_bounds__(TC5_WARPS * 32) tree_attention_tc_kernel(const
                     float2 l2[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
                     for (int part = 0; part < TC5_KEYS; part += 32) {
-                        uint32_t pw[16];
+                        uint32_t pw[16], first[32];
+                        if (part < 64) tmem_load32(lane_base + s_col + (uint32_t)part, first);      // (P lies over scores that have been read)
 #pragma unroll
                         for (int c = 0; c < 32; c += 2) {
-                            const float2 y = __ffma2_rn(make_float2(__uint_as_float(sv[part + c]), __uint_as_float(sv[part + c + 1])), scale2, off2);
+                            const uint32_t s0 = part < 64 ? first[c] : sv[(part + c) & 63], s1 = part < 64 ? first[c + 1] : sv[(part + c + 1) & 63];
+                            const float2 y = __ffma2_rn(make_float2(__uint_as_float(s0), __uint_as_float(s1)), scale2, off2);
                             const float2 p = make_float2(tc5_exp2(y.x), tc5_exp2(y.y));
                             l2[(c >> 1) & 3] = __fadd2_rn(l2[(c >> 1) & 3], p);
                             pw[c >> 1] = pack2(__float_as_uint(p.x), __float_as_uint(p.y));
