@@ -11,7 +11,7 @@
 
 #include <cooperative_groups.h>
 
-constexpr int TM_KEYS = 64, TM_STAGES = 3, TM_MAX_PAGES = 1024;
+constexpr int TM_KEYS = 64, TM_STAGES = 3, TM_MAX_PAGES = 1024, TM_MAX_CLUSTER = 8;
 
 __device__ __forceinline__ uint32_t tm_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void tm_copy16(uint32_t to, const void* from, bool valid) {
@@ -39,14 +39,16 @@ __device__ __forceinline__ uint32_t tm_pack(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// Of the 32 rows of the tree from d0 on (negative: keys before the tree, all seen), those that a row of the batch sees.
-__device__ __forceinline__ unsigned tm_bits(const TreeArgs& a, int rows, int row, int d0) {
+// Of the 32 rows of the tree from d0 on (negative: keys before the tree, all seen), those that a row of the batch sees. `only`: its bits, where they are one word.
+__device__ __forceinline__ unsigned tm_bits(const TreeArgs& a, int rows, int row, unsigned only, int d0) {
     if (d0 <= -32) return 0xffffffffu;
     if (row < 0) return 0u;
     const unsigned* bits = reinterpret_cast<const unsigned*>(a.visible) + (size_t)row * a.words;
     unsigned v;
     if (d0 < 0) {
-        v = ((1u << -d0) - 1u) | (bits[0] << -d0);
+        v = ((1u << -d0) - 1u) | ((a.words == 1 ? only : bits[0]) << -d0);
+    } else if (a.words == 1) {
+        v = d0 < 32 ? only >> d0 : 0u;
     } else {
         const int w = d0 >> 5, sh = d0 & 31;
         v = w < a.words ? bits[w] >> sh : 0u;
@@ -103,15 +105,12 @@ __global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const T
             const int m = m0 + wm * 16 + g + 8 * h;
             row[h] = m < M ? s.row0 + m / G : -1;
             head[h] = kvh * G + m % G;
-            pos[h] = row[h] >= 0 ? a.positions[row[h]] : -1;
         }
         const int base = s.key_lo / TM_KEYS * TM_KEYS, k_begin = base + tile0 * TM_KEYS, k_end = min(s.length, base + tile1 * TM_KEYS), tiles = tile1 - tile0;
         const int page_lo = k_begin >> shift, n_pages = tiles > 0 ? ((k_end - 1) >> shift) - page_lo + 1 : 0;
         const bool staged = n_pages <= TM_MAX_PAGES;
         bool bad = false;
-        __syncthreads();                              // (what the block did before is done with shared memory)
-        if (staged)
-            for (int i = tid; i < n_pages; i += Sh::THREADS) pages[i] = s.page(a, page_lo + i);
+        // (loads whose results are not used at once come first: a warp waits where it needs one)
         uint32_t qf[KS][4];
 #pragma unroll
         for (int k = 0; k < KS; ++k)
@@ -120,6 +119,15 @@ __global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const T
                 const int h = i & 1;
                 qf[k][i] = row[h] >= 0 ? *reinterpret_cast<const uint32_t*>((const __nv_bfloat16*)a.q + (size_t)row[h] * a.q_stride + head[h] * HD + 16 * k + 8 * (i >> 1) + 2 * t) : 0u;
             }
+        unsigned word[2];                             // of the rows' bits, where there is one
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            pos[h] = row[h] >= 0 ? a.positions[row[h]] : -1;
+            word[h] = row[h] >= 0 && a.words == 1 ? (unsigned)a.visible[row[h]] : 0u;
+        }
+        __syncthreads();                              // (what the block did before is done with shared memory)
+        if (staged)
+            for (int i = tid; i < n_pages; i += Sh::THREADS) pages[i] = s.page(a, page_lo + i);
         __syncthreads();
         auto load = [&](int tile) {
             const int k0 = k_begin + tile * TM_KEYS, stage = tile % TM_STAGES;
@@ -178,7 +186,7 @@ __global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const T
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int w = 0; w < (KW + 31) / 32; ++w) see[h][w] = tm_bits(a, s.rows, row[h], k0 + 32 * w - s.start);
+                    for (int w = 0; w < (KW + 31) / 32; ++w) see[h][w] = tm_bits(a, s.rows, row[h], word[h], k0 + 32 * w - s.start);
 #pragma unroll
                 for (int j = 0; j < KT; ++j)
 #pragma unroll
@@ -388,25 +396,35 @@ __global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const T
         for (int i = tid; i < (Sh::ROWS - rank + parts - 1) / parts * (HD / 2); i += Sh::THREADS) {
             const int r = i / (HD / 2) * parts + rank, c = i % (HD / 2) * 2, m = m0 + r;
             if (m >= M) break;
-            float top = -INFINITY, l = 0.f, x = 0.f, y = 0.f;
-            for (int b = 0; b < parts; ++b) {
-                const float* from = CLUSTER && parts > 1 ? cg::this_cluster().map_shared_rank(res, b) : res;
+            // (all loads of other blocks' results first: one trip; blocks behind the last have no weight)
+            constexpr int MOST = CLUSTER ? TM_MAX_CLUSTER : 1;
+            float2 ml[MOST][WK], v[MOST][WK];
 #pragma unroll
-                for (int w = 0; w < WK; ++w) top = fmaxf(top, from[((size_t)w * Sh::ROWS + r) * P + HD]);
-            }
-            const float o = top == -INFINITY ? 0.f : top;
-            for (int b = 0; b < parts; ++b) {
-                const float* all = CLUSTER && parts > 1 ? cg::this_cluster().map_shared_rank(res, b) : res;
+            for (int b = 0; b < MOST; ++b) {
+                const float* all = CLUSTER && parts > 1 ? cg::this_cluster().map_shared_rank(res, min(b, parts - 1)) : res;
 #pragma unroll
                 for (int w = 0; w < WK; ++w) {
                     const float* from = all + ((size_t)w * Sh::ROWS + r) * P;
-                    const float2 ml = *reinterpret_cast<const float2*>(from + HD), v = *reinterpret_cast<const float2*>(from + c);
-                    const float f = tm_exp2(ml.x - o);
-                    l = fmaf(ml.y, f, l);
-                    x = fmaf(v.x, f, x);
-                    y = fmaf(v.y, f, y);
+                    ml[b][w] = *reinterpret_cast<const float2*>(from + HD);
+                    v[b][w] = *reinterpret_cast<const float2*>(from + c);
+                    if (b >= parts) ml[b][w] = make_float2(-INFINITY, 0.f);
                 }
             }
+            float top = -INFINITY, l = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+            for (int b = 0; b < MOST; ++b)
+#pragma unroll
+                for (int w = 0; w < WK; ++w) top = fmaxf(top, ml[b][w].x);
+            const float o = top == -INFINITY ? 0.f : top;
+#pragma unroll
+            for (int b = 0; b < MOST; ++b)
+#pragma unroll
+                for (int w = 0; w < WK; ++w) {
+                    const float f = tm_exp2(ml[b][w].x - o);
+                    l = fmaf(ml[b][w].y, f, l);
+                    x = fmaf(v[b][w].x, f, x);
+                    y = fmaf(v[b][w].y, f, y);
+                }
             if (CLUSTER || tile1 - tile0 == tiles_all) {
                 const float inv = l != 0.f ? 1.0f / l : 0.f;
                 *reinterpret_cast<uint32_t*>(out + (size_t)(s.row0 + m / G) * a.out_stride + (kvh * G + m % G) * HD + c) = tm_pack(x * inv, y * inv);
@@ -599,7 +617,7 @@ TreePlan tree_plan_mma(int num_seqs, int max_rows, int nh, int nkv, int hd, int 
     const int room = 148 * (hd > 64 ? (p.rows == 128 && hd == 128 ? 1 : 2) : hd == 64 ? 3 : 4);
     const long long items = (long long)num_seqs * nkv * gb_ceil_div(M, p.rows);
     const int reach = window > 0 && window + max_rows < max_context ? window + max_rows : max_context, tiles = gb_ceil_div(reach > 0 ? reach : 1, TM_KEYS);
-    int c = 8;
+    int c = TM_MAX_CLUSTER;
     while (c > 1 && (items * c > room || tiles < 2 * c)) c /= 2;
     const double tile_us = 0.5, waves = (double)((items * c + room - 1) / room), cluster_us = waves * gb_ceil_div(tiles, c) * tile_us, even_us = (double)items * tiles / room * tile_us + 4.0;
     p.cluster = cluster_us <= even_us ? c : 0;
