@@ -7,13 +7,13 @@
 //
 // Masks are looked at only where a warp's keys hold some that a row may not see: bits of the tree come as 32 at a time. There a value that is not a finite
 // number must not meet a weight of zero, so such keys go one by one.
+#include "tcgen05.cuh"
 #include "tree_attention.cuh"
 
 #include <cooperative_groups.h>
 
 constexpr int TM_KEYS = 64, TM_STAGES = 3, TM_MAX_PAGES = 1024, TM_MAX_CLUSTER = 8;
 
-__device__ __forceinline__ uint32_t tm_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void tm_copy16(uint32_t to, const void* from, bool valid) {
     const int bytes = valid ? 16 : 0;
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
@@ -60,7 +60,9 @@ __device__ __forceinline__ unsigned tm_bits(const TreeArgs& a, int rows, int row
 
 template <int HD, int WM, int WK>
 struct TmShape {
-    static constexpr int PITCH = HD * 2 + 16, TILE = TM_KEYS * PITCH, THREADS = WM * WK * 32, ROWS = WM * 16, KW = TM_KEYS / WK, P = HD + 2;
+    static constexpr bool TMA = HD % 64 == 0;      // blocks of 64 channels in 128-byte-swizzled rows, else padded rows that threads copy
+    static constexpr int COLS = HD / 64, BLOCK = TM_KEYS * 128;
+    static constexpr int PITCH = TMA ? 128 : HD * 2 + 16, TILE = TMA ? COLS * BLOCK : TM_KEYS * PITCH, THREADS = WM * WK * 32, ROWS = WM * 16, KW = TM_KEYS / WK, P = HD + 2;
     static constexpr int SMEM = 2 * TM_STAGES * TILE + TM_MAX_PAGES * 4;
     static_assert(WM * WK * 16 * P * 4 <= 2 * TM_STAGES * TILE, "the warps' results lie over the stages");
 };
@@ -72,12 +74,17 @@ struct TmShape {
 enum TmMode { TM_EVEN, TM_CLUSTER, TM_TAIL };
 
 template <int HD, int WM, int WK, TmMode MODE>
-__global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const TreeArgs a, int num_seqs, int tc_blocks, bool tc_same) {
+__global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                                                                         const TreeArgs a, int num_seqs, int tc_blocks, bool tc_same) {
     namespace cg = cooperative_groups;
     using Sh = TmShape<HD, WM, WK>;
     constexpr bool CLUSTER = MODE == TM_CLUSTER;
+    constexpr bool TMA = Sh::TMA;
     constexpr int CH = HD / 8, KS = HD / 16, NT = HD / 8, KW = Sh::KW, KT = KW / 8, P = Sh::P;
-    extern __shared__ __align__(16) unsigned char tm_mem[];
+    extern __shared__ __align__(1024) unsigned char tm_mem[];
+    __shared__ __align__(8) uint64_t full[TM_STAGES];      // TMA -> the warps: a stage's keys and values are there
+    __shared__ int abort_word;
+    volatile int* abort_flag = &abort_word;
     unsigned char* Ks = tm_mem;
     unsigned char* Vs = tm_mem + TM_STAGES * Sh::TILE;
     int* pages = reinterpret_cast<int*>(tm_mem + 2 * TM_STAGES * Sh::TILE);
@@ -94,6 +101,18 @@ __global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const T
     const float sl2 = a.scale * 1.4426950408889634f;
     int shift = 0;
     while ((1 << shift) < a.page_size) ++shift;
+    int loaded = 0;                                           // tiles that the block has taken from its stages
+    if constexpr (TMA) {
+        if (smem_u32(tm_mem) & 1023u) {                       // swizzled tiles want 1024-byte alignment: refuse rather than compute nonsense
+            if (tid == 0) atomicOr(a.status, GB_STATUS_WAIT_TIMEOUT);
+            return;
+        }
+        if (tid == 0) {
+            for (int i = 0; i < TM_STAGES; ++i) mbar_init(&full[i], 1);
+            abort_word = 0;
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+    }
 
     // One item's tiles [tile0, tile1) of keys (from the first that any row sees); `tiles` it has in all; `piece`: where a part of them goes.
     auto work = [&](const TreeSeq& s, int kvh, int m0, int tile0, int tile1, int tiles_all, long long piece) {
@@ -125,13 +144,34 @@ __global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const T
             pos[h] = row[h] >= 0 ? a.positions[row[h]] : -1;
             word[h] = row[h] >= 0 && a.words == 1 ? (unsigned)a.visible[row[h]] : 0u;
         }
-        __syncthreads();                              // (what the block did before is done with shared memory)
+        // (what the block did before is done with shared memory, and what it wrote over the stages lies before the copies to come)
+        if constexpr (TMA) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncthreads();
         if (staged)
             for (int i = tid; i < n_pages; i += Sh::THREADS) pages[i] = s.page(a, page_lo + i);
         __syncthreads();
         auto load = [&](int tile) {
-            const int k0 = k_begin + tile * TM_KEYS, stage = tile % TM_STAGES;
-            const uint32_t kb = tm_smem(Ks + stage * Sh::TILE), vb = tm_smem(Vs + stage * Sh::TILE);
+            const int k0 = k_begin + tile * TM_KEYS, stage = (loaded + tile) % TM_STAGES;
+            if constexpr (TMA) {
+                // A lane a box of 64 channels of a page's keys. What no row sees, or is missing, lies behind all pages, where a copy reads zeros; keys behind the
+                // request's last in its page are masked.
+                if (warp != 0) return;
+                const int box = min(a.page_size, TM_KEYS), count = TM_KEYS / box, which = lane & 1, col = lane >> 1 & (Sh::COLS - 1), i = lane / (2 * Sh::COLS);
+                if (lane == 0) mbar_expect_tx(&full[stage], 2 * Sh::TILE);
+                __syncwarp();
+                for (int j = i; j < count; j += 16 / Sh::COLS) {
+                    const int key = k0 + j * box;
+                    int at = (int)(a.num_pages * a.nkv * a.page_size);
+                    if (key < k_end && key + box > s.key_lo) {
+                        const int page = staged ? pages[(key >> shift) - page_lo] : s.page(a, key >> shift);
+                        if (page >= 0) at = (page * a.nkv + kvh) * a.page_size + (key & (a.page_size - 1));
+                        else bad = true;
+                    }
+                    tma_load_2d((which ? Vs : Ks) + stage * Sh::TILE + col * Sh::BLOCK + j * box * 128, which ? &map_v : &map_k, &full[stage], col * 64, at);
+                }
+                return;
+            }
+            const uint32_t kb = smem_u32(Ks + stage * Sh::TILE), vb = smem_u32(Vs + stage * Sh::TILE);
 #pragma unroll
             for (int i = 0; i < TM_KEYS * CH / Sh::THREADS; ++i) {
                 const int idx = tid + i * Sh::THREADS, r = idx / CH, c = idx % CH, key = k0 + r;
@@ -145,10 +185,16 @@ __global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const T
                 tm_copy16(vb + r * Sh::PITCH + c * 16, vc + at, page >= 0);
             }
         };
+        // 16 bytes of a lane's row of a tile for ldmatrix: keys' rows by (lane >> 4) and lane & 7, values' by (lane >> 3) & 1 and lane & 7; pieces in pairs
+        const int k_half = lane >> 3 & 1, v_half = lane >> 4, turn = lane & 7;
+        auto piece_at = [&](int pair, int half) -> uint32_t {
+            if constexpr (TMA) return (uint32_t)(pair / 4 * Sh::BLOCK + (((pair % 4 * 2 + half) ^ turn) << 4));
+            return (uint32_t)(pair * 32 + half * 16);
+        };
 #pragma unroll
         for (int i = 0; i < TM_STAGES - 1; ++i) {
             if (i < tiles) load(i);
-            asm volatile("cp.async.commit_group;" ::: "memory");
+            if constexpr (!TMA) asm volatile("cp.async.commit_group;" ::: "memory");
         }
         float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f}, acc[NT][4];
 #pragma unroll
@@ -156,14 +202,16 @@ __global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const T
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
         for (int tile = 0; tile < tiles; ++tile) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(TM_STAGES - 2) : "memory");
-            __syncthreads();                              // the tile is there, and the one before has been read
+            // the tile is there, and the one before has been read
+            const int stage = (loaded + tile) % TM_STAGES;
+            if constexpr (!TMA) asm volatile("cp.async.wait_group %0;" ::"n"(TM_STAGES - 2) : "memory");
+            __syncthreads();
             if (tile + TM_STAGES - 1 < tiles) load(tile + TM_STAGES - 1);
-            asm volatile("cp.async.commit_group;" ::: "memory");
+            if constexpr (!TMA) asm volatile("cp.async.commit_group;" ::: "memory");
+            if constexpr (TMA) mbar_wait(&full[stage], (loaded + tile) / TM_STAGES & 1, abort_flag, a.status);      // (one that runs out is reported)
             const int k0 = k_begin + tile * TM_KEYS + wk * KW;      // of the warp's keys
-            const unsigned char* vs = Vs + (tile % TM_STAGES) * Sh::TILE + wk * KW * Sh::PITCH;
-            const uint32_t kb = tm_smem(Ks + (tile % TM_STAGES) * Sh::TILE) + (wk * KW + (lane >> 4) * 8 + (lane & 7)) * Sh::PITCH + ((lane >> 3) & 1) * 16;
-            const uint32_t vb = tm_smem(vs) + (((lane >> 3) & 1) * 8 + (lane & 7)) * Sh::PITCH + (lane >> 4) * 16;
+            const unsigned char* vs = Vs + stage * Sh::TILE + wk * KW * Sh::PITCH;
+            const uint32_t kb = smem_u32(Ks + stage * Sh::TILE) + (wk * KW + v_half * 8 + turn) * Sh::PITCH, vb = smem_u32(vs) + (k_half * 8 + turn) * Sh::PITCH;
             float sc[KT][4];
 #pragma unroll
             for (int j = 0; j < KT; ++j)
@@ -174,7 +222,7 @@ __global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const T
 #pragma unroll
                 for (int k = 0; k < KS; ++k) {
                     uint32_t b[4];
-                    tm_ldmatrix(b, kb + j * 8 * Sh::PITCH + k * 32);
+                    tm_ldmatrix(b, kb + j * 8 * Sh::PITCH + piece_at(k, k_half));
                     tm_mma(sc[j], qf[k], b[0], b[1]);
                     tm_mma(sc[j + 1], qf[k], b[2], b[3]);
                 }
@@ -197,7 +245,8 @@ __global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const T
                         if (!ok) sc[j][e] = -INFINITY;
                     }
                 for (int i = lane; i < KW * CH; i += 32) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(vs + i / CH * Sh::PITCH + i % CH * 16);
+                    const int key = i / CH, c = i % CH;
+                    const uint4 v = *reinterpret_cast<const uint4*>(vs + key * Sh::PITCH + (TMA ? c / 8 * Sh::BLOCK + ((c % 8) ^ (key & 7)) * 16 : c * 16));
                     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                     for (int e = 0; e < 4; ++e) odd = odd || (w[e] & 0x7f80u) == 0x7f80u || (w[e] & 0x7f800000u) == 0x7f800000u;
@@ -242,7 +291,7 @@ __global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const T
 #pragma unroll
                     for (int j = 0; j < NT; j += 2) {
                         uint32_t v[4];
-                        tm_ldmatrix_t(v, vb + b * 16 * Sh::PITCH + j * 16);
+                        tm_ldmatrix_t(v, vb + b * 16 * Sh::PITCH + piece_at(j / 2, v_half));
                         tm_mma(acc[j], p, v[0], v[1]);
                         tm_mma(acc[j + 1], p, v[2], v[3]);
                     }
@@ -254,10 +303,11 @@ __global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const T
                     for (int e = 0; e < 2; ++e)
                         for (int tt = 0; tt < 4; ++tt) {
                             const float p0 = __shfl_sync(0xffffffffu, sc[j][e], (lane & ~3) | tt), p1 = __shfl_sync(0xffffffffu, sc[j][2 + e], (lane & ~3) | tt);
-                            const unsigned char* v = vs + (8 * j + 2 * tt + e) * Sh::PITCH + 4 * t;
+                            const int key = 8 * j + 2 * tt + e;
+                            const unsigned char* v = vs + key * Sh::PITCH + 4 * t;
 #pragma unroll
                             for (int c = 0; c < NT; ++c) {
-                                const uint32_t two = *reinterpret_cast<const uint32_t*>(v + 16 * c);
+                                const uint32_t two = *reinterpret_cast<const uint32_t*>(v + (TMA ? c / 8 * Sh::BLOCK + ((c % 8) ^ (key & 7)) * 16 : c * 16));
                                 const float lo = __uint_as_float(two << 16), hi = __uint_as_float(two & 0xffff0000u);
                                 if (p0 != 0.f) { acc[c][0] = fmaf(p0, lo, acc[c][0]); acc[c][1] = fmaf(p0, hi, acc[c][1]); }
                                 if (p1 != 0.f) { acc[c][2] = fmaf(p1, lo, acc[c][2]); acc[c][3] = fmaf(p1, hi, acc[c][3]); }
@@ -265,7 +315,14 @@ __global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const T
                         }
             }
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        if constexpr (!TMA) asm volatile("cp.async.wait_group 0;" ::: "memory");
+        if constexpr (TMA)
+            if (*abort_flag && tid == 0)                  // copies that were issued and not waited for to the end may still be in flight: once more, bounded
+                for (int tile = max(0, tiles - TM_STAGES); tile < tiles; ++tile) {
+                    const long long t0 = clock64();
+                    while (!mbar_try_wait(&full[(loaded + tile) % TM_STAGES], (loaded + tile) / TM_STAGES & 1) && clock64() - t0 < TC_WAIT_CYCLES) {}
+                }
+        loaded += tiles;
         if (bad) atomicOr(a.status, GB_STATUS_BAD_SLOT);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -527,6 +584,12 @@ int gb_tree_attention_tc(const TreeArgs& a, const TreePlan& plan, int num_seqs, 
 template <int HD, int WM, int WK>
 static int tm_launch(const TreeArgs& a, const TreePlan& plan, int num_seqs, int max_rows, cudaStream_t stream) {
     using Sh = TmShape<HD, WM, WK>;
+    CUtensorMap mk = {}, mv = {};
+    if constexpr (Sh::TMA) {
+        const int box = a.page_size < TM_KEYS ? a.page_size : TM_KEYS;
+        if (tc_make_map_2d(&mk, a.kcache, a.num_pages * a.nkv * a.page_size, HD, HD, box, 64, "gb_tree_attention")) return 1;
+        if (tc_make_map_2d(&mv, a.vcache, a.num_pages * a.nkv * a.page_size, HD, HD, box, 64, "gb_tree_attention")) return 1;
+    }
     const int m_tiles = gb_ceil_div((long long)max_rows * (a.nh / a.nkv), Sh::ROWS);
     GB_REQUIRE((long long)m_tiles * a.nkv * (Sh::ROWS / 8) <= 65535ll * 1024 && (long long)m_tiles * a.nkv <= 65535, "gb_tree_attention: %d rows a request are too many for one launch", max_rows);
     cudaError_t e;
@@ -536,7 +599,7 @@ static int tm_launch(const TreeArgs& a, const TreePlan& plan, int num_seqs, int 
             const auto kernel = tree_attention_mma_kernel<HD, WM, WK, TM_TAIL>;
             e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM);
             GB_REQUIRE(e == cudaSuccess, "gb_tree_attention: %d bytes of shared memory refused: %s", Sh::SMEM, cudaGetErrorString(e));
-            e = gb_launch(GB_PDL_ATTENTION, kernel, dim3(1, m_tiles * a.nkv, num_seqs), dim3(Sh::THREADS), Sh::SMEM, stream, a, num_seqs, plan.blocks, plan.same);
+            e = gb_launch(GB_PDL_ATTENTION, kernel, dim3(1, m_tiles * a.nkv, num_seqs), dim3(Sh::THREADS), Sh::SMEM, stream, mk, mv, a, num_seqs, plan.blocks, plan.same);
             GB_REQUIRE(e == cudaSuccess, "gb_tree_attention: launch failed: %s", cudaGetErrorString(e));
             return gb_check_launch("gb_tree_attention");
         }
@@ -563,14 +626,14 @@ static int tm_launch(const TreeArgs& a, const TreePlan& plan, int num_seqs, int 
         ++na;
         cfg.attrs = attr;
         cfg.numAttrs = na;
-        e = cudaLaunchKernelEx(&cfg, kernel, a, num_seqs, 0, false);
+        e = cudaLaunchKernelEx(&cfg, kernel, mk, mv, a, num_seqs, 0, false);
         GB_REQUIRE(e == cudaSuccess, "gb_tree_attention: launch failed: %s", cudaGetErrorString(e));
         return gb_check_launch("gb_tree_attention");
     }
     const auto kernel = tree_attention_mma_kernel<HD, WM, WK, TM_EVEN>;
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM);
     GB_REQUIRE(e == cudaSuccess, "gb_tree_attention: %d bytes of shared memory refused: %s", Sh::SMEM, cudaGetErrorString(e));
-    e = gb_launch(GB_PDL_ATTENTION, kernel, dim3(plan.blocks), dim3(Sh::THREADS), Sh::SMEM, stream, a, num_seqs, 0, false);
+    e = gb_launch(GB_PDL_ATTENTION, kernel, dim3(plan.blocks), dim3(Sh::THREADS), Sh::SMEM, stream, mk, mv, a, num_seqs, 0, false);
     GB_REQUIRE(e == cudaSuccess, "gb_tree_attention: launch failed: %s", cudaGetErrorString(e));
     e = gb_launch(GB_PDL_ATTENTION, tree_pieces_kernel<HD, Sh::ROWS>, dim3(m_tiles * a.nkv * (Sh::ROWS / 8), num_seqs), dim3(128), 0, stream, a, num_seqs, m_tiles, plan.blocks);
     GB_REQUIRE(e == cudaSuccess, "gb_tree_attention: launch failed: %s", cudaGetErrorString(e));
@@ -588,7 +651,8 @@ static int tm_dispatch(const TreeArgs& a, const TreePlan& plan, int num_seqs, in
 }
 
 int gb_tree_attention_mma(const TreeArgs& a, const TreePlan& plan, int num_seqs, int max_rows, cudaStream_t stream) {
-    GB_REQUIRE(a.page_size > 0 && (a.page_size & (a.page_size - 1)) == 0, "gb_tree_attention: pages of %d tokens (a power of two) are not built here", a.page_size);
+    GB_REQUIRE(a.page_size >= 8 && (a.page_size & (a.page_size - 1)) == 0, "gb_tree_attention: pages of %d tokens (a power of two from 8 on) are not built here", a.page_size);
+    GB_REQUIRE(a.num_pages * a.nkv * a.page_size < (1ll << 31), "gb_tree_attention: the pages hold too many rows");
     GB_REQUIRE((uintptr_t)a.kcache % 16 == 0 && (uintptr_t)a.vcache % 16 == 0 && (uintptr_t)a.q % 4 == 0 && a.q_stride % 2 == 0 && (uintptr_t)a.out % 4 == 0 && a.out_stride % 2 == 0,
                "gb_tree_attention: rows must be 4-byte aligned, pages 16-byte aligned");
     if (a.hd == 32) return tm_dispatch<32>(a, plan, num_seqs, max_rows, stream);

@@ -2652,14 +2652,14 @@ TREE_MAX_ROWS = 1024           # rows of a request's tree
 VERIFY_MAX_VOCAB = 4096 * 512
 
 
-def tree_attention_kind(q: torch.Tensor, out: torch.Tensor, hd: int, page_size: int, scale: float) -> int:
+def tree_attention_kind(q: torch.Tensor, out: torch.Tensor, hd: int, page_size: int, scale: float, rows: int) -> int:
     """Which kernels ``tree_attention`` runs: 1 the tensor cores' (bfloat16, head sizes 32, 64, 96 and 128, rows that start at 4 bytes, pages of a
-    power of two), 2 tcgen05's, too, where there is enough for them (rows of q at 16 bytes, pages of 8 to 128 tokens, a scale above 0), 0 the one for
+    power of two from 8 on, below 2^31 rows of them), 2 tcgen05's, too, where there is enough for them (rows of q at 16 bytes, pages of 8 to 128 tokens, a scale above 0), 0 the one for
     everything else."""
-    if not (q.dtype == torch.bfloat16 and hd in (32, 64, 96, 128) and page_size & (page_size - 1) == 0
+    if not (q.dtype == torch.bfloat16 and hd in (32, 64, 96, 128) and page_size >= 8 and page_size & (page_size - 1) == 0 and rows < 1 << 31
             and q.stride(0) % 2 == 0 and q.data_ptr() % 4 == 0 and out.stride(0) % 2 == 0 and out.data_ptr() % 4 == 0):
         return 0
-    return 2 if scale > 0 and 8 <= page_size <= 128 and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0 else 1
+    return 2 if scale > 0 and page_size <= 128 and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0 else 1
 
 
 @functools.lru_cache(maxsize=4096)
@@ -2725,7 +2725,7 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vca
     stream = _here(q, out, kcache, vcache, block_tables, seq_first_row, seq_start_pos, positions, visible, parts, status)
     if not n or not num_seqs or not max_rows_per_seq:
         return
-    kind = tree_attention_kind(q, out, hd, page_size, scale)
+    kind = tree_attention_kind(q, out, hd, page_size, scale, kcache.shape[0] * nkv * page_size)
     max_context, window = int(max_context), int(window or 0)
     floats = _tree_floats(kind, n, num_seqs, max_rows_per_seq, nh, nkv, hd, max_context, window)
     if floats and (parts is None or parts.dtype != torch.float32 or not parts.is_contiguous() or parts.numel() < floats):
