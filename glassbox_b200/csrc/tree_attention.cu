@@ -252,7 +252,7 @@ GB_EXPORT int gb_tree_attention(int kind, const void* q, long long q_stride, voi
                    "gb_tree_attention: this scale, page size or alignment is not built for tcgen05");
         GB_REQUIRE(dtype == GB_BF16, "gb_tree_attention: the tensor cores' kernel takes bfloat16");
         const TreePlan plan = tree_plan_mma(num_seqs, max_rows, nh, nkv, hd, max_context, window, kind == 2);
-        GB_REQUIRE(plan.floats == 0 || parts != nullptr, "gb_tree_attention: the scratch is missing");
+        GB_REQUIRE(plan.floats == 0 || (parts != nullptr && (uintptr_t)parts % 16 == 0), "gb_tree_attention: the scratch is missing or not 16-byte aligned");
         return gb_tree_attention_mma(a, plan, num_seqs, max_rows, stream);
     }
     a.splits = ta_splits(num_seqs, max_rows, nh, nkv, max_context, window);

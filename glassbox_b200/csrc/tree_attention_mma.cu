@@ -11,8 +11,9 @@
 #include "tree_attention.cuh"
 
 #include <cooperative_groups.h>
+#include <type_traits>
 
-constexpr int TM_KEYS = 64, TM_STAGES = 3, TM_MAX_PAGES = 1024, TM_MAX_CLUSTER = 8;
+constexpr int TM_KEYS = 64, TM_MAX_PAGES = 1024, TM_MAX_CLUSTER = 8;
 
 __device__ __forceinline__ void tm_copy16(uint32_t to, const void* from, bool valid) {
     const int bytes = valid ? 16 : 0;
@@ -61,10 +62,11 @@ __device__ __forceinline__ unsigned tm_bits(const TreeArgs& a, int rows, int row
 template <int HD, int WM, int WK>
 struct TmShape {
     static constexpr bool TMA = HD % 64 == 0;      // blocks of 64 channels in 128-byte-swizzled rows, else padded rows that threads copy
+    static constexpr int STAGES = HD == 64 ? 4 : 3;
     static constexpr int COLS = HD / 64, BLOCK = TM_KEYS * 128;
     static constexpr int PITCH = TMA ? 128 : HD * 2 + 16, TILE = TMA ? COLS * BLOCK : TM_KEYS * PITCH, THREADS = WM * WK * 32, ROWS = WM * 16, KW = TM_KEYS / WK, P = HD + 2;
-    static constexpr int SMEM = 2 * TM_STAGES * TILE + TM_MAX_PAGES * 4;
-    static_assert(WM * WK * 16 * P * 4 <= 2 * TM_STAGES * TILE, "the warps' results lie over the stages");
+    static constexpr int SMEM = 2 * STAGES * TILE + TM_MAX_PAGES * 4;
+    static_assert(WM * WK * 16 * P * 4 <= 2 * STAGES * TILE, "the warps' results lie over the stages");
 };
 
 // CLUSTER: the blocks of a cluster share one item's keys (blockIdx.x of gridDim.x of them; item: blockIdx.y, request: blockIdx.z) and add up through distributed
@@ -80,14 +82,18 @@ __global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const _
     using Sh = TmShape<HD, WM, WK>;
     constexpr bool CLUSTER = MODE == TM_CLUSTER;
     constexpr bool TMA = Sh::TMA;
+    constexpr int STAGES = Sh::STAGES, NW = WM * WK;
+    // Tiles that are under way beside the one worked on: with TMA one stage less than there are, so that a warp may be a tile behind the one that asks for
+    // the next (all warps at a barrier a tile: 136 us where this takes %s).
+    constexpr int AHEAD = TMA ? STAGES - 2 : STAGES - 1;
     constexpr int CH = HD / 8, KS = HD / 16, NT = HD / 8, KW = Sh::KW, KT = KW / 8, P = Sh::P;
     extern __shared__ __align__(1024) unsigned char tm_mem[];
-    __shared__ __align__(8) uint64_t full[TM_STAGES];      // TMA -> the warps: a stage's keys and values are there
+    __shared__ __align__(8) uint64_t full[STAGES], done[STAGES];      // TMA -> the warps: a stage's keys and values are there; the warps -> warp 0: they are read
     __shared__ int abort_word;
     volatile int* abort_flag = &abort_word;
     unsigned char* Ks = tm_mem;
-    unsigned char* Vs = tm_mem + TM_STAGES * Sh::TILE;
-    int* pages = reinterpret_cast<int*>(tm_mem + 2 * TM_STAGES * Sh::TILE);
+    unsigned char* Vs = tm_mem + STAGES * Sh::TILE;
+    int* pages = reinterpret_cast<int*>(tm_mem + 2 * STAGES * Sh::TILE);
     float* res = reinterpret_cast<float*>(tm_mem);           // the warps' results: [WK][ROWS][channels, maximum, sum]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wm = warp % WM, wk = warp / WM, g = lane >> 2, t = lane & 3;
     const int G = a.nh / a.nkv;
@@ -108,7 +114,7 @@ __global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const _
             return;
         }
         if (tid == 0) {
-            for (int i = 0; i < TM_STAGES; ++i) mbar_init(&full[i], 1);
+            for (int i = 0; i < STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&done[i], NW); }
             abort_word = 0;
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
@@ -151,12 +157,15 @@ __global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const _
             for (int i = tid; i < n_pages; i += Sh::THREADS) pages[i] = s.page(a, page_lo + i);
         __syncthreads();
         auto load = [&](int tile) {
-            const int k0 = k_begin + tile * TM_KEYS, stage = (loaded + tile) % TM_STAGES;
+            const int k0 = k_begin + tile * TM_KEYS, stage = (loaded + tile) % STAGES;
             if constexpr (TMA) {
                 // A lane a box of 64 channels of a page's keys. What no row sees, or is missing, lies behind all pages, where a copy reads zeros; keys behind the
                 // request's last in its page are masked.
                 if (warp != 0) return;
                 const int box = min(a.page_size, TM_KEYS), count = TM_KEYS / box, which = lane & 1, col = lane >> 1 & (Sh::COLS - 1), i = lane / (2 * Sh::COLS);
+                const int use = (loaded + tile) / STAGES;      // of the stage
+                if (use > 0) mbar_wait(&done[stage], (use - 1) & 1, abort_flag, a.status);
+                if (__any_sync(0xffffffffu, *abort_flag)) return;
                 if (lane == 0) mbar_expect_tx(&full[stage], 2 * Sh::TILE);
                 __syncwarp();
                 for (int j = i; j < count; j += 16 / Sh::COLS) {
@@ -192,7 +201,7 @@ __global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const _
             return (uint32_t)(pair * 32 + half * 16);
         };
 #pragma unroll
-        for (int i = 0; i < TM_STAGES - 1; ++i) {
+        for (int i = 0; i < AHEAD; ++i) {
             if (i < tiles) load(i);
             if constexpr (!TMA) asm volatile("cp.async.commit_group;" ::: "memory");
         }
@@ -203,12 +212,14 @@ __global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const _
             for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
         for (int tile = 0; tile < tiles; ++tile) {
             // the tile is there, and the one before has been read
-            const int stage = (loaded + tile) % TM_STAGES;
-            if constexpr (!TMA) asm volatile("cp.async.wait_group %0;" ::"n"(TM_STAGES - 2) : "memory");
-            __syncthreads();
-            if (tile + TM_STAGES - 1 < tiles) load(tile + TM_STAGES - 1);
+            const int stage = (loaded + tile) % STAGES;
+            if constexpr (!TMA) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory");
+                __syncthreads();
+            }
+            if (tile + AHEAD < tiles) load(tile + AHEAD);
             if constexpr (!TMA) asm volatile("cp.async.commit_group;" ::: "memory");
-            if constexpr (TMA) mbar_wait(&full[stage], (loaded + tile) / TM_STAGES & 1, abort_flag, a.status);      // (one that runs out is reported)
+            if constexpr (TMA) mbar_wait(&full[stage], (loaded + tile) / STAGES & 1, abort_flag, a.status);      // (one that runs out is reported)
             const int k0 = k_begin + tile * TM_KEYS + wk * KW;      // of the warp's keys
             const unsigned char* vs = Vs + stage * Sh::TILE + wk * KW * Sh::PITCH;
             const uint32_t kb = smem_u32(Ks + stage * Sh::TILE) + (wk * KW + v_half * 8 + turn) * Sh::PITCH, vb = smem_u32(vs) + (k_half * 8 + turn) * Sh::PITCH;
@@ -314,13 +325,17 @@ __global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const _
                             }
                         }
             }
+            if constexpr (TMA) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&done[stage]);
+            }
         }
         if constexpr (!TMA) asm volatile("cp.async.wait_group 0;" ::: "memory");
         if constexpr (TMA)
             if (*abort_flag && tid == 0)                  // copies that were issued and not waited for to the end may still be in flight: once more, bounded
-                for (int tile = max(0, tiles - TM_STAGES); tile < tiles; ++tile) {
+                for (int tile = max(0, tiles - STAGES); tile < tiles; ++tile) {
                     const long long t0 = clock64();
-                    while (!mbar_try_wait(&full[(loaded + tile) % TM_STAGES], (loaded + tile) / TM_STAGES & 1) && clock64() - t0 < TC_WAIT_CYCLES) {}
+                    while (!mbar_try_wait(&full[(loaded + tile) % STAGES], (loaded + tile) / STAGES & 1) && clock64() - t0 < TC_WAIT_CYCLES) {}
                 }
         loaded += tiles;
         if (bad) atomicOr(a.status, GB_STATUS_BAD_SLOT);
@@ -357,12 +372,11 @@ __global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const _
             // The pieces' rows (both units where they have the same rows, else the one that has the row) and the warps' own: first every row's maximum and sum over
             // all of them, then their channels in fours, several sources' loads under way at once.
             const int each = tc_same ? 2 : 1, count = (int)(b1 - b0 + 1) * each, step = tc_same ? TREE_TC_ROWS * P : 2 * TREE_TC_ROWS * P;
+            // The rows' place in the pieces: [units of 128 rows][blocks of 32][channels, maximum, sum][32 rows]. (Rows behind the request's last hold numbers that
+            // are not written out.)
+            const float* mine = pieces + (tc_same ? 0 : m0 % tc_rows / TREE_TC_ROWS) * (TREE_TC_ROWS * P);
+            auto row_at = [&](int r) -> const float* { return mine + (m0 + r) % TREE_TC_ROWS / 32 * (32 * P) + (m0 + r) % 32; };
             float2* stats = reinterpret_cast<float2*>(pages);      // of a row: maximum, 1 / sum
-            // (rows behind the request's last are the last one once more, and not written; sources behind the last have no weight)
-            auto piece_row = [&](int r) -> const float* {
-                const int m = min(m0 + r, M - 1);
-                return pieces + (size_t)((tc_same ? 0 : m % tc_rows / TREE_TC_ROWS) * TREE_TC_ROWS + m % TREE_TC_ROWS) * P;
-            };
             __syncthreads();
             constexpr int LANES = Sh::THREADS / Sh::ROWS;      // threads of a row: 8 or 2
             {
@@ -376,11 +390,14 @@ __global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const _
                 if (tid % LANES == 0)
 #pragma unroll
                     for (int w = 0; w < WK; ++w) add(*reinterpret_cast<const float2*>(res + ((size_t)w * Sh::ROWS + r) * P + HD));
-                const float* from = piece_row(r) + HD;
+                const float* from = row_at(r) + HD * 32;
                 for (int b = tid % LANES; b < count; b += 8 * LANES) {
                     float2 ml[8];
 #pragma unroll
-                    for (int u = 0; u < 8; ++u) ml[u] = *reinterpret_cast<const float2*>(from + (size_t)min(b + u * LANES, count - 1) * step);
+                    for (int u = 0; u < 8; ++u) {
+                        const float* at = from + (size_t)min(b + u * LANES, count - 1) * step;
+                        ml[u] = make_float2(at[0], at[32]);
+                    }
 #pragma unroll
                     for (int u = 0; u < 8; ++u)
                         if (b + u * LANES < count) add(ml[u]);
@@ -395,102 +412,99 @@ __global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const _
                 if (tid % LANES == 0) stats[r] = make_float2(o, l != 0.f ? 1.0f / l : 0.f);
             }
             __syncthreads();
-            constexpr int QUADS = HD / 4, AT_ONCE = Sh::THREADS / QUADS, TURNS = 2, BATCH = 6;
-            for (int r0 = tid / QUADS; r0 < Sh::ROWS; r0 += AT_ONCE * TURNS) {
-                const int c = tid % QUADS * 4;
-                float4 sum[TURNS] = {};
-                float2 stat[TURNS];
-                const float* from[TURNS];
-                auto add = [&](int k, float2 lo, float2 hi, float m) {
-                    const float f = tm_exp2(m - stat[k].x) * stat[k].y;
-                    sum[k].x = fmaf(lo.x, f, sum[k].x);
-                    sum[k].y = fmaf(lo.y, f, sum[k].y);
-                    sum[k].z = fmaf(hi.x, f, sum[k].z);
-                    sum[k].w = fmaf(hi.y, f, sum[k].w);
-                };
+            // A thread has four rows of a channel, a warp 16 rows of eight; several sources' loads are under way at once. The sums go where the warps' own results
+            // were, whose channel nobody else reads.
+            constexpr int BATCH = 8, QUADS = Sh::ROWS / 4;
+            for (int i = tid; i < QUADS * HD; i += Sh::THREADS) {
+                const int r = i % 4 * 4 + i / (4 * HD) * 16, c = i / 4 % HD;
+                float top[4], inv[4], sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int k = 0; k < TURNS; ++k) {
-                    const int r = min(r0 + k * AT_ONCE, Sh::ROWS - 1);
-                    stat[k] = stats[r];
-                    from[k] = piece_row(r);
+                for (int k = 0; k < 4; ++k) {
+                    top[k] = stats[r + k].x;
+                    inv[k] = stats[r + k].y;
 #pragma unroll
                     for (int w = 0; w < WK; ++w) {
-                        const float* own = res + ((size_t)w * Sh::ROWS + r) * P;
-                        add(k, *reinterpret_cast<const float2*>(own + c), *reinterpret_cast<const float2*>(own + c + 2), own[HD]);
+                        const float* own = res + ((size_t)w * Sh::ROWS + r + k) * P;
+                        sum[k] = fmaf(own[c], tm_exp2(own[HD] - top[k]), sum[k]);
                     }
                 }
+                const float* from = row_at(r);
                 for (int b = 0; b < count; b += BATCH) {
-                    float2 lo[BATCH][TURNS], hi[BATCH][TURNS];
-                    float top[BATCH][TURNS];
+                    float4 v[BATCH], m[BATCH];
+#pragma unroll
+                    for (int u = 0; u < BATCH; ++u) {
+                        const float* at = from + (size_t)min(b + u, count - 1) * step;
+                        v[u] = *reinterpret_cast<const float4*>(at + c * 32);
+                        m[u] = *reinterpret_cast<const float4*>(at + HD * 32);
+                    }
 #pragma unroll
                     for (int u = 0; u < BATCH; ++u)
-#pragma unroll
-                        for (int k = 0; k < TURNS; ++k) {
-                            const float* at = from[k] + (size_t)min(b + u, count - 1) * step;      // (rows of HD + 2 numbers: 8-byte aligned)
-                            lo[u][k] = *reinterpret_cast<const float2*>(at + c);
-                            hi[u][k] = *reinterpret_cast<const float2*>(at + c + 2);
-                            top[u][k] = b + u < count ? at[HD] : -INFINITY;
+                        if (b + u < count) {
+                            sum[0] = fmaf(v[u].x, tm_exp2(m[u].x - top[0]), sum[0]);
+                            sum[1] = fmaf(v[u].y, tm_exp2(m[u].y - top[1]), sum[1]);
+                            sum[2] = fmaf(v[u].z, tm_exp2(m[u].z - top[2]), sum[2]);
+                            sum[3] = fmaf(v[u].w, tm_exp2(m[u].w - top[3]), sum[3]);
                         }
-#pragma unroll
-                    for (int u = 0; u < BATCH; ++u)
-#pragma unroll
-                        for (int k = 0; k < TURNS; ++k) add(k, lo[u][k], hi[u][k], top[u][k]);
                 }
 #pragma unroll
-                for (int k = 0; k < TURNS; ++k) {
-                    const int r = r0 + k * AT_ONCE, m = m0 + r;
-                    if (r >= Sh::ROWS || m >= M) continue;
-                    uint32_t* to = reinterpret_cast<uint32_t*>(out + (size_t)(s.row0 + m / G) * a.out_stride + (kvh * G + m % G) * HD + c);
-                    to[0] = tm_pack(sum[k].x, sum[k].y);
-                    to[1] = tm_pack(sum[k].z, sum[k].w);
-                }
+                for (int k = 0; k < 4; ++k) res[(size_t)(r + k) * P + c] = sum[k] * inv[k];
+            }
+            __syncthreads();
+            for (int i = tid; i < Sh::ROWS * (HD / 2); i += Sh::THREADS) {
+                const int r = i / (HD / 2), c = i % (HD / 2) * 2, m = m0 + r;
+                if (m >= M) break;
+                *reinterpret_cast<uint32_t*>(out + (size_t)(s.row0 + m / G) * a.out_stride + (kvh * G + m % G) * HD + c) = tm_pack(res[(size_t)r * P + c], res[(size_t)r * P + c + 1]);
             }
             return;
         }
         const int parts = CLUSTER ? gridDim.x : 1, rank = CLUSTER ? blockIdx.x : 0;
         if (CLUSTER && parts > 1) cg::this_cluster().sync(); else __syncthreads();
-        // a pair of channels of every parts-th row
-        for (int i = tid; i < (Sh::ROWS - rank + parts - 1) / parts * (HD / 2); i += Sh::THREADS) {
-            const int r = i / (HD / 2) * parts + rank, c = i % (HD / 2) * 2, m = m0 + r;
-            if (m >= M) break;
-            // (all loads of other blocks' results first: one trip; blocks behind the last have no weight)
-            constexpr int MOST = CLUSTER ? TM_MAX_CLUSTER : 1;
-            float2 ml[MOST][WK], v[MOST][WK];
+        // A pair of channels of every parts-th row; all loads of other blocks' results come first: one trip.
+        auto add_up = [&](auto blocks) {
+            constexpr int MOST = decltype(blocks)::value;
+            for (int i = tid; i < (Sh::ROWS - rank + MOST - 1) / MOST * (HD / 2); i += Sh::THREADS) {
+                const int r = i / (HD / 2) * MOST + rank, c = i % (HD / 2) * 2, m = m0 + r;
+                if (m >= M) break;
+                float2 ml[MOST][WK], v[MOST][WK];
 #pragma unroll
-            for (int b = 0; b < MOST; ++b) {
-                const float* all = CLUSTER && parts > 1 ? cg::this_cluster().map_shared_rank(res, min(b, parts - 1)) : res;
+                for (int b = 0; b < MOST; ++b) {
+                    const float* all = MOST > 1 ? cg::this_cluster().map_shared_rank(res, b) : res;
 #pragma unroll
-                for (int w = 0; w < WK; ++w) {
-                    const float* from = all + ((size_t)w * Sh::ROWS + r) * P;
-                    ml[b][w] = *reinterpret_cast<const float2*>(from + HD);
-                    v[b][w] = *reinterpret_cast<const float2*>(from + c);
-                    if (b >= parts) ml[b][w] = make_float2(-INFINITY, 0.f);
+                    for (int w = 0; w < WK; ++w) {
+                        const float* from = all + ((size_t)w * Sh::ROWS + r) * P;
+                        ml[b][w] = *reinterpret_cast<const float2*>(from + HD);
+                        v[b][w] = *reinterpret_cast<const float2*>(from + c);
+                    }
+                }
+                float top = -INFINITY, l = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+                for (int b = 0; b < MOST; ++b)
+#pragma unroll
+                    for (int w = 0; w < WK; ++w) top = fmaxf(top, ml[b][w].x);
+                const float o = top == -INFINITY ? 0.f : top;
+#pragma unroll
+                for (int b = 0; b < MOST; ++b)
+#pragma unroll
+                    for (int w = 0; w < WK; ++w) {
+                        const float f = tm_exp2(ml[b][w].x - o);
+                        l = fmaf(ml[b][w].y, f, l);
+                        x = fmaf(v[b][w].x, f, x);
+                        y = fmaf(v[b][w].y, f, y);
+                    }
+                if (CLUSTER || tile1 - tile0 == tiles_all) {
+                    const float inv = l != 0.f ? 1.0f / l : 0.f;
+                    *reinterpret_cast<uint32_t*>(out + (size_t)(s.row0 + m / G) * a.out_stride + (kvh * G + m % G) * HD + c) = tm_pack(x * inv, y * inv);
+                } else {
+                    float* part = a.parts + ((size_t)piece * Sh::ROWS + r) * P;
+                    *reinterpret_cast<float2*>(part + c) = make_float2(x, y);
+                    if (c == 0) *reinterpret_cast<float2*>(part + HD) = make_float2(top, l);
                 }
             }
-            float top = -INFINITY, l = 0.f, x = 0.f, y = 0.f;
-#pragma unroll
-            for (int b = 0; b < MOST; ++b)
-#pragma unroll
-                for (int w = 0; w < WK; ++w) top = fmaxf(top, ml[b][w].x);
-            const float o = top == -INFINITY ? 0.f : top;
-#pragma unroll
-            for (int b = 0; b < MOST; ++b)
-#pragma unroll
-                for (int w = 0; w < WK; ++w) {
-                    const float f = tm_exp2(ml[b][w].x - o);
-                    l = fmaf(ml[b][w].y, f, l);
-                    x = fmaf(v[b][w].x, f, x);
-                    y = fmaf(v[b][w].y, f, y);
-                }
-            if (CLUSTER || tile1 - tile0 == tiles_all) {
-                const float inv = l != 0.f ? 1.0f / l : 0.f;
-                *reinterpret_cast<uint32_t*>(out + (size_t)(s.row0 + m / G) * a.out_stride + (kvh * G + m % G) * HD + c) = tm_pack(x * inv, y * inv);
-            } else {
-                float* part = a.parts + ((size_t)piece * Sh::ROWS + r) * P;
-                *reinterpret_cast<float2*>(part + c) = make_float2(x, y);
-                if (c == 0) *reinterpret_cast<float2*>(part + HD) = make_float2(top, l);
-            }
-        }
+        };
+        if (!CLUSTER || parts == 1) add_up(std::integral_constant<int, 1>());
+        else if (parts == 2) add_up(std::integral_constant<int, 2>());
+        else if (parts == 4) add_up(std::integral_constant<int, 4>());
+        else add_up(std::integral_constant<int, TM_MAX_CLUSTER>());
         if (CLUSTER && parts > 1) cg::this_cluster().sync();      // (shared memory is read until here)
     };
     auto zeros = [&](const TreeSeq& s) {              // a padding request's rows

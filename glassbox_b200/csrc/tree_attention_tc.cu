@@ -33,7 +33,7 @@ struct __align__(16) Tc5Shared {
     uint64_t q_full;                      // softmax -> MMA: the queries of a piece lie in shared memory (and O of the one before has been read)
     uint64_t k_full[6], v_full[6], k_free[6], v_free[6];
     uint64_t s_full[2], p_most[2], p_ready[2], pv_done[2];
-    long long at, end;                    // tiles of all items: the block's next, and the end of its share
+    long long at;                         // the tile of all items behind those of the list
     uint32_t tmem_base;
     int abort_flag, segs;                 // (segs: negative where the share ends with them)
     int issued[2], consumed[2];
@@ -83,13 +83,34 @@ __global__ void __launch_bounds__(TC5_WARPS * 32) tree_attention_tc_kernel(const
         if (tid == 0) atomicOr(a.status, GB_STATUS_WAIT_TIMEOUT);
         return;
     }
-    {
-        const TreeCut cut(a, num_seqs, ROWS, TC5_KEYS, gridDim.x, TREE_LEAST_SHARE, true);
-        const long long at = min(cut.total, blockIdx.x * cut.share), end = min(cut.total, at + cut.share);
-        if (at >= end) return;                    // uniform for the block, before anything is allocated
-        if (tid == 0) { sh.at = at; sh.end = end; }
-    }
-    if (tid == 0) {
+    // The next pieces of the block's share, up to TC5_SEGS, from tile `at` on (all of warp 0); count 0: there are none.
+    auto list = [&](bool begin) {
+        TreeCut cut(a, num_seqs, ROWS, TC5_KEYS, gridDim.x, TREE_LEAST_SHARE, true);
+        const long long end = min(cut.total, (blockIdx.x + 1) * cut.share);
+        long long at = begin ? min(cut.total, blockIdx.x * cut.share) : sh.at;
+        int count = 0;
+        if (at < end) cut.seek(at);
+        for (; at < end && count < TC5_SEGS; ++count) {
+            const TreeSeq s(a, cut.seq);
+            const int all = s.start / TC5_KEYS;
+            const long long off = at - cut.tile0;
+            const int item = (int)(off / all), tile0 = (int)(off - (long long)item * all), tiles = (int)min((long long)all - tile0, end - at);
+            if (lane == 0) {
+                sh.seg[count] = make_int4(cut.seq, item, tile0, tiles);
+                sh.piece[count] = (int)(cut.item0 + item + blockIdx.x);
+            }
+            at += tiles;
+            if (at < end) cut.reach(at);
+        }
+        __syncwarp();
+        if (lane == 0) { sh.segs = at < end ? count : -count; sh.at = at; }
+    };
+    if (warp == 0) {
+        list(true);
+    } else if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem_base)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    } else if (tid == 64) {
         mbar_init(&sh.q_full, 8);
         for (int b = 0; b < SK; ++b) { mbar_init(&sh.k_full[b], 1); mbar_init(&sh.k_free[b], 1); }
         for (int b = 0; b < SV; ++b) { mbar_init(&sh.v_full[b], 1); mbar_init(&sh.v_free[b], 1); }
@@ -103,10 +124,6 @@ __global__ void __launch_bounds__(TC5_WARPS * 32) tree_attention_tc_kernel(const
         sh.issued[0] = sh.issued[1] = sh.consumed[0] = sh.consumed[1] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 0) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem_base)) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -118,29 +135,6 @@ __global__ void __launch_bounds__(TC5_WARPS * 32) tree_attention_tc_kernel(const
     int pieces_done = 0, steps = 0, steps1 = 0;   // the issuer and the softmax: pieces, and their unit's tiles (the issuer: unit 0's and unit 1's)
     bool ok = true;
     while (true) {
-        // ------------------------------------------------------------------------- the next pieces, up to TC5_SEGS
-        if (warp == 0) {
-            int count = 0;
-            long long at = sh.at;
-            const long long end = sh.end;
-            TreeCut cut(a, num_seqs, ROWS, TC5_KEYS, gridDim.x, TREE_LEAST_SHARE, true);
-            cut.seek(at);
-            for (; at < end && count < TC5_SEGS; ++count) {
-                const TreeSeq s(a, cut.seq);
-                const int all = s.start / TC5_KEYS;
-                const long long off = at - cut.tile0;
-                const int item = (int)(off / all), tile0 = (int)(off % all), tiles = (int)min((long long)all - tile0, end - at);
-                if (lane == 0) {
-                    sh.seg[count] = make_int4(cut.seq, item, tile0, tiles);
-                    sh.piece[count] = (int)(cut.item0 + item + blockIdx.x);
-                }
-                at += tiles;
-                if (at < end) cut.reach(at);
-            }
-            __syncwarp();
-            if (lane == 0) { sh.segs = at < end ? count : -count; sh.at = at; }
-        }
-        __syncthreads();
         const bool more = sh.segs > 0;
         const int segs = abs(sh.segs);
 
@@ -359,26 +353,30 @@ __global__ void __launch_bounds__(TC5_WARPS * 32) tree_attention_tc_kernel(const
                 if (ok && mine > 0) ok = mbar_wait_warp(&sh.pv_done[g], (steps - 1) & 1, abort_flag, a.status);
                 if (!ok) continue;
                 tc_fence_after();
-                // O, maximum (base 2) and sum to the scratch
-                float* to = a.parts + ((size_t)sh.piece[i] * 2 + g) * TC5_M * P + (size_t)r * P;
+                // O, maximum (base 2) and sum to the scratch, 32 rows side by side
+                float* to = a.parts + ((size_t)sh.piece[i] * 2 + g) * (TC5_M * P) + (size_t)q * (32 * P) + lane;
 #pragma unroll
                 for (int c = 0; c < HD; c += 32) {
                     uint32_t ov[32];
                     if (mine > 0) tmem_load32(lane_base + o_col + (uint32_t)c, ov);
 #pragma unroll
-                    for (int k = 0; k < 32; k += 2) *reinterpret_cast<float2*>(to + c + k) = mine > 0 ? make_float2(__uint_as_float(ov[k]), __uint_as_float(ov[k + 1])) : make_float2(0.f, 0.f);
+                    for (int k = 0; k < 32; ++k) to[(c + k) * 32] = mine > 0 ? __uint_as_float(ov[k]) : 0.f;
                 }
-                *reinterpret_cast<float2*>(to + HD) = mine > 0 ? make_float2(m_run, l_run) : make_float2(-INFINITY, 0.f);
+                to[HD * 32] = mine > 0 ? m_run : -INFINITY;
+                to[HD * 32 + 32] = l_run;
             }
         }
+        if (!more) break;
         __syncthreads();                          // (the list has been read)
-        if (*abort_flag || !more) break;
+        if (*abort_flag) break;
+        if (warp == 0) list(false);
+        __syncthreads();
     }
 
     // ------------------------------------------------------------------------------- wind down
     tc_fence_before();
     __syncthreads();
-    if (warp == 0) {
+    if (warp == 1) {
         if (lane == 0 && sh.abort_flag) {
             // copies that were issued but never consumed may still be in flight: wait for them (bounded)
             for (int what = 0; what < 2; ++what)
