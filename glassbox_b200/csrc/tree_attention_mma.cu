@@ -72,7 +72,7 @@ struct TmShape {
 // CLUSTER: the blocks of a cluster share one item's keys (blockIdx.x of gridDim.x of them; item: blockIdx.y, request: blockIdx.z) and add up through distributed
 // shared memory. Otherwise all items' tiles of keys are cut evenly among the blocks; what a block finds of an item that it shares with others goes to the
 // scratch, piece number (item + block), and tree_pieces_kernel adds up. TAIL: a block an item, the keys behind the whole tiles that tree_attention_tc.cu takes in
-// `tc_blocks` blocks, whose pieces (in units of 128 rows, two a piece) are added to them.
+// `tc_blocks` blocks, whose pieces (in units of 128 rows, `tc_same`: one a piece, else two) are added to them.
 enum TmMode { TM_EVEN, TM_CLUSTER, TM_TAIL };
 
 template <int HD, int WM, int WK, TmMode MODE>
@@ -365,14 +365,14 @@ __global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const _
                 const long long t0 = cut.tile0 + (long long)item * all;
                 b0 = t0 / cut.share;
                 b1 = (t0 + all - 1) / cut.share;
-                pieces = a.parts + (size_t)(cut.item0 + item + b0) * (2 * TREE_TC_ROWS * P);
+                pieces = a.parts + (size_t)(cut.item0 + item + b0) * ((tc_same ? 1 : 2) * TREE_TC_ROWS * P);
             }
         }
         if constexpr (MODE == TM_TAIL) {
             // The pieces' rows (both units where they have the same rows, else the one that has the row) and the warps' own: first every row's maximum and sum over
             // all of them, then their channels in fours, several sources' loads under way at once.
-            const int each = tc_same ? 2 : 1, count = (int)(b1 - b0 + 1) * each, step = tc_same ? TREE_TC_ROWS * P : 2 * TREE_TC_ROWS * P;
-            // The rows' place in the pieces: [units of 128 rows][blocks of 32][channels, maximum, sum][32 rows]. (Rows behind the request's last hold numbers that
+            const int count = (int)(b1 - b0 + 1), step = (tc_same ? 1 : 2) * TREE_TC_ROWS * P;
+            // The rows' place in a piece: [units of 128 rows][blocks of 32][channels, maximum, sum][32 rows]. (Rows behind the request's last hold numbers that
             // are not written out.)
             const float* mine = pieces + (tc_same ? 0 : m0 % tc_rows / TREE_TC_ROWS) * (TREE_TC_ROWS * P);
             auto row_at = [&](int r) -> const float* { return mine + (m0 + r) % TREE_TC_ROWS / 32 * (32 * P) + (m0 + r) % 32; };
@@ -688,7 +688,7 @@ TreePlan tree_plan_mma(int num_seqs, int max_rows, int nh, int nkv, int hd, int 
         p.same = M <= TREE_TC_ROWS;
         p.blocks = 148;
         p.rows = (long long)num_seqs * nkv * gb_ceil_div(M, 16) <= 4 * 148 ? 16 : 64;
-        p.floats = ((long long)num_seqs * nkv * gb_ceil_div(M, p.same ? TREE_TC_ROWS : 2 * TREE_TC_ROWS) + p.blocks) * 2 * TREE_TC_ROWS * (hd + 2);
+        p.floats = ((long long)num_seqs * nkv * gb_ceil_div(M, p.same ? TREE_TC_ROWS : 2 * TREE_TC_ROWS) + p.blocks) * (p.same ? 1 : 2) * TREE_TC_ROWS * (hd + 2);
         return p;
     }
     p.rows = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;

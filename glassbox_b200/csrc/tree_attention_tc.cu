@@ -15,7 +15,7 @@
 #include "tcgen05.cuh"
 #include "tree_attention.cuh"
 
-constexpr int TC5_M = 128, TC5_KEYS = 128, TC5_WARPS = 11, TC5_SEGS = 64;
+constexpr int TC5_M = 128, TC5_KEYS = 128, TC5_WARPS = 11, TC5_SEGS = 32;
 constexpr int TC5_BLOCK = 128 * 128;      // bytes of 128 rows of 64 channels
 constexpr float TC5_NEG_BIG = -1.0e30f;
 
@@ -30,6 +30,7 @@ struct Tc5Shape {
 struct __align__(16) Tc5Shared {
     int4 seg[TC5_SEGS];                   // request, item of the request, first tile, tiles
     int piece[TC5_SEGS];
+    float2 stat[2][TC5_M];                // (SAME) of a unit's row: maximum, sum
     uint64_t q_full;                      // softmax -> MMA: the queries of a piece lie in shared memory (and O of the one before has been read)
     uint64_t k_full[6], v_full[6], k_free[6], v_free[6];
     uint64_t s_full[2], p_most[2], p_ready[2], pv_done[2];
@@ -38,7 +39,7 @@ struct __align__(16) Tc5Shared {
     int abort_flag, segs;                 // (segs: negative where the share ends with them)
     int issued[2], consumed[2];
 };
-static_assert(sizeof(Tc5Shared) <= 2048, "shared memory layout");
+static_assert(sizeof(Tc5Shared) <= 3072, "shared memory layout");
 
 __device__ __forceinline__ uint64_t tc5_desc_mn(uint32_t smem_addr) {      // MN-major B operand: column blocks of 64 channels TC5_BLOCK bytes apart
     uint64_t d = 0;
@@ -266,7 +267,10 @@ __global__ void __launch_bounds__(TC5_WARPS * 32) tree_attention_tc_kernel(const
                 int mine, units = 2;                      // tiles of this unit
                 // both units are done with the piece before (every warp comes here for every piece, also one that has given up)
                 asm volatile("barrier.cta.sync 1, 256;" ::: "memory");
-                if (!ok) continue;
+                if (!ok) {
+                    if constexpr (SAME) asm volatile("barrier.cta.sync 2, 256;" ::: "memory");
+                    continue;
+                }
                 {
                     const TreeSeq s(a, seg.x);
                     const int M = s.rows * G, pairs = (M + ROWS - 1) / ROWS, m = seg.y % pairs * ROWS + (SAME ? 0 : g * TC5_M) + r;
@@ -351,10 +355,42 @@ __global__ void __launch_bounds__(TC5_WARPS * 32) tree_attention_tc_kernel(const
                     ++steps;
                 }
                 if (ok && mine > 0) ok = mbar_wait_warp(&sh.pv_done[g], (steps - 1) & 1, abort_flag, a.status);
+                if constexpr (SAME) {
+                    // The two units' parts of a row: each thread adds up half of the row's channels of both, whose columns all warps of the row's lanes can read.
+                    // (Every warp meets this barrier for every piece, too.)
+                    sh.stat[g][r] = mine > 0 ? make_float2(m_run, l_run) : make_float2(-INFINITY, 0.f);
+                    tc_fence_before();
+                    asm volatile("barrier.cta.sync 2, 256;" ::: "memory");
+                    tc_fence_after();
+                    const float2 other = sh.stat[g ^ 1][r];
+                    const float top = fmaxf(mine > 0 ? m_run : -INFINITY, other.x);      // (unit 0 has a tile always)
+                    const float f = mine > 0 ? tc5_exp2(m_run - top) : 0.f, f_other = tc5_exp2(other.x - top);
+                    const bool both = seg.w > 1;
+                    if (!__any_sync(0xffffffffu, *abort_flag)) {
+                        float* to = a.parts + (size_t)sh.piece[i] * (TC5_M * P) + (size_t)q * (32 * P) + lane;
+#pragma unroll
+                        for (int c = g * (HD / 2); c < HD; c += 16) {
+                            if (c >= (g + 1) * (HD / 2)) break;
+                            uint32_t o0[16], o1[16];
+                            tmem_load16(lane_base + (uint32_t)(Sh::O_COL + c), o0);
+                            if (both) tmem_load16(lane_base + (uint32_t)(Sh::O_COL + HD + c), o1);
+                            const float f0 = g ? f_other : f, f1 = g ? f : f_other;
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) to[(c + k) * 32] = both ? fmaf(__uint_as_float(o1[k]), f1, __uint_as_float(o0[k]) * f0) : __uint_as_float(o0[k]);
+                        }
+                        if (g == 0) {
+                            to[HD * 32] = top;
+                            to[HD * 32 + 32] = fmaf(other.y, f_other, l_run * f);
+                        }
+                    } else {
+                        ok = false;
+                    }
+                    continue;
+                }
                 if (!ok) continue;
                 tc_fence_after();
                 // O, maximum (base 2) and sum to the scratch, 32 rows side by side
-                float* to = a.parts + ((size_t)sh.piece[i] * 2 + g) * (TC5_M * P) + (size_t)q * (32 * P) + lane;
+                float* to = a.parts + ((size_t)sh.piece[i] * (SAME ? 1 : 2) + g) * (TC5_M * P) + (size_t)q * (32 * P) + lane;
 #pragma unroll
                 for (int c = 0; c < HD; c += 32) {
                     uint32_t ov[32];
