@@ -207,7 +207,8 @@ static int ta_dispatch(const TreeArgs& a, int num_seqs, int max_rows, cudaStream
     return rc ? rc : gb_check_launch("gb_tree_attention");
 }
 
-// tree_attention_mma.cu
+// tree_attention_mma.cu, tree_attention_tc.cu
+int gb_tree_attention_tc(const TreeArgs& a, const TreePlan& plan, int num_seqs, int max_rows, cudaStream_t stream);
 int gb_tree_attention_mma(const TreeArgs& a, const TreePlan& plan, int num_seqs, int max_rows, cudaStream_t stream);
 TreePlan tree_plan_mma(int num_seqs, int max_rows, int nh, int nkv, int hd, int max_context, int window, bool tc);
 
@@ -232,7 +233,7 @@ GB_EXPORT int gb_tree_attention_floats(int kind, int n, int num_seqs, int max_ro
     return floats < (1ll << 31) ? (int)floats : -1;
 }
 
-// kind 0: this file's kernel; 1: the tensor cores (bfloat16); 2: tcgen05, too, for keys before the tree (scale above 0, pages of 8 to 128, rows of q at 16 bytes). q, out: [n, nh * hd], rows `stride` numbers apart; kcache, vcache: [num_pages, nkv, page_size, hd];
+// kind 0: this file's kernel; 1: the tensor cores (bfloat16); 2: tcgen05 where there is enough for it (scale above 0, pages of 8 to 128, rows of q and out at 16 bytes). q, out: [n, nh * hd], rows `stride` numbers apart; kcache, vcache: [num_pages, nkv, page_size, hd];
 // parts: gb_tree_attention_floats of the same sizes.
 GB_EXPORT int gb_tree_attention(int kind, const void* q, long long q_stride, void* out, long long out_stride, int dtype, const void* kcache, const void* vcache,
                                 const int* block_tables, int max_pages, const int* first_row, const int* start_pos, const int* positions, const int* visible,
@@ -248,12 +249,12 @@ GB_EXPORT int gb_tree_attention(int kind, const void* q, long long q_stride, voi
     TreeArgs a = {q, q_stride, out, out_stride, kcache, vcache, block_tables, max_pages, first_row, start_pos, positions, visible, words, n, nh, nkv, hd, page_size,
                   num_pages, scale, window, 1, parts, status};
     if (kind >= 1) {
-        GB_REQUIRE(kind == 1 || (scale > 0.f && page_size >= 8 && page_size <= TREE_TC_KEYS && (uintptr_t)q % 16 == 0 && q_stride % 8 == 0),
+        GB_REQUIRE(kind == 1 || (scale > 0.f && page_size >= 8 && page_size <= TREE_TC_KEYS && (uintptr_t)q % 16 == 0 && q_stride % 8 == 0 && (uintptr_t)out % 16 == 0 && out_stride % 8 == 0),
                    "gb_tree_attention: this scale, page size or alignment is not built for tcgen05");
         GB_REQUIRE(dtype == GB_BF16, "gb_tree_attention: the tensor cores' kernel takes bfloat16");
         const TreePlan plan = tree_plan_mma(num_seqs, max_rows, nh, nkv, hd, max_context, window, kind == 2);
         GB_REQUIRE(plan.floats == 0 || (parts != nullptr && (uintptr_t)parts % 16 == 0), "gb_tree_attention: the scratch is missing or not 16-byte aligned");
-        return gb_tree_attention_mma(a, plan, num_seqs, max_rows, stream);
+        return plan.tc ? gb_tree_attention_tc(a, plan, num_seqs, max_rows, stream) : gb_tree_attention_mma(a, plan, num_seqs, max_rows, stream);
     }
     a.splits = ta_splits(num_seqs, max_rows, nh, nkv, max_context, window);
     GB_REQUIRE(a.splits == 1 || parts != nullptr, "gb_tree_attention: the scratch is missing");

@@ -35,7 +35,7 @@ struct TreePlan {
     int rows = 0;            // query rows of an item
     int cluster = 0;         // blocks that share an item's keys, a cluster; 0: all items' keys are cut evenly among `blocks`
     int blocks = 0;
-    bool tc = false;         // whole tiles before the trees by tree_attention_tc.cu, `blocks` of it; items of what is left have `rows` query rows
+    bool tc = false;         // by tree_attention_tc.cu, in `blocks` blocks
     bool same = false;       // its items have at most 128 query rows
     long long floats = 0;    // of scratch
 };
@@ -73,6 +73,30 @@ struct TreeSeq {
     }
 };
 
+// Of the 32 rows of the tree from d0 on (negative: keys before the tree, all seen), those that a row of the batch sees. `only`: its
+// bits, where they are one word.
+__device__ __forceinline__ unsigned tree_bits(const TreeArgs& a, int rows, int row, int d0, unsigned only) {
+    if (d0 <= -32) return 0xffffffffu;
+    if (row < 0) return 0u;
+    const unsigned* bits = reinterpret_cast<const unsigned*>(a.visible) + (size_t)row * a.words;
+    unsigned v;
+    if (d0 < 0) {
+        v = ((1u << -d0) - 1u) | ((a.words == 1 ? only : bits[0]) << -d0);
+    } else if (a.words == 1) {
+        v = d0 < 32 ? only >> d0 : 0u;
+    } else {
+        const int w = d0 >> 5, sh = d0 & 31;
+        v = w < a.words ? bits[w] >> sh : 0u;
+        if (sh && w + 1 < a.words) v |= bits[w + 1] << (32 - sh);
+    }
+    const int left = rows - d0;
+    return left >= 32 ? v : left <= 0 ? 0u : v & ((1u << left) - 1u);
+}
+
+__device__ __forceinline__ unsigned tree_bits(const TreeArgs& a, int rows, int row, int d0) {
+    return tree_bits(a, rows, row, d0, row >= 0 && a.words == 1 && d0 > -32 ? (unsigned)a.visible[row] : 0u);
+}
+
 constexpr int TREE_TC_KEYS = 128, TREE_TC_ROWS = 128;      // keys of a tile and rows of a unit of tree_attention_tc.cu
 constexpr int TREE_LEAST_SHARE = 4;      // tiles of keys of a block, where there are enough
 
@@ -81,7 +105,6 @@ constexpr int TREE_LEAST_SHARE = 4;      // tiles of keys of a block, where ther
 struct TreeCut {
     const TreeArgs& a;
     int num_seqs, rows, keys;
-    bool before;             // only whole tiles before the trees
     long long total, share;
     int seq;                 // a request, the tiles and items before it
     long long tile0, item0, tiles_here;
@@ -92,7 +115,7 @@ struct TreeCut {
         if (n <= 0 || start < 0 || a.first_row[s] < 0 || a.first_row[s] > a.n - n) return;
         const int low = a.window > 0 ? max(0, start - a.window + 1) : 0;
         items = (long long)a.nkv * ((n * (a.nh / a.nkv) + rows - 1) / rows);
-        tiles = items * (before ? start / keys : (start + n + keys - 1) / keys - low / keys);
+        tiles = items * ((start + n + keys - 1) / keys - low / keys);
     }
     __device__ __forceinline__ static long long scan(long long v) {
         const int lane = threadIdx.x & 31;
@@ -103,8 +126,8 @@ struct TreeCut {
         }
         return v;
     }
-    __device__ __forceinline__ TreeCut(const TreeArgs& a, int num_seqs, int rows, int keys, int blocks, int least, bool before = false)
-        : a(a), num_seqs(num_seqs), rows(rows), keys(keys), before(before) {
+    __device__ __forceinline__ TreeCut(const TreeArgs& a, int num_seqs, int rows, int keys, int blocks, int least)
+        : a(a), num_seqs(num_seqs), rows(rows), keys(keys) {
         long long sum = 0;
         for (int s0 = 0; s0 < num_seqs; s0 += 32) {
             long long t, i;

@@ -40,25 +40,6 @@ __device__ __forceinline__ uint32_t tm_pack(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// Of the 32 rows of the tree from d0 on (negative: keys before the tree, all seen), those that a row of the batch sees. `only`: its bits, where they are one word.
-__device__ __forceinline__ unsigned tm_bits(const TreeArgs& a, int rows, int row, unsigned only, int d0) {
-    if (d0 <= -32) return 0xffffffffu;
-    if (row < 0) return 0u;
-    const unsigned* bits = reinterpret_cast<const unsigned*>(a.visible) + (size_t)row * a.words;
-    unsigned v;
-    if (d0 < 0) {
-        v = ((1u << -d0) - 1u) | ((a.words == 1 ? only : bits[0]) << -d0);
-    } else if (a.words == 1) {
-        v = d0 < 32 ? only >> d0 : 0u;
-    } else {
-        const int w = d0 >> 5, sh = d0 & 31;
-        v = w < a.words ? bits[w] >> sh : 0u;
-        if (sh && w + 1 < a.words) v |= bits[w + 1] << (32 - sh);
-    }
-    const int left = rows - d0;
-    return left >= 32 ? v : left <= 0 ? 0u : v & ((1u << left) - 1u);
-}
-
 template <int HD, int WM, int WK>
 struct TmShape {
     static constexpr bool TMA = HD % 64 == 0;      // blocks of 64 channels in 128-byte-swizzled rows, else padded rows that threads copy
@@ -71,16 +52,12 @@ struct TmShape {
 
 // CLUSTER: the blocks of a cluster share one item's keys (blockIdx.x of gridDim.x of them; item: blockIdx.y, request: blockIdx.z) and add up through distributed
 // shared memory. Otherwise all items' tiles of keys are cut evenly among the blocks; what a block finds of an item that it shares with others goes to the
-// scratch, piece number (item + block), and tree_pieces_kernel adds up. TAIL: a block an item, the keys behind the whole tiles that tree_attention_tc.cu takes in
-// `tc_blocks` blocks, whose pieces (in units of 128 rows, `tc_same`: one a piece, else two) are added to them.
-enum TmMode { TM_EVEN, TM_CLUSTER, TM_TAIL };
-
-template <int HD, int WM, int WK, TmMode MODE>
+// scratch, piece number (item + block), and tree_pieces_kernel adds up.
+template <int HD, int WM, int WK, bool CLUSTER>
 __global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                                                                         const TreeArgs a, int num_seqs, int tc_blocks, bool tc_same) {
+                                                                         const TreeArgs a, int num_seqs) {
     namespace cg = cooperative_groups;
     using Sh = TmShape<HD, WM, WK>;
-    constexpr bool CLUSTER = MODE == TM_CLUSTER;
     constexpr bool TMA = Sh::TMA;
     constexpr int STAGES = Sh::STAGES, NW = WM * WK;
     // Tiles that are under way beside the one worked on: with TMA one stage less than there are, so that a warp may be a tile behind the one that asks for
@@ -98,9 +75,7 @@ __global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const _
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wm = warp % WM, wk = warp / WM, g = lane >> 2, t = lane & 3;
     const int G = a.nh / a.nkv;
     gb_pdl_launch_dependents();
-    // (the kernel before a tail is tree_attention_tc.cu's, which lets this one start once it has waited for all before it: its pieces alone are waited for, where
-    // they are read)
-    if constexpr (MODE != TM_TAIL) gb_pdl_wait();
+    gb_pdl_wait();
     __nv_bfloat16* out = (__nv_bfloat16*)a.out;
     const __nv_bfloat16* kc = (const __nv_bfloat16*)a.kcache;
     const __nv_bfloat16* vc = (const __nv_bfloat16*)a.vcache;
@@ -245,7 +220,7 @@ __global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const _
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int w = 0; w < (KW + 31) / 32; ++w) see[h][w] = tm_bits(a, s.rows, row[h], word[h], k0 + 32 * w - s.start);
+                    for (int w = 0; w < (KW + 31) / 32; ++w) see[h][w] = tree_bits(a, s.rows, row[h], k0 + 32 * w - s.start, word[h]);
 #pragma unroll
                 for (int j = 0; j < KT; ++j)
 #pragma unroll
@@ -352,111 +327,6 @@ __global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const _
             for (int j = 0; j < NT; ++j) *reinterpret_cast<float2*>(to + 8 * j + 2 * t) = make_float2(acc[j][2 * h], acc[j][2 * h + 1]);
             if (t == 0) *reinterpret_cast<float2*>(to + HD) = make_float2(m_run[h], l_run[h]);
         }
-        long long b0 = 0, b1 = -1;                    // the blocks that have pieces of the item, and the first of them
-        const float* pieces = nullptr;
-        const int tc_rows = tc_same ? TREE_TC_ROWS : 2 * TREE_TC_ROWS;
-        if constexpr (MODE == TM_TAIL) {
-            gb_pdl_wait();
-            const int all = s.start / TREE_TC_KEYS;
-            if (all > 0) {
-                TreeCut cut(a, num_seqs, tc_rows, TREE_TC_KEYS, tc_blocks, TREE_LEAST_SHARE, true);
-                cut.seek_seq(blockIdx.z);
-                const int item = kvh * ((M + tc_rows - 1) / tc_rows) + m0 / tc_rows;
-                const long long t0 = cut.tile0 + (long long)item * all;
-                b0 = t0 / cut.share;
-                b1 = (t0 + all - 1) / cut.share;
-                pieces = a.parts + (size_t)(cut.item0 + item + b0) * ((tc_same ? 1 : 2) * TREE_TC_ROWS * P);
-            }
-        }
-        if constexpr (MODE == TM_TAIL) {
-            // The pieces' rows (both units where they have the same rows, else the one that has the row) and the warps' own: first every row's maximum and sum over
-            // all of them, then their channels in fours, several sources' loads under way at once.
-            const int count = (int)(b1 - b0 + 1), step = (tc_same ? 1 : 2) * TREE_TC_ROWS * P;
-            // The rows' place in a piece: [units of 128 rows][blocks of 32][channels, maximum, sum][32 rows]. (Rows behind the request's last hold numbers that
-            // are not written out.)
-            const float* mine = pieces + (tc_same ? 0 : m0 % tc_rows / TREE_TC_ROWS) * (TREE_TC_ROWS * P);
-            auto row_at = [&](int r) -> const float* { return mine + (m0 + r) % TREE_TC_ROWS / 32 * (32 * P) + (m0 + r) % 32; };
-            float2* stats = reinterpret_cast<float2*>(pages);      // of a row: maximum, 1 / sum
-            __syncthreads();
-            constexpr int LANES = Sh::THREADS / Sh::ROWS;      // threads of a row: 8 or 2
-            {
-                const int r = tid / LANES;
-                float top = -INFINITY, l = 0.f;
-                auto add = [&](float2 ml) {
-                    const float up = fmaxf(top, ml.x), o = up == -INFINITY ? 0.f : up;
-                    l = l * tm_exp2(top - o) + ml.y * tm_exp2(ml.x - o);
-                    top = up;
-                };
-                if (tid % LANES == 0)
-#pragma unroll
-                    for (int w = 0; w < WK; ++w) add(*reinterpret_cast<const float2*>(res + ((size_t)w * Sh::ROWS + r) * P + HD));
-                const float* from = row_at(r) + HD * 32;
-                for (int b = tid % LANES; b < count; b += 8 * LANES) {
-                    float2 ml[8];
-#pragma unroll
-                    for (int u = 0; u < 8; ++u) {
-                        const float* at = from + (size_t)min(b + u * LANES, count - 1) * step;
-                        ml[u] = make_float2(at[0], at[32]);
-                    }
-#pragma unroll
-                    for (int u = 0; u < 8; ++u)
-                        if (b + u * LANES < count) add(ml[u]);
-                }
-                float most = top;
-#pragma unroll
-                for (int o = 1; o < LANES; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-                const float o = most == -INFINITY ? 0.f : most;
-                l *= tm_exp2(top - o);
-#pragma unroll
-                for (int k = 1; k < LANES; k <<= 1) l += __shfl_xor_sync(0xffffffffu, l, k);
-                if (tid % LANES == 0) stats[r] = make_float2(o, l != 0.f ? 1.0f / l : 0.f);
-            }
-            __syncthreads();
-            // A thread has four rows of a channel, a warp 16 rows of eight; several sources' loads are under way at once. The sums go where the warps' own results
-            // were, whose channel nobody else reads.
-            constexpr int BATCH = 8, QUADS = Sh::ROWS / 4;
-            for (int i = tid; i < QUADS * HD; i += Sh::THREADS) {
-                const int r = i % 4 * 4 + i / (4 * HD) * 16, c = i / 4 % HD;
-                float top[4], inv[4], sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    top[k] = stats[r + k].x;
-                    inv[k] = stats[r + k].y;
-#pragma unroll
-                    for (int w = 0; w < WK; ++w) {
-                        const float* own = res + ((size_t)w * Sh::ROWS + r + k) * P;
-                        sum[k] = fmaf(own[c], tm_exp2(own[HD] - top[k]), sum[k]);
-                    }
-                }
-                const float* from = row_at(r);
-                for (int b = 0; b < count; b += BATCH) {
-                    float4 v[BATCH], m[BATCH];
-#pragma unroll
-                    for (int u = 0; u < BATCH; ++u) {
-                        const float* at = from + (size_t)min(b + u, count - 1) * step;
-                        v[u] = *reinterpret_cast<const float4*>(at + c * 32);
-                        m[u] = *reinterpret_cast<const float4*>(at + HD * 32);
-                    }
-#pragma unroll
-                    for (int u = 0; u < BATCH; ++u)
-                        if (b + u < count) {
-                            sum[0] = fmaf(v[u].x, tm_exp2(m[u].x - top[0]), sum[0]);
-                            sum[1] = fmaf(v[u].y, tm_exp2(m[u].y - top[1]), sum[1]);
-                            sum[2] = fmaf(v[u].z, tm_exp2(m[u].z - top[2]), sum[2]);
-                            sum[3] = fmaf(v[u].w, tm_exp2(m[u].w - top[3]), sum[3]);
-                        }
-                }
-#pragma unroll
-                for (int k = 0; k < 4; ++k) res[(size_t)(r + k) * P + c] = sum[k] * inv[k];
-            }
-            __syncthreads();
-            for (int i = tid; i < Sh::ROWS * (HD / 2); i += Sh::THREADS) {
-                const int r = i / (HD / 2), c = i % (HD / 2) * 2, m = m0 + r;
-                if (m >= M) break;
-                *reinterpret_cast<uint32_t*>(out + (size_t)(s.row0 + m / G) * a.out_stride + (kvh * G + m % G) * HD + c) = tm_pack(res[(size_t)r * P + c], res[(size_t)r * P + c + 1]);
-            }
-            return;
-        }
         const int parts = CLUSTER ? gridDim.x : 1, rank = CLUSTER ? blockIdx.x : 0;
         if (CLUSTER && parts > 1) cg::this_cluster().sync(); else __syncthreads();
         // A pair of channels of every parts-th row; all loads of other blocks' results come first: one trip.
@@ -521,15 +391,6 @@ __global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const _
         }
         const int all = s.tiles(TM_KEYS), share = (all + gridDim.x - 1) / gridDim.x, tile0 = min(all, (int)blockIdx.x * share);
         work(s, blockIdx.y % a.nkv, m0, tile0, min(all, tile0 + share), all, 0);
-    } else if constexpr (MODE == TM_TAIL) {
-        const TreeSeq s(a, blockIdx.z);
-        const int m0 = blockIdx.y / a.nkv * Sh::ROWS;
-        if (s.start < 0 || m0 >= s.rows * G) {
-            gb_pdl_wait();
-            if (s.start < 0 && blockIdx.y == 0) zeros(s);
-            return;
-        }
-        work(s, blockIdx.y % a.nkv, m0, s.start / TREE_TC_KEYS * (TREE_TC_KEYS / TM_KEYS), s.tiles(TM_KEYS), s.tiles(TM_KEYS), 0);
     } else {
         TreeCut cut(a, num_seqs, Sh::ROWS, TM_KEYS, gridDim.x, TREE_LEAST_SHARE);
         long long at = min(cut.total, blockIdx.x * cut.share);
@@ -593,8 +454,6 @@ __global__ void __launch_bounds__(128) tree_pieces_kernel(const TreeArgs a, int 
     }
 }
 
-int gb_tree_attention_tc(const TreeArgs& a, const TreePlan& plan, int num_seqs, cudaStream_t stream);      // tree_attention_tc.cu
-
 template <int HD, int WM, int WK>
 static int tm_launch(const TreeArgs& a, const TreePlan& plan, int num_seqs, int max_rows, cudaStream_t stream) {
     using Sh = TmShape<HD, WM, WK>;
@@ -607,19 +466,8 @@ static int tm_launch(const TreeArgs& a, const TreePlan& plan, int num_seqs, int 
     const int m_tiles = gb_ceil_div((long long)max_rows * (a.nh / a.nkv), Sh::ROWS);
     GB_REQUIRE((long long)m_tiles * a.nkv * (Sh::ROWS / 8) <= 65535ll * 1024 && (long long)m_tiles * a.nkv <= 65535, "gb_tree_attention: %d rows a request are too many for one launch", max_rows);
     cudaError_t e;
-    if constexpr ((HD == 64 || HD == 128) && ((WM == 1 && WK == 4) || (WM == 4 && WK == 1)))
-        if (plan.tc) {
-            if (gb_tree_attention_tc(a, plan, num_seqs, stream)) return 1;
-            const auto kernel = tree_attention_mma_kernel<HD, WM, WK, TM_TAIL>;
-            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM);
-            GB_REQUIRE(e == cudaSuccess, "gb_tree_attention: %d bytes of shared memory refused: %s", Sh::SMEM, cudaGetErrorString(e));
-            e = gb_launch(GB_PDL_ATTENTION, kernel, dim3(1, m_tiles * a.nkv, num_seqs), dim3(Sh::THREADS), Sh::SMEM, stream, mk, mv, a, num_seqs, plan.blocks, plan.same);
-            GB_REQUIRE(e == cudaSuccess, "gb_tree_attention: launch failed: %s", cudaGetErrorString(e));
-            return gb_check_launch("gb_tree_attention");
-        }
-    GB_REQUIRE(!plan.tc, "gb_tree_attention: no such plan");
     if (plan.cluster) {
-        const auto kernel = tree_attention_mma_kernel<HD, WM, WK, TM_CLUSTER>;
+        const auto kernel = tree_attention_mma_kernel<HD, WM, WK, true>;
         e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM);
         GB_REQUIRE(e == cudaSuccess, "gb_tree_attention: %d bytes of shared memory refused: %s", Sh::SMEM, cudaGetErrorString(e));
         cudaLaunchConfig_t cfg = {};
@@ -640,14 +488,14 @@ static int tm_launch(const TreeArgs& a, const TreePlan& plan, int num_seqs, int 
         ++na;
         cfg.attrs = attr;
         cfg.numAttrs = na;
-        e = cudaLaunchKernelEx(&cfg, kernel, mk, mv, a, num_seqs, 0, false);
+        e = cudaLaunchKernelEx(&cfg, kernel, mk, mv, a, num_seqs);
         GB_REQUIRE(e == cudaSuccess, "gb_tree_attention: launch failed: %s", cudaGetErrorString(e));
         return gb_check_launch("gb_tree_attention");
     }
-    const auto kernel = tree_attention_mma_kernel<HD, WM, WK, TM_EVEN>;
+    const auto kernel = tree_attention_mma_kernel<HD, WM, WK, false>;
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM);
     GB_REQUIRE(e == cudaSuccess, "gb_tree_attention: %d bytes of shared memory refused: %s", Sh::SMEM, cudaGetErrorString(e));
-    e = gb_launch(GB_PDL_ATTENTION, kernel, dim3(plan.blocks), dim3(Sh::THREADS), Sh::SMEM, stream, mk, mv, a, num_seqs, 0, false);
+    e = gb_launch(GB_PDL_ATTENTION, kernel, dim3(plan.blocks), dim3(Sh::THREADS), Sh::SMEM, stream, mk, mv, a, num_seqs);
     GB_REQUIRE(e == cudaSuccess, "gb_tree_attention: launch failed: %s", cudaGetErrorString(e));
     e = gb_launch(GB_PDL_ATTENTION, tree_pieces_kernel<HD, Sh::ROWS>, dim3(m_tiles * a.nkv * (Sh::ROWS / 8), num_seqs), dim3(128), 0, stream, a, num_seqs, m_tiles, plan.blocks);
     GB_REQUIRE(e == cudaSuccess, "gb_tree_attention: launch failed: %s", cudaGetErrorString(e));
@@ -687,7 +535,6 @@ TreePlan tree_plan_mma(int num_seqs, int max_rows, int nh, int nkv, int hd, int 
         p.tc = true;
         p.same = M <= TREE_TC_ROWS;
         p.blocks = 148;
-        p.rows = (long long)num_seqs * nkv * gb_ceil_div(M, 16) <= 4 * 148 ? 16 : 64;
         p.floats = ((long long)num_seqs * nkv * gb_ceil_div(M, p.same ? TREE_TC_ROWS : 2 * TREE_TC_ROWS) + p.blocks) * (p.same ? 1 : 2) * TREE_TC_ROWS * (hd + 2);
         return p;
     }

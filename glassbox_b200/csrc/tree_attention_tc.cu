@@ -1,17 +1,17 @@
-// Attention of trees of drafted tokens over the paged cache on the 5th-generation tensor cores (sm_100a), bfloat16 at head sizes 64 and 128: the part of the
-// keys that every row of a request's tree sees, whole tiles of 128 before the tree. What is left of them, the tree itself, its masks and the sum of all parts
-// is tree_attention_mma.cu's.
+// Attention of trees of drafted tokens over the paged cache on the 5th-generation tensor cores (sm_100a), bfloat16 at head sizes 64 and 128, without a window.
 //
 // A block has two units of 128 query rows (rows of the tree x query heads that share a key/value head; TMEM lanes). Where a request has at most 128 of them
-// (SAME) both units have the same ones and take the tiles of keys in turn, else they are 256 rows that take every tile. Either way two chains of
-// scores -> softmax -> product keep tensor cores and exponentials busy in turn. Tiles of all items (request, key/value head, 256 rows) are cut evenly among one
-// block a multiprocessor; a block goes through its pieces of items without draining its pipelines.
+// (SAME) both units have the same ones and take the tiles of 128 keys in turn, else they are 256 rows that take every tile. Either way two chains of
+// scores -> softmax -> product keep tensor cores and exponentials busy in turn. Tiles of all items (request, key/value head, 256 or 128 rows) are cut evenly among
+// one block a multiprocessor; a block goes through its pieces of items without draining its pipelines. An item that one block has whole is written out, the others'
+// pieces go to the scratch, 32 rows side by side, and tree_tc_pieces_kernel adds up.
 //   warp 0, 10  producers of keys and of values: a page is HD / 64 boxes of 64 channels, rings of stages in 128-byte-swizzled rows.
 //   warp 1      issues S_g = Q_g K^T (M 128, N 128, K HD) and O_g += P_g V (M 128, N HD, K 128); the next scores of a unit right behind the product that reads P,
 //               which lies over the first half of the scores' columns.
-//   warps 2-9   softmax, four a unit, a row a thread; they lay the unit's queries out in shared memory, and write O, maxima and sums to the scratch.
-// Without masks there is nothing to compare: a row's tile is 128 exponentials. The scale is above 0. What bounds it: memory where rows are few, else a unit's chain.
-// Every wait is bounded: a wait that runs out sets GB_STATUS_WAIT_TIMEOUT and the block winds down.
+//   warps 2-9   softmax, four a unit, a row a thread; they lay the unit's queries out in shared memory, and write what comes out.
+// Masks are looked at only in the tiles that reach into the tree (bits, 32 keys at a time). There values that are not finite numbers are taken out of shared
+// memory, so that no weight of zero meets them; rows that see such a key get its part one key at a time.
+// What bounds it: memory where rows are few, else a unit's chain. Every wait is bounded: a wait that runs out sets GB_STATUS_WAIT_TIMEOUT and the block winds down.
 #include "tcgen05.cuh"
 #include "tree_attention.cuh"
 
@@ -36,6 +36,7 @@ struct __align__(16) Tc5Shared {
     uint64_t s_full[2], p_most[2], p_ready[2], pv_done[2];
     long long at;                         // the tile of all items behind those of the list
     uint32_t tmem_base;
+    int odd;                              // a value of the piece's tiles that reach into the tree is not a finite number
     int abort_flag, segs;                 // (segs: negative where the share ends with them)
     int issued[2], consumed[2];
 };
@@ -67,6 +68,32 @@ __device__ __forceinline__ void tc5_store16(uint32_t taddr, const uint32_t (&r)[
                  : "memory");
 }
 
+// 16 channels of a row's O get the part of the keys from `k0` to `k1` whose values are not all finite, one at a time (they were taken out of the products).
+template <int HD>
+__device__ __forceinline__ void tree_odd_keys(const TreeArgs& a, const TreeSeq& s, int row, int m, int kvh, int G, int k0, int k1, float top, int c, uint32_t (&o)[16]) {
+    const __nv_bfloat16* q = (const __nv_bfloat16*)a.q + (size_t)row * a.q_stride + (size_t)(kvh * G + m % G) * HD;
+    const int pos = a.positions[row];
+#pragma unroll 1
+    for (int key = k0; key < k1; ++key) {
+        const int page = s.page(a, key / a.page_size);
+        if (page < 0 || !s.sees(a, row, pos, key)) continue;
+        const size_t at = (((size_t)page * a.nkv + kvh) * a.page_size + key % a.page_size) * HD;
+        const __nv_bfloat16* k = (const __nv_bfloat16*)a.kcache + at;
+        const __nv_bfloat16* v = (const __nv_bfloat16*)a.vcache + at;
+        float dot = 0.f;
+        bool odd = false;
+#pragma unroll 1
+        for (int i = 0; i < HD; ++i) {
+            dot = fmaf(__bfloat162float(q[i]), __bfloat162float(k[i]), dot);
+            odd = odd || !isfinite(__bfloat162float(v[i]));
+        }
+        if (!odd) continue;
+        const float p = tc5_exp2(dot * a.scale * 1.4426950408889634f - top);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(fmaf(p, __bfloat162float(v[c + i]), __uint_as_float(o[i])));
+    }
+}
+
 template <int HD, bool SAME>
 __global__ void __launch_bounds__(TC5_WARPS * 32) tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                                                                            const TreeArgs a, int num_seqs, int page_shift) {
@@ -86,14 +113,14 @@ __global__ void __launch_bounds__(TC5_WARPS * 32) tree_attention_tc_kernel(const
     }
     // The next pieces of the block's share, up to TC5_SEGS, from tile `at` on (all of warp 0); count 0: there are none.
     auto list = [&](bool begin) {
-        TreeCut cut(a, num_seqs, ROWS, TC5_KEYS, gridDim.x, TREE_LEAST_SHARE, true);
+        TreeCut cut(a, num_seqs, ROWS, TC5_KEYS, gridDim.x, TREE_LEAST_SHARE);
         const long long end = min(cut.total, (blockIdx.x + 1) * cut.share);
         long long at = begin ? min(cut.total, blockIdx.x * cut.share) : sh.at;
         int count = 0;
         if (at < end) cut.seek(at);
         for (; at < end && count < TC5_SEGS; ++count) {
             const TreeSeq s(a, cut.seq);
-            const int all = s.start / TC5_KEYS;
+            const int all = s.tiles(TC5_KEYS);
             const long long off = at - cut.tile0;
             const int item = (int)(off / all), tile0 = (int)(off - (long long)item * all), tiles = (int)min((long long)all - tile0, end - at);
             if (lane == 0) {
@@ -132,7 +159,7 @@ __global__ void __launch_bounds__(TC5_WARPS * 32) tree_attention_tc_kernel(const
     volatile int* abort_flag = &sh.abort_flag;
 
     // what each role counts over all pieces
-    int tiles_done = 0;                           // producers and the issuer: tiles of keys and values
+    int tiles_done = 0;                           // tiles of keys and values
     int pieces_done = 0, steps = 0, steps1 = 0;   // the issuer and the softmax: pieces, and their unit's tiles (the issuer: unit 0's and unit 1's)
     bool ok = true;
     while (true) {
@@ -154,8 +181,9 @@ __global__ void __launch_bounds__(TC5_WARPS * 32) tree_attention_tc_kernel(const
                 const int kvh = seg.y / ((s.rows * G + ROWS - 1) / ROWS);
                 // the first row of this lane's page of a tile (lanes COLS i .. have page i); one that is missing lies behind all pages, where a copy reads zeros
                 auto row_of = [&](int tile) -> int {
-                    if (lane >= COLS * ppt) return nowhere;
-                    const long long page = s.page(a, ((tile * TC5_KEYS) >> page_shift) + lane / COLS);
+                    const int index = ((tile * TC5_KEYS) >> page_shift) + lane / COLS;
+                    if (lane >= COLS * ppt || (index << page_shift) >= s.length) return nowhere;
+                    const long long page = s.page(a, index);
                     if (page >= 0) return (int)((page * a.nkv + kvh) * a.page_size);
                     bad = true;
                     return nowhere;
@@ -262,9 +290,9 @@ __global__ void __launch_bounds__(TC5_WARPS * 32) tree_attention_tc_kernel(const
                 ok = false;
                 return true;
             };
-            for (int i = 0; i < segs; ++i) {
-                const int4 seg = sh.seg[i];
+            for (int i = 0; i < segs; tiles_done += sh.seg[i].w, ++i) {
                 int mine, units = 2;                      // tiles of this unit
+                int before;                               // its tiles that all lie before the tree
                 // both units are done with the piece before (every warp comes here for every piece, also one that has given up)
                 asm volatile("barrier.cta.sync 1, 256;" ::: "memory");
                 if (!ok) {
@@ -272,11 +300,15 @@ __global__ void __launch_bounds__(TC5_WARPS * 32) tree_attention_tc_kernel(const
                     continue;
                 }
                 {
+                    const int4 seg = sh.seg[i];
                     const TreeSeq s(a, seg.x);
                     const int M = s.rows * G, pairs = (M + ROWS - 1) / ROWS, m = seg.y % pairs * ROWS + (SAME ? 0 : g * TC5_M) + r;
                     if constexpr (!SAME) units = M - seg.y % pairs * ROWS > TC5_M ? 2 : 1;
                     mine = SAME ? (seg.w + 1 - g) / 2 : g < units ? seg.w : 0;
                     // the unit's queries into swizzled rows (zeros behind the last)
+                    if (tid == 64) sh.odd = 0;
+                    before = s.start / TC5_KEYS - seg.z;
+                    before = SAME ? (before + 1 - g) / 2 : before;      // (negative where the piece begins behind: all are masked)
                     if (!SAME || g == 0) {
                         const uint4* from = reinterpret_cast<const uint4*>((const __nv_bfloat16*)a.q + (size_t)(s.row0 + m / G) * a.q_stride + (size_t)(seg.y / pairs * G + m % G) * HD);
                         unsigned char* to = Qs + (SAME ? 0 : g * Sh::TILE) + r * 128;
@@ -293,6 +325,42 @@ __global__ void __launch_bounds__(TC5_WARPS * 32) tree_attention_tc_kernel(const
                 for (int j = 0; j < mine; ++j) {
                     if (!mbar_wait_warp(&sh.s_full[g], steps & 1, abort_flag, a.status)) { ok = false; break; }
                     tc_fence_after();
+                    if (j >= before) {
+                        const int4 seg = sh.seg[i];
+                        const TreeSeq s(a, seg.x);
+                        const int M = s.rows * G, m = seg.y % ((M + ROWS - 1) / ROWS) * ROWS + (SAME ? 0 : g * TC5_M) + r, row = m < M ? s.row0 + m / G : -1;
+                        const int tile = seg.z + (SAME ? 2 * j + g : j), first_key = tile * TC5_KEYS;
+                        // scores of keys that the row does not see become minus infinity where they lie
+                        for (int w = 0; w < 4; ++w) {
+                            const unsigned see = tree_bits(a, s.rows, row, first_key + 32 * w - s.start);
+                            uint32_t part[32];
+                            tmem_load32(lane_base + s_col + (uint32_t)(32 * w), part);
+#pragma unroll
+                            for (int k = 0; k < 32; ++k)
+                                if (!(see >> k & 1u)) part[k] = 0xff800000u;
+                            tmem_store32(lane_base + s_col + (uint32_t)(32 * w), part);
+                        }
+                        if (SAME || g == 0) {
+                            // a key's values a thread; the product waits for this unit's weights, which come behind
+                            const int ring = (tiles_done + tile - seg.z) % SV, use = (tiles_done + tile - seg.z) / SV;
+                            if (!mbar_wait_warp(&sh.v_full[ring], use & 1, abort_flag, a.status)) { ok = false; break; }
+                            unsigned char* v = Vs + ring * Sh::TILE + r * 128;
+                            bool odd = false;
+#pragma unroll
+                            for (int c = 0; c < HD / 8; ++c) {
+                                const uint4 x = *reinterpret_cast<const uint4*>(v + c / 8 * TC5_BLOCK + c % 8 * 16);      // (in whatever order)
+                                const uint32_t w4[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) odd = odd || (w4[e] & 0x7f80u) == 0x7f80u || (w4[e] & 0x7f800000u) == 0x7f800000u;
+                            }
+                            if (odd) {
+#pragma unroll
+                                for (int c = 0; c < HD / 8; ++c) *reinterpret_cast<uint4*>(v + c / 8 * TC5_BLOCK + c % 8 * 16) = make_uint4(0, 0, 0, 0);
+                                if (first_key + r < s.length) sh.odd = 1;
+                            }
+                            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        }
+                    }
                     // The scores of the last 64 keys stay in registers; the first 64 are read once more (all 128 beside the rest spill)
                     float mx4[4] = {TC5_NEG_BIG, TC5_NEG_BIG, TC5_NEG_BIG, TC5_NEG_BIG};
                     uint32_t sv[TC5_KEYS / 2];
@@ -355,51 +423,69 @@ __global__ void __launch_bounds__(TC5_WARPS * 32) tree_attention_tc_kernel(const
                     ++steps;
                 }
                 if (ok && mine > 0) ok = mbar_wait_warp(&sh.pv_done[g], (steps - 1) & 1, abort_flag, a.status);
+                // A row's result: O, relative to its maximum `top` (base 2), and the sum of its weights. SAME: the two units' parts are added up, each thread has half
+                // of the row's channels of both, whose columns all warps of the row's lanes can read. (Every warp meets that barrier for every piece.)
+                float top = m_run, l = l_run, f0 = 1.0f, f1 = 0.f;
+                int from_c = 0, to_c = HD;
+                const bool both = SAME && sh.seg[i].w > 1;      // (unit 0 has a tile always)
                 if constexpr (SAME) {
-                    // The two units' parts of a row: each thread adds up half of the row's channels of both, whose columns all warps of the row's lanes can read.
-                    // (Every warp meets this barrier for every piece, too.)
                     sh.stat[g][r] = mine > 0 ? make_float2(m_run, l_run) : make_float2(-INFINITY, 0.f);
                     tc_fence_before();
                     asm volatile("barrier.cta.sync 2, 256;" ::: "memory");
-                    tc_fence_after();
-                    const float2 other = sh.stat[g ^ 1][r];
-                    const float top = fmaxf(mine > 0 ? m_run : -INFINITY, other.x);      // (unit 0 has a tile always)
-                    const float f = mine > 0 ? tc5_exp2(m_run - top) : 0.f, f_other = tc5_exp2(other.x - top);
-                    const bool both = seg.w > 1;
-                    if (!__any_sync(0xffffffffu, *abort_flag)) {
-                        float* to = a.parts + (size_t)sh.piece[i] * (TC5_M * P) + (size_t)q * (32 * P) + lane;
-#pragma unroll
-                        for (int c = g * (HD / 2); c < HD; c += 16) {
-                            if (c >= (g + 1) * (HD / 2)) break;
-                            uint32_t o0[16], o1[16];
-                            tmem_load16(lane_base + (uint32_t)(Sh::O_COL + c), o0);
-                            if (both) tmem_load16(lane_base + (uint32_t)(Sh::O_COL + HD + c), o1);
-                            const float f0 = g ? f_other : f, f1 = g ? f : f_other;
-#pragma unroll
-                            for (int k = 0; k < 16; ++k) to[(c + k) * 32] = both ? fmaf(__uint_as_float(o1[k]), f1, __uint_as_float(o0[k]) * f0) : __uint_as_float(o0[k]);
-                        }
-                        if (g == 0) {
-                            to[HD * 32] = top;
-                            to[HD * 32 + 32] = fmaf(other.y, f_other, l_run * f);
-                        }
-                    } else {
-                        ok = false;
-                    }
-                    continue;
+                    const float2 s0 = sh.stat[0][r], s1 = sh.stat[1][r];
+                    top = fmaxf(s0.x, s1.x);
+                    f0 = tc5_exp2(s0.x - top);
+                    f1 = both ? tc5_exp2(s1.x - top) : 0.f;
+                    l = fmaf(s1.y, f1, s0.y * f0);
+                    from_c = g * (HD / 2);
+                    to_c = from_c + HD / 2;
+                    if (__any_sync(0xffffffffu, *abort_flag)) ok = false;
                 }
                 if (!ok) continue;
                 tc_fence_after();
-                // O, maximum (base 2) and sum to the scratch, 32 rows side by side
-                float* to = a.parts + ((size_t)sh.piece[i] * (SAME ? 1 : 2) + g) * (TC5_M * P) + (size_t)q * (32 * P) + lane;
+                const int4 seg = sh.seg[i];
+                const TreeSeq s(a, seg.x);
+                const int M = s.rows * G, pairs = (M + ROWS - 1) / ROWS, kvh = seg.y / pairs, m = seg.y % pairs * ROWS + (SAME ? 0 : g * TC5_M) + r, row = m < M ? s.row0 + m / G : -1;
+                const bool whole = seg.z == 0 && seg.w == s.tiles(TC5_KEYS);
+                const float inv = l != 0.f ? 1.0f / l : 0.f;
+                float* part = a.parts + ((size_t)sh.piece[i] * (SAME ? 1 : 2) + (SAME ? 0 : g)) * (TC5_M * P) + (size_t)q * (32 * P) + lane;
+                __nv_bfloat16* dst = (__nv_bfloat16*)a.out + (size_t)(row < 0 ? 0 : row) * a.out_stride + (size_t)(kvh * G + m % G) * HD;
+                for (int c = from_c; c < to_c; c += 16) {
+                    uint32_t o[16];
+                    if (SAME || mine > 0) tmem_load16(lane_base + (uint32_t)(Sh::O_COL + (SAME ? 0 : g * HD) + c), o);
+                    else
 #pragma unroll
-                for (int c = 0; c < HD; c += 32) {
-                    uint32_t ov[32];
-                    if (mine > 0) tmem_load32(lane_base + o_col + (uint32_t)c, ov);
+                        for (int k = 0; k < 16; ++k) o[k] = 0u;
+                    if constexpr (SAME) {
+                        if (both) {
+                            uint32_t o1[16];
+                            tmem_load16(lane_base + (uint32_t)(Sh::O_COL + HD + c), o1);
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) to[(c + k) * 32] = mine > 0 ? __uint_as_float(ov[k]) : 0.f;
+                            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(fmaf(__uint_as_float(o1[k]), f1, __uint_as_float(o[k]) * f0));
+                        }
+                    }
+                    if (sh.odd && row >= 0) tree_odd_keys<HD>(a, s, row, m, kvh, G, max(seg.z, s.start / TC5_KEYS) * TC5_KEYS, min(s.length, (seg.z + seg.w) * TC5_KEYS), top, c, o);
+                    if (whole) {
+                        if (row >= 0) {
+#pragma unroll
+                            for (int k = 0; k < 16; k += 8) {
+                                uint4 w;
+                                w.x = pack2(__float_as_uint(__uint_as_float(o[k]) * inv), __float_as_uint(__uint_as_float(o[k + 1]) * inv));
+                                w.y = pack2(__float_as_uint(__uint_as_float(o[k + 2]) * inv), __float_as_uint(__uint_as_float(o[k + 3]) * inv));
+                                w.z = pack2(__float_as_uint(__uint_as_float(o[k + 4]) * inv), __float_as_uint(__uint_as_float(o[k + 5]) * inv));
+                                w.w = pack2(__float_as_uint(__uint_as_float(o[k + 6]) * inv), __float_as_uint(__uint_as_float(o[k + 7]) * inv));
+                                *reinterpret_cast<uint4*>(dst + c + k) = w;
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) part[(c + k) * 32] = __uint_as_float(o[k]);
+                    }
                 }
-                to[HD * 32] = mine > 0 ? m_run : -INFINITY;
-                to[HD * 32 + 32] = l_run;
+                if (!whole && from_c == 0) {
+                    part[HD * 32] = SAME || mine > 0 ? top : -INFINITY;
+                    part[HD * 32 + 32] = l;
+                }
             }
         }
         if (!more) break;
@@ -409,6 +495,13 @@ __global__ void __launch_bounds__(TC5_WARPS * 32) tree_attention_tc_kernel(const
         __syncthreads();
     }
 
+    // padding requests' rows are zeros
+    for (int seq = blockIdx.x; seq < num_seqs; seq += gridDim.x) {
+        if (a.start_pos[seq] >= 0) continue;
+        const TreeSeq s(a, seq);
+        for (int i = tid; i < s.rows * a.nh * (HD / 2); i += TC5_WARPS * 32)
+            *reinterpret_cast<uint32_t*>((__nv_bfloat16*)a.out + (size_t)(s.row0 + i / (a.nh * (HD / 2))) * a.out_stride + i % (a.nh * (HD / 2)) * 2) = 0u;
+    }
     // ------------------------------------------------------------------------------- wind down
     tc_fence_before();
     __syncthreads();
@@ -428,8 +521,83 @@ __global__ void __launch_bounds__(TC5_WARPS * 32) tree_attention_tc_kernel(const
     }
 }
 
+// Adds up the pieces of items that several blocks share: EACH rows of a unit a block (x: rows and item, y: request). A thread has four rows of a channel.
+template <int HD, bool SAME, int EACH>
+__global__ void __launch_bounds__(256) tree_tc_pieces_kernel(const TreeArgs a, int num_seqs, int pairs_most, int blocks) {
+    constexpr int P = HD + 2, ROWS = SAME ? TC5_M : 2 * TC5_M, BATCH = 8, GROUPS = ROWS / EACH, QUADS = EACH / 4, LANES = 256 / EACH;
+    __shared__ float2 stats[EACH];                // of a row: maximum, 1 / sum
+    __shared__ float sums[EACH][HD + 1];
+    gb_pdl_launch_dependents();
+    gb_pdl_wait();
+    const int seq = blockIdx.y, G = a.nh / a.nkv, group = blockIdx.x % GROUPS, pair = blockIdx.x / GROUPS % pairs_most, kvh = blockIdx.x / GROUPS / pairs_most, tid = threadIdx.x;
+    const TreeSeq s(a, seq);
+    const int M = s.rows * G, m0 = pair * ROWS + group * EACH;
+    if (s.start < 0 || m0 >= M) return;
+    TreeCut cut(a, num_seqs, ROWS, TC5_KEYS, blocks, TREE_LEAST_SHARE);
+    cut.seek_seq(seq);
+    const int all = s.tiles(TC5_KEYS), item = kvh * ((M + ROWS - 1) / ROWS) + pair;
+    const long long t0 = cut.tile0 + (long long)item * all, b0 = t0 / cut.share;
+    const int count = (int)((t0 + all - 1) / cut.share - b0) + 1;
+    if (count == 1) return;
+    constexpr int STEP = ROWS * P;
+    const int u0 = group * EACH;                  // of the first row in the item
+    const float* first = a.parts + (size_t)(cut.item0 + item + b0) * STEP + u0 / 32 * (32 * P) + u0 % 32;
+    {
+        const int r = tid / LANES;
+        const float* from = first + HD * 32 + r;
+        float top = -INFINITY, l = 0.f;
+        for (int b = tid % LANES; b < count; b += LANES) {
+            const float m = from[(size_t)b * STEP], up = fmaxf(top, m), o = up == -INFINITY ? 0.f : up;
+            l = l * tc5_exp2(top - o) + from[(size_t)b * STEP + 32] * tc5_exp2(m - o);
+            top = up;
+        }
+        float most = top;
+#pragma unroll
+        for (int o = 1; o < LANES; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        const float o = most == -INFINITY ? 0.f : most;
+        l *= tc5_exp2(top - o);
+#pragma unroll
+        for (int k = 1; k < LANES; k <<= 1) l += __shfl_xor_sync(0xffffffffu, l, k);
+        if (tid % LANES == 0) stats[r] = make_float2(o, l != 0.f ? 1.0f / l : 0.f);
+    }
+    __syncthreads();
+    for (int i = tid; i < QUADS * HD; i += 256) {
+        const int r = i % QUADS * 4, c = i / QUADS;
+        float top[4], sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) top[k] = stats[r + k].x;
+        const float* from = first + r;
+        for (int b = 0; b < count; b += BATCH) {
+            float4 v[BATCH], m[BATCH];
+#pragma unroll
+            for (int u = 0; u < BATCH; ++u) {
+                const float* at = from + (size_t)min(b + u, count - 1) * STEP;
+                v[u] = *reinterpret_cast<const float4*>(at + c * 32);
+                m[u] = *reinterpret_cast<const float4*>(at + HD * 32);
+            }
+#pragma unroll
+            for (int u = 0; u < BATCH; ++u)
+                if (b + u < count) {
+                    sum[0] = fmaf(v[u].x, tc5_exp2(m[u].x - top[0]), sum[0]);
+                    sum[1] = fmaf(v[u].y, tc5_exp2(m[u].y - top[1]), sum[1]);
+                    sum[2] = fmaf(v[u].z, tc5_exp2(m[u].z - top[2]), sum[2]);
+                    sum[3] = fmaf(v[u].w, tc5_exp2(m[u].w - top[3]), sum[3]);
+                }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sums[r + k][c] = sum[k] * stats[r + k].y;
+    }
+    __syncthreads();
+    for (int i = tid; i < EACH * (HD / 2); i += 256) {
+        const int r = i / (HD / 2), c = i % (HD / 2) * 2, m = m0 + r;
+        if (m >= M) break;
+        *reinterpret_cast<uint32_t*>((__nv_bfloat16*)a.out + (size_t)(s.row0 + m / G) * a.out_stride + (kvh * G + m % G) * HD + c) =
+            pack2(__float_as_uint(sums[r][c]), __float_as_uint(sums[r][c + 1]));
+    }
+}
+
 template <int HD, bool SAME>
-static int tc5_launch(const TreeArgs& a, int blocks, int num_seqs, cudaStream_t stream) {
+static int tc5_launch(const TreeArgs& a, int blocks, int num_seqs, int max_rows, cudaStream_t stream) {
     using Sh = Tc5Shape<HD, SAME>;
     constexpr int SMEM = Sh::SH_OFF + (int)sizeof(Tc5Shared);
     static_assert(SMEM <= 227 * 1024, "the block does not fit");
@@ -442,11 +610,17 @@ static int tc5_launch(const TreeArgs& a, int blocks, int num_seqs, cudaStream_t 
     while ((1 << page_shift) < a.page_size) ++page_shift;
     e = gb_launch(GB_PDL_ATTENTION, tree_attention_tc_kernel<HD, SAME>, dim3(blocks), dim3(TC5_WARPS * 32), SMEM, stream, mk, mv, a, num_seqs, page_shift);
     GB_REQUIRE(e == cudaSuccess, "gb_tree_attention: launch failed: %s", cudaGetErrorString(e));
+    const int rows = SAME ? TC5_M : 2 * TC5_M, pairs = gb_ceil_div((long long)max_rows * (a.nh / a.nkv), rows);
+    // (8 rows a block where that leaves few of them)
+    const bool fine = (long long)pairs * a.nkv * num_seqs * (rows / 8) <= 8 * 148;
+    const dim3 grid(pairs * a.nkv * (rows / (fine ? 8 : 32)), num_seqs);
+    e = gb_launch(GB_PDL_ATTENTION, fine ? tree_tc_pieces_kernel<HD, SAME, 8> : tree_tc_pieces_kernel<HD, SAME, 32>, grid, dim3(256), 0, stream, a, num_seqs, pairs, blocks);
+    GB_REQUIRE(e == cudaSuccess, "gb_tree_attention: launch failed: %s", cudaGetErrorString(e));
     return gb_check_launch("gb_tree_attention");
 }
 
-int gb_tree_attention_tc(const TreeArgs& a, const TreePlan& plan, int num_seqs, cudaStream_t stream) {
+int gb_tree_attention_tc(const TreeArgs& a, const TreePlan& plan, int num_seqs, int max_rows, cudaStream_t stream) {
     GB_REQUIRE(a.num_pages * a.nkv * a.page_size < (1ll << 31), "gb_tree_attention: the pages hold too many rows");
-    if (a.hd == 64) return plan.same ? tc5_launch<64, true>(a, plan.blocks, num_seqs, stream) : tc5_launch<64, false>(a, plan.blocks, num_seqs, stream);
-    return plan.same ? tc5_launch<128, true>(a, plan.blocks, num_seqs, stream) : tc5_launch<128, false>(a, plan.blocks, num_seqs, stream);
+    if (a.hd == 64) return plan.same ? tc5_launch<64, true>(a, plan.blocks, num_seqs, max_rows, stream) : tc5_launch<64, false>(a, plan.blocks, num_seqs, max_rows, stream);
+    return plan.same ? tc5_launch<128, true>(a, plan.blocks, num_seqs, max_rows, stream) : tc5_launch<128, false>(a, plan.blocks, num_seqs, max_rows, stream);
 }

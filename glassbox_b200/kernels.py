@@ -2654,12 +2654,13 @@ VERIFY_MAX_VOCAB = 4096 * 512
 
 def tree_attention_kind(q: torch.Tensor, out: torch.Tensor, hd: int, page_size: int, scale: float, rows: int) -> int:
     """Which kernels ``tree_attention`` runs: 1 the tensor cores' (bfloat16, head sizes 32, 64, 96 and 128, rows that start at 4 bytes, pages of a
-    power of two from 8 on, below 2^31 rows of them), 2 tcgen05's, too, where there is enough for them (rows of q at 16 bytes, pages of 8 to 128 tokens, a scale above 0), 0 the one for
+    power of two from 8 on, below 2^31 rows of them), 2 tcgen05's where there is enough for it (rows of q and out at 16 bytes, pages of 8 to 128 tokens, a scale above 0), 0 the one for
     everything else."""
     if not (q.dtype == torch.bfloat16 and hd in (32, 64, 96, 128) and page_size >= 8 and page_size & (page_size - 1) == 0 and rows < 1 << 31
             and q.stride(0) % 2 == 0 and q.data_ptr() % 4 == 0 and out.stride(0) % 2 == 0 and out.data_ptr() % 4 == 0):
         return 0
-    return 2 if scale > 0 and page_size <= 128 and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0 else 1
+    return 2 if (scale > 0 and page_size <= 128 and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0 and out.stride(0) % 8 == 0
+                 and out.data_ptr() % 16 == 0) else 1
 
 
 @functools.lru_cache(maxsize=4096)

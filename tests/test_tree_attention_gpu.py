@@ -160,6 +160,60 @@ def test_masked_places_hold_anything(dtype, hd, value):
         assert torch.isnan(dirty[2]).all()
 
 
+@pytest.mark.parametrize("hd,nh,nkv", [(64, 4, 2), (128, 4, 2), (128, 4, 1)])
+@pytest.mark.parametrize("shapes", [[(600, 40)], [(513, 64), (40, 33)], [(127, 64), (128, 1), (129, 50), (0, 64), (1030, 40)], [(-1, 40), (700, 50), (-1, 2)],
+                                    [(640, 128), (640, 100)], [(100, 300)], [(2000, 65), (0, 0), (90, 64)]])
+@pytest.mark.parametrize("reach", [None, 2048])
+def test_many_rows(hd, nh, nkv, shapes, reach):
+    """Enough query rows a key/value head for tcgen05 (contexts are said to be long): one unit's rows, two, several pairs."""
+    b = Batch(BF, nh, nkv, hd, shapes, seed=hd + nkv)
+    b.check(b.run(reach=reach))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("nkv", [1, 2])
+@pytest.mark.parametrize("page", [8, 16, 32, 128, 256])
+def test_many_rows_and_pages(hd, nkv, page):
+    b = Batch(BF, 4, nkv, hd, [(700, 45), (1300, 33), (5, 40)], page=page, seed=page)
+    b.check(b.run())
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_many_rows_of_many_requests(hd):
+    """More pieces a block than its list holds."""
+    rng = random.Random(hd)
+    b = Batch(BF, 4, 1, hd, [(rng.choice([0, 5, 130, 600]), rng.choice([1, 20, 33])) for _ in range(700)], seed=5)
+    b.check(b.run(reach=1024))
+
+
+@pytest.mark.parametrize("hd,nkv", [(64, 2), (128, 2), (128, 1)])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("past", [590, 639, 5000])
+def test_masked_places_of_many_rows_hold_anything(hd, nkv, value, past):
+    rng = random.Random(4)
+    parents = plain.random_tree(rng, 64, 4)
+    see = plain.ancestors(parents)
+    b = Batch(BF, 4, nkv, hd, [(past, 64)], seed=9, see=lambda rng, rows: see)
+    clean = b.run()
+    where = past + 20
+    page = int(b.dev["tables"][0, where // 16])
+    b.dev["v"][page, :, where % 16, 3:5] = value
+    dirty = b.run()
+    hit = torch.from_numpy(see[:, 20])
+    assert 0 < hit.sum() < 63
+    off = (dirty[:64][~hit].float() - clean[:64][~hit].float()).abs().max()
+    assert torch.isfinite(dirty[:64][~hit]).all() and off == 0
+    got = dirty[:64][hit].view(-1, 4, hd)
+    assert (torch.isnan(got[..., 3:5]) if math.isnan(value) else torch.isinf(got[..., 3:5])).all()
+    assert torch.isfinite(got[..., :3]).all() and torch.isfinite(got[..., 5:]).all()
+    want = clean[:64][hit].view(-1, 4, hd)
+    rest = [c for c in range(hd) if c not in (3, 4)]
+    assert (got[..., rest].float() - want[..., rest].float()).abs().max() <= 2.0 ** -7 * want.float().abs().max()      # (its weight is not rounded there)
+    b.dev["k"][page, :, where % 16] = value               # a key, too
+    dirty = b.run()
+    assert torch.isfinite(dirty[:64][~hit]).all() and (dirty[:64][~hit].float() - clean[:64][~hit].float()).abs().max() == 0
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_strides_and_other_pools(dtype):
     b = Batch(dtype, 6, 2, 64, [(90, 12), (200, 3)], seed=4)
