@@ -1,109 +1,145 @@
 // Attention of trees of drafted tokens over the paged cache, for every type, head size and page size: float32 arithmetic.
-// (bfloat16 at the head sizes of tree_attention_mma.cu runs there.)
+// (bfloat16 at the head sizes of tree_attention_mma.cu and tree_attention_tc.cu runs there.)
 //
-// A block takes 32 query rows of a request and key/value head over its share of the keys, 32 at a time from shared memory; a thread forms the scores of
-// 2 rows and 4 keys, and the outputs of the 2 rows at every eighth piece of four channels. What is masked never enters a sum: its weight is not formed.
+// A block takes 16 RT query rows of a request and key/value head over its share of the keys, 32 at a time from two buffers of shared memory, one of which is
+// filled while the other is worked on. A thread forms the scores of RT rows and 4 keys, and the outputs of these rows at every eighth piece of four channels, so
+// that a number from shared memory meets four others. Masks are looked at only in tiles that reach into the tree or out of a window; where one of these holds a
+// value that is not a finite number, values go to the rows that see them one at a time, so that no weight of zero meets it. What bounds it: the multiply-adds where rows are many, else a block's chain.
 #include "tree_attention.cuh"
 
-constexpr int TA_THREADS = 128, TA_ROWS = 32, TA_KEYS = 32, TA_MAX_HD = 256;
+constexpr int TA_THREADS = 128, TA_KEYS = 32, TA_MAX_HD = 256, TA_PP = TA_KEYS + 4;
 
-static __host__ __device__ __forceinline__ int ta_pitch(int hd) { return (hd + 3) / 4 * 4 + 4; }      // floats of a row in shared memory
+template <typename T> __device__ __forceinline__ float4 ta_four(const T* p);
+template <> __device__ __forceinline__ float4 ta_four<float>(const float* p) { return *reinterpret_cast<const float4*>(p); }
+template <> __device__ __forceinline__ float4 ta_four<__nv_bfloat16>(const __nv_bfloat16* p) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
+}
+// Numbers of a row in shared memory: channels in fours (zeros behind the last), and 16 bytes so that eight rows' pieces lie in different banks.
+template <typename T> static __host__ __device__ __forceinline__ int ta_pitch(int hd) { return (hd + 7) / 8 * 8 + 16 / (int)sizeof(T); }
 
-template <typename T, int PIECES>      // pieces of four channels of a thread: hd <= 32 * PIECES
+template <typename T, int RT, int PIECES>      // rows of a thread; its pieces of four channels: hd <= 32 * PIECES
 __global__ void __launch_bounds__(TA_THREADS) tree_attention_kernel(const TreeArgs a) {
-    extern __shared__ __align__(16) float ta_smem[];
-    const int hd = a.hd, pitch = ta_pitch(hd), tid = threadIdx.x, tx = tid & 7, ty = tid >> 3;
-    float* Qs = ta_smem;
-    float* Ks = Qs + TA_ROWS * pitch;
-    float* Vs = Ks + TA_KEYS * pitch;
-    float* Ps = Vs + TA_KEYS * pitch;                 // [TA_ROWS][TA_KEYS + 1]
+    extern __shared__ __align__(16) unsigned char ta_smem[];
+    constexpr int ROWS = 16 * RT;
+    const int hd = a.hd, pitch = ta_pitch<T>(hd), qpitch = ta_pitch<float>(hd), fours = (hd + 3) / 4, tid = threadIdx.x, tx = tid & 7, ty = tid >> 3;
+    float* Qs = reinterpret_cast<float*>(ta_smem);
+    float* Ps = Qs + ROWS * qpitch;                   // [ROWS][TA_PP]
+    T* KVs = reinterpret_cast<T*>(Ps + ROWS * TA_PP); // [2 buffers][keys, values][TA_KEYS][pitch]
     gb_pdl_launch_dependents();
     gb_pdl_wait();
     const TreeSeq s(a, blockIdx.z);
-    const int G = a.nh / a.nkv, kvh = blockIdx.y % a.nkv, m0 = blockIdx.y / a.nkv * TA_ROWS, M = s.rows * G, split = blockIdx.x;
+    const int G = a.nh / a.nkv, kvh = blockIdx.y % a.nkv, m0 = blockIdx.y / a.nkv * ROWS, M = s.rows * G, split = blockIdx.x;
     if (m0 >= M) return;
     T* out = (T*)a.out;
-    // the thread's two rows: 2 ty and 2 ty + 1 of the tile
-    int row[2], head[2], pos[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int m = m0 + 2 * ty + h;
-        row[h] = m < M ? s.row0 + m / G : -1;
-        head[h] = kvh * G + m % G;
-        pos[h] = row[h] >= 0 ? a.positions[row[h]] : -1;
-    }
     if (s.start < 0) {                                // a padding request: zeros
         if (split == 0)
-            for (int h = 0; h < 2; ++h)
-                for (int c = tx; row[h] >= 0 && c < hd; c += 8) out[(size_t)row[h] * a.out_stride + head[h] * hd + c] = gb_from_float<T>(0.f);
+            for (int i = tid; i < min(ROWS, M - m0) * hd; i += TA_THREADS) {
+                const int m = m0 + i / hd;
+                out[(size_t)(s.row0 + m / G) * a.out_stride + (kvh * G + m % G) * hd + i % hd] = gb_from_float<T>(0.f);
+            }
         return;
     }
     const int keys = s.length - s.key_lo, share = (keys + a.splits - 1) / a.splits, k_begin = s.key_lo + split * share, k_end = min(s.length, k_begin + share);
-    for (int i = tid; i < TA_ROWS * pitch; i += TA_THREADS) {
-        const int m = m0 + i / pitch, c = i % pitch;
-        Qs[i] = m < M && c < hd ? gb_to_float(((const T*)a.q)[(size_t)(s.row0 + m / G) * a.q_stride + (kvh * G + m % G) * hd + c]) : 0.f;
+    const bool vec = hd * sizeof(T) % 16 == 0 && ((uintptr_t)a.kcache | (uintptr_t)a.vcache) % 16 == 0;
+    bool bad = false;
+    auto load = [&](int k0, int buffer) {             // 32 keys and values; zeros behind the share's last key
+        T* to = KVs + buffer * 2 * TA_KEYS * pitch;
+        if (vec) {
+            const int pieces = hd * (int)sizeof(T) / 16;
+            for (int i = tid; i < TA_KEYS * pieces; i += TA_THREADS) {
+                const int r = i / pieces, c = i % pieces, key = k0 + r, page = key < k_end ? s.page(a, key / a.page_size) : -1;
+                if (key < k_end && page < 0) bad = true;
+                const size_t at = page < 0 ? 0 : (((size_t)page * a.nkv + kvh) * a.page_size + key % a.page_size) * hd * sizeof(T) + c * 16;
+                const int bytes = page < 0 ? 0 : 16;
+                const unsigned dst = (unsigned)__cvta_generic_to_shared(to + r * pitch) + c * 16;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"((const char*)a.kcache + at), "r"(bytes) : "memory");
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + TA_KEYS * pitch * (int)sizeof(T)), "l"((const char*)a.vcache + at), "r"(bytes) : "memory");
+            }
+        } else {
+            for (int i = tid; i < TA_KEYS * 4 * fours; i += TA_THREADS) {
+                const int r = i / (4 * fours), c = i % (4 * fours), key = k0 + r, page = key < k_end ? s.page(a, key / a.page_size) : -1;
+                if (key < k_end && page < 0) bad = true;
+                const size_t at = page < 0 ? 0 : (((size_t)page * a.nkv + kvh) * a.page_size + key % a.page_size) * hd + c;
+                to[r * pitch + c] = page >= 0 && c < hd ? ((const T*)a.kcache)[at] : gb_from_float<T>(0.f);
+                to[(TA_KEYS + r) * pitch + c] = page >= 0 && c < hd ? ((const T*)a.vcache)[at] : gb_from_float<T>(0.f);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    if (k_begin < k_end) load(k_begin, 0);
+    for (int i = tid; i < ROWS * 4 * fours; i += TA_THREADS) {
+        const int r = i / (4 * fours), c = i % (4 * fours), m = m0 + r;
+        Qs[r * qpitch + c] = m < M && c < hd ? gb_to_float(((const T*)a.q)[(size_t)(s.row0 + m / G) * a.q_stride + (kvh * G + m % G) * hd + c]) : 0.f;
+    }
+    // the thread's rows: RT ty ... of the tile
+    int row[RT], pos[RT];
+#pragma unroll
+    for (int h = 0; h < RT; ++h) {
+        const int m = m0 + RT * ty + h;
+        row[h] = m < M ? s.row0 + m / G : -1;
+        pos[h] = row[h] >= 0 ? a.positions[row[h]] : -1;
     }
     const float sl2 = a.scale * 1.4426950408889634f;
-    float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f}, acc[2][PIECES][4];
+    float m_run[RT], l_run[RT], acc[RT][PIECES][4];
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < RT; ++h) {
+        m_run[h] = -INFINITY;
+        l_run[h] = 0.f;
 #pragma unroll
         for (int p = 0; p < PIECES; ++p)
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[h][p][e] = 0.f;
-    bool bad = false;
-    for (int k0 = k_begin; k0 < k_end; k0 += TA_KEYS) {
-        __syncthreads();                              // (the tile before has been read)
-        for (int i = tid; i < TA_KEYS * pitch; i += TA_THREADS) {
-            const int key = k0 + i / pitch, c = i % pitch;
-            float kv = 0.f, vv = 0.f;
-            if (key < k_end && c < hd) {
-                const int page = s.page(a, key / a.page_size);
-                if (page >= 0) {
-                    const size_t at = (((size_t)page * a.nkv + kvh) * a.page_size + key % a.page_size) * hd + c;
-                    kv = gb_to_float(((const T*)a.kcache)[at]);
-                    vv = gb_to_float(((const T*)a.vcache)[at]);
-                } else {
-                    bad = true;
-                }
-            }
-            Ks[i] = kv;
-            Vs[i] = vv;
-        }
-        __syncthreads();
-        float sc[2][4] = {};
-        for (int c = 0; c < pitch - 4; c += 4) {
-            float4 qv[2], kv[4];
+    }
+    for (int k0 = k_begin, buffer = 0; k0 < k_end; k0 += TA_KEYS, buffer ^= 1) {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();                              // the tile is there, the one before has been read
+        if (k0 + TA_KEYS < k_end) load(k0 + TA_KEYS, buffer ^ 1);
+        const T* Ks = KVs + buffer * 2 * TA_KEYS * pitch;
+        const T* Vs = Ks + TA_KEYS * pitch;
+        float sc[RT][4] = {};
+        for (int c = 0; c < 4 * fours; c += 4) {
+            float4 qv[RT], kv[4];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) qv[h] = *reinterpret_cast<const float4*>(Qs + (2 * ty + h) * pitch + c);
+            for (int h = 0; h < RT; ++h) qv[h] = *reinterpret_cast<const float4*>(Qs + (RT * ty + h) * qpitch + c);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) kv[i] = *reinterpret_cast<const float4*>(Ks + (tx + 8 * i) * pitch + c);
+            for (int i = 0; i < 4; ++i) kv[i] = ta_four(Ks + (tx + 8 * i) * pitch + c);
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < RT; ++h)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     sc[h][i] = fmaf(qv[h].x, kv[i].x, fmaf(qv[h].y, kv[i].y, fmaf(qv[h].z, kv[i].z, fmaf(qv[h].w, kv[i].w, sc[h][i]))));
         }
-        const bool masked = k0 + TA_KEYS > min(s.start, k_end) || a.window > 0;
-        unsigned seen[2];                             // of the tile's keys, for each of the two rows
+        const bool masked = k0 + TA_KEYS > min(s.start, k_end) || a.window > 0;      // (the same for the block)
+        unsigned seen[RT];                            // of the tile's keys, by each of the rows
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < RT; ++h) {
             float mx = -INFINITY;
-            unsigned mine = 0;
+            unsigned mine = 0xffffffffu;
+            if (masked) {
+                mine = row[h] < 0 ? 0u : tree_bits(a, s.rows, row[h], k0 - s.start);
+                if (k_end - k0 < TA_KEYS) mine &= (1u << (k_end - k0)) - 1u;
+                if (a.window > 0) {
+                    unsigned near = 0u;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int key = k0 + tx + 8 * i;
-                const bool ok = row[h] >= 0 && (!masked || (key < k_end && s.sees(a, row[h], pos[h], key)));
-                mine |= (unsigned)ok << (tx + 8 * i);
-                sc[h][i] *= sl2;
-                if (ok) mx = fmaxf(mx, sc[h][i]);
-            }
+                    for (int i = 0; i < 4; ++i) {
+                        const int key = k0 + tx + 8 * i;
+                        if (mine >> (tx + 8 * i) & 1u)
+                            near |= (unsigned)(pos[h] - (key < s.start ? key : a.positions[s.row0 + key - s.start]) < a.window) << (tx + 8 * i);
+                    }
 #pragma unroll
-            for (int o = 1; o < 8; o <<= 1) {
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                mine |= __shfl_xor_sync(0xffffffffu, mine, o);
+                    for (int o = 1; o < 8; o <<= 1) near |= __shfl_xor_sync(0xffffffffu, near, o);
+                    mine = near;
+                }
             }
             seen[h] = mine;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                sc[h][i] = mine >> (tx + 8 * i) & 1u ? sc[h][i] * sl2 : -INFINITY;
+                mx = fmaxf(mx, sc[h][i]);
+            }
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
             const float m_new = fmaxf(m_run[h], mx), off = m_new == -INFINITY ? 0.f : m_new, corr = exp2f(m_run[h] - off);
             m_run[h] = m_new;
             l_run[h] *= corr;
@@ -113,34 +149,71 @@ __global__ void __launch_bounds__(TA_THREADS) tree_attention_kernel(const TreeAr
                 for (int e = 0; e < 4; ++e) acc[h][p][e] *= corr;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float p = mine >> (tx + 8 * i) & 1u ? exp2f(sc[h][i] - off) : 0.f;
+                const float p = exp2f(sc[h][i] - off);
                 l_run[h] += p;
-                Ps[(2 * ty + h) * (TA_KEYS + 1) + tx + 8 * i] = p;
+                Ps[(RT * ty + h) * TA_PP + tx + 8 * i] = p;
             }
         }
-        __syncwarp();                                 // (a row's eight threads are neighbours)
-        const unsigned either = seen[0] | seen[1];
-        for (int k = 0; k < TA_KEYS; ++k) {
-            if (!(either >> k & 1u)) continue;
-            const float p0 = Ps[(2 * ty) * (TA_KEYS + 1) + k], p1 = Ps[(2 * ty + 1) * (TA_KEYS + 1) + k];
-            const bool s0 = seen[0] >> k & 1u, s1 = seen[1] >> k & 1u;
-#pragma unroll
-            for (int p = 0; p < PIECES; ++p) {
-                const int c = 4 * tx + 32 * p;
-                if (c >= hd) continue;
-                const float4 v = *reinterpret_cast<const float4*>(Vs + k * pitch + c);
-                if (s0) { acc[0][p][0] = fmaf(p0, v.x, acc[0][p][0]); acc[0][p][1] = fmaf(p0, v.y, acc[0][p][1]); acc[0][p][2] = fmaf(p0, v.z, acc[0][p][2]); acc[0][p][3] = fmaf(p0, v.w, acc[0][p][3]); }
-                if (s1) { acc[1][p][0] = fmaf(p1, v.x, acc[1][p][0]); acc[1][p][1] = fmaf(p1, v.y, acc[1][p][1]); acc[1][p][2] = fmaf(p1, v.z, acc[1][p][2]); acc[1][p][3] = fmaf(p1, v.w, acc[1][p][3]); }
+        // (a row's eight threads are neighbours; a value that is no finite number must not meet a weight of zero)
+        bool odd = false;
+        if (masked) {
+            for (int i = tid; i < TA_KEYS * fours; i += TA_THREADS) {
+                const float4 v = ta_four(Vs + i / fours * pitch + i % fours * 4);
+                odd = odd || !isfinite(v.x) || !isfinite(v.y) || !isfinite(v.z) || !isfinite(v.w);
             }
+            odd = __syncthreads_or(odd);
+        } else {
+            __syncwarp();
+        }
+        if (!odd) {
+            for (int k = 0; k < TA_KEYS; k += 4) {
+                float4 p4[RT];
+#pragma unroll
+                for (int h = 0; h < RT; ++h) p4[h] = *reinterpret_cast<const float4*>(Ps + (RT * ty + h) * TA_PP + k);
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int p = 0; p < PIECES; ++p) {
+                        const int c = 4 * tx + 32 * p;
+                        if (c >= hd) continue;
+                        const float4 v = ta_four(Vs + (k + u) * pitch + c);
+#pragma unroll
+                        for (int h = 0; h < RT; ++h) {
+                            const float w = u == 0 ? p4[h].x : u == 1 ? p4[h].y : u == 2 ? p4[h].z : p4[h].w;
+                            acc[h][p][0] = fmaf(w, v.x, acc[h][p][0]);
+                            acc[h][p][1] = fmaf(w, v.y, acc[h][p][1]);
+                            acc[h][p][2] = fmaf(w, v.z, acc[h][p][2]);
+                            acc[h][p][3] = fmaf(w, v.w, acc[h][p][3]);
+                        }
+                    }
+            }
+        } else {
+            for (int k = 0; k < TA_KEYS; ++k)
+#pragma unroll
+                for (int h = 0; h < RT; ++h) {
+                    if (!(seen[h] >> k & 1u)) continue;
+                    const float w = Ps[(RT * ty + h) * TA_PP + k];
+#pragma unroll
+                    for (int p = 0; p < PIECES; ++p) {
+                        const int c = 4 * tx + 32 * p;
+                        if (c >= hd) continue;
+                        const float4 v = ta_four(Vs + k * pitch + c);
+                        acc[h][p][0] = fmaf(w, v.x, acc[h][p][0]);
+                        acc[h][p][1] = fmaf(w, v.y, acc[h][p][1]);
+                        acc[h][p][2] = fmaf(w, v.z, acc[h][p][2]);
+                        acc[h][p][3] = fmaf(w, v.w, acc[h][p][3]);
+                    }
+                }
         }
     }
     if (bad) atomicOr(a.status, GB_STATUS_BAD_SLOT);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < RT; ++h) {
 #pragma unroll
         for (int o = 1; o < 8; o <<= 1) l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], o);
         if (row[h] < 0) continue;
-        const size_t cell = (size_t)row[h] * a.nh + head[h], cells = (size_t)a.n * a.nh;
+        const int head = kvh * G + (m0 + RT * ty + h) % G;
+        const size_t cell = (size_t)row[h] * a.nh + head, cells = (size_t)a.n * a.nh;
         float* part = a.parts + ((size_t)split * cells + cell) * hd;
         const float inv = l_run[h] != 0.f ? 1.0f / l_run[h] : 0.f;
 #pragma unroll
@@ -149,7 +222,7 @@ __global__ void __launch_bounds__(TA_THREADS) tree_attention_kernel(const TreeAr
             for (int e = 0; e < 4; ++e) {
                 const int c = 4 * tx + 32 * p + e;
                 if (c >= hd) continue;
-                if (a.splits == 1) out[(size_t)row[h] * a.out_stride + head[h] * hd + c] = gb_from_float<T>(acc[h][p][e] * inv);
+                if (a.splits == 1) out[(size_t)row[h] * a.out_stride + head * hd + c] = gb_from_float<T>(acc[h][p][e] * inv);
                 else part[c] = acc[h][p][e];
             }
         if (a.splits > 1 && tx == 0)
@@ -157,54 +230,86 @@ __global__ void __launch_bounds__(TA_THREADS) tree_attention_kernel(const TreeAr
     }
 }
 
-// Adds up the shares of a row and head: a warp each.
+// Adds up the shares of a row and head: a warp each, a lane a share's weight.
 template <typename T>
 __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeArgs a, int num_seqs) {
     gb_pdl_launch_dependents();
     gb_pdl_wait();
     const int lane = threadIdx.x & 31;
     const size_t cells = (size_t)a.n * a.nh, cell = (size_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (cell >= cells) return;
     const int row = (int)(cell / a.nh);
-    if (cell >= cells || row < a.first_row[0] || row >= a.first_row[num_seqs]) return;
-    int lo = 0, hi = num_seqs;                        // the row's request: a padding one has been written
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (a.first_row[mid] <= row) lo = mid; else hi = mid;
+    bool live = false;                                // the row belongs to a request that is no padding (whose rows have been written)
+    for (int s0 = 0; s0 < num_seqs && !live; s0 += 32) {
+        const int s = s0 + lane;
+        live = __any_sync(0xffffffffu, s < num_seqs && a.first_row[s] <= row && row < a.first_row[s + 1] && a.start_pos[s] >= 0);
     }
-    if (a.start_pos[lo] < 0) return;
+    if (!live) return;
     const float2* ml = reinterpret_cast<const float2*>(a.parts + a.splits * cells * a.hd) + cell;
-    float m = -INFINITY, l = 0.f;
-    for (int i = 0; i < a.splits; ++i) m = fmaxf(m, ml[i * cells].x);
-    const float off = m == -INFINITY ? 0.f : m;
-    for (int i = 0; i < a.splits; ++i) l = fmaf(ml[i * cells].y, exp2f(ml[i * cells].x - off), l);
-    const float inv = l != 0.f ? 1.0f / l : 0.f;
-    for (int c = lane; c < a.hd; c += 32) {
-        float v = 0.f;
-#pragma unroll 4
-        for (int i = 0; i < a.splits; ++i) v = fmaf(a.parts[(i * cells + cell) * a.hd + c], exp2f(ml[i * cells].x - off), v);
-        ((T*)a.out)[(size_t)row * a.out_stride + (cell % a.nh) * a.hd + c] = gb_from_float<T>(v * inv);
+    float top = -INFINITY;
+    for (int i = lane; i < a.splits; i += 32) top = fmaxf(top, ml[i * cells].x);
+    top = gb_warp_max(top);
+    const float off = top == -INFINITY ? 0.f : top;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, l = 0.f;
+    for (int i0 = 0; i0 < a.splits; i0 += 32) {
+        const float2 own = i0 + lane < a.splits ? ml[(i0 + lane) * cells] : make_float2(-INFINITY, 0.f);
+        const float f = exp2f(own.x - off);
+        l = fmaf(own.y, f, l);
+        const int count = min(32, a.splits - i0);
+#pragma unroll 8
+        for (int i = 0; i < count; ++i) {
+            const float w = __shfl_sync(0xffffffffu, f, i);
+            const float* part = a.parts + ((size_t)(i0 + i) * cells + cell) * a.hd;
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+                if (lane + 32 * c < a.hd) v[c] = fmaf(part[lane + 32 * c], w, v[c]);
+        }
     }
+    l = gb_warp_sum(l);
+    const float inv = l != 0.f ? 1.0f / l : 0.f;
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+        if (lane + 32 * c < a.hd) ((T*)a.out)[(size_t)row * a.out_stride + (cell % a.nh) * a.hd + lane + 32 * c] = gb_from_float<T>(v[c] * inv);
+}
+
+// Query rows of a block, up to 64 (32 of heads above 128 channels, whose outputs fill the registers): those that leave few of them empty, and rather more, since
+// the keys that a thread reads meet all of its rows. (72 rows a request and key/value head, 4 requests of 15/5 heads of 64 behind 1,500 keys, float32.)
+static int ta_rows(long long m, int hd) {
+    int best = 16;
+    double least = 0.0;
+    for (int rows = 16; rows <= (hd > 128 ? 32 : 64); rows += 16) {
+        const double cost = (double)gb_ceil_div(m, rows) * rows * (1.0 + 10.0 / rows);
+        if (rows == 16 || cost < least) { best = rows; least = cost; }
+    }
+    return best;
+}
+
+template <typename T, int RT, int PIECES>
+static int ta_launch(const TreeArgs& a, int num_seqs, int max_rows, cudaStream_t stream) {
+    const int tiles = gb_ceil_div((long long)max_rows * (a.nh / a.nkv), 16 * RT);
+    GB_REQUIRE((long long)tiles * a.nkv <= 65535, "gb_tree_attention: %d rows a request are too many for one launch", max_rows);
+    const int smem = 16 * RT * (ta_pitch<float>(a.hd) + TA_PP) * 4 + 4 * TA_KEYS * ta_pitch<T>(a.hd) * (int)sizeof(T);
+    cudaError_t e = cudaFuncSetAttribute(tree_attention_kernel<T, RT, PIECES>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    GB_REQUIRE(e == cudaSuccess, "gb_tree_attention: %d bytes of shared memory refused: %s", smem, cudaGetErrorString(e));
+    e = gb_launch(GB_PDL_ATTENTION, tree_attention_kernel<T, RT, PIECES>, dim3(a.splits, tiles * a.nkv, num_seqs), dim3(TA_THREADS), smem, stream, a);
+    GB_REQUIRE(e == cudaSuccess, "gb_tree_attention: launch failed: %s", cudaGetErrorString(e));
+    return gb_check_launch("gb_tree_attention");
 }
 
 template <typename T, int PIECES>
-static int ta_launch(const TreeArgs& a, int num_seqs, int tiles, cudaStream_t stream) {
-    const int smem = ((TA_ROWS + 2 * TA_KEYS) * ta_pitch(a.hd) + TA_ROWS * (TA_KEYS + 1)) * (int)sizeof(float);
-    cudaError_t e = cudaFuncSetAttribute(tree_attention_kernel<T, PIECES>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    GB_REQUIRE(e == cudaSuccess, "gb_tree_attention: %d bytes of shared memory refused: %s", smem, cudaGetErrorString(e));
-    e = gb_launch(GB_PDL_ATTENTION, tree_attention_kernel<T, PIECES>, dim3(a.splits, tiles * a.nkv, num_seqs), dim3(TA_THREADS), smem, stream, a);
-    GB_REQUIRE(e == cudaSuccess, "gb_tree_attention: launch failed: %s", cudaGetErrorString(e));
-    return 0;
+static int ta_sized(const TreeArgs& a, int num_seqs, int max_rows, cudaStream_t stream) {
+    const int rows = ta_rows((long long)max_rows * (a.nh / a.nkv), a.hd);
+    if (rows == 16) return ta_launch<T, 1, PIECES>(a, num_seqs, max_rows, stream);
+    if (rows == 32) return ta_launch<T, 2, PIECES>(a, num_seqs, max_rows, stream);
+    if constexpr (PIECES <= 4) return rows == 48 ? ta_launch<T, 3, PIECES>(a, num_seqs, max_rows, stream) : ta_launch<T, 4, PIECES>(a, num_seqs, max_rows, stream);
+    return 1;
 }
 
 template <typename T>
 static int ta_dispatch(const TreeArgs& a, int num_seqs, int max_rows, cudaStream_t stream) {
-    const int tiles = gb_ceil_div((long long)max_rows * (a.nh / a.nkv), TA_ROWS);
-    GB_REQUIRE((long long)tiles * a.nkv <= 65535, "gb_tree_attention: %d rows a request are too many for one launch", max_rows);
-    int rc;
-    if (a.hd <= 64) rc = ta_launch<T, 2>(a, num_seqs, tiles, stream);
-    else if (a.hd <= 128) rc = ta_launch<T, 4>(a, num_seqs, tiles, stream);
-    else rc = ta_launch<T, 8>(a, num_seqs, tiles, stream);
-    return rc ? rc : gb_check_launch("gb_tree_attention");
+    if (a.hd <= 64) return ta_sized<T, 2>(a, num_seqs, max_rows, stream);
+    if (a.hd <= 128) return ta_sized<T, 4>(a, num_seqs, max_rows, stream);
+    return ta_sized<T, 8>(a, num_seqs, max_rows, stream);
 }
 
 // tree_attention_mma.cu, tree_attention_tc.cu
@@ -212,11 +317,11 @@ int gb_tree_attention_tc(const TreeArgs& a, const TreePlan& plan, int num_seqs, 
 int gb_tree_attention_mma(const TreeArgs& a, const TreePlan& plan, int num_seqs, int max_rows, cudaStream_t stream);
 TreePlan tree_plan_mma(int num_seqs, int max_rows, int nh, int nkv, int hd, int max_context, int window, bool tc);
 
-// Shares of a request's keys in this file's kernel, so that blocks fill the GPU, of 128 keys at least.
-static int ta_splits(int num_seqs, int max_rows, int nh, int nkv, int max_context, int window) {
-    const long long blocks = (long long)num_seqs * nkv * gb_ceil_div((long long)max_rows * (nh / nkv), TA_ROWS);
-    const int reach = window > 0 && window + max_rows < max_context ? window + max_rows : max_context, most = reach <= 128 ? 1 : gb_ceil_div(reach, 128);
-    const long long splits = 148ll * 3 / blocks;
+// Shares of a request's keys in this file's kernel, so that blocks fill the GPU, of 64 keys at least.
+static int ta_splits(int num_seqs, int max_rows, int nh, int nkv, int hd, int max_context, int window) {
+    const long long m = (long long)max_rows * (nh / nkv), blocks = (long long)num_seqs * nkv * gb_ceil_div(m, ta_rows(m, hd));
+    const int reach = window > 0 && window + max_rows < max_context ? window + max_rows : max_context, most = reach <= 64 ? 1 : gb_ceil_div(reach, 64);
+    const long long splits = 148ll * 4 / blocks;
     return splits > most ? most : splits < 1 ? 1 : (int)splits;
 }
 
@@ -227,7 +332,7 @@ GB_EXPORT int gb_tree_attention_floats(int kind, int n, int num_seqs, int max_ro
     if (kind >= 1) {
         floats = tree_plan_mma(num_seqs, max_rows, nh, nkv, hd, max_context, window, kind == 2).floats;
     } else {
-        const int splits = ta_splits(num_seqs, max_rows, nh, nkv, max_context, window);
+        const int splits = ta_splits(num_seqs, max_rows, nh, nkv, hd, max_context, window);
         floats = splits > 1 ? (long long)splits * n * nh * (hd + 2) : 0;
     }
     return floats < (1ll << 31) ? (int)floats : -1;
@@ -256,7 +361,7 @@ GB_EXPORT int gb_tree_attention(int kind, const void* q, long long q_stride, voi
         GB_REQUIRE(plan.floats == 0 || (parts != nullptr && (uintptr_t)parts % 16 == 0), "gb_tree_attention: the scratch is missing or not 16-byte aligned");
         return plan.tc ? gb_tree_attention_tc(a, plan, num_seqs, max_rows, stream) : gb_tree_attention_mma(a, plan, num_seqs, max_rows, stream);
     }
-    a.splits = ta_splits(num_seqs, max_rows, nh, nkv, max_context, window);
+    a.splits = ta_splits(num_seqs, max_rows, nh, nkv, hd, max_context, window);
     GB_REQUIRE(a.splits == 1 || parts != nullptr, "gb_tree_attention: the scratch is missing");
     const int rc = dtype == GB_F32 ? ta_dispatch<float>(a, num_seqs, max_rows, stream) : ta_dispatch<__nv_bfloat16>(a, num_seqs, max_rows, stream);
     if (rc || a.splits == 1) return rc;
