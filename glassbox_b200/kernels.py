@@ -2652,15 +2652,14 @@ TREE_MAX_ROWS = 1024           # rows of a request's tree
 VERIFY_MAX_VOCAB = 4096 * 512
 
 
-def tree_attention_kind(q: torch.Tensor, out: torch.Tensor, hd: int, page_size: int, scale: float, rows: int) -> int:
+def _tree_kind(dtype: int, addresses: int, strides: int, hd: int, page_size: int, scaled: bool, rows: int) -> int:
     """Which kernels ``tree_attention`` runs: 1 the tensor cores' (bfloat16, head sizes 32, 64, 96 and 128, rows that start at 4 bytes, pages of a
-    power of two from 8 on, below 2^31 rows of them), 2 tcgen05's where there is enough for it (rows of q and out at 16 bytes, pages of 8 to 128 tokens, a scale above 0), 0 the one for
-    everything else."""
-    if not (q.dtype == torch.bfloat16 and hd in (32, 64, 96, 128) and page_size >= 8 and page_size & (page_size - 1) == 0 and rows < 1 << 31
-            and q.stride(0) % 2 == 0 and q.data_ptr() % 4 == 0 and out.stride(0) % 2 == 0 and out.data_ptr() % 4 == 0):
+    power of two from 8 on, below 2^31 rows of them), 2 tcgen05's where there is enough for it (rows of q and out at 16 bytes, pages of 8 to 128 tokens, a scale
+    above 0), 0 the one for everything else."""
+    if not (dtype == BF16 and hd in (32, 64, 96, 128) and page_size >= 8 and page_size & (page_size - 1) == 0 and rows < 1 << 31
+            and strides % 2 == 0 and addresses % 4 == 0):
         return 0
-    return 2 if (scale > 0 and page_size <= 128 and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0 and out.stride(0) % 8 == 0
-                 and out.data_ptr() % 16 == 0) else 1
+    return 2 if scaled and page_size <= 128 and strides % 8 == 0 and addresses % 16 == 0 else 1
 
 
 @functools.lru_cache(maxsize=4096)
@@ -2684,13 +2683,14 @@ def tree_attention_floats(n: int, nh: int, nkv: int, hd: int, num_seqs: int, max
     return max(_tree_floats(kind, n, num_seqs, max_rows_per_seq, nh, nkv, hd, int(max_context), int(window or 0)) for kind in (0, 1, 2))
 
 
-def _tree_batch(block_tables, seq_first_row, seq_start_pos) -> int:
-    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.shape[1] < 1 or not block_tables.is_contiguous():
+def _tree_batch(block_tables, seq_first_row, seq_start_pos):
+    """(requests, pages of a table) of a batch."""
+    shape = block_tables.shape
+    if block_tables.dtype != torch.int32 or len(shape) != 2 or shape[1] < 1 or not block_tables.is_contiguous():
         raise KernelError("block_tables must be contiguous int32 [requests, pages]")
-    num_seqs = block_tables.shape[0]
-    _vector("seq_first_row", seq_first_row, num_seqs + 1)
-    _vector("seq_start_pos", seq_start_pos, num_seqs)
-    return num_seqs
+    _vector("seq_first_row", seq_first_row, shape[0] + 1)
+    _vector("seq_start_pos", seq_start_pos, shape[0])
+    return shape
 
 
 def tree_attention(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, block_tables: torch.Tensor,
@@ -2704,19 +2704,22 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vca
     with a negative start; rows that belong to no request stay as they are. q, out: bfloat16 or float32 [n, nh * hd], rows may be strided; kcache, vcache
     [pages, nkv, page_size, hd] of the same type. No request has more than ``max_rows_per_seq`` rows; ``max_context`` sizes the shares of the keys
     (longer contexts are still right), ``parts`` comes from ``tree_attention_parts`` of the same sizes."""
-    if not (q.dim() == 2 and q.shape[1] == nh * hd and q.stride(1) == 1 and out.shape == q.shape and out.stride(1) == 1):
+    shape, q_strides, out_strides = q.shape, q.stride(), out.stride()
+    if not (len(shape) == 2 and shape[1] == nh * hd and q_strides[1] == 1 and out.shape == shape and out_strides[1] == 1):
         raise KernelError(f"q and out must be [n, {nh * hd}] with neighbouring numbers")
-    n = q.shape[0]
+    n = shape[0]
     if nkv < 1 or nh < 1 or nh % nkv or not 0 < hd <= 256:
         raise KernelError(f"{nh}/{nkv} heads of {hd} channels are not built")
     if not (q.dtype == out.dtype == kcache.dtype == vcache.dtype):
         raise KernelError("q, out and the cache must be of one type")
-    for name, t in (("kcache", kcache), ("vcache", vcache)):
-        if t.dim() != 4 or t.shape[1:] != (nkv, page_size, hd) or t.shape[0] < 1 or t.shape != kcache.shape or not t.is_contiguous():
-            raise KernelError(f"{name} must be contiguous [pages, {nkv}, {page_size}, {hd}]")
-    num_seqs = _tree_batch(block_tables, seq_first_row, seq_start_pos)
+    pool = kcache.shape
+    if not (len(pool) == 4 and pool[0] > 0 and pool[1] == nkv and pool[2] == page_size and pool[3] == hd and vcache.shape == pool
+            and kcache.is_contiguous() and vcache.is_contiguous()):
+        raise KernelError(f"kcache and vcache must be contiguous [pages, {nkv}, {page_size}, {hd}]")
+    num_seqs, max_pages = _tree_batch(block_tables, seq_first_row, seq_start_pos)
     _vector("positions", positions, n)
-    if visible.dtype != torch.int32 or visible.dim() != 2 or visible.shape[0] < n or visible.shape[1] < 1 or not visible.is_contiguous():
+    seen = visible.shape
+    if visible.dtype != torch.int32 or len(seen) != 2 or seen[0] < n or seen[1] < 1 or not visible.is_contiguous():
         raise KernelError(f"visible must be contiguous int32 [{n}, words]")
     if not 0 <= max_rows_per_seq <= TREE_MAX_ROWS:
         raise KernelError(f"a tree of {max_rows_per_seq} rows is not built (up to {TREE_MAX_ROWS})")
@@ -2726,14 +2729,15 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vca
     stream = _here(q, out, kcache, vcache, block_tables, seq_first_row, seq_start_pos, positions, visible, parts, status)
     if not n or not num_seqs or not max_rows_per_seq:
         return
-    kind = tree_attention_kind(q, out, hd, page_size, scale, kcache.shape[0] * nkv * page_size)
+    q_at, out_at = q.data_ptr(), out.data_ptr()
+    kind = _tree_kind(dtype, q_at | out_at, q_strides[0] | out_strides[0], hd, page_size, scale > 0, pool[0] * nkv * page_size)
     max_context, window = int(max_context), int(window or 0)
     floats = _tree_floats(kind, n, num_seqs, max_rows_per_seq, nh, nkv, hd, max_context, window)
     if floats and (parts is None or parts.dtype != torch.float32 or not parts.is_contiguous() or parts.numel() < floats):
         raise KernelError(f"this batch needs contiguous float32 scratch of {floats} numbers (tree_attention_parts)")
-    _call("gb_tree_attention", kind, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), dtype, kcache.data_ptr(), vcache.data_ptr(),
-          block_tables.data_ptr(), block_tables.shape[1], seq_first_row.data_ptr(), seq_start_pos.data_ptr(), positions.data_ptr(), visible.data_ptr(),
-          visible.shape[1], n, num_seqs, int(max_rows_per_seq), nh, nkv, hd, page_size, kcache.shape[0], float(scale), window, max_context, _ptr(parts),
+    _call("gb_tree_attention", kind, q_at, q_strides[0], out_at, out_strides[0], dtype, kcache.data_ptr(), vcache.data_ptr(),
+          block_tables.data_ptr(), max_pages, seq_first_row.data_ptr(), seq_start_pos.data_ptr(), positions.data_ptr(), visible.data_ptr(),
+          seen[1], n, num_seqs, int(max_rows_per_seq), nh, nkv, hd, page_size, pool[0], float(scale), window, max_context, _ptr(parts),
           status.data_ptr(), stream)
 
 
@@ -2762,13 +2766,14 @@ def verify_tree(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tenso
     Results, int32: accepted[s] rows are kept (row 0 always is; 0 for a request without rows), path[seq_first_row[s] + j] is the j-th of them (-1 behind the
     last), next_token[s] the token that follows (-1: the logits that the walk reached hold a NaN or plus infinity, or nothing but minus infinity; a greedy walk
     passes over NaN). A child whose token is outside the vocabulary is never taken."""
-    if not (logits.dim() == 2 and logits.stride(1) == 1):
+    shape, strides = logits.shape, logits.stride()
+    if not (len(shape) == 2 and strides[1] == 1):
         raise KernelError("logits must be [rows, vocab] with neighbouring numbers")
-    n, vocab = logits.shape
+    n, vocab = shape
     num_seqs = temperature.shape[0]
     if not 0 < vocab <= VERIFY_MAX_VOCAB:
         raise KernelError(f"a vocabulary of {vocab} is not built (up to {VERIFY_MAX_VOCAB})")
-    if draft_logits is not None and not (draft_logits.shape == logits.shape and draft_logits.dtype == logits.dtype and draft_logits.stride(1) == 1):
+    if draft_logits is not None and not (draft_logits.shape == shape and draft_logits.dtype == logits.dtype and draft_logits.stride(1) == 1):
         raise KernelError(f"draft_logits must be {logits.dtype} [{n}, {vocab}] with neighbouring numbers, as logits are")
     for name, t, size in (("tokens", tokens, n), ("parents", parents, n), ("seq_first_row", seq_first_row, num_seqs + 1), ("path", path, n),
                           ("accepted", accepted, num_seqs), ("next_token", next_token, num_seqs)):
@@ -2779,7 +2784,7 @@ def verify_tree(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tenso
         raise KernelError(f"uniform must be contiguous float32 [{n}, 2]")
     dtype = _dt(logits)
     stream = _here(logits, tokens, parents, seq_first_row, uniform, temperature, path, accepted, next_token, draft_logits)
-    _call("gb_verify_tree", logits.data_ptr(), dtype, logits.stride(0), _ptr(draft_logits), 0 if draft_logits is None else draft_logits.stride(0),
+    _call("gb_verify_tree", logits.data_ptr(), dtype, strides[0], _ptr(draft_logits), 0 if draft_logits is None else draft_logits.stride(0),
           tokens.data_ptr(), parents.data_ptr(), seq_first_row.data_ptr(), uniform.data_ptr(), temperature.data_ptr(), path.data_ptr(), accepted.data_ptr(),
           next_token.data_ptr(), n, num_seqs, vocab, int(verify_walks(n, num_seqs, vocab, logits.element_size(), draft_logits is not None)), stream)
 
@@ -2790,16 +2795,17 @@ def keep_rows(kpool: torch.Tensor, vpool: torch.Tensor, block_tables: torch.Tens
     seq_start_pos[s] + path[seq_first_row[s] + j] goes to seq_start_pos[s] + j for j < accepted[s], path ascending. kpool, vpool: contiguous [layers, pages,
     heads, page_size, channels] of any type of 2 bytes or more, values may have other channels than keys. Requests with a negative start are passed over; where a
     path leaves its tree or a page is missing nothing of the request moves, and ``status`` says so."""
-    for name, t in (("kpool", kpool), ("vpool", vpool)):
-        if t.dim() != 5 or t.shape[:4] != kpool.shape[:4] or t.shape[3] != page_size or not t.is_contiguous() or t.element_size() < 2 or not t.numel():
-            raise KernelError(f"{name} must be contiguous [layers, pages, heads, {page_size}, channels] of numbers of 2 bytes or more")
-    num_seqs = _tree_batch(block_tables, seq_first_row, seq_start_pos)
+    keys, values, key_size, value_size = kpool.shape, vpool.shape, kpool.element_size(), vpool.element_size()
+    if not (len(keys) == len(values) == 5 and (keys == values or keys[:4] == values[:4]) and keys[3] == page_size and kpool.is_contiguous() and vpool.is_contiguous()
+            and key_size >= 2 and value_size >= 2 and 0 not in keys and values[4] > 0):
+        raise KernelError(f"kpool and vpool must be contiguous [layers, pages, heads, {page_size}, channels] of numbers of 2 bytes or more")
+    num_seqs, max_pages = _tree_batch(block_tables, seq_first_row, seq_start_pos)
     n = path.shape[0]
     _vector("path", path, n)
     _vector("accepted", accepted, num_seqs)
     if not 0 <= max_rows_per_seq <= TREE_MAX_ROWS:
         raise KernelError(f"a tree of {max_rows_per_seq} rows is not built (up to {TREE_MAX_ROWS})")
     stream = _here(kpool, vpool, block_tables, seq_first_row, seq_start_pos, path, accepted, status)
-    _call("gb_keep_rows", kpool.data_ptr(), vpool.data_ptr(), kpool.shape[4] * kpool.element_size(), vpool.shape[4] * vpool.element_size(), kpool.shape[0],
-          kpool.shape[1], kpool.shape[2], page_size, block_tables.data_ptr(), block_tables.shape[1], seq_first_row.data_ptr(), seq_start_pos.data_ptr(),
-          path.data_ptr(), accepted.data_ptr(), n, num_seqs, status.data_ptr(), stream)
+    _call("gb_keep_rows", kpool.data_ptr(), vpool.data_ptr(), keys[4] * key_size, values[4] * value_size, keys[0], keys[1], keys[2], page_size,
+          block_tables.data_ptr(), max_pages, seq_first_row.data_ptr(), seq_start_pos.data_ptr(), path.data_ptr(), accepted.data_ptr(), n, num_seqs,
+          status.data_ptr(), stream)
