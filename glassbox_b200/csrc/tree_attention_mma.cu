@@ -40,10 +40,12 @@ __device__ __forceinline__ uint32_t tm_pack(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-template <int HD, int WM, int WK>
+template <int HD, int WM, int WK, bool CLUSTER>
 struct TmShape {
     static constexpr bool TMA = HD % 64 == 0;      // blocks of 64 channels in 128-byte-swizzled rows, else padded rows that threads copy
-    static constexpr int STAGES = HD == 64 ? 4 : 3;
+    // (an even cut of 16 trees of 32 rows, 32/32 heads of 64, 4,095 tokens: four blocks a multiprocessor of three stages 129 us, three of four 143; clusters of 8 trees
+    // of 16 rows, 15/5 heads of 64, 2,500 tokens: 18 and 16.5)
+    static constexpr int STAGES = HD == 64 && CLUSTER ? 4 : 3, BLOCKS = WM * WK == 8 ? (HD > 64 ? 1 : 2) : HD > 64 ? 2 : HD == 64 && CLUSTER ? 3 : 4;
     static constexpr int COLS = HD / 64, BLOCK = TM_KEYS * 128;
     static constexpr int PITCH = TMA ? 128 : HD * 2 + 16, TILE = TMA ? COLS * BLOCK : TM_KEYS * PITCH, THREADS = WM * WK * 32, ROWS = WM * 16, KW = TM_KEYS / WK, P = HD + 2;
     static constexpr int SMEM = 2 * STAGES * TILE + TM_MAX_PAGES * 4;
@@ -54,14 +56,14 @@ struct TmShape {
 // shared memory. Otherwise all items' tiles of keys are cut evenly among the blocks; what a block finds of an item that it shares with others goes to the
 // scratch, piece number (item + block), and tree_pieces_kernel adds up.
 template <int HD, int WM, int WK, bool CLUSTER>
-__global__ void __launch_bounds__(WM* WK * 32) tree_attention_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+__global__ void __launch_bounds__(WM* WK * 32, TmShape<HD, WM, WK, CLUSTER>::BLOCKS) tree_attention_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                                                                          const TreeArgs a, int num_seqs) {
     namespace cg = cooperative_groups;
-    using Sh = TmShape<HD, WM, WK>;
+    using Sh = TmShape<HD, WM, WK, CLUSTER>;
     constexpr bool TMA = Sh::TMA;
     constexpr int STAGES = Sh::STAGES, NW = WM * WK;
-    // Tiles that are under way beside the one worked on: with TMA one stage less than there are, so that a warp may be a tile behind the one that asks for
-    // the next (all warps at a barrier a tile: 136 us where this takes %s).
+    // Tiles that are under way beside the one worked on: with TMA one stage less than there are, so that a warp may be a tile behind the one that asks for the
+    // next.
     constexpr int AHEAD = TMA ? STAGES - 2 : STAGES - 1;
     constexpr int CH = HD / 8, KS = HD / 16, NT = HD / 8, KW = Sh::KW, KT = KW / 8, P = Sh::P;
     extern __shared__ __align__(1024) unsigned char tm_mem[];
@@ -456,7 +458,7 @@ __global__ void __launch_bounds__(128) tree_pieces_kernel(const TreeArgs a, int 
 
 template <int HD, int WM, int WK>
 static int tm_launch(const TreeArgs& a, const TreePlan& plan, int num_seqs, int max_rows, cudaStream_t stream) {
-    using Sh = TmShape<HD, WM, WK>;
+    using Sh = TmShape<HD, WM, WK, true>;             // (what both forms share)
     CUtensorMap mk = {}, mv = {};
     if constexpr (Sh::TMA) {
         const int box = a.page_size < TM_KEYS ? a.page_size : TM_KEYS;
@@ -493,9 +495,9 @@ static int tm_launch(const TreeArgs& a, const TreePlan& plan, int num_seqs, int 
         return gb_check_launch("gb_tree_attention");
     }
     const auto kernel = tree_attention_mma_kernel<HD, WM, WK, false>;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM);
-    GB_REQUIRE(e == cudaSuccess, "gb_tree_attention: %d bytes of shared memory refused: %s", Sh::SMEM, cudaGetErrorString(e));
-    e = gb_launch(GB_PDL_ATTENTION, kernel, dim3(plan.blocks), dim3(Sh::THREADS), Sh::SMEM, stream, mk, mv, a, num_seqs);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TmShape<HD, WM, WK, false>::SMEM);
+    GB_REQUIRE(e == cudaSuccess, "gb_tree_attention: %d bytes of shared memory refused: %s", TmShape<HD, WM, WK, false>::SMEM, cudaGetErrorString(e));
+    e = gb_launch(GB_PDL_ATTENTION, kernel, dim3(plan.blocks), dim3(Sh::THREADS), TmShape<HD, WM, WK, false>::SMEM, stream, mk, mv, a, num_seqs);
     GB_REQUIRE(e == cudaSuccess, "gb_tree_attention: launch failed: %s", cudaGetErrorString(e));
     e = gb_launch(GB_PDL_ATTENTION, tree_pieces_kernel<HD, Sh::ROWS>, dim3(m_tiles * a.nkv * (Sh::ROWS / 8), num_seqs), dim3(128), 0, stream, a, num_seqs, m_tiles, plan.blocks);
     GB_REQUIRE(e == cudaSuccess, "gb_tree_attention: launch failed: %s", cudaGetErrorString(e));
@@ -539,14 +541,15 @@ TreePlan tree_plan_mma(int num_seqs, int max_rows, int nh, int nkv, int hd, int 
         return p;
     }
     p.rows = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
-    const int room = 148 * (hd > 64 ? (p.rows == 128 && hd == 128 ? 1 : 2) : hd == 64 ? 3 : 4);
+    const int room = 148 * (p.rows == 128 ? (hd > 64 ? 1 : 2) : hd > 64 ? 2 : hd == 64 ? 3 : 4);      // (as TmShape::BLOCKS)
     const long long items = (long long)num_seqs * nkv * gb_ceil_div(M, p.rows);
     const int reach = window > 0 && window + max_rows < max_context ? window + max_rows : max_context, tiles = gb_ceil_div(reach > 0 ? reach : 1, TM_KEYS);
     int c = TM_MAX_CLUSTER;
     while (c > 1 && (items * c > room || tiles < 2 * c)) c /= 2;
+    const int even = hd == 64 && p.rows < 128 ? 148 * 4 : room;      // blocks of the even cut
     const double tile_us = 0.5, waves = (double)((items * c + room - 1) / room), cluster_us = waves * gb_ceil_div(tiles, c) * tile_us, even_us = (double)items * tiles / room * tile_us + 4.0;
     p.cluster = cluster_us <= even_us ? c : 0;
-    p.blocks = p.cluster ? 0 : room;
-    p.floats = p.cluster ? 0 : (items + room) * p.rows * (hd + 2);
+    p.blocks = p.cluster ? 0 : even;
+    p.floats = p.cluster ? 0 : (items + even) * p.rows * (hd + 2);
     return p;
 }
