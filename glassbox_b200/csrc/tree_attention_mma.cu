@@ -1,12 +1,16 @@
 // Attention of trees of drafted tokens over the paged cache in bfloat16 on the tensor cores (mma.sync m16n8k16), head sizes 32, 64, 96 and 128.
 //
-// A block takes 16 WM query rows (rows of the tree x query heads that share the key/value head) of a request over its share of the keys, 64 at a time
-// through a ring of three stages that asynchronous copies fill; WM x WK warps, each with 16 of the rows and 64 / WK of a stage's keys, so that small trees
-// keep four warps at work. Rows of shared memory are padded by 16 bytes: eight rows' pieces lie in different banks. Softmax statistics and outputs are
-// float32 (a maximum and a sum per row and warp, added up at the end); weights are rounded to bfloat16 on their way into the second product, 2^-9 of each.
+// A block takes 16 WM query rows (rows of the tree x query heads that share the key/value head) of a request over its share of the keys, 64 at a time through a
+// ring of stages: one thread's TMA copies of boxes of the page's keys x 64 channels in 128-byte-swizzled rows, for heads of 64 and 128; for 32
+// and 96 every thread's 16-byte copies into rows padded by 16 bytes. WM x WK warps, each with 16 of the rows and 64 / WK of a stage's keys, so that small trees
+// keep four warps at work. Softmax statistics and outputs are float32 (a maximum and a sum per row and warp, added up at the end); weights are rounded to bfloat16
+// on their way into the second product, 2^-9 of each.
 //
 // Masks are looked at only where a warp's keys hold some that a row may not see: bits of the tree come as 32 at a time. There a value that is not a finite
-// number must not meet a weight of zero, so such keys go one by one.
+// number must not meet a weight of zero, so such values are zero in the product and go to the rows that see them one by one.
+//
+// What bounds it: keys and values are read once, 256 bytes of them for a row's 128 products and an exponential. 16 trees of 32 rows, 32/32 heads of 64, behind
+// 4,095 tokens: MMA_CASE. Where items are few, a tile's trip and a block's start and end (about 7 us).
 #include "tcgen05.cuh"
 #include "tree_attention.cuh"
 
@@ -38,6 +42,12 @@ __device__ __forceinline__ float tm_exp2(float x) {
 __device__ __forceinline__ uint32_t tm_pack(float lo, float hi) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
+}
+// Two values, those that are not finite numbers as zero.
+__device__ __forceinline__ uint32_t tm_finite(uint32_t two) {
+    if ((two & 0x7f80u) == 0x7f80u) two &= 0xffff0000u;
+    if ((two & 0x7f800000u) == 0x7f800000u) two &= 0xffffu;
+    return two;
 }
 
 template <int HD, int WM, int WK, bool CLUSTER>
@@ -271,7 +281,7 @@ __global__ void __launch_bounds__(WM* WK * 32, TmShape<HD, WM, WK, CLUSTER>::BLO
             for (int j = 0; j < NT; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[j][e] *= corr[e >> 1];
-            if (!odd) {
+            auto product = [&](auto some_odd) {
 #pragma unroll
                 for (int b = 0; b < KW / 16; ++b) {
                     const uint32_t p[4] = {tm_pack(sc[2 * b][0], sc[2 * b][1]), tm_pack(sc[2 * b][2], sc[2 * b][3]), tm_pack(sc[2 * b + 1][0], sc[2 * b + 1][1]),
@@ -280,11 +290,19 @@ __global__ void __launch_bounds__(WM* WK * 32, TmShape<HD, WM, WK, CLUSTER>::BLO
                     for (int j = 0; j < NT; j += 2) {
                         uint32_t v[4];
                         tm_ldmatrix_t(v, vb + b * 16 * Sh::PITCH + piece_at(j / 2, v_half));
+                        if constexpr (decltype(some_odd)::value) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) v[e] = tm_finite(v[e]);
+                        }
                         tm_mma(acc[j], p, v[0], v[1]);
                         tm_mma(acc[j + 1], p, v[2], v[3]);
                     }
                 }
+            };
+            if (!odd) {
+                product(std::false_type());
             } else {
+                product(std::true_type());
 #pragma unroll
                 for (int j = 0; j < KT; ++j)
 #pragma unroll
@@ -297,8 +315,11 @@ __global__ void __launch_bounds__(WM* WK * 32, TmShape<HD, WM, WK, CLUSTER>::BLO
                             for (int c = 0; c < NT; ++c) {
                                 const uint32_t two = *reinterpret_cast<const uint32_t*>(v + (TMA ? c / 8 * Sh::BLOCK + ((c % 8) ^ (key & 7)) * 16 : c * 16));
                                 const float lo = __uint_as_float(two << 16), hi = __uint_as_float(two & 0xffff0000u);
-                                if (p0 != 0.f) { acc[c][0] = fmaf(p0, lo, acc[c][0]); acc[c][1] = fmaf(p0, hi, acc[c][1]); }
-                                if (p1 != 0.f) { acc[c][2] = fmaf(p1, lo, acc[c][2]); acc[c][3] = fmaf(p1, hi, acc[c][3]); }
+                                const bool odd_lo = (two & 0x7f80u) == 0x7f80u, odd_hi = (two & 0x7f800000u) == 0x7f800000u;
+                                if (p0 != 0.f && odd_lo) acc[c][0] += p0 * lo;
+                                if (p0 != 0.f && odd_hi) acc[c][1] += p0 * hi;
+                                if (p1 != 0.f && odd_lo) acc[c][2] += p1 * lo;
+                                if (p1 != 0.f && odd_hi) acc[c][3] += p1 * hi;
                             }
                         }
             }
@@ -526,14 +547,22 @@ int gb_tree_attention_mma(const TreeArgs& a, const TreePlan& plan, int num_seqs,
     return tm_dispatch<128>(a, plan, num_seqs, max_rows, stream);
 }
 
-constexpr int TREE_TC_ABOVE = 64, TREE_TC_CONTEXT = 512;
+// More than 32 rows, and either many keys in all (of every request and key/value head, times the groups of 64 rows that read them here) or long ones: the kernel
+// on tcgen05 has about 20 us of its own, and less for each key. Measured, this one and that (us): 16 trees of 24 rows, 32/8 heads of 128, behind 250 tokens 33 and
+// 33, 600 41 and 23, 2,400 107 and 57; one of them behind 2,400 23 and 29, 4,800 35 and 31, 9,600 70 and 35; one of 64 rows behind 600 25 and 39, 2,400 57 and 33;
+// 16 trees of 64 rows, 9/3 heads of 64, behind 600 31 and 31, 1,200 43 and 31; 4 of 40 rows, 32/32 heads of 128, behind 600 29 and 21, 2,400 66 and 51.
+constexpr int TREE_TC_ABOVE = 32, TREE_TC_CONTEXT = 4096;
+constexpr long long TREE_TC_KEYS_READ = 112 * 1024;
 
 // Clusters while every item's blocks find room at once, or all tiles evenly among the blocks that do and a second launch that adds up: whichever this estimate
-// has end sooner.
+// has end sooner. Measured, clusters and even (us): 32/32 heads of 64, trees of 5 rows: 1 behind 4,000 tokens 16 and 27, 4 behind 4,000 43 and 41, 16,000 152 and
+// 100, 16 behind 250 16 and 18, 1,000 46 and 41, 64 behind 1,000 114 and 117; of 32 rows: 4 behind 1,000 21 and 31, 16,000 175 and 121. 32/8 heads of 128, trees of
+// 1 row: 1 behind 16,000 53 and 43, 4 57 and 66, 16 200 and 185; of 8 rows: 1 61 and 71, 4 70 and 88, 16 242 and 230.
 TreePlan tree_plan_mma(int num_seqs, int max_rows, int nh, int nkv, int hd, int max_context, int window, bool tc) {
     TreePlan p;
     const long long M = (long long)max_rows * (nh / nkv);
-    if (tc && (hd == 64 || hd == 128) && window == 0 && M > TREE_TC_ABOVE && max_context >= TREE_TC_CONTEXT) {
+    if (tc && (hd == 64 || hd == 128) && window == 0 && M > TREE_TC_ABOVE &&
+        (max_context * gb_ceil_div(M, 128) >= TREE_TC_CONTEXT || max_context * gb_ceil_div(M, 64) * num_seqs * nkv >= TREE_TC_KEYS_READ)) {
         p.tc = true;
         p.same = M <= TREE_TC_ROWS;
         p.blocks = 148;
@@ -547,7 +576,15 @@ TreePlan tree_plan_mma(int num_seqs, int max_rows, int nh, int nkv, int hd, int 
     int c = TM_MAX_CLUSTER;
     while (c > 1 && (items * c > room || tiles < 2 * c)) c /= 2;
     const int even = hd == 64 && p.rows < 128 ? 148 * 4 : room;      // blocks of the even cut
-    const double tile_us = 0.5, waves = (double)((items * c + room - 1) / room), cluster_us = waves * gb_ceil_div(tiles, c) * tile_us, even_us = (double)items * tiles / room * tile_us + 4.0;
+    // microseconds of a tile in a block (what it waits for, or its share of a multiprocessor that moves 6.5 TB/s / 148 and multiplies 32 rows with 64 keys of 64
+    // channels in 0.5), of a block's start, of the second launch, and of the pieces that it adds up
+    auto tile_us = [&](long long blocks) {
+        const double alone = 0.8 + hd / 160.0 + (p.rows > 16 ? 0.25 : 0.0), shared = hd / 64.0 * (p.rows > 16 ? p.rows / 64.0 : 0.37) * gb_ceil_div(blocks, 148);
+        return alone > shared ? alone : shared;
+    };
+    const long long all = items * tiles, cut = gb_ceil_div(all, TREE_LEAST_SHARE) < even ? gb_ceil_div(all, TREE_LEAST_SHARE) : even;
+    const double cluster_us = gb_ceil_div(items * c, room) * (gb_ceil_div(tiles, c) * tile_us(items * c < room ? items * c : room) + 6.0);
+    const double even_us = gb_ceil_div(all, cut) * tile_us(cut) + 6.0 * items / cut + 20.0 + M / 4.0 + 0.3 * M / 16.0 * hd / 64.0 * cut / items;
     p.cluster = cluster_us <= even_us ? c : 0;
     p.blocks = p.cluster ? 0 : even;
     p.floats = p.cluster ? 0 : (items + even) * p.rows * (hd + 2);

@@ -40,7 +40,7 @@ struct __align__(16) Tc5Shared {
     int abort_flag, segs;                 // (segs: negative where the share ends with them)
     int issued[2], consumed[2];
 };
-static_assert(sizeof(Tc5Shared) <= 3072, "shared memory layout");
+static_assert(sizeof(Tc5Shared) <= 3 * 1024, "shared memory layout");
 
 __device__ __forceinline__ uint64_t tc5_desc_mn(uint32_t smem_addr) {      // MN-major B operand: column blocks of 64 channels TC5_BLOCK bytes apart
     uint64_t d = 0;

@@ -2741,12 +2741,19 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vca
           status.data_ptr(), stream)
 
 
-def verify_walks(n: int, num_seqs: int, vocab: int, size: int, drafted: bool) -> bool:
-    """Whether ``verify_tree`` reads only the rows that the walk reaches, one after the other, and not all rows at once."""
-    return n * vocab * size * (2 if drafted else 1) > VERIFY_ROWS_BYTES
+def verify_walks(n: int, num_seqs: int, vocab: int) -> bool:
+    """Whether ``verify_tree`` reads only the rows that the walk reaches, one after the other, and not all rows at once.
+
+    Both are bound by the weights they compute; a step of the walk waits as long as VERIFY_STEP of them take. How far a walk goes is not known here: it is
+    taken to go through half of a tree's rows, seven at most. Measured (us, the walk's rows and all rows; float32, vocabularies of 32,000): 64 trees of 1 row 12
+    and 14, of 8 rows 40 and 34, of 24 33 and 79; 128 trees of 8 rows 48 and 56; 4 of 64 33 and 26; 16 of 64 51 and 55. Of 128,256: 16 trees of 8 rows 43 and
+    36, 64 84 and 93; 4 of 24 37 and 31, 16 37 and 80. With a drafting model's logits, 32,000: 16 trees of 24 rows 139 and 76, 128 of 8 116 and 159.
+    """
+    steps = min((n + num_seqs) / max(2 * num_seqs, 1), 7)
+    return n * vocab >= (steps - 1) * VERIFY_STEP + steps * num_seqs * vocab
 
 
-VERIFY_ROWS_BYTES = 400 << 20
+VERIFY_STEP = 4 << 20
 
 
 def verify_tree(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, seq_first_row: torch.Tensor, uniform: torch.Tensor,
@@ -2786,7 +2793,7 @@ def verify_tree(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tenso
     stream = _here(logits, tokens, parents, seq_first_row, uniform, temperature, path, accepted, next_token, draft_logits)
     _call("gb_verify_tree", logits.data_ptr(), dtype, strides[0], _ptr(draft_logits), 0 if draft_logits is None else draft_logits.stride(0),
           tokens.data_ptr(), parents.data_ptr(), seq_first_row.data_ptr(), uniform.data_ptr(), temperature.data_ptr(), path.data_ptr(), accepted.data_ptr(),
-          next_token.data_ptr(), n, num_seqs, vocab, int(verify_walks(n, num_seqs, vocab, logits.element_size(), draft_logits is not None)), stream)
+          next_token.data_ptr(), n, num_seqs, vocab, int(verify_walks(n, num_seqs, vocab)), stream)
 
 
 def keep_rows(kpool: torch.Tensor, vpool: torch.Tensor, block_tables: torch.Tensor, seq_first_row: torch.Tensor, seq_start_pos: torch.Tensor,

@@ -281,3 +281,88 @@ def test_the_last_page_of_a_large_pool():
             b.dev["tables"][0, i] = pages - 1 - i
     b.dev["k"], b.dev["v"] = k, v
     b.check(b.run())
+
+
+FAR = 1 << 17      # contexts said to be this long
+
+
+@pytest.mark.parametrize("hd,nh,nkv", [(64, 4, 2), (128, 4, 2), (128, 4, 1), (64, 6, 6)])
+@pytest.mark.parametrize("shapes", [[(600, 40)], [(513, 64), (40, 33)], [(127, 64), (128, 1), (129, 50), (0, 64), (1030, 40)], [(-1, 40), (700, 50), (-1, 2)],
+                                    [(640, 128), (640, 100)], [(100, 300)], [(2000, 65), (0, 0), (90, 64)], [(0, 33)], [(5300, 70), (1, 36)]])
+def test_many_rows_said_to_be_far(hd, nh, nkv, shapes):
+    b = Batch(BF, nh, nkv, hd, shapes, seed=hd + nkv + 1)
+    b.check(b.run(reach=FAR))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("nkv", [1, 2])
+@pytest.mark.parametrize("page", [8, 16, 32, 128, 256])
+def test_many_rows_said_to_be_far_and_pages(hd, nkv, page):
+    b = Batch(BF, 4, nkv, hd, [(700, 45), (1300, 33), (5, 40)], page=page, seed=page + 1)
+    b.check(b.run(reach=FAR))
+
+
+@pytest.mark.parametrize("hd,nkv", [(64, 2), (128, 2), (128, 1)])
+@pytest.mark.parametrize("past", [0, 40, 590, 639])
+def test_masked_places_said_to_be_far_hold_anything(hd, nkv, past):
+    rng = random.Random(4)
+    see = plain.ancestors(plain.random_tree(rng, 64, 4))
+    b = Batch(BF, 4, nkv, hd, [(past, 64)], seed=10, see=lambda rng, rows: see)
+    clean = b.run(reach=FAR)
+    where = past + 20
+    page = int(b.dev["tables"][0, where // 16])
+    b.dev["k"][page, :, where % 16] = float("nan")
+    b.dev["v"][page, :, where % 16, 3:5] = float("inf")
+    dirty = b.run(reach=FAR)
+    hit = torch.from_numpy(see[:, 20])
+    assert 0 < hit.sum() < 63
+    assert torch.equal(dirty[:64][~hit], clean[:64][~hit])
+    assert torch.isnan(dirty[:64][hit]).all()
+
+
+@pytest.mark.parametrize("reach", [None, FAR])
+def test_missing_pages_of_many_rows_are_reported(reach):
+    b = Batch(BF, 4, 2, 64, [(300, 64), (700, 40)], seed=5)
+    b.dev["tables"][0, 3] = b.dev["k"].shape[0] + 5
+    out = b.run(reach=reach)
+    assert int(b.status.item()) == 2
+    b.status.zero_()
+    b.shapes = [(-1, 64), (700, 40)]
+    out[:64] = 0
+    b.check(out)
+
+
+@pytest.mark.parametrize("nh,nkv,hd,shapes", [(4, 4, 64, [(2000, 20)] * 40), (3, 1, 64, [(30000, 1)]), (8, 8, 128, [(9000, 1), (7000, 1)]), (6, 6, 32, [(1500, 12)] * 60),
+                                              (6, 6, 96, [(700, 33)] * 30)])
+def test_keys_cut_evenly(nh, nkv, hd, shapes):
+    b = Batch(BF, nh, nkv, hd, shapes, seed=nh)
+    b.check(b.run())
+
+
+def test_two_recorded_calls_that_share_scratch():
+    a, b = Batch(BF, 4, 4, 64, [(3000, 20)] * 20, seed=1), Batch(BF, 8, 2, 128, [(2500, 40), (900, 64)], seed=2)
+    first, second = torch.full((a.n, 256), 7.0, dtype=BF, device=DEV), torch.full((b.n, 1024), 7.0, dtype=BF, device=DEV)
+    qs = a.q.to(DEV), b.q.to(DEV)
+    sizes = [kernels.tree_attention_floats(x.n, x.nh, x.nkv, x.hd, len(x.shapes), x.most, FAR) for x in (a, b)]
+    parts = torch.full((max(max(sizes), 1),), float("nan"), device=DEV)
+
+    def call(x, q, out):
+        d = x.dev
+        kernels.tree_attention(q, out, d["k"], d["v"], d["tables"], d["first"], d["start"], d["pos"], d["bits"], x.most, x.nh, x.nkv, x.hd, x.page, x.scale,
+                               None, FAR, parts, x.status)
+    call(a, qs[0], first)
+    call(b, qs[1], second)
+    torch.cuda.synchronize()
+    graphs = []
+    for x, q, out in ((a, qs[0], first), (b, qs[1], second)):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            call(x, q, out)
+    for _ in range(3):
+        first.fill_(7.0)
+        second.fill_(7.0)
+        parts.fill_(float("nan"))
+        for g in (graphs[0], graphs[1], graphs[0]):
+            g.replay()
+        a.check(first)
+        b.check(second)
