@@ -562,7 +562,7 @@ TreePlan tree_plan_mma(int num_seqs, int max_rows, int nh, int nkv, int hd, int 
     TreePlan p;
     const long long M = (long long)max_rows * (nh / nkv);
     if (tc && (hd == 64 || hd == 128) && window == 0 && M > TREE_TC_ABOVE &&
-        (max_context * gb_ceil_div(M, 128) >= TREE_TC_CONTEXT || max_context * gb_ceil_div(M, 64) * num_seqs * nkv >= TREE_TC_KEYS_READ)) {
+        ((long long)max_context * gb_ceil_div(M, 128) >= TREE_TC_CONTEXT || (double)max_context * gb_ceil_div(M, 64) * num_seqs * nkv >= TREE_TC_KEYS_READ)) {
         p.tc = true;
         p.same = M <= TREE_TC_ROWS;
         p.blocks = 148;
