@@ -4,7 +4,11 @@
 // A block takes 16 RT query rows of a request and key/value head over its share of the keys, 32 at a time from two buffers of shared memory, one of which is
 // filled while the other is worked on. A thread forms the scores of RT rows and 4 keys, and the outputs of these rows at every eighth piece of four channels, so
 // that a number from shared memory meets four others. Masks are looked at only in tiles that reach into the tree or out of a window; where one of these holds a
-// value that is not a finite number, values go to the rows that see them one at a time, so that no weight of zero meets it. What bounds it: the multiply-adds where rows are many, else a block's chain.
+// value that is not a finite number, values go to the rows that see them one at a time, so that no weight of zero meets it. Shares of a request's keys that several
+// blocks have go to the scratch as outputs, maximum and sum, and tree_merge_kernel adds them up.
+//
+// What bounds it: the multiply-adds, and the reads of shared memory that feed them (4 trees of 24 rows, 15/5 heads of 64, behind 1,500 tokens in float32: 57 us, 6
+// TFLOP/s of multiply-adds); of few rows a block's chain.
 #include "tree_attention.cuh"
 
 constexpr int TA_THREADS = 128, TA_KEYS = 32, TA_MAX_HD = 256, TA_PP = TA_KEYS + 4;
@@ -272,12 +276,13 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeArgs a, int n
         if (lane + 32 * c < a.hd) ((T*)a.out)[(size_t)row * a.out_stride + (cell % a.nh) * a.hd + lane + 32 * c] = gb_from_float<T>(v[c] * inv);
 }
 
-// Query rows of a block, up to 64 (32 of heads above 128 channels, whose outputs fill the registers): those that leave few of them empty, and rather more, since
-// the keys that a thread reads meet all of its rows. (72 rows a request and key/value head, 4 requests of 15/5 heads of 64 behind 1,500 keys, float32.)
+// Query rows of a block, up to 48 (32 of heads above 128 channels, whose outputs fill the registers): those that leave few of them empty, and rather more, since
+// the keys that a thread reads meet all of its rows. Measured in float32, blocks of 16 / 32 / 48 / 64 rows (us): 72 rows a request and key/value head, 4 requests
+// of 15/5 heads of 64 behind 1,500 keys 75 / 68 / 67 / 103; 18 rows 43 / 39 / 43 / 66; 33 rows 53 / 54 / 46 / 70; 4 of 80 rows, 32/8 heads of 128, 200 / 174 / 157 / 178.
 static int ta_rows(long long m, int hd) {
     int best = 16;
     double least = 0.0;
-    for (int rows = 16; rows <= (hd > 128 ? 32 : 64); rows += 16) {
+    for (int rows = 16; rows <= (hd > 128 ? 32 : 48); rows += 16) {
         const double cost = (double)gb_ceil_div(m, rows) * rows * (1.0 + 10.0 / rows);
         if (rows == 16 || cost < least) { best = rows; least = cost; }
     }
@@ -301,7 +306,7 @@ static int ta_sized(const TreeArgs& a, int num_seqs, int max_rows, cudaStream_t 
     const int rows = ta_rows((long long)max_rows * (a.nh / a.nkv), a.hd);
     if (rows == 16) return ta_launch<T, 1, PIECES>(a, num_seqs, max_rows, stream);
     if (rows == 32) return ta_launch<T, 2, PIECES>(a, num_seqs, max_rows, stream);
-    if constexpr (PIECES <= 4) return rows == 48 ? ta_launch<T, 3, PIECES>(a, num_seqs, max_rows, stream) : ta_launch<T, 4, PIECES>(a, num_seqs, max_rows, stream);
+    if constexpr (PIECES <= 4) return ta_launch<T, 3, PIECES>(a, num_seqs, max_rows, stream);
     return 1;
 }
 

@@ -11,7 +11,9 @@
 //   warps 2-9   softmax, four a unit, a row a thread; they lay the unit's queries out in shared memory, and write what comes out.
 // Masks are looked at only in the tiles that reach into the tree (bits, 32 keys at a time). There values that are not finite numbers are taken out of shared
 // memory, so that no weight of zero meets them; rows that see such a key get its part one key at a time.
-// What bounds it: memory where rows are few, else a unit's chain. Every wait is bounded: a wait that runs out sets GB_STATUS_WAIT_TIMEOUT and the block winds down.
+// What bounds it: memory where rows are few (1 tree of 26 rows, 32/8 heads of 128, behind 131,071 tokens, 537 MB: 115 us, 4.7 TB/s; a longer context costs 6.6 TB/s
+// of its keys, the rest is the first tiles, a piece's end and the launch that adds up), else a unit's chain (4 trees of 64 rows behind 12,000 tokens, 41 GFLOP:
+// 78 us, 520 TFLOP/s). Every wait is bounded: a wait that runs out sets GB_STATUS_WAIT_TIMEOUT and the block winds down.
 #include "tcgen05.cuh"
 #include "tree_attention.cuh"
 
@@ -611,8 +613,8 @@ static int tc5_launch(const TreeArgs& a, int blocks, int num_seqs, int max_rows,
     e = gb_launch(GB_PDL_ATTENTION, tree_attention_tc_kernel<HD, SAME>, dim3(blocks), dim3(TC5_WARPS * 32), SMEM, stream, mk, mv, a, num_seqs, page_shift);
     GB_REQUIRE(e == cudaSuccess, "gb_tree_attention: launch failed: %s", cudaGetErrorString(e));
     const int rows = SAME ? TC5_M : 2 * TC5_M, pairs = gb_ceil_div((long long)max_rows * (a.nh / a.nkv), rows);
-    // (8 rows a block where that leaves few of them)
-    const bool fine = (long long)pairs * a.nkv * num_seqs * (rows / 8) <= 8 * 148;
+    // 8 rows a block, else 32, where that leaves few of them: 1 tree of 64 rows, 32/8 heads of 128, behind 5,800 tokens 43 and 45 us, 4 behind 12,000 89 and 80
+    const bool fine = (long long)pairs * a.nkv * num_seqs * (rows / 8) <= 4 * 148;
     const dim3 grid(pairs * a.nkv * (rows / (fine ? 8 : 32)), num_seqs);
     e = gb_launch(GB_PDL_ATTENTION, fine ? tree_tc_pieces_kernel<HD, SAME, 8> : tree_tc_pieces_kernel<HD, SAME, 32>, grid, dim3(256), 0, stream, a, num_seqs, pairs, blocks);
     GB_REQUIRE(e == cudaSuccess, "gb_tree_attention: launch failed: %s", cudaGetErrorString(e));
