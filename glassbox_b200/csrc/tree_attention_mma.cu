@@ -10,8 +10,8 @@
 // number must not meet a weight of zero, so such values are zero in the product and go to the rows that see them one by one.
 //
 // What bounds it: keys and values are read once, 256 bytes of them for a row's 128 products and an exponential. 16 trees of 32 rows, 32/32 heads of 64, behind
-// 4,095 tokens (541 MB): 129 us, 4.2 TB/s; there tensor cores, exponentials and shared memory are each about half busy, and a block has about 7 us of a start and an end
-// beside each item. Where items are few, that and a tile's trip: 1 tree of 26 rows, 9/3 heads of 64, behind 1,000 tokens 10 us.
+// 4,095 tokens (541 MB): 129 us, 4.2 TB/s; there a warp's chain of scores, softmax and product, of which a multiprocessor has 16 under way (1.9 instructions a cycle, tensor
+// cores 28 % busy), and about 7 us of a start and an end beside each item. Where items are few, that and a tile's trip: 1 tree of 26 rows, 9/3 heads of 64, behind 1,000 tokens 10 us.
 #include "tcgen05.cuh"
 #include "tree_attention.cuh"
 
@@ -552,8 +552,15 @@ int gb_tree_attention_mma(const TreeArgs& a, const TreePlan& plan, int num_seqs,
 // on tcgen05 has about 20 us of its own, and less for each key. Measured, this one and that (us): 16 trees of 24 rows, 32/8 heads of 128, behind 250 tokens 33 and
 // 33, 600 41 and 23, 2,400 107 and 57; one of them behind 2,400 23 and 29, 4,800 35 and 31, 9,600 70 and 35; one of 64 rows behind 600 25 and 39, 2,400 57 and 33;
 // 16 trees of 64 rows, 9/3 heads of 64, behind 600 31 and 31, 1,200 43 and 31; 4 of 40 rows, 32/32 heads of 128, behind 600 29 and 21, 2,400 66 and 51.
-constexpr int TREE_TC_ABOVE = 32, TREE_TC_CONTEXT = 4096;
-constexpr long long TREE_TC_KEYS_READ = 112 * 1024;
+// With fewer query rows half of that kernel's work is on empty ones, and memory feeds either; it is ahead with long keys of few requests and heads, which clusters
+// of eight blocks leave part of the GPU without (8 rows, 15/5 heads of 64, behind 4,095 tokens 16 and 23, 16,000 41 and 26, 64,000 74 and 39; 4 requests behind
+// 16,000 45 and 33; 32/32 heads 45 and 47), and with 17 rows or more of 128 channels, whose products bound this kernel (32 rows, 32/8 heads, 4 requests behind
+// 4,095 27 and 33, 16,000 69 and 65, 64,000 236 and 185; 16 rows 201 and 185).
+static bool tree_takes_tc(int num_seqs, long long M, int nkv, int hd, int max_context) {
+    const double keys = (double)max_context * num_seqs * nkv;
+    if (M > 32) return (long long)max_context * gb_ceil_div(M, 128) >= 4096 || keys * gb_ceil_div(M, 64) >= 112 * 1024;
+    return (max_context >= 8192 && num_seqs * nkv <= 24) || (hd == 128 && M > 16 && keys >= 512 * 1024);
+}
 
 // Clusters while every item's blocks find room at once, or all tiles evenly among the blocks that do and a second launch that adds up: whichever this estimate
 // has end sooner. Measured, clusters and even (us): 32/32 heads of 64, trees of 5 rows: 1 behind 4,000 tokens 16 and 27, 4 behind 4,000 43 and 41, 16,000 152 and
@@ -562,8 +569,7 @@ constexpr long long TREE_TC_KEYS_READ = 112 * 1024;
 TreePlan tree_plan_mma(int num_seqs, int max_rows, int nh, int nkv, int hd, int max_context, int window, bool tc) {
     TreePlan p;
     const long long M = (long long)max_rows * (nh / nkv);
-    if (tc && (hd == 64 || hd == 128) && window == 0 && M > TREE_TC_ABOVE &&
-        ((long long)max_context * gb_ceil_div(M, 128) >= TREE_TC_CONTEXT || (double)max_context * gb_ceil_div(M, 64) * num_seqs * nkv >= TREE_TC_KEYS_READ)) {
+    if (tc && (hd == 64 || hd == 128) && window == 0 && tree_takes_tc(num_seqs, M, nkv, hd, max_context)) {
         p.tc = true;
         p.same = M <= TREE_TC_ROWS;
         p.blocks = 148;

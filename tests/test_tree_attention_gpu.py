@@ -366,3 +366,10 @@ def test_two_recorded_calls_that_share_scratch():
             g.replay()
         a.check(first)
         b.check(second)
+
+
+@pytest.mark.parametrize("nh,nkv,hd", [(9, 3, 64), (4, 2, 128), (6, 6, 64), (2, 2, 128)])
+@pytest.mark.parametrize("shapes", [[(9000, 1)], [(8300, 7), (40, 3)], [(0, 1), (128, 8), (127, 5)], [(-1, 3), (511, 2), (0, 0), (6, 6)]])
+def test_few_rows_said_to_be_far(nh, nkv, hd, shapes):
+    b = Batch(BF, nh, nkv, hd, shapes, seed=hd + nkv + 2)
+    b.check(b.run(reach=FAR))
