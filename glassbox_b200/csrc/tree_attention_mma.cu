@@ -356,10 +356,11 @@ __global__ void __launch_bounds__(WM* WK * 32, TmShape<HD, WM, WK, CLUSTER>::BLO
         // A pair of channels of every parts-th row; all loads of other blocks' results come first: one trip.
         auto add_up = [&](auto blocks) {
             constexpr int MOST = decltype(blocks)::value;
-            for (int i = tid; i < (Sh::ROWS - rank + MOST - 1) / MOST * (HD / 2); i += Sh::THREADS) {
-                const int r = i / (HD / 2) * MOST + rank, c = i % (HD / 2) * 2, m = m0 + r;
+            constexpr int E = MOST * WK <= 2 ? 4 : MOST * WK <= 8 ? 2 : 1, LANES = HD / 2 / E;      // pairs of a thread, LANES pairs apart: as many as its registers hold
+            for (int i = tid; i < (Sh::ROWS - rank + MOST - 1) / MOST * LANES; i += Sh::THREADS) {
+                const int r = i / LANES * MOST + rank, c = i % LANES * 2, m = m0 + r;
                 if (m >= M) break;
-                float2 ml[MOST][WK], v[MOST][WK];
+                float2 ml[MOST][WK], v[MOST][WK][E];
 #pragma unroll
                 for (int b = 0; b < MOST; ++b) {
                     const float* all = MOST > 1 ? cg::this_cluster().map_shared_rank(res, b) : res;
@@ -367,10 +368,13 @@ __global__ void __launch_bounds__(WM* WK * 32, TmShape<HD, WM, WK, CLUSTER>::BLO
                     for (int w = 0; w < WK; ++w) {
                         const float* from = all + ((size_t)w * Sh::ROWS + r) * P;
                         ml[b][w] = *reinterpret_cast<const float2*>(from + HD);
-                        v[b][w] = *reinterpret_cast<const float2*>(from + c);
+#pragma unroll
+                        for (int e = 0; e < E; ++e) v[b][w][e] = *reinterpret_cast<const float2*>(from + c + 2 * LANES * e);
                     }
                 }
-                float top = -INFINITY, l = 0.f, x = 0.f, y = 0.f;
+                float top = -INFINITY, l = 0.f, x[E], y[E];
+#pragma unroll
+                for (int e = 0; e < E; ++e) x[e] = y[e] = 0.f;
 #pragma unroll
                 for (int b = 0; b < MOST; ++b)
 #pragma unroll
@@ -382,15 +386,21 @@ __global__ void __launch_bounds__(WM* WK * 32, TmShape<HD, WM, WK, CLUSTER>::BLO
                     for (int w = 0; w < WK; ++w) {
                         const float f = tm_exp2(ml[b][w].x - o);
                         l = fmaf(ml[b][w].y, f, l);
-                        x = fmaf(v[b][w].x, f, x);
-                        y = fmaf(v[b][w].y, f, y);
+#pragma unroll
+                        for (int e = 0; e < E; ++e) {
+                            x[e] = fmaf(v[b][w][e].x, f, x[e]);
+                            y[e] = fmaf(v[b][w][e].y, f, y[e]);
+                        }
                     }
                 if (CLUSTER || tile1 - tile0 == tiles_all) {
                     const float inv = l != 0.f ? 1.0f / l : 0.f;
-                    *reinterpret_cast<uint32_t*>(out + (size_t)(s.row0 + m / G) * a.out_stride + (kvh * G + m % G) * HD + c) = tm_pack(x * inv, y * inv);
+                    __nv_bfloat16* to = out + (size_t)(s.row0 + m / G) * a.out_stride + (kvh * G + m % G) * HD + c;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) *reinterpret_cast<uint32_t*>(to + 2 * LANES * e) = tm_pack(x[e] * inv, y[e] * inv);
                 } else {
                     float* part = a.parts + ((size_t)piece * Sh::ROWS + r) * P;
-                    *reinterpret_cast<float2*>(part + c) = make_float2(x, y);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) *reinterpret_cast<float2*>(part + c + 2 * LANES * e) = make_float2(x[e], y[e]);
                     if (c == 0) *reinterpret_cast<float2*>(part + HD) = make_float2(top, l);
                 }
             }
