@@ -11,7 +11,7 @@
 //
 // What bounds it: keys and values are read once, 256 bytes of them for a row's 128 products and an exponential. 16 trees of 32 rows, 32/32 heads of 64, behind
 // 4,095 tokens (541 MB): 129 us, 4.2 TB/s; there a warp's chain of scores, softmax and product, of which a multiprocessor has 16 under way (1.9 instructions a cycle, tensor
-// cores 28 % busy), and about 7 us of a start and an end beside each item. Where items are few, that and a tile's trip: 1 tree of 26 rows, 9/3 heads of 64, behind 1,000 tokens 10 us.
+// cores 28 % busy), and about 7 us of a start and an end beside each item. Where items are few, that and a tile's trip: 1 tree of 8 rows, 9/3 heads of 64, behind 1,023 tokens 10 us.
 #include "tcgen05.cuh"
 #include "tree_attention.cuh"
 

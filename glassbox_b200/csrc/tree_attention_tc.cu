@@ -12,7 +12,7 @@
 // Masks are looked at only in the tiles that reach into the tree (bits, 32 keys at a time). There values that are not finite numbers are taken out of shared
 // memory, so that no weight of zero meets them; rows that see such a key get its part one key at a time.
 // What bounds it: memory where rows are few (1 tree of 26 rows, 32/8 heads of 128, behind 131,071 tokens, 537 MB: 115 us, 4.7 TB/s; a longer context costs 6.6 TB/s
-// of its keys, the rest is the first tiles, a piece's end and the launch that adds up), else a unit's chain (4 trees of 64 rows behind 12,000 tokens, 41 GFLOP:
+// of its keys, the rest is the first tiles, a piece's end and the launch that adds up), else a unit's chain (4 trees of 64 rows behind 8,000 to 16,001 tokens, 41 GFLOP:
 // 78 us, 520 TFLOP/s). Every wait is bounded: a wait that runs out sets GB_STATUS_WAIT_TIMEOUT and the block winds down.
 #include "tcgen05.cuh"
 #include "tree_attention.cuh"
