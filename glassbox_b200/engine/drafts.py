@@ -127,7 +127,8 @@ def generate(engine: Engine, prompts: Sequence[Sequence[int]], max_tokens: int, 
              max_seqs: Optional[int] = None) -> Tuple[List[List[int]], List[str], DraftCounts]:
     """Generate after each prompt with ``drafts`` (a ``PromptLookup`` or ``DraftModel``); request i samples with seed ``config.seed + i``. Returns the new tokens and
     why each request ended, in the order given, and how the drafts fared. Prompts are read one by one, all running requests go through the model in one
-    step. When pages run out drafts go first, then the request that was admitted last waits and is read again."""
+    step. When pages run out drafts go first, then the request that was admitted last waits and is read again; one that does not fit by itself ends by its
+    length, or raises ``OutOfPages`` where other requests of the engine hold slots or pages."""
     if config.needs_host:
         raise ValueError("drafted generation is greedy or at a temperature: top_k, top_p, min_p and repetition_penalty are not built for it")
     if not engine.model.takes_trees:
@@ -153,6 +154,11 @@ def generate(engine: Engine, prompts: Sequence[Sequence[int]], max_tokens: int, 
         if engine.cache.has(t.rid):
             engine.free_request(t.rid)
         drafts.drop(t.rid)
+
+    def others() -> bool:
+        """Whether requests that are not of this run hold slots and pages: what does not fit may fit without them."""
+        mine = {t.rid for t in texts}
+        return any(rid not in mine for rid in engine.cache.request_ids())
 
     def read(t: _Text) -> None:
         """All of a text but its last token into the cache."""
@@ -199,6 +205,8 @@ def generate(engine: Engine, prompts: Sequence[Sequence[int]], max_tokens: int, 
                 try:
                     read(t)
                 except OutOfPages:
+                    if not running and others():
+                        raise
                     leave(t, LENGTH if not running else None)      # alone it is too long for the cache
                     if running:
                         break
@@ -221,7 +229,10 @@ def generate(engine: Engine, prompts: Sequence[Sequence[int]], max_tokens: int, 
                         continue
                     t = running.pop()
                     if not running:
+                        crowded = others()
                         leave(t, LENGTH)
+                        if crowded:
+                            raise
                         break
                     leave(t, None)
                     waiting.appendleft(t)

@@ -253,3 +253,25 @@ def test_command_line(model_dirs):
         assert r.returncode == 0, r.stderr
     assert runs[0].stdout == runs[1].stdout == runs[2].stdout
     assert "drafted tokens accepted" in runs[1].stderr and "drafted tokens accepted" in runs[2].stderr
+
+
+@pytest.mark.parametrize("held", ["pages", "slots", "pages later"])
+def test_beside_requests_that_hold_the_cache(model_dirs, held):
+    """What does not fit because of others is an error, and no text that ends early."""
+    from glassbox_b200.cache.manager import OutOfPages
+    from glassbox_b200.engine.drafts import PromptLookup, generate
+    from glassbox_b200.engine.engine import StepEntry
+    from glassbox_b200.sampling.sampler import SamplerConfig
+    eng = make_engine(model_dirs("A", "float32"), "float32", cache_tokens=128, max_requests=1 if held == "slots" else 4)
+    page = eng.page_size
+    total = sum(eng.cache.free_pages(g) for g in range(1)) * page
+    other = [1 + i % 7 for i in range(total - {"pages": 1, "slots": total - 3, "pages later": 2 * page + 1}[held])]
+    eng.add_request("other")
+    for a in range(0, len(other), 64):
+        eng.step([StepEntry("other", other[a:a + 64])])
+    with pytest.raises(OutOfPages):
+        generate(eng, [[3, 4, 5, 3, 4]], 100, PromptLookup(3), SamplerConfig(temperature=0.0))
+    assert eng.cache.request_ids() == ["other"] and eng.length("other") == len(other)
+    eng.free_request("other")
+    tokens, reasons, _ = generate(eng, [[3, 4, 5, 3, 4]], 5, PromptLookup(3), SamplerConfig(temperature=0.0))
+    assert len(tokens[0]) == 5 and reasons == ["length"]
