@@ -16,9 +16,20 @@ import torch
 
 from .. import kernels
 from ..cache.manager import OutOfPages
-from ..sampling.sampler import Rng, Sampler, SamplerConfig
+from ..sampling.sampler import Sampler, SamplerConfig
 from .engine import Engine, StepEntry
 from .scheduler import LENGTH, STOP
+
+
+_DRAFTS, _COINS = 1, 2
+
+
+def _numbers(what: int, seeds: Sequence[int], at: int, count: int) -> np.ndarray:
+    """``count`` random numbers in [0, 1) for one use, by a request whose text has ``at`` tokens: a stream for each use, seeds and place, of a generator that is
+    not the one that requests draw their tokens with. Rejection holds only where what was drafted, the coins that take it and what is drawn in its place are
+    independent, also where all seeds are equal."""
+    words = [half for s in seeds for half in (int(s) & 0xFFFFFFFF, int(s) >> 32 & 0xFFFFFFFF)]
+    return np.random.default_rng([what, at] + words).random(count, dtype=np.float32)
 
 
 class PromptLookup:
@@ -59,15 +70,18 @@ class PromptLookup:
 
 class DraftModel:
     """Drafts from a smaller model: ``tokens`` of them, written one after another by ``engine`` (an ``Engine`` of a model with the same vocabulary, used for
-    nothing else meanwhile), greedily for greedy requests, else drawn at the request's temperature by random numbers of its own (``seed``)."""
+    nothing else meanwhile), greedily for greedy requests, else drawn at the request's temperature by random numbers that are none of the request's own: they
+    follow from ``seed``, the request's seed and its text's length, so a run with the same seeds drafts the same."""
 
     def __init__(self, engine: Engine, tokens: int = 4, seed: int = 0):
         if tokens < 1:
             raise ValueError("a drafting model needs to write at least one token")
-        self.engine, self.tokens, self.rng = engine, int(tokens), Rng(seed)
+        self.engine, self.tokens, self.seed = engine, int(tokens), int(seed)
 
-    def propose_all(self, rids: Sequence[object], texts: Sequence[Sequence[int]], rooms: Sequence[int], temperatures: Sequence[float]):
-        """For each request ``(tokens, parents)`` as ``PromptLookup.propose``, and of all rows the logits that their children were drawn from."""
+    def propose_all(self, rids: Sequence[object], texts: Sequence[Sequence[int]], rooms: Sequence[int], temperatures: Sequence[float],
+                    seeds: Sequence[int]):
+        """For each request ``(tokens, parents)`` as ``PromptLookup.propose``, and of all rows the logits that their children were drawn from. ``seeds`` of the
+        requests."""
         engine = self.engine
         for rid, text in zip(rids, texts):
             if not engine.cache.has(rid):
@@ -87,12 +101,13 @@ class DraftModel:
         logits = torch.zeros(int(firsts[-1]), engine.config.vocab_size, device=engine.device)
         drafts = [[int(text[-1])] for text in texts]
         heat = torch.tensor(temperatures, dtype=torch.float32)
+        numbers = [_numbers(_DRAFTS, (self.seed, seed), len(text), c) for seed, text, c in zip(seeds, texts, counts)]
         for i in range(max(counts, default=0)):
             live = [j for j, c in enumerate(counts) if c > i]
             rows = engine.step([StepEntry(rids[j], [drafts[j][-1]], [0]) for j in live])
             logits.index_copy_(0, torch.tensor([int(firsts[j]) + i for j in live], device=engine.device), rows)
             picked = torch.empty(len(live), dtype=torch.int32, device=engine.device)
-            draws = torch.tensor([self.rng.next_f32() for _ in live], dtype=torch.float32).to(engine.device)
+            draws = torch.tensor([float(numbers[j][i]) for j in live], dtype=torch.float32).to(engine.device)
             kernels.sample(rows, picked, heat[live].to(engine.device), draws)
             for j, t in zip(live, picked.tolist()):
                 drafts[j].append(t)
@@ -170,7 +185,8 @@ def generate(engine: Engine, prompts: Sequence[Sequence[int]], max_tokens: int, 
         rooms = [max(0, min(room, max_tokens - (len(t.tokens) - t.prompt) - 1, limit - len(t.tokens))) for t in running]
         if isinstance(drafts, DraftModel) and max(rooms) > 0:
             try:
-                trees, logits = drafts.propose_all([t.rid for t in running], [t.tokens for t in running], rooms, [config.temperature] * len(running))
+                trees, logits = drafts.propose_all([t.rid for t in running], [t.tokens for t in running], rooms, [config.temperature] * len(running),
+                                                   [t.sampler.config.seed for t in running])
                 return trees, None if config.greedy else logits
             except OutOfPages:                           # (of the drafting model: it begins anew with the next step)
                 for t in running:
@@ -179,7 +195,7 @@ def generate(engine: Engine, prompts: Sequence[Sequence[int]], max_tokens: int, 
 
     def numbers(trees) -> Optional[np.ndarray]:
         """The requests' random numbers: a row's second one is that of the token behind it, counted from the text's end, so that what is drawn
-        does not depend on what was drafted; the first ones, of drafts with a distribution, come behind those."""
+        does not depend on what was drafted; the first ones, coins for drafts with a distribution, are of a generator of their own."""
         if config.greedy:
             return None
         parts = []
@@ -189,11 +205,10 @@ def generate(engine: Engine, prompts: Sequence[Sequence[int]], max_tokens: int, 
                 depth.append(depth[p] + 1 if depth else 0)
             while len(t.draws) <= max(depth):
                 t.draws.append(t.sampler.rng.next_f32())
-            coins = [coin.next_f32() for _ in parents]
-            parts.append(np.stack([np.array(coins, np.float32), np.array([t.draws[d] for d in depth], np.float32)], axis=1))
+            coins = _numbers(_COINS, (t.sampler.config.seed,), len(t.tokens), len(parents))
+            parts.append(np.stack([coins, np.array([t.draws[d] for d in depth], np.float32)], axis=1))
         return np.concatenate(parts)
 
-    coin = Rng(config.seed ^ 0x5DEECE66D)
     try:
         while waiting or running:
             while waiting and len(running) < most:
