@@ -84,18 +84,7 @@ class DraftModel:
         requests."""
         engine = self.engine
         for rid, text in zip(rids, texts):
-            if not engine.cache.has(rid):
-                engine.add_request(rid, list(text))
-            held = engine.cache.tokens(rid)[:engine.length(rid)]
-            same = 0
-            limit = min(len(held), len(text) - 1)
-            if limit:
-                differ = np.nonzero(np.asarray(held[:limit]) != np.asarray(text[:limit]))[0]
-                same = int(differ[0]) if len(differ) else limit
-            if same < len(held):
-                engine.cache.truncate(rid, same)         # (what was drafted and not kept)
-            for a in range(same, len(text) - 1, engine.max_batch_tokens):
-                engine.step([StepEntry(rid, list(text[a:min(a + engine.max_batch_tokens, len(text) - 1)]))])
+            self._catch_up(rid, text)
         counts = [max(0, min(self.tokens, room, engine.max_position - len(text))) for room, text in zip(rooms, texts)]
         firsts = np.concatenate([[0], np.cumsum([c + 1 for c in counts])])
         logits = torch.zeros(int(firsts[-1]), engine.config.vocab_size, device=engine.device)
@@ -112,6 +101,32 @@ class DraftModel:
             for j, t in zip(live, picked.tolist()):
                 drafts[j].append(t)
         return [(d, list(range(-1, len(d) - 1))) for d in drafts], logits
+
+    def _catch_up(self, rid, text: Sequence[int]) -> None:
+        """The request's cache holds all of the text but its last token. What was drafted and not kept is taken back; where that cannot be (a state has taken it in,
+        a window has given back the pages before it) the text is read anew."""
+        engine = self.engine
+        if not engine.cache.has(rid):
+            engine.add_request(rid, list(text))
+        held = engine.cache.tokens(rid)[:engine.length(rid)]
+        same = limit = min(len(held), len(text) - 1)
+        if limit:
+            differ = np.nonzero(np.asarray(held[:limit]) != np.asarray(text[:limit]))[0]
+            same = int(differ[0]) if len(differ) else limit
+        if same < len(held) and not self._take_back(rid, same):
+            engine.free_request(rid)
+            engine.add_request(rid, list(text))
+        for a in range(engine.length(rid), len(text) - 1, engine.max_batch_tokens):
+            engine.step([StepEntry(rid, list(text[a:min(a + engine.max_batch_tokens, len(text) - 1)]))])
+
+    def _take_back(self, rid, length: int) -> bool:
+        if self.engine.device_cache.has_state:
+            return False
+        try:
+            self.engine.cache.truncate(rid, length)
+        except ValueError:                               # (of pages that are gone, before anything changes)
+            return False
+        return True
 
     def drop(self, rid) -> None:
         if self.engine.cache.has(rid):

@@ -1,0 +1,70 @@
+"""Drafted generation on the CPU, with stand-ins for the engines: drafting models of other kinds than the model they draft for, and what happens when something
+runs out."""
+import numpy as np
+import pytest
+
+import draft_fakes as fakes
+import tree_plain as plain
+from glassbox_b200.engine import drafts
+from glassbox_b200.sampling.sampler import Sampler, SamplerConfig
+
+VOCAB = 11
+
+
+@pytest.fixture(autouse=True)
+def on_the_cpu(monkeypatch):
+    monkeypatch.setattr(drafts.kernels, "sample", fakes.sample)
+
+
+def likes(text):
+    return (sum(text) * 7 + len(text) * 3 + text[-1]) % VOCAB
+
+
+def logits_of(text):
+    x = np.cos(np.arange(VOCAB) * (1 + likes(text)))
+    x[likes(text)] = 2.0
+    return x
+
+
+def nearly(text):
+    """A drafting model that is wrong behind every third text or so."""
+    x = logits_of(text)
+    if (sum(text) + len(text)) % 3 == 0:
+        x[(likes(text) + 1) % VOCAB] = 3.0
+    return x
+
+
+def alone(prompt, count, temperature, seed, most=64):
+    """The text that comes token by token."""
+    text, rng = list(prompt), Sampler(SamplerConfig(seed=seed)).rng
+    while len(text) < len(prompt) + count and (len(text) < most or len(text) == len(prompt)):
+        x = logits_of(text).astype(np.float32)
+        text.append(plain.draw(plain.softmax(x, temperature), rng.next_f32()) if temperature > 0 else int(x.argmax()))
+    return text[len(prompt):]
+
+
+PROMPTS = [[1, 2, 3, 4, 5], [6], [7, 8, 9, 1, 2, 3, 4, 5, 6]]
+
+
+def run(model, target=None, prompts=PROMPTS, count=30, temperature=0.0, **kw):
+    target = target or fakes.FakeEngine(VOCAB, logits_of)
+    outs, reasons, counts = drafts.generate(target, prompts, count, model, SamplerConfig(temperature=temperature, seed=3), **kw)
+    assert not target.cache.request_ids()
+    if isinstance(model, drafts.DraftModel):
+        assert not model.engine.cache.request_ids()
+    return outs, counts
+
+
+def small(**kw):
+    return drafts.DraftModel(fakes.FakeEngine(VOCAB, nearly, **kw), tokens=4)
+
+
+@pytest.mark.parametrize("kind", [dict(state=True), dict(window=3, page_size=2), dict(window=3, page_size=2, state=True)])
+@pytest.mark.parametrize("temperature", [0.0, 0.7])
+def test_models_that_cannot_go_back_draft_alike(kind, temperature):
+    """What was drafted and not kept is no part of what comes next, whatever the drafting model carries along."""
+    want, plain_counts = run(small(), temperature=temperature)
+    got, counts = run(small(**kind), temperature=temperature)
+    assert got == want and counts == plain_counts and 0 < counts.accepted < counts.drafted
+    if not temperature:
+        assert got == [alone(p, 30, 0.0, 0) for p in PROMPTS]
