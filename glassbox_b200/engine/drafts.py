@@ -83,9 +83,12 @@ class DraftModel:
         """For each request ``(tokens, parents)`` as ``PromptLookup.propose``, and of all rows the logits that their children were drawn from. ``seeds`` of the
         requests."""
         engine = self.engine
-        for rid, text in zip(rids, texts):
-            self._catch_up(rid, text)
         counts = [max(0, min(self.tokens, room, engine.max_position - len(text))) for room, text in zip(rooms, texts)]
+        for rid, text, count in zip(rids, texts, counts):
+            if count:
+                self._catch_up(rid, text)
+            elif len(text) >= engine.max_position:       # (a text that its context does not hold)
+                self.drop(rid)
         firsts = np.concatenate([[0], np.cumsum([c + 1 for c in counts])])
         logits = torch.zeros(int(firsts[-1]), engine.config.vocab_size, device=engine.device)
         drafts = [[int(text[-1])] for text in texts]

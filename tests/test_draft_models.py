@@ -68,3 +68,11 @@ def test_models_that_cannot_go_back_draft_alike(kind, temperature):
     assert got == want and counts == plain_counts and 0 < counts.accepted < counts.drafted
     if not temperature:
         assert got == [alone(p, 30, 0.0, 0) for p in PROMPTS]
+
+
+def test_a_drafting_model_of_a_shorter_context():
+    got, counts = run(small(max_position=16))
+    assert got == [alone(p, 30, 0.0, 0) for p in PROMPTS] and counts.accepted > 0
+    got, counts = run(small(max_position=4))
+    assert got == [alone(p, 30, 0.0, 0) for p in PROMPTS]
+    assert drafts.generate(fakes.FakeEngine(VOCAB, logits_of), PROMPTS, 30, small(max_position=16), SamplerConfig(temperature=0.7))[0]
