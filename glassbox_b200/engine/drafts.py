@@ -95,14 +95,16 @@ class DraftModel:
         heat = torch.tensor(temperatures, dtype=torch.float32)
         numbers = [_numbers(_DRAFTS, (self.seed, seed), len(text), c) for seed, text, c in zip(seeds, texts, counts)]
         for i in range(max(counts, default=0)):
-            live = [j for j, c in enumerate(counts) if c > i]
-            rows = engine.step([StepEntry(rids[j], [drafts[j][-1]], [0]) for j in live])
-            logits.index_copy_(0, torch.tensor([int(firsts[j]) + i for j in live], device=engine.device), rows)
-            picked = torch.empty(len(live), dtype=torch.int32, device=engine.device)
-            draws = torch.tensor([float(numbers[j][i]) for j in live], dtype=torch.float32).to(engine.device)
-            kernels.sample(rows, picked, heat[live].to(engine.device), draws)
-            for j, t in zip(live, picked.tolist()):
-                drafts[j].append(t)
+            every = [j for j, c in enumerate(counts) if c > i]
+            for a in range(0, len(every), engine.max_batch_tokens):
+                live = every[a:a + engine.max_batch_tokens]
+                rows = engine.step([StepEntry(rids[j], [drafts[j][-1]], [0]) for j in live])
+                logits.index_copy_(0, torch.tensor([int(firsts[j]) + i for j in live], device=engine.device), rows)
+                picked = torch.empty(len(live), dtype=torch.int32, device=engine.device)
+                draws = torch.tensor([float(numbers[j][i]) for j in live], dtype=torch.float32).to(engine.device)
+                kernels.sample(rows, picked, heat[live].to(engine.device), draws)
+                for j, t in zip(live, picked.tolist()):
+                    drafts[j].append(t)
         return [(d, list(range(-1, len(d) - 1))) for d in drafts], logits
 
     def _catch_up(self, rid, text: Sequence[int]) -> None:

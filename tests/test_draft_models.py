@@ -76,3 +76,11 @@ def test_a_drafting_model_of_a_shorter_context():
     got, counts = run(small(max_position=4))
     assert got == [alone(p, 30, 0.0, 0) for p in PROMPTS]
     assert drafts.generate(fakes.FakeEngine(VOCAB, logits_of), PROMPTS, 30, small(max_position=16), SamplerConfig(temperature=0.7))[0]
+
+
+@pytest.mark.parametrize("budget", [1, 2, 3])
+def test_a_drafting_model_of_a_small_budget(budget):
+    want, plain_counts = run(small())
+    assert run(small(budget=budget)) == (want, plain_counts)
+    want = run(small(), temperature=0.7)
+    assert run(small(budget=budget), temperature=0.7) == want
