@@ -207,7 +207,8 @@ def generate(engine: Engine, prompts: Sequence[Sequence[int]], max_tokens: int, 
             try:
                 trees, logits = drafts.propose_all([t.rid for t in running], [t.tokens for t in running], rooms, [config.temperature] * len(running),
                                                    [t.sampler.config.seed for t in running])
-                return trees, None if config.greedy else logits
+                # (without drafts there is nothing that came from a distribution)
+                return trees, None if config.greedy or all(len(tokens) == 1 for tokens, _ in trees) else logits
             except OutOfPages:                           # (of the drafting model: it begins anew with the next step)
                 for t in running:
                     drafts.drop(t.rid)

@@ -84,3 +84,11 @@ def test_a_drafting_model_of_a_small_budget(budget):
     assert run(small(budget=budget)) == (want, plain_counts)
     want = run(small(), temperature=0.7)
     assert run(small(budget=budget), temperature=0.7) == want
+
+
+def test_pages_run_out_where_nothing_was_drafted():
+    """The drafting model is at its last position; the last request waits and is read again."""
+    prompts = [[1, 2, 3, 4, 5, 6, 7, 8, 9], [9, 8, 7, 6, 5, 4, 3, 2, 1]]
+    few = fakes.FakeEngine(VOCAB, logits_of, pages=5, page_size=4)
+    got, _ = run(small(max_position=9), few, prompts, 3, 0.7)
+    assert got == [alone(p, 3, 0.7, 3 + i) for i, p in enumerate(prompts)]
