@@ -234,7 +234,7 @@ def generate(engine: Engine, prompts: Sequence[Sequence[int]], max_tokens: int, 
         while waiting or running:
             while waiting and len(running) < most:
                 t = waiting[0]
-                if max_tokens <= len(t.tokens) - t.prompt or len(t.tokens) >= limit:
+                if max_tokens <= len(t.tokens) - t.prompt or len(t.tokens) > limit:
                     waiting.popleft()
                     leave(t, LENGTH)
                     continue

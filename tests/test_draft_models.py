@@ -92,3 +92,14 @@ def test_pages_run_out_where_nothing_was_drafted():
     few = fakes.FakeEngine(VOCAB, logits_of, pages=5, page_size=4)
     got, _ = run(small(max_position=9), few, prompts, 3, 0.7)
     assert got == [alone(p, 3, 0.7, 3 + i) for i, p in enumerate(prompts)]
+
+
+@pytest.mark.parametrize("temperature", [0.0, 0.7])
+def test_a_prompt_that_fills_the_context(temperature):
+    """One token follows it, as without drafts."""
+    prompts = [[1 + i % 9 for i in range(n)] for n in (16, 15, 14)]
+    full = lambda: fakes.FakeEngine(VOCAB, logits_of, max_position=16)
+    want = [alone(p, 30, temperature, 3 + i, most=16) for i, p in enumerate(prompts)]
+    assert [len(w) for w in want] == [1, 1, 2]
+    assert run(drafts.PromptLookup(), full(), prompts, temperature=temperature)[0] == want
+    assert run(small(max_position=16), full(), prompts, temperature=temperature)[0] == want
