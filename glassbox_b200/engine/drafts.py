@@ -168,12 +168,13 @@ def generate(engine: Engine, prompts: Sequence[Sequence[int]], max_tokens: int, 
         raise ValueError("drafted generation is greedy or at a temperature: top_k, top_p, min_p and repetition_penalty are not built for it")
     if not engine.model.takes_trees:
         raise ValueError(f"{engine.config.architecture} takes no drafted trees with this cache (a part carries something from row to row, or the cache holds 4 bits)")
+    most = min(max_seqs or engine.max_requests, engine.max_requests, engine.max_batch_tokens)      # requests that run at once
     if isinstance(drafts, DraftModel):
         if drafts.engine is engine:
             raise ValueError("a model cannot draft for itself")
         if drafts.engine.config.vocab_size != engine.config.vocab_size:
             raise ValueError(f"the drafting model knows {drafts.engine.config.vocab_size} tokens, the model {engine.config.vocab_size}")
-        if drafts.engine.max_requests < min(len(prompts), max_seqs or engine.max_requests):
+        if drafts.engine.max_requests < min(len(prompts), most):
             raise ValueError(f"the drafting model's engine holds {drafts.engine.max_requests} requests, fewer than run at once")
     limit = engine.max_position
     generate.runs += 1
@@ -182,7 +183,6 @@ def generate(engine: Engine, prompts: Sequence[Sequence[int]], max_tokens: int, 
     counts = DraftCounts()
     waiting: Deque[_Text] = deque(texts)
     running: List[_Text] = []
-    most = min(max_seqs or engine.max_requests, engine.max_requests, engine.max_batch_tokens)
 
     def leave(t: _Text, reason: Optional[str]) -> None:
         t.reason = reason

@@ -86,6 +86,15 @@ def test_a_drafting_model_of_a_small_budget(budget):
     assert run(small(budget=budget), temperature=0.7) == want
 
 
+def test_a_drafting_model_holds_as_many_requests_as_run_at_once():
+    two = fakes.FakeEngine(VOCAB, logits_of, max_requests=2)
+    assert run(small(max_requests=2), two, max_seqs=8)[0] == [alone(p, 30, 0.0, 0) for p in PROMPTS]
+    two = fakes.FakeEngine(VOCAB, logits_of, budget=2)
+    assert run(small(max_requests=2), two)[0] == [alone(p, 30, 0.0, 0) for p in PROMPTS]
+    with pytest.raises(ValueError, match="requests"):
+        run(small(max_requests=2))
+
+
 def test_pages_run_out_where_nothing_was_drafted():
     """The drafting model is at its last position; the last request waits and is read again."""
     prompts = [[1, 2, 3, 4, 5, 6, 7, 8, 9], [9, 8, 7, 6, 5, 4, 3, 2, 1]]
