@@ -147,6 +147,7 @@ class _Text:
     sampler: Sampler
     order: int = 0
     reason: Optional[str] = None
+    waits: bool = False      # it had to make room once
     draws: List[float] = field(default_factory=list)     # random numbers ahead of the generator: one for each token that is next to be drawn
 
 
@@ -195,6 +196,14 @@ def generate(engine: Engine, prompts: Sequence[Sequence[int]], max_tokens: int, 
         mine = {t.rid for t in texts}
         return any(rid not in mine for rid in engine.cache.request_ids())
 
+    def fits(t: _Text) -> bool:
+        """Whether there are pages for all of a text and one to grow into: one that had to make room waits for them, or it would be read over and over."""
+        for g, group in enumerate(engine.cache.groups):
+            held = len(t.tokens) if group.reach is None else min(len(t.tokens), group.reach + engine.max_batch_tokens)
+            if engine.cache.free_pages(g) < engine.cache.pages_needed(held, g) + 1:
+                return False
+        return True
+
     def read(t: _Text) -> None:
         """All of a text but its last token into the cache."""
         engine.add_request(t.rid, t.tokens)
@@ -238,9 +247,12 @@ def generate(engine: Engine, prompts: Sequence[Sequence[int]], max_tokens: int, 
                     waiting.popleft()
                     leave(t, LENGTH)
                     continue
+                if running and t.waits and not fits(t):
+                    break
                 try:
                     read(t)
                 except OutOfPages:
+                    t.waits = True
                     if not running and others():
                         raise
                     leave(t, LENGTH if not running else None)      # alone it is too long for the cache
@@ -271,6 +283,7 @@ def generate(engine: Engine, prompts: Sequence[Sequence[int]], max_tokens: int, 
                             raise
                         break
                     leave(t, None)
+                    t.waits = True
                     waiting.appendleft(t)
                     trees = trees[:-1]
             if kept is None:

@@ -112,3 +112,12 @@ def test_a_prompt_that_fills_the_context(temperature):
     assert [len(w) for w in want] == [1, 1, 2]
     assert run(drafts.PromptLookup(), full(), prompts, temperature=temperature)[0] == want
     assert run(small(max_position=16), full(), prompts, temperature=temperature)[0] == want
+
+
+@pytest.mark.parametrize("pages", [16, 17, 20, 24])
+def test_a_request_that_waits_for_pages_is_not_read_over_and_over(pages):
+    prompts = [[1 + (i * j) % 9 for i in range(32)] for j in (1, 2, 3)]
+    few = fakes.FakeEngine(VOCAB, logits_of, pages=pages, page_size=4, budget=8)
+    got, _ = run(drafts.PromptLookup(tokens=2), few, prompts, 24)
+    assert got == [alone(p, 24, 0.0, 0) for p in prompts]
+    assert sum(n for step in few.log for _, n in step) <= 3 * sum(32 + 24 for _ in prompts)
