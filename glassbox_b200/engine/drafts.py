@@ -168,7 +168,7 @@ def generate(engine: Engine, prompts: Sequence[Sequence[int]], max_tokens: int, 
     if config.needs_host:
         raise ValueError("drafted generation is greedy or at a temperature: top_k, top_p, min_p and repetition_penalty are not built for it")
     if not engine.model.takes_trees:
-        raise ValueError(f"{engine.config.architecture} takes no drafted trees with this cache (a part carries something from row to row, or the cache holds 4 bits)")
+        raise ValueError(f"{engine.config.architecture} takes no drafted trees: {engine.model.why_no_trees()}")
     most = min(max_seqs or engine.max_requests, engine.max_requests, engine.max_batch_tokens)      # requests that run at once
     if isinstance(drafts, DraftModel):
         if drafts.engine is engine:

@@ -432,8 +432,7 @@ class Engine:
 
     def _validate_trees(self, entries) -> None:
         if not self.model.takes_trees:
-            raise ValueError(f"{self.config.architecture} takes no drafted trees with this cache (a part carries something from row to row, "
-                             f"or the cache holds 4 bits)")
+            raise ValueError(f"{self.config.architecture} takes no drafted trees: {self.model.why_no_trees()}")
         most = max(len(e.tokens) for e in entries)
         if most > kernels.TREE_MAX_ROWS:
             raise ValueError(f"a tree of {most} tokens is not built (up to {kernels.TREE_MAX_ROWS})")

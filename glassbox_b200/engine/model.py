@@ -63,6 +63,11 @@ class DecoderModel:
         for top in (self.embed, *self.layers, self.final_norm, self.head):
             yield from _all_parts(top)
 
+    def why_no_trees(self) -> str:
+        """The parts that are not built for trees of drafted tokens, for the refusal."""
+        return "not built for " + ", ".join(sorted({type(p).__name__ + (" over a cache in 4 bits" if getattr(p.spec, "cache_bits", None) else "")
+                                                    for p in self.parts() if not p.takes_trees}))
+
     def recordable(self, decode_only: bool) -> bool:
         """Whether every part lets a step of this kind be replayed as a CUDA graph (see ``Part.recordable``)."""
         return all(p.recordable(decode_only) for p in self.parts())
