@@ -23,7 +23,7 @@ constexpr int VT_MOST_WARPS = 8;
 constexpr int VT_SEG = 512, VT_EACH = VT_SEG / 32;      // tokens of a segment, and of a lane
 constexpr int VT_MAX_SEGS = 4097;
 constexpr int VT_MAX_CLUSTER = 8;
-constexpr int VT_TABLE = 64, VT_COPIES = 16;            // 2^(j / 64), for every lane of a half warp in banks of its own
+constexpr int VT_TABLE = 64, VT_COPIES = 16;            // 2^(j / 64), j / 64 taken off its exponent's bits, for every lane of a half warp in banks of its own
 constexpr double VT_NOTHING = 1e-290;                     // sums of weights below it hold none
 constexpr int VT_MAX_ROWS = 8192;                        // rows of a batch whose outcomes fit shared memory
 constexpr int VT_ROWS = 512;                            // rows of a tree whose parents and tokens stay in shared memory
@@ -77,6 +77,11 @@ __device__ __forceinline__ float vt_max(float a, float b) {                 // N
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
+__device__ __forceinline__ float vt_fma_up(float a, float b, float c) {     // rounded up
+    float r;
+    asm("fma.rp.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 __device__ __forceinline__ float vt_warp_max(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v = vt_max(v, __shfl_xor_sync(0xffffffffu, v, o));
@@ -98,14 +103,15 @@ __device__ __forceinline__ double vt_warp_scan(double v) {                  // s
 }
 
 // Weights exp((x - most) / T) of logits x <= most: 2^(k / 64) from a table, whole powers of two added to its exponent, and a polynomial for the rest, at most
-// h = ln 2 / 128 in the exponent: 1 + r + r^2 / 2 + r^3 / 6 + r^4 / 24 with h^2 r^2 in the place of r^4, a relative error of at most h^4 / 96 = 2^-36.7. Below
-// e^-700 all weights are that, nothing (VT_NOTHING). (One table of 256 for all lanes: 800 rows of 49,152 tokens 81 us, its banks' conflicts half of it.)
+// h = ln 2 / 128 in the exponent: 1 + r + r^2 / 2 + r^3 / 6 + r^4 / 24 with h^2 r^2 in the place of r^4, a relative error of at most h^4 / 96 = 2^-36.7. A weight
+// below e^-700 is nothing (below 2^-1000; VT_NOTHING): that of a logit below `least`, which is rounded up, so that at no temperature an exponent of what is not below
+// it leaves the range of numbers, and is finite, so that minus infinity has no weight at any. (One table of 256 for all lanes: 800 rows of 49,152 tokens 81 us, its banks' conflicts half of it.)
 struct VtWeight {
     unsigned table;                    // (its address in shared memory: where it lies has to be known to be read there without detours)
     double heat, most;                 // 64 / (T ln 2)
     float least;
     __device__ __forceinline__ VtWeight(const double* table, double heat, float temp, float most)
-        : table((unsigned)__cvta_generic_to_shared(table) + (threadIdx.x & (VT_COPIES - 1)) * 8), heat(heat), most((double)most), least(fmaxf(fmaf(-700.0f, temp, most), -FLT_MAX)) {}
+        : table((unsigned)__cvta_generic_to_shared(table) + (threadIdx.x & (VT_COPIES - 1)) * 8), heat(heat), most((double)most), least(fmaxf(vt_fma_up(-700.0f, temp, most), -FLT_MAX)) {}
     __device__ __forceinline__ double operator()(float x) const {
         constexpr double MAGIC = 6755399441055744.0;                  // 1.5 2^52: the low word of a sum with it is the nearest whole number
         constexpr double C1 = 0.010830424696249145, C2 = 5.864919287185391e-05, C3 = 2.1173137155464774e-07;
@@ -115,7 +121,8 @@ struct VtWeight {
         const double r = fma(d, heat, MAGIC - s);
         double t;
         asm("ld.shared.f64 %0, [%1];" : "=d"(t) : "r"(table + (unsigned)(k & (VT_TABLE - 1)) * (VT_COPIES * 8)));
-        const double w = __hiloint2double(__double2hiint(t) + (k & ~(VT_TABLE - 1)) * (1 << 14), __double2loint(t));
+        const int high = __double2hiint(t) + k * (1 << 14);               // (the entry's share of k is taken off it)
+        const double w = __hiloint2double(x >= least ? high : 0, __double2loint(t));
         return fma(w * r, fma(fma(C3, r, C2), r, C1), w);
     }
 };
@@ -179,7 +186,8 @@ struct VtRow {
         p_most = reinterpret_cast<float*>(DRAFTED ? r_sum + per : q_sum);
         q_most = p_most + per;
         static_assert(VT_THREADS % VT_TABLE == 0, "a thread has copies of one entry");
-        const double entry = exp2((double)(threadIdx.x % VT_TABLE) / VT_TABLE);
+        const double power = exp2((double)(threadIdx.x % VT_TABLE) / VT_TABLE);
+        const double entry = __hiloint2double(__double2hiint(power) - (int)(threadIdx.x % VT_TABLE) * (1 << 14), __double2loint(power));
         for (int i = threadIdx.x / VT_TABLE; i < VT_COPIES; i += VT_THREADS / VT_TABLE) sh.table[threadIdx.x % VT_TABLE * VT_COPIES + i] = entry;
     }
     __device__ __forceinline__ void request(int first, int count, float t) {
