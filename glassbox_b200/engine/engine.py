@@ -137,9 +137,11 @@ class Engine:
         self.use_graphs = bool(use_graphs)
         self.max_graph_batch = 64
         self._graphs: Dict[tuple, dict] = {}
+        self._tree_graphs: Dict[tuple, dict] = {}
         self._layouts: Dict[tuple, dict] = {}
         self._seen: Dict[tuple, int] = {}
         self.max_graphs = 128
+        self.max_tree_graphs = 64        # (of their own: drafts change size from step to step and would leave prompts none)
         self.graph_replays = 0
         self.sampled: Optional[torch.Tensor] = None
         self._draws = self._trees = None
@@ -455,12 +457,12 @@ class Engine:
             S_b = 1 << (S - 1).bit_length()
             shape = (rounded(n + S_b - S), S_b, rounded(n_want), max(8, 1 << max(max_pages - 1, 0).bit_length()))
             key = ("trees",) + shape + (most,)
-            g = self._graphs.get(key)
+            g = self._tree_graphs.get(key)
             if g is None:
                 if len(self._seen) > 4096:
                     self._seen.clear()
                 self._seen[key] = self._seen.get(key, 0) + 1
-                if self._seen[key] < 2 or len(self._graphs) >= self.max_graphs:
+                if self._seen[key] < 2 or len(self._tree_graphs) >= self.max_tree_graphs:
                     recorded, shape = False, (n, S, n_want, max_pages)
         off = self._layout(*shape, words)
         host = self._fill(entries, off, *shape)
@@ -722,7 +724,7 @@ class Engine:
                 gc.enable()
         g = {"graph": graph, "meta": meta, "logits": logits, "sampled": sampled, "ctx": ctx,
              "nodes": kernels.launch_count - before, "exec": int(graph.raw_cuda_graph_exec())}
-        self._graphs[key] = g
+        (self._tree_graphs if words else self._graphs)[key] = g
         return g
 
     @property
