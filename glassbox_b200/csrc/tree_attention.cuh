@@ -21,7 +21,7 @@ struct TreeArgs {
     const int* positions;
     const int* visible;      // [n, words], 32 rows of the tree a word
     int words;
-    int n, nh, nkv, hd, page_size;
+    int n, max_rows, nh, nkv, hd, page_size;
     long long num_pages;
     float scale;
     int window;              // 0: none
@@ -40,16 +40,22 @@ struct TreePlan {
     long long floats = 0;    // of scratch
 };
 
+// Rows of a request; -1: they lie outside the batch, or are more than was said, for which neither grid nor scratch is made.
+__device__ __forceinline__ int tree_rows(const TreeArgs& a, int seq) {
+    const int row0 = a.first_row[seq], rows = a.first_row[seq + 1] - row0;
+    return row0 < 0 || rows < 0 || row0 > a.n - rows || rows > a.max_rows ? -1 : rows;
+}
+
 // A request of the step. rows 0: nothing to do.
 struct TreeSeq {
     int row0, rows, start, key_lo, length;
     const int* table;
     __device__ __forceinline__ TreeSeq(const TreeArgs& a, int seq) {
         row0 = a.first_row[seq];
-        rows = a.first_row[seq + 1] - row0;
+        rows = tree_rows(a, seq);
         start = a.start_pos[seq];
         table = a.block_tables + (size_t)seq * a.max_pages;
-        if (row0 < 0 || rows < 0 || row0 > a.n - rows) {          // (rows outside the batch: reported, nothing is read or written)
+        if (rows < 0) {                                   // (reported, nothing is read or written)
             atomicOr(a.status, GB_STATUS_BAD_SLOT);
             rows = 0;
         }
@@ -111,8 +117,8 @@ struct TreeCut {
     __device__ __forceinline__ void of(int s, long long& tiles, long long& items) const {
         tiles = items = 0;
         if (s >= num_seqs) return;
-        const int n = a.first_row[s + 1] - a.first_row[s], start = a.start_pos[s];
-        if (n <= 0 || start < 0 || a.first_row[s] < 0 || a.first_row[s] > a.n - n) return;
+        const int n = tree_rows(a, s), start = a.start_pos[s];
+        if (n <= 0 || start < 0) return;
         const int low = a.window > 0 ? max(0, start - a.window + 1) : 0;
         items = (long long)a.nkv * ((n * (a.nh / a.nkv) + rows - 1) / rows);
         tiles = items * ((start + n + keys - 1) / keys - low / keys);
