@@ -246,7 +246,8 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeArgs a, int n
     bool live = false;                                // the row belongs to a request that the shares are of (a padding request's rows have been written)
     for (int s0 = 0; s0 < num_seqs && !live; s0 += 32) {
         const int s = s0 + lane;
-        live = __any_sync(0xffffffffu, s < num_seqs && a.start_pos[s] >= 0 && a.first_row[s] <= row && row < a.first_row[s] + tree_rows(a, s));
+        live = __any_sync(0xffffffffu, s < num_seqs && a.start_pos[s] >= 0 && a.start_pos[s] <= a.places - tree_rows(a, s) && a.first_row[s] <= row &&
+                                             row < a.first_row[s] + tree_rows(a, s));
     }
     if (!live) return;
     const float2* ml = reinterpret_cast<const float2*>(a.parts + a.splits * cells * a.hd) + cell;
@@ -356,7 +357,7 @@ GB_EXPORT int gb_tree_attention(int kind, const void* q, long long q_stride, voi
     GB_REQUIRE((long long)max_pages * page_size < (1ll << 31) - 4096, "gb_tree_attention: the block tables reach too far");
     if (n == 0 || num_seqs == 0 || max_rows == 0) return 0;
     GB_REQUIRE(q && out && kcache && vcache && block_tables && first_row && start_pos && positions && visible && status, "gb_tree_attention: a tensor is missing");
-    TreeArgs a = {q, q_stride, out, out_stride, kcache, vcache, block_tables, max_pages, first_row, start_pos, positions, visible, words, n, max_rows, nh, nkv, hd, page_size,
+    TreeArgs a = {q, q_stride, out, out_stride, kcache, vcache, block_tables, max_pages, max_pages * page_size, first_row, start_pos, positions, visible, words, n, max_rows, nh, nkv, hd, page_size,
                   num_pages, scale, window, 1, parts, status};
     if (kind >= 1) {
         GB_REQUIRE(kind == 1 || (scale > 0.f && page_size >= 8 && page_size <= TREE_TC_KEYS && (uintptr_t)q % 16 == 0 && q_stride % 8 == 0 && (uintptr_t)out % 16 == 0 && out_stride % 8 == 0),

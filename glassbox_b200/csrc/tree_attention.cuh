@@ -15,7 +15,7 @@ struct TreeArgs {
     const void* kcache;
     const void* vcache;
     const int* block_tables;
-    int max_pages;
+    int max_pages, places;   // (places: of the pages' tokens)
     const int* first_row;
     const int* start_pos;
     const int* positions;
@@ -57,6 +57,9 @@ struct TreeSeq {
         table = a.block_tables + (size_t)seq * a.max_pages;
         if (rows < 0) {                                   // (reported, nothing is read or written)
             atomicOr(a.status, GB_STATUS_BAD_SLOT);
+            rows = 0;
+        } else if (rows > 0 && start > a.places - rows) { // (nor where the tables do not reach)
+            atomicOr(a.status, GB_STATUS_BAD_POSITION);
             rows = 0;
         }
         length = start + rows;
@@ -118,7 +121,7 @@ struct TreeCut {
         tiles = items = 0;
         if (s >= num_seqs) return;
         const int n = tree_rows(a, s), start = a.start_pos[s];
-        if (n <= 0 || start < 0) return;
+        if (n <= 0 || start < 0 || start > a.places - n) return;
         const int low = a.window > 0 ? max(0, start - a.window + 1) : 0;
         items = (long long)a.nkv * ((n * (a.nh / a.nkv) + rows - 1) / rows);
         tiles = items * ((start + n + keys - 1) / keys - low / keys);

@@ -2703,7 +2703,7 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vca
     a ``window``, of these the ones that are fewer than that many positions back. A row that sees nothing comes out as zeros, so do the rows of a request
     with a negative start; rows that belong to no request stay as they are. q, out: bfloat16 or float32 [n, nh * hd], rows may be strided; kcache, vcache
     [pages, nkv, page_size, hd] of the same type. No request has more than ``max_rows_per_seq`` rows (one that does is
-    reported in ``status`` and its rows stay as they are, as where they lie outside the batch); ``max_context`` sizes the shares of the keys
+    reported in ``status`` and its rows stay as they are, as where they lie outside the batch or behind what the tables hold); ``max_context`` sizes the shares of the keys
     (longer contexts are still right), ``parts`` comes from ``tree_attention_parts`` of the same sizes."""
     shape, q_strides, out_strides = q.shape, q.stride(), out.stride()
     if not (len(shape) == 2 and shape[1] == nh * hd and q_strides[1] == 1 and out.shape == shape and out_strides[1] == 1):

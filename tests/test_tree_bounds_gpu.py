@@ -41,3 +41,12 @@ def test_rows_outside_the_batch(dtype, reach):
     b = Batch(dtype, 4, 2, 64, [(1200, 40), (900, 33), (1500, 20)], seed=32, behind=0)
     b.dev["first"][3] = b.n + 7
     others(b, b.run(reach=reach), [2], 2)
+
+
+@pytest.mark.parametrize("start", [1 << 14, (1 << 31) - 1000, (1 << 31) - 30])
+@pytest.mark.parametrize("dtype,hd,reach,rows", [(F32, 64, None, 9), (BF, 64, None, 9), (BF, 64, None, 60), (BF, 128, FAR, 40)])
+def test_beyond_the_tables(start, dtype, hd, reach, rows):
+    """Positions that the tables do not reach, the last ones with sums that pass 2^31."""
+    b = Batch(dtype, 4, 2, hd, [(1200, rows), (900, rows), (30, 4)], seed=33)
+    b.dev["start"][1] = start
+    others(b, b.run(reach=reach), [1], 4)
