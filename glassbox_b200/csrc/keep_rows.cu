@@ -38,11 +38,11 @@ __global__ void __launch_bounds__(KR_THREADS) keep_rows_kernel(const KeepArgs a,
     }
     if (tid < 32) {
         const int* table = a.block_tables + (size_t)seq * a.max_pages;
-        auto place = [&](int at) -> long long {
-            const int index = at / a.page_size;
-            const int page = index < a.max_pages ? table[index] : -1;
+        auto place = [&](int from, int rows) -> long long {
+            const unsigned at = (unsigned)from + (unsigned)rows, index = at / (unsigned)a.page_size;      // (may pass 2^31)
+            const int page = index < (unsigned)a.max_pages ? table[index] : -1;
             if (page < 0 || page >= a.num_pages) return -1;
-            return (long long)page * a.heads * a.page_size + at % a.page_size;
+            return (long long)page * a.heads * a.page_size + at % (unsigned)a.page_size;
         };
         int count = 0;
         bool bad = false;
@@ -51,8 +51,8 @@ __global__ void __launch_bounds__(KR_THREADS) keep_rows_kernel(const KeepArgs a,
             long long src = 0, dst = 0;
             if (r != j) {
                 if (r > j && r < rows) {
-                    src = place(start + r);
-                    dst = place(start + j);
+                    src = place(start, r);
+                    dst = place(start, j);
                 }
                 bad = bad || src == dst || src < 0 || dst < 0;      // (a path that leaves its tree or does not ascend, or a page that is missing)
             }
