@@ -344,7 +344,7 @@ struct VtRow {
     // turn: 0 and 1 from call to call, so that what blocks still read of one is not written by the next.
     __device__ __forceinline__ VtOutcome outcome(int cur, int turn) const {
         const int vocab = a.vocab;
-        const bool drafted = DRAFTED && draws;
+        const bool drafted = DRAFTED && draws && next_child(cur, cur, -1) >= 0;      // (a row without children has no q)
         const T* x = (const T*)a.logits + (size_t)(row0 + cur) * a.stride;
         const T* y = drafted ? (const T*)a.draft + (size_t)(row0 + cur) * a.draft_stride : nullptr;
         const int lead = (int)((uintptr_t)x & 15) / (int)sizeof(T), segs = (lead + vocab + VT_SEG - 1) / VT_SEG;

@@ -2767,13 +2767,13 @@ def verify_tree(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tenso
     ``draft_logits`` a token is drawn at the row it has reached: the first one, in the order of the ids, at which the sum of softmax(logits / temperature[s])
     exceeds uniform[row, 1] (at a temperature that is not above 0: the largest logit, of equal ones the lowest id); the walk goes on at the first child that
     holds that token, and ends where none does. With ``draft_logits`` (like logits: what the children of each row were drawn from, independently and at the
-    same temperature, as q) a child of token x is taken where uniform[child, 0] * q(x) * sum(r) < r(x), r being p = softmax(logits / temperature) at first and
+    same temperature, as q; a row without children may hold anything there) a child of token x is taken where uniform[child, 0] * q(x) * sum(r) < r(x), r being p = softmax(logits / temperature) at first and
     max(r - sum(r) q, 0) behind a child that was not taken; behind the last child the token that follows is drawn from r by uniform[row, 1] (from p where
     nothing is left). So what comes out is distributed as what the model writes by itself. At temperature 0 drafted distributions play no part.
 
     Results, int32: accepted[s] rows are kept (row 0 always is; 0 for a request without rows), path[seq_first_row[s] + j] is the j-th of them (-1 behind the
-    last), next_token[s] the token that follows (-1: the logits that the walk reached hold a NaN or plus infinity, or nothing but minus infinity; a greedy walk
-    passes over NaN). A child whose token is outside the vocabulary is never taken."""
+    last), next_token[s] the token that follows (-1: the logits at the row that the walk has reached, or what its children were drawn from, hold a NaN or plus
+    infinity, or nothing but minus infinity; a greedy walk passes over NaN, and gives -1 only where there is nothing else). A child whose token is outside the vocabulary is never taken."""
     shape, strides = logits.shape, logits.stride()
     if not (len(shape) == 2 and strides[1] == 1):
         raise KernelError("logits must be [rows, vocab] with neighbouring numbers")
