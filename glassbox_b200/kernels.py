@@ -2652,12 +2652,12 @@ TREE_MAX_ROWS = 1024           # rows of a request's tree
 VERIFY_MAX_VOCAB = 4096 * 512
 
 
-def _tree_kind(dtype: int, addresses: int, strides: int, hd: int, page_size: int, scaled: bool, rows: int) -> int:
+def _tree_kind(dtype: int, addresses: int, strides: int, pools: int, hd: int, page_size: int, scaled: bool, rows: int) -> int:
     """Which kernels ``tree_attention`` runs: 1 the tensor cores' (bfloat16, head sizes 32, 64, 96 and 128, rows that start at 4 bytes, pages of a
-    power of two from 8 on, below 2^31 rows of them), 2 tcgen05's where there is enough for it (rows of q and out at 16 bytes, pages of 8 to 128 tokens, a scale
+    power of two from 8 on, below 2^31 rows of them, in pools that start at 16 bytes), 2 tcgen05's where there is enough for it (rows of q and out at 16 bytes, pages of 8 to 128 tokens, a scale
     above 0), 0 the one for everything else."""
     if not (dtype == BF16 and hd in (32, 64, 96, 128) and page_size >= 8 and page_size & (page_size - 1) == 0 and rows < 1 << 31
-            and strides % 2 == 0 and addresses % 4 == 0):
+            and pools % 16 == 0 and strides % 2 == 0 and addresses % 4 == 0):
         return 0
     return 2 if scaled and page_size <= 128 and strides % 8 == 0 and addresses % 16 == 0 else 1
 
@@ -2730,13 +2730,13 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vca
     stream = _here(q, out, kcache, vcache, block_tables, seq_first_row, seq_start_pos, positions, visible, parts, status)
     if not n or not num_seqs or not max_rows_per_seq:
         return
-    q_at, out_at = q.data_ptr(), out.data_ptr()
-    kind = _tree_kind(dtype, q_at | out_at, q_strides[0] | out_strides[0], hd, page_size, scale > 0, pool[0] * nkv * page_size)
+    q_at, out_at, k_at, v_at = q.data_ptr(), out.data_ptr(), kcache.data_ptr(), vcache.data_ptr()
+    kind = _tree_kind(dtype, q_at | out_at, q_strides[0] | out_strides[0], k_at | v_at, hd, page_size, scale > 0, pool[0] * nkv * page_size)
     max_context, window = int(max_context), int(window or 0)
     floats = _tree_floats(kind, n, num_seqs, max_rows_per_seq, nh, nkv, hd, max_context, window)
     if floats and (parts is None or parts.dtype != torch.float32 or not parts.is_contiguous() or parts.numel() < floats):
         raise KernelError(f"this batch needs contiguous float32 scratch of {floats} numbers (tree_attention_parts)")
-    _call("gb_tree_attention", kind, q_at, q_strides[0], out_at, out_strides[0], dtype, kcache.data_ptr(), vcache.data_ptr(),
+    _call("gb_tree_attention", kind, q_at, q_strides[0], out_at, out_strides[0], dtype, k_at, v_at,
           block_tables.data_ptr(), max_pages, seq_first_row.data_ptr(), seq_start_pos.data_ptr(), positions.data_ptr(), visible.data_ptr(),
           seen[1], n, num_seqs, int(max_rows_per_seq), nh, nkv, hd, page_size, pool[0], float(scale), window, max_context, _ptr(parts),
           status.data_ptr(), stream)
