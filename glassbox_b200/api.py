@@ -68,8 +68,8 @@ class LLM:
         """Generate up to ``max_tokens`` tokens after each prompt. ``prompts`` is one list of token
         ids or a list of such lists; request i samples with seed ``seed + i``. Returns the new
         tokens (one list, or a list of lists in the order given). With ``drafts`` (``PromptLookup``, ``DraftModel``) several tokens a step are
-        guessed and verified (``engine.drafts``; greedy or with a temperature alone): the model's own text, in fewer steps where the guesses
-        are good; ``self.draft_counts`` says how they fared. Such requests go by themselves, not through the scheduler's queue."""
+        guessed and verified (``engine.drafts``; greedy or with a temperature alone): the model's own text up to the rounding of its logits, in fewer steps where
+        the guesses are good; ``self.draft_counts`` says how they fared. Such requests go by themselves, not through the scheduler's queue."""
         single = len(prompts) > 0 and not isinstance(prompts[0], (list, tuple, np.ndarray))
         batch = [prompts] if single else list(prompts)
         limit = self.engine.max_position

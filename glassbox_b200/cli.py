@@ -14,7 +14,7 @@ or commas; ``;`` separates several prompts, which are then batched) and the repl
 token ids. ``score`` prints, for each token but the first, its id, its log probability given those before it, the entropy of the
 distribution it came from and, with ``--top K``, the K most probable tokens as id:log probability; the perplexity of each prompt
 goes to the error stream. ``--draft-lookup`` guesses up to K tokens a step from the text itself, ``--draft-model`` lets a smaller model write K (4) ahead; what
-comes out is the model's own text either way. ``--raw`` is accepted and changes nothing: there is no chat template to skip. The
+comes out is the model's own text either way, up to the rounding of its logits. ``--raw`` is accepted and changes nothing: there is no chat template to skip. The
 chat, serve, anatomy, trace and spec-trace subcommands of the reference belong to its server,
 visualizer and are not part of this engine; what its speculative decoder does is ``generate`` with drafts.
 """

@@ -14,7 +14,7 @@
 // whose share holds the target finds the segment and reads it once more.
 //
 // What bounds it: the weights' arithmetic, 27 instructions a token and warp of which 9 are of 64 bits, and in the walk a row's trips one after the other, 6 us.
-// 1 tree of 8 rows, 49,152 tokens, 8.2 us; 64 trees of 16 rows walked at T = 0.8 64 us, 512 rows of 100,003 in bfloat16 at T = 0 all at once 49 us.
+// 1 tree of 8 rows, 49,152 tokens, 8.2 us; 64 trees of 16 rows walked at T = 0.8 65 us, 512 rows of 100,003 in bfloat16 at T = 0 all at once 49 us.
 #include "common.cuh"
 
 #include <cooperative_groups.h>

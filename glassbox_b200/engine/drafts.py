@@ -1,6 +1,7 @@
 """Generation with drafted tokens (crates/glassbox-core/src/spec.rs:79-240): a cheap guess at a request's next tokens, one step of the model over all of
 them, and what the model would have written itself is kept (``Engine.verify_step``). The text that comes out is the model's: greedy requests get
-the tokens that they would get one by one, requests with a temperature tokens of the same distribution.
+the tokens that they would get one by one, requests with a temperature tokens of the same distribution, both from logits that a step of several rows may round
+otherwise than a step of one (in bfloat16 nearly equal ones may fall the other way).
 
 Two sources of drafts, as there: ``PromptLookup`` takes what followed earlier where the text's last tokens occurred before (of several such places a
 tree), ``DraftModel`` lets a smaller model of the same vocabulary write ahead (a chain, with the distributions it was drawn from).
