@@ -85,9 +85,9 @@ class DraftModel:
         requests."""
         engine = self.engine
         counts = [max(0, min(self.tokens, room, engine.max_position - len(text))) for room, text in zip(rooms, texts)]
-        for rid, text, count in zip(rids, texts, counts):
-            if count:
-                self._catch_up(rid, text)
+        for j, (rid, text) in enumerate(zip(rids, texts)):
+            if counts[j] and not self._catch_up(rid, text):
+                counts[j] = 0
             elif len(text) >= engine.max_position:       # (a text that its context does not hold)
                 self.drop(rid)
         firsts = np.concatenate([[0], np.cumsum([c + 1 for c in counts])])
@@ -99,18 +99,47 @@ class DraftModel:
             every = [j for j, c in enumerate(counts) if c > i]
             for a in range(0, len(every), engine.max_batch_tokens):
                 live = every[a:a + engine.max_batch_tokens]
-                rows = engine.step([StepEntry(rids[j], [drafts[j][-1]], [0]) for j in live])
+                rows = None
+                while live and rows is None:
+                    try:
+                        rows = engine.step([StepEntry(rids[j], [drafts[j][-1]], [0]) for j in live])
+                    except OutOfPages:                   # the last one's pages are for the others; what it has drafted stands
+                        j = live.pop()
+                        counts[j] = i
+                        self.drop(rids[j])
+                if rows is None:
+                    continue
                 logits.index_copy_(0, torch.tensor([int(firsts[j]) + i for j in live], device=engine.device), rows)
                 picked = torch.empty(len(live), dtype=torch.int32, device=engine.device)
                 draws = torch.tensor([float(numbers[j][i]) for j in live], dtype=torch.float32).to(engine.device)
                 kernels.sample(rows, picked, heat[live].to(engine.device), draws)
                 for j, t in zip(live, picked.tolist()):
                     drafts[j].append(t)
+        done = [int(f) + k for f, d in zip(firsts, drafts) for k in range(len(d))]
+        if len(done) < len(logits):
+            logits = logits[torch.tensor(done, device=engine.device)]
         return [(d, list(range(-1, len(d) - 1))) for d in drafts], logits
 
-    def _catch_up(self, rid, text: Sequence[int]) -> None:
+    def _catch_up(self, rid, text: Sequence[int]) -> bool:
         """The request's cache holds all of the text but its last token. What was drafted and not kept is taken back; where that cannot be (a state has taken it in,
-        a window has given back the pages before it) the text is read anew."""
+        a window has given back the pages before it) the text is read anew. False: there are no pages or no slot for it now, and it holds none."""
+        try:
+            if self.engine.cache.has(rid) or self._fits(text):
+                self._read(rid, text)
+                return True
+        except OutOfPages:
+            self.drop(rid)
+        return False
+
+    def _fits(self, text: Sequence[int]) -> bool:
+        cache = self.engine.cache
+        for g, group in enumerate(cache.groups):
+            held = len(text) if group.reach is None else min(len(text), group.reach + self.engine.max_batch_tokens)
+            if cache.free_pages(g) < cache.pages_needed(held, g) + 1:
+                return False
+        return True
+
+    def _read(self, rid, text: Sequence[int]) -> None:
         engine = self.engine
         if not engine.cache.has(rid):
             engine.add_request(rid, list(text))
@@ -214,14 +243,10 @@ def generate(engine: Engine, prompts: Sequence[Sequence[int]], max_tokens: int, 
     def propose(room: int):
         rooms = [max(0, min(room, max_tokens - (len(t.tokens) - t.prompt) - 1, limit - len(t.tokens))) for t in running]
         if isinstance(drafts, DraftModel) and max(rooms) > 0:
-            try:
-                trees, logits = drafts.propose_all([t.rid for t in running], [t.tokens for t in running], rooms, [config.temperature] * len(running),
-                                                   [t.sampler.config.seed for t in running])
-                # (without drafts there is nothing that came from a distribution)
-                return trees, None if config.greedy or all(len(tokens) == 1 for tokens, _ in trees) else logits
-            except OutOfPages:                           # (of the drafting model: it begins anew with the next step)
-                for t in running:
-                    drafts.drop(t.rid)
+            trees, logits = drafts.propose_all([t.rid for t in running], [t.tokens for t in running], rooms, [config.temperature] * len(running),
+                                               [t.sampler.config.seed for t in running])
+            # (without drafts there is nothing that came from a distribution)
+            return trees, None if config.greedy or all(len(tokens) == 1 for tokens, _ in trees) else logits
         return [drafts.propose(t.tokens, r) if r and isinstance(drafts, PromptLookup) else ([t.tokens[-1]], [-1]) for t, r in zip(running, rooms)], None
 
     def numbers(trees) -> Optional[np.ndarray]:

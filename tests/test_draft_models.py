@@ -121,3 +121,15 @@ def test_a_request_that_waits_for_pages_is_not_read_over_and_over(pages):
     got, _ = run(drafts.PromptLookup(tokens=2), few, prompts, 24)
     assert got == [alone(p, 24, 0.0, 0) for p in prompts]
     assert sum(n for step in few.log for _, n in step) <= 3 * sum(32 + 24 for _ in prompts)
+
+
+@pytest.mark.parametrize("pages", [3, 9, 14, 20])
+@pytest.mark.parametrize("temperature", [0.0, 0.7])
+def test_a_drafting_model_whose_pages_do_not_hold_every_text(pages, temperature):
+    """The texts that fit are drafted for, the others go on without, and none is read in every step."""
+    prompts = [[1 + (i * j) % 9 for i in range(20)] for j in (1, 2, 3, 4)]
+    model = small(pages=pages, page_size=4, budget=8)
+    got, counts = run(model, prompts=prompts, count=24, temperature=temperature)
+    assert temperature or got == [alone(p, 24, 0.0, 0) for p in prompts]
+    assert counts.accepted > 0 or pages < 7
+    assert sum(n for step in model.engine.log for _, n in step if n > 1) <= 3 * sum(20 + 24 for _ in prompts)
