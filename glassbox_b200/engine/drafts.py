@@ -33,6 +33,15 @@ def _numbers(what: int, seeds: Sequence[int], at: int, count: int) -> np.ndarray
     return np.random.default_rng([what, at] + words).random(count, dtype=np.float32)
 
 
+def _fits(engine: Engine, text: Sequence[int]) -> bool:
+    """Whether there are pages for all of a text and one to grow into. One that found too few waits for them, or it would be read over and over."""
+    for g, group in enumerate(engine.cache.groups):
+        held = len(text) if group.reach is None else min(len(text), group.reach + engine.max_batch_tokens)
+        if engine.cache.free_pages(g) < engine.cache.pages_needed(held, g) + 1:
+            return False
+    return True
+
+
 class PromptLookup:
     """Drafts from the text itself: where its last ``match`` tokens (or fewer, down to one) occurred before, what followed there, up to ``tokens`` of
     them, for up to ``branches`` such places, the latest first. Places that go on alike share the tokens that are alike."""
@@ -124,20 +133,12 @@ class DraftModel:
         """The request's cache holds all of the text but its last token. What was drafted and not kept is taken back; where that cannot be (a state has taken it in,
         a window has given back the pages before it) the text is read anew. False: there are no pages or no slot for it now, and it holds none."""
         try:
-            if self.engine.cache.has(rid) or self._fits(text):
+            if self.engine.cache.has(rid) or _fits(self.engine, text):
                 self._read(rid, text)
                 return True
         except OutOfPages:
             self.drop(rid)
         return False
-
-    def _fits(self, text: Sequence[int]) -> bool:
-        cache = self.engine.cache
-        for g, group in enumerate(cache.groups):
-            held = len(text) if group.reach is None else min(len(text), group.reach + self.engine.max_batch_tokens)
-            if cache.free_pages(g) < cache.pages_needed(held, g) + 1:
-                return False
-        return True
 
     def _read(self, rid, text: Sequence[int]) -> None:
         engine = self.engine
@@ -226,14 +227,6 @@ def generate(engine: Engine, prompts: Sequence[Sequence[int]], max_tokens: int, 
         mine = {t.rid for t in texts}
         return any(rid not in mine for rid in engine.cache.request_ids())
 
-    def fits(t: _Text) -> bool:
-        """Whether there are pages for all of a text and one to grow into: one that had to make room waits for them, or it would be read over and over."""
-        for g, group in enumerate(engine.cache.groups):
-            held = len(t.tokens) if group.reach is None else min(len(t.tokens), group.reach + engine.max_batch_tokens)
-            if engine.cache.free_pages(g) < engine.cache.pages_needed(held, g) + 1:
-                return False
-        return True
-
     def read(t: _Text) -> None:
         """All of a text but its last token into the cache."""
         engine.add_request(t.rid, t.tokens)
@@ -273,7 +266,7 @@ def generate(engine: Engine, prompts: Sequence[Sequence[int]], max_tokens: int, 
                     waiting.popleft()
                     leave(t, LENGTH)
                     continue
-                if running and t.waits and not fits(t):
+                if running and t.waits and not _fits(engine, t.tokens):
                     break
                 try:
                     read(t)
