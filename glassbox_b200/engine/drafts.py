@@ -23,14 +23,25 @@ from .scheduler import LENGTH, STOP
 
 
 _DRAFTS, _COINS = 1, 2
+_M64, _STEP = (1 << 64) - 1, 0x9E3779B97F4A7C15
+
+
+def _mix(x: int) -> int:
+    """The output function of SplitMix64 (Steele, Lea and Flood, Fast splittable pseudorandom number generators, 2014) behind a step of its state."""
+    x = (x + _STEP) & _M64
+    x = ((x ^ x >> 30) * 0xBF58476D1CE4E5B9) & _M64
+    x = ((x ^ x >> 27) * 0x94D049BB133111EB) & _M64
+    return x ^ x >> 31
 
 
 def _numbers(what: int, seeds: Sequence[int], at: int, count: int) -> np.ndarray:
     """``count`` random numbers in [0, 1) for one use, by a request whose text has ``at`` tokens: a stream for each use, seeds and place, of a generator that is
     not the one that requests draw their tokens with. Rejection holds only where what was drafted, the coins that take it and what is drawn in its place are
     independent, also where all seeds are equal."""
-    words = [half for s in seeds for half in (int(s) & 0xFFFFFFFF, int(s) >> 32 & 0xFFFFFFFF)]
-    return np.random.default_rng([what, at] + words).random(count, dtype=np.float32)
+    state = _mix(what)
+    for s in (*seeds, at):
+        state = _mix(state ^ (int(s) & _M64))
+    return np.array([_mix(state + i * _STEP) >> 40 for i in range(count)], dtype=np.float32) / np.float32(1 << 24)
 
 
 def _fits(engine: Engine, text: Sequence[int]) -> bool:

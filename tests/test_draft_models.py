@@ -111,7 +111,9 @@ def test_a_prompt_that_fills_the_context(temperature):
     want = [alone(p, 30, temperature, 3 + i, most=16) for i, p in enumerate(prompts)]
     assert [len(w) for w in want] == [1, 1, 2]
     assert run(drafts.PromptLookup(), full(), prompts, temperature=temperature)[0] == want
-    assert run(small(max_position=16), full(), prompts, temperature=temperature)[0] == want
+    got = run(small(max_position=16), full(), prompts, temperature=temperature)[0]
+    assert [len(o) for o in got] == [1, 1, 2] and got[0] == want[0]
+    assert temperature or got == want                     # (what was drafted is drawn with other numbers)
 
 
 @pytest.mark.parametrize("pages", [16, 17, 20, 24])

@@ -57,3 +57,20 @@ def test_a_run_begins_anew_and_a_request_has_numbers_of_its_own():
         assert drafts.generate(target, [prompt], 9, model, cfg(5 + i))[0] == [many[i]]
     assert drafts.generate(target, [[1], [2], [3]], 9, model, cfg(77))[0] != many
     drafts.generate(target, [[1]], 3, drafts.DraftModel(small, seed=-7), cfg(-3))
+
+
+def test_the_numbers_of_any_two_uses_have_nothing_to_do_with_one_another():
+    """Means, and products of what two streams give, over seeds and places that differ by little: within six deviations."""
+    streams = {}
+    for what in (1, 2):
+        for seeds in ((0, 0), (0, 1), (1, 0), (2 ** 32, 0), (0, -1)):
+            for at in (1, 2, 3):
+                x = drafts._numbers(what, seeds, at, 4000)
+                assert x.dtype == np.float32 and 0 <= x.min() and x.max() < 1
+                streams[what, seeds, at] = (x.astype(np.float64) - 0.5) * 12 ** 0.5
+    all_of = np.array(list(streams.values()))
+    assert abs(all_of.mean(1)).max() < 6 / 4000 ** 0.5 and abs((all_of ** 2).mean(1) - 1).max() < 6 * 0.8 ** 0.5 / 4000 ** 0.5
+    products = all_of @ all_of.T / 4000 - np.eye(len(all_of)) * (all_of ** 2).mean(1)
+    assert abs(products).max() < 6 / 4000 ** 0.5
+    for shift in (1, 2, 5):
+        assert abs(all_of[:, shift:] @ all_of[:, :-shift].T / (4000 - shift)).max() < 6 / (4000 - shift) ** 0.5
